@@ -10,9 +10,13 @@ import torch  # noqa: F401  (loads the HIP runtime that libghost_hip.so binds to
 from .graddotprod_engine import GradDotProdEngine
 from .engine_manager import GhostEngineManager
 from .gradProjection.gradproj_engine import GradProjLoraEngine, GradProjLoRAEngine
+from .lm_layers import (QKNormRotary, ScaledEmbedding, distillation_loss, embedding_lookup,
+                        qk_norm_rotary, qkv_norm_rotary, rotary_table)
 
 __all__ = ['GradDotProdEngine', 'GhostEngineManager', 'GradProjLoraEngine',
-           'GradProjLoRAEngine', 'install_as_ghostEngines']
+           'GradProjLoRAEngine', 'install_as_ghostEngines', 'ScaledEmbedding', 'QKNormRotary',
+           'embedding_lookup', 'rotary_table', 'qkv_norm_rotary', 'qk_norm_rotary',
+           'distillation_loss']
 
 
 def install_as_ghostEngines() -> None:

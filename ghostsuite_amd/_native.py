@@ -10,8 +10,10 @@ samplers call ``ops()``); product code never does.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
+import math
 import threading
 from typing import Optional, Tuple
 
@@ -19,12 +21,13 @@ import torch
 
 from . import build as _build
 
-# gs_dtype / gs_semantics / gs_algo / gs_rounding / gs_proj_layout (include/ghost_hip.h)
+# gs_dtype / gs_semantics / gs_algo / gs_rounding / gs_proj_layout / gs_reduction (include/ghost_hip.h)
 DTYPE_BF16, DTYPE_F32, DTYPE_F16 = 0, 1, 2
 SEM_PAIRWISE_SUM, SEM_PRESUM = 0, 1
 ALGO_AUTO, ALGO_GHOST, ALGO_VALGRAD = 0, 1, 2
 ROUND_FP32, ROUND_REF_BF16 = 0, 1
 PROJ_KO_KI, PROJ_KI_KO = 0, 1
+REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 ERR_UNSUPPORTED = -5  # gs_status GS_ERR_UNSUPPORTED: a valid request outside the kernels' limits
 ABI_VERSION = 2
 
@@ -101,7 +104,35 @@ _SIGNATURES = {
     "gs_linear_bias_dot": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I, _P, _P, _P,
                                 _I, _F, _P, _SZ, _P]),
     "gs_ordered_sum": (_I, [_P, _P, _I, _I64, _P, _I, _P]),
+    "gs_embedding_lookup": (_I, [_P, _I, _I64, _P, _I, _I64, _I64, _F, _I64, _P, _P, _P]),
+    "gs_qk_rotary": (_I, [_P, _P, _P, _P]),
+    "gs_qk_rotary_grad_workspace": (_SZ, [_P]),
+    "gs_qk_rotary_grad": (_I, [_P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "gs_qk_rotary_dots_workspace": (_SZ, [_P]),
+    "gs_qk_rotary_dots": (_I, [_P, _P, _P, _I64, _I64, _P, _P, _P, _P, _F, _P, _SZ, _P]),
+    "gs_distill_workspace": (_SZ, [_P]),
+    "gs_distill_loss": (_I, [_P, _P, _P, _P, _SZ, _P]),
+    "gs_distill_grad": (_I, [_P, _P, _I, _P, _P, _SZ, _P]),
 }
+
+
+class _QKShape(ctypes.Structure):   # gs_qk_shape
+    _fields_ = [("dtype", _I), ("B", _I64), ("T", _I64), ("D", _I64), ("n_rot", _I64),
+                ("heads", ctypes.c_int32 * 3), ("norm", _I), ("interleaved", _I), ("eps", _F),
+                ("weight", _P * 2), ("weight_dtype", _I * 2), ("table", _P),
+                ("n_positions", _I64), ("positions", _P), ("position_bits", _I),
+                ("position_stride_b", _I64), ("position_stride_t", _I64)]
+
+
+class _QKRows(ctypes.Structure):    # gs_qk_rows
+    _fields_ = [("data", _P), ("stride_b", _I64), ("stride_t", _I64), ("stride_h", _I64)]
+
+
+class _Distill(ctypes.Structure):   # gs_distill
+    _fields_ = [("Z", _P), ("dtype", _I), ("N", _I64), ("V", _I64), ("inner", _I64),
+                ("stride_outer", _I64), ("stride_inner", _I64), ("teacher_ids", _P),
+                ("teacher", _P), ("teacher_dtype", _I), ("K", _I64), ("labels", _P),
+                ("ignore_index", _I64), ("temperature", _F), ("alpha", _F), ("reduction", _I)]
 
 
 def load_library() -> ctypes.CDLL:
@@ -186,6 +217,117 @@ def _tokens(x: torch.Tensor, n: int, feat: int) -> int:
     if x.dim() < 2 or x.shape[0] != n:
         raise GhostHipError(f"expected a [N, ..., F] tensor with N={n}, got {tuple(x.shape)}")
     return x.numel() // (n * feat) if n * feat > 0 else 0
+
+
+def _on(dev: torch.device):
+    """Kernels launch on the current device: makes `dev` that one for the body."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _kernel_dtype(t: torch.Tensor, what: str) -> int:
+    if t.dtype not in (torch.bfloat16, torch.float32):
+        raise GhostHipError(f"{what}: bf16 or fp32, got {t.dtype}")
+    return _TORCH_TO_GS[t.dtype]
+
+
+def _features_contiguous(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+class _QKCall:
+    """The arguments of a gs_qk_rotary* call from a plan (the keywords of
+    lm_layers.qkv_norm_rotary) and its input rows: one packed tensor, or queries and keys."""
+
+    def __init__(self, plan, parts, qw, kw):
+        heads, table, positions = plan["heads"], plan["table"], plan["positions"]
+        self.dev = _require_device(*parts, qw, kw, table, positions)
+        x = parts[0]
+        self.total = sum(heads)
+        if min(heads[:2]) <= 0:
+            raise GhostHipError(f"{heads[0]} query and {heads[1]} key heads")
+        packed = len(parts) == 1
+        if packed and not (x.dim() == 3 and x.shape[2] % self.total == 0) and \
+                not (x.dim() == 4 and x.shape[2] == self.total):
+            raise GhostHipError(f"qkv {tuple(x.shape)} does not hold {self.total} heads")
+        self.B, self.T = x.shape[:2]
+        self.D = x.shape[2] // self.total if packed and x.dim() == 3 else x.shape[3]
+        D, n_rot = self.D, 2 * table.shape[-1]
+        if D <= 0:
+            raise GhostHipError("heads without features")
+        self.dtype = x.dtype
+        for p in parts[1:]:
+            if p.shape[:2] != x.shape[:2] or p.shape[3] != D or p.dtype != x.dtype:
+                raise GhostHipError(f"queries {tuple(x.shape)} {x.dtype} and keys "
+                                    f"{tuple(p.shape)} {p.dtype} disagree")
+        if table.dim() != 3 or table.shape[1] != 2 or table.dtype != torch.float32 or \
+                not table.is_contiguous() or n_rot > D:
+            raise GhostHipError(f"table {tuple(table.shape)} {table.dtype}: contiguous fp32 "
+                                f"[positions, 2, n_rot / 2] with n_rot up to {D} expected")
+        s = self.shape = _QKShape()
+        s.dtype = _kernel_dtype(x, "queries and keys")
+        s.B, s.T, s.D, s.n_rot = self.B, self.T, D, n_rot
+        s.heads[:] = heads
+        s.norm, s.interleaved, s.eps = plan["norm"], plan["interleaved"], plan["eps"]
+        self.keep = [table, positions]   # alive until the call is enqueued
+        for i, w in enumerate((qw, kw)):
+            if w is None:
+                s.weight_dtype[i] = s.dtype
+                continue
+            if w.shape != (D,):
+                raise GhostHipError(f"norm weight {tuple(w.shape)}: [{D}] expected")
+            s.weight_dtype[i] = _kernel_dtype(w, "norm weights")
+            w = w.contiguous()
+            self.keep.append(w)
+            s.weight[i] = w.data_ptr()
+        if n_rot:
+            s.table, s.n_positions = table.data_ptr(), table.shape[0]
+        if positions is not None and n_rot:
+            if positions.dtype not in (torch.int32, torch.int64) or \
+                    tuple(positions.shape) not in ((self.T,), (1, self.T), (self.B, self.T)):
+                raise GhostHipError(f"positions {tuple(positions.shape)} {positions.dtype}: int32 "
+                                    f"or int64 [{self.T}] or [{self.B}, {self.T}] expected")
+            s.positions = positions.data_ptr()
+            s.position_bits = 32 if positions.dtype == torch.int32 else 64
+            s.position_stride_t = positions.stride(-1)
+            if positions.dim() == 2 and positions.shape[0] == self.B:
+                s.position_stride_b = positions.stride(0)
+
+    def split(self, parts):
+        """gs_qk_rows[3] of input-shaped tensors ([B, T, heads, D] each, or one packed)."""
+        rows, esz = (_QKRows * 3)(), 4 if self.dtype == torch.float32 else 2
+        first = 0
+        for i, h in enumerate(self.shape.heads):
+            if h == 0:
+                continue
+            x = parts[0] if len(parts) == 1 else parts[i]
+            sh = x.stride(2) if x.dim() == 4 else self.D
+            at = first * sh if len(parts) == 1 else 0
+            rows[i] = _QKRows(x.data_ptr() + at * esz, x.stride(0), x.stride(1), sh)
+            first += h
+        return rows
+
+    def heads_first(self, tensors):
+        """gs_qk_rows[3] of [B, heads, T, D] tensors (None: data NULL)."""
+        rows = (_QKRows * 3)()
+        for i, t in enumerate(tensors):
+            if t is not None:
+                rows[i] = _QKRows(t.data_ptr(), t.stride(0), t.stride(2), t.stride(1))
+        return rows
+
+    def gradients(self, grads):
+        """The output gradients as the kernels take them (features contiguous)."""
+        out = []
+        for i, h in enumerate(self.shape.heads):
+            g = grads[i] if h else None
+            if g is not None:
+                if g.shape != (self.B, h, self.T, self.D) or g.dtype != self.dtype:
+                    raise GhostHipError(f"output gradient {tuple(g.shape)} {g.dtype}")
+                _require_device(g)
+                g = _features_contiguous(g)
+            out.append(g)
+        return out
 
 
 class HipOps:
@@ -751,6 +893,217 @@ class HipOps:
                                            _TORCH_TO_GS[total.dtype], _stream(dev))
         _check(rc, "gs_ordered_sum")
         return total
+
+    # ---- embedding lookup, query / key norms with rotation, distillation (lm_layers) ----
+
+    def embedding_lookup(self, ids: torch.Tensor, weight: torch.Tensor, scale: float,
+                         padding_idx: Optional[int] = None, want_grad_ids: bool = False):
+        """(scale * weight[ids], ids for embedding_grad or None): gs_embedding_lookup."""
+        dev = _require_device(ids, weight)
+        dt = _kernel_dtype(weight, "embedding weight")
+        if ids.dtype not in (torch.int32, torch.int64):
+            raise GhostHipError(f"token ids of dtype {ids.dtype}: int32 or int64 expected")
+        if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+            raise GhostHipError(f"embedding weight {tuple(weight.shape)}: [vocab, d] expected")
+        ids, weight = ids.contiguous(), weight.contiguous()
+        vocab, d = weight.shape
+        out = torch.empty((*ids.shape, d), dtype=weight.dtype, device=dev)
+        grad_ids = None
+        if want_grad_ids:
+            same = padding_idx is None and ids.dtype == torch.int64
+            grad_ids = ids if same else torch.empty(ids.shape, dtype=torch.int64, device=dev)
+        if ids.numel():
+            with _on(dev):
+                rc = load_library().gs_embedding_lookup(
+                    ids.data_ptr(), 32 if ids.dtype == torch.int32 else 64, ids.numel(),
+                    weight.data_ptr(), dt, vocab, d, scale,
+                    -1 if padding_idx is None else padding_idx, out.data_ptr(),
+                    None if grad_ids is ids else _ptr(grad_ids), _stream(dev))
+            _check(rc, "gs_embedding_lookup")
+        return out, grad_ids
+
+    def embedding_grad(self, ids: torch.Tensor, G: torch.Tensor, shape, dtype: torch.dtype,
+                       scale: float) -> torch.Tensor:
+        """scale * the rows of G added up by id, [vocab, d]: gs_embedding_train_grad over one
+        sample of all the tokens."""
+        dev = _require_device(ids, G)
+        if not ids.numel():
+            return torch.zeros(shape, dtype=dtype, device=dev)
+        out = torch.empty(shape, dtype=dtype, device=dev)
+        with _on(dev):
+            self.embedding_train_grad(ids.reshape(1, -1), G.reshape(1, -1, shape[1]), 0, scale,
+                                      out)
+        return out
+
+    def qk_norm_rotary(self, plan, parts, qw, kw):
+        """Rotated queries and keys (and values), heads first: gs_qk_rotary.  plan: heads, table,
+        positions, norm, eps, interleaved; parts: (qkv,) or (q, k)."""
+        parts = [_features_contiguous(p) for p in parts]
+        c = _QKCall(plan, parts, qw, kw)
+        out = [torch.empty((c.B, h, c.T, c.D), dtype=c.dtype, device=c.dev)
+               for h in plan["heads"] if h]
+        if c.B and c.T:
+            with _on(c.dev):
+                rc = load_library().gs_qk_rotary(ctypes.byref(c.shape), c.split(parts),
+                                                 c.heads_first(out), _stream(c.dev))
+            _check(rc, "gs_qk_rotary")
+        return out
+
+    def qk_norm_rotary_grad(self, plan, parts, qw, kw, grads, *, want_x: bool, want_qw: bool,
+                            want_kw: bool):
+        """([input gradients] as parts or Nones, q weight gradient, k weight gradient):
+        gs_qk_rotary_grad; grads: the outputs' gradients, None for zeros."""
+        parts = [_features_contiguous(p) for p in parts]
+        c = _QKCall(plan, parts, qw, kw)
+        grads = c.gradients(grads)
+        dparts = [torch.empty(p.shape, dtype=c.dtype, device=c.dev) if want_x else None
+                  for p in parts]
+        make = torch.empty if c.B and c.T else torch.zeros
+        dqw = make(c.D, dtype=qw.dtype, device=c.dev) if want_qw else None
+        dkw = make(c.D, dtype=kw.dtype, device=c.dev) if want_kw else None
+        if c.B and c.T and (want_x or want_qw or want_kw):
+            with _on(c.dev):
+                lib = load_library()
+                nbytes = 0
+                if want_qw or want_kw:
+                    nbytes = lib.gs_qk_rotary_grad_workspace(ctypes.byref(c.shape))
+                ws = _workspace(nbytes, c.dev)
+                rc = lib.gs_qk_rotary_grad(
+                    ctypes.byref(c.shape), c.split(parts), c.heads_first(grads),
+                    c.split(dparts) if want_x else None, _ptr(dqw), _ptr(dkw), ws.data_ptr(),
+                    nbytes, _stream(c.dev))
+            _check(rc, "gs_qk_rotary_grad")
+        return dparts, dqw, dkw
+
+    def qk_norm_rotary_dots(self, plan, parts, qw, kw, grads, n_val: int, *, val_start=None,
+                            grad_scale: Optional[float] = None):
+        """(dot_q, dot_k, grad_q, grad_k) of the norm weights: gs_qk_rotary_dots; the train
+        gradients None without grad_scale."""
+        parts = [_features_contiguous(p) for p in parts]
+        c = _QKCall(plan, parts, qw, kw)
+        if not (c.B and c.T):
+            raise GhostHipError("qk_norm_rotary_dots: no tokens")
+        grads = c.gradients(grads)
+        n_t = c.B - n_val
+        vs = n_t if val_start is None else int(val_start)
+        dots = [torch.empty(max(n_t, 0), dtype=torch.float32, device=c.dev) for _ in range(2)]
+        gw = [None, None]
+        if grad_scale is not None:
+            gw = [torch.empty(c.D, dtype=c.dtype if w is None else w.dtype, device=c.dev)
+                  for w in (qw, kw)]
+        with _on(c.dev):
+            lib = load_library()
+            nbytes = lib.gs_qk_rotary_dots_workspace(ctypes.byref(c.shape))
+            ws = _workspace(nbytes, c.dev)
+            rc = lib.gs_qk_rotary_dots(
+                ctypes.byref(c.shape), c.split(parts), c.heads_first(grads), n_val, vs,
+                dots[0].data_ptr(), dots[1].data_ptr(), _ptr(gw[0]), _ptr(gw[1]),
+                float(grad_scale or 0.0), ws.data_ptr(), nbytes, _stream(c.dev))
+        _check(rc, "gs_qk_rotary_dots")
+        return dots[0], dots[1], gw[0], gw[1]
+
+    def _distill_args(self, logits, teacher_ids, teacher, labels, temperature, alpha,
+                      ignore_index, reduction):
+        """(struct, device, what it points to) of a gs_distill call, and logits as it reads them:
+        rows of V contiguous logits at one stride, or two for [B, T, V]."""
+        dev = _require_device(logits, teacher_ids, teacher, labels)
+        lead = logits.shape[:-1]
+        if logits.dim() < 1 or logits.shape[-1] == 0 or teacher.shape != teacher_ids.shape or \
+                teacher.dim() != logits.dim() or teacher.shape[:-1] != lead or \
+                teacher.shape[-1] == 0 or (labels is not None and labels.shape != lead):
+            raise GhostHipError(
+                f"logits {tuple(logits.shape)}, teacher ids {tuple(teacher_ids.shape)}, teacher "
+                f"logits {tuple(teacher.shape)}, labels "
+                f"{None if labels is None else tuple(labels.shape)}: [..., V], [..., K] twice and "
+                "[...] expected")
+        if labels is not None and labels.is_floating_point() or teacher_ids.is_floating_point():
+            raise GhostHipError("teacher ids and labels have to be integers")
+        d = _Distill()
+        d.dtype = _kernel_dtype(logits, "logits")
+        if teacher.dtype not in (torch.bfloat16, torch.float32):
+            teacher = teacher.float()
+        teacher, teacher_ids = teacher.contiguous(), teacher_ids.to(torch.int64).contiguous()
+        labels = None if labels is None else labels.to(torch.int64).contiguous()
+        d.N, d.V, d.K = math.prod(lead), logits.shape[-1], teacher.shape[-1]
+        logits = _rows_of_logits(logits)
+        d.inner, d.stride_outer, d.stride_inner = d.N, 0, d.V
+        if logits.dim() == 3:
+            d.inner = logits.shape[1]
+            d.stride_outer, d.stride_inner = logits.stride(0), logits.stride(1)
+        elif logits.dim() == 2:
+            d.stride_inner = logits.stride(0)
+        d.Z, d.teacher_ids, d.teacher = logits.data_ptr(), teacher_ids.data_ptr(), teacher.data_ptr()
+        d.labels = _ptr(labels)
+        d.teacher_dtype = _TORCH_TO_GS[teacher.dtype]
+        d.ignore_index, d.temperature, d.alpha = ignore_index, temperature, alpha
+        d.reduction = REDUCTIONS[reduction]
+        return d, dev, (logits, teacher_ids, teacher, labels)
+
+    def distill_loss(self, logits, teacher_ids, teacher_logits, labels, *, temperature: float,
+                     alpha: float, ignore_index: int, reduction: str, want_grad: bool = False):
+        """(loss, gradient for an upstream of one or None): gs_distill_loss."""
+        d, dev, held = self._distill_args(logits, teacher_ids, teacher_logits, labels, temperature,
+                                          alpha, ignore_index, reduction)
+        shape = logits.shape[:-1] if reduction == "none" else ()
+        if d.N == 0:
+            empty = math.nan if reduction == "mean" else 0.0
+            return (torch.full(shape, empty, device=dev),
+                    torch.empty_like(logits) if want_grad else None)
+        loss = torch.empty(shape, dtype=torch.float32, device=dev)
+        grad = _empty_as(held[0]) if want_grad else None
+        with _on(dev):
+            lib = load_library()
+            nbytes = lib.gs_distill_workspace(ctypes.byref(d))
+            ws = _workspace(nbytes, dev)
+            rc = lib.gs_distill_loss(ctypes.byref(d), loss.data_ptr(), _ptr(grad), ws.data_ptr(),
+                                     nbytes, _stream(dev))
+        _check(rc, "gs_distill_loss")
+        return loss, None if grad is None else grad.view(logits.shape)
+
+    def distill_grad(self, logits, teacher_ids, teacher_logits, labels, *, temperature: float,
+                     alpha: float, ignore_index: int, reduction: str, upstream: torch.Tensor,
+                     unit_grad: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The logits' gradient for a loss gradient `upstream`: gs_distill_grad.  unit_grad: the
+        gradient distill_loss gave, used up by this call."""
+        d, dev, held = self._distill_args(logits, teacher_ids, teacher_logits, labels, temperature,
+                                          alpha, ignore_index, reduction)
+        if d.N == 0:
+            return torch.empty_like(logits)
+        upstream = upstream.to(torch.float32).contiguous()
+        _require_device(logits, upstream)
+        grad = _empty_as(held[0]) if unit_grad is None else unit_grad
+        with _on(dev):
+            lib = load_library()
+            nbytes = lib.gs_distill_workspace(ctypes.byref(d))
+            ws = _workspace(nbytes, dev)
+            rc = lib.gs_distill_grad(ctypes.byref(d), upstream.data_ptr(),
+                                     int(unit_grad is not None), grad.data_ptr(), ws.data_ptr(),
+                                     nbytes, _stream(dev))
+        _check(rc, "gs_distill_grad")
+        return grad.view(logits.shape)
+
+
+def _rows_of_logits(z: torch.Tensor) -> torch.Tensor:
+    """z as [N, V] or [B, T, V] with contiguous, non-overlapping rows; a copy where its strides
+    do not allow that."""
+    V = z.shape[-1]
+    if z.dim() != 3:
+        z = z.reshape(-1, V)
+    T = z.shape[-2]
+    ok = (V == 1 or z.stride(-1) == 1) and (T == 1 or z.stride(-2) >= V)
+    if z.dim() == 3 and z.shape[0] > 1:
+        ok = ok and z.stride(0) >= (T - 1) * z.stride(1) + V
+    return z if ok else z.contiguous()
+
+
+def _empty_as(z: torch.Tensor) -> torch.Tensor:
+    """An uninitialised tensor of z's shape and strides at z's offset from a 16-byte boundary (the
+    kernels read and write the same 16-byte pieces of both)."""
+    esz = z.element_size()
+    off = z.data_ptr() % 16 // esz
+    span = 1 + sum((n - 1) * s for n, s in zip(z.shape, z.stride()))
+    base = torch.empty(off + span, dtype=z.dtype, device=z.device)
+    return base.as_strided(z.shape, z.stride(), off)
 
 
 _backend = None

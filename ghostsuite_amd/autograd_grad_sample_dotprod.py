@@ -19,6 +19,7 @@ import torch
 import torch.nn as nn
 
 from . import _overlap
+from .lm_layers import QKNormRotary
 from .supported_layers_grad_samplers_dotprod import (
     APPLIED,
     _param,
@@ -102,8 +103,15 @@ def _capture_activations(layer: nn.Module, inputs: Tuple, outputs: Tuple):
 def _prepare_sample_grad_or_dotprod(layer: nn.Module, grad_output: Tuple[torch.Tensor],
                                     val_batch_size: int, loss_reduction: str = 'mean'):
     """Backward-hook stage 1: the layer's dot products (reference :97-137)."""
-    backprops = grad_output[0].detach()
     d = layer.__dict__
+    others = ()
+    if isinstance(layer, QKNormRotary):   # three outputs, any of which may have no gradient
+        d["_gs_grad_outputs"] = others = tuple(None if g is None else g.detach()
+                                               for g in grad_output)
+        others += (d.get("_gs_positions"),)
+        backprops = next(g for g in others if g is not None)
+    else:
+        backprops = grad_output[0].detach()
     d.setdefault("activations", None)
     compute_layer_dotprod, _ = _supported_layers_dotprod.get(type(layer))
 
@@ -117,7 +125,7 @@ def _prepare_sample_grad_or_dotprod(layer: nn.Module, grad_output: Tuple[torch.T
 
     acts = d["activations"]
     # The dot kernels run on a side stream, overlapped with the rest of backward.
-    side = _overlap.on_side_stream(acts, backprops) \
+    side = _overlap.on_side_stream(acts, backprops, *others) \
         if options["overlap"] and _worth_overlapping(layer, acts, backprops) else \
         contextlib.nullcontext()
     with side:
@@ -163,7 +171,7 @@ def _apply_train_grad(layer: nn.Module, val_batch_size: int, loss_reduction: str
     finally:
         for attr in ('activations', 'backprops', 'backprops_scale', '_gs_bias_train_grad',
                      '_gs_weight_train_grad', '_gs_ln_train_grads', '_gs_bias_grad_scale',
-                     '_gs_ln_grad_scale'):
+                     '_gs_ln_grad_scale', '_gs_grad_outputs', '_gs_positions'):
             layer.__dict__.pop(attr, None)
 
 
@@ -186,7 +194,7 @@ def _worth_overlapping(layer: nn.Module, acts, backprops) -> bool:
         return True
     if acts.numel() + backprops.numel() > _INLINE_ELEMENTS:
         return True
-    if isinstance(layer, (nn.LayerNorm, nn.Embedding)):
+    if isinstance(layer, (nn.LayerNorm, nn.Embedding, QKNormRotary)):
         return False
     if isinstance(layer, nn.Conv2d):   # channels first: every output element takes a filter's size
         return 2.0 * backprops.numel() * layer.weight[0].numel() > _INLINE_FLOPS
@@ -196,7 +204,7 @@ def _worth_overlapping(layer: nn.Module, acts, backprops) -> bool:
 def _train_grads_parked(layer: nn.Module) -> bool:
     """True when the dot stage parked every train gradient this layer applies."""
     d = layer.__dict__
-    if isinstance(layer, nn.LayerNorm):
+    if isinstance(layer, (nn.LayerNorm, QKNormRotary)):
         return "_gs_ln_train_grads" in d
     w = _param(layer, "weight")
     if w is None or not getattr(w, "initially_requires_grad", False) or \
@@ -210,7 +218,7 @@ def _train_grads_parked(layer: nn.Module) -> bool:
 def _apply_train_grad_body(layer: nn.Module, compute_layer_train_grad, val_batch_size: int,
                            scale: float, loss_reduction: str):
     """The train gradients of one layer (weight, then bias) into ``param.train_grad``."""
-    if isinstance(layer, nn.LayerNorm):
+    if isinstance(layer, (nn.LayerNorm, QKNormRotary)):   # apply their gradients themselves
         compute_layer_train_grad(layer, layer.activations, layer.backprops, val_batch_size,
                                  scale=scale)
     else:

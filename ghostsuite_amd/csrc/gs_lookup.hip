@@ -1,0 +1,115 @@
+// Embedding lookup with a scale, gfx950:
+//
+//   out[i] = scale * W[id_i]        out: [n, d], W: [vocab, d]
+//
+// formed in fp32 and rounded once to W's dtype; ids outside [0, vocab) give rows of zeros.  For
+// the gradient (gs_embedding_train_grad over the same ids) the pass also writes the ids as the
+// gradient takes them: 64-bit, the padding id replaced by -1.
+//
+// Nothing is computed twice and every byte moves once, so the rate of a copy bounds it.  Each
+// thread owns one piece of the output (16 bytes, or one element where rows are not a whole number
+// of those): pieces are numbered through the whole output, so all lanes work whatever d is, and a
+// wave writes one contiguous range.
+#include <algorithm>
+
+#include "gs_common.h"
+
+namespace gs {
+namespace {
+
+constexpr int LK_THREADS = 256;
+constexpr int LK_PIECES = 4;   // per thread, loads of all in flight together
+
+__device__ __forceinline__ int64_t lk_id(const void* __restrict__ ids, int ids32, int64_t i) {
+  return ids32 ? static_cast<const int32_t*>(ids)[i] : static_cast<const int64_t*>(ids)[i];
+}
+
+// V: elements of a piece; ppr: pieces per row; pieces = n * ppr.
+template <class E, int V>
+__global__ void __launch_bounds__(LK_THREADS) lookup_kernel(
+    const void* __restrict__ ids, int ids32, int64_t n, const E* __restrict__ W, int64_t vocab,
+    int64_t d, int64_t ppr, float scale, int64_t padding, E* __restrict__ out,
+    int64_t* __restrict__ grad_ids) {
+  struct alignas(V * sizeof(E)) Piece { E e[V]; };
+  const int64_t p0 = static_cast<int64_t>(blockIdx.x) * (LK_THREADS * LK_PIECES);
+  const int64_t pieces = n * ppr;
+  // A workgroup's pieces are within few rows: one 64-bit division, then 32-bit ones.
+  const int64_t row0 = p0 / ppr;
+  const uint32_t col0 = static_cast<uint32_t>(p0 - row0 * ppr);
+  const uint32_t w = static_cast<uint32_t>(ppr);
+  Piece x[LK_PIECES];
+#pragma unroll
+  for (int k = 0; k < LK_PIECES; ++k) {
+    const uint32_t off = static_cast<uint32_t>(k * LK_THREADS + threadIdx.x);
+    if (p0 + off < pieces) {
+      const uint32_t c = col0 + off, r = c / w;
+      const int64_t i = row0 + r;
+      const uint32_t col = c - r * w;
+      const int64_t id = lk_id(ids, ids32, i);
+      if (id >= 0 && id < vocab) {
+        x[k] = *reinterpret_cast<const Piece*>(W + id * d + static_cast<int64_t>(col) * V);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[k].e[e] = from_f32<E>(0.f);
+      }
+      if (grad_ids != nullptr && col == 0) grad_ids[i] = id == padding ? -1 : id;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < LK_PIECES; ++k) {
+    const int64_t p = p0 + k * LK_THREADS + threadIdx.x;
+    if (p < pieces) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[k].e[e] = from_f32<E>(scale * to_f32<E>(x[k].e[e]));
+      *reinterpret_cast<Piece*>(out + p * V) = x[k];
+    }
+  }
+}
+
+template <class E, int V>
+int launch_lookup(const void* ids, int ids32, int64_t n, const void* W, int64_t vocab, int64_t d,
+                  float scale, int64_t padding, void* out, int64_t* grad_ids, hipStream_t s) {
+  const int64_t ppr = d / V;
+  const int64_t blocks = (n * ppr + LK_THREADS * LK_PIECES - 1) / (LK_THREADS * LK_PIECES);
+  hipLaunchKernelGGL((lookup_kernel<E, V>), dim3(static_cast<unsigned>(blocks)),
+                     dim3(LK_THREADS), 0, s, ids, ids32, n, static_cast<const E*>(W), vocab, d,
+                     ppr, scale, padding, static_cast<E*>(out), grad_ids);
+  return check_launch("lookup_kernel");
+}
+
+template <class E>
+int launch_lookup_any(const void* ids, int ids32, int64_t n, const void* W, int64_t vocab,
+                      int64_t d, float scale, int64_t padding, void* out, int64_t* grad_ids,
+                      hipStream_t s) {
+  constexpr int V = 16 / sizeof(E);
+  const bool whole = d % V == 0 && reinterpret_cast<uintptr_t>(W) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  return whole ? launch_lookup<E, V>(ids, ids32, n, W, vocab, d, scale, padding, out, grad_ids, s)
+               : launch_lookup<E, 1>(ids, ids32, n, W, vocab, d, scale, padding, out, grad_ids, s);
+}
+
+}  // namespace
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" int gs_embedding_lookup(const void* ids, int ids_bits, int64_t n, const void* W,
+                                   int dtype, int64_t vocab, int64_t d, float scale,
+                                   int64_t padding_idx, void* out, int64_t* grad_ids,
+                                   void* stream) {
+  if (dtype != GS_DTYPE_BF16 && dtype != GS_DTYPE_F32)
+    return fail(GS_ERR_DTYPE, "gs_embedding_lookup: dtype must be bf16 or fp32");
+  if (ids == nullptr || W == nullptr || out == nullptr || n <= 0 || vocab <= 0 || d <= 0 ||
+      (ids_bits != 32 && ids_bits != 64))
+    return fail(GS_ERR_INVALID, "gs_embedding_lookup: invalid arguments");
+  // 32-bit piece numbers within a workgroup; the grid's x.
+  if (d >= (int64_t{1} << 30) || n > (int64_t{INT32_MAX} * LK_THREADS) / d)
+    return fail(GS_ERR_UNSUPPORTED, "gs_embedding_lookup: 2^30 features or 2^39 elements or more");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int ids32 = ids_bits == 32;
+  return dtype == GS_DTYPE_BF16
+             ? launch_lookup_any<uint16_t>(ids, ids32, n, W, vocab, d, scale, padding_idx, out,
+                                           grad_ids, s)
+             : launch_lookup_any<float>(ids, ids32, n, W, vocab, d, scale, padding_idx, out,
+                                        grad_ids, s);
+}

@@ -1,0 +1,793 @@
+// Per-head norms of queries and keys with their rotation by position, gfx950.  Per head row x of
+// D features (queries and keys, each with a weight w):
+//
+//   r = (mean x^2 + eps)^(-1/2)    u = w x r                       (norm; else u = x)
+//   (y_a, y_b) = (u_a c - u_b s, u_b c + u_a s)   for the n_rot / 2 pairs (a, b), c and s the
+//                cosine and sine of the row's position; the features past n_rot stay as u
+//
+// and values are copied, all into heads-first layout [B, H, T, D].  Backward, with h = R^T g (the
+// rotation by -angle):
+//
+//   dw = sum h x r      dx = r (w h - x r mean(w h x r))
+//
+// Everything in fp32 registers, rounded once at the end; a row is read once and written once, so
+// the rate of a copy bounds both passes.  A row is cut into units of two chunks: for pairs half
+// the rotated width apart a unit holds chunk [V u, V u + V) of each half, for neighbouring pairs
+// 2 V features in a row, so that a pair's two features are always in one lane and only the row
+// sums cross lanes.  A group of 2^k lanes owns a row; it takes one token, keeps the token's
+// angles and the lane's weights in registers, and walks that token's heads, so the angles are
+// read once per token and the groups of a wave write neighbouring rows of one head.
+//
+// V is 16 bytes of features where the widths and strides allow it, else 2 or 1 features.
+//
+// Weight gradients: a lane adds up its features over its tokens and heads, a workgroup adds its
+// groups through LDS in a fixed order and leaves one fp32 row; a second launch adds those per
+// sample or in all, also in a fixed order (the same bits on every run).
+#include <algorithm>
+
+#include "gs_common.h"
+
+namespace gs {
+namespace {
+
+constexpr int QK_THREADS = 256;
+constexpr int QK_BATCH = 4;      // heads whose loads are in flight together
+
+// Rows of one of the three parts (queries, keys, values): element (b, t, h, f) at
+// p[b sb + t st + h sh + f].
+struct QkRows {
+  char* p;
+  int64_t sb, st, sh;
+};
+
+struct QkArgs {
+  QkRows x[3];       // layer input rows (forward and backward)
+  QkRows g[3];       // forward: the outputs; backward: the output gradients (p may be null)
+  QkRows dx[3];      // backward: input gradients (p null: not formed)
+  const void* w[2];  // query / key weights, or null: ones
+  int w_bf16[2];
+  int heads[3];
+  int64_t B, T;      // samples and tokens of each
+  int D, rot, lanes_log2;   // features, rotated features, log2 of the lanes of a row
+  int norm;
+  float eps;
+  const float* table;       // [positions][2][rot / 2]: cosines, sines
+  int64_t n_pos;
+  const void* pos;          // null: a token's place in its sample
+  int pos_bits;
+  int64_t pos_sb, pos_st;
+  // The work of a workgroup: tokens [y * span, + span) of its segment (the segments: one of B T
+  // tokens, or B of T), heads [h0, h0 + per) of a part.
+  int64_t segments, seg_tokens, span, chunks;
+  int groups[3], per[3];    // head groups of each part, heads of a group
+  float* part[2];           // [segment][chunk][group][D] weight-gradient sums (backward)
+};
+
+template <class E, int V>
+struct alignas(V * sizeof(E)) QkChunk {
+  E e[V];
+};
+
+// Lane-local view of a row: unit j of this lane and its two chunks' places.
+template <int V, bool INTER>
+struct QkPlace {
+  int o0, o1;     // first features of the chunks (>= D: nothing there)
+  int pair;       // first pair of the unit's angles (half: pairs [pair, pair + V))
+  __device__ QkPlace(int u, int D, int rot) {
+    if (INTER) {
+      o0 = 2 * V * u;
+      o1 = o0 + V;
+      pair = V * u;
+    } else {
+      const int half = rot / 2, nr = half / V;   // V divides half
+      if (u < nr) {
+        o0 = V * u;
+        o1 = half + V * u;
+        pair = V * u;
+      } else {
+        o0 = rot + 2 * V * (u - nr);
+        o1 = o0 + V;
+        pair = half;
+      }
+    }
+    if (o0 >= D) o0 = D;
+    if (o1 >= D) o1 = D;
+  }
+};
+
+template <class E, int V>
+__device__ __forceinline__ void qk_load(const E* __restrict__ row, int o, int D, float (&x)[V]) {
+  if (o < D) {
+    const QkChunk<E, V> c = *reinterpret_cast<const QkChunk<E, V>*>(row + o);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = to_f32<E>(c.e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = 0.f;
+  }
+}
+
+template <class E, int V>
+__device__ __forceinline__ void qk_store(E* __restrict__ row, int o, int D, const float (&x)[V]) {
+  if (o < D) {
+    QkChunk<E, V> c;
+#pragma unroll
+    for (int i = 0; i < V; ++i) c.e[i] = from_f32<E>(x[i]);
+    *reinterpret_cast<QkChunk<E, V>*>(row + o) = c;
+  }
+}
+
+// One unit's values: the two chunks.
+template <int V>
+struct QkUnit {
+  float a[V], b[V];
+};
+
+// The rotation of a unit by its angles (sign +1) or back (-1).
+template <int V, bool INTER>
+__device__ __forceinline__ void qk_rotate(QkUnit<V>& u, const float (&c)[V], const float (&s)[V],
+                                          float sign) {
+  if constexpr (!INTER) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float x = u.a[i], y = u.b[i], si = sign * s[i];
+      u.a[i] = x * c[i] - y * si;
+      u.b[i] = y * c[i] + x * si;
+    }
+  } else {
+    // Pair i is features 2 i and 2 i + 1 of the unit's 2 V.
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float& x = 2 * i < V ? u.a[2 * i < V ? 2 * i : 0] : u.b[2 * i < V ? 0 : 2 * i - V];
+      float& y = 2 * i + 1 < V ? u.a[2 * i + 1 < V ? 2 * i + 1 : 0]
+                               : u.b[2 * i + 1 < V ? 0 : 2 * i + 1 - V];
+      const float x0 = x, y0 = y, si = sign * s[i];
+      x = x0 * c[i] - y0 * si;
+      y = y0 * c[i] + x0 * si;
+    }
+  }
+}
+
+// The sum over the 2^k lanes of a row's group, in each of them.
+__device__ __forceinline__ float qk_group_sum(float v, int lanes_log2) {
+  for (int k = 0; k < lanes_log2; ++k) v += __shfl_xor(v, 1 << k, 64);
+  return v;
+}
+
+__device__ __forceinline__ int64_t qk_position(const QkArgs& a, int64_t b, int64_t t) {
+  if (a.pos == nullptr) return t;
+  const int64_t i = b * a.pos_sb + t * a.pos_st;
+  return a.pos_bits == 32 ? static_cast<const int32_t*>(a.pos)[i]
+                          : static_cast<const int64_t*>(a.pos)[i];
+}
+
+// Cosines and sines of a unit's pairs at a position; those past the rotated features: 1 and 0; a
+// position outside the table: NaN.
+template <int V>
+__device__ __forceinline__ void qk_angles(const QkArgs& a, int64_t pos, int pair, float (&c)[V],
+                                          float (&s)[V]) {
+  const int half = a.rot / 2;
+  const bool in = pos >= 0 && pos < a.n_pos;
+  const float* row = a.table + (in ? pos : 0) * a.rot;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const bool turns = pair + i < half;
+    c[i] = turns ? (in ? row[pair + i] : __builtin_nanf("")) : 1.f;
+    s[i] = turns ? (in ? row[half + pair + i] : __builtin_nanf("")) : 0.f;
+  }
+}
+
+__device__ __forceinline__ float qk_weight(const QkArgs& a, int part, int f) {
+  if (a.w[part] == nullptr || f >= a.D) return 1.f;
+  return a.w_bf16[part] ? bf16_to_f32(static_cast<const uint16_t*>(a.w[part])[f])
+                        : static_cast<const float*>(a.w[part])[f];
+}
+
+// The workgroup's part, head range and token range.
+struct QkBlock {
+  int part, h0, h1, group;
+  int64_t seg, chunk, m0, m1;   // tokens [m0, m1), numbered over all samples
+  __device__ explicit QkBlock(const QkArgs& a) {
+    int y = blockIdx.y;
+    part = 0;
+    while (part < 2 && y >= a.groups[part]) y -= a.groups[part++];
+    group = y;
+    h0 = y * a.per[part];
+    h1 = min(a.heads[part], h0 + a.per[part]);
+    seg = blockIdx.x / a.chunks;
+    chunk = blockIdx.x - seg * a.chunks;
+    m0 = seg * a.seg_tokens + chunk * a.span;
+    m1 = min(m0 + a.span, (seg + 1) * a.seg_tokens);
+  }
+};
+
+template <class E, int V, int UPL, bool INTER>
+__global__ void __launch_bounds__(QK_THREADS) qk_forward_kernel(QkArgs a) {
+  const QkBlock blk(a);
+  const int lanes = 1 << a.lanes_log2;
+  const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x >> a.lanes_log2;
+  const int slots = QK_THREADS >> a.lanes_log2;
+  const bool turn = blk.part < 2 && a.rot > 0, norm = blk.part < 2 && a.norm;
+  QkUnit<V> w[UPL];
+  if (norm) {
+#pragma unroll
+    for (int j = 0; j < UPL; ++j) {
+      const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        w[j].a[i] = qk_weight(a, blk.part, pl.o0 + i);
+        w[j].b[i] = qk_weight(a, blk.part, pl.o1 + i);
+      }
+    }
+  }
+  const QkRows in = a.x[blk.part], out = a.g[blk.part];
+  const float inv_d = 1.f / static_cast<float>(a.D);
+  for (int64_t m = blk.m0 + slot; m < blk.m1; m += slots) {
+    const int64_t b = m / a.T, t = m - b * a.T;
+    float c[UPL][V], s[UPL][V];
+    if (turn) {
+      const int64_t pos = qk_position(a, b, t);
+#pragma unroll
+      for (int j = 0; j < UPL; ++j) {
+        const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
+        qk_angles<V>(a, pos, pl.pair, c[j], s[j]);
+      }
+    }
+    const E* xr = reinterpret_cast<const E*>(in.p) + b * in.sb + t * in.st;
+    E* yr = reinterpret_cast<E*>(out.p) + b * out.sb + t * out.st;
+    for (int h = blk.h0; h < blk.h1; h += QK_BATCH) {
+      QkUnit<V> u[QK_BATCH][UPL];
+#pragma unroll
+      for (int q = 0; q < QK_BATCH; ++q) {
+        const int hh = min(h + q, blk.h1 - 1);
+#pragma unroll
+        for (int j = 0; j < UPL; ++j) {
+          const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
+          qk_load<E, V>(xr + hh * in.sh, pl.o0, a.D, u[q][j].a);
+          qk_load<E, V>(xr + hh * in.sh, pl.o1, a.D, u[q][j].b);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < QK_BATCH; ++q) {
+        if (norm) {
+          float ss = 0.f;
+#pragma unroll
+          for (int j = 0; j < UPL; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+              ss += u[q][j].a[i] * u[q][j].a[i] + u[q][j].b[i] * u[q][j].b[i];
+          const float r = rsqrtf(qk_group_sum(ss, a.lanes_log2) * inv_d + a.eps);
+#pragma unroll
+          for (int j = 0; j < UPL; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              u[q][j].a[i] *= r * w[j].a[i];
+              u[q][j].b[i] *= r * w[j].b[i];
+            }
+        }
+        if (h + q < blk.h1) {
+#pragma unroll
+          for (int j = 0; j < UPL; ++j) {
+            if (turn) qk_rotate<V, INTER>(u[q][j], c[j], s[j], 1.f);
+            const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
+            qk_store<E, V>(yr + (h + q) * out.sh, pl.o0, a.D, u[q][j].a);
+            qk_store<E, V>(yr + (h + q) * out.sh, pl.o1, a.D, u[q][j].b);
+          }
+        }
+      }
+    }
+  }
+}
+
+template <class E, int V, int UPL, bool INTER>
+__global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(QkArgs a) {
+  const QkBlock blk(a);
+  const int lanes = 1 << a.lanes_log2;
+  const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x >> a.lanes_log2;
+  const int slots = QK_THREADS >> a.lanes_log2;
+  const QkRows in = a.x[blk.part], go = a.g[blk.part], dx = a.dx[blk.part];
+  const bool any_g = go.p != nullptr;   // else every gradient of the part is zero
+  const bool turn = blk.part < 2 && a.rot > 0 && any_g, norm = blk.part < 2 && a.norm && any_g;
+  const bool want_w = blk.part < 2 && a.part[blk.part] != nullptr;
+  QkUnit<V> w[UPL], dw[UPL];
+#pragma unroll
+  for (int j = 0; j < UPL; ++j) {
+    const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      w[j].a[i] = norm ? qk_weight(a, blk.part, pl.o0 + i) : 1.f;
+      w[j].b[i] = norm ? qk_weight(a, blk.part, pl.o1 + i) : 1.f;
+      dw[j].a[i] = dw[j].b[i] = 0.f;
+    }
+  }
+  const float inv_d = 1.f / static_cast<float>(a.D);
+  for (int64_t m = blk.m0 + slot; m < blk.m1; m += slots) {
+    const int64_t b = m / a.T, t = m - b * a.T;
+    float c[UPL][V], s[UPL][V];
+    if (turn) {
+      const int64_t pos = qk_position(a, b, t);
+#pragma unroll
+      for (int j = 0; j < UPL; ++j) {
+        const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
+        qk_angles<V>(a, pos, pl.pair, c[j], s[j]);
+      }
+    }
+    const E* xr = reinterpret_cast<const E*>(in.p) + b * in.sb + t * in.st;
+    const E* gr = reinterpret_cast<const E*>(go.p) + b * go.sb + t * go.st;
+    E* dr = reinterpret_cast<E*>(dx.p) + b * dx.sb + t * dx.st;
+    for (int h = blk.h0; h < blk.h1; ++h) {
+      QkUnit<V> x[UPL], g[UPL];
+#pragma unroll
+      for (int j = 0; j < UPL; ++j) {
+        const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
+        qk_load<E, V>(gr + h * go.sh, any_g ? pl.o0 : a.D, a.D, g[j].a);
+        qk_load<E, V>(gr + h * go.sh, any_g ? pl.o1 : a.D, a.D, g[j].b);
+        if (norm) {
+          qk_load<E, V>(xr + h * in.sh, pl.o0, a.D, x[j].a);
+          qk_load<E, V>(xr + h * in.sh, pl.o1, a.D, x[j].b);
+        }
+      }
+      if (turn) {
+#pragma unroll
+        for (int j = 0; j < UPL; ++j) qk_rotate<V, INTER>(g[j], c[j], s[j], -1.f);
+      }
+      if (norm) {
+        float ss = 0.f, sd = 0.f;
+#pragma unroll
+        for (int j = 0; j < UPL; ++j)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            ss += x[j].a[i] * x[j].a[i] + x[j].b[i] * x[j].b[i];
+            sd += w[j].a[i] * g[j].a[i] * x[j].a[i] + w[j].b[i] * g[j].b[i] * x[j].b[i];
+          }
+        ss = qk_group_sum(ss, a.lanes_log2);
+        sd = qk_group_sum(sd, a.lanes_log2);
+        const float r = rsqrtf(ss * inv_d + a.eps);
+        const float k = sd * r * r * inv_d;   // mean(w h x r) r
+#pragma unroll
+        for (int j = 0; j < UPL; ++j)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            dw[j].a[i] += g[j].a[i] * (x[j].a[i] * r);
+            dw[j].b[i] += g[j].b[i] * (x[j].b[i] * r);
+            g[j].a[i] = r * (w[j].a[i] * g[j].a[i] - x[j].a[i] * k);
+            g[j].b[i] = r * (w[j].b[i] * g[j].b[i] - x[j].b[i] * k);
+          }
+      }
+      if (dx.p != nullptr) {
+#pragma unroll
+        for (int j = 0; j < UPL; ++j) {
+          const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
+          qk_store<E, V>(dr + h * dx.sh, pl.o0, a.D, g[j].a);
+          qk_store<E, V>(dr + h * dx.sh, pl.o1, a.D, g[j].b);
+        }
+      }
+    }
+  }
+  if (!want_w) return;   // the same for the whole workgroup
+  // The workgroup's sum: groups of a wave by shuffles, waves through LDS, in wave order.
+  __shared__ float red[QK_THREADS / 64][2 * V * UPL * 64];
+  const int wid = threadIdx.x >> 6, wl = threadIdx.x & 63;
+#pragma unroll
+  for (int j = 0; j < UPL; ++j)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float p = dw[j].a[i], q = dw[j].b[i];
+      for (int k = lanes; k < 64; k <<= 1) {
+        p += __shfl_xor(p, k, 64);
+        q += __shfl_xor(q, k, 64);
+      }
+      if (wl < lanes) {
+        red[wid][((j * 2 + 0) * V + i) * 64 + wl] = p;
+        red[wid][((j * 2 + 1) * V + i) * 64 + wl] = q;
+      }
+    }
+  __syncthreads();
+  float* out = a.part[blk.part] +
+               ((blk.seg * a.chunks + blk.chunk) * a.groups[blk.part] + blk.group) * a.D;
+  for (int k = threadIdx.x; k < 2 * V * UPL * lanes; k += QK_THREADS) {
+    const int l = k & (lanes - 1), v = k >> a.lanes_log2;   // v = (j * 2 + side) * V + i
+    const int i = v % V, side = (v / V) & 1, j = v / (2 * V);
+    const QkPlace<V, INTER> pl(l + j * lanes, a.D, a.rot);
+    const int f = (side ? pl.o1 : pl.o0) + i;
+    float t = 0.f;
+#pragma unroll
+    for (int q = 0; q < QK_THREADS / 64; ++q) t += red[q][v * 64 + l];
+    if (f < a.D) out[f] = t;
+  }
+}
+
+// Sums of the partial rows.  Row y of the grid below `samples`: out[part][y][f] = the sum of sample
+// y's rows; y = samples: `val`, the val samples' rows; y = samples + 1 (or y = 0 without samples):
+// the train samples' rows times the scale, as a weight gradient.  Partial rows lie in sample order,
+// so each is one range of rows or two.  A workgroup takes 16 features; its 64 groups of 16 threads
+// take every 64th row and are added in a fixed order.
+constexpr int QR_COLS = 16, QR_GROUPS = 64;
+struct QkSums {
+  const float* part[2];
+  int64_t rows[2];      // partial rows of a sample (all of them without samples)
+  int64_t samples;      // 0: only the train sum, over everything
+  int64_t n_val, val_start;
+  float* out[2];        // [samples][D]
+  float* val[2];        // [D]
+  void* grad[2];        // [D] or null
+  int grad_bf16[2];
+  float scale;
+  int D;
+};
+__global__ void __launch_bounds__(QR_COLS * QR_GROUPS) qk_sums_kernel(QkSums q) {
+  __shared__ float red[QR_GROUPS][QR_COLS];
+  const int part = blockIdx.z;
+  const int64_t y = blockIdx.y;
+  const int col = threadIdx.x % QR_COLS, grp = threadIdx.x / QR_COLS;
+  const int f = blockIdx.x * QR_COLS + col;
+  const int64_t rows = q.rows[part], n = q.samples > 0 ? q.samples : 1;
+  const bool is_sample = y < q.samples, is_val = y == q.samples && q.samples > 0;
+  const int64_t v0 = q.samples > 0 ? q.val_start : n, v1 = v0 + q.n_val;
+  const int64_t lo[2] = {is_sample ? y : is_val ? v0 : 0, is_sample || is_val ? 0 : v1};
+  const int64_t hi[2] = {is_sample ? y + 1 : is_val ? v1 : v0, is_sample || is_val ? 0 : n};
+  float t0 = 0.f, t1 = 0.f;
+  if (f < q.D && q.part[part] != nullptr) {
+    const float* p = q.part[part] + f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      int64_t r = lo[k] * rows + grp;
+      const int64_t end = hi[k] * rows;
+      for (; r + QR_GROUPS < end; r += 2 * QR_GROUPS) {
+        t0 += p[r * q.D];
+        t1 += p[(r + QR_GROUPS) * q.D];
+      }
+      if (r < end) t0 += p[r * q.D];
+    }
+  }
+  red[grp][col] = t0 + t1;
+  for (int k = QR_GROUPS / 2; k > 0; k >>= 1) {
+    __syncthreads();
+    if (grp < k) red[grp][col] += red[grp + k][col];
+  }
+  if (grp != 0 || f >= q.D) return;
+  const float t = red[0][col];
+  if (is_sample) {
+    q.out[part][y * q.D + f] = t;
+  } else if (is_val) {
+    q.val[part][f] = t;
+  } else if (q.grad[part] != nullptr) {
+    if (q.grad_bf16[part])
+      static_cast<uint16_t*>(q.grad[part])[f] = f32_to_bf16(q.scale * t);
+    else
+      static_cast<float*>(q.grad[part])[f] = q.scale * t;
+  }
+}
+
+// dot[part][i] = <S[part][train sample i], val[part]>, a wave each.
+struct QkDots {
+  const float* S[2];
+  const float* val[2];
+  float* dot[2];
+};
+__global__ void __launch_bounds__(64) qk_dots_kernel(QkDots q, RowMap train, int D) {
+  const int part = blockIdx.y;
+  if (q.dot[part] == nullptr) return;
+  const float* row = q.S[part] + train.phys_sample(blockIdx.x) * D;
+  float t = 0.f;
+  for (int f = threadIdx.x; f < D; f += 64) t += row[f] * q.val[part][f];
+  t = wave_sum(t);
+  if (threadIdx.x == 0) q.dot[part][blockIdx.x] = t;
+}
+
+constexpr int QK_MAX_D = 512;
+
+// Features a lane takes at once: 16 bytes of them where every row starts and splits there.
+int qk_vec(const QkArgs& a, size_t esz, bool inter, bool backward) {
+  const int half = a.rot / 2;
+  for (int v : {static_cast<int>(16 / esz), 2}) {
+    bool ok = a.D % v == 0 && (inter || half % v == 0) && (inter || a.rot % v == 0);
+    for (int k = 0; k < 3 && ok; ++k) {
+      if (a.heads[k] == 0) continue;
+      for (const QkRows* r : {&a.x[k], &a.g[k], &a.dx[k]}) {
+        if (r == &a.dx[k] && !backward) continue;
+        if (r->p == nullptr) continue;
+        ok = ok && reinterpret_cast<uintptr_t>(r->p) % (v * esz) == 0 && r->sb % v == 0 &&
+             r->st % v == 0 && r->sh % v == 0;
+      }
+    }
+    if (ok) return v;
+  }
+  return 1;
+}
+
+int qk_units(int D, int rot, int V, bool inter) {
+  if (inter) return (D + 2 * V - 1) / (2 * V);
+  return rot / 2 / V + (D - rot + 2 * V - 1) / (2 * V);
+}
+
+int ceil_log2(int64_t x) {
+  int k = 0;
+  while ((int64_t{1} << k) < x) ++k;
+  return k;
+}
+
+// How the work is shared out.  Head groups and token spans are made so that there are about
+// QK_WAVES waves (8 for each SIMD) while the work lasts: longer walks reuse the angles and, in the
+// backward pass, add more into a lane before the workgroup's sum.  Per-sample sums cut the spans
+// at samples.
+constexpr int64_t QK_WAVES = 8192;
+void qk_share(QkArgs& a, int upl, int units, bool per_sample) {
+  a.lanes_log2 = std::min(6, ceil_log2((units + upl - 1) / upl));
+  const int64_t slots = QK_THREADS >> a.lanes_log2;
+  a.segments = per_sample ? a.B : 1;
+  a.seg_tokens = per_sample ? a.T : a.B * a.T;
+  a.span = std::min<int64_t>(slots, a.seg_tokens);
+  a.chunks = (a.seg_tokens + a.span - 1) / a.span;
+  const int total = a.heads[0] + a.heads[1] + a.heads[2];
+  const int64_t want = std::max<int64_t>(1, QK_WAVES / (QK_THREADS / 64));
+  // groups of heads for the workgroups wanted, at least one head each
+  const int64_t y = std::max<int64_t>(1, std::min<int64_t>(total, want / (a.segments * a.chunks)));
+  const int per = static_cast<int>((total + y - 1) / y);
+  for (int k = 0; k < 3; ++k) {
+    a.groups[k] = (a.heads[k] + per - 1) / per;
+    a.per[k] = a.groups[k] ? (a.heads[k] + a.groups[k] - 1) / a.groups[k] : 1;
+  }
+  // more tokens to a workgroup where that still leaves enough of them
+  const int64_t gy = a.groups[0] + a.groups[1] + a.groups[2];
+  const int64_t times = std::max<int64_t>(1, a.segments * a.chunks * gy / want);
+  a.span = std::min<int64_t>(a.span * times, a.seg_tokens);
+  a.chunks = (a.seg_tokens + a.span - 1) / a.span;
+}
+
+template <class E, bool BWD, bool INTER>
+int qk_launch(const QkArgs& a, int v, hipStream_t s) {
+  constexpr int V16 = 16 / sizeof(E);
+  const dim3 grid(static_cast<unsigned>(a.segments * a.chunks),
+                  static_cast<unsigned>(a.groups[0] + a.groups[1] + a.groups[2]));
+#define GS_QK_GO(V, UPL)                                                                       \
+  do {                                                                                         \
+    if constexpr (BWD)                                                                         \
+      hipLaunchKernelGGL((qk_backward_kernel<E, V, UPL, INTER>), grid, dim3(QK_THREADS), 0, s, \
+                         a);                                                                   \
+    else                                                                                       \
+      hipLaunchKernelGGL((qk_forward_kernel<E, V, UPL, INTER>), grid, dim3(QK_THREADS), 0, s,  \
+                         a);                                                                   \
+  } while (0)
+  if (v == V16)
+    GS_QK_GO(V16, 1);
+  else if (v == 2)
+    GS_QK_GO(2, 2);
+  else
+    GS_QK_GO(1, 4);
+#undef GS_QK_GO
+  return check_launch(BWD ? "qk_backward_kernel" : "qk_forward_kernel");
+}
+
+int qk_units_per_lane(int v, size_t esz) {
+  return v == static_cast<int>(16 / esz) ? 1 : v == 2 ? 2 : 4;
+}
+
+template <bool BWD>
+int qk_run(const QkArgs& a, int dtype, bool inter, int v, hipStream_t s) {
+  if (dtype == GS_DTYPE_BF16)
+    return inter ? qk_launch<uint16_t, BWD, true>(a, v, s)
+                 : qk_launch<uint16_t, BWD, false>(a, v, s);
+  return inter ? qk_launch<float, BWD, true>(a, v, s) : qk_launch<float, BWD, false>(a, v, s);
+}
+
+QkRows rows_of(const gs_qk_rows& r) {
+  return QkRows{static_cast<char*>(r.data), r.stride_b, r.stride_t, r.stride_h};
+}
+
+// Fills the common arguments; a status other than GS_OK refuses the call.
+int qk_args(QkArgs& a, const char* name, const gs_qk_shape* sh, const gs_qk_rows x[3],
+            const gs_qk_rows g[3], const gs_qk_rows dx[3]) {
+  const std::string n(name);
+  if (sh == nullptr) return fail(GS_ERR_INVALID, n + ": no shape");
+  if (sh->dtype != GS_DTYPE_BF16 && sh->dtype != GS_DTYPE_F32)
+    return fail(GS_ERR_DTYPE, n + ": dtype must be bf16 or fp32");
+  for (int k = 0; k < 2; ++k)
+    if (sh->weight[k] != nullptr && sh->weight_dtype[k] != GS_DTYPE_BF16 &&
+        sh->weight_dtype[k] != GS_DTYPE_F32)
+      return fail(GS_ERR_DTYPE, n + ": weight dtypes must be bf16 or fp32");
+  if (sh->B <= 0 || sh->T <= 0 || sh->D <= 0 || sh->n_rot < 0 || sh->n_rot > sh->D ||
+      sh->n_rot % 2 != 0 || sh->heads[0] < 0 || sh->heads[1] < 0 || sh->heads[2] < 0 ||
+      sh->heads[0] + sh->heads[1] + sh->heads[2] <= 0 || !(sh->eps >= 0.f) ||
+      (sh->positions != nullptr && sh->position_bits != 32 && sh->position_bits != 64) ||
+      (sh->n_rot > 0 && (sh->table == nullptr || sh->n_positions <= 0)))
+    return fail(GS_ERR_INVALID, n + ": invalid arguments");
+  if (sh->D > QK_MAX_D)
+    return fail(GS_ERR_UNSUPPORTED, n + ": more than 512 features to a head");
+  // the grid's y, 32-bit head numbers, and the token count in the grid's x
+  if (static_cast<int64_t>(sh->heads[0]) + sh->heads[1] + sh->heads[2] > 65535 ||
+      sh->B > INT32_MAX / sh->T)
+    return fail(GS_ERR_UNSUPPORTED, n + ": more than 65535 heads or 2^31 tokens");
+  a = QkArgs{};
+  for (int k = 0; k < 3; ++k) {
+    a.heads[k] = sh->heads[k];
+    if (a.heads[k] == 0) continue;
+    if (x != nullptr) a.x[k] = rows_of(x[k]);
+    if (g != nullptr) a.g[k] = rows_of(g[k]);
+    if (dx != nullptr) a.dx[k] = rows_of(dx[k]);
+  }
+  for (int k = 0; k < 2; ++k) {
+    a.w[k] = sh->weight[k];
+    a.w_bf16[k] = sh->weight_dtype[k] == GS_DTYPE_BF16;
+  }
+  a.B = sh->B, a.T = sh->T, a.D = static_cast<int>(sh->D), a.rot = static_cast<int>(sh->n_rot);
+  a.norm = sh->norm, a.eps = sh->eps;
+  a.table = sh->table, a.n_pos = sh->n_positions;
+  a.pos = sh->positions, a.pos_bits = sh->position_bits;
+  a.pos_sb = sh->position_stride_b, a.pos_st = sh->position_stride_t;
+  return GS_OK;
+}
+
+struct QkPlan {
+  int v;
+  int64_t rows[2];   // partial rows of a segment
+};
+
+QkPlan qk_plan(QkArgs& a, int dtype, bool inter, bool backward, bool per_sample, int force_v = 0) {
+  QkPlan p;
+  const size_t esz = elem_size(dtype);
+  p.v = force_v ? force_v : qk_vec(a, esz, inter, backward);
+  qk_share(a, qk_units_per_lane(p.v, esz), qk_units(a.D, a.rot, p.v, inter), per_sample);
+  for (int k = 0; k < 2; ++k) p.rows[k] = a.chunks * a.groups[k];
+  return p;
+}
+
+struct QkScratch {
+  float *part[2], *sums[2], *val[2];
+  template <class S>
+  QkScratch(S& c, const QkArgs& a, const QkPlan& p, bool per_sample) {
+    for (int k = 0; k < 2; ++k) {
+      part[k] = c.template take<float>(a.segments * p.rows[k] * a.D);
+      sums[k] = c.template take<float>(per_sample ? a.segments * a.D : 0);
+      val[k] = c.template take<float>(per_sample ? a.D : 0);
+    }
+  }
+};
+
+// The strides decide the vector width and so the plan; the query does not know them, so it takes
+// the most any plan needs, with and without the values' heads.
+size_t qk_workspace(const gs_qk_shape* sh, bool per_sample) {
+  QkArgs a;
+  if (qk_args(a, "gs_qk_rotary", sh, nullptr, nullptr, nullptr) != GS_OK) return 0;
+  size_t most = 0;
+  for (int values : {a.heads[2], 0}) {
+    for (int v : {static_cast<int>(16 / elem_size(sh->dtype)), 2, 1}) {
+      QkArgs t = a;
+      t.heads[2] = values;
+      if (t.heads[0] + t.heads[1] == 0 || (sh->interleaved == 0 && a.rot / 2 % v != 0)) continue;
+      const QkPlan p = qk_plan(t, sh->dtype, sh->interleaved != 0, true, per_sample, v);
+      Sizer sz;
+      QkScratch unused(sz, t, p, per_sample);
+      most = std::max(most, sz.used);
+    }
+  }
+  return most + 256;
+}
+
+int qk_check_rows(const char* name, const gs_qk_shape* sh, const gs_qk_rows* r, bool needed) {
+  for (int k = 0; k < 3; ++k)
+    if (needed && sh->heads[k] > 0 && r[k].data == nullptr)
+      return fail(GS_ERR_INVALID, std::string(name) + ": invalid arguments");
+  return GS_OK;
+}
+
+}  // namespace
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" int gs_qk_rotary(const gs_qk_shape* shape, const gs_qk_rows x[3],
+                            const gs_qk_rows y[3], void* stream) {
+  QkArgs a;
+  if (int rc = qk_args(a, "gs_qk_rotary", shape, x, y, nullptr)) return rc;
+  if (x == nullptr || y == nullptr || qk_check_rows("gs_qk_rotary", shape, x, true) != GS_OK ||
+      qk_check_rows("gs_qk_rotary", shape, y, true) != GS_OK)
+    return fail(GS_ERR_INVALID, "gs_qk_rotary: invalid arguments");
+  const bool inter = shape->interleaved != 0;
+  const QkPlan p = qk_plan(a, shape->dtype, inter, false, false);
+  return qk_run<false>(a, shape->dtype, inter, p.v, static_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t gs_qk_rotary_grad_workspace(const gs_qk_shape* shape) {
+  return qk_workspace(shape, false);
+}
+
+extern "C" int gs_qk_rotary_grad(const gs_qk_shape* shape, const gs_qk_rows x[3],
+                                 const gs_qk_rows dy[3], const gs_qk_rows dx[3], void* grad_qw,
+                                 void* grad_kw, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  QkArgs a;
+  if (int rc = qk_args(a, "gs_qk_rotary_grad", shape, x, dy, dx)) return rc;
+  if (x == nullptr || dy == nullptr || (dx == nullptr && grad_qw == nullptr && grad_kw == nullptr) ||
+      qk_check_rows("gs_qk_rotary_grad", shape, x, shape->norm != 0) != GS_OK ||
+      (dx != nullptr && qk_check_rows("gs_qk_rotary_grad", shape, dx, true) != GS_OK))
+    return fail(GS_ERR_INVALID, "gs_qk_rotary_grad: invalid arguments");
+  void* gw[2] = {grad_qw, grad_kw};
+  for (int k = 0; k < 2; ++k)
+    if (gw[k] != nullptr && (shape->norm == 0 || shape->weight[k] == nullptr))
+      return fail(GS_ERR_INVALID, "gs_qk_rotary_grad: a weight's gradient without the weight");
+  if (dx == nullptr) a.heads[2] = 0;   // values have no part in the weights' gradients
+  if (a.heads[0] + a.heads[1] + a.heads[2] == 0)
+    return fail(GS_ERR_INVALID, "gs_qk_rotary_grad: invalid arguments");
+  const bool inter = shape->interleaved != 0, want_w = gw[0] != nullptr || gw[1] != nullptr;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const QkPlan p = qk_plan(a, shape->dtype, inter, true, false);
+  QkSums q{};
+  if (want_w) {
+    Sizer sz;
+    QkScratch unused(sz, a, p, false);
+    if (workspace == nullptr || workspace_bytes < sz.used)
+      return fail(GS_ERR_WORKSPACE, "gs_qk_rotary_grad: workspace too small");
+    Carver cv(workspace, workspace_bytes);
+    const QkScratch w(cv, a, p, false);
+    for (int k = 0; k < 2; ++k) {
+      if (gw[k] != nullptr && a.heads[k] > 0) q.part[k] = a.part[k] = w.part[k];
+      q.rows[k] = p.rows[k];
+      q.grad[k] = gw[k];
+      q.grad_bf16[k] = shape->weight_dtype[k] == GS_DTYPE_BF16;
+    }
+  }
+  if (int rc = qk_run<true>(a, shape->dtype, inter, p.v, s)) return rc;
+  if (!want_w) return GS_OK;
+  q.scale = 1.f;
+  q.D = a.D;
+  hipLaunchKernelGGL(qk_sums_kernel, dim3((a.D + QR_COLS - 1) / QR_COLS, 1, 2),
+                     dim3(QR_COLS * QR_GROUPS), 0, s, q);
+  return check_launch("qk_sums_kernel");
+}
+
+extern "C" size_t gs_qk_rotary_dots_workspace(const gs_qk_shape* shape) {
+  return qk_workspace(shape, true);
+}
+
+extern "C" int gs_qk_rotary_dots(const gs_qk_shape* shape, const gs_qk_rows x[3],
+                                 const gs_qk_rows dy[3], int64_t n_val, int64_t val_start,
+                                 float* out_dot_q, float* out_dot_k, void* out_grad_q,
+                                 void* out_grad_k, float grad_scale, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  QkArgs a;
+  if (int rc = qk_args(a, "gs_qk_rotary_dots", shape, x, dy, nullptr)) return rc;
+  void* gw[2] = {out_grad_q, out_grad_k};
+  float* dot[2] = {out_dot_q, out_dot_k};
+  if (x == nullptr || dy == nullptr || shape->norm == 0 || n_val <= 0 || n_val >= shape->B ||
+      val_start < 0 || val_start + n_val > shape->B ||
+      qk_check_rows("gs_qk_rotary_dots", shape, x, true) != GS_OK)
+    return fail(GS_ERR_INVALID, "gs_qk_rotary_dots: invalid arguments");
+  if (a.B > 65533)   // the sums' grid
+    return fail(GS_ERR_UNSUPPORTED, "gs_qk_rotary_dots: more than 65533 samples");
+  a.heads[2] = 0;
+  if (a.heads[0] + a.heads[1] == 0)
+    return fail(GS_ERR_INVALID, "gs_qk_rotary_dots: invalid arguments");
+  const bool inter = shape->interleaved != 0;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const QkPlan p = qk_plan(a, shape->dtype, inter, true, true);
+  Sizer sz;
+  QkScratch unused(sz, a, p, true);
+  if (workspace == nullptr || workspace_bytes < sz.used)
+    return fail(GS_ERR_WORKSPACE, "gs_qk_rotary_dots: workspace too small");
+  Carver cv(workspace, workspace_bytes);
+  const QkScratch w(cv, a, p, true);
+  QkSums q{};
+  QkDots o{};
+  for (int k = 0; k < 2; ++k) {
+    if (a.heads[k] > 0) q.part[k] = a.part[k] = w.part[k];
+    q.rows[k] = p.rows[k];
+    q.out[k] = w.sums[k];
+    q.val[k] = w.val[k];
+    q.grad[k] = gw[k];
+    q.grad_bf16[k] = shape->weight_dtype[k] == GS_DTYPE_BF16;
+    o.S[k] = w.sums[k];
+    o.val[k] = w.val[k];
+    o.dot[k] = dot[k];
+  }
+  q.samples = a.B, q.n_val = n_val, q.val_start = val_start;
+  q.scale = grad_scale;
+  q.D = a.D;
+  if (int rc = qk_run<true>(a, shape->dtype, inter, p.v, s)) return rc;
+  hipLaunchKernelGGL(qk_sums_kernel,
+                     dim3((a.D + QR_COLS - 1) / QR_COLS, static_cast<unsigned>(a.B + 2), 2),
+                     dim3(QR_COLS * QR_GROUPS), 0, s, q);
+  hipLaunchKernelGGL(qk_dots_kernel, dim3(static_cast<unsigned>(a.B - n_val), 2), dim3(64), 0, s,
+                     o, train_rows(a.B, n_val, val_start, a.T), a.D);
+  return check_launch("qk_sums_kernel / qk_dots_kernel");
+}

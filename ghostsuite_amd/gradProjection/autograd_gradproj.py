@@ -16,6 +16,7 @@ import torch.nn as nn
 
 from .. import _native, _overlap
 from .._native import ops
+from ..lm_layers import ScaledEmbedding
 
 
 def _flatten_tokens(x: torch.Tensor) -> torch.Tensor:
@@ -103,7 +104,12 @@ class GradProjHooks:
             self._cast[('embT', dt)] = (self.P_i.t().to(dt).contiguous(),
                                         self.P_o.to(dt).contiguous())
         P_iT, P_o = self._cast[('embT', dt)]
-        module._ghost_grad_proj = ops().kron_embed_proj(indices, g, P_iT, P_o, 1.0,
+        scale = 1.0
+        if isinstance(module, ScaledEmbedding):   # its rows' factor; its padding id (-1: none)
+            scale = module.scale
+            if module.padding_idx is not None:
+                indices = indices.masked_fill(indices == module.padding_idx, -1)
+        module._ghost_grad_proj = ops().kron_embed_proj(indices, g, P_iT, P_o, scale,
                                                         out_dtype=torch.float32)
 
     def attach(self, module: nn.Module) -> None:

@@ -26,6 +26,7 @@ from torch import nn
 
 from . import _native, _overlap
 from ._native import ops
+from .lm_layers import QKNormRotary, ScaledEmbedding
 
 try:  # HF Conv1D is a registry key only when transformers is importable
     import transformers.pytorch_utils as _hf_utils
@@ -388,6 +389,13 @@ def _scaled_mm(x: torch.Tensor, y: torch.Tensor, alpha: float) -> torch.Tensor:
 def _compute_embedding_dot_product(layer: nn.Embedding, A: torch.Tensor, B: torch.Tensor,
                                    val_batch_size: int):
     """Gradient dot-product of an nn.Embedding (reference :181-211)."""
+    _embedding_dots(layer, A, B, val_batch_size)
+
+
+def _embedding_dots(layer: nn.Embedding, A: torch.Tensor, B: torch.Tensor, val_batch_size: int,
+                    factor: float = 1.0, padding_idx: Optional[int] = None):
+    """The dots, and the train gradient when its scale was announced, of an embedding whose
+    forward multiplies its rows by `factor` and whose `padding_idx` has no gradient."""
     A = A.detach()
     B = B.detach()
     train_bs = A.size(0) - val_batch_size
@@ -397,30 +405,34 @@ def _compute_embedding_dot_product(layer: nn.Embedding, A: torch.Tensor, B: torc
         B = B.float()
     elif B.dtype not in (torch.bfloat16, torch.float32):
         B = B.float()
+    # The train gradient is built from the ids the layer saw: the reference's gradient stage reads
+    # layer.activations (autograd_grad_sample_dotprod.py:166-181), not the ids its dot stage
+    # promoted to the backprops' dtype (:116-123), which may have rounded.
+    ids = layer.__dict__.get("activations")
+    ids = A if ids is None or ids.is_floating_point() else ids.detach()
+    same = ids.data_ptr() == A.data_ptr() and ids.dtype == A.dtype and ids.stride() == A.stride()
+    if padding_idx is not None:   # -1 takes no part
+        pad = ids == padding_idx
+        A = A.masked_fill(pad, -1)
+        ids = A if same else ids.masked_fill(pad, -1)
     # With the train-grad scale announced, the train gradient is formed here as well (same
     # stream as the dot, no second hook-stage launch sequence) and parked for
     # _compute_embedding_train_grad.
     scale = layer.__dict__.get("_gs_bias_grad_scale")
+    dot = None
     if scale is not None and getattr(layer.weight, "initially_requires_grad", False):
-        # The train gradient is built from the ids the layer saw: the reference's gradient
-        # stage reads layer.activations (autograd_grad_sample_dotprod.py:166-181), not the ids
-        # its dot stage promoted to the backprops' dtype (:116-123), which may have rounded.
-        ids = layer.__dict__.get("activations")
-        ids = A if ids is None or ids.is_floating_point() else ids.detach()
         out, grad, accumulate = _embedding_grad_out(layer)
-        dot = None
-        if ids.data_ptr() == A.data_ptr() and ids.dtype == A.dtype and \
-                ids.stride() == A.stride():   # the same ids for both
-            dot = ops().embedding_layer_pass(A, B, val_batch_size, scale, out,
+        if same:   # the same ids for both
+            dot = ops().embedding_layer_pass(A, B, val_batch_size, scale * factor, out,
                                              accumulate=accumulate)
         if dot is None:
             dot = ops().embedding_dot(A, B, val_batch_size, vocab=layer.weight.shape[0])
-            ops().embedding_train_grad(ids, B, val_batch_size, scale, out, accumulate=accumulate)
-        layer.weight.grad_dot_prod = dot
+            ops().embedding_train_grad(ids, B, val_batch_size, scale * factor, out,
+                                       accumulate=accumulate)
         layer.__dict__["_gs_weight_train_grad"] = grad
-        return
-    layer.weight.grad_dot_prod = ops().embedding_dot(A, B, val_batch_size,
-                                                     vocab=layer.weight.shape[0])
+    else:
+        dot = ops().embedding_dot(A, B, val_batch_size, vocab=layer.weight.shape[0])
+    layer.weight.grad_dot_prod = dot if factor == 1.0 else dot.mul_(factor * factor)
 
 
 # Returned by a train-grad sampler that has already added its gradient into
@@ -466,6 +478,24 @@ def _embedding_grad_out(layer: nn.Embedding):
         return prev, APPLIED, True
     grad = torch.empty_like(layer.weight)
     return grad, grad, False
+
+
+# Scaled embedding ###########################################################################
+
+def _compute_scaled_embedding_dot_product(layer: ScaledEmbedding, A: torch.Tensor,
+                                          B: torch.Tensor, val_batch_size: int):
+    """Gradient dot-product of a ScaledEmbedding: an nn.Embedding's, every row gradient times the
+    layer's scale; rows of its padding id have none."""
+    _embedding_dots(layer, A, B, val_batch_size, layer.scale, layer.padding_idx)
+
+
+def _compute_scaled_embedding_train_grad(layer: ScaledEmbedding, A: torch.Tensor, B: torch.Tensor,
+                                         val_batch_size: int, scale: float = 1.0):
+    """scale * the layer's scale * (sum of the train rows per token id) / n_train, without the
+    padding id's; the rest as for an nn.Embedding."""
+    if layer.padding_idx is not None and "_gs_weight_train_grad" not in layer.__dict__:
+        A = A.masked_fill(A == layer.padding_idx, -1)
+    return _compute_embedding_train_grad(layer, A, B, val_batch_size, scale * layer.scale)
 
 
 # LayerNorm Layer ###########################################################################
@@ -521,6 +551,47 @@ def _compute_layernorm_train_grad(layer: nn.LayerNorm, A: torch.Tensor, B: torch
     _create_or_accumulate_train_grad(_param(layer, "weight"), gw)
     if _param(layer, "bias") is not None:
         _create_or_accumulate_train_grad(_param(layer, "bias"), gb)
+    return None
+
+
+# Norms of queries and keys with their rotation ##############################################
+
+def _compute_qk_norm_dot_product(layer: QKNormRotary, A: torch.Tensor, B: torch.Tensor,
+                                 val_batch_size: int):
+    """Dot-products of a QKNormRotary's two weights: sample i's gradient of q_weight is the sum
+    over its tokens and query heads of the back-rotated output gradient times the normed row, and
+    likewise for k_weight.  The same pass produces the train gradients when the hook announced
+    their scale.  B is one of the layer's output gradients; all of them are the hook's."""
+    if A.size(0) - val_batch_size <= 0:
+        raise ValueError("No training samples to compute dot product, check batch sizes.")
+    _qk_norm_pass(layer, A, B, val_batch_size, layer.__dict__.get("_gs_ln_grad_scale"), True)
+
+
+def _qk_norm_pass(layer: QKNormRotary, A, B, val_batch_size, grad_scale, dots: bool):
+    grads = layer.__dict__.get("_gs_grad_outputs") or (B, None, None)
+    plan = {"heads": (layer.n_head, layer.n_kv_head, layer.n_kv_head), "table": layer.table,
+            "positions": layer.__dict__.get("_gs_positions"), "norm": True, "eps": layer.eps,
+            "interleaved": layer.interleaved}
+    q, k = _param(layer, "q_weight"), _param(layer, "k_weight")
+    dot_q, dot_k, grad_q, grad_k = ops().qk_norm_rotary_dots(
+        plan, (A.detach(),), q.detach(), k.detach(), grads, val_batch_size, grad_scale=grad_scale)
+    if dots:
+        q.grad_dot_prod, k.grad_dot_prod = dot_q, dot_k
+    if grad_q is not None:
+        layer.__dict__["_gs_ln_train_grads"] = (grad_q, grad_k)
+
+
+def _compute_qk_norm_train_grad(layer: QKNormRotary, A: torch.Tensor, B: torch.Tensor,
+                                val_batch_size: int, scale: float = 1.0) -> None:
+    """Applies the train gradients of a QKNormRotary's weights itself and returns None."""
+    train_bs = A.size(0) - val_batch_size
+    if train_bs <= 0:
+        raise ValueError("No training samples to compute gradients, check batch sizes.")
+    if "_gs_ln_train_grads" not in layer.__dict__:
+        _qk_norm_pass(layer, A, B, val_batch_size, scale / train_bs, False)
+    grads = layer.__dict__.pop("_gs_ln_train_grads")
+    for param, grad in zip((_param(layer, "q_weight"), _param(layer, "k_weight")), grads):
+        _create_or_accumulate_train_grad(param, grad)
     return None
 
 
@@ -662,6 +733,8 @@ _supported_layers_dotprod = {
     nn.Embedding: (_compute_embedding_dot_product, _compute_embedding_train_grad),
     nn.LayerNorm: (_compute_layernorm_dot_product, _compute_layernorm_train_grad),
     nn.Conv2d: (_compute_conv2d_dot_product, _compute_conv2d_train_grad),
+    ScaledEmbedding: (_compute_scaled_embedding_dot_product, _compute_scaled_embedding_train_grad),
+    QKNormRotary: (_compute_qk_norm_dot_product, _compute_qk_norm_train_grad),
 }
 if _HFConv1D is not None:
     _supported_layers_dotprod[_HFConv1D] = (_compute_Conv1D_dot_product,

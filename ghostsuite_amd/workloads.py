@@ -10,10 +10,13 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from typing import Optional
 
 import torch
 import torch.nn.functional as F
 from torch import nn
+
+from .lm_layers import QKNormRotary, ScaledEmbedding, distillation_loss
 
 
 class MLP(nn.Module):
@@ -43,6 +46,10 @@ class LMConfig:
     rotary: bool = False
     tied: bool = True
     rotary_pct: float = 0.25
+    # Queries and keys normed per head, with the rotation in the same pass (QKNormRotary).
+    qk_norm: bool = False
+    # Token embeddings times this (ScaledEmbedding); None: a plain embedding.
+    embed_scale: Optional[float] = None
 
 
 GPT2_SMALL = LMConfig()
@@ -76,6 +83,10 @@ class Block(nn.Module):
         self.ln_1 = nn.LayerNorm(d)
         self.qkv = nn.Linear(d, 3 * d)
         self.proj = nn.Linear(d, d)
+        if cfg.qk_norm:
+            hd = d // cfg.n_head
+            self.qk = QKNormRotary(cfg.n_head, cfg.n_head, hd, n_positions=cfg.n_ctx,
+                                   n_rot=int(hd * cfg.rotary_pct) if cfg.rotary else 0)
         self.ln_2 = nn.LayerNorm(d)
         self.fc = nn.Linear(d, cfg.d_mlp)
         self.fc_out = nn.Linear(cfg.d_mlp, d)
@@ -83,14 +94,18 @@ class Block(nn.Module):
     def forward(self, x, rope=None):
         B, T, d = x.shape
         H = self.cfg.n_head
-        q, k, v = self.qkv(self.ln_1(x)).split(d, dim=-1)
-        q = q.view(B, T, H, d // H).transpose(1, 2)
-        k = k.view(B, T, H, d // H).transpose(1, 2)
-        v = v.view(B, T, H, d // H).transpose(1, 2)
-        if rope is not None:
-            cos, sin, n_rot = rope
-            q = _rotary(q, cos, sin, n_rot)
-            k = _rotary(k, cos, sin, n_rot)
+        qkv = self.qkv(self.ln_1(x))
+        if self.cfg.qk_norm:
+            q, k, v = self.qk(qkv)
+        else:
+            q, k, v = qkv.split(d, dim=-1)
+            q = q.view(B, T, H, d // H).transpose(1, 2)
+            k = k.view(B, T, H, d // H).transpose(1, 2)
+            v = v.view(B, T, H, d // H).transpose(1, 2)
+            if rope is not None:
+                cos, sin, n_rot = rope
+                q = _rotary(q, cos, sin, n_rot)
+                k = _rotary(k, cos, sin, n_rot)
         y = _attention(q.contiguous(), k.contiguous(), v.contiguous())
         x = x + self.proj(y.transpose(1, 2).reshape(B, T, d))
         return x + self.fc_out(F.gelu(self.fc(self.ln_2(x)), approximate="tanh"))
@@ -102,7 +117,8 @@ class CausalLM(nn.Module):
     def __init__(self, cfg: LMConfig):
         super().__init__()
         self.cfg = cfg
-        self.wte = nn.Embedding(cfg.vocab, cfg.d_model)
+        self.wte = nn.Embedding(cfg.vocab, cfg.d_model) if cfg.embed_scale is None else \
+            ScaledEmbedding(cfg.vocab, cfg.d_model, cfg.embed_scale)
         if not cfg.rotary:
             self.wpe = nn.Embedding(cfg.n_ctx, cfg.d_model)
         self.h = nn.ModuleList([Block(cfg) for _ in range(cfg.n_layer)])
@@ -129,19 +145,25 @@ class CausalLM(nn.Module):
         emb = torch.cat((fr, fr), dim=-1)
         return emb.cos().to(dtype), emb.sin().to(dtype), n_rot
 
-    def forward(self, input_ids, labels=None):
+    def forward(self, input_ids, labels=None, teacher=None, temperature=1.0, alpha=0.5):
+        """Logits; with labels the mean cross entropy; with `teacher`, a pair of the teacher's top
+        ids and logits [B, T, K], the distillation loss (labels: its hard-label part, weighted
+        1 - alpha; without labels the teacher alone)."""
         B, T = input_ids.shape
         x = self.wte(input_ids)
         rope = None
-        if self.cfg.rotary:
+        if self.cfg.rotary and not self.cfg.qk_norm:
             rope = self._rope(T, input_ids.device, x.dtype)
-        else:
+        elif not self.cfg.rotary:
             # per-sample position ids so the position embedding's hook sees [B, T]
             pos = torch.arange(T, device=input_ids.device).unsqueeze(0).repeat(B, 1)
             x = x + self.wpe(pos)
         for blk in self.h:
             x = blk(x, rope)
         logits = self.lm_head(self.ln_f(x))
+        if teacher is not None:
+            return distillation_loss(logits, *teacher, labels, temperature=temperature,
+                                     alpha=1.0 if labels is None else alpha)
         if labels is None:
             return logits
         return F.cross_entropy(logits.float().view(-1, logits.shape[-1]), labels.reshape(-1))

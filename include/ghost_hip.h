@@ -377,6 +377,110 @@ int gs_kron_embed_proj(const int64_t* ids, const void* G, int dtype, int64_t B, 
 int gs_ordered_sum(const void* const* srcs, const int* dtypes, int count, int64_t n, void* out,
                    int out_dtype, void* stream);
 
+/* ---- Embedding lookup with a scale -----------------------------------------------------
+ * The forward of an embedding layer (no counterpart among the reference's samplers):
+ *   out[i] = scale * W[ids[i]], formed in fp32, rounded once to dtype    out: [n, d]
+ * ids: n token ids of ids_bits (32 or 64) bits; those outside [0, vocab) give rows of zeros.
+ * W: [vocab, d] (dtype).  grad_ids: NULL, or [n] int64 = ids as gs_embedding_train_grad takes
+ * them for this layer's gradient (with scale there): padding_idx replaced by -1, which takes no
+ * part (padding_idx < 0: no such id).  No workspace. */
+int gs_embedding_lookup(const void* ids, int ids_bits, int64_t n, const void* W, int dtype,
+                        int64_t vocab, int64_t d, float scale, int64_t padding_idx, void* out,
+                        int64_t* grad_ids, void* stream);
+
+/* ---- Per-head norms of queries and keys with their rotation ------------------------------
+ * The attention prologue (no counterpart among the reference's samplers).  Three parts -- 0
+ * queries, 1 keys, 2 values -- of heads[p] heads each, D features a head; a part of no heads is
+ * left out.  Per head row x of a query or key, w its weight (NULL: ones):
+ *   u = w x (mean x^2 + eps)^(-1/2)  with norm, else u = x
+ *   y: the n_rot / 2 pairs of the first n_rot features turned by their position's angles,
+ *      (u_a c - u_b s, u_b c + u_a s); pairs (i, i + n_rot / 2), or with `interleaved`
+ *      (2 i, 2 i + 1); the features past n_rot are u's
+ * and a value row is copied.  Formed in fp32, rounded once to dtype.
+ * table: [n_positions][2][n_rot / 2] fp32, each position's cosines then its sines.  positions:
+ * NULL (token t of a sample is at position t), or integers of position_bits (32 or 64) bits at
+ * strides of position_stride_b and _t elements (0: shared); one outside the table gives NaN in
+ * the rotated features. */
+typedef struct {
+  int dtype;               /* of all rows */
+  int64_t B, T, D, n_rot;  /* samples, tokens of each, features of a head, rotated features */
+  int32_t heads[3];
+  int norm, interleaved;
+  float eps;
+  const void* weight[2];   /* [D] each, or NULL */
+  int weight_dtype[2];     /* of the weight and of its gradient */
+  const float* table;
+  int64_t n_positions;
+  const void* positions;
+  int position_bits;
+  int64_t position_stride_b, position_stride_t;
+} gs_qk_shape;
+/* The rows of one part: head h of token t of sample b at data + (b stride_b + t stride_t +
+ * h stride_h) elements, its D features contiguous. */
+typedef struct {
+  void* data;
+  int64_t stride_b, stride_t, stride_h;
+} gs_qk_rows;
+
+int gs_qk_rotary(const gs_qk_shape* shape, const gs_qk_rows x[3], const gs_qk_rows y[3],
+                 void* stream);
+
+/* Backward of gs_qk_rotary: dy the gradients of y (data NULL: zeros), x its inputs.
+ * dx: NULL, or the input gradients.  grad_qw, grad_kw: NULL, or [D] gradients of the weights
+ * (sums in fp32 in a fixed order, rounded once). */
+size_t gs_qk_rotary_grad_workspace(const gs_qk_shape* shape);
+int gs_qk_rotary_grad(const gs_qk_shape* shape, const gs_qk_rows x[3], const gs_qk_rows dy[3],
+                      const gs_qk_rows dx[3], void* grad_qw, void* grad_kw, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* The weights' gradient dot products and train gradients, as gs_layernorm_dot's for a LayerNorm:
+ * with s_i the gradient of a weight from sample i alone,
+ *   out_dot[i] = <s_i, the sum of s_j over the val samples>  (fp32, [n_train])
+ *   out_grad   = grad_scale * the sum of s_i over the train samples  ([D], the weight's dtype)
+ * any of the four may be NULL.  Values have no part. */
+size_t gs_qk_rotary_dots_workspace(const gs_qk_shape* shape);
+int gs_qk_rotary_dots(const gs_qk_shape* shape, const gs_qk_rows x[3], const gs_qk_rows dy[3],
+                      int64_t n_val, int64_t val_start, float* out_dot_q, float* out_dot_k,
+                      void* out_grad_q, void* out_grad_k, float grad_scale, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* ---- Loss against a teacher's top logits -------------------------------------------------
+ * Per row z of V student logits, K teacher entries (id, logit t) and a label y:
+ *   p = softmax of t / temperature over the entries whose id is in [0, V) (others take no part)
+ *   q = softmax of z / temperature, s = softmax of z
+ *   loss = alpha temperature^2 sum_k p_k (log p_k - log q[id_k]) + (1 - alpha) (-log s_y)
+ * A row without such an entry has no first term; a repeated id counts as often as it stands.
+ * labels NULL: alpha must be 1.  Rows whose label is ignore_index have loss 0 and gradient 0; another
+ * label outside [0, V) makes the row's loss and gradient NaN (alpha < 1).
+ * reduction: GS_REDUCE_NONE (out_loss: [N]), GS_REDUCE_SUM, or GS_REDUCE_MEAN over the rows not
+ * ignored (NaN when there are none, as 0 / 0).
+ * Rows: n = (o, i), i < inner, at Z + (o stride_outer + i stride_inner) elements, V contiguous.
+ * grad: NULL, or the gradient
+ *   upstream (1 / rows not ignored with MEAN) (alpha temperature (q - P) + (1 - alpha)(s - 1_y)),
+ * P the p_k at their ids, at the same strides and the same offset from a 16-byte boundary as Z.
+ * upstream: NULL (ones), or fp32, [N] with NONE and [1] otherwise.
+ * gs_distill_grad with `filled`: grad already holds the gradient for an upstream of one, and is
+ * left as it is where the upstream is one. */
+typedef enum { GS_REDUCE_NONE = 0, GS_REDUCE_SUM = 1, GS_REDUCE_MEAN = 2 } gs_reduction;
+typedef struct {
+  const void* Z;
+  int dtype;
+  int64_t N, V, inner, stride_outer, stride_inner;
+  const int64_t* teacher_ids;  /* [N, K] */
+  const void* teacher;         /* [N, K] */
+  int teacher_dtype;
+  int64_t K;
+  const int64_t* labels;       /* [N] or NULL */
+  int64_t ignore_index;
+  float temperature, alpha;
+  int reduction;
+} gs_distill;
+size_t gs_distill_workspace(const gs_distill* d);
+int gs_distill_loss(const gs_distill* d, float* out_loss, void* grad, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int gs_distill_grad(const gs_distill* d, const float* upstream, int filled, void* grad,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
