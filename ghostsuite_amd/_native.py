@@ -124,8 +124,8 @@ class _QKShape(ctypes.Structure):   # gs_qk_shape
                 ("position_stride_b", _I64), ("position_stride_t", _I64)]
 
 
-class _QKRows(ctypes.Structure):    # gs_qk_rows
-    _fields_ = [("data", _P), ("stride_b", _I64), ("stride_t", _I64), ("stride_h", _I64)]
+# gs_qk_rows[3]: (data, stride_b, stride_t, stride_h) of each part, eight bytes each.
+_QKRows3 = _I64 * 12
 
 
 class _Distill(ctypes.Structure):   # gs_distill
@@ -240,94 +240,114 @@ class _QKCall:
     """The arguments of a gs_qk_rotary* call from a plan (the keywords of
     lm_layers.qkv_norm_rotary) and its input rows: one packed tensor, or queries and keys."""
 
+    __slots__ = ("dev", "heads", "B", "T", "D", "dtype", "dt", "parts", "keep", "shape")
+
     def __init__(self, plan, parts, qw, kw):
         heads, table, positions = plan["heads"], plan["table"], plan["positions"]
         self.dev = _require_device(*parts, qw, kw, table, positions)
-        x = parts[0]
-        self.total = sum(heads)
-        if min(heads[:2]) <= 0:
+        self.parts = parts = [_features_contiguous(p) for p in parts]
+        self.heads = heads
+        x, total = parts[0], sum(heads)
+        if min(heads[0], heads[1]) <= 0:
             raise GhostHipError(f"{heads[0]} query and {heads[1]} key heads")
-        packed = len(parts) == 1
-        if packed and not (x.dim() == 3 and x.shape[2] % self.total == 0) and \
-                not (x.dim() == 4 and x.shape[2] == self.total):
-            raise GhostHipError(f"qkv {tuple(x.shape)} does not hold {self.total} heads")
-        self.B, self.T = x.shape[:2]
-        self.D = x.shape[2] // self.total if packed and x.dim() == 3 else x.shape[3]
-        D, n_rot = self.D, 2 * table.shape[-1]
+        size = x.shape
+        if len(parts) == 1 and not (len(size) == 3 and size[2] % total == 0) and \
+                not (len(size) == 4 and size[2] == total):
+            raise GhostHipError(f"qkv {tuple(size)} does not hold {total} heads")
+        self.B, self.T = B, T = size[0], size[1]
+        self.D = D = size[2] // total if len(size) == 3 else size[3]
         if D <= 0:
             raise GhostHipError("heads without features")
         self.dtype = x.dtype
+        self.dt = dt = _kernel_dtype(x, "queries and keys")
         for p in parts[1:]:
-            if p.shape[:2] != x.shape[:2] or p.shape[3] != D or p.dtype != x.dtype:
-                raise GhostHipError(f"queries {tuple(x.shape)} {x.dtype} and keys "
+            if p.shape[:2] != size[:2] or p.shape[3] != D or p.dtype != x.dtype:
+                raise GhostHipError(f"queries {tuple(size)} {x.dtype} and keys "
                                     f"{tuple(p.shape)} {p.dtype} disagree")
         if table.dim() != 3 or table.shape[1] != 2 or table.dtype != torch.float32 or \
-                not table.is_contiguous() or n_rot > D:
+                not table.is_contiguous() or 2 * table.shape[2] > D:
             raise GhostHipError(f"table {tuple(table.shape)} {table.dtype}: contiguous fp32 "
                                 f"[positions, 2, n_rot / 2] with n_rot up to {D} expected")
-        s = self.shape = _QKShape()
-        s.dtype = _kernel_dtype(x, "queries and keys")
-        s.B, s.T, s.D, s.n_rot = self.B, self.T, D, n_rot
-        s.heads[:] = heads
-        s.norm, s.interleaved, s.eps = plan["norm"], plan["interleaved"], plan["eps"]
+        n_rot = 2 * table.shape[2]
+        w_ptr, w_dt = [None, None], [dt, dt]
         self.keep = [table, positions]   # alive until the call is enqueued
         for i, w in enumerate((qw, kw)):
             if w is None:
-                s.weight_dtype[i] = s.dtype
                 continue
             if w.shape != (D,):
                 raise GhostHipError(f"norm weight {tuple(w.shape)}: [{D}] expected")
-            s.weight_dtype[i] = _kernel_dtype(w, "norm weights")
-            w = w.contiguous()
-            self.keep.append(w)
-            s.weight[i] = w.data_ptr()
-        if n_rot:
-            s.table, s.n_positions = table.data_ptr(), table.shape[0]
+            w_dt[i] = _kernel_dtype(w, "norm weights")
+            if not w.is_contiguous():
+                w = w.contiguous()
+                self.keep.append(w)
+            w_ptr[i] = w.data_ptr()
+        pos, bits, p_sb, p_st = None, 0, 0, 0
         if positions is not None and n_rot:
             if positions.dtype not in (torch.int32, torch.int64) or \
-                    tuple(positions.shape) not in ((self.T,), (1, self.T), (self.B, self.T)):
+                    tuple(positions.shape) not in ((T,), (1, T), (B, T)):
                 raise GhostHipError(f"positions {tuple(positions.shape)} {positions.dtype}: int32 "
-                                    f"or int64 [{self.T}] or [{self.B}, {self.T}] expected")
-            s.positions = positions.data_ptr()
-            s.position_bits = 32 if positions.dtype == torch.int32 else 64
-            s.position_stride_t = positions.stride(-1)
-            if positions.dim() == 2 and positions.shape[0] == self.B:
-                s.position_stride_b = positions.stride(0)
+                                    f"or int64 [{T}] or [{B}, {T}] expected")
+            pos, bits = positions.data_ptr(), 32 if positions.dtype == torch.int32 else 64
+            p_st = positions.stride(-1)
+            if positions.dim() == 2 and positions.shape[0] == B:
+                p_sb = positions.stride(0)
+        self.shape = _QKShape(dt, B, T, D, n_rot, heads, plan["norm"], plan["interleaved"],
+                              plan["eps"], tuple(w_ptr), tuple(w_dt),
+                              table.data_ptr() if n_rot else None, table.shape[0], pos, bits, p_sb,
+                              p_st)
 
-    def split(self, parts):
+    def rows(self, parts):
         """gs_qk_rows[3] of input-shaped tensors ([B, T, heads, D] each, or one packed)."""
-        rows, esz = (_QKRows * 3)(), 4 if self.dtype == torch.float32 else 2
-        first = 0
-        for i, h in enumerate(self.shape.heads):
-            if h == 0:
-                continue
-            x = parts[0] if len(parts) == 1 else parts[i]
-            sh = x.stride(2) if x.dim() == 4 else self.D
-            at = first * sh if len(parts) == 1 else 0
-            rows[i] = _QKRows(x.data_ptr() + at * esz, x.stride(0), x.stride(1), sh)
-            first += h
-        return rows
+        out, D, (hq, hk, hv) = [], self.D, self.heads
+        if len(parts) == 1:
+            x, = parts
+            st = x.stride()
+            sh = st[2] if len(st) == 4 else D
+            p, step = x.data_ptr(), sh * x.element_size()
+            return _QKRows3(p, st[0], st[1], sh, p + hq * step, st[0], st[1], sh,
+                            p + (hq + hk) * step if hv else 0, st[0], st[1], sh)
+        for x in parts:
+            out += [x.data_ptr(), *x.stride()[:3]]
+        return _QKRows3(*out)
 
-    def heads_first(self, tensors):
+    @staticmethod
+    def heads_first(tensors):
         """gs_qk_rows[3] of [B, heads, T, D] tensors (None: data NULL)."""
-        rows = (_QKRows * 3)()
-        for i, t in enumerate(tensors):
-            if t is not None:
-                rows[i] = _QKRows(t.data_ptr(), t.stride(0), t.stride(2), t.stride(1))
-        return rows
+        out = []
+        for t in tensors:
+            if t is None:
+                out += (0, 0, 0, 0)
+            else:
+                st = t.stride()
+                out += (t.data_ptr(), st[0], st[2], st[1])
+        return _QKRows3(*out)
 
     def gradients(self, grads):
         """The output gradients as the kernels take them (features contiguous)."""
         out = []
-        for i, h in enumerate(self.shape.heads):
-            g = grads[i] if h else None
+        for h, g in zip(self.heads, grads):
             if g is not None:
                 if g.shape != (self.B, h, self.T, self.D) or g.dtype != self.dtype:
                     raise GhostHipError(f"output gradient {tuple(g.shape)} {g.dtype}")
-                _require_device(g)
+                if g.device != self.dev:
+                    raise GhostHipError(f"tensors on different devices: {self.dev} and {g.device}")
                 g = _features_contiguous(g)
             out.append(g)
         return out
+
+    def workspace(self, query: str) -> int:
+        """The bytes a query answers: they follow from the sizes alone."""
+        s = self.shape
+        return _qk_size(query, self.dt, self.B, self.T, self.D, s.n_rot, self.heads,
+                        s.interleaved)
+
+
+@functools.lru_cache(maxsize=4096)
+def _qk_size(query, dt, B, T, D, n_rot, heads, interleaved) -> int:
+    # (any table: nothing of it is read)
+    shape = _QKShape(dt, B, T, D, n_rot, heads, 1, interleaved, 0.0, (None, None), (dt, dt), 256,
+                     1, None, 0, 0, 0)
+    return getattr(load_library(), query)(ctypes.byref(shape))
 
 
 class HipOps:
@@ -930,21 +950,26 @@ class HipOps:
         if not ids.numel():
             return torch.zeros(shape, dtype=dtype, device=dev)
         out = torch.empty(shape, dtype=dtype, device=dev)
+        G, n, (vocab, d) = G.contiguous(), ids.numel(), shape
+        ws_bytes = _size("gs_embedding_train_grad_workspace", 1, 0, n, d, vocab)
+        ws = _workspace(ws_bytes, dev)
         with _on(dev):
-            self.embedding_train_grad(ids.reshape(1, -1), G.reshape(1, -1, shape[1]), 0, scale,
-                                      out)
+            rc = load_library().gs_embedding_train_grad(
+                ids.data_ptr(), G.data_ptr(), _kernel_dtype(G, "output gradient"), 1, 0, 1, n, d,
+                vocab, scale, out.data_ptr(), _TORCH_TO_GS[dtype], 0, ws.data_ptr(), ws_bytes,
+                _stream(dev))
+        _check(rc, "gs_embedding_train_grad")
         return out
 
     def qk_norm_rotary(self, plan, parts, qw, kw):
         """Rotated queries and keys (and values), heads first: gs_qk_rotary.  plan: heads, table,
         positions, norm, eps, interleaved; parts: (qkv,) or (q, k)."""
-        parts = [_features_contiguous(p) for p in parts]
         c = _QKCall(plan, parts, qw, kw)
         out = [torch.empty((c.B, h, c.T, c.D), dtype=c.dtype, device=c.dev)
-               for h in plan["heads"] if h]
+               for h in c.heads if h]
         if c.B and c.T:
             with _on(c.dev):
-                rc = load_library().gs_qk_rotary(ctypes.byref(c.shape), c.split(parts),
+                rc = load_library().gs_qk_rotary(ctypes.byref(c.shape), c.rows(c.parts),
                                                  c.heads_first(out), _stream(c.dev))
             _check(rc, "gs_qk_rotary")
         return out
@@ -953,7 +978,6 @@ class HipOps:
                             want_kw: bool):
         """([input gradients] as parts or Nones, q weight gradient, k weight gradient):
         gs_qk_rotary_grad; grads: the outputs' gradients, None for zeros."""
-        parts = [_features_contiguous(p) for p in parts]
         c = _QKCall(plan, parts, qw, kw)
         grads = c.gradients(grads)
         dparts = [torch.empty(p.shape, dtype=c.dtype, device=c.dev) if want_x else None
@@ -962,16 +986,15 @@ class HipOps:
         dqw = make(c.D, dtype=qw.dtype, device=c.dev) if want_qw else None
         dkw = make(c.D, dtype=kw.dtype, device=c.dev) if want_kw else None
         if c.B and c.T and (want_x or want_qw or want_kw):
-            with _on(c.dev):
-                lib = load_library()
-                nbytes = 0
-                if want_qw or want_kw:
-                    nbytes = lib.gs_qk_rotary_grad_workspace(ctypes.byref(c.shape))
+            nbytes, ws = 0, None
+            if want_qw or want_kw:
+                nbytes = c.workspace("gs_qk_rotary_grad_workspace")
                 ws = _workspace(nbytes, c.dev)
-                rc = lib.gs_qk_rotary_grad(
-                    ctypes.byref(c.shape), c.split(parts), c.heads_first(grads),
-                    c.split(dparts) if want_x else None, _ptr(dqw), _ptr(dkw), ws.data_ptr(),
-                    nbytes, _stream(c.dev))
+            with _on(c.dev):
+                rc = load_library().gs_qk_rotary_grad(
+                    ctypes.byref(c.shape), c.rows(c.parts), c.heads_first(grads),
+                    c.rows(dparts) if want_x else None, _ptr(dqw), _ptr(dkw), _ptr(ws), nbytes,
+                    _stream(c.dev))
             _check(rc, "gs_qk_rotary_grad")
         return dparts, dqw, dkw
 
@@ -979,7 +1002,6 @@ class HipOps:
                             grad_scale: Optional[float] = None):
         """(dot_q, dot_k, grad_q, grad_k) of the norm weights: gs_qk_rotary_dots; the train
         gradients None without grad_scale."""
-        parts = [_features_contiguous(p) for p in parts]
         c = _QKCall(plan, parts, qw, kw)
         if not (c.B and c.T):
             raise GhostHipError("qk_norm_rotary_dots: no tokens")
@@ -991,22 +1013,68 @@ class HipOps:
         if grad_scale is not None:
             gw = [torch.empty(c.D, dtype=c.dtype if w is None else w.dtype, device=c.dev)
                   for w in (qw, kw)]
+        nbytes = c.workspace("gs_qk_rotary_dots_workspace")
+        ws = _workspace(nbytes, c.dev)
         with _on(c.dev):
-            lib = load_library()
-            nbytes = lib.gs_qk_rotary_dots_workspace(ctypes.byref(c.shape))
-            ws = _workspace(nbytes, c.dev)
-            rc = lib.gs_qk_rotary_dots(
-                ctypes.byref(c.shape), c.split(parts), c.heads_first(grads), n_val, vs,
+            rc = load_library().gs_qk_rotary_dots(
+                ctypes.byref(c.shape), c.rows(c.parts), c.heads_first(grads), n_val, vs,
                 dots[0].data_ptr(), dots[1].data_ptr(), _ptr(gw[0]), _ptr(gw[1]),
                 float(grad_scale or 0.0), ws.data_ptr(), nbytes, _stream(c.dev))
         _check(rc, "gs_qk_rotary_dots")
         return dots[0], dots[1], gw[0], gw[1]
 
-    def _distill_args(self, logits, teacher_ids, teacher, labels, temperature, alpha,
-                      ignore_index, reduction):
-        """(struct, device, what it points to) of a gs_distill call, and logits as it reads them:
-        rows of V contiguous logits at one stride, or two for [B, T, V]."""
-        dev = _require_device(logits, teacher_ids, teacher, labels)
+    def distill_loss(self, logits, teacher_ids, teacher_logits, labels, *, temperature: float,
+                     alpha: float, ignore_index: int, reduction: str, want_grad: bool = False):
+        """(loss, None), or with want_grad (loss, a _DistillCall that holds the gradient for an
+        upstream of one): gs_distill_loss."""
+        c = _DistillCall(logits, teacher_ids, teacher_logits, labels, temperature, alpha,
+                         ignore_index, reduction)
+        shape = logits.shape[:-1] if reduction == "none" else ()
+        if c.d.N == 0:
+            c.grad = torch.empty_like(logits)
+            return (torch.full(shape, math.nan if reduction == "mean" else 0.0, device=c.dev),
+                    c if want_grad else None)
+        loss = torch.empty(shape, dtype=torch.float32, device=c.dev)
+        c.allocate(want_grad)
+        with _on(c.dev):
+            rc = load_library().gs_distill_loss(ctypes.byref(c.d), loss.data_ptr(), _ptr(c.grad),
+                                                c.ws.data_ptr(), c.ws.numel(), _stream(c.dev))
+        _check(rc, "gs_distill_loss")
+        return loss, c if want_grad else None
+
+    def distill_grad(self, logits, teacher_ids, teacher_logits, labels, *, temperature: float,
+                     alpha: float, ignore_index: int, reduction: str, upstream: torch.Tensor,
+                     unit: Optional["_DistillCall"] = None) -> torch.Tensor:
+        """The logits' gradient for a loss gradient `upstream`: gs_distill_grad.  unit: what
+        distill_loss gave for these tensors, used up by this call."""
+        c = unit
+        if c is None or not c.reads(logits, teacher_ids, teacher_logits, labels):
+            c = _DistillCall(logits, teacher_ids, teacher_logits, labels, temperature, alpha,
+                             ignore_index, reduction)
+        if c.d.N == 0:
+            return torch.empty_like(logits)
+        filled = c.grad is not None
+        if not filled:
+            c.allocate(True)
+        if upstream.dtype != torch.float32 or not upstream.is_contiguous():
+            upstream = upstream.to(torch.float32).contiguous()
+        with _on(c.dev):
+            rc = load_library().gs_distill_grad(ctypes.byref(c.d), upstream.data_ptr(),
+                                                int(filled), c.grad.data_ptr(), c.ws.data_ptr(),
+                                                c.ws.numel(), _stream(c.dev))
+        _check(rc, "gs_distill_grad")
+        return c.grad if c.grad.shape == logits.shape else c.grad.view(logits.shape)
+
+
+class _DistillCall:
+    """The arguments of a gs_distill_* call, the tensors they point to, its scratch memory and
+    the gradient it fills."""
+
+    __slots__ = ("dev", "d", "given", "held", "ws", "grad")
+
+    def __init__(self, logits, teacher_ids, teacher, labels, temperature, alpha, ignore_index,
+                 reduction):
+        self.dev = _require_device(logits, teacher_ids, teacher, labels)
         lead = logits.shape[:-1]
         if logits.dim() < 1 or logits.shape[-1] == 0 or teacher.shape != teacher_ids.shape or \
                 teacher.dim() != logits.dim() or teacher.shape[:-1] != lead or \
@@ -1018,69 +1086,37 @@ class HipOps:
                 "[...] expected")
         if labels is not None and labels.is_floating_point() or teacher_ids.is_floating_point():
             raise GhostHipError("teacher ids and labels have to be integers")
-        d = _Distill()
-        d.dtype = _kernel_dtype(logits, "logits")
+        self.given = tuple(None if t is None else (t.data_ptr(), t.stride())
+                           for t in (logits, teacher_ids, teacher, labels))
+        dtype = _kernel_dtype(logits, "logits")
         if teacher.dtype not in (torch.bfloat16, torch.float32):
             teacher = teacher.float()
         teacher, teacher_ids = teacher.contiguous(), teacher_ids.to(torch.int64).contiguous()
         labels = None if labels is None else labels.to(torch.int64).contiguous()
-        d.N, d.V, d.K = math.prod(lead), logits.shape[-1], teacher.shape[-1]
-        logits = _rows_of_logits(logits)
-        d.inner, d.stride_outer, d.stride_inner = d.N, 0, d.V
-        if logits.dim() == 3:
-            d.inner = logits.shape[1]
-            d.stride_outer, d.stride_inner = logits.stride(0), logits.stride(1)
-        elif logits.dim() == 2:
-            d.stride_inner = logits.stride(0)
-        d.Z, d.teacher_ids, d.teacher = logits.data_ptr(), teacher_ids.data_ptr(), teacher.data_ptr()
-        d.labels = _ptr(labels)
-        d.teacher_dtype = _TORCH_TO_GS[teacher.dtype]
-        d.ignore_index, d.temperature, d.alpha = ignore_index, temperature, alpha
-        d.reduction = REDUCTIONS[reduction]
-        return d, dev, (logits, teacher_ids, teacher, labels)
+        z = _rows_of_logits(logits)
+        N, V = math.prod(lead), z.shape[-1]
+        inner, outer, row = N, 0, z.stride(-2)
+        if z.dim() == 3:
+            inner, outer = z.shape[1], z.stride(0)
+        elif N == 1:
+            row = V
+        self.held = (z, teacher_ids, teacher, labels)
+        self.d = _Distill(z.data_ptr(), dtype, N, V, inner, outer, row, teacher_ids.data_ptr(),
+                          teacher.data_ptr(), _TORCH_TO_GS[teacher.dtype], teacher.shape[-1],
+                          _ptr(labels), ignore_index, temperature, alpha, REDUCTIONS[reduction])
+        self.ws = self.grad = None
 
-    def distill_loss(self, logits, teacher_ids, teacher_logits, labels, *, temperature: float,
-                     alpha: float, ignore_index: int, reduction: str, want_grad: bool = False):
-        """(loss, gradient for an upstream of one or None): gs_distill_loss."""
-        d, dev, held = self._distill_args(logits, teacher_ids, teacher_logits, labels, temperature,
-                                          alpha, ignore_index, reduction)
-        shape = logits.shape[:-1] if reduction == "none" else ()
-        if d.N == 0:
-            empty = math.nan if reduction == "mean" else 0.0
-            return (torch.full(shape, empty, device=dev),
-                    torch.empty_like(logits) if want_grad else None)
-        loss = torch.empty(shape, dtype=torch.float32, device=dev)
-        grad = _empty_as(held[0]) if want_grad else None
-        with _on(dev):
-            lib = load_library()
-            nbytes = lib.gs_distill_workspace(ctypes.byref(d))
-            ws = _workspace(nbytes, dev)
-            rc = lib.gs_distill_loss(ctypes.byref(d), loss.data_ptr(), _ptr(grad), ws.data_ptr(),
-                                     nbytes, _stream(dev))
-        _check(rc, "gs_distill_loss")
-        return loss, None if grad is None else grad.view(logits.shape)
+    def reads(self, *tensors) -> bool:
+        """Whether these are the tensors it was made from (autograd may have moved what it saved)."""
+        return self.given == tuple(None if t is None else (t.data_ptr(), t.stride())
+                                   for t in tensors)
 
-    def distill_grad(self, logits, teacher_ids, teacher_logits, labels, *, temperature: float,
-                     alpha: float, ignore_index: int, reduction: str, upstream: torch.Tensor,
-                     unit_grad: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """The logits' gradient for a loss gradient `upstream`: gs_distill_grad.  unit_grad: the
-        gradient distill_loss gave, used up by this call."""
-        d, dev, held = self._distill_args(logits, teacher_ids, teacher_logits, labels, temperature,
-                                          alpha, ignore_index, reduction)
-        if d.N == 0:
-            return torch.empty_like(logits)
-        upstream = upstream.to(torch.float32).contiguous()
-        _require_device(logits, upstream)
-        grad = _empty_as(held[0]) if unit_grad is None else unit_grad
-        with _on(dev):
-            lib = load_library()
-            nbytes = lib.gs_distill_workspace(ctypes.byref(d))
-            ws = _workspace(nbytes, dev)
-            rc = lib.gs_distill_grad(ctypes.byref(d), upstream.data_ptr(),
-                                     int(unit_grad is not None), grad.data_ptr(), ws.data_ptr(),
-                                     nbytes, _stream(dev))
-        _check(rc, "gs_distill_grad")
-        return grad.view(logits.shape)
+    def allocate(self, want_grad: bool) -> None:
+        if self.ws is None:
+            nbytes = load_library().gs_distill_workspace(ctypes.byref(self.d))
+            self.ws = _workspace(nbytes, self.dev)
+        if want_grad:
+            self.grad = _empty_as(self.held[0])
 
 
 def _rows_of_logits(z: torch.Tensor) -> torch.Tensor:
@@ -1099,8 +1135,9 @@ def _rows_of_logits(z: torch.Tensor) -> torch.Tensor:
 def _empty_as(z: torch.Tensor) -> torch.Tensor:
     """An uninitialised tensor of z's shape and strides at z's offset from a 16-byte boundary (the
     kernels read and write the same 16-byte pieces of both)."""
-    esz = z.element_size()
-    off = z.data_ptr() % 16 // esz
+    off = z.data_ptr() % 16 // z.element_size()
+    if off == 0 and z.is_contiguous():
+        return torch.empty(z.shape, dtype=z.dtype, device=z.device)
     span = 1 + sum((n - 1) * s for n, s in zip(z.shape, z.stride()))
     base = torch.empty(off + span, dtype=z.dtype, device=z.device)
     return base.as_strided(z.shape, z.stride(), off)

@@ -490,11 +490,14 @@ extern "C" int gs_distill_grad(const gs_distill* d, const float* upstream, int f
   Carver cv(workspace, workspace_bytes);
   const DsScratch w(cv, d);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (int rc = ds_count(a, w.count, s)) return rc;
+  a.filled = filled && !a.per_row;
+  if (a.filled)   // the loss's call left the count
+    a.count = a.mean && a.labels != nullptr ? w.count : nullptr;
+  else if (int rc = ds_count(a, w.count, s))
+    return rc;
   const bool two = ds_two(a);
   a.grad = grad;
   a.upstream = upstream;
-  a.filled = filled && !a.per_row;
   // A filled gradient is mostly left as it is: few workgroups then look at the upstream and end.
   const int64_t grid = a.filled ? std::min<int64_t>(a.N, 512) : a.N;
   return d->dtype == GS_DTYPE_BF16 ? ds_run<uint16_t>(a, two, grid, s)

@@ -33,6 +33,16 @@ def _records(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _once(backward):
+    """once_differentiable, whose wrapping costs a backward pass 8 us on the host, only where the
+    backward pass itself is recorded."""
+    recorded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return staticmethod(run)
+
+
 # Embedding lookup ###########################################################################
 
 class _Lookup(torch.autograd.Function):
@@ -43,8 +53,7 @@ class _Lookup(torch.autograd.Function):
         ctx.scale, ctx.shape, ctx.dtype = scale, weight.shape, weight.dtype
         return out
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         ids, = ctx.saved_tensors
         return None, ops().embedding_grad(ids, g, ctx.shape, ctx.dtype, ctx.scale), None, None
@@ -101,25 +110,24 @@ def rotary_table(n_positions: int, n_rot: int, base: float = 10000.0, device=Non
 
 
 class _QKNormRotary(torch.autograd.Function):
-    """x: one packed tensor (split in the kernels by `heads`), or None with q, k in `more`."""
+    """parts: one packed tensor, or queries and keys."""
 
     @staticmethod
     def forward(ctx, plan, qw, kw, *parts):
         ctx.set_materialize_grads(False)
-        out = ops().qk_norm_rotary(plan, parts, qw, kw)
-        ctx.plan, ctx.n_parts = plan, len(parts)
+        ctx.plan = plan
         ctx.save_for_backward(qw, kw, plan["table"], plan["positions"], *parts)
-        return tuple(out)
+        return tuple(ops().qk_norm_rotary(plan, parts, qw, kw))
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, *grads):
         qw, kw, table, positions, *parts = ctx.saved_tensors
         need = ctx.needs_input_grad
-        want_x = any(need[3:])
+        plan = ctx.plan
+        if table is not plan["table"] or positions is not plan["positions"]:
+            plan = dict(plan, table=table, positions=positions)   # as unpacked for this pass
         dparts, dqw, dkw = ops().qk_norm_rotary_grad(
-            dict(ctx.plan, table=table, positions=positions), parts, qw, kw, grads, want_x=want_x,
-            want_qw=need[1], want_kw=need[2])
+            plan, parts, qw, kw, grads, want_x=any(need[3:]), want_qw=need[1], want_kw=need[2])
         return (None, dqw, dkw, *dparts)
 
 
@@ -216,20 +224,18 @@ class _Distillation(torch.autograd.Function):
     def forward(ctx, logits, teacher_ids, teacher_logits, labels, how):
         # A mean's or sum's gradient is written in the loss's own pass, for an upstream gradient of
         # one; the backward pass keeps it or, for another upstream, forms it again.
-        fused = how["reduction"] != "none"
-        loss, grad = ops().distill_loss(logits, teacher_ids, teacher_logits, labels, **how,
-                                        want_grad=fused)
+        loss, ctx.unit = ops().distill_loss(logits, teacher_ids, teacher_logits, labels, **how,
+                                            want_grad=how["reduction"] != "none")
         ctx.save_for_backward(logits, teacher_ids, teacher_logits, labels)
-        ctx.how, ctx.unit_grad = how, grad
+        ctx.how = how
         return loss
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         logits, teacher_ids, teacher_logits, labels = ctx.saved_tensors
-        unit, ctx.unit_grad = ctx.unit_grad, None   # handed out once: the caller may change it
+        unit, ctx.unit = ctx.unit, None   # handed out once: the caller may change it
         grad = ops().distill_grad(logits, teacher_ids, teacher_logits, labels, **ctx.how,
-                                  upstream=g, unit_grad=unit)
+                                  upstream=g, unit=unit)
         return grad, None, None, None, None
 
 

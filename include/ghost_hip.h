@@ -459,8 +459,9 @@ int gs_qk_rotary_dots(const gs_qk_shape* shape, const gs_qk_rows x[3], const gs_
  *   upstream (1 / rows not ignored with MEAN) (alpha temperature (q - P) + (1 - alpha)(s - 1_y)),
  * P the p_k at their ids, at the same strides and the same offset from a 16-byte boundary as Z.
  * upstream: NULL (ones), or fp32, [N] with NONE and [1] otherwise.
- * gs_distill_grad with `filled`: grad already holds the gradient for an upstream of one, and is
- * left as it is where the upstream is one. */
+ * gs_distill_grad with `filled`: grad and the workspace are those of a gs_distill_loss call with the
+ * same arguments and inputs, as it left them; the gradient stays as it is where the upstream is one
+ * (not with NONE). */
 typedef enum { GS_REDUCE_NONE = 0, GS_REDUCE_SUM = 1, GS_REDUCE_MEAN = 2 } gs_reduction;
 typedef struct {
   const void* Z;

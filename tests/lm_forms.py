@@ -212,7 +212,7 @@ class LmOracleOps(OracleOps):
 
     @torch.enable_grad()
     def distill_grad(self, logits, ids, t, labels, *, temperature, alpha, ignore_index, reduction,
-                     upstream, unit_grad=None):
+                     upstream, unit=None):
         z = f64(logits).requires_grad_()
         rows, kept = self._rows(z, ids, t, labels, temperature, alpha, ignore_index)
         loss = reduced(rows, kept, reduction)

@@ -75,10 +75,7 @@ def _qk_shape(**changes):
 
 
 def _qk_rows(n=3):
-    rows = (_native._QKRows * 3)()
-    for i in range(n):
-        rows[i] = _native._QKRows(P16, 1024, 256, 64)
-    return rows
+    return _native._QKRows3(*(n * [P16, 1024, 256, 64] + (3 - n) * [0, 0, 0, 0]))
 
 
 @pytest.mark.parametrize("changes,status", [
