@@ -63,52 +63,39 @@ __device__ __forceinline__ uint4 ds_map(const uint4& v, F f) {
                       pack_bf16x2(f(ds_elem<E>(v, 4)), f(ds_elem<E>(v, 5))),
                       pack_bf16x2(f(ds_elem<E>(v, 6)), f(ds_elem<E>(v, 7))));
 }
-// Keeps the compiler from carrying the unpacked elements of one sweep to the next: twice the
-// registers for bf16, and spills.
-__device__ __forceinline__ void ds_packed(uint4& v) {
-  asm("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));
+// Ends one sweep over a piece: its sums are formed (`a`, `b` are taken in) before the piece counts as
+// a new value, so the compiler neither carries unpacked elements to the next sweep (twice the
+// registers for bf16) nor keeps two copies of the piece for sums that it puts off.
+__device__ __forceinline__ void ds_swept(uint4& v, float& a, float& b) {
+  asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w), "+v"(a), "+v"(b));
 }
 
-// Maximum / sums over the workgroup, for three values at once (max for the first two of `max3`,
-// sum for all of `sum3`).
-template <int WAVES>
-__device__ __forceinline__ void block_max2(float& a, float& b, float (*red)[4]) {
-#pragma unroll
-  for (int k = 32; k > 0; k >>= 1) {
-    a = fmaxf(a, __shfl_xor(a, k, 64));
-    b = fmaxf(b, __shfl_xor(b, k, 64));
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) {
-    red[threadIdx.x >> 6][0] = a;
-    red[threadIdx.x >> 6][1] = b;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    a = fmaxf(a, red[w][0]);
-    b = fmaxf(b, red[w][1]);
-  }
+// A value the compiler takes for a new one: what it made of the old one is formed again, not kept.
+__device__ __forceinline__ uint32_t ds_fresh(uint32_t v) {
+  asm("" : "+v"(v));
+  return v;
 }
-template <int WAVES>
-__device__ __forceinline__ void block_sum3(float& a, float& b, float& c, float (*red)[4]) {
-  a = wave_sum(a);
-  b = wave_sum(b);
-  c = wave_sum(c);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) {
-    red[threadIdx.x >> 6][0] = a;
-    red[threadIdx.x >> 6][1] = b;
-    red[threadIdx.x >> 6][2] = c;
-  }
-  __syncthreads();
-  a = b = c = 0.f;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    a += red[w][0];
-    b += red[w][1];
-    c += red[w][2];
-  }
+
+// Piece p of a row: a scalar base and 32 bits of offset (rows are below 2^32 bytes where pieces are
+// kept), so that no 64-bit address takes registers for each of them.
+__device__ __forceinline__ uint4 ds_piece(const uint4* row, uint32_t p) {
+  return *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(row) + p * 16u);
+}
+
+// The wave's maximum (wave-uniform), by DPP as wave_sum_dpp; lanes without a source keep their own.
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+  const int i = __builtin_bit_cast(int, v);
+  return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false)));
+}
+__device__ __forceinline__ float wave_max_dpp(float v) {
+  v = dpp_max<0x111>(v);   // row_shr:1, 2, 4, 8: lane 15 of each row holds the row's
+  v = dpp_max<0x112>(v);
+  v = dpp_max<0x114>(v);
+  v = dpp_max<0x118>(v);
+  v = dpp_max<0x142>(v);   // row_bcast:15, :31: lane 63 holds the wave's
+  v = dpp_max<0x143>(v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 // exp(x / tau) for x <= 0, `k` = log2(e) / tau.
@@ -116,89 +103,115 @@ __device__ __forceinline__ float ds_exp(float x, float k) { return __builtin_amd
 
 constexpr float DS_LOG2E = 1.44269504088896340736f;
 
+// One teacher entry (the label is entry K): its id (-1: none), the thread that writes the id's
+// element, the entry's logit, then its mass in the gradient, the student's logit there, and the
+// masses of all entries of its id.
+struct DsEntries {
+  int *id, *owner;
+  float *t, *z, *mass;
+  __device__ DsEntries(void* lds, int n) {
+    id = static_cast<int*>(lds);
+    owner = id + n;
+    t = reinterpret_cast<float*>(owner + n);
+    z = t + n;
+    mass = z + n;
+  }
+};
+__host__ __device__ inline int ds_entries(int K) { return (K + 1 + 3) & ~3; }   // whole int4s
+
 // NP: pieces a thread keeps (0: none are kept, the row is read twice).  TWO: the two softmaxes
-// differ and both count.
-template <class E, int THREADS, int NP, bool TWO>
-__global__ void __launch_bounds__(THREADS) distill_kernel(DsArgs a) {
+// differ and both count.  WPE: waves on a SIMD the registers are held to.
+template <class E, int THREADS, int NP, bool TWO, int WPE>
+__global__ void __launch_bounds__(THREADS, WPE) distill_kernel(DsArgs a) {
   constexpr int VE = 16 / sizeof(E);
   constexpr int WAVES = THREADS / 64;
-  __shared__ float red[WAVES][4];
-  extern __shared__ char dyn[];
-  // Per entry (the label last): its id (-1: none), and its mass in the gradient.
-  int* const e_id = reinterpret_cast<int*>(dyn);
-  float* const e_mass = reinterpret_cast<float*>(dyn) + a.K + 1;
+  __shared__ float red[3][WAVES][4];
+  extern __shared__ int4 dyn[];
+  const DsEntries ent(dyn, ds_entries(a.K));
   const float NEG_INF = -__builtin_inff();
-  const int tid = threadIdx.x;
+  const uint32_t wid = threadIdx.x >> 6, K = a.K, V = a.V;
+  const bool lead = (threadIdx.x & 63) == 0;
   const float kq = DS_LOG2E * a.inv_tau;
 
   if (a.filled && !a.per_row && a.upstream[0] == 1.f) return;   // nothing to change
 
-  for (int64_t n = blockIdx.x; n < a.N; n += gridDim.x) {
-    const int64_t at = a.inner == a.N ? n * a.s_inner
-                                      : n / a.inner * a.s_outer + n % a.inner * a.s_inner;
+  for (uint32_t n = blockIdx.x; n < static_cast<uint32_t>(a.N); n += gridDim.x) {
+    const uint32_t tid = ds_fresh(threadIdx.x);
+    if (n != blockIdx.x) __syncthreads();   // the last row's LDS has been read
+    const uint32_t outer = a.inner == a.N ? 0 : n / static_cast<uint32_t>(a.inner);
+    const int64_t at = outer * a.s_outer + (n - outer * static_cast<uint32_t>(a.inner)) * a.s_inner;
     const E* z = static_cast<const E*>(a.z) + at;
     E* dz = static_cast<E*>(a.grad) + at;
     const int64_t y = a.labels != nullptr ? a.labels[n] : 0;
     const bool ignored = a.labels != nullptr && y == a.ignore;
-    // The row from its first 16-byte boundary in whole pieces; `head` and `tail` single elements
-    // around them belong to the first threads of the first two waves.
-    const int head = min(a.V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) /
-                                  static_cast<int>(sizeof(E)));
-    const int pieces = (a.V - head) / VE, tail0 = head + pieces * VE;
-    const int single = tid < head ? tid
-                       : tid >= 64 && tid - 64 < a.V - tail0 ? tail0 + tid - 64 : -1;
+    // The row from its first 16-byte boundary in whole pieces, piece p = k S + tid with thread tid
+    // (S = the threads that NP pieces each need); the single elements around them belong to the
+    // first threads of the first two waves.
+    const uint32_t head = min(V, static_cast<uint32_t>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) /
+                                     static_cast<uint32_t>(sizeof(E)));
+    const uint32_t pieces = (V - head) / VE, tail0 = head + pieces * VE;
+    const uint32_t S = NP > 0 ? (pieces + NP - 1) / (NP > 0 ? NP : 1) : THREADS;
+    const int single = tid < head ? static_cast<int>(tid)
+                       : tid >= 64 && tid - 64 < V - tail0 ? static_cast<int>(tail0 + tid - 64) : -1;
+    const uint4* zp = reinterpret_cast<const uint4*>(z + head);
+    uint4* dzp = reinterpret_cast<uint4*>(dz + head);
     if (ignored) {
       if (a.rows != nullptr && tid == 0) a.rows[n] = 0.f;
       if (a.grad != nullptr) {
-        for (int p = tid; p < pieces; p += THREADS)
-          reinterpret_cast<uint4*>(dz + head)[p] = make_uint4(0u, 0u, 0u, 0u);
+        for (uint32_t p = tid; p < pieces; p += THREADS) dzp[p] = make_uint4(0u, 0u, 0u, 0u);
         if (single >= 0) dz[single] = from_f32<E>(0.f);
       }
       continue;
     }
-    const uint4* zp = reinterpret_cast<const uint4*>(z + head);
 
     // ---- the row and the teacher's entries
-    uint4 x[NP > 0 ? NP : 1];
-    float m = NEG_INF, sq = 0.f, s1 = 0.f;
-    if constexpr (NP > 0) {
-#pragma unroll
-      for (int k = 0; k < NP; ++k)
-        if (k * THREADS + tid < pieces) x[k] = zp[k * THREADS + tid];
-    }
+    const auto entry_id = [&](uint32_t k) { return a.ids[static_cast<int64_t>(n) * a.K + k]; };
+    const auto entry_t = [&](uint32_t k) {
+      const int64_t i = static_cast<int64_t>(n) * a.K + k;
+      return a.t_bf16 ? bf16_to_f32(static_cast<const uint16_t*>(a.t)[i])
+                      : static_cast<const float*>(a.t)[i];
+    };
+    const int64_t id0 = tid < K ? entry_id(tid) : -1;   // the loads ahead of the row's
+    const float t0 = tid < K ? entry_t(tid) : NEG_INF;
     const float xs = single >= 0 ? to_f32<E>(z[single]) : NEG_INF;
-    float tm = NEG_INF;
-    for (int k = tid; k < a.K; k += THREADS) {
-      const int64_t id = a.ids[n * a.K + k];
-      const bool use = id >= 0 && id < a.V;
-      const float t = !use ? NEG_INF
-                      : a.t_bf16 ? bf16_to_f32(static_cast<const uint16_t*>(a.t)[n * a.K + k])
-                                 : static_cast<const float*>(a.t)[n * a.K + k];
-      e_id[k] = use ? static_cast<int>(id) : -1;
-      e_mass[k] = t;
-      tm = t != t ? t : fmaxf(tm, t);
-    }
+    // A thread past S holds copies of another's pieces, and one whose last piece (only the last:
+    // S >= NP) is past the row's end a copy of the row's: neither is added nor stored.
+    const bool mine = NP == 0 || tid < S, last = NP == 0 || tid + (NP - 1) * S < pieces;
+    uint4 x[NP > 0 ? NP : 1];
     if constexpr (NP > 0) {
-      m = xs;
+      uint32_t p = min(tid, S - 1);
 #pragma unroll
-      for (int k = 0; k < NP; ++k)
-        if (k * THREADS + tid < pieces) {
+      for (int k = 0; k < NP; ++k, p += S) x[k] = ds_piece(zp, k < NP - 1 ? p : min(p, pieces - 1));
+    }
+    float tm = NEG_INF;
+    const auto take = [&](uint32_t k, int64_t id, float t) {
+      const bool use = id >= 0 && id < V;
+      t = use ? t : NEG_INF;
+      ent.id[k] = use ? static_cast<int>(id) : -1;
+      ent.t[k] = t;
+      ent.z[k] = use ? to_f32<E>(z[id]) : 0.f;
+      tm = t != t ? t : fmaxf(tm, t);
+    };
+    if (tid < K) take(tid, id0, t0);
+    for (uint32_t k = tid + THREADS; k < K; k += THREADS) take(k, entry_id(k), entry_t(k));
+    float m = xs, sq = 0.f, s1 = 0.f;
+    if constexpr (NP > 0) {
 #pragma unroll
-          for (int e = 0; e < VE; ++e) m = fmaxf(m, ds_elem<E>(x[k], e));
-        }
+      for (int k = 0; k < NP; ++k) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) m = fmaxf(m, ds_elem<E>(x[k], e));
+        ds_swept(x[k], m, tm);
+      }
     } else {
       // running maximum and sums of this thread
-      m = xs;
       sq = xs == NEG_INF ? 0.f : 1.f;
       s1 = sq;
-      for (int p = tid; p < pieces; p += THREADS) {
+      for (uint32_t p = tid; p < pieces; p += THREADS) {
         const uint4 v = zp[p];
         float pm = m;
 #pragma unroll
         for (int e = 0; e < VE; ++e) pm = fmaxf(pm, ds_elem<E>(v, e));
-        if (pm == NEG_INF) {   // nothing yet (a NaN among them is seen by the sums)
-          pm = 0.f;
-        }
+        if (pm == NEG_INF) pm = 0.f;   // nothing yet (a NaN among them is seen by the sums)
         const float d = m == NEG_INF ? 0.f : m - pm;
         sq *= ds_exp(d, kq);
         if (TWO) s1 *= ds_exp(d, DS_LOG2E);
@@ -212,113 +225,159 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(DsArgs a) {
       }
     }
     const float m_own = m;
-    if constexpr (NP > 0) {
-#pragma unroll
-      for (int k = 0; k < NP; ++k) ds_packed(x[k]);
+    m = wave_max_dpp(m);
+    tm = wave_max_dpp(tm);
+    if (lead) {
+      red[0][wid][0] = m;
+      red[0][wid][1] = tm;
     }
-    block_max2<WAVES>(m, tm, red);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      m = fmaxf(m, red[0][w][0]);
+      tm = fmaxf(tm, red[0][w][1]);
+    }
 
     // ---- sums of exponentials
     if constexpr (NP > 0) {
-      if (single >= 0) {
-        sq = ds_exp(xs - m, kq);
-        if (TWO) s1 = ds_exp(xs - m, DS_LOG2E);
-      }
 #pragma unroll
-      for (int k = 0; k < NP; ++k)
-        if (k * THREADS + tid < pieces) {
+      for (int k = 0; k < NP; ++k) {
+        float pq = 0.f, p1 = 0.f;
 #pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const float w = ds_elem<E>(x[k], e) - m;
-            sq += ds_exp(w, kq);
-            if (TWO) s1 += ds_exp(w, DS_LOG2E);
-          }
+        for (int e = 0; e < VE; ++e) {
+          const float w = ds_elem<E>(x[k], e) - m;
+          pq += ds_exp(w, kq);
+          if (TWO) p1 += ds_exp(w, DS_LOG2E);
         }
+        if (k < NP - 1 || last) {
+          sq += pq;
+          s1 += p1;
+        }
+        ds_swept(x[k], sq, s1);
+      }
+      if (!mine) sq = s1 = 0.f;
+      if (single >= 0) {
+        sq += ds_exp(xs - m, kq);
+        if (TWO) s1 += ds_exp(xs - m, DS_LOG2E);
+      }
     } else {
       const float d = m_own == NEG_INF ? 0.f : m_own - m;
       sq *= ds_exp(d, kq);
       if (TWO) s1 *= ds_exp(d, DS_LOG2E);
     }
-    if constexpr (NP > 0) {
-#pragma unroll
-      for (int k = 0; k < NP; ++k) ds_packed(x[k]);
-    }
     float ts = 0.f;
-    for (int k = tid; k < a.K; k += THREADS)
-      if (e_id[k] >= 0 && e_mass[k] != NEG_INF) ts += ds_exp(e_mass[k] - tm, kq);
-    block_sum3<WAVES>(sq, s1, ts, red);
+    for (uint32_t k = tid; k < K; k += THREADS)
+      if (ent.id[k] >= 0 && ent.t[k] != NEG_INF) ts += ds_exp(ent.t[k] - tm, kq);
+    sq = wave_sum_dpp(sq);
+    if (TWO) s1 = wave_sum_dpp(s1);
+    ts = wave_sum_dpp(ts);
+    if (lead) {
+      red[1][wid][0] = sq;
+      red[1][wid][1] = s1;
+      red[1][wid][2] = ts;
+    }
+    __syncthreads();
+    sq = s1 = ts = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      sq += red[1][w][0];
+      s1 += red[1][w][1];
+      ts += red[1][w][2];
+    }
     if (!TWO) s1 = sq;   // temperature one, or only one of the two counts
     const bool teacher = a.alpha != 0.f && ts != 0.f;   // NaN counts
 
-    // ---- the loss
-    if (a.rows != nullptr) {
-      float kl = 0.f;
-      if (teacher) {
-        const float ltq = logf(sq), lts = logf(ts);
-        for (int k = tid; k < a.K; k += THREADS) {
-          if (e_id[k] < 0) continue;
-          const float u = (e_mass[k] - tm) * a.inv_tau - lts;
-          const float p = ds_exp(e_mass[k] - tm, kq) / ts;
-          const float lq = (to_f32<E>(z[e_id[k]]) - m) * a.inv_tau - ltq;
-          if (p != 0.f) kl += p * (u - lq);
-        }
-      }
-      float u1 = 0.f, u2 = 0.f;
-      block_sum3<WAVES>(kl, u1, u2, red);
-      if (tid == 0) {
-        float loss = a.alpha * a.tau * a.tau * kl;
-        if (a.alpha != 1.f) {
-          const bool in = y >= 0 && y < a.V;
-          const float ce = in ? logf(s1) - (to_f32<E>(z[y]) - m) : __builtin_nanf("");
-          loss += (1.f - a.alpha) * ce;
-        }
-        a.rows[n] = loss;
-      }
-    }
-    if (a.grad == nullptr) {
-      __syncthreads();   // the entries' LDS is written again for the next row
-      continue;
-    }
-
-    // ---- the gradient
+    // ---- the entries' part: the loss, and each id's mass in the gradient
     float w = a.upstream != nullptr ? a.upstream[a.per_row ? n : 0] : 1.f;
     if (a.mean) w /= a.count != nullptr ? a.count[0] : static_cast<float>(a.N);
     const float wq = teacher ? w * a.alpha * a.tau : 0.f, w1 = w * (1.f - a.alpha);
-    const float cq = wq / sq;
-    float c1 = a.alpha != 1.f ? w1 / s1 : 0.f;
-    if (a.alpha != 1.f && (y < 0 || y >= a.V)) c1 = __builtin_nanf("");
+    const bool hard = a.alpha != 1.f, in = y >= 0 && y < V;
+    float kl = 0.f;
+    {
+      const float ltq = logf(sq), lts = logf(ts), inv_ts = 1.f / ts;
+      for (uint32_t k = tid; k <= K; k += THREADS) {
+        const int id = k < K ? ent.id[k] : hard && in ? static_cast<int>(y) : -1;
+        float mass = 0.f;
+        if (k == K) {
+          ent.z[K] = id >= 0 ? to_f32<E>(z[id]) : 0.f;
+          ent.id[K] = id;
+          mass = w1;
+        } else if (teacher && id >= 0) {
+          const float d = ent.t[k] - tm, p = ds_exp(d, kq) * inv_ts;
+          if (p != 0.f) kl += p * (d * a.inv_tau - lts - ((ent.z[k] - m) * a.inv_tau - ltq));
+          mass = wq * p;
+        }
+        ent.t[k] = mass;
+        const uint32_t i = id - head, p = i / VE;
+        ent.owner[k] = id < 0 ? -1
+                       : static_cast<uint32_t>(id) < head ? id
+                       : static_cast<uint32_t>(id) >= tail0 ? static_cast<int>(id - tail0 + 64)
+                                                            : static_cast<int>(p % S);
+      }
+      if (a.rows != nullptr) {
+        kl = wave_sum_dpp(kl);
+        if (lead) red[2][wid][0] = kl;
+      }
+    }
+    __syncthreads();
+    if (a.rows != nullptr && tid == 0) {
+      float loss = 0.f;
+#pragma unroll
+      for (int q = 0; q < WAVES; ++q) loss += red[2][q][0];
+      loss *= a.alpha * a.tau * a.tau;
+      if (hard) loss += (1.f - a.alpha) * (in ? logf(s1) - (ent.z[K] - m) : __builtin_nanf(""));
+      a.rows[n] = loss;
+    }
+    if (a.grad == nullptr) continue;
+
+    // ---- the gradient: the row as if no entry stood there, then each thread its entries' elements
+    // again (its own stores stay in order)
+    float c1 = hard ? w1 / s1 : 0.f;
+    if (hard && !in) c1 = __builtin_nanf("");
+    const float cq = TWO ? wq / sq : wq / sq + c1;
     const auto value = [&](float v) {
       const float d = v - m;
-      if (TWO) return cq * ds_exp(d, kq) + c1 * ds_exp(d, DS_LOG2E);
-      return (cq + c1) * ds_exp(d, kq);
+      const float g = cq * ds_exp(d, kq);
+      return TWO ? g + c1 * ds_exp(d, DS_LOG2E) : g;
     };
-    uint4* dzp = reinterpret_cast<uint4*>(dz + head);
     if constexpr (NP > 0) {
+      uint32_t p = ds_fresh(tid);
+      if (mine) {
 #pragma unroll
-      for (int k = 0; k < NP; ++k)
-        if (k * THREADS + tid < pieces) dzp[k * THREADS + tid] = ds_map<E>(x[k], value);
+        for (int k = 0; k < NP; ++k, p += S) {
+          const uint4 o = ds_map<E>(x[k], value);
+          if (k < NP - 1 || last)
+            *reinterpret_cast<uint4*>(reinterpret_cast<char*>(dzp) + p * 16u) = o;
+          __builtin_amdgcn_sched_barrier(0);   // one piece after the other: few registers
+        }
+      }
     } else {
-      for (int p = tid; p < pieces; p += THREADS) dzp[p] = ds_map<E>(zp[p], value);
+      for (uint32_t p = tid; p < pieces; p += THREADS) dzp[p] = ds_map<E>(zp[p], value);
     }
     if (single >= 0) dz[single] = from_f32<E>(value(xs));
-    // Masses of the entries; the label is entry K.
-    for (int k = tid; k < a.K; k += THREADS)
-      e_mass[k] = teacher && e_id[k] >= 0 ? wq * (ds_exp(e_mass[k] - tm, kq) / ts) : 0.f;
-    if (tid == 0) {
-      e_id[a.K] = a.alpha != 1.f && y >= 0 && y < a.V ? static_cast<int>(y) : -1;
-      e_mass[a.K] = w1;
-    }
-    __syncthreads();
-    for (int k = tid; k <= a.K; k += THREADS) {
-      const int id = e_id[k];
-      if (id < 0) continue;
-      // every entry of this id, in order: the same sum whichever of them writes it
+    // while the stores drain: the masses of every id, added in the entries' order by each of them
+    for (uint32_t k = tid; k <= K; k += THREADS) {
+      const int id = ent.id[k];
       float mass = 0.f;
-      for (int j = 0; j <= a.K; ++j)
-        if (e_id[j] == id) mass += e_mass[j];
-      dz[id] = from_f32<E>(value(to_f32<E>(z[id])) - mass);
+      for (uint32_t j = 0; j <= K; j += 4) {
+        const int4 o = *reinterpret_cast<const int4*>(ent.id + j);
+        if (o.x == id) mass += ent.t[j];
+        if (o.y == id && j + 1 <= K) mass += ent.t[j + 1];
+        if (o.z == id && j + 2 <= K) mass += ent.t[j + 2];
+        if (o.w == id && j + 3 <= K) mass += ent.t[j + 3];
+      }
+      ent.mass[k] = mass;
     }
     __syncthreads();
+    const int me = static_cast<int>(tid);
+    for (uint32_t j = 0; j <= K; j += 4) {
+      const int4 o = *reinterpret_cast<const int4*>(ent.owner + j);
+      if (o.x != me && o.y != me && o.z != me && o.w != me) continue;
+#pragma unroll
+      for (uint32_t q = 0; q < 4; ++q)
+        if (j + q <= K && ent.owner[j + q] == me)
+          dz[ent.id[j + q]] = from_f32<E>(value(ent.z[j + q]) - ent.mass[j + q]);
+    }
   }
 }
 
@@ -358,33 +417,45 @@ struct DsScratch {
   }
 };
 
-template <class E, int THREADS, int NP>
+template <class E, int THREADS, int NP, int WPE>
 void ds_launch(const DsArgs& a, bool two, int64_t grid, hipStream_t s) {
-  const unsigned lds = static_cast<unsigned>((a.K + 1) * 8);
+  const unsigned lds = static_cast<unsigned>(ds_entries(a.K) * 20);
   if (two)
-    hipLaunchKernelGGL((distill_kernel<E, THREADS, NP, true>), dim3(static_cast<unsigned>(grid)),
+    hipLaunchKernelGGL((distill_kernel<E, THREADS, NP, true, WPE>), dim3(static_cast<unsigned>(grid)),
                        dim3(THREADS), lds, s, a);
   else
-    hipLaunchKernelGGL((distill_kernel<E, THREADS, NP, false>), dim3(static_cast<unsigned>(grid)),
+    hipLaunchKernelGGL((distill_kernel<E, THREADS, NP, false, WPE>), dim3(static_cast<unsigned>(grid)),
                        dim3(THREADS), lds, s, a);
 }
 
-// The smallest workgroup whose threads hold the row in 8 pieces each; 1024 threads of 16 for longer
-// rows; beyond those the row is read twice.
+// The fewest threads that can hold the row, and then the fewest pieces a thread (all NP of them are
+// gone through, so a row should fill them); fewer threads with more pieces leave more rows on a CU at
+// different stages, and reading, exponentials and writing overlap between them.  Measured on MI355X
+// (loss and gradient): 8192 rows of 50257 bf16, two softmaxes, 256 threads of 26 pieces 404 us, 512 of
+// 13 441, 1024 of 7 677; 2031 rows of 32003 fp32, 512 of 16 140 us, of 26 222, 1024 of 8 195.
+// Registers: 4 NP and about 45 more.  Rows of a few pieces, or of more than 16384, are read twice.
 template <class E>
 int ds_run(const DsArgs& a, bool two, int64_t grid, hipStream_t s) {
   constexpr int VE = 16 / sizeof(E);
-  const int pieces = a.V / VE + 1;
-  if (pieces <= 256 * 8)
-    ds_launch<E, 256, 8>(a, two, grid, s);
-  else if (pieces <= 512 * 8)
-    ds_launch<E, 512, 8>(a, two, grid, s);
-  else if (pieces <= 1024 * 8)
-    ds_launch<E, 1024, 8>(a, two, grid, s);
-  else if (pieces <= 1024 * 16)
-    ds_launch<E, 1024, 16>(a, two, grid, s);
+  const int most = a.V / VE, least = (a.V - VE + 1) / VE;   // pieces of a row, whatever its offset
+#define GS_DS_TRY(THREADS, NP, WPE)                                               \
+  if (most <= THREADS * NP && least > NP * (NP - 1)) {                            \
+    ds_launch<E, THREADS, NP, WPE>(a, two, grid, s);                              \
+    return check_launch("distill_kernel");                                        \
+  }
+  GS_DS_TRY(256, 4, 4)
+  GS_DS_TRY(256, 8, 4)
+  GS_DS_TRY(256, 13, 4)
+  GS_DS_TRY(256, 18, 4)
+  GS_DS_TRY(256, 26, 3)
+  GS_DS_TRY(512, 18, 4)
+  GS_DS_TRY(512, 26, 2)
+  GS_DS_TRY(512, 32, 2)
+#undef GS_DS_TRY
+  if (a.V < 4096)
+    ds_launch<E, 256, 0, 4>(a, two, grid, s);
   else
-    ds_launch<E, 1024, 0>(a, two, grid, s);
+    ds_launch<E, 1024, 0, 4>(a, two, grid, s);
   return check_launch("distill_kernel");
 }
 
