@@ -24,6 +24,7 @@
 // groups through LDS in a fixed order and leaves one fp32 row; a second launch adds those per
 // sample or in all, also in a fixed order (the same bits on every run).
 #include <algorithm>
+#include <type_traits>
 
 #include "gs_common.h"
 
@@ -31,7 +32,7 @@ namespace gs {
 namespace {
 
 constexpr int QK_THREADS = 256;
-constexpr int QK_BATCH = 4;      // heads whose loads are in flight together
+constexpr int QK_BATCH = 4;   // heads whose loads are in flight together (forward)
 
 // Rows of one of the three parts (queries, keys, values): element (b, t, h, f) at
 // p[b sb + t st + h sh + f].
@@ -63,10 +64,32 @@ struct QkArgs {
   float* part[2];           // [segment][chunk][group][D] weight-gradient sums (backward)
 };
 
+// V features as they lie in memory, in whole 32-bit words where there are such.
 template <class E, int V>
 struct alignas(V * sizeof(E)) QkChunk {
-  E e[V];
+  static constexpr int W = V * sizeof(E) >= 4 ? V * sizeof(E) / 4 : 1;
+  std::conditional_t<V * sizeof(E) >= 4, uint32_t, uint16_t> w[W];
 };
+template <class E, int V>
+__device__ __forceinline__ float qk_elem(const QkChunk<E, V>& c, int i) {
+  if constexpr (sizeof(E) == 4) return __uint_as_float(c.w[i]);
+  else if constexpr (V == 1) return bf16_to_f32(c.w[0]);
+  else return __uint_as_float(i & 1 ? c.w[i >> 1] & 0xffff0000u : c.w[i >> 1] << 16);
+}
+template <class E, int V>
+__device__ __forceinline__ QkChunk<E, V> qk_pack(const float (&x)[V]) {
+  QkChunk<E, V> c;
+  if constexpr (sizeof(E) == 4) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) c.w[i] = __float_as_uint(x[i]);
+  } else if constexpr (V == 1) {
+    c.w[0] = f32_to_bf16(x[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) c.w[i >> 1] = pack_bf16x2(x[i], x[i + 1]);
+  }
+  return c;
+}
 
 // Lane-local view of a row: unit j of this lane and its two chunks' places.
 template <int V, bool INTER>
@@ -95,26 +118,22 @@ struct QkPlace {
   }
 };
 
+// A chunk as it lies in memory (whatever where the lane has nothing), and its features.
 template <class E, int V>
-__device__ __forceinline__ void qk_load(const E* __restrict__ row, int o, int D, float (&x)[V]) {
-  if (o < D) {
-    const QkChunk<E, V> c = *reinterpret_cast<const QkChunk<E, V>*>(row + o);
+__device__ __forceinline__ QkChunk<E, V> qk_load(const E* __restrict__ row, int o, int D) {
+  QkChunk<E, V> c;
+  if (o < D) c = *reinterpret_cast<const QkChunk<E, V>*>(row + o);
+  return c;
+}
+template <class E, int V>
+__device__ __forceinline__ void qk_unpack(const QkChunk<E, V>& c, int o, int D, float (&x)[V]) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = to_f32<E>(c.e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = 0.f;
-  }
+  for (int i = 0; i < V; ++i) x[i] = o < D ? qk_elem<E, V>(c, i) : 0.f;
 }
 
 template <class E, int V>
 __device__ __forceinline__ void qk_store(E* __restrict__ row, int o, int D, const float (&x)[V]) {
-  if (o < D) {
-    QkChunk<E, V> c;
-#pragma unroll
-    for (int i = 0; i < V; ++i) c.e[i] = from_f32<E>(x[i]);
-    *reinterpret_cast<QkChunk<E, V>*>(row + o) = c;
-  }
+  if (o < D) *reinterpret_cast<QkChunk<E, V>*>(row + o) = qk_pack<E, V>(x);
 }
 
 // One unit's values: the two chunks.
@@ -148,9 +167,15 @@ __device__ __forceinline__ void qk_rotate(QkUnit<V>& u, const float (&c)[V], con
   }
 }
 
-// The sum over the 2^k lanes of a row's group, in each of them.
+// The sum over the 2^k lanes of a row's group, in each of them: by DPP within 16 lanes (pairs, quads,
+// then mirrored halves, which are even by then), by shuffles beyond.
 __device__ __forceinline__ float qk_group_sum(float v, int lanes_log2) {
-  for (int k = 0; k < lanes_log2; ++k) v += __shfl_xor(v, 1 << k, 64);
+  if (lanes_log2 >= 1) v += dpp_f32<0xb1, 0xf, 0xf>(v);
+  if (lanes_log2 >= 2) v += dpp_f32<0x4e, 0xf, 0xf>(v);
+  if (lanes_log2 >= 3) v += dpp_f32<0x141, 0xf, 0xf>(v);
+  if (lanes_log2 >= 4) v += dpp_f32<0x140, 0xf, 0xf>(v);
+  if (lanes_log2 >= 5) v += __shfl_xor(v, 16, 64);
+  if (lanes_log2 >= 6) v += __shfl_xor(v, 32, 64);
   return v;
 }
 
@@ -236,43 +261,44 @@ __global__ void __launch_bounds__(QK_THREADS) qk_forward_kernel(QkArgs a) {
     const E* xr = reinterpret_cast<const E*>(in.p) + b * in.sb + t * in.st;
     E* yr = reinterpret_cast<E*>(out.p) + b * out.sb + t * out.st;
     for (int h = blk.h0; h < blk.h1; h += QK_BATCH) {
-      QkUnit<V> u[QK_BATCH][UPL];
+      QkChunk<E, V> raw[QK_BATCH][UPL][2];
 #pragma unroll
       for (int q = 0; q < QK_BATCH; ++q) {
-        const int hh = min(h + q, blk.h1 - 1);
+        if (h + q >= blk.h1) break;
 #pragma unroll
         for (int j = 0; j < UPL; ++j) {
           const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
-          qk_load<E, V>(xr + hh * in.sh, pl.o0, a.D, u[q][j].a);
-          qk_load<E, V>(xr + hh * in.sh, pl.o1, a.D, u[q][j].b);
+          raw[q][j][0] = qk_load<E, V>(xr + (h + q) * in.sh, pl.o0, a.D);
+          raw[q][j][1] = qk_load<E, V>(xr + (h + q) * in.sh, pl.o1, a.D);
         }
       }
 #pragma unroll
       for (int q = 0; q < QK_BATCH; ++q) {
-        if (norm) {
-          float ss = 0.f;
+        if (h + q >= blk.h1) break;
+        QkUnit<V> u[UPL];
+        float ss = 0.f;
 #pragma unroll
-          for (int j = 0; j < UPL; ++j)
+        for (int j = 0; j < UPL; ++j) {
+          const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
+          qk_unpack<E, V>(raw[q][j][0], pl.o0, a.D, u[j].a);
+          qk_unpack<E, V>(raw[q][j][1], pl.o1, a.D, u[j].b);
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-              ss += u[q][j].a[i] * u[q][j].a[i] + u[q][j].b[i] * u[q][j].b[i];
-          const float r = rsqrtf(qk_group_sum(ss, a.lanes_log2) * inv_d + a.eps);
+          for (int i = 0; i < V; ++i) ss += u[j].a[i] * u[j].a[i] + u[j].b[i] * u[j].b[i];
+        }
+        const float r = norm ? rsqrtf(qk_group_sum(ss, a.lanes_log2) * inv_d + a.eps) : 1.f;
 #pragma unroll
-          for (int j = 0; j < UPL; ++j)
+        for (int j = 0; j < UPL; ++j) {
+          if (norm) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-              u[q][j].a[i] *= r * w[j].a[i];
-              u[q][j].b[i] *= r * w[j].b[i];
+              u[j].a[i] *= r * w[j].a[i];
+              u[j].b[i] *= r * w[j].b[i];
             }
-        }
-        if (h + q < blk.h1) {
-#pragma unroll
-          for (int j = 0; j < UPL; ++j) {
-            if (turn) qk_rotate<V, INTER>(u[q][j], c[j], s[j], 1.f);
-            const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
-            qk_store<E, V>(yr + (h + q) * out.sh, pl.o0, a.D, u[q][j].a);
-            qk_store<E, V>(yr + (h + q) * out.sh, pl.o1, a.D, u[q][j].b);
           }
+          if (turn) qk_rotate<V, INTER>(u[j], c[j], s[j], 1.f);
+          const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
+          qk_store<E, V>(yr + (h + q) * out.sh, pl.o0, a.D, u[j].a);
+          qk_store<E, V>(yr + (h + q) * out.sh, pl.o1, a.D, u[j].b);
         }
       }
     }
@@ -315,18 +341,36 @@ __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(QkArgs a) {
     const E* xr = reinterpret_cast<const E*>(in.p) + b * in.sb + t * in.st;
     const E* gr = reinterpret_cast<const E*>(go.p) + b * go.sb + t * go.st;
     E* dr = reinterpret_cast<E*>(dx.p) + b * dx.sb + t * dx.st;
+    // the next head's rows are on their way while one is worked on
+    QkChunk<E, V> graw[UPL][2], xraw[UPL][2];
+    const auto fetch = [&](int h) {
+#pragma unroll
+      for (int j = 0; j < UPL; ++j) {
+        const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
+        if (any_g) {
+          graw[j][0] = qk_load<E, V>(gr + h * go.sh, pl.o0, a.D);
+          graw[j][1] = qk_load<E, V>(gr + h * go.sh, pl.o1, a.D);
+        }
+        if (norm) {
+          xraw[j][0] = qk_load<E, V>(xr + h * in.sh, pl.o0, a.D);
+          xraw[j][1] = qk_load<E, V>(xr + h * in.sh, pl.o1, a.D);
+        }
+      }
+    };
+    fetch(blk.h0);
     for (int h = blk.h0; h < blk.h1; ++h) {
       QkUnit<V> x[UPL], g[UPL];
 #pragma unroll
       for (int j = 0; j < UPL; ++j) {
         const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
-        qk_load<E, V>(gr + h * go.sh, any_g ? pl.o0 : a.D, a.D, g[j].a);
-        qk_load<E, V>(gr + h * go.sh, any_g ? pl.o1 : a.D, a.D, g[j].b);
+        qk_unpack<E, V>(graw[j][0], any_g ? pl.o0 : a.D, a.D, g[j].a);
+        qk_unpack<E, V>(graw[j][1], any_g ? pl.o1 : a.D, a.D, g[j].b);
         if (norm) {
-          qk_load<E, V>(xr + h * in.sh, pl.o0, a.D, x[j].a);
-          qk_load<E, V>(xr + h * in.sh, pl.o1, a.D, x[j].b);
+          qk_unpack<E, V>(xraw[j][0], pl.o0, a.D, x[j].a);
+          qk_unpack<E, V>(xraw[j][1], pl.o1, a.D, x[j].b);
         }
       }
+      if (h + 1 < blk.h1) fetch(h + 1);
       if (turn) {
 #pragma unroll
         for (int j = 0; j < UPL; ++j) qk_rotate<V, INTER>(g[j], c[j], s[j], -1.f);
@@ -507,11 +551,14 @@ int ceil_log2(int64_t x) {
   return k;
 }
 
-// How the work is shared out.  Head groups and token spans are made so that there are about
-// QK_WAVES waves (8 for each SIMD) while the work lasts: longer walks reuse the angles and, in the
-// backward pass, add more into a lane before the workgroup's sum.  Per-sample sums cut the spans
-// at samples.
-constexpr int64_t QK_WAVES = 8192;
+// How the work is shared out: into about QK_WAVES waves (3 for each SIMD, what the backward kernel's
+// registers let stay there at once) while the work lasts, by head groups first and longer token spans
+// after.  Fewer, longer walks reuse the angles and add more into a lane before the workgroup's sum.
+// Per-sample sums cut the spans at samples.  Measured on MI355X, 20 x 1024 tokens of 12 + 12 + 12 heads
+// of 64, bf16 (forward / backward, us): 32768 waves 56 / 95, 16384 46 / 77, 8192 39 / 64, 4096 34 / 57,
+// 3072 34 / 56, 2048 34 / 56; 8 x 2048 of 8 + 8 + 8 of 256: 110 / 169, 106 / 149, 98 / 133, 98 / 138,
+// 95 / 135, 103 / 137.
+constexpr int64_t QK_WAVES = 3072;
 void qk_share(QkArgs& a, int upl, int units, bool per_sample) {
   a.lanes_log2 = std::min(6, ceil_log2((units + upl - 1) / upl));
   const int64_t slots = QK_THREADS >> a.lanes_log2;
