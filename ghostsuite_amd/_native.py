@@ -10,10 +10,9 @@ samplers call ``ops()``); product code never does.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
-import math
+import importlib.util
 import threading
 from typing import Optional, Tuple
 
@@ -116,24 +115,6 @@ _SIGNATURES = {
 }
 
 
-class _QKShape(ctypes.Structure):   # gs_qk_shape
-    _fields_ = [("dtype", _I), ("B", _I64), ("T", _I64), ("D", _I64), ("n_rot", _I64),
-                ("heads", ctypes.c_int32 * 3), ("norm", _I), ("interleaved", _I), ("eps", _F),
-                ("weight", _P * 2), ("weight_dtype", _I * 2), ("table", _P),
-                ("n_positions", _I64), ("positions", _P), ("position_bits", _I),
-                ("position_stride_b", _I64), ("position_stride_t", _I64)]
-
-
-# gs_qk_rows[3]: (data, stride_b, stride_t, stride_h) of each part, eight bytes each.
-_QKRows3 = _I64 * 12
-
-
-class _Distill(ctypes.Structure):   # gs_distill
-    _fields_ = [("Z", _P), ("dtype", _I), ("N", _I64), ("V", _I64), ("inner", _I64),
-                ("stride_outer", _I64), ("stride_inner", _I64), ("teacher_ids", _P),
-                ("teacher", _P), ("teacher_dtype", _I), ("K", _I64), ("labels", _P),
-                ("ignore_index", _I64), ("temperature", _F), ("alpha", _F), ("reduction", _I)]
-
 
 def load_library() -> ctypes.CDLL:
     """Loads libghost_hip.so (built in-tree by ghostsuite_amd.build) once per process."""
@@ -182,13 +163,13 @@ def _require_device(*ts: torch.Tensor) -> torch.device:
     for t in ts:
         if t is None:
             continue
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise GhostHipError(
                 "ghostsuite_amd kernels need tensors on a ROCm GPU device; got a tensor on "
                 f"{t.device} (there is no CPU path)")
         if dev is None:
             dev = t.device
-        elif t.device != dev:
+        elif t.get_device() != dev.index:
             raise GhostHipError(f"tensors on different devices: {dev} and {t.device}")
     return dev
 
@@ -219,135 +200,23 @@ def _tokens(x: torch.Tensor, n: int, feat: int) -> int:
     return x.numel() // (n * feat) if n * feat > 0 else 0
 
 
-def _on(dev: torch.device):
-    """Kernels launch on the current device: makes `dev` that one for the body."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+_ext = None
 
 
-def _kernel_dtype(t: torch.Tensor, what: str) -> int:
-    if t.dtype not in (torch.bfloat16, torch.float32):
-        raise GhostHipError(f"{what}: bf16 or fp32, got {t.dtype}")
-    return _TORCH_TO_GS[t.dtype]
-
-
-def _features_contiguous(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-class _QKCall:
-    """The arguments of a gs_qk_rotary* call from a plan (the keywords of
-    lm_layers.qkv_norm_rotary) and its input rows: one packed tensor, or queries and keys."""
-
-    __slots__ = ("dev", "heads", "B", "T", "D", "dtype", "dt", "parts", "keep", "shape")
-
-    def __init__(self, plan, parts, qw, kw):
-        heads, table, positions = plan["heads"], plan["table"], plan["positions"]
-        self.dev = _require_device(*parts, qw, kw, table, positions)
-        self.parts = parts = [_features_contiguous(p) for p in parts]
-        self.heads = heads
-        x, total = parts[0], sum(heads)
-        if min(heads[0], heads[1]) <= 0:
-            raise GhostHipError(f"{heads[0]} query and {heads[1]} key heads")
-        size = x.shape
-        if len(parts) == 1 and not (len(size) == 3 and size[2] % total == 0) and \
-                not (len(size) == 4 and size[2] == total):
-            raise GhostHipError(f"qkv {tuple(size)} does not hold {total} heads")
-        self.B, self.T = B, T = size[0], size[1]
-        self.D = D = size[2] // total if len(size) == 3 else size[3]
-        if D <= 0:
-            raise GhostHipError("heads without features")
-        self.dtype = x.dtype
-        self.dt = dt = _kernel_dtype(x, "queries and keys")
-        for p in parts[1:]:
-            if p.shape[:2] != size[:2] or p.shape[3] != D or p.dtype != x.dtype:
-                raise GhostHipError(f"queries {tuple(size)} {x.dtype} and keys "
-                                    f"{tuple(p.shape)} {p.dtype} disagree")
-        if table.dim() != 3 or table.shape[1] != 2 or table.dtype != torch.float32 or \
-                not table.is_contiguous() or 2 * table.shape[2] > D:
-            raise GhostHipError(f"table {tuple(table.shape)} {table.dtype}: contiguous fp32 "
-                                f"[positions, 2, n_rot / 2] with n_rot up to {D} expected")
-        n_rot = 2 * table.shape[2]
-        w_ptr, w_dt = [None, None], [dt, dt]
-        self.keep = [table, positions]   # alive until the call is enqueued
-        for i, w in enumerate((qw, kw)):
-            if w is None:
-                continue
-            if w.shape != (D,):
-                raise GhostHipError(f"norm weight {tuple(w.shape)}: [{D}] expected")
-            w_dt[i] = _kernel_dtype(w, "norm weights")
-            if not w.is_contiguous():
-                w = w.contiguous()
-                self.keep.append(w)
-            w_ptr[i] = w.data_ptr()
-        pos, bits, p_sb, p_st = None, 0, 0, 0
-        if positions is not None and n_rot:
-            if positions.dtype not in (torch.int32, torch.int64) or \
-                    tuple(positions.shape) not in ((T,), (1, T), (B, T)):
-                raise GhostHipError(f"positions {tuple(positions.shape)} {positions.dtype}: int32 "
-                                    f"or int64 [{T}] or [{B}, {T}] expected")
-            pos, bits = positions.data_ptr(), 32 if positions.dtype == torch.int32 else 64
-            p_st = positions.stride(-1)
-            if positions.dim() == 2 and positions.shape[0] == B:
-                p_sb = positions.stride(0)
-        self.shape = _QKShape(dt, B, T, D, n_rot, heads, plan["norm"], plan["interleaved"],
-                              plan["eps"], tuple(w_ptr), tuple(w_dt),
-                              table.data_ptr() if n_rot else None, table.shape[0], pos, bits, p_sb,
-                              p_st)
-
-    def rows(self, parts):
-        """gs_qk_rows[3] of input-shaped tensors ([B, T, heads, D] each, or one packed)."""
-        out, D, (hq, hk, hv) = [], self.D, self.heads
-        if len(parts) == 1:
-            x, = parts
-            st = x.stride()
-            sh = st[2] if len(st) == 4 else D
-            p, step = x.data_ptr(), sh * x.element_size()
-            return _QKRows3(p, st[0], st[1], sh, p + hq * step, st[0], st[1], sh,
-                            p + (hq + hk) * step if hv else 0, st[0], st[1], sh)
-        for x in parts:
-            out += [x.data_ptr(), *x.stride()[:3]]
-        return _QKRows3(*out)
-
-    @staticmethod
-    def heads_first(tensors):
-        """gs_qk_rows[3] of [B, heads, T, D] tensors (None: data NULL)."""
-        out = []
-        for t in tensors:
-            if t is None:
-                out += (0, 0, 0, 0)
-            else:
-                st = t.stride()
-                out += (t.data_ptr(), st[0], st[2], st[1])
-        return _QKRows3(*out)
-
-    def gradients(self, grads):
-        """The output gradients as the kernels take them (features contiguous)."""
-        out = []
-        for h, g in zip(self.heads, grads):
-            if g is not None:
-                if g.shape != (self.B, h, self.T, self.D) or g.dtype != self.dtype:
-                    raise GhostHipError(f"output gradient {tuple(g.shape)} {g.dtype}")
-                if g.device != self.dev:
-                    raise GhostHipError(f"tensors on different devices: {self.dev} and {g.device}")
-                g = _features_contiguous(g)
-            out.append(g)
-        return out
-
-    def workspace(self, query: str) -> int:
-        """The bytes a query answers: they follow from the sizes alone."""
-        s = self.shape
-        return _qk_size(query, self.dt, self.B, self.T, self.D, s.n_rot, self.heads,
-                        s.interleaved)
-
-
-@functools.lru_cache(maxsize=4096)
-def _qk_size(query, dt, B, T, D, n_rot, heads, interleaved) -> int:
-    # (any table: nothing of it is read)
-    shape = _QKShape(dt, B, T, D, n_rot, heads, 1, interleaved, 0.0, (None, None), (dt, dt), 256,
-                     1, None, 0, 0, 0)
-    return getattr(load_library(), query)(ctypes.byref(shape))
+def _lm():
+    """The extension module around the language-model operators (csrc/lm_autograd.cpp)."""
+    global _ext
+    if _ext is None:
+        load_library()   # says how to build, when nothing is
+        path = _build.extension_path()
+        if not path.exists():
+            raise GhostHipError(f"{path} is not built: run `python ghostsuite_amd/build.py` first")
+        spec = importlib.util.spec_from_file_location(_build.EXTNAME, path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.raise_as(GhostHipError)
+        _ext = mod
+    return _ext
 
 
 class HipOps:
@@ -914,233 +783,35 @@ class HipOps:
         _check(rc, "gs_ordered_sum")
         return total
 
-    # ---- embedding lookup, query / key norms with rotation, distillation (lm_layers) ----
+    # ---- embedding lookup, query / key norms with rotation, distillation (lm_layers): through the
+    # extension, which checks, allocates and records them for autograd
 
     def embedding_lookup(self, ids: torch.Tensor, weight: torch.Tensor, scale: float,
-                         padding_idx: Optional[int] = None, want_grad_ids: bool = False):
-        """(scale * weight[ids], ids for embedding_grad or None): gs_embedding_lookup."""
-        dev = _require_device(ids, weight)
-        dt = _kernel_dtype(weight, "embedding weight")
-        if ids.dtype not in (torch.int32, torch.int64):
-            raise GhostHipError(f"token ids of dtype {ids.dtype}: int32 or int64 expected")
-        if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
-            raise GhostHipError(f"embedding weight {tuple(weight.shape)}: [vocab, d] expected")
-        ids, weight = ids.contiguous(), weight.contiguous()
-        vocab, d = weight.shape
-        out = torch.empty((*ids.shape, d), dtype=weight.dtype, device=dev)
-        grad_ids = None
-        if want_grad_ids:
-            same = padding_idx is None and ids.dtype == torch.int64
-            grad_ids = ids if same else torch.empty(ids.shape, dtype=torch.int64, device=dev)
-        if ids.numel():
-            with _on(dev):
-                rc = load_library().gs_embedding_lookup(
-                    ids.data_ptr(), 32 if ids.dtype == torch.int32 else 64, ids.numel(),
-                    weight.data_ptr(), dt, vocab, d, scale,
-                    -1 if padding_idx is None else padding_idx, out.data_ptr(),
-                    None if grad_ids is ids else _ptr(grad_ids), _stream(dev))
-            _check(rc, "gs_embedding_lookup")
-        return out, grad_ids
+                         padding_idx: Optional[int] = None) -> torch.Tensor:
+        """scale * weight[ids] (gs_embedding_lookup; its gradient gs_embedding_train_grad)."""
+        return _lm().embedding_lookup(ids, weight, scale, padding_idx)
 
-    def embedding_grad(self, ids: torch.Tensor, G: torch.Tensor, shape, dtype: torch.dtype,
-                       scale: float) -> torch.Tensor:
-        """scale * the rows of G added up by id, [vocab, d]: gs_embedding_train_grad over one
-        sample of all the tokens."""
-        dev = _require_device(ids, G)
-        if not ids.numel():
-            return torch.zeros(shape, dtype=dtype, device=dev)
-        out = torch.empty(shape, dtype=dtype, device=dev)
-        G, n, (vocab, d) = G.contiguous(), ids.numel(), shape
-        ws_bytes = _size("gs_embedding_train_grad_workspace", 1, 0, n, d, vocab)
-        ws = _workspace(ws_bytes, dev)
-        with _on(dev):
-            rc = load_library().gs_embedding_train_grad(
-                ids.data_ptr(), G.data_ptr(), _kernel_dtype(G, "output gradient"), 1, 0, 1, n, d,
-                vocab, scale, out.data_ptr(), _TORCH_TO_GS[dtype], 0, ws.data_ptr(), ws_bytes,
-                _stream(dev))
-        _check(rc, "gs_embedding_train_grad")
-        return out
+    def qk_norm_rotary(self, q: torch.Tensor, k: Optional[torch.Tensor], heads, table, positions, qw,
+                       kw, norm: bool, eps: float, interleaved: bool):
+        """[queries, keys] of q and k, or with k None [queries, keys, values] of a packed q, heads
+        first (gs_qk_rotary, gs_qk_rotary_grad); heads: of each of the three parts."""
+        return _lm().qk_norm_rotary(q, k, heads, table, positions, qw, kw, norm, eps, interleaved)
 
-    def qk_norm_rotary(self, plan, parts, qw, kw):
-        """Rotated queries and keys (and values), heads first: gs_qk_rotary.  plan: heads, table,
-        positions, norm, eps, interleaved; parts: (qkv,) or (q, k)."""
-        c = _QKCall(plan, parts, qw, kw)
-        out = [torch.empty((c.B, h, c.T, c.D), dtype=c.dtype, device=c.dev)
-               for h in c.heads if h]
-        if c.B and c.T:
-            with _on(c.dev):
-                rc = load_library().gs_qk_rotary(ctypes.byref(c.shape), c.rows(c.parts),
-                                                 c.heads_first(out), _stream(c.dev))
-            _check(rc, "gs_qk_rotary")
-        return out
+    def qk_norm_rotary_dots(self, q: torch.Tensor, k: Optional[torch.Tensor], heads, table,
+                            positions, qw, kw, eps: float, interleaved: bool, grads, n_val: int, *,
+                            val_start: Optional[int] = None, grad_scale: Optional[float] = None):
+        """[dot_q, dot_k, grad_q, grad_k] of the norm weights from the outputs' gradients (None:
+        zeros): gs_qk_rotary_dots; the train gradients None without grad_scale."""
+        return _lm().qk_norm_rotary_dots(q, k, heads, table, positions, qw, kw, eps, interleaved,
+                                         grads, n_val, val_start, grad_scale)
 
-    def qk_norm_rotary_grad(self, plan, parts, qw, kw, grads, *, want_x: bool, want_qw: bool,
-                            want_kw: bool):
-        """([input gradients] as parts or Nones, q weight gradient, k weight gradient):
-        gs_qk_rotary_grad; grads: the outputs' gradients, None for zeros."""
-        c = _QKCall(plan, parts, qw, kw)
-        grads = c.gradients(grads)
-        dparts = [torch.empty(p.shape, dtype=c.dtype, device=c.dev) if want_x else None
-                  for p in parts]
-        make = torch.empty if c.B and c.T else torch.zeros
-        dqw = make(c.D, dtype=qw.dtype, device=c.dev) if want_qw else None
-        dkw = make(c.D, dtype=kw.dtype, device=c.dev) if want_kw else None
-        if c.B and c.T and (want_x or want_qw or want_kw):
-            nbytes, ws = 0, None
-            if want_qw or want_kw:
-                nbytes = c.workspace("gs_qk_rotary_grad_workspace")
-                ws = _workspace(nbytes, c.dev)
-            with _on(c.dev):
-                rc = load_library().gs_qk_rotary_grad(
-                    ctypes.byref(c.shape), c.rows(c.parts), c.heads_first(grads),
-                    c.rows(dparts) if want_x else None, _ptr(dqw), _ptr(dkw), _ptr(ws), nbytes,
-                    _stream(c.dev))
-            _check(rc, "gs_qk_rotary_grad")
-        return dparts, dqw, dkw
-
-    def qk_norm_rotary_dots(self, plan, parts, qw, kw, grads, n_val: int, *, val_start=None,
-                            grad_scale: Optional[float] = None):
-        """(dot_q, dot_k, grad_q, grad_k) of the norm weights: gs_qk_rotary_dots; the train
-        gradients None without grad_scale."""
-        c = _QKCall(plan, parts, qw, kw)
-        if not (c.B and c.T):
-            raise GhostHipError("qk_norm_rotary_dots: no tokens")
-        grads = c.gradients(grads)
-        n_t = c.B - n_val
-        vs = n_t if val_start is None else int(val_start)
-        dots = [torch.empty(max(n_t, 0), dtype=torch.float32, device=c.dev) for _ in range(2)]
-        gw = [None, None]
-        if grad_scale is not None:
-            gw = [torch.empty(c.D, dtype=c.dtype if w is None else w.dtype, device=c.dev)
-                  for w in (qw, kw)]
-        nbytes = c.workspace("gs_qk_rotary_dots_workspace")
-        ws = _workspace(nbytes, c.dev)
-        with _on(c.dev):
-            rc = load_library().gs_qk_rotary_dots(
-                ctypes.byref(c.shape), c.rows(c.parts), c.heads_first(grads), n_val, vs,
-                dots[0].data_ptr(), dots[1].data_ptr(), _ptr(gw[0]), _ptr(gw[1]),
-                float(grad_scale or 0.0), ws.data_ptr(), nbytes, _stream(c.dev))
-        _check(rc, "gs_qk_rotary_dots")
-        return dots[0], dots[1], gw[0], gw[1]
-
-    def distill_loss(self, logits, teacher_ids, teacher_logits, labels, *, temperature: float,
-                     alpha: float, ignore_index: int, reduction: str, want_grad: bool = False):
-        """(loss, None), or with want_grad (loss, a _DistillCall that holds the gradient for an
-        upstream of one): gs_distill_loss."""
-        c = _DistillCall(logits, teacher_ids, teacher_logits, labels, temperature, alpha,
-                         ignore_index, reduction)
-        shape = logits.shape[:-1] if reduction == "none" else ()
-        if c.d.N == 0:
-            c.grad = torch.empty_like(logits)
-            return (torch.full(shape, math.nan if reduction == "mean" else 0.0, device=c.dev),
-                    c if want_grad else None)
-        loss = torch.empty(shape, dtype=torch.float32, device=c.dev)
-        c.allocate(want_grad)
-        with _on(c.dev):
-            rc = load_library().gs_distill_loss(ctypes.byref(c.d), loss.data_ptr(), _ptr(c.grad),
-                                                c.ws.data_ptr(), c.ws.numel(), _stream(c.dev))
-        _check(rc, "gs_distill_loss")
-        return loss, c if want_grad else None
-
-    def distill_grad(self, logits, teacher_ids, teacher_logits, labels, *, temperature: float,
-                     alpha: float, ignore_index: int, reduction: str, upstream: torch.Tensor,
-                     unit: Optional["_DistillCall"] = None) -> torch.Tensor:
-        """The logits' gradient for a loss gradient `upstream`: gs_distill_grad.  unit: what
-        distill_loss gave for these tensors, used up by this call."""
-        c = unit
-        if c is None or not c.reads(logits, teacher_ids, teacher_logits, labels):
-            c = _DistillCall(logits, teacher_ids, teacher_logits, labels, temperature, alpha,
-                             ignore_index, reduction)
-        if c.d.N == 0:
-            return torch.empty_like(logits)
-        filled = c.grad is not None
-        if not filled:
-            c.allocate(True)
-        if upstream.dtype != torch.float32 or not upstream.is_contiguous():
-            upstream = upstream.to(torch.float32).contiguous()
-        with _on(c.dev):
-            rc = load_library().gs_distill_grad(ctypes.byref(c.d), upstream.data_ptr(),
-                                                int(filled), c.grad.data_ptr(), c.ws.data_ptr(),
-                                                c.ws.numel(), _stream(c.dev))
-        _check(rc, "gs_distill_grad")
-        return c.grad if c.grad.shape == logits.shape else c.grad.view(logits.shape)
-
-
-class _DistillCall:
-    """The arguments of a gs_distill_* call, the tensors they point to, its scratch memory and
-    the gradient it fills."""
-
-    __slots__ = ("dev", "d", "given", "held", "ws", "grad")
-
-    def __init__(self, logits, teacher_ids, teacher, labels, temperature, alpha, ignore_index,
-                 reduction):
-        self.dev = _require_device(logits, teacher_ids, teacher, labels)
-        lead = logits.shape[:-1]
-        if logits.dim() < 1 or logits.shape[-1] == 0 or teacher.shape != teacher_ids.shape or \
-                teacher.dim() != logits.dim() or teacher.shape[:-1] != lead or \
-                teacher.shape[-1] == 0 or (labels is not None and labels.shape != lead):
-            raise GhostHipError(
-                f"logits {tuple(logits.shape)}, teacher ids {tuple(teacher_ids.shape)}, teacher "
-                f"logits {tuple(teacher.shape)}, labels "
-                f"{None if labels is None else tuple(labels.shape)}: [..., V], [..., K] twice and "
-                "[...] expected")
-        if labels is not None and labels.is_floating_point() or teacher_ids.is_floating_point():
-            raise GhostHipError("teacher ids and labels have to be integers")
-        self.given = tuple(None if t is None else (t.data_ptr(), t.stride())
-                           for t in (logits, teacher_ids, teacher, labels))
-        dtype = _kernel_dtype(logits, "logits")
-        if teacher.dtype not in (torch.bfloat16, torch.float32):
-            teacher = teacher.float()
-        teacher, teacher_ids = teacher.contiguous(), teacher_ids.to(torch.int64).contiguous()
-        labels = None if labels is None else labels.to(torch.int64).contiguous()
-        z = _rows_of_logits(logits)
-        N, V = math.prod(lead), z.shape[-1]
-        inner, outer, row = N, 0, z.stride(-2)
-        if z.dim() == 3:
-            inner, outer = z.shape[1], z.stride(0)
-        elif N == 1:
-            row = V
-        self.held = (z, teacher_ids, teacher, labels)
-        self.d = _Distill(z.data_ptr(), dtype, N, V, inner, outer, row, teacher_ids.data_ptr(),
-                          teacher.data_ptr(), _TORCH_TO_GS[teacher.dtype], teacher.shape[-1],
-                          _ptr(labels), ignore_index, temperature, alpha, REDUCTIONS[reduction])
-        self.ws = self.grad = None
-
-    def reads(self, *tensors) -> bool:
-        """Whether these are the tensors it was made from (autograd may have moved what it saved)."""
-        return self.given == tuple(None if t is None else (t.data_ptr(), t.stride())
-                                   for t in tensors)
-
-    def allocate(self, want_grad: bool) -> None:
-        if self.ws is None:
-            nbytes = load_library().gs_distill_workspace(ctypes.byref(self.d))
-            self.ws = _workspace(nbytes, self.dev)
-        if want_grad:
-            self.grad = _empty_as(self.held[0])
-
-
-def _rows_of_logits(z: torch.Tensor) -> torch.Tensor:
-    """z as [N, V] or [B, T, V] with contiguous, non-overlapping rows; a copy where its strides
-    do not allow that."""
-    V = z.shape[-1]
-    if z.dim() != 3:
-        z = z.reshape(-1, V)
-    T = z.shape[-2]
-    ok = (V == 1 or z.stride(-1) == 1) and (T == 1 or z.stride(-2) >= V)
-    if z.dim() == 3 and z.shape[0] > 1:
-        ok = ok and z.stride(0) >= (T - 1) * z.stride(1) + V
-    return z if ok else z.contiguous()
-
-
-def _empty_as(z: torch.Tensor) -> torch.Tensor:
-    """An uninitialised tensor of z's shape and strides at z's offset from a 16-byte boundary (the
-    kernels read and write the same 16-byte pieces of both)."""
-    off = z.data_ptr() % 16 // z.element_size()
-    if off == 0 and z.is_contiguous():
-        return torch.empty(z.shape, dtype=z.dtype, device=z.device)
-    span = 1 + sum((n - 1) * s for n, s in zip(z.shape, z.stride()))
-    base = torch.empty(off + span, dtype=z.dtype, device=z.device)
-    return base.as_strided(z.shape, z.stride(), off)
+    def distillation_loss(self, logits: torch.Tensor, teacher_ids: torch.Tensor,
+                          teacher_logits: torch.Tensor, labels: Optional[torch.Tensor],
+                          temperature: float, alpha: float, ignore_index: int,
+                          reduction: str) -> torch.Tensor:
+        """gs_distill_loss; its gradient gs_distill_grad."""
+        return _lm().distillation_loss(logits, teacher_ids, teacher_logits, labels, temperature,
+                                       alpha, ignore_index, REDUCTIONS[reduction])
 
 
 _backend = None

@@ -1,4 +1,5 @@
-"""Build recipe for libghost_hip.so: hipcc for gfx950, one object per source, in-tree.
+"""Build recipe for libghost_hip.so: hipcc for gfx950, one object per source, in-tree; and for
+_lm_autograd.so, the Python extension (C++, torch's headers) around its language-model operators.
 
 The library is a plain C-ABI shared object (include/ghost_hip.h); it depends only on the HIP
 runtime.  At run time it binds to the libamdhip64.so.7 that torch has already loaded (the
@@ -12,12 +13,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIBDIR = PKG / "lib"
 LIBNAME = "libghost_hip.so"
+EXTNAME = "_lm_autograd"
 INCLUDE = PKG.parent / "include"
 ARCH = "gfx950"
 
@@ -49,8 +52,38 @@ def library_path() -> Path:
     return LIBDIR / LIBNAME
 
 
+def extension_path() -> Path:
+    return LIBDIR / (EXTNAME + ".so")
+
+
+def _run(cmd: list[str], what: str, verbose: bool) -> None:
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{what} failed:\n{res.stderr}")
+
+
+def _torch_flags() -> tuple[list[str], list[str]]:
+    """Compiler and linker flags of a Python extension over the installed torch."""
+    import torch
+    root = Path(torch.__path__[0])
+    rocm = Path(shutil.which(hipcc()) or hipcc()).resolve().parent.parent
+    compile_flags = [
+        "-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+        "-DTORCH_API_INCLUDE_EXTENSION_H",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        f"-I{INCLUDE}", f"-isystem{root / 'include'}",
+        f"-isystem{root / 'include/torch/csrc/api/include'}", f"-isystem{rocm / 'include'}",
+        f"-isystem{sysconfig.get_paths()['include']}"]
+    link_flags = [f"-L{root / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch",
+                  "-ltorch_python"]
+    return compile_flags, link_flags
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
-    """Compiles every csrc/*.hip for gfx950 and links libghost_hip.so (always rebuilds)."""
+    """Compiles every csrc/*.hip for gfx950 and links libghost_hip.so, then the extension (always
+    rebuilds)."""
     cc = hipcc()
     objdir = PKG / "_build"
     objdir.mkdir(exist_ok=True)
@@ -73,9 +106,16 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
             print(errs, file=sys.stderr)
         return obj
 
-    n = jobs or min(len(srcs), max(1, min(8, os.cpu_count() or 1)))
+    cxx = os.environ.get("CXX") or "g++"
+    ext_compile, ext_link = _torch_flags()
+    ext_obj = objdir / (EXTNAME + ".ext.o")
+
+    n = jobs or min(len(srcs) + 1, max(1, min(8, os.cpu_count() or 1)))
     with cf.ThreadPoolExecutor(max_workers=n) as ex:
+        ext = ex.submit(_run, [cxx, *ext_compile, "-c", str(CSRC / "lm_autograd.cpp"), "-o",
+                               str(ext_obj)], "g++ for lm_autograd.cpp", verbose)
         objs = list(ex.map(compile_one, srcs))
+        ext.result()
     out = library_path()
     tmp = out.with_suffix(".so.tmp")
     cmd = [cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
@@ -85,6 +125,11 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stderr}")
     os.replace(tmp, out)
+    # next to libghost_hip.so, which it finds there
+    ext_tmp = extension_path().with_suffix(".so.tmp")
+    _run([cxx, "-shared", "-fPIC", str(ext_obj), "-o", str(ext_tmp), f"-L{LIBDIR}",
+          f"-l:{LIBNAME}", *ext_link, "-Wl,-rpath,$ORIGIN"], "link of the extension", verbose)
+    os.replace(ext_tmp, extension_path())
     return out
 
 

@@ -20,7 +20,6 @@ from typing import Optional, Tuple
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from ._native import GhostHipError, ops
 
@@ -28,36 +27,7 @@ __all__ = ["embedding_lookup", "ScaledEmbedding", "rotary_table", "qkv_norm_rota
            "qk_norm_rotary", "QKNormRotary", "distillation_loss"]
 
 
-def _records(*tensors) -> bool:
-    """Whether autograd has to see an operation on these tensors."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _once(backward):
-    """once_differentiable, whose wrapping costs a backward pass 8 us on the host, only where the
-    backward pass itself is recorded."""
-    recorded = once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
-    return staticmethod(run)
-
-
 # Embedding lookup ###########################################################################
-
-class _Lookup(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids, weight, scale, padding_idx):
-        out, grad_ids = ops().embedding_lookup(ids, weight, scale, padding_idx, want_grad_ids=True)
-        ctx.save_for_backward(grad_ids)
-        ctx.scale, ctx.shape, ctx.dtype = scale, weight.shape, weight.dtype
-        return out
-
-    @_once
-    def backward(ctx, g):
-        ids, = ctx.saved_tensors
-        return None, ops().embedding_grad(ids, g, ctx.shape, ctx.dtype, ctx.scale), None, None
-
 
 def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
                      padding_idx: Optional[int] = None) -> torch.Tensor:
@@ -71,9 +41,7 @@ def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
             raise GhostHipError(f"padding_idx {padding_idx} outside the table of "
                                 f"{weight.shape[0]} rows")
         padding_idx %= weight.shape[0]
-    if _records(weight):
-        return _Lookup.apply(ids, weight, float(scale), padding_idx)
-    return ops().embedding_lookup(ids, weight, float(scale), padding_idx)[0]
+    return ops().embedding_lookup(ids, weight, float(scale), padding_idx)
 
 
 class ScaledEmbedding(nn.Embedding):
@@ -109,36 +77,9 @@ def rotary_table(n_positions: int, n_rot: int, base: float = 10000.0, device=Non
     return torch.stack((a.cos(), a.sin()), dim=1).float()
 
 
-class _QKNormRotary(torch.autograd.Function):
-    """parts: one packed tensor, or queries and keys."""
-
-    @staticmethod
-    def forward(ctx, plan, qw, kw, *parts):
-        ctx.set_materialize_grads(False)
-        ctx.plan = plan
-        ctx.save_for_backward(qw, kw, plan["table"], plan["positions"], *parts)
-        return tuple(ops().qk_norm_rotary(plan, parts, qw, kw))
-
-    @_once
-    def backward(ctx, *grads):
-        qw, kw, table, positions, *parts = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        plan = ctx.plan
-        if table is not plan["table"] or positions is not plan["positions"]:
-            plan = dict(plan, table=table, positions=positions)   # as unpacked for this pass
-        dparts, dqw, dkw = ops().qk_norm_rotary_grad(
-            plan, parts, qw, kw, grads, want_x=any(need[3:]), want_qw=need[1], want_kw=need[2])
-        return (None, dqw, dkw, *dparts)
-
-
-def _rotated_heads(parts, heads, table, positions, q_weight, k_weight, norm, eps, interleaved):
+def _check_norm(norm, q_weight, k_weight) -> None:
     if not norm and (q_weight is not None or k_weight is not None):
         raise GhostHipError("norm weights without the norm")
-    plan = {"heads": heads, "table": table, "positions": positions, "norm": bool(norm),
-            "eps": float(eps), "interleaved": bool(interleaved)}
-    if _records(q_weight, k_weight, *parts):
-        return _QKNormRotary.apply(plan, q_weight, k_weight, *parts)
-    return tuple(ops().qk_norm_rotary(plan, parts, q_weight, k_weight))
 
 
 def qkv_norm_rotary(qkv: torch.Tensor, n_head: int, n_kv_head: int, table: torch.Tensor,
@@ -156,8 +97,10 @@ def qkv_norm_rotary(qkv: torch.Tensor, n_head: int, n_kv_head: int, table: torch
     (n_rot 0: no rotation), the pairs n_rot / 2 apart, or neighbours with ``interleaved``.
     positions: None (0, 1, ... in each sample) or integers [T] or [B, T]; one outside the table
     makes the rotated features NaN.  Formed in fp32, rounded once; D up to 512."""
-    return _rotated_heads((qkv,), (n_head, n_kv_head, n_kv_head), table, positions, q_weight,
-                          k_weight, norm, eps, interleaved)
+    _check_norm(norm, q_weight, k_weight)
+    q, k, v = ops().qk_norm_rotary(qkv, None, (n_head, n_kv_head, n_kv_head), table, positions,
+                                   q_weight, k_weight, bool(norm), float(eps), bool(interleaved))
+    return q, k, v
 
 
 def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor,
@@ -171,8 +114,10 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor,
     if q.dim() != 4 or k.dim() != 4:
         raise GhostHipError(f"expected queries and keys [B, T, heads, D], got {tuple(q.shape)} "
                             f"and {tuple(k.shape)}")
-    return _rotated_heads((q, k), (q.shape[2], k.shape[2], 0), table, positions, q_weight,
-                          k_weight, norm, eps, interleaved)
+    _check_norm(norm, q_weight, k_weight)
+    q, k = ops().qk_norm_rotary(q, k, (q.shape[2], k.shape[2], 0), table, positions, q_weight,
+                                k_weight, bool(norm), float(eps), bool(interleaved))
+    return q, k
 
 
 class QKNormRotary(nn.Module):
@@ -219,26 +164,6 @@ class QKNormRotary(nn.Module):
 
 # Loss against a teacher's top logits #########################################################
 
-class _Distillation(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, teacher_ids, teacher_logits, labels, how):
-        # A mean's or sum's gradient is written in the loss's own pass, for an upstream gradient of
-        # one; the backward pass keeps it or, for another upstream, forms it again.
-        loss, ctx.unit = ops().distill_loss(logits, teacher_ids, teacher_logits, labels, **how,
-                                            want_grad=how["reduction"] != "none")
-        ctx.save_for_backward(logits, teacher_ids, teacher_logits, labels)
-        ctx.how = how
-        return loss
-
-    @_once
-    def backward(ctx, g):
-        logits, teacher_ids, teacher_logits, labels = ctx.saved_tensors
-        unit, ctx.unit = ctx.unit, None   # handed out once: the caller may change it
-        grad = ops().distill_grad(logits, teacher_ids, teacher_logits, labels, **ctx.how,
-                                  upstream=g, unit=unit)
-        return grad, None, None, None, None
-
-
 def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor,
                       teacher_logits: torch.Tensor, labels: Optional[torch.Tensor] = None, *,
                       temperature: float = 1.0, alpha: float = 1.0, ignore_index: int = -100,
@@ -262,9 +187,5 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor,
         raise GhostHipError(f"reduction {reduction!r}: 'mean', 'sum' or 'none'")
     if labels is None and alpha != 1.0:
         raise GhostHipError("labels are needed unless alpha is 1")
-    how = {"temperature": float(temperature), "alpha": float(alpha),
-           "ignore_index": int(ignore_index), "reduction": reduction}
-    if _records(logits):
-        return _Distillation.apply(logits, teacher_ids.detach(), teacher_logits.detach(), labels,
-                                   how)
-    return ops().distill_loss(logits, teacher_ids, teacher_logits, labels, **how)[0]
+    return ops().distillation_loss(logits, teacher_ids, teacher_logits, labels, float(temperature),
+                                   float(alpha), int(ignore_index), reduction)

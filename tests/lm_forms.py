@@ -167,28 +167,25 @@ class LmOracleOps(OracleOps):
     def embedding_layer_pass(self, ids, G, *args, **kw):
         return super().embedding_layer_pass(*self._inside(ids, G), *args, **kw)
 
-    def embedding_lookup(self, ids, weight, scale, padding_idx=None, want_grad_ids=False):
-        grad_ids = ids if padding_idx is None else ids.masked_fill(ids == padding_idx, -1)
-        out = lookup(ids, f64(weight), scale).to(weight.dtype)
-        return out, grad_ids if want_grad_ids else None
+    # (differentiable as they stand: autograd records the float64 forms)
+    def embedding_lookup(self, ids, weight, scale, padding_idx=None):
+        w = weight.double()
+        if padding_idx is not None:
+            w = torch.where((torch.arange(len(w)) == padding_idx)[:, None], w.detach(), w)
+        return lookup(ids, w, scale).to(weight.dtype)
 
-    def embedding_grad(self, ids, G, shape, dtype, scale):
-        return lookup_grad(ids, f64(G), shape[0], scale)[0].to(dtype)
+    def qk_norm_rotary(self, q, k, heads, table, positions, qw, kw, norm, eps, interleaved):
+        parts = [p.double() for p in (q, k) if p is not None]
+        w = [None if x is None else x.double() for x in (qw, kw)]
+        return [y.to(q.dtype).contiguous()
+                for y in qk_all(plan(heads, table, positions, norm, eps, interleaved), parts, *w)]
 
-    def qk_norm_rotary(self, plan, parts, qw, kw):
-        return [y.to(parts[0].dtype).contiguous()
-                for y in qk_all(plan, [f64(p) for p in parts], f64(qw), f64(kw))]
-
-    def qk_norm_rotary_grad(self, plan, parts, qw, kw, grads, *, want_x, want_qw, want_kw):
-        dx, dq, dk = qk_grads(plan, parts, qw, kw, grads)
-        dt = parts[0].dtype
-        return ([d.to(dt) if want_x else None for d in dx], dq.to(qw.dtype) if want_qw else None,
-                dk.to(kw.dtype) if want_kw else None)
-
-    def qk_norm_rotary_dots(self, plan, parts, qw, kw, grads, n_val, *, val_start=None,
-                            grad_scale=None):
-        self.calls.append(("qk_norm_rotary_dots", tuple(parts[0].shape)))
-        _, dq, dk = qk_grads(plan, parts, qw, kw, grads, per_sample=True)
+    def qk_norm_rotary_dots(self, q, k, heads, table, positions, qw, kw, eps, interleaved, grads,
+                            n_val, *, val_start=None, grad_scale=None):
+        self.calls.append(("qk_norm_rotary_dots", tuple(q.shape)))
+        parts = [p for p in (q, k) if p is not None]
+        _, dq, dk = qk_grads(plan(heads, table, positions, True, eps, interleaved), parts, qw, kw,
+                             grads, per_sample=True)
         B = dq.shape[0]
         vs = B - n_val if val_start is None else val_start
         val = torch.zeros(B, dtype=torch.bool)
@@ -198,25 +195,14 @@ class LmOracleOps(OracleOps):
             out.append(None if grad_scale is None else (s[~val].sum(0) * grad_scale).to(w.dtype))
         return out
 
-    def _rows(self, logits, ids, t, labels, temperature, alpha, ignore_index):
+    def distillation_loss(self, logits, ids, t, labels, temperature, alpha, ignore_index, reduction):
         V, K = logits.shape[-1], ids.shape[-1]
-        return distill_rows(logits.reshape(-1, V), ids.reshape(-1, K), f64(t).reshape(-1, K),
-                            None if labels is None else labels.reshape(-1), temperature, alpha,
-                            ignore_index)
-
-    def distill_loss(self, logits, ids, t, labels, *, temperature, alpha, ignore_index, reduction,
-                     want_grad=False):
-        rows, kept = self._rows(f64(logits), ids, t, labels, temperature, alpha, ignore_index)
+        rows, kept = distill_rows(logits.double().reshape(-1, V), ids.reshape(-1, K),
+                                  f64(t).reshape(-1, K),
+                                  None if labels is None else labels.reshape(-1), temperature, alpha,
+                                  ignore_index)
         loss = reduced(rows, kept, reduction).float()
-        return loss.reshape(logits.shape[:-1] if reduction == "none" else ()), None
-
-    @torch.enable_grad()
-    def distill_grad(self, logits, ids, t, labels, *, temperature, alpha, ignore_index, reduction,
-                     upstream, unit=None):
-        z = f64(logits).requires_grad_()
-        rows, kept = self._rows(z, ids, t, labels, temperature, alpha, ignore_index)
-        loss = reduced(rows, kept, reduction)
-        return torch.autograd.grad(loss, z, f64(upstream).reshape(loss.shape))[0].to(logits.dtype)
+        return loss.reshape(logits.shape[:-1] if reduction == "none" else ())
 
 
 def plan(heads, table, positions=None, norm=True, eps=1e-6, interleaved=False):

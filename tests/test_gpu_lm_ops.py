@@ -368,7 +368,8 @@ def test_qk_dots(gpu, dtype, B, n_val, T, heads, D, n_rot, val_start):
     plan = L.plan(heads, gs.rotary_table(T, n_rot, device=gpu))
     x, qw, kw, grads = qk_inputs(gpu, B, T, heads, D, dtype, 71)
     x = x.detach()
-    got = _native.ops().qk_norm_rotary_dots(plan, (x,), qw.detach(), kw.detach(), grads, n_val,
+    got = _native.ops().qk_norm_rotary_dots(x, None, heads, plan["table"], None, qw.detach(),
+                                            kw.detach(), 1e-6, False, grads, n_val,
                                             val_start=val_start, grad_scale=0.25)
     _, dq, dk = L.qk_grads(plan, (x,), qw, kw, grads, per_sample=True)
     xs = L.split_heads(plan, (f64(x),))
@@ -797,3 +798,61 @@ def test_engine_step_of_a_model_with_all_three(gpu, rotary):
     eng.aggregate_and_log()
     assert eng.dot_product_log[-1]["dot_product"].isfinite().all()
     eng.detach()
+
+
+def test_gradients_are_not_differentiable_again(gpu):
+    w = randn((9, 8), 1).to(gpu).requires_grad_()
+    ids = torch.tensor([1, 2, 2], device=gpu)
+    table = gs.rotary_table(4, 8, device=gpu)
+    x = randn((1, 2, 32), 2).to(gpu).requires_grad_()
+    z, t_ids, t, y = (v.to(gpu) for v in distill_inputs(3, 11, 2, 3, FP32))
+    z.requires_grad_()
+    outs = [(gs.embedding_lookup(ids, w, 2.0), w), (gs.qkv_norm_rotary(x, 2, 1, table)[0], x),
+            (gs.distillation_loss(z, t_ids, t, y, alpha=0.5), z)]
+    for out, inp in outs:
+        want, = torch.autograd.grad(out.sum(), inp, retain_graph=True)
+        got, = torch.autograd.grad(out.sum(), inp, create_graph=True)   # allowed: once
+        assert torch.equal(got, want)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            got.sum().backward()
+
+
+def test_saved_tensors_that_moved(gpu):
+    """What autograd saved may come back elsewhere (offloaded to host memory meanwhile): an odd
+    offset of the logits is gone then, and the gradient is formed again for the new place."""
+    step, *_ = _three(gpu, 6)
+    with torch.autograd.graph.save_on_cpu():
+        got = step()
+    for a, b in zip(got, step()):
+        assert torch.equal(a, b)
+    z, t_ids, t, y = (v.to(gpu) for v in distill_inputs(5, 103, 4, 3, BF16))
+    odd = torch.empty(5 * 103 + 1, dtype=BF16, device=gpu)[1:].view(5, 103)
+    odd.copy_(z)
+    odd.requires_grad_()
+    want, = torch.autograd.grad(gs.distillation_loss(odd, t_ids, t, y, alpha=0.5), odd)
+    with torch.autograd.graph.save_on_cpu():
+        loss = gs.distillation_loss(odd, t_ids, t, y, alpha=0.5)
+    got, = torch.autograd.grad(loss, odd)
+    # another split of the row into pieces: another order of its sums, one rounding step of bf16
+    assert ((f64(got) - f64(want)).abs() <= f64(want).abs() * 2 * HALF[BF16] + 1e-9).all()
+
+
+def test_only_what_is_asked_for(gpu):
+    """Gradients of some inputs alone, inputs that need none, and what a loss does not reach."""
+    table = gs.rotary_table(8, 16, device=gpu)
+    x, qw, kw, grads = qk_inputs(gpu, 2, 6, (3, 1, 1), 32, FP32, 91)
+    y = gs.qkv_norm_rotary(x, 3, 1, table, None, qw, kw)
+    dx, dq, dk = torch.autograd.grad(y, (x, qw, kw), grads, retain_graph=True)
+    for inputs, want in (((x,), (dx,)), ((qw,), (dq,)), ((kw,), (dk,)), ((qw, kw), (dq, dk))):
+        got = torch.autograd.grad(y, inputs, grads, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    frozen = gs.qkv_norm_rotary(x, 3, 1, table, None, qw.detach(), kw.detach())
+    assert torch.equal(torch.autograd.grad(frozen, x, grads)[0], dx)
+    weights = gs.qkv_norm_rotary(x.detach(), 3, 1, table, None, qw, kw)
+    assert torch.equal(torch.autograd.grad(weights, qw, grads)[0], dq)
+    q = x.detach()[..., :96].unflatten(-1, (3, 32)).clone().requires_grad_()
+    k = x.detach()[..., 96:128].unflatten(-1, (1, 32)).clone().requires_grad_()
+    rq, rk = gs.qk_norm_rotary(q, k, table, None, qw, kw)
+    got, = torch.autograd.grad(rk, k, grads[1], retain_graph=True)
+    assert torch.equal(got.flatten(2), dx[..., 96:128])
+    assert torch.autograd.grad(rk, q, grads[1], allow_unused=True)[0].eq(0).all()

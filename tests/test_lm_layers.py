@@ -31,7 +31,8 @@ def test_cpu_tensors_are_rejected_loudly():
     with pytest.raises(_native.GhostHipError, match="ROCm GPU"):
         ops.embedding_lookup(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8), 1.0)
     with pytest.raises(_native.GhostHipError, match="ROCm GPU"):
-        ops.qk_norm_rotary(L.plan((1, 1, 1), table), (torch.zeros(1, 2, 12),), None, None)
+        ops.qk_norm_rotary(torch.zeros(1, 2, 12), None, (1, 1, 1), table, None, None, None, True,
+                           1e-6, False)
     with pytest.raises(_native.GhostHipError, match="ROCm GPU"):
         gs.distillation_loss(torch.zeros(2, 5), torch.zeros(2, 1, dtype=torch.int64),
                              torch.zeros(2, 1))
@@ -57,11 +58,31 @@ def test_python_refusals_before_any_device():
         gs.QKNormRotary(1, 1, 8, n_rot=10)
 
 
+class _QKShape(ctypes.Structure):   # gs_qk_shape
+    _fields_ = [("dtype", ctypes.c_int), ("B", ctypes.c_int64), ("T", ctypes.c_int64),
+                ("D", ctypes.c_int64), ("n_rot", ctypes.c_int64), ("heads", ctypes.c_int32 * 3),
+                ("norm", ctypes.c_int), ("interleaved", ctypes.c_int), ("eps", ctypes.c_float),
+                ("weight", ctypes.c_void_p * 2), ("weight_dtype", ctypes.c_int * 2),
+                ("table", ctypes.c_void_p), ("n_positions", ctypes.c_int64),
+                ("positions", ctypes.c_void_p), ("position_bits", ctypes.c_int),
+                ("position_stride_b", ctypes.c_int64), ("position_stride_t", ctypes.c_int64)]
+
+
+class _Distill(ctypes.Structure):   # gs_distill
+    _fields_ = [("Z", ctypes.c_void_p), ("dtype", ctypes.c_int), ("N", ctypes.c_int64),
+                ("V", ctypes.c_int64), ("inner", ctypes.c_int64), ("stride_outer", ctypes.c_int64),
+                ("stride_inner", ctypes.c_int64), ("teacher_ids", ctypes.c_void_p),
+                ("teacher", ctypes.c_void_p), ("teacher_dtype", ctypes.c_int), ("K", ctypes.c_int64),
+                ("labels", ctypes.c_void_p), ("ignore_index", ctypes.c_int64),
+                ("temperature", ctypes.c_float), ("alpha", ctypes.c_float),
+                ("reduction", ctypes.c_int)]
+
+
 P16 = 1 << 20   # an address that is never followed: the checks come first
 
 
 def _qk_shape(**changes):
-    s = _native._QKShape()
+    s = _QKShape()
     s.dtype, s.B, s.T, s.D, s.n_rot, s.norm, s.eps = 0, 2, 3, 64, 64, 1, 1e-6
     s.heads[:] = (2, 1, 1)
     s.table, s.n_positions = P16, 16
@@ -75,7 +96,7 @@ def _qk_shape(**changes):
 
 
 def _qk_rows(n=3):
-    return _native._QKRows3(*(n * [P16, 1024, 256, 64] + (3 - n) * [0, 0, 0, 0]))
+    return (ctypes.c_int64 * 12)(*(n * [P16, 1024, 256, 64] + (3 - n) * [0, 0, 0, 0]))
 
 
 @pytest.mark.parametrize("changes,status", [
@@ -125,7 +146,7 @@ def test_qk_pointers_and_workspaces_are_checked_on_the_host():
 
 
 def _distill(**changes):
-    d = _native._Distill()
+    d = _Distill()
     d.Z, d.dtype, d.N, d.V, d.inner, d.stride_outer, d.stride_inner = P16, 0, 6, 100, 6, 0, 100
     d.teacher_ids = d.teacher = d.labels = P16
     d.teacher_dtype, d.K, d.ignore_index = 0, 4, -100
