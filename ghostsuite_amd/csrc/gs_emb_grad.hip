@@ -576,25 +576,25 @@ struct EgVec {
   };
 };
 
-// Loads the VE elements at f0 of a row (zeros past d); whole 16 bytes when `full`.
+// Loads the VE elements at f0, f0 + step, ... of a row (zeros past d); whole 16 bytes when `full`.
 template <class E>
 __device__ __forceinline__ uint4 eg_load(const E* __restrict__ row, int64_t f0, int64_t d,
-                                         bool full) {
+                                         bool full, int step = 1) {
   typename EgVec<E>::U x;
   if (full) {
     x.u = *reinterpret_cast<const uint4*>(row + f0);
   } else {
 #pragma unroll
-    for (int i = 0; i < EgVec<E>::VE; ++i) x.e[i] = f0 + i < d ? row[f0 + i] : E(0);
+    for (int i = 0; i < EgVec<E>::VE; ++i) x.e[i] = f0 + i * step < d ? row[f0 + i * step] : E(0);
   }
   return x.u;
 }
 
-// Writes scale * acc (+ the old row when accumulating) at f0 of an output row.
+// Writes scale * acc (+ the old row when accumulating) at f0, f0 + step, ... of an output row.
 template <class GE, int VE>
 __device__ __forceinline__ void eg_store(GE* __restrict__ out, int64_t f0, int64_t d,
                                          const float (&acc)[VE], float scale, int accumulate,
-                                         bool full) {
+                                         bool full, int step = 1) {
   constexpr int NV = VE * static_cast<int>(sizeof(GE)) / 16;  // whole 16-byte vectors
   if (NV > 0 && full) {
     union { uint4 u[NV > 0 ? NV : 1]; GE e[VE]; } o;
@@ -613,16 +613,19 @@ __device__ __forceinline__ void eg_store(GE* __restrict__ out, int64_t f0, int64
   } else {
 #pragma unroll
     for (int i = 0; i < VE; ++i) {
-      if (f0 + i >= d) break;
+      const int64_t f = f0 + i * step;
+      if (f >= d) break;
       float x = scale * acc[i];
-      if (accumulate) x += to_f32<GE>(out[f0 + i]);
-      out[f0 + i] = from_f32<GE>(x);
+      if (accumulate) x += to_f32<GE>(out[f]);
+      out[f] = from_f32<GE>(x);
     }
   }
 }
 
 // Waves [0, windows): window w = list places [w EG_WIN, (w + 1) EG_WIN).  Lanes own 16-byte
-// chunks of the feature row (several passes when d > 64 VE); per pass a lane loads its chunk
+// chunks of the feature row, or where rows are not whole numbers of those every 64th element, so that
+// a wave's accesses stay contiguous (24432 tokens, 515 fp32 features, 30011 ids: the windows 34 to 17 us)
+// (several passes when d > 64 VE); per pass a lane loads its chunk
 // of every row of the window (all in flight), then walks the window's runs in place order,
 // summing in fp32.  A run wholly inside the window writes its row; the run holding the
 // window's first place, when it began in an earlier window, goes to part[w][0], and the run
@@ -640,6 +643,8 @@ __device__ __forceinline__ void eg_window(const E* __restrict__ G, const EgList&
   const EgOrder order = list.order;
   const int64_t windows = list.windows;
   const int lane = threadIdx.x & 63;
+  const int step = vec ? 1 : 64;
+  const int64_t first = vec ? static_cast<int64_t>(lane) * VE : lane;   // the lane's first feature
   const int64_t w = block * (EG_THREADS / 64) + (threadIdx.x >> 6);
   if (w >= windows) {
     // absent rows, overwrite mode only (the last workgroup's surplus waves land here in
@@ -651,11 +656,11 @@ __device__ __forceinline__ void eg_window(const E* __restrict__ G, const EgList&
     for (int r = 0; r < 16 && v0 + r < vocab; ++r) {
       if ((bits >> r) & 1u) continue;
       GE* out = grad + (v0 + r) * d;
-      for (int64_t f0 = static_cast<int64_t>(lane) * VE; f0 < d; f0 += 64 * VE) {
+      for (int64_t f0 = first; f0 < d; f0 += 64 * VE) {
         float z[VE];
 #pragma unroll
         for (int i = 0; i < VE; ++i) z[i] = 0.f;
-        eg_store<GE, VE>(out, f0, d, z, 0.f, 0, vec && f0 + VE <= d);
+        eg_store<GE, VE>(out, f0, d, z, 0.f, 0, vec && f0 + VE <= d, step);
       }
     }
     return;
@@ -673,7 +678,7 @@ __device__ __forceinline__ void eg_window(const E* __restrict__ G, const EgList&
   // two feature passes per round (lanes own chunks f0 and f0 + 64 VE); the window's rows in
   // batches, each batch's loads of both passes issued together, the sums carried across
   // batches
-  for (int64_t fb = static_cast<int64_t>(lane) * VE; fb < d; fb += 128 * VE) {
+  for (int64_t fb = first; fb < d; fb += 128 * VE) {
     float acc[2][VE];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -691,7 +696,7 @@ __device__ __forceinline__ void eg_window(const E* __restrict__ G, const EgList&
 #pragma unroll
         for (int i = 0; i < EG_BATCH; ++i)
           x[h][i] = b0 + i < n && f0 < d
-                        ? eg_load<E>(G + readlane_i64(my_row, b0 + i) * d, f0, d, full)
+                        ? eg_load<E>(G + readlane_i64(my_row, b0 + i) * d, f0, d, full, step)
                         : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
@@ -721,10 +726,10 @@ __device__ __forceinline__ void eg_window(const E* __restrict__ G, const EgList&
                 if (pp != nullptr) {
 #pragma unroll
                   for (int e = 0; e < VE; ++e)
-                    if (f0 + e < d) pp[f0 + e] = acc[h][e];
+                    if (f0 + e * step < d) pp[f0 + e * step] = acc[h][e];
                 } else {
                   eg_store<GE, VE>(grad + order.id(id_p) * d, f0, d, acc[h], scale, accumulate,
-                                   vec && f0 + VE <= d);
+                                   vec && f0 + VE <= d, step);
                 }
               }
 #pragma unroll
