@@ -8,10 +8,13 @@
 // A workgroup owns a row.  The row is read once, in 16-byte pieces that stay in registers as they
 // came: the maximum, then both sums of exponentials, then the gradient are formed from them, so a
 // training step's loss and gradient cost one read and one write of the logits, and the rate of a
-// copy bounds them.  Rows too long for the registers are read again in the second sweep (running
-// maximum and sums in the first).  The gradient is written for the whole row as if no entry stood
-// there; after a barrier the K entries and the label are written again with their masses taken off,
-// from the logits themselves, so each element is rounded once.
+// copy bounds them (8192 rows of 50257 bf16: 390 us, 4.2 of a copy's 4.7 TB/s; with two softmaxes the
+// exponentials, four to an element, come close behind).  Rows too long for the registers are read
+// again in a second sweep, out of the caches (running maximum and sums in the first).  The gradient is
+// written for the whole row as if no entry stood there; the elements of the K entries and the label are
+// then written again with their masses taken off, by the threads that wrote them, from the logits
+// themselves, so that each element is rounded once.  An id that stands several times gets its masses
+// added up in the entries' order.
 //
 // Sums, maxima and exponentials are fp32; a thread adds its own pieces, a wave its threads and the
 // workgroup its waves, in a fixed order (the same bits on every run).
@@ -119,12 +122,15 @@ struct DsEntries {
 };
 __host__ __device__ inline int ds_entries(int K) { return (K + 1 + 3) & ~3; }   // whole int4s
 
-// NP: pieces a thread keeps (0: none are kept, the row is read twice).  TWO: the two softmaxes
-// differ and both count.  WPE: waves on a SIMD the registers are held to.
+// NP: pieces a thread keeps; below zero none are kept, the row is read twice with -NP pieces of a thread
+// on their way at once.  TWO: the two softmaxes differ and both count.  WPE: waves on a SIMD the
+// registers are held to.
 template <class E, int THREADS, int NP, bool TWO, int WPE>
 __global__ void __launch_bounds__(THREADS, WPE) distill_kernel(DsArgs a) {
   constexpr int VE = 16 / sizeof(E);
   constexpr int WAVES = THREADS / 64;
+  constexpr bool KEEP = NP > 0;
+  constexpr uint32_t AHEAD = KEEP ? 1 : -NP;
   __shared__ float red[3][WAVES][4];
   extern __shared__ int4 dyn[];
   const DsEntries ent(dyn, ds_entries(a.K));
@@ -150,7 +156,7 @@ __global__ void __launch_bounds__(THREADS, WPE) distill_kernel(DsArgs a) {
     const uint32_t head = min(V, static_cast<uint32_t>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) /
                                      static_cast<uint32_t>(sizeof(E)));
     const uint32_t pieces = (V - head) / VE, tail0 = head + pieces * VE;
-    const uint32_t S = NP > 0 ? (pieces + NP - 1) / (NP > 0 ? NP : 1) : THREADS;
+    const uint32_t S = KEEP ? (pieces + NP - 1) / (KEEP ? NP : 1) : THREADS;
     const int single = tid < head ? static_cast<int>(tid)
                        : tid >= 64 && tid - 64 < V - tail0 ? static_cast<int>(tail0 + tid - 64) : -1;
     const uint4* zp = reinterpret_cast<const uint4*>(z + head);
@@ -176,9 +182,9 @@ __global__ void __launch_bounds__(THREADS, WPE) distill_kernel(DsArgs a) {
     const float xs = single >= 0 ? to_f32<E>(z[single]) : NEG_INF;
     // A thread past S holds copies of another's pieces, and one whose last piece (only the last:
     // S >= NP) is past the row's end a copy of the row's: neither is added nor stored.
-    const bool mine = NP == 0 || tid < S, last = NP == 0 || tid + (NP - 1) * S < pieces;
-    uint4 x[NP > 0 ? NP : 1];
-    if constexpr (NP > 0) {
+    const bool mine = !KEEP || tid < S, last = !KEEP || tid + (NP - 1) * S < pieces;
+    uint4 x[KEEP ? NP : 1];
+    if constexpr (KEEP) {
       uint32_t p = min(tid, S - 1);
 #pragma unroll
       for (int k = 0; k < NP; ++k, p += S) x[k] = ds_piece(zp, k < NP - 1 ? p : min(p, pieces - 1));
@@ -195,7 +201,7 @@ __global__ void __launch_bounds__(THREADS, WPE) distill_kernel(DsArgs a) {
     if (tid < K) take(tid, id0, t0);
     for (uint32_t k = tid + THREADS; k < K; k += THREADS) take(k, entry_id(k), entry_t(k));
     float m = xs, sq = 0.f, s1 = 0.f;
-    if constexpr (NP > 0) {
+    if constexpr (KEEP) {
 #pragma unroll
       for (int k = 0; k < NP; ++k) {
 #pragma unroll
@@ -206,20 +212,32 @@ __global__ void __launch_bounds__(THREADS, WPE) distill_kernel(DsArgs a) {
       // running maximum and sums of this thread
       sq = xs == NEG_INF ? 0.f : 1.f;
       s1 = sq;
-      for (uint32_t p = tid; p < pieces; p += THREADS) {
-        const uint4 v = zp[p];
-        float pm = m;
+      for (uint32_t p = tid; p < pieces; p += AHEAD * THREADS) {
+        uint4 v[AHEAD];
 #pragma unroll
-        for (int e = 0; e < VE; ++e) pm = fmaxf(pm, ds_elem<E>(v, e));
-        if (pm == NEG_INF) pm = 0.f;   // nothing yet (a NaN among them is seen by the sums)
-        const float d = m == NEG_INF ? 0.f : m - pm;
+        for (uint32_t q = 0; q < AHEAD; ++q) v[q] = zp[min(p + q * THREADS, pieces - 1)];
+        float pm = m;   // (a piece past the end is a copy of the last)
+#pragma unroll
+        for (uint32_t q = 0; q < AHEAD; ++q)
+#pragma unroll
+          for (int e = 0; e < VE; ++e) pm = fmaxf(pm, ds_elem<E>(v[q], e));
+        // no maximum yet: any reference will do (a NaN among them is seen by the sums)
+        const float ref = pm == NEG_INF ? 0.f : pm, d = m == NEG_INF ? 0.f : m - ref;
         sq *= ds_exp(d, kq);
         if (TWO) s1 *= ds_exp(d, DS_LOG2E);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          const float w = ds_elem<E>(v, e) - pm;
-          sq += ds_exp(w, kq);
-          if (TWO) s1 += ds_exp(w, DS_LOG2E);
+        for (uint32_t q = 0; q < AHEAD; ++q) {
+          float pq = 0.f, p1 = 0.f;
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            const float w = ds_elem<E>(v[q], e) - ref;
+            pq += ds_exp(w, kq);
+            if (TWO) p1 += ds_exp(w, DS_LOG2E);
+          }
+          if (p + q * THREADS < pieces) {
+            sq += pq;
+            s1 += p1;
+          }
         }
         m = pm;
       }
@@ -239,7 +257,7 @@ __global__ void __launch_bounds__(THREADS, WPE) distill_kernel(DsArgs a) {
     }
 
     // ---- sums of exponentials
-    if constexpr (NP > 0) {
+    if constexpr (KEEP) {
 #pragma unroll
       for (int k = 0; k < NP; ++k) {
         float pq = 0.f, p1 = 0.f;
@@ -340,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, WPE) distill_kernel(DsArgs a) {
       const float g = cq * ds_exp(d, kq);
       return TWO ? g + c1 * ds_exp(d, DS_LOG2E) : g;
     };
-    if constexpr (NP > 0) {
+    if constexpr (KEEP) {
       uint32_t p = ds_fresh(tid);
       if (mine) {
 #pragma unroll
@@ -352,7 +370,14 @@ __global__ void __launch_bounds__(THREADS, WPE) distill_kernel(DsArgs a) {
         }
       }
     } else {
-      for (uint32_t p = tid; p < pieces; p += THREADS) dzp[p] = ds_map<E>(zp[p], value);
+      for (uint32_t p = tid; p < pieces; p += AHEAD * THREADS) {
+        uint4 v[AHEAD];
+#pragma unroll
+        for (uint32_t q = 0; q < AHEAD; ++q) v[q] = zp[min(p + q * THREADS, pieces - 1)];
+#pragma unroll
+        for (uint32_t q = 0; q < AHEAD; ++q)
+          if (p + q * THREADS < pieces) dzp[p + q * THREADS] = ds_map<E>(v[q], value);
+      }
     }
     if (single >= 0) dz[single] = from_f32<E>(value(xs));
     // while the stores drain: the masses of every id, added in the entries' order by each of them
@@ -428,12 +453,17 @@ void ds_launch(const DsArgs& a, bool two, int64_t grid, hipStream_t s) {
                        dim3(THREADS), lds, s, a);
 }
 
-// The fewest threads that can hold the row, and then the fewest pieces a thread (all NP of them are
-// gone through, so a row should fill them); fewer threads with more pieces leave more rows on a CU at
-// different stages, and reading, exponentials and writing overlap between them.  Measured on MI355X
-// (loss and gradient): 8192 rows of 50257 bf16, two softmaxes, 256 threads of 26 pieces 404 us, 512 of
-// 13 441, 1024 of 7 677; 2031 rows of 32003 fp32, 512 of 16 140 us, of 26 222, 1024 of 8 195.
-// Registers: 4 NP and about 45 more.  Rows of a few pieces, or of more than 16384, are read twice.
+// Rows of up to 6656 pieces are kept by 256 threads, of up to 9216 by 512 (the fewest pieces a thread:
+// all NP are gone through, so a row should fill them); others, and rows of a few pieces, are read
+// twice, the second time from the caches: few rows are worked on at once.  Few threads with many
+// pieces leave several rows on a CU at different stages, where reading, exponentials and writing
+// overlap.  Registers: 4 NP and about 45 more.  Measured on MI355X (loss and gradient of 4e8 bf16 / 4e8
+// fp32 logits, K = 64, two softmaxes, us), by vocabulary:
+//     50257: kept by 256 threads 408 / -, by 512 441 / 821, read twice by 512 475 / 772
+//     32003: kept by 256 418 / -, by 512 - / 703, read twice 546 / 785
+//     65000: kept by 512 (18, 32 pieces) 444 / 773, read twice 425 / 807
+//    128256: kept by 512 (32) 511 / -, read twice by 512 415 / 938, by 1024 456 / 822
+//    262144: read twice by 512 448 / 924, by 1024 446 / 866
 template <class E>
 int ds_run(const DsArgs& a, bool two, int64_t grid, hipStream_t s) {
   constexpr int VE = 16 / sizeof(E);
@@ -449,13 +479,13 @@ int ds_run(const DsArgs& a, bool two, int64_t grid, hipStream_t s) {
   GS_DS_TRY(256, 18, 4)
   GS_DS_TRY(256, 26, 3)
   GS_DS_TRY(512, 18, 4)
-  GS_DS_TRY(512, 26, 2)
-  GS_DS_TRY(512, 32, 2)
 #undef GS_DS_TRY
-  if (a.V < 4096)
-    ds_launch<E, 256, 0, 4>(a, two, grid, s);
+  if (most < 512)
+    ds_launch<E, 256, -4, 4>(a, two, grid, s);
+  else if (most <= 20480)
+    ds_launch<E, 512, -8, 4>(a, two, grid, s);
   else
-    ds_launch<E, 1024, 0, 4>(a, two, grid, s);
+    ds_launch<E, 1024, -4, 4>(a, two, grid, s);
   return check_launch("distill_kernel");
 }
 
@@ -469,7 +499,7 @@ int ds_args(DsArgs& a, const char* name, const gs_distill* d) {
       d->V <= 0 || d->K <= 0 || d->inner <= 0 || d->inner > d->N || d->N % d->inner != 0 ||
       (d->N > 1 && (d->stride_inner < d->V && d->inner > 1)) ||
       (d->N > d->inner && d->stride_outer < d->V) || !(d->temperature > 0.f) ||
-      !std::isfinite(d->temperature) || !(d->alpha >= 0.f && d->alpha <= 1.f) ||
+      !std::isfinite(d->temperature * d->temperature) || !std::isfinite(1.f / d->temperature) || !(d->alpha >= 0.f && d->alpha <= 1.f) ||
       (d->labels == nullptr && d->alpha != 1.f) || d->reduction < GS_REDUCE_NONE ||
       d->reduction > GS_REDUCE_MEAN ||
       reinterpret_cast<uintptr_t>(d->Z) % elem_size(d->dtype) != 0)

@@ -554,11 +554,11 @@ int ceil_log2(int64_t x) {
 // How the work is shared out: into about QK_WAVES waves (3 for each SIMD, what the backward kernel's
 // registers let stay there at once) while the work lasts, by head groups first and longer token spans
 // after.  Fewer, longer walks reuse the angles and add more into a lane before the workgroup's sum.
-// Per-sample sums cut the spans at samples.  Measured on MI355X, 20 x 1024 tokens of 12 + 12 + 12 heads
-// of 64, bf16 (forward / backward, us): 32768 waves 56 / 95, 16384 46 / 77, 8192 39 / 64, 4096 34 / 57,
-// 3072 34 / 56, 2048 34 / 56; 8 x 2048 of 8 + 8 + 8 of 256: 110 / 169, 106 / 149, 98 / 133, 98 / 138,
-// 95 / 135, 103 / 137.
-constexpr int64_t QK_WAVES = 3072;
+// Per-sample sums cut the spans at samples.  Measured on MI355X with 32, 16, 8, 4, 3 and 2 waves for
+// each SIMD (forward / backward, us): 20 x 1024 tokens of 12 + 12 + 12 heads of 64, bf16, 56 / 95,
+// 46 / 77, 39 / 64, 34 / 57, 34 / 56, 34 / 56; 8 x 2048 of 8 + 8 + 8 of 256, 110 / 169, 106 / 149,
+// 98 / 133, 98 / 138, 95 / 135, 103 / 137.
+constexpr int64_t QK_WAVES = 3 * 4 * 256;
 void qk_share(QkArgs& a, int upl, int units, bool per_sample) {
   a.lanes_log2 = std::min(6, ceil_log2((units + upl - 1) / upl));
   const int64_t slots = QK_THREADS >> a.lanes_log2;

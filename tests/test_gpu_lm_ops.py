@@ -512,11 +512,11 @@ def test_distill_per_row_upstream_and_other_ignore_index(gpu):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
-@pytest.mark.parametrize("V", [301, 9000])
+@pytest.mark.parametrize("V", [41, 301, 9000, 83001])
 def test_distill_rows_with_little_or_nothing_left(gpu, dtype, V):
     """Teacher entries masked by id or by -inf, ids that stand several times (the label's among
     them), masked student logits, the lowest finite values, and NaN where nothing reads."""
-    z, ids, t, labels = distill_inputs(14, V, 8, 7, dtype)
+    z, ids, t, labels = distill_inputs(15, V, 8, 7, dtype)
     ids[0] = -1                                   # no teacher, by id
     t[1] = -math.inf                              # no teacher, by logit
     t[2] = torch.finfo(dtype).min                 # all at the lowest value: even shares
@@ -536,6 +536,9 @@ def test_distill_rows_with_little_or_nothing_left(gpu, dtype, V):
     z[11] = torch.finfo(dtype).min                # a flat row
     t[12, 1:] = torch.finfo(dtype).min            # one entry takes all
     ids[13, 1] = 2 ** 40                          # far outside
+    z[14] -= 400                                  # far below zero, masked from the first id on
+    z[14, :V // 2] = -math.inf
+    ids[14], labels[14] = torch.arange(V - 8, V), V - 1
     for tau, alpha in ((2.0, 0.5), (1.0, 1.0), (1.0, 0.5), (3.0, 0.0)):
         check_distill(gpu, z, ids, t, labels, tau, alpha)
         check_distill(gpu, z, ids, t, labels, tau, alpha, "none", 0.5)
@@ -556,6 +559,11 @@ def test_distill_infinities_where_they_count(gpu):
     assert loss[0] == math.inf and loss[1:4].isnan().all() and loss[4].isfinite()
     g, = torch.autograd.grad(loss, zg, torch.ones_like(loss))
     assert g[0].isfinite().all() and g[1:4].isnan().all() and g[4].isfinite().all()
+    t[4, 1] = math.nan                            # a teacher entry that counts
+    loss = gs.distillation_loss(zg, ids.to(gpu), t.to(gpu), labels.to(gpu), temperature=2.0,
+                                alpha=0.5, reduction="none")
+    g, = torch.autograd.grad(loss, zg, torch.ones_like(loss))
+    assert loss[4].isnan() and g[4].isnan().all() and loss[0] == math.inf
     none = torch.full_like(labels, -100).to(gpu)
     loss = gs.distillation_loss(zg, ids.to(gpu), t.to(gpu), none)
     assert loss.isnan() and (torch.autograd.grad(loss, zg)[0] == 0).all()

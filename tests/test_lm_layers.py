@@ -161,7 +161,8 @@ def _distill(**changes):
     (dict(teacher_ids=None), -1), (dict(teacher=None), -1), (dict(N=0), -1), (dict(V=0), -1),
     (dict(K=0), -1), (dict(inner=4), -1), (dict(inner=0), -1), (dict(stride_inner=99), -1),
     (dict(inner=3, stride_outer=99), -1), (dict(temperature=0.0), -1),
-    (dict(temperature=math.inf), -1), (dict(temperature=math.nan), -1), (dict(alpha=-0.1), -1),
+    (dict(temperature=math.inf), -1), (dict(temperature=math.nan), -1),
+    (dict(temperature=1e-39), -1), (dict(temperature=1e30), -1), (dict(alpha=-0.1), -1),
     (dict(alpha=1.1), -1), (dict(alpha=math.nan), -1), (dict(labels=None), -1),
     (dict(reduction=3), -1), (dict(Z=P16 + 1), -1), (dict(K=1025), -5), (dict(N=1 << 31,
                                                                              inner=1 << 31), -5)])
