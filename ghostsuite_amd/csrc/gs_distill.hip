@@ -308,7 +308,8 @@ __global__ void __launch_bounds__(THREADS, WPE) distill_kernel(DsArgs a) {
     // ---- the entries' part: the loss, and each id's mass in the gradient
     float w = a.upstream != nullptr ? a.upstream[a.per_row ? n : 0] : 1.f;
     if (a.mean) w /= a.count != nullptr ? a.count[0] : static_cast<float>(a.N);
-    const float wq = teacher ? w * a.alpha * a.tau : 0.f, w1 = w * (1.f - a.alpha);
+    const float nan_or_one = ts != ts ? ts : 1.f;   // a NaN entry leaves no element of the row as if valid
+    const float wq = teacher ? w * a.alpha * a.tau * nan_or_one : 0.f, w1 = w * (1.f - a.alpha);
     const bool hard = a.alpha != 1.f, in = y >= 0 && y < V;
     float kl = 0.f;
     {

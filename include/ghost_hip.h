@@ -451,7 +451,8 @@ int gs_qk_rotary_dots(const gs_qk_shape* shape, const gs_qk_rows x[3], const gs_
  *   loss = alpha temperature^2 sum_k p_k (log p_k - log q[id_k]) + (1 - alpha) (-log s_y)
  * A row without such an entry has no first term; a repeated id counts as often as it stands.
  * labels NULL: alpha must be 1.  Rows whose label is ignore_index have loss 0 and gradient 0; another
- * label outside [0, V) makes the row's loss and gradient NaN (alpha < 1).
+ * label outside [0, V) makes the row's loss and gradient NaN (alpha < 1), as does a NaN logit, the
+ * teacher's among the entries that count.
  * reduction: GS_REDUCE_NONE (out_loss: [N]), GS_REDUCE_SUM, or GS_REDUCE_MEAN over the rows not
  * ignored (NaN when there are none, as 0 / 0).
  * Rows: n = (o, i), i < inner, at Z + (o stride_outer + i stride_inner) elements, V contiguous.
