@@ -105,8 +105,11 @@ _SIGNATURES = {
     "gs_ordered_sum": (_I, [_P, _P, _I, _I64, _P, _I, _P]),
     "gs_embedding_lookup": (_I, [_P, _I, _I64, _P, _I, _I64, _I64, _F, _I64, _P, _P, _P]),
     "gs_qk_rotary": (_I, [_P, _P, _P, _P]),
-    "gs_qk_rotary_grad_workspace": (_SZ, [_P]),
-    "gs_qk_rotary_grad": (_I, [_P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "gs_qk_rotary_grad_workspace": (_SZ, [_P, _I]),
+    "gs_qk_rotary_grad": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "gs_qk_sample_dots_workspace": (_SZ, [_I64]),
+    "gs_qk_sample_dots": (_I, [_P, _I64, _I64, _I64, _I64, _P, _P, _P, _I, _P, _I, _F, _P, _SZ,
+                               _P]),
     "gs_qk_rotary_dots_workspace": (_SZ, [_P]),
     "gs_qk_rotary_dots": (_I, [_P, _P, _P, _I64, _I64, _P, _P, _P, _P, _F, _P, _SZ, _P]),
     "gs_distill_workspace": (_SZ, [_P]),
@@ -792,10 +795,19 @@ class HipOps:
         return _lm().embedding_lookup(ids, weight, scale, padding_idx)
 
     def qk_norm_rotary(self, q: torch.Tensor, k: Optional[torch.Tensor], heads, table, positions, qw,
-                       kw, norm: bool, eps: float, interleaved: bool):
+                       kw, norm: bool, eps: float, interleaved: bool,
+                       sample_grads: Optional[torch.Tensor] = None):
         """[queries, keys] of q and k, or with k None [queries, keys, values] of a packed q, heads
-        first (gs_qk_rotary, gs_qk_rotary_grad); heads: of each of the three parts."""
-        return _lm().qk_norm_rotary(q, k, heads, table, positions, qw, kw, norm, eps, interleaved)
+        first (gs_qk_rotary, gs_qk_rotary_grad); heads: of each of the three parts.  sample_grads
+        ([2, B, D] fp32): the backward pass writes each sample's gradients of qw and kw there."""
+        return _lm().qk_norm_rotary(q, k, heads, table, positions, qw, kw, norm, eps, interleaved,
+                                    sample_grads)
+
+    def qk_sample_dots(self, sample_grads: torch.Tensor, qw, kw, n_val: int, *,
+                       val_start: Optional[int] = None, grad_scale: Optional[float] = None):
+        """[dot_q, dot_k, grad_q, grad_k] from qk_norm_rotary's sample_grads: gs_qk_sample_dots; the
+        train gradients, of qw's and kw's dtypes, None without grad_scale."""
+        return _lm().qk_sample_dots(sample_grads, qw, kw, n_val, val_start, grad_scale)
 
     def qk_norm_rotary_dots(self, q: torch.Tensor, k: Optional[torch.Tensor], heads, table,
                             positions, qw, kw, eps: float, interleaved: bool, grads, n_val: int, *,

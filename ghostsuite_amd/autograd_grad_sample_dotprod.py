@@ -108,7 +108,7 @@ def _prepare_sample_grad_or_dotprod(layer: nn.Module, grad_output: Tuple[torch.T
     if isinstance(layer, QKNormRotary):   # three outputs, any of which may have no gradient
         d["_gs_grad_outputs"] = others = tuple(None if g is None else g.detach()
                                                for g in grad_output)
-        others += (d.get("_gs_positions"),)
+        others += (d.get("_gs_positions"), d.get("_gs_sample_grads"))
         backprops = next(g for g in others if g is not None)
     else:
         backprops = grad_output[0].detach()
@@ -171,7 +171,8 @@ def _apply_train_grad(layer: nn.Module, val_batch_size: int, loss_reduction: str
     finally:
         for attr in ('activations', 'backprops', 'backprops_scale', '_gs_bias_train_grad',
                      '_gs_weight_train_grad', '_gs_ln_train_grads', '_gs_bias_grad_scale',
-                     '_gs_ln_grad_scale', '_gs_grad_outputs', '_gs_positions'):
+                     '_gs_ln_grad_scale', '_gs_grad_outputs', '_gs_positions',
+                     '_gs_sample_grads'):
             layer.__dict__.pop(attr, None)
 
 
@@ -192,6 +193,8 @@ _INLINE_FLOPS = 1e9            # of one product of the two
 def _worth_overlapping(layer: nn.Module, acts, backprops) -> bool:
     if not isinstance(acts, torch.Tensor) or not isinstance(backprops, torch.Tensor):
         return True
+    if layer.__dict__.get("_gs_sample_grads") is not None:
+        return False   # each sample's gradients are there: a few kilobytes are left to do
     if acts.numel() + backprops.numel() > _INLINE_ELEMENTS:
         return True
     if isinstance(layer, (nn.LayerNorm, nn.Embedding, QKNormRotary)):

@@ -441,19 +441,18 @@ __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(QkArgs a) {
   }
 }
 
-// Sums of the partial rows.  Row y of the grid below `samples`: out[part][y][f] = the sum of sample
-// y's rows; y = samples: `val`, the val samples' rows; y = samples + 1 (or y = 0 without samples):
-// the train samples' rows times the scale, as a weight gradient.  Partial rows lie in sample order,
-// so each is one range of rows or two.  A workgroup takes 16 features; its 64 groups of 16 threads
-// take every 64th row and are added in a fixed order.
+// Sums of the partial rows, one for each row y of the grid (from y0 on).  y below `samples`:
+// out[part][y][f] = the sum of sample y's rows; y = samples: `val`, the val samples' rows; y = samples
+// + 1: the train samples' rows times the scale, as a weight gradient (outputs that are null are left
+// out).  Partial rows lie in sample order, so each is one range of rows or two.  A workgroup takes 16
+// features; its 64 groups of 16 threads take every 64th row and are added in a fixed order.
 constexpr int QR_COLS = 16, QR_GROUPS = 64;
 struct QkSums {
   const float* part[2];
-  int64_t rows[2];      // partial rows of a sample (all of them without samples)
-  int64_t samples;      // 0: only the train sum, over everything
-  int64_t n_val, val_start;
-  float* out[2];        // [samples][D]
-  float* val[2];        // [D]
+  int64_t rows[2];      // partial rows of a sample
+  int64_t samples, n_val, val_start, y0;
+  float* out[2];        // [samples][D] or null
+  float* val[2];        // [D] or null
   void* grad[2];        // [D] or null
   int grad_bf16[2];
   float scale;
@@ -462,12 +461,11 @@ struct QkSums {
 __global__ void __launch_bounds__(QR_COLS * QR_GROUPS) qk_sums_kernel(QkSums q) {
   __shared__ float red[QR_GROUPS][QR_COLS];
   const int part = blockIdx.z;
-  const int64_t y = blockIdx.y;
+  const int64_t y = q.y0 + blockIdx.y, n = q.samples;
   const int col = threadIdx.x % QR_COLS, grp = threadIdx.x / QR_COLS;
   const int f = blockIdx.x * QR_COLS + col;
-  const int64_t rows = q.rows[part], n = q.samples > 0 ? q.samples : 1;
-  const bool is_sample = y < q.samples, is_val = y == q.samples && q.samples > 0;
-  const int64_t v0 = q.samples > 0 ? q.val_start : n, v1 = v0 + q.n_val;
+  const int64_t rows = q.rows[part], v0 = q.val_start, v1 = v0 + q.n_val;
+  const bool is_sample = y < n, is_val = y == n;
   const int64_t lo[2] = {is_sample ? y : is_val ? v0 : 0, is_sample || is_val ? 0 : v1};
   const int64_t hi[2] = {is_sample ? y + 1 : is_val ? v1 : v0, is_sample || is_val ? 0 : n};
   float t0 = 0.f, t1 = 0.f;
@@ -492,9 +490,9 @@ __global__ void __launch_bounds__(QR_COLS * QR_GROUPS) qk_sums_kernel(QkSums q) 
   if (grp != 0 || f >= q.D) return;
   const float t = red[0][col];
   if (is_sample) {
-    q.out[part][y * q.D + f] = t;
+    if (q.out[part] != nullptr) q.out[part][y * q.D + f] = t;
   } else if (is_val) {
-    q.val[part][f] = t;
+    if (q.val[part] != nullptr) q.val[part][f] = t;
   } else if (q.grad[part] != nullptr) {
     if (q.grad_bf16[part])
       static_cast<uint16_t*>(q.grad[part])[f] = f32_to_bf16(q.scale * t);
@@ -682,11 +680,11 @@ QkPlan qk_plan(QkArgs& a, int dtype, bool inter, bool backward, bool per_sample,
 struct QkScratch {
   float *part[2], *sums[2], *val[2];
   template <class S>
-  QkScratch(S& c, const QkArgs& a, const QkPlan& p, bool per_sample) {
+  QkScratch(S& c, const QkArgs& a, const QkPlan& p) {
     for (int k = 0; k < 2; ++k) {
       part[k] = c.template take<float>(a.segments * p.rows[k] * a.D);
-      sums[k] = c.template take<float>(per_sample ? a.segments * a.D : 0);
-      val[k] = c.template take<float>(per_sample ? a.D : 0);
+      sums[k] = c.template take<float>(a.segments * a.D);
+      val[k] = c.template take<float>(a.D);
     }
   }
 };
@@ -704,7 +702,7 @@ size_t qk_workspace(const gs_qk_shape* sh, bool per_sample) {
       if (t.heads[0] + t.heads[1] == 0 || (sh->interleaved == 0 && a.rot / 2 % v != 0)) continue;
       const QkPlan p = qk_plan(t, sh->dtype, sh->interleaved != 0, true, per_sample, v);
       Sizer sz;
-      QkScratch unused(sz, t, p, per_sample);
+      QkScratch unused(sz, t, p);
       most = std::max(most, sz.used);
     }
   }
@@ -735,52 +733,124 @@ extern "C" int gs_qk_rotary(const gs_qk_shape* shape, const gs_qk_rows x[3],
   return qk_run<false>(a, shape->dtype, inter, p.v, static_cast<hipStream_t>(stream));
 }
 
-extern "C" size_t gs_qk_rotary_grad_workspace(const gs_qk_shape* shape) {
-  return qk_workspace(shape, false);
+namespace gs {
+namespace {
+
+// The dots from the samples' and the val samples' sums; one launch.
+int qk_launch_dots(const float* const S[2], float* const val[2], float* const dot[2], int64_t B,
+                   int64_t n_val, int64_t val_start, int D, hipStream_t s) {
+  QkDots o{};
+  for (int k = 0; k < 2; ++k) o.S[k] = S[k], o.val[k] = val[k], o.dot[k] = dot[k];
+  hipLaunchKernelGGL(qk_dots_kernel, dim3(static_cast<unsigned>(B - n_val), 2), dim3(64), 0, s, o,
+                     train_rows(B, n_val, val_start, 1), D);
+  return check_launch("qk_dots_kernel");
+}
+
+void qk_launch_sums(const QkSums& q, int64_t rows, hipStream_t s) {
+  hipLaunchKernelGGL(qk_sums_kernel,
+                     dim3((q.D + QR_COLS - 1) / QR_COLS, static_cast<unsigned>(rows), 2),
+                     dim3(QR_COLS * QR_GROUPS), 0, s, q);
+}
+
+bool qk_split_ok(int64_t B, int64_t n_val, int64_t val_start) {
+  return n_val > 0 && n_val < B && val_start >= 0 && val_start + n_val <= B;
+}
+constexpr int64_t QK_MAX_SAMPLES = 65533;   // the sums' grid
+
+}  // namespace
+}  // namespace gs
+
+extern "C" size_t gs_qk_rotary_grad_workspace(const gs_qk_shape* shape, int per_sample) {
+  return qk_workspace(shape, per_sample != 0);
 }
 
 extern "C" int gs_qk_rotary_grad(const gs_qk_shape* shape, const gs_qk_rows x[3],
                                  const gs_qk_rows dy[3], const gs_qk_rows dx[3], void* grad_qw,
-                                 void* grad_kw, void* workspace, size_t workspace_bytes,
-                                 void* stream) {
+                                 void* grad_kw, float* sample_grads, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
   QkArgs a;
   if (int rc = qk_args(a, "gs_qk_rotary_grad", shape, x, dy, dx)) return rc;
-  if (x == nullptr || dy == nullptr || (dx == nullptr && grad_qw == nullptr && grad_kw == nullptr) ||
+  void* gw[2] = {grad_qw, grad_kw};
+  const bool samples = sample_grads != nullptr;
+  const bool want_w = grad_qw != nullptr || grad_kw != nullptr || samples;
+  if (x == nullptr || dy == nullptr || (dx == nullptr && !want_w) ||
       qk_check_rows("gs_qk_rotary_grad", shape, x, shape->norm != 0) != GS_OK ||
       (dx != nullptr && qk_check_rows("gs_qk_rotary_grad", shape, dx, true) != GS_OK))
     return fail(GS_ERR_INVALID, "gs_qk_rotary_grad: invalid arguments");
-  void* gw[2] = {grad_qw, grad_kw};
   for (int k = 0; k < 2; ++k)
-    if (gw[k] != nullptr && (shape->norm == 0 || shape->weight[k] == nullptr))
+    if ((gw[k] != nullptr && shape->weight[k] == nullptr) || (want_w && shape->norm == 0))
       return fail(GS_ERR_INVALID, "gs_qk_rotary_grad: a weight's gradient without the weight");
+  if (samples && a.B > QK_MAX_SAMPLES)
+    return fail(GS_ERR_UNSUPPORTED, "gs_qk_rotary_grad: sums of more than 65533 samples");
   if (dx == nullptr) a.heads[2] = 0;   // values have no part in the weights' gradients
   if (a.heads[0] + a.heads[1] + a.heads[2] == 0)
     return fail(GS_ERR_INVALID, "gs_qk_rotary_grad: invalid arguments");
-  const bool inter = shape->interleaved != 0, want_w = gw[0] != nullptr || gw[1] != nullptr;
+  const bool inter = shape->interleaved != 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const QkPlan p = qk_plan(a, shape->dtype, inter, true, false);
+  const QkPlan p = qk_plan(a, shape->dtype, inter, true, samples);
   QkSums q{};
   if (want_w) {
     Sizer sz;
-    QkScratch unused(sz, a, p, false);
+    QkScratch unused(sz, a, p);
     if (workspace == nullptr || workspace_bytes < sz.used)
       return fail(GS_ERR_WORKSPACE, "gs_qk_rotary_grad: workspace too small");
     Carver cv(workspace, workspace_bytes);
-    const QkScratch w(cv, a, p, false);
+    const QkScratch w(cv, a, p);
     for (int k = 0; k < 2; ++k) {
-      if (gw[k] != nullptr && a.heads[k] > 0) q.part[k] = a.part[k] = w.part[k];
+      if ((gw[k] != nullptr || samples) && a.heads[k] > 0) q.part[k] = a.part[k] = w.part[k];
       q.rows[k] = p.rows[k];
+      q.out[k] = samples ? sample_grads + k * a.B * a.D : nullptr;
       q.grad[k] = gw[k];
       q.grad_bf16[k] = shape->weight_dtype[k] == GS_DTYPE_BF16;
     }
   }
   if (int rc = qk_run<true>(a, shape->dtype, inter, p.v, s)) return rc;
   if (!want_w) return GS_OK;
+  // every segment is a "train sample" here: the total is the sum over all of them
+  q.samples = a.segments;
+  q.y0 = samples ? 0 : a.segments + 1;
   q.scale = 1.f;
   q.D = a.D;
-  hipLaunchKernelGGL(qk_sums_kernel, dim3((a.D + QR_COLS - 1) / QR_COLS, 1, 2),
-                     dim3(QR_COLS * QR_GROUPS), 0, s, q);
+  qk_launch_sums(q, a.segments + 2 - q.y0, s);
   return check_launch("qk_sums_kernel");
+}
+
+extern "C" size_t gs_qk_sample_dots_workspace(int64_t D) {
+  return D > 0 ? static_cast<size_t>(2 * D) * sizeof(float) + 512 : 0;
+}
+
+extern "C" int gs_qk_sample_dots(const float* sample_grads, int64_t B, int64_t D, int64_t n_val,
+                                 int64_t val_start, float* out_dot_q, float* out_dot_k,
+                                 void* out_grad_q, int grad_q_dtype, void* out_grad_k,
+                                 int grad_k_dtype, float grad_scale, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  for (int dt : {grad_q_dtype, grad_k_dtype})
+    if (dt != GS_DTYPE_BF16 && dt != GS_DTYPE_F32)
+      return fail(GS_ERR_DTYPE, "gs_qk_sample_dots: gradients must be bf16 or fp32");
+  if (sample_grads == nullptr || B <= 0 || D <= 0 || !qk_split_ok(B, n_val, val_start))
+    return fail(GS_ERR_INVALID, "gs_qk_sample_dots: invalid arguments");
+  if (B > QK_MAX_SAMPLES || D > QK_MAX_D)
+    return fail(GS_ERR_UNSUPPORTED, "gs_qk_sample_dots: more than 65533 samples or 512 features");
+  if (workspace == nullptr || workspace_bytes < gs_qk_sample_dots_workspace(D))
+    return fail(GS_ERR_WORKSPACE, "gs_qk_sample_dots: workspace too small");
+  Carver cv(workspace, workspace_bytes);
+  const float* S[2] = {sample_grads, sample_grads + B * D};
+  float* dot[2] = {out_dot_q, out_dot_k};
+  float* val[2];
+  void* gw[2] = {out_grad_q, out_grad_k};
+  const int dt[2] = {grad_q_dtype, grad_k_dtype};
+  QkSums q{};
+  for (int k = 0; k < 2; ++k) {
+    val[k] = cv.take<float>(D);
+    q.part[k] = S[k], q.rows[k] = 1, q.val[k] = val[k];
+    q.grad[k] = gw[k], q.grad_bf16[k] = dt[k] == GS_DTYPE_BF16;
+  }
+  q.samples = B, q.n_val = n_val, q.val_start = val_start, q.y0 = B;
+  q.scale = grad_scale;
+  q.D = static_cast<int>(D);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  qk_launch_sums(q, 2, s);
+  return qk_launch_dots(S, val, dot, B, n_val, val_start, q.D, s);
 }
 
 extern "C" size_t gs_qk_rotary_dots_workspace(const gs_qk_shape* shape) {
@@ -796,11 +866,10 @@ extern "C" int gs_qk_rotary_dots(const gs_qk_shape* shape, const gs_qk_rows x[3]
   if (int rc = qk_args(a, "gs_qk_rotary_dots", shape, x, dy, nullptr)) return rc;
   void* gw[2] = {out_grad_q, out_grad_k};
   float* dot[2] = {out_dot_q, out_dot_k};
-  if (x == nullptr || dy == nullptr || shape->norm == 0 || n_val <= 0 || n_val >= shape->B ||
-      val_start < 0 || val_start + n_val > shape->B ||
+  if (x == nullptr || dy == nullptr || shape->norm == 0 || !qk_split_ok(shape->B, n_val, val_start) ||
       qk_check_rows("gs_qk_rotary_dots", shape, x, true) != GS_OK)
     return fail(GS_ERR_INVALID, "gs_qk_rotary_dots: invalid arguments");
-  if (a.B > 65533)   // the sums' grid
+  if (a.B > QK_MAX_SAMPLES)
     return fail(GS_ERR_UNSUPPORTED, "gs_qk_rotary_dots: more than 65533 samples");
   a.heads[2] = 0;
   if (a.heads[0] + a.heads[1] == 0)
@@ -809,13 +878,12 @@ extern "C" int gs_qk_rotary_dots(const gs_qk_shape* shape, const gs_qk_rows x[3]
   hipStream_t s = static_cast<hipStream_t>(stream);
   const QkPlan p = qk_plan(a, shape->dtype, inter, true, true);
   Sizer sz;
-  QkScratch unused(sz, a, p, true);
+  QkScratch unused(sz, a, p);
   if (workspace == nullptr || workspace_bytes < sz.used)
     return fail(GS_ERR_WORKSPACE, "gs_qk_rotary_dots: workspace too small");
   Carver cv(workspace, workspace_bytes);
-  const QkScratch w(cv, a, p, true);
+  const QkScratch w(cv, a, p);
   QkSums q{};
-  QkDots o{};
   for (int k = 0; k < 2; ++k) {
     if (a.heads[k] > 0) q.part[k] = a.part[k] = w.part[k];
     q.rows[k] = p.rows[k];
@@ -823,18 +891,12 @@ extern "C" int gs_qk_rotary_dots(const gs_qk_shape* shape, const gs_qk_rows x[3]
     q.val[k] = w.val[k];
     q.grad[k] = gw[k];
     q.grad_bf16[k] = shape->weight_dtype[k] == GS_DTYPE_BF16;
-    o.S[k] = w.sums[k];
-    o.val[k] = w.val[k];
-    o.dot[k] = dot[k];
   }
   q.samples = a.B, q.n_val = n_val, q.val_start = val_start;
   q.scale = grad_scale;
   q.D = a.D;
   if (int rc = qk_run<true>(a, shape->dtype, inter, p.v, s)) return rc;
-  hipLaunchKernelGGL(qk_sums_kernel,
-                     dim3((a.D + QR_COLS - 1) / QR_COLS, static_cast<unsigned>(a.B + 2), 2),
-                     dim3(QR_COLS * QR_GROUPS), 0, s, q);
-  hipLaunchKernelGGL(qk_dots_kernel, dim3(static_cast<unsigned>(a.B - n_val), 2), dim3(64), 0, s,
-                     o, train_rows(a.B, n_val, val_start, a.T), a.D);
-  return check_launch("qk_sums_kernel / qk_dots_kernel");
+  qk_launch_sums(q, a.B + 2, s);
+  const float* S[2] = {w.sums[0], w.sums[1]};
+  return qk_launch_dots(S, w.val, dot, a.B, n_val, val_start, a.D, s);
 }

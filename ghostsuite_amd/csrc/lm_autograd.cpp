@@ -72,6 +72,7 @@ c10::Device device_of(std::initializer_list<const Tensor*> ts) {
 void* stream_on(c10::Device dev) { return c10::hip::getCurrentHIPStream(dev.index()).stream(); }
 
 Tensor given(const OptTensor& t) { return t ? *t : Tensor(); }
+OptTensor some(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* mut(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 
@@ -207,7 +208,8 @@ struct QkHow {
   int64_t heads[3];
   bool norm, interleaved;
   double eps;
-  int edge[4];   // each input's place among the node's edges, or -1
+  Tensor samples;   // where the backward pass writes each sample's weight gradients, or undefined
+  int edge[4];      // each input's place among the node's edges, or -1
 };
 
 // The arguments of a gs_qk_rotary* call.  `a`: one packed tensor (b undefined), or queries a, keys b.
@@ -367,19 +369,21 @@ struct QkNormRotary : torch::autograd::Function<QkNormRotary> {
     if (c.empty()) {
       for (Tensor& w : dw)
         if (w.defined()) w.zero_();
-    } else if (want_x || dw[0].defined() || dw[1].defined()) {
+      if (how.samples.defined()) how.samples.zero_();
+    } else if (want_x || dw[0].defined() || dw[1].defined() || how.samples.defined()) {
       gs_qk_rows dy[3]{}, dx[3]{};
       heads_first(grads, dy);
       if (want_x) c.rows(da, db, dx);
       Tensor ws;
       size_t bytes = 0;
-      if (dw[0].defined() || dw[1].defined()) {
-        bytes = gs_qk_rotary_grad_workspace(&c.shape);
+      if (dw[0].defined() || dw[1].defined() || how.samples.defined()) {
+        bytes = gs_qk_rotary_grad_workspace(&c.shape, how.samples.defined());
         ws = scratch(bytes, s[0]);
       }
       c10::DeviceGuard guard(c.dev);
       check(gs_qk_rotary_grad(&c.shape, c.x, dy, want_x ? dx : nullptr, mut(dw[0]), mut(dw[1]),
-                              mut(ws), bytes, stream_on(c.dev)),
+                              static_cast<float*>(mut(how.samples)), mut(ws), bytes,
+                              stream_on(c.dev)),
             "gs_qk_rotary_grad");
     }
     return once({da, db, dw[0], dw[1], Tensor(), Tensor(), Tensor()});
@@ -387,14 +391,26 @@ struct QkNormRotary : torch::autograd::Function<QkNormRotary> {
 };
 
 QkHow qk_how(const std::vector<int64_t>& heads, bool norm, double eps, bool interleaved) {
-  return QkHow{{heads.at(0), heads.at(1), heads.at(2)}, norm, interleaved, eps, {-1, -1, -1, -1}};
+  return QkHow{{heads.at(0), heads.at(1), heads.at(2)}, norm, interleaved, eps, Tensor(),
+               {-1, -1, -1, -1}};
 }
 
-// (queries, keys[, values]) of a packed tensor a, or of queries a and keys b.
+// (queries, keys[, values]) of a packed tensor a, or of queries a and keys b; the backward pass fills
+// `samples`.
 variable_list qk_norm_rotary(const Tensor& a, const OptTensor& b, const std::vector<int64_t>& heads,
                              const Tensor& table, const OptTensor& positions, const OptTensor& qw,
-                             const OptTensor& kw, bool norm, double eps, bool interleaved) {
-  const QkHow how = qk_how(heads, norm, eps, interleaved);
+                             const OptTensor& kw, bool norm, double eps, bool interleaved,
+                             const OptTensor& samples) {
+  QkHow how = qk_how(heads, norm, eps, interleaved);
+  how.samples = given(samples);
+  if (how.samples.defined())
+    require(norm && how.samples.is_cuda() && how.samples.device() == a.device() &&
+                how.samples.scalar_type() == at::kFloat && how.samples.is_contiguous() &&
+                how.samples.dim() == 3 && how.samples.size(0) == 2 &&
+                how.samples.size(1) == a.size(0) &&
+                how.samples.size(2) * (heads[0] + heads[1] + heads[2]) * a.size(1) * a.size(0) ==
+                    a.numel(),
+            "sample gradients ", how.samples.sizes(), ": fp32 [2, B, D] for a packed input expected");
   const Tensor bt = given(b), q = given(qw), k = given(kw);
   if (recorded({&a, &bt, &q, &k}))
     return QkNormRotary::apply(a, b, qw, kw, table, positions, how);
@@ -433,7 +449,34 @@ std::vector<OptTensor> qk_norm_rotary_dots(const Tensor& a, const OptTensor& b,
                           mut(dw[0]), mut(dw[1]), static_cast<float>(grad_scale.value_or(0.0)), mut(ws),
                           bytes, stream_on(c.dev)),
         "gs_qk_rotary_dots");
-  const auto some = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+  return {dots[0], dots[1], some(dw[0]), some(dw[1])};
+}
+
+std::vector<OptTensor> qk_sample_dots(const Tensor& samples, const Tensor& qw, const Tensor& kw,
+                                      int64_t n_val, std::optional<int64_t> val_start,
+                                      std::optional<double> grad_scale) {
+  const c10::Device dev = device_of({&samples, &qw, &kw});
+  require(samples.dim() == 3 && samples.size(0) == 2 && samples.scalar_type() == at::kFloat &&
+              samples.is_contiguous(),
+          "sample gradients ", samples.sizes(), ": fp32 [2, B, D] expected");
+  const int64_t B = samples.size(1), D = samples.size(2), n_train = B - n_val;
+  require(n_train > 0, "qk_sample_dots: ", n_val, " validation samples of ", B);
+  const auto fp32 = samples.options().requires_grad(false);
+  const Tensor dots[2] = {at::empty({n_train}, fp32), at::empty({n_train}, fp32)};
+  const int dt[2] = {gs_dtype_of(qw, "norm weights"), gs_dtype_of(kw, "norm weights")};
+  Tensor dw[2];
+  if (grad_scale) {
+    dw[0] = at::empty({D}, qw.options().requires_grad(false));
+    dw[1] = at::empty({D}, kw.options().requires_grad(false));
+  }
+  const size_t bytes = gs_qk_sample_dots_workspace(D);
+  const Tensor ws = scratch(bytes, samples);
+  c10::DeviceGuard guard(dev);
+  check(gs_qk_sample_dots(static_cast<const float*>(ptr(samples)), B, D, n_val,
+                          val_start.value_or(n_train), static_cast<float*>(mut(dots[0])),
+                          static_cast<float*>(mut(dots[1])), mut(dw[0]), dt[0], mut(dw[1]), dt[1],
+                          static_cast<float>(grad_scale.value_or(0.0)), mut(ws), bytes, stream_on(dev)),
+        "gs_qk_sample_dots");
   return {dots[0], dots[1], some(dw[0]), some(dw[1])};
 }
 
@@ -597,5 +640,6 @@ PYBIND11_MODULE(_lm_autograd, m) {
   m.def("embedding_lookup", &embedding_lookup);
   m.def("qk_norm_rotary", &qk_norm_rotary);
   m.def("qk_norm_rotary_dots", &qk_norm_rotary_dots);
+  m.def("qk_sample_dots", &qk_sample_dots);
   m.def("distillation_loss", &distillation_loss);
 }

@@ -151,11 +151,19 @@ class QKNormRotary(nn.Module):
         return self
 
     def forward(self, qkv: torch.Tensor, positions: Optional[torch.Tensor] = None):
+        sample_grads = None
         if self.norm and hasattr(self.q_weight, "initially_requires_grad"):
-            self.__dict__["_gs_positions"] = positions   # an engine's backward hook reads them
-        return qkv_norm_rotary(qkv, self.n_head, self.n_kv_head, self.table, positions,
-                               self.q_weight, self.k_weight, norm=self.norm, eps=self.eps,
-                               interleaved=self.interleaved)
+            # An engine's backward hook reads these: the positions, and each sample's gradients of
+            # the weights, which the backward pass forms on its way (it runs before the hook when
+            # the input has a gradient).
+            if torch.is_grad_enabled() and qkv.requires_grad:
+                sample_grads = torch.empty(2, qkv.shape[0], self.head_dim, device=qkv.device)
+            self.__dict__["_gs_positions"] = positions
+            self.__dict__["_gs_sample_grads"] = sample_grads
+        q, k, v = ops().qk_norm_rotary(
+            qkv, None, (self.n_head, self.n_kv_head, self.n_kv_head), self.table, positions,
+            self.q_weight, self.k_weight, self.norm, self.eps, self.interleaved, sample_grads)
+        return q, k, v
 
     def extra_repr(self) -> str:
         return (f"{self.n_head}, {self.n_kv_head}, {self.head_dim}, n_rot={self.n_rot}, "

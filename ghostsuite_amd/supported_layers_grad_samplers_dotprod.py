@@ -568,12 +568,17 @@ def _compute_qk_norm_dot_product(layer: QKNormRotary, A: torch.Tensor, B: torch.
 
 
 def _qk_norm_pass(layer: QKNormRotary, A, B, val_batch_size, grad_scale, dots: bool):
-    grads = layer.__dict__.get("_gs_grad_outputs") or (B, None, None)
+    d = layer.__dict__
     q, k = _param(layer, "q_weight"), _param(layer, "k_weight")
-    dot_q, dot_k, grad_q, grad_k = ops().qk_norm_rotary_dots(
-        A.detach(), None, (layer.n_head, layer.n_kv_head, layer.n_kv_head), layer.table,
-        layer.__dict__.get("_gs_positions"), q.detach(), k.detach(), layer.eps, layer.interleaved,
-        grads, val_batch_size, grad_scale=grad_scale)
+    samples = d.get("_gs_sample_grads")
+    if samples is not None:   # formed by the layer's backward pass
+        dot_q, dot_k, grad_q, grad_k = ops().qk_sample_dots(
+            samples, q.detach(), k.detach(), val_batch_size, grad_scale=grad_scale)
+    else:
+        dot_q, dot_k, grad_q, grad_k = ops().qk_norm_rotary_dots(
+            A.detach(), None, (layer.n_head, layer.n_kv_head, layer.n_kv_head), layer.table,
+            d.get("_gs_positions"), q.detach(), k.detach(), layer.eps, layer.interleaved,
+            d.get("_gs_grad_outputs") or (B, None, None), val_batch_size, grad_scale=grad_scale)
     if dots:
         q.grad_dot_prod, k.grad_dot_prod = dot_q, dot_k
     if grad_q is not None:

@@ -427,11 +427,13 @@ int gs_qk_rotary(const gs_qk_shape* shape, const gs_qk_rows x[3], const gs_qk_ro
 
 /* Backward of gs_qk_rotary: dy the gradients of y (data NULL: zeros), x its inputs.
  * dx: NULL, or the input gradients.  grad_qw, grad_kw: NULL, or [D] gradients of the weights
- * (sums in fp32 in a fixed order, rounded once). */
-size_t gs_qk_rotary_grad_workspace(const gs_qk_shape* shape);
+ * (sums in fp32 in a fixed order, rounded once).  sample_grads: NULL, or [2, B, D] fp32: the
+ * gradients of q's weight, then of k's, from each sample alone (per_sample of the query: whether it is
+ * passed); up to 65533 samples. */
+size_t gs_qk_rotary_grad_workspace(const gs_qk_shape* shape, int per_sample);
 int gs_qk_rotary_grad(const gs_qk_shape* shape, const gs_qk_rows x[3], const gs_qk_rows dy[3],
-                      const gs_qk_rows dx[3], void* grad_qw, void* grad_kw, void* workspace,
-                      size_t workspace_bytes, void* stream);
+                      const gs_qk_rows dx[3], void* grad_qw, void* grad_kw, float* sample_grads,
+                      void* workspace, size_t workspace_bytes, void* stream);
 
 /* The weights' gradient dot products and train gradients, as gs_layernorm_dot's for a LayerNorm:
  * with s_i the gradient of a weight from sample i alone,
@@ -443,6 +445,14 @@ int gs_qk_rotary_dots(const gs_qk_shape* shape, const gs_qk_rows x[3], const gs_
                       int64_t n_val, int64_t val_start, float* out_dot_q, float* out_dot_k,
                       void* out_grad_q, void* out_grad_k, float grad_scale, void* workspace,
                       size_t workspace_bytes, void* stream);
+
+/* The same from the sample_grads of gs_qk_rotary_grad, where the layer's backward pass formed them
+ * beside its input gradients. */
+size_t gs_qk_sample_dots_workspace(int64_t D);
+int gs_qk_sample_dots(const float* sample_grads, int64_t B, int64_t D, int64_t n_val,
+                      int64_t val_start, float* out_dot_q, float* out_dot_k, void* out_grad_q,
+                      int grad_q_dtype, void* out_grad_k, int grad_k_dtype, float grad_scale,
+                      void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- Loss against a teacher's top logits -------------------------------------------------
  * Per row z of V student logits, K teacher entries (id, logit t) and a label y:

@@ -174,8 +174,17 @@ class LmOracleOps(OracleOps):
             w = torch.where((torch.arange(len(w)) == padding_idx)[:, None], w.detach(), w)
         return lookup(ids, w, scale).to(weight.dtype)
 
-    def qk_norm_rotary(self, q, k, heads, table, positions, qw, kw, norm, eps, interleaved):
+    def qk_norm_rotary(self, q, k, heads, table, positions, qw, kw, norm, eps, interleaved,
+                       sample_grads=None):
         parts = [p.double() for p in (q, k) if p is not None]
+        if sample_grads is not None:   # weights of each sample, whose gradients a hook keeps
+            B, D = sample_grads.shape[1:]
+            w = [x.detach().double().expand(B, D).clone().requires_grad_() for x in (qw, kw)]
+            for i in range(2):
+                w[i].register_hook(lambda g, i=i: sample_grads[i].copy_(g) * 0 + g)
+            out = qk_all(plan(heads, table, positions, norm, eps, interleaved), parts,
+                         w[0][:, None, None], w[1][:, None, None])
+            return [y.to(q.dtype).contiguous() for y in out]
         w = [None if x is None else x.double() for x in (qw, kw)]
         return [y.to(q.dtype).contiguous()
                 for y in qk_all(plan(heads, table, positions, norm, eps, interleaved), parts, *w)]
@@ -192,6 +201,17 @@ class LmOracleOps(OracleOps):
         val[vs:vs + n_val] = True
         out = [(s[~val] @ s[val].sum(0)).float() for s in (dq, dk)]
         for s, w in ((dq, qw), (dk, kw)):
+            out.append(None if grad_scale is None else (s[~val].sum(0) * grad_scale).to(w.dtype))
+        return out
+
+    def qk_sample_dots(self, sample_grads, qw, kw, n_val, *, val_start=None, grad_scale=None):
+        self.calls.append(("qk_sample_dots", tuple(sample_grads.shape)))
+        B = sample_grads.shape[1]
+        vs = B - n_val if val_start is None else val_start
+        val = torch.zeros(B, dtype=torch.bool)
+        val[vs:vs + n_val] = True
+        out = [(s[~val] @ s[val].sum(0)).float() for s in sample_grads]
+        for s, w in zip(sample_grads, (qw, kw)):
             out.append(None if grad_scale is None else (s[~val].sum(0) * grad_scale).to(w.dtype))
         return out
 

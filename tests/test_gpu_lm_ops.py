@@ -371,6 +371,26 @@ def test_qk_dots(gpu, dtype, B, n_val, T, heads, D, n_rot, val_start):
     got = _native.ops().qk_norm_rotary_dots(x, None, heads, plan["table"], None, qw.detach(),
                                             kw.detach(), 1e-6, False, grads, n_val,
                                             val_start=val_start, grad_scale=0.25)
+    check_dots(got, plan, x, qw, kw, grads, n_val, val_start)
+    # the same from the sums that a layer's backward pass leaves
+    samples = torch.full((2, B, D), math.nan, device=gpu)
+    y = _native.ops().qk_norm_rotary(x.requires_grad_(), None, heads, plan["table"], None, qw, kw,
+                                     True, 1e-6, False, samples)
+    dx, dqw, dkw = torch.autograd.grad(y, (x, qw, kw), grads)
+    got = _native.ops().qk_sample_dots(samples, qw.detach(), kw.detach(), n_val,
+                                       val_start=val_start, grad_scale=0.25)
+    check_dots(got, plan, x, qw, kw, grads, n_val, val_start)
+    plain = gs.qkv_norm_rotary(x, heads[0], heads[1], plan["table"], None, qw, kw)
+    assert torch.equal(dx, torch.autograd.grad(plain, x, grads)[0])
+    _, dq, dk = L.qk_grads(plan, (x,), qw, kw, grads)
+    addends = qk_bounds(plan, (x,), qw, kw, grads)[2]
+    for g, want, mag, h in zip((dqw, dkw), (dq, dk), addends, heads):
+        within(g, want, (B * T * h + D / 2 + 24) * U * mag + want.abs() * HALF[dtype], "total")
+
+
+def check_dots(got, plan, x, qw, kw, grads, n_val, val_start):
+    heads, (B, T) = plan["heads"], x.shape[:2]
+    D, n_rot = L.grads_dim(plan, (x,)), 2 * plan["table"].shape[-1]
     _, dq, dk = L.qk_grads(plan, (x,), qw, kw, grads, per_sample=True)
     xs = L.split_heads(plan, (f64(x),))
     vs = B - n_val if val_start is None else val_start

@@ -112,10 +112,12 @@ def test_qk_arguments_are_checked_on_the_host(changes, status):
     ref = ctypes.byref(s)
     rows = _qk_rows()
     assert lib.gs_qk_rotary(ref, rows, rows, None) == status
-    assert lib.gs_qk_rotary_grad(ref, rows, rows, rows, P16, P16, None, 0, None) == status
+    assert lib.gs_qk_rotary_grad(ref, rows, rows, rows, P16, P16, None, None, 0, None) == status
+    assert lib.gs_qk_rotary_grad(ref, rows, rows, rows, None, None, P16, None, 0, None) == status
     assert lib.gs_qk_rotary_dots(ref, rows, rows, 1, 1, P16, P16, P16, P16, 1.0, None, 0,
                                  None) == status
-    assert lib.gs_qk_rotary_grad_workspace(ref) == 0
+    assert lib.gs_qk_rotary_grad_workspace(ref, 0) == 0
+    assert lib.gs_qk_rotary_grad_workspace(ref, 1) == 0
     assert lib.gs_qk_rotary_dots_workspace(ref) == 0
     assert b"gs_qk_rotary" in lib.gs_last_error()
 
@@ -126,15 +128,20 @@ def test_qk_pointers_and_workspaces_are_checked_on_the_host():
     assert lib.gs_qk_rotary(None, rows, rows, None) == -1
     assert lib.gs_qk_rotary(ref, None, rows, None) == -1
     assert lib.gs_qk_rotary(ref, rows, none, None) == -1
-    assert lib.gs_qk_rotary_grad(ref, rows, rows, None, None, None, None, 0, None) == -1
-    assert lib.gs_qk_rotary_grad(ref, none, rows, rows, None, None, None, 0, None) == -1
-    assert lib.gs_qk_rotary_grad(ref, rows, rows, rows, P16, None, None, 0, None) == -3
-    need = lib.gs_qk_rotary_grad_workspace(ref)
+    assert lib.gs_qk_rotary_grad(ref, rows, rows, None, None, None, None, None, 0, None) == -1
+    assert lib.gs_qk_rotary_grad(ref, none, rows, rows, None, None, None, None, 0, None) == -1
+    assert lib.gs_qk_rotary_grad(ref, rows, rows, rows, P16, None, None, None, 0, None) == -3
+    assert lib.gs_qk_rotary_grad(ref, rows, rows, rows, None, None, P16, None, 0, None) == -3
+    many = ctypes.byref(_qk_shape(B=65534, T=1))
+    assert lib.gs_qk_rotary_grad(many, rows, rows, rows, None, None, P16, P16, 1 << 40, None) == -5
+    need = lib.gs_qk_rotary_grad_workspace(ref, 0)
     assert need > 0
     unweighted = _qk_shape()
     unweighted.weight[:] = (None, None)
-    assert lib.gs_qk_rotary_grad(ctypes.byref(unweighted), rows, rows, rows, P16, None, P16, need,
-                                 None) == -1
+    assert lib.gs_qk_rotary_grad(ctypes.byref(unweighted), rows, rows, rows, P16, None, None, P16,
+                                 need, None) == -1
+    assert lib.gs_qk_rotary_grad(ctypes.byref(_qk_shape(norm=0)), rows, rows, rows, None, None, P16,
+                                 P16, need, None) == -1          # sums of weights without the norm
     assert lib.gs_qk_rotary_dots(ref, rows, rows, 2, 0, P16, P16, P16, P16, 1.0, P16, 1 << 20,
                                  None) == -1                     # no train sample
     assert lib.gs_qk_rotary_dots(ref, rows, rows, 1, 2, P16, P16, P16, P16, 1.0, P16, 1 << 20,
@@ -143,6 +150,18 @@ def test_qk_pointers_and_workspaces_are_checked_on_the_host():
                                  None) == -3
     assert lib.gs_qk_rotary_dots(ctypes.byref(_qk_shape(norm=0)), rows, rows, 1, 1, P16, P16, P16,
                                  P16, 1.0, P16, 1 << 20, None) == -1
+
+
+def test_qk_sample_dots_arguments_are_checked_on_the_host():
+    f = _native.load_library().gs_qk_sample_dots
+    need = _native.load_library().gs_qk_sample_dots_workspace(64)
+    ok = [P16, 5, 64, 2, 3, P16, P16, P16, 0, P16, 1, 1.0, P16, need, None]
+    for change, status in (({0: None}, -1), ({1: 0}, -1), ({2: 0}, -1), ({3: 0}, -1), ({3: 5}, -1),
+                           ({4: 4}, -1), ({4: -1}, -1), ({8: 2}, -2), ({10: 7}, -2),
+                           ({1: 65534}, -5), ({2: 513, 13: 1 << 20}, -5), ({12: None}, -3),
+                           ({13: need - 1}, -3)):
+        args = [change.get(i, v) for i, v in enumerate(ok)]
+        assert f(*args) == status, change
 
 
 def _distill(**changes):
@@ -355,6 +374,8 @@ def test_engine_dots_and_train_gradients(oracle_ops, positions, padding_idx, dum
     dots = {k: params[k].grad_dot_prod for k in names}
     grads = {k: params[k].train_grad for k in names}
     eng.detach()
+    # a frozen or a trained embedding: the layer's input has a gradient, its backward pass the sums
+    assert [c[0] for c in oracle_ops.calls if c[0].startswith("qk_")] == ["qk_sample_dots"]
     per = {k: [] for k in names}
     for i in range(n):
         if net.positions is not None:
@@ -370,6 +391,26 @@ def test_engine_dots_and_train_gradients(oracle_ops, positions, padding_idx, dum
             assert_close(dots[k], want, 1e-4, k)
         # the engine averages the N-scaled train rows
         assert_close(grads[k], G[:n - n_val].sum(0) * n / (n - n_val), 1e-4, k)
+
+
+def test_engine_dots_of_a_layer_without_input_gradient(oracle_ops):
+    """Nothing before the layer has a gradient: the hook runs first and makes its own pass."""
+    torch.manual_seed(2)
+    layer = gs.QKNormRotary(2, 1, 6, n_positions=16)
+    x = torch.randn(5, 4, 24)
+    grads = [torch.randn(5, h, 4, 6) for h in (2, 1, 1)]
+    eng = GradDotProdEngine(layer, val_batch_size=2, precision="fp32")
+    eng.attach(torch.optim.SGD(layer.parameters(), lr=0.0))
+    torch.autograd.backward(layer(x, torch.arange(4) + 3)[:2], grads[:2])
+    grads[2] = None
+    assert [c[0] for c in oracle_ops.calls] == ["qk_norm_rotary_dots"]
+    got = [(w.grad_dot_prod, w.train_grad) for w in (layer.q_weight, layer.k_weight)]
+    eng.detach()
+    plan = L.plan((2, 1, 1), layer.table, torch.arange(4) + 3)
+    _, dq, dk = L.qk_grads(plan, (x,), layer.q_weight, layer.k_weight, grads, per_sample=True)
+    for (dot, grad), s in zip(got, (dq, dk)):
+        assert_close(dot, s[:3] @ s[3:].sum(0), 1e-5)
+        assert_close(grad, s[:3].sum(0) * 5 / 3, 1e-5)
 
 
 def test_tied_scaled_embedding_keeps_both_parts(oracle_ops):
