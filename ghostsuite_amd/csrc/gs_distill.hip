@@ -28,6 +28,7 @@ namespace {
 
 constexpr int DS_MAX_K = 1024;
 constexpr int DS_COUNT_THREADS = 1024;
+constexpr int64_t DS_MAX_BLOCKS = int64_t{1} << 21;   // below 2^32 threads; more rows are looped over
 
 struct DsArgs {
   const void* z;
@@ -498,9 +499,9 @@ int ds_args(DsArgs& a, const char* name, const gs_distill* d) {
     return fail(GS_ERR_DTYPE, n + ": logits must be bf16 or fp32");
   if (d->Z == nullptr || d->teacher_ids == nullptr || d->teacher == nullptr || d->N <= 0 ||
       d->V <= 0 || d->K <= 0 || d->inner <= 0 || d->inner > d->N || d->N % d->inner != 0 ||
-      (d->N > 1 && (d->stride_inner < d->V && d->inner > 1)) ||
-      (d->N > d->inner && d->stride_outer < d->V) || !(d->temperature > 0.f) ||
-      !std::isfinite(d->temperature * d->temperature) || !std::isfinite(1.f / d->temperature) || !(d->alpha >= 0.f && d->alpha <= 1.f) ||
+      (d->inner > 1 && d->stride_inner < d->V) || (d->N > d->inner && d->stride_outer < d->V) ||
+      !(d->temperature > 0.f) || !std::isfinite(d->temperature * d->temperature) ||
+      !std::isfinite(1.f / d->temperature) || !(d->alpha >= 0.f && d->alpha <= 1.f) ||
       (d->labels == nullptr && d->alpha != 1.f) || d->reduction < GS_REDUCE_NONE ||
       d->reduction > GS_REDUCE_MEAN ||
       reinterpret_cast<uintptr_t>(d->Z) % elem_size(d->dtype) != 0)
@@ -570,8 +571,9 @@ extern "C" int gs_distill_loss(const gs_distill* d, float* out_loss, void* grad,
   const bool two = ds_two(a);
   a.rows = a.per_row ? out_loss : w.rows;
   a.grad = grad;
-  const int rc = d->dtype == GS_DTYPE_BF16 ? ds_run<uint16_t>(a, two, a.N, s)
-                                           : ds_run<float>(a, two, a.N, s);
+  const int64_t grid = std::min(a.N, DS_MAX_BLOCKS);
+  const int rc = d->dtype == GS_DTYPE_BF16 ? ds_run<uint16_t>(a, two, grid, s)
+                                           : ds_run<float>(a, two, grid, s);
   if (rc || a.per_row) return rc;
   hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(DS_COUNT_THREADS), 0, s, w.rows, a.N,
                      a.mean, a.count, out_loss);
@@ -601,7 +603,7 @@ extern "C" int gs_distill_grad(const gs_distill* d, const float* upstream, int f
   a.grad = grad;
   a.upstream = upstream;
   // A filled gradient is mostly left as it is: few workgroups then look at the upstream and end.
-  const int64_t grid = a.filled ? std::min<int64_t>(a.N, 512) : a.N;
+  const int64_t grid = a.filled ? std::min<int64_t>(a.N, 512) : std::min(a.N, DS_MAX_BLOCKS);
   return d->dtype == GS_DTYPE_BF16 ? ds_run<uint16_t>(a, two, grid, s)
                                    : ds_run<float>(a, two, grid, s);
 }

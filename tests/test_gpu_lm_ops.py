@@ -101,6 +101,20 @@ def test_lookup_beyond_32_bit_offsets(gpu):
     assert (y[-1] == 6.0).all() and (y[-2] == 10.0).all() and (y[0] == 10.0).all()
 
 
+def test_lookup_of_more_pieces_than_a_launch_has_threads(gpu):
+    """Single elements, 2^34 and more of them: several launches."""
+    d, n = 4097, (1 << 22) + 5
+    w = randn((3, d), 1, 1.0, BF16).to(gpu)
+    ids = (torch.arange(n, device=gpu) % 4)            # 3: outside
+    y = gs.embedding_lookup(ids, w, 1.0)
+    assert y.numel() > 1 << 34
+    rows = torch.cat((w, torch.zeros_like(w[:1])))
+    for i in range(0, n, 1 << 20):
+        part = y[i:i + 1024]
+        assert torch.equal(part, rows[ids[i:i + 1024]])
+    assert torch.equal(y[-9:], rows[ids[-9:]])
+
+
 # ------------------------------------------------------------ norms, rotation, heads first
 def qk_bounds(plan, parts, qw, kw, grads):
     """Error bounds (of y per part, dx per part, and of dq, dk the magnitude of their addends).
@@ -675,6 +689,27 @@ def test_distill_beyond_32_bit_offsets(gpu):
     # another offset from a 16-byte boundary adds in another order: one rounding step of bf16
     off = (f64(g[-2:]) - f64(alone)).abs()
     assert (off <= f64(alone).abs() * 2 * HALF[BF16] + 1e-9).all()
+
+
+def test_distill_more_rows_than_a_launch_has_workgroups(gpu):
+    """2^21 workgroups take the rows in turn: the same rows again have the same bits."""
+    N, V, part = (1 << 21) + 3, 5, 1000
+    z, ids, t, labels = distill_inputs(part, V, 2, 3, FP32)
+    z, ids, t, labels = (x.to(gpu).repeat(N // part + 1, *[1] * (x.dim() - 1))[:N].contiguous()
+                         for x in (z, ids, t, labels))
+    z.requires_grad_()
+    how = dict(temperature=2.0, alpha=0.5, reduction="none")
+    loss = gs.distillation_loss(z, ids, t, labels, **how)
+    g, = torch.autograd.grad(loss, z, torch.ones_like(loss))
+    few = [x[:part].detach() for x in (z, ids, t, labels)]
+    few[0].requires_grad_()
+    want = gs.distillation_loss(*few, **how)
+    dwant, = torch.autograd.grad(want, few[0], torch.ones_like(want))
+    # rows of 20 bytes start at other places of a 16-byte piece every four rows; 1000 is their multiple
+    for i in (0, 5 * part, N // part * part):
+        k = min(part, N - i)
+        torch.testing.assert_close(loss[i:i + k], want[:k], rtol=0, atol=0, equal_nan=True)
+        torch.testing.assert_close(g[i:i + k], dwant[:k], rtol=0, atol=0, equal_nan=True)
 
 
 # ---------------------------------------------------------- together, graphs, streams, reuse
