@@ -118,7 +118,6 @@ _SIGNATURES = {
 }
 
 
-
 def load_library() -> ctypes.CDLL:
     """Loads libghost_hip.so (built in-tree by ghostsuite_amd.build) once per process."""
     global _lib
@@ -209,16 +208,20 @@ _ext = None
 def _lm():
     """The extension module around the language-model operators (csrc/lm_autograd.cpp)."""
     global _ext
-    if _ext is None:
-        load_library()   # says how to build, when nothing is
-        path = _build.extension_path()
-        if not path.exists():
-            raise GhostHipError(f"{path} is not built: run `python ghostsuite_amd/build.py` first")
-        spec = importlib.util.spec_from_file_location(_build.EXTNAME, path)
-        mod = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(mod)
-        mod.raise_as(GhostHipError)
-        _ext = mod
+    if _ext is not None:
+        return _ext
+    load_library()   # says how to build, when nothing is
+    with _lock:
+        if _ext is None:
+            path = _build.extension_path()
+            if not path.exists():
+                raise GhostHipError(
+                    f"{path} is not built: run `python ghostsuite_amd/build.py` first")
+            spec = importlib.util.spec_from_file_location(_build.EXTNAME, path)
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+            mod.raise_as(GhostHipError)
+            _ext = mod
     return _ext
 
 

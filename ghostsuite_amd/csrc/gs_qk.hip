@@ -633,7 +633,7 @@ int qk_args(QkArgs& a, const char* name, const gs_qk_shape* sh, const gs_qk_rows
       return fail(GS_ERR_DTYPE, n + ": weight dtypes must be bf16 or fp32");
   if (sh->B <= 0 || sh->T <= 0 || sh->D <= 0 || sh->n_rot < 0 || sh->n_rot > sh->D ||
       sh->n_rot % 2 != 0 || sh->heads[0] < 0 || sh->heads[1] < 0 || sh->heads[2] < 0 ||
-      sh->heads[0] + sh->heads[1] + sh->heads[2] <= 0 || !(sh->eps >= 0.f) ||
+      static_cast<int64_t>(sh->heads[0]) + sh->heads[1] + sh->heads[2] <= 0 || !(sh->eps >= 0.f) ||
       (sh->positions != nullptr && sh->position_bits != 32 && sh->position_bits != 64) ||
       (sh->n_rot > 0 && (sh->table == nullptr || sh->n_positions <= 0)))
     return fail(GS_ERR_INVALID, n + ": invalid arguments");
@@ -643,6 +643,8 @@ int qk_args(QkArgs& a, const char* name, const gs_qk_shape* sh, const gs_qk_rows
   if (static_cast<int64_t>(sh->heads[0]) + sh->heads[1] + sh->heads[2] > 65535 ||
       sh->B > INT32_MAX / sh->T)
     return fail(GS_ERR_UNSUPPORTED, n + ": more than 65535 heads or 2^31 tokens");
+  if (sh->n_rot > 0 && sh->positions == nullptr && sh->T > sh->n_positions)
+    return fail(GS_ERR_INVALID, n + ": more tokens to a sample than positions in the table");
   a = QkArgs{};
   for (int k = 0; k < 3; ++k) {
     a.heads[k] = sh->heads[k];

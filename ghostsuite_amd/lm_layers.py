@@ -95,8 +95,9 @@ def qkv_norm_rotary(qkv: torch.Tensor, n_head: int, n_kv_head: int, table: torch
     its root mean square (with ``norm``) and multiplied by q_weight / k_weight ([D], or None), then
     its first n_rot features are rotated: ``table`` is ``rotary_table``'s [positions, 2, n_rot / 2]
     (n_rot 0: no rotation), the pairs n_rot / 2 apart, or neighbours with ``interleaved``.
-    positions: None (0, 1, ... in each sample) or integers [T] or [B, T]; one outside the table
-    makes the rotated features NaN.  Formed in fp32, rounded once; D up to 512."""
+    positions: None (0, 1, ... in each sample; the table has to hold them) or integers [T] or
+    [B, T]; one of those outside the table makes the rotated features NaN.  Formed in fp32,
+    rounded once; D up to 512."""
     _check_norm(norm, q_weight, k_weight)
     q, k, v = ops().qk_norm_rotary(qkv, None, (n_head, n_kv_head, n_kv_head), table, positions,
                                    q_weight, k_weight, bool(norm), float(eps), bool(interleaved))
@@ -152,12 +153,13 @@ class QKNormRotary(nn.Module):
 
     def forward(self, qkv: torch.Tensor, positions: Optional[torch.Tensor] = None):
         sample_grads = None
-        if self.norm and hasattr(self.q_weight, "initially_requires_grad"):
+        if self.norm and self._backward_hooks and hasattr(self.q_weight, "initially_requires_grad"):
             # An engine's backward hook reads these: the positions, and each sample's gradients of
             # the weights, which the backward pass forms on its way (it runs before the hook when
             # the input has a gradient).
             if torch.is_grad_enabled() and qkv.requires_grad:
-                sample_grads = torch.empty(2, qkv.shape[0], self.head_dim, device=qkv.device)
+                sample_grads = torch.empty(2, qkv.shape[0], self.head_dim, device=qkv.device,
+                                           dtype=torch.float32)
             self.__dict__["_gs_positions"] = positions
             self.__dict__["_gs_sample_grads"] = sample_grads
         q, k, v = ops().qk_norm_rotary(

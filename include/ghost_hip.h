@@ -398,7 +398,7 @@ int gs_embedding_lookup(const void* ids, int ids_bits, int64_t n, const void* W,
  *      (2 i, 2 i + 1); the features past n_rot are u's
  * and a value row is copied.  Formed in fp32, rounded once to dtype.
  * table: [n_positions][2][n_rot / 2] fp32, each position's cosines then its sines.  positions:
- * NULL (token t of a sample is at position t), or integers of position_bits (32 or 64) bits at
+ * NULL (token t of a sample is at position t; T up to n_positions), or integers of position_bits (32 or 64) bits at
  * strides of position_stride_b and _t elements (0: shared); one outside the table gives NaN in
  * the rotated features. */
 typedef struct {

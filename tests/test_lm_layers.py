@@ -104,6 +104,7 @@ def _qk_rows(n=3):
     (dict(n_rot=63), -1), (dict(n_rot=66), -1), (dict(n_rot=-2), -1), (dict(heads=(0, 0, 0)), -1),
     (dict(heads=(-1, 1, 1)), -1), (dict(table=None), -1), (dict(n_positions=0), -1),
     (dict(positions=P16, position_bits=16), -1), (dict(eps=-1.0), -1), (dict(eps=math.nan), -1),
+    (dict(T=17), -1), (dict(heads=(0x7fffffff, 0x7fffffff, 2)), -5),
     (dict(D=513, n_rot=0), -5), (dict(heads=(65535, 1, 0)), -5),
     (dict(B=1 << 20, T=1 << 12), -5)])
 def test_qk_arguments_are_checked_on_the_host(changes, status):
@@ -411,6 +412,24 @@ def test_engine_dots_of_a_layer_without_input_gradient(oracle_ops):
     for (dot, grad), s in zip(got, (dq, dk)):
         assert_close(dot, s[:3] @ s[3:].sum(0), 1e-5)
         assert_close(grad, s[:3].sum(0) * 5 / 3, 1e-5)
+
+
+def test_sample_gradients_are_kept_in_fp32_and_only_under_an_engine(oracle_ops):
+    layer = gs.QKNormRotary(2, 1, 6, n_positions=16)
+    x = torch.randn(5, 4, 24, requires_grad=True)
+    eng = GradDotProdEngine(layer, val_batch_size=2, precision="fp32")
+    eng.attach(torch.optim.SGD(layer.parameters(), lr=0.0))
+    torch.set_default_dtype(torch.float64)
+    try:
+        y = layer(x)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert layer._gs_sample_grads.dtype == torch.float32
+    sum(t.sum() for t in y).backward()
+    assert layer.q_weight.grad_dot_prod.dtype == torch.float32
+    eng.detach()
+    layer(x)
+    assert "_gs_sample_grads" not in layer.__dict__
 
 
 def test_tied_scaled_embedding_keeps_both_parts(oracle_ops):
