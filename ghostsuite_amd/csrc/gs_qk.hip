@@ -11,12 +11,15 @@
 //   dw = sum h x r      dx = r (w h - x r mean(w h x r))
 //
 // Everything in fp32 registers, rounded once at the end; a row is read once and written once, so
-// the rate of a copy bounds both passes.  A row is cut into units of two chunks: for pairs half
-// the rotated width apart a unit holds chunk [V u, V u + V) of each half, for neighbouring pairs
-// 2 V features in a row, so that a pair's two features are always in one lane and only the row
-// sums cross lanes.  A group of 2^k lanes owns a row; it takes one token, keeps the token's
-// angles and the lane's weights in registers, and walks that token's heads, so the angles are
-// read once per token and the groups of a wave write neighbouring rows of one head.
+// the rate of a copy bounds both passes.  A row is cut into units of two chunks of V features: for
+// pairs half the rotated width apart a unit holds chunk u of each half, and likewise of the halves of
+// the features past them; for neighbouring pairs chunk u of each half of the row.  So a pair's two
+// features are always in one lane, only the row sums cross lanes, and the lanes of a load or store lie
+// side by side (both chunks in a row, 16 of every 32 bytes to a load, took 93 us for 89 in the forward
+// pass of 8 x 2048 tokens of 24 heads of 256, 64 of them turned).  A group of 2^k lanes owns a row; it
+// takes one token, keeps the token's angles and the lane's weights in registers, and walks that token's
+// heads, so the angles are read once per token and the groups of a wave write neighbouring rows of one
+// head.
 //
 // V is 16 bytes of features where the widths and strides allow it, else 2 or 1 features.
 //
@@ -45,8 +48,8 @@ struct QkArgs {
   QkRows x[3];       // layer input rows (forward and backward)
   QkRows g[3];       // forward: the outputs; backward: the output gradients (p may be null)
   QkRows dx[3];      // backward: input gradients (p null: not formed)
-  const void* w[2];  // query / key weights, or null: ones
-  int w_bf16[2];
+  const void* w[3];  // query / key weights, or null: ones (the values': null)
+  int w_bf16[3];
   int heads[3];
   int64_t B, T;      // samples and tokens of each
   int D, rot, lanes_log2;   // features, rotated features, log2 of the lanes of a row
@@ -54,12 +57,13 @@ struct QkArgs {
   float eps;
   const float* table;       // [positions][2][rot / 2]: cosines, sines
   int64_t n_pos;
+  int wide;                 // units' angles lie in whole vectors of V / 2
   const void* pos;          // null: a token's place in its sample
   int pos_bits;
   int64_t pos_sb, pos_st;
-  // The work of a workgroup: tokens [y * span, + span) of its segment (the segments: one of B T
-  // tokens, or B of T), heads [h0, h0 + per) of a part.
-  int64_t segments, seg_tokens, span, chunks;
+  // The work of a workgroup: heads [h0, h0 + per) of a part, and of its segment's tokens (the
+  // segments: one of B T tokens, or B of T) every chunks-th piece of as many as it has lane groups.
+  int64_t segments, seg_tokens, chunks;
   int groups[3], per[3];    // head groups of each part, heads of a group
   float* part[2];           // [segment][chunk][group][D] weight-gradient sums (backward)
 };
@@ -91,27 +95,28 @@ __device__ __forceinline__ QkChunk<E, V> qk_pack(const float (&x)[V]) {
   return c;
 }
 
-// Lane-local view of a row: unit j of this lane and its two chunks' places.
+// Unit u of a row: where its two chunks lie and which pairs' angles turn them.
 template <int V, bool INTER>
 struct QkPlace {
-  int o0, o1;     // first features of the chunks (>= D: nothing there)
-  int pair;       // first pair of the unit's angles (half: pairs [pair, pair + V))
+  int o0, o1;         // first features of the chunks (>= D: nothing there)
+  int pair0, pair1;   // pairs of angles [0, V / 2) and [V / 2, V) of the unit
   __device__ QkPlace(int u, int D, int rot) {
-    if (INTER) {
-      o0 = 2 * V * u;
-      o1 = o0 + V;
-      pair = V * u;
+    const int half = rot / 2, n = INTER ? 0 : half / V;   // V divides half
+    const int m = (D - 2 * V * n + 2 * V - 1) / (2 * V);  // units past the turned halves
+    if (INTER && V == 1) {
+      o0 = 2 * u;
+      o1 = o0 + 1;
+      pair0 = pair1 = u;
+    } else if (u < n) {
+      o0 = V * u;
+      o1 = half + o0;
+      pair0 = o0;
+      pair1 = pair0 + V / 2;
     } else {
-      const int half = rot / 2, nr = half / V;   // V divides half
-      if (u < nr) {
-        o0 = V * u;
-        o1 = half + V * u;
-        pair = V * u;
-      } else {
-        o0 = rot + 2 * V * (u - nr);
-        o1 = o0 + V;
-        pair = half;
-      }
+      o0 = u < n + m ? 2 * V * n + V * (u - n) : D;
+      o1 = o0 + V * m;
+      pair0 = INTER ? o0 / 2 : half;
+      pair1 = INTER ? o1 / 2 : half;
     }
     if (o0 >= D) o0 = D;
     if (o1 >= D) o1 = D;
@@ -187,42 +192,87 @@ __device__ __forceinline__ int64_t qk_position(const QkArgs& a, int64_t b, int64
 }
 
 // Cosines and sines of a unit's pairs at a position; those past the rotated features: 1 and 0; a
-// position outside the table: NaN.
+// position outside the table: NaN.  In whole vectors where the table's rows split there: 20 x 1024
+// tokens of 12 + 12 + 12 heads of 64, bf16, 16 loads of one number take 46.6 us forward, 4 of four 43.4.
 template <int V>
-__device__ __forceinline__ void qk_angles(const QkArgs& a, int64_t pos, int pair, float (&c)[V],
-                                          float (&s)[V]) {
+__device__ __forceinline__ void qk_angles(const QkArgs& a, int64_t pos, int pair0, int pair1,
+                                          float (&c)[V], float (&s)[V]) {
+  constexpr int H = V > 1 ? V / 2 : 1;
+  struct alignas(H * sizeof(float)) Angles { float f[H]; };
   const int half = a.rot / 2;
   const bool in = pos >= 0 && pos < a.n_pos;
   const float* row = a.table + (in ? pos : 0) * a.rot;
+  const float nan = __builtin_nanf("");
+  if (H > 1 && a.wide) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int pair = k ? pair1 : pair0;
+      const bool turns = pair < half;
+      Angles x, y;
+      if (turns) {
+        x = *reinterpret_cast<const Angles*>(row + pair);
+        y = *reinterpret_cast<const Angles*>(row + half + pair);
+      }
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        c[k * H + i] = turns ? (in ? x.f[i] : nan) : 1.f;
+        s[k * H + i] = turns ? (in ? y.f[i] : nan) : 0.f;
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const bool turns = pair + i < half;
-    c[i] = turns ? (in ? row[pair + i] : __builtin_nanf("")) : 1.f;
-    s[i] = turns ? (in ? row[half + pair + i] : __builtin_nanf("")) : 0.f;
+    const int pair = i < V / 2 ? pair0 + i : pair1 + i - V / 2;
+    const bool turns = pair < half;
+    c[i] = turns ? (in ? row[pair] : nan) : 1.f;
+    s[i] = turns ? (in ? row[half + pair] : nan) : 0.f;
   }
 }
 
-__device__ __forceinline__ float qk_weight(const QkArgs& a, int part, int f) {
-  if (a.w[part] == nullptr || f >= a.D) return 1.f;
-  return a.w_bf16[part] ? bf16_to_f32(static_cast<const uint16_t*>(a.w[part])[f])
-                        : static_cast<const float*>(a.w[part])[f];
+// V weights of a part from feature f on (ones past the row, or without weights).
+template <int V>
+__device__ __forceinline__ void qk_weights(const QkArgs& a, int part, int f, float (&w)[V]) {
+  const void* p = a.w[part];
+  if (p == nullptr || f >= a.D) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = 1.f;
+  } else if (a.w_bf16[part]) {
+    const QkChunk<uint16_t, V> x = qk_load<uint16_t, V>(static_cast<const uint16_t*>(p), f, a.D);
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = qk_elem<uint16_t, V>(x, i);
+  } else {
+    constexpr int N = V > 4 ? 4 : V;   // 16 bytes at most
+#pragma unroll
+    for (int k = 0; k < V; k += N) {
+      const QkChunk<float, N> x = qk_load<float, N>(static_cast<const float*>(p), f + k, a.D);
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[k + i] = qk_elem<float, N>(x, i);
+    }
+  }
 }
 
-// The workgroup's part, head range and token range.
+// The workgroup's part and heads, and the lane group's tokens.  Workgroups are numbered through the head
+// groups of a piece of tokens first, so that those at work at one time read and write near each other.
 struct QkBlock {
   int part, h0, h1, group;
-  int64_t seg, chunk, m0, m1;   // tokens [m0, m1), numbered over all samples
+  uint32_t seg, chunk;
+  uint32_t m0, m1, step;   // tokens m0, m0 + step, ... below m1, numbered over all samples (below 2^31)
   __device__ explicit QkBlock(const QkArgs& a) {
-    int y = blockIdx.y;
+    const uint32_t gy = a.groups[0] + a.groups[1] + a.groups[2], bx = blockIdx.x / gy;
+    int y = blockIdx.x - bx * gy;
     part = 0;
     while (part < 2 && y >= a.groups[part]) y -= a.groups[part++];
     group = y;
     h0 = y * a.per[part];
     h1 = min(a.heads[part], h0 + a.per[part]);
-    seg = blockIdx.x / a.chunks;
-    chunk = blockIdx.x - seg * a.chunks;
-    m0 = seg * a.seg_tokens + chunk * a.span;
-    m1 = min(m0 + a.span, (seg + 1) * a.seg_tokens);
+    const uint32_t chunks = static_cast<uint32_t>(a.chunks), slots = QK_THREADS >> a.lanes_log2;
+    seg = bx / chunks;
+    chunk = bx - seg * chunks;
+    m0 = seg * static_cast<uint32_t>(a.seg_tokens);
+    m1 = m0 + static_cast<uint32_t>(a.seg_tokens);
+    m0 += chunk * slots + (threadIdx.x >> a.lanes_log2);
+    step = chunks * slots;
   }
 };
 
@@ -230,32 +280,29 @@ template <class E, int V, int UPL, bool INTER>
 __global__ void __launch_bounds__(QK_THREADS) qk_forward_kernel(QkArgs a) {
   const QkBlock blk(a);
   const int lanes = 1 << a.lanes_log2;
-  const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x >> a.lanes_log2;
-  const int slots = QK_THREADS >> a.lanes_log2;
+  const int lane = threadIdx.x & (lanes - 1);
   const bool turn = blk.part < 2 && a.rot > 0, norm = blk.part < 2 && a.norm;
   QkUnit<V> w[UPL];
   if (norm) {
 #pragma unroll
     for (int j = 0; j < UPL; ++j) {
       const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        w[j].a[i] = qk_weight(a, blk.part, pl.o0 + i);
-        w[j].b[i] = qk_weight(a, blk.part, pl.o1 + i);
-      }
+      qk_weights<V>(a, blk.part, pl.o0, w[j].a);
+      qk_weights<V>(a, blk.part, pl.o1, w[j].b);
     }
   }
   const QkRows in = a.x[blk.part], out = a.g[blk.part];
   const float inv_d = 1.f / static_cast<float>(a.D);
-  for (int64_t m = blk.m0 + slot; m < blk.m1; m += slots) {
-    const int64_t b = m / a.T, t = m - b * a.T;
+  for (uint32_t m = blk.m0; m < blk.m1; m += blk.step) {
+    const uint32_t of = m / static_cast<uint32_t>(a.T);
+    const int64_t b = of, t = m - of * static_cast<uint32_t>(a.T);
     float c[UPL][V], s[UPL][V];
     if (turn) {
       const int64_t pos = qk_position(a, b, t);
 #pragma unroll
       for (int j = 0; j < UPL; ++j) {
         const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
-        qk_angles<V>(a, pos, pl.pair, c[j], s[j]);
+        qk_angles<V>(a, pos, pl.pair0, pl.pair1, c[j], s[j]);
       }
     }
     const E* xr = reinterpret_cast<const E*>(in.p) + b * in.sb + t * in.st;
@@ -309,8 +356,7 @@ template <class E, int V, int UPL, bool INTER>
 __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(QkArgs a) {
   const QkBlock blk(a);
   const int lanes = 1 << a.lanes_log2;
-  const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x >> a.lanes_log2;
-  const int slots = QK_THREADS >> a.lanes_log2;
+  const int lane = threadIdx.x & (lanes - 1);
   const QkRows in = a.x[blk.part], go = a.g[blk.part], dx = a.dx[blk.part];
   const bool any_g = go.p != nullptr;   // else every gradient of the part is zero
   const bool turn = blk.part < 2 && a.rot > 0 && any_g, norm = blk.part < 2 && a.norm && any_g;
@@ -319,23 +365,22 @@ __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(QkArgs a) {
 #pragma unroll
   for (int j = 0; j < UPL; ++j) {
     const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
+    qk_weights<V>(a, norm ? blk.part : 2, pl.o0, w[j].a);
+    qk_weights<V>(a, norm ? blk.part : 2, pl.o1, w[j].b);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      w[j].a[i] = norm ? qk_weight(a, blk.part, pl.o0 + i) : 1.f;
-      w[j].b[i] = norm ? qk_weight(a, blk.part, pl.o1 + i) : 1.f;
-      dw[j].a[i] = dw[j].b[i] = 0.f;
-    }
+    for (int i = 0; i < V; ++i) dw[j].a[i] = dw[j].b[i] = 0.f;
   }
   const float inv_d = 1.f / static_cast<float>(a.D);
-  for (int64_t m = blk.m0 + slot; m < blk.m1; m += slots) {
-    const int64_t b = m / a.T, t = m - b * a.T;
+  for (uint32_t m = blk.m0; m < blk.m1; m += blk.step) {
+    const uint32_t of = m / static_cast<uint32_t>(a.T);
+    const int64_t b = of, t = m - of * static_cast<uint32_t>(a.T);
     float c[UPL][V], s[UPL][V];
     if (turn) {
       const int64_t pos = qk_position(a, b, t);
 #pragma unroll
       for (int j = 0; j < UPL; ++j) {
         const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
-        qk_angles<V>(a, pos, pl.pair, c[j], s[j]);
+        qk_angles<V>(a, pos, pl.pair0, pl.pair1, c[j], s[j]);
       }
     }
     const E* xr = reinterpret_cast<const E*>(in.p) + b * in.sb + t * in.st;
@@ -524,6 +569,10 @@ int qk_vec(const QkArgs& a, size_t esz, bool inter, bool backward) {
   const int half = a.rot / 2;
   for (int v : {static_cast<int>(16 / esz), 2}) {
     bool ok = a.D % v == 0 && (inter || half % v == 0) && (inter || a.rot % v == 0);
+    for (int k = 0; k < 2 && ok; ++k)   // weights are read in chunks of 16 bytes at most
+      ok = a.w[k] == nullptr || a.heads[k] == 0 ||
+           reinterpret_cast<uintptr_t>(a.w[k]) %
+                   std::min<size_t>(16, v * (a.w_bf16[k] ? 2 : 4)) == 0;
     for (int k = 0; k < 3 && ok; ++k) {
       if (a.heads[k] == 0) continue;
       for (const QkRows* r : {&a.x[k], &a.g[k], &a.dx[k]}) {
@@ -549,42 +598,55 @@ int ceil_log2(int64_t x) {
   return k;
 }
 
-// How the work is shared out: into about QK_WAVES waves (3 for each SIMD, what the backward kernel's
-// registers let stay there at once) while the work lasts, by head groups first and longer token spans
-// after.  Fewer, longer walks reuse the angles and add more into a lane before the workgroup's sum.
-// Per-sample sums cut the spans at samples.  Measured on MI355X with 32, 16, 8, 4, 3 and 2 waves for
-// each SIMD (forward / backward, us): 20 x 1024 tokens of 12 + 12 + 12 heads of 64, bf16, 56 / 95,
-// 46 / 77, 39 / 64, 34 / 57, 34 / 56, 34 / 56; 8 x 2048 of 8 + 8 + 8 of 256, 110 / 169, 106 / 149,
-// 98 / 133, 98 / 138, 95 / 135, 103 / 137.
-constexpr int64_t QK_WAVES = 3 * 4 * 256;
-void qk_share(QkArgs& a, int upl, int units, bool per_sample) {
+// How the work is shared out.  Backward into the waves whose registers fit at once (3 for each SIMD; a
+// wave's end, its sum of weight gradients, costs more than its start), forward into 16 for each SIMD.
+// Few heads to a workgroup give many workgroups to a token, which then read its row together; a few
+// heads share the angles: 4 forward; backward, of 4, 6 and 3, the number that leaves the fewest turns, a
+// turn costing its heads and half of one more for the angles; fewer where two workgroups to a CU would
+// not be reached.  Measured on MI355X, two inputs in turn (forward / both passes, us), with tokens in
+// ranges of their own, part after part, 3 waves a SIMD -> this: 20 x 1024 tokens of 12 + 12 + 12 heads
+// of 64, bf16, 42.5 / 107 -> 37.5 / 104; 8 x 2048 of 8 + 8 + 8 of 256, 64 turned, 93 / 226 -> 79 / 190;
+// 20 x 512 of 16 + 4 + 4 of 128, 23.5 / 71 -> 24 / 71, fp32 54 / 158 -> 44.5 / 125 (copies of the forward
+// pass's bytes: 35, 76, 20 in bf16).
+constexpr int64_t QK_FORWARD_GROUPS = 16 * 256, QK_BACKWARD_GROUPS = 3 * 256;   // workgroups of 4 waves
+constexpr int64_t QK_FEW_GROUPS = 2 * 256;
+constexpr int64_t QK_MAX_GROUPS = int64_t{1} << 22;   // of a launch: below 2^32 threads
+void qk_share(QkArgs& a, int upl, int units, bool per_sample, bool backward) {
   a.lanes_log2 = std::min(6, ceil_log2((units + upl - 1) / upl));
   const int64_t slots = QK_THREADS >> a.lanes_log2;
   a.segments = per_sample ? a.B : 1;
   a.seg_tokens = per_sample ? a.T : a.B * a.T;
-  a.span = std::min<int64_t>(slots, a.seg_tokens);
-  a.chunks = (a.seg_tokens + a.span - 1) / a.span;
-  const int total = a.heads[0] + a.heads[1] + a.heads[2];
-  const int64_t want = std::max<int64_t>(1, QK_WAVES / (QK_THREADS / 64));
-  // groups of heads for the workgroups wanted, at least one head each
-  const int64_t y = std::max<int64_t>(1, std::min<int64_t>(total, want / (a.segments * a.chunks)));
-  const int per = static_cast<int>((total + y - 1) / y);
+  const int64_t pieces = (a.seg_tokens + slots - 1) / slots;
+  const int64_t want = backward ? QK_BACKWARD_GROUPS : QK_FORWARD_GROUPS;
+  const auto groups = [&](int per) {
+    int64_t y = 0;
+    for (int k = 0; k < 3; ++k) y += (a.heads[k] + per - 1) / per;
+    return y;
+  };
+  const auto chunks = [&](int per) {
+    return std::max<int64_t>(1, std::min(pieces, want / (a.segments * groups(per))));
+  };
+  const auto turns = [&](int per) {
+    const int64_t c = chunks(per), n = a.segments * c * groups(per);
+    return (pieces + c - 1) / c * ((n + want - 1) / want);
+  };
+  int per = 4;
+  for (int p : {6, 3})
+    if (backward && turns(p) * (2 * p + 1) < turns(per) * (2 * per + 1)) per = p;
+  while (per > 1 && a.segments * chunks(per) * groups(per) < QK_FEW_GROUPS) --per;
+  if (a.segments * groups(per) > QK_MAX_GROUPS) per = std::max({a.heads[0], a.heads[1], a.heads[2]});
   for (int k = 0; k < 3; ++k) {
     a.groups[k] = (a.heads[k] + per - 1) / per;
     a.per[k] = a.groups[k] ? (a.heads[k] + a.groups[k] - 1) / a.groups[k] : 1;
   }
-  // more tokens to a workgroup where that still leaves enough of them
-  const int64_t gy = a.groups[0] + a.groups[1] + a.groups[2];
-  const int64_t times = std::max<int64_t>(1, a.segments * a.chunks * gy / want);
-  a.span = std::min<int64_t>(a.span * times, a.seg_tokens);
-  a.chunks = (a.seg_tokens + a.span - 1) / a.span;
+  a.chunks = chunks(per);
 }
 
 template <class E, bool BWD, bool INTER>
 int qk_launch(const QkArgs& a, int v, hipStream_t s) {
   constexpr int V16 = 16 / sizeof(E);
-  const dim3 grid(static_cast<unsigned>(a.segments * a.chunks),
-                  static_cast<unsigned>(a.groups[0] + a.groups[1] + a.groups[2]));
+  const dim3 grid(static_cast<unsigned>(a.segments * a.chunks *
+                                        (a.groups[0] + a.groups[1] + a.groups[2])));
 #define GS_QK_GO(V, UPL)                                                                       \
   do {                                                                                         \
     if constexpr (BWD)                                                                         \
@@ -674,7 +736,9 @@ QkPlan qk_plan(QkArgs& a, int dtype, bool inter, bool backward, bool per_sample,
   QkPlan p;
   const size_t esz = elem_size(dtype);
   p.v = force_v ? force_v : qk_vec(a, esz, inter, backward);
-  qk_share(a, qk_units_per_lane(p.v, esz), qk_units(a.D, a.rot, p.v, inter), per_sample);
+  a.wide = p.v > 2 && a.rot / 2 % (p.v / 2) == 0 &&
+           reinterpret_cast<uintptr_t>(a.table) % (p.v / 2 * sizeof(float)) == 0;
+  qk_share(a, qk_units_per_lane(p.v, esz), qk_units(a.D, a.rot, p.v, inter), per_sample, backward);
   for (int k = 0; k < 2; ++k) p.rows[k] = a.chunks * a.groups[k];
   return p;
 }
