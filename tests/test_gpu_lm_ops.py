@@ -538,6 +538,17 @@ def test_distill_options(gpu, tau, alpha, reduction, upstream):
         check_distill(gpu, z, ids, t, None, tau, alpha, reduction, upstream)
 
 
+@pytest.mark.parametrize("N", [63, 64, 65, 256, 257, 600])
+@pytest.mark.parametrize("upstream", [None, -0.5])
+def test_distill_mean_over_the_rows_that_count(gpu, N, upstream):
+    """The rows are counted in two ways, by their number; from none ignored to all but one."""
+    z, ids, t, labels = distill_inputs(N, 37, 3, N, FP32)
+    for kept in (N, N // 2, 1):
+        labels[kept:] = -100
+        order = torch.randperm(N, generator=gen(kept))
+        check_distill(gpu, z, ids, t, labels[order], 2.0, 0.5, "mean", upstream)
+
+
 def test_distill_per_row_upstream_and_other_ignore_index(gpu):
     z, ids, t, labels = distill_inputs(6, 301, 4, 6, FP32)
     labels[1] = 7
