@@ -216,7 +216,8 @@ def qk_inputs(gpu, B, T, heads, D, dtype, seed, w_dtype=None):
     (3, 17, (2, 2, 2), 256, 64), (2, 9, (5, 1, 1), 80, 20), (2, 33, (1, 1, 1), 33, 32),
     (1, 3, (2, 1, 1), 1, 0), (2, 4, (2, 1, 1), 2, 2), (2, 7, (3, 3, 3), 48, 0),
     (1, 300, (2, 1, 1), 20, 6), (2, 5, (2, 1, 1), 512, 512), (1, 4, (2, 1, 1), 511, 302),
-    (1, 6, (2, 1, 1), 100, 50), (4, 260, (12, 12, 12), 64, 64), (2, 40, (9, 3, 3), 96, 94)])
+    (1, 6, (2, 1, 1), 100, 50), (4, 260, (12, 12, 12), 64, 64), (2, 40, (9, 3, 3), 96, 94),
+    (1, 20011, (3, 1, 1), 64, 32), (2, 9001, (2, 7, 7), 128, 128)])
 def test_qkv_shapes(gpu, dtype, interleaved, B, T, heads, D, n_rot):
     plan = L.plan(heads, gs.rotary_table(T + 3, n_rot, device=gpu), interleaved=interleaved)
     x, qw, kw, grads = qk_inputs(gpu, B, T, heads, D, dtype, 11)
@@ -234,6 +235,21 @@ def test_qk_weights_of_another_dtype_and_none(gpu, dtype, w_dtype):
     y = gs.qkv_norm_rotary(x, 4, 2, plan["table"], None, qw, None)   # one weight only
     got = torch.autograd.grad(y, (x, qw), grads)
     assert all(g.isfinite().all() for g in got)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("off", [1, 2, 3, 4, 8])
+def test_qk_table_and_weights_off_16_byte_boundaries(gpu, dtype, interleaved, off):
+    def moved(t):
+        return torch.cat((t.new_zeros(off), t.detach().flatten()))[off:].view(t.shape)
+
+    heads = (2, 1, 1)
+    x, qw, kw, grads = qk_inputs(gpu, 2, 5, heads, 64, dtype, 31)
+    plan = L.plan(heads, moved(gs.rotary_table(9, 64, device=gpu)), interleaved=interleaved)
+    check_qk(gpu, plan, (x,), qw, kw, grads)
+    plan = L.plan(heads, gs.rotary_table(9, 64, device=gpu), interleaved=interleaved)
+    check_qk(gpu, plan, (x,), moved(qw).requires_grad_(), moved(kw).requires_grad_(), grads)
 
 
 @pytest.mark.parametrize("pos_dtype", [torch.int32, torch.int64])
@@ -377,7 +393,8 @@ def test_qk_beyond_32_bit_offsets(gpu):
 @pytest.mark.parametrize("B,n_val,T,heads,D,n_rot,val_start", [
     (2, 1, 1, (1, 1, 1), 64, 64, None), (5, 2, 33, (4, 1, 1), 128, 64, None),
     (7, 3, 300, (2, 2, 2), 80, 20, 0), (6, 1, 9, (3, 3, 3), 33, 10, 2),
-    (40, 30, 3, (2, 1, 1), 48, 48, 5)])
+    (40, 30, 3, (2, 1, 1), 48, 48, 5), (3, 1, 7001, (5, 1, 1), 64, 32, None),
+    (65533, 2, 1, (260, 1, 1), 2, 2, None)])
 def test_qk_dots(gpu, dtype, B, n_val, T, heads, D, n_rot, val_start):
     plan = L.plan(heads, gs.rotary_table(T, n_rot, device=gpu))
     x, qw, kw, grads = qk_inputs(gpu, B, T, heads, D, dtype, 71)
