@@ -58,6 +58,19 @@ def test_lookup_and_gradient(gpu, dtype, shape, vocab, d):
     check_lookup(ids, randn((vocab, d), 1, 1.0, dtype), math.sqrt(d), None, gpu, 5)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("d", [1, 3, 4, 5, 7, 8, 9, 15, 16, 17, 31, 33, 100, 257])
+@pytest.mark.parametrize("off", [0, 1, 2, 4])
+def test_lookup_rows_off_16_byte_boundaries(gpu, dtype, d, off):
+    """Every width around a piece, the table at other places than allocations start at."""
+    w = randn((off + 19 * d,), d, 1.0, dtype).to(gpu)[off:].view(19, d)
+    for n in (1, 2, 37, 700):
+        ids = torch.randint(-1, 20, (n,), generator=gen(n))
+        y = gs.embedding_lookup(ids.to(gpu), w, 1.5)
+        want = torch.where(((ids >= 0) & (ids < 19))[:, None], f64(w)[ids.clamp(0, 18)] * 1.5, 0.0)
+        within(y, want, want.abs() * (HALF[dtype] + U), "rows")
+
+
 @pytest.mark.parametrize("id_dtype", [torch.int32, torch.int64])
 @pytest.mark.parametrize("padding_idx", [None, 0, 3, -1])
 def test_lookup_padding_strides_and_ids_outside(gpu, id_dtype, padding_idx):
@@ -102,17 +115,15 @@ def test_lookup_beyond_32_bit_offsets(gpu):
 
 
 def test_lookup_of_more_pieces_than_a_launch_has_threads(gpu):
-    """Single elements, 2^34 and more of them: several launches."""
-    d, n = 4097, (1 << 22) + 5
+    """Rows shorter than 16 bytes: 2^33 single elements and more, in several launches."""
+    d, n = 7, (1 << 33) // 7 + 5
     w = randn((3, d), 1, 1.0, BF16).to(gpu)
-    ids = (torch.arange(n, device=gpu) % 4)            # 3: outside
+    ids = torch.arange(n, dtype=torch.int32, device=gpu) % 4     # 3: outside
     y = gs.embedding_lookup(ids, w, 1.0)
-    assert y.numel() > 1 << 34
+    assert y.numel() > 1 << 33
     rows = torch.cat((w, torch.zeros_like(w[:1])))
-    for i in range(0, n, 1 << 20):
-        part = y[i:i + 1024]
-        assert torch.equal(part, rows[ids[i:i + 1024]])
-    assert torch.equal(y[-9:], rows[ids[-9:]])
+    for i in [*range(0, n, n // 9), n - 1000]:
+        assert torch.equal(y[i:i + 1000], rows[ids[i:i + 1000].long()])
 
 
 # ------------------------------------------------------------ norms, rotation, heads first
