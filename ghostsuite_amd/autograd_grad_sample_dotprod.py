@@ -106,10 +106,11 @@ def _prepare_sample_grad_or_dotprod(layer: nn.Module, grad_output: Tuple[torch.T
     d = layer.__dict__
     others = ()
     if isinstance(layer, QKNormRotary):   # three outputs, any of which may have no gradient
-        d["_gs_grad_outputs"] = others = tuple(None if g is None else g.detach()
-                                               for g in grad_output)
-        others += (d.get("_gs_positions"), d.get("_gs_sample_grads"))
-        backprops = next(g for g in others if g is not None)
+        backprops = next(g for g in grad_output if g is not None).detach()
+        if d.get("_gs_sample_grads") is None:   # else the output gradients have been used
+            d["_gs_grad_outputs"] = others = tuple(None if g is None else g.detach()
+                                                   for g in grad_output)
+            others += (d.get("_gs_positions"),)
     else:
         backprops = grad_output[0].detach()
     d.setdefault("activations", None)
