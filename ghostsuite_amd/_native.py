@@ -104,6 +104,8 @@ _SIGNATURES = {
                                 _I, _F, _P, _SZ, _P]),
     "gs_ordered_sum": (_I, [_P, _P, _I, _I64, _P, _I, _P]),
     "gs_embedding_lookup": (_I, [_P, _I, _I64, _P, _I, _I64, _I64, _F, _I64, _P, _P, _P]),
+    "gs_embedding_lookup_grad_workspace": (_SZ, [_I64, _I64, _I64]),
+    "gs_embedding_lookup_grad": (_I, [_P, _P, _I, _I64, _I64, _I64, _F, _P, _P, _SZ, _P]),
     "gs_qk_rotary": (_I, [_P, _P, _P, _P]),
     "gs_qk_rotary_grad_workspace": (_SZ, [_P, _I]),
     "gs_qk_rotary_grad": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
@@ -794,7 +796,7 @@ class HipOps:
 
     def embedding_lookup(self, ids: torch.Tensor, weight: torch.Tensor, scale: float,
                          padding_idx: Optional[int] = None) -> torch.Tensor:
-        """scale * weight[ids] (gs_embedding_lookup; its gradient gs_embedding_train_grad)."""
+        """scale * weight[ids] (gs_embedding_lookup; its gradient gs_embedding_lookup_grad)."""
         return _lm().embedding_lookup(ids, weight, scale, padding_idx)
 
     def qk_norm_rotary(self, q: torch.Tensor, k: Optional[torch.Tensor], heads, table, positions, qw,

@@ -3,8 +3,8 @@
 //   out[i] = scale * W[id_i]        out: [n, d], W: [vocab, d]
 //
 // formed in fp32 and rounded once to W's dtype; ids outside [0, vocab) give rows of zeros.  For
-// the gradient (gs_embedding_train_grad over the same ids) the pass also writes the ids as the
-// gradient takes them: 64-bit, the padding id replaced by -1.
+// the gradient (for few tokens the second kernel below, else gs_embedding_train_grad over the same
+// ids) the pass also writes the ids as the gradient takes them: 64-bit, the padding id replaced by -1.
 //
 // Nothing is computed twice and every byte moves once, so the rate of a copy bounds it.  Each thread
 // owns pieces of 16 bytes of the output: they are numbered through the whole output, so all lanes work
@@ -13,6 +13,7 @@
 // (element by element 24432 rows of 515 fp32 features took 26.9 us for 18.0, bf16 25.7 for 12.1).
 // 16384 rows of 768 bf16: 9.1 us, 5.5 TB/s read and written.
 #include <algorithm>
+#include <type_traits>
 
 #include "gs_common.h"
 
@@ -102,10 +103,120 @@ int launch_lookup_any(const void* ids, int ids32, int64_t n, const void* W, int6
   return launch_lookup<E, 1, A>(ids, ids32, n, W, vocab, d, scale, padding, out, grad_ids, s);
 }
 
+// A piece as it came, unpacked where it is used.
+template <class E, int V>
+struct LkRaw {
+  std::conditional_t<(V * sizeof(E) >= 4), uint32_t, uint16_t> w[V > 1 ? 4 : 1];
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (sizeof(E) == 4) return __uint_as_float(w[e]);
+    else if constexpr (V == 1) return bf16_to_f32(w[0]);
+    else return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+  }
+};
+
+// The gradient of few tokens in one launch: a wave owns 16 rows of the table, looks at all the ids (kept
+// one to a lane), and sums each row's tokens in order in fp32; most rows are written as zeros, which bounds
+// it.  Nothing is sorted, and no wave waits for another.  Lookup and gradient, 768 features in bf16, 64
+// tokens of 1000 ids spread / all one id, then of 50257 (us; in brackets by the sorted list): 18 (24) /
+// 22 (23), 20 (34) / 29 (34), and three launches less for the host, 30 -> 24 us a pass; of 128 tokens
+// 27 (25) / 34 (23), 24 (35) / 43 (33).
+constexpr int LK_FEW = 64, LK_ROWS = 16, LK_BATCH = 8;   // tokens; rows of a wave; loads in flight
+template <class E, int V, int ALIGN>
+__global__ void __launch_bounds__(LK_THREADS) lookup_few_grad_kernel(
+    const int64_t* __restrict__ ids, int n, const E* __restrict__ G, int64_t vocab, int64_t d,
+    float scale, E* __restrict__ grad) {
+  static_assert(LK_FEW == 64, "a lane for every token");
+  struct alignas(ALIGN) Piece { E e[V]; };
+  const int lane = threadIdx.x & 63;
+  const int64_t v0 =
+      (static_cast<int64_t>(blockIdx.x) * (LK_THREADS / 64) + (threadIdx.x >> 6)) * LK_ROWS;
+  // the lane's token's row among the wave's (any other number: not among them)
+  const uint64_t row =
+      lane < n ? static_cast<uint64_t>(ids[lane]) - static_cast<uint64_t>(v0) : ~uint64_t{0};
+  for (int r = 0; r < LK_ROWS && v0 + r < vocab; ++r) {
+    const unsigned long long mine = __ballot(row == static_cast<uint64_t>(r));
+    E* out = grad + (v0 + r) * d;
+    for (int64_t f0 = static_cast<int64_t>(lane) * V; f0 < d; f0 += 64 * V) {
+      const int64_t f = min(f0, d - V);   // a row's last piece ends with the row
+      float acc[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] = 0.f;
+      for (unsigned long long left = mine; left != 0;) {   // the same for the whole wave
+        // all loads are made (past the last token its row again), so that none waits for another
+        LkRaw<E, V> x[LK_BATCH];
+        const int count = min(LK_BATCH, __popcll(left));
+        int token = 0;
+#pragma unroll
+        for (int q = 0; q < LK_BATCH; ++q) {
+          token = left != 0 ? __builtin_ctzll(left) : token;
+          left &= left - 1;
+          __builtin_memcpy(&x[q], reinterpret_cast<const Piece*>(G + token * d + f), sizeof(Piece));
+        }
+#pragma unroll
+        for (int q = 0; q < LK_BATCH; ++q)
+          if (q < count) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] += x[q].get(e);
+          }
+      }
+      Piece o;
+#pragma unroll
+      for (int e = 0; e < V; ++e) o.e[e] = from_f32<E>(scale * acc[e]);
+      *reinterpret_cast<Piece*>(out + f) = o;
+    }
+  }
+}
+
+template <class E>
+int launch_few_grad(const int64_t* ids, int64_t n, const void* G, int64_t vocab, int64_t d,
+                    float scale, void* grad, hipStream_t s) {
+  constexpr int V = 16 / sizeof(E), A = sizeof(E);
+  constexpr int64_t rows = LK_ROWS * (LK_THREADS / 64);
+  const dim3 grid(static_cast<unsigned>((vocab + rows - 1) / rows));
+  const E* g = static_cast<const E*>(G);
+  E* out = static_cast<E*>(grad);
+  const int m = static_cast<int>(n);
+  if (d % V == 0 && reinterpret_cast<uintptr_t>(G) % 16 == 0 &&
+      reinterpret_cast<uintptr_t>(grad) % 16 == 0)
+    hipLaunchKernelGGL((lookup_few_grad_kernel<E, V, 16>), grid, dim3(LK_THREADS), 0, s, ids, m, g,
+                       vocab, d, scale, out);
+  else if (d >= V)
+    hipLaunchKernelGGL((lookup_few_grad_kernel<E, V, A>), grid, dim3(LK_THREADS), 0, s, ids, m, g,
+                       vocab, d, scale, out);
+  else
+    hipLaunchKernelGGL((lookup_few_grad_kernel<E, 1, A>), grid, dim3(LK_THREADS), 0, s, ids, m, g,
+                       vocab, d, scale, out);
+  return check_launch("lookup_few_grad_kernel");
+}
+
+bool lookup_is_few(int64_t n, int64_t vocab) {
+  return n <= LK_FEW && vocab <= LK_MAX_BLOCKS * LK_ROWS;
+}
+
 }  // namespace
 }  // namespace gs
 
 using namespace gs;
+
+extern "C" size_t gs_embedding_lookup_grad_workspace(int64_t n, int64_t vocab, int64_t d) {
+  return n > 0 && lookup_is_few(n, vocab) ? 0
+                                          : gs_embedding_train_grad_workspace(1, 0, n, d, vocab);
+}
+
+extern "C" int gs_embedding_lookup_grad(const int64_t* ids, const void* G, int dtype, int64_t n,
+                                        int64_t vocab, int64_t d, float scale, void* grad,
+                                        void* workspace, size_t workspace_bytes, void* stream) {
+  if (dtype != GS_DTYPE_BF16 && dtype != GS_DTYPE_F32)
+    return fail(GS_ERR_DTYPE, "gs_embedding_lookup_grad: dtype must be bf16 or fp32");
+  if (ids == nullptr || G == nullptr || grad == nullptr || n <= 0 || vocab <= 0 || d <= 0)
+    return fail(GS_ERR_INVALID, "gs_embedding_lookup_grad: invalid arguments");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!lookup_is_few(n, vocab))   // one sample of all the tokens, none of them for validation
+    return gs_embedding_train_grad(ids, G, dtype, 1, 0, 1, n, d, vocab, scale, grad, dtype, 0,
+                                   workspace, workspace_bytes, stream);
+  return dtype == GS_DTYPE_BF16 ? launch_few_grad<uint16_t>(ids, n, G, vocab, d, scale, grad, s)
+                                : launch_few_grad<float>(ids, n, G, vocab, d, scale, grad, s);
+}
 
 extern "C" int gs_embedding_lookup(const void* ids, int ids_bits, int64_t n, const void* W,
                                    int dtype, int64_t vocab, int64_t d, float scale,

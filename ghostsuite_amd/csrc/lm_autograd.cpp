@@ -1,5 +1,5 @@
 // Host side of the language-model operators: argument checks, allocation and automatic
-// differentiation around gs_embedding_lookup, gs_embedding_train_grad, gs_qk_rotary* and gs_distill_*
+// differentiation around gs_embedding_lookup*, gs_qk_rotary* and gs_distill_*
 // (include/ghost_hip.h), as a Python extension module.
 //
 // C++ because a training step calls these in every layer: a Python autograd function costs the host
@@ -166,16 +166,17 @@ Tensor lookup_grad(const Tensor& ids, const Tensor& g_in, const LookupHow& how) 
   const auto options = g_in.options().dtype(how.dtype).requires_grad(false);
   const int64_t n = ids.numel(), vocab = how.table[0], d = how.table[1];
   if (n == 0) return at::zeros(how.table, options);
+  require(g_in.scalar_type() == how.dtype, "output gradient of dtype ", g_in.scalar_type(), ", table of ",
+          how.dtype);
   const Tensor g = g_in.contiguous(), out = at::empty(how.table, options);
-  const int dt = gs_dtype_of(g, "output gradient"), odt = gs_dtype_of(out, "embedding weight");
-  // one sample of all the tokens, none of them for validation
-  const size_t bytes = gs_embedding_train_grad_workspace(1, 0, n, d, vocab);
-  const Tensor ws = scratch(bytes, g);
+  const size_t bytes = gs_embedding_lookup_grad_workspace(n, vocab, d);
+  Tensor ws;
+  if (bytes > 0) ws = scratch(bytes, g);
   c10::DeviceGuard guard(dev);
-  check(gs_embedding_train_grad(static_cast<const int64_t*>(ptr(ids)), ptr(g), dt, 1, 0, 1, n, d,
-                                vocab, static_cast<float>(how.scale), mut(out), odt, 0, mut(ws), bytes,
-                                stream_on(dev)),
-        "gs_embedding_train_grad");
+  check(gs_embedding_lookup_grad(static_cast<const int64_t*>(ptr(ids)), ptr(g),
+                                 gs_dtype_of(g, "output gradient"), n, vocab, d,
+                                 static_cast<float>(how.scale), mut(out), mut(ws), bytes, stream_on(dev)),
+        "gs_embedding_lookup_grad");
   return out;
 }
 

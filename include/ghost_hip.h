@@ -381,12 +381,20 @@ int gs_ordered_sum(const void* const* srcs, const int* dtypes, int count, int64_
  * The forward of an embedding layer (no counterpart among the reference's samplers):
  *   out[i] = scale * W[ids[i]], formed in fp32, rounded once to dtype    out: [n, d]
  * ids: n token ids of ids_bits (32 or 64) bits; those outside [0, vocab) give rows of zeros.
- * W: [vocab, d] (dtype).  grad_ids: NULL, or [n] int64 = ids as gs_embedding_train_grad takes
- * them for this layer's gradient (with scale there): padding_idx replaced by -1, which takes no
- * part (padding_idx < 0: no such id).  No workspace. */
+ * W: [vocab, d] (dtype).  grad_ids: NULL, or [n] int64 = ids as gs_embedding_lookup_grad takes
+ * them: padding_idx replaced by -1, which takes no part (padding_idx < 0: no such id).  No
+ * workspace. */
 int gs_embedding_lookup(const void* ids, int ids_bits, int64_t n, const void* W, int dtype,
                         int64_t vocab, int64_t d, float scale, int64_t padding_idx, void* out,
                         int64_t* grad_ids, void* stream);
+
+/* Its gradient: grad[v] = scale * the sum of G's rows whose id is v, in fp32 in a fixed order,
+ * rounded once; zeros where there is none.  ids: [n] int64, those outside [0, vocab) take no
+ * part.  G: [n, d], grad: [vocab, d], both of dtype.  A workspace of 0 bytes may be NULL. */
+size_t gs_embedding_lookup_grad_workspace(int64_t n, int64_t vocab, int64_t d);
+int gs_embedding_lookup_grad(const int64_t* ids, const void* G, int dtype, int64_t n,
+                             int64_t vocab, int64_t d, float scale, void* grad, void* workspace,
+                             size_t workspace_bytes, void* stream);
 
 /* ---- Per-head norms of queries and keys with their rotation ------------------------------
  * The attention prologue (no counterpart among the reference's samplers).  Three parts -- 0

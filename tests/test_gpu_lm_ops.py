@@ -71,6 +71,20 @@ def test_lookup_rows_off_16_byte_boundaries(gpu, dtype, d, off):
         within(y, want, want.abs() * (HALF[dtype] + U), "rows")
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("n", [2, 63, 64, 65, 513])
+@pytest.mark.parametrize("d", [3, 64, 333])
+@pytest.mark.parametrize("ids", ["all", "one", "few", "outside"])
+def test_lookup_gradient_around_its_two_ways(gpu, dtype, n, d, ids):
+    """Up to 64 tokens are summed without a sort: ids spread, all the same, a dozen, or extreme."""
+    vocab = 1003
+    x = {"all": torch.randint(0, vocab, (n,), generator=gen(n)), "one": torch.full((n,), vocab - 1),
+         "few": torch.randint(0, 12, (n,), generator=gen(n)) * 90,
+         "outside": torch.tensor([0, -1, vocab, 2 ** 63 - 1, -2 ** 63, 7, 2 ** 32 + 7]).repeat(
+             n // 7 + 1)[:n]}[ids]
+    check_lookup(x, randn((vocab, d), 1, 1.0, dtype), 1.7, None, gpu, n + d)
+
+
 @pytest.mark.parametrize("id_dtype", [torch.int32, torch.int64])
 @pytest.mark.parametrize("padding_idx", [None, 0, 3, -1])
 def test_lookup_padding_strides_and_ids_outside(gpu, id_dtype, padding_idx):
