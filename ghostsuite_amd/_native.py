@@ -109,7 +109,7 @@ _SIGNATURES = {
     "gs_qk_rotary": (_I, [_P, _P, _P, _P]),
     "gs_qk_rotary_grad_workspace": (_SZ, [_P, _I]),
     "gs_qk_rotary_grad": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
-    "gs_qk_sample_dots_workspace": (_SZ, [_I64]),
+    "gs_qk_sample_dots_workspace": (_SZ, [_I64, _I64]),
     "gs_qk_sample_dots": (_I, [_P, _I64, _I64, _I64, _I64, _P, _P, _P, _I, _P, _I, _F, _P, _SZ,
                                _P]),
     "gs_qk_rotary_dots_workspace": (_SZ, [_P]),

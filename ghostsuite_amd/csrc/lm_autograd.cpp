@@ -470,8 +470,9 @@ std::vector<OptTensor> qk_sample_dots(const Tensor& samples, const Tensor& qw, c
     dw[0] = at::empty({D}, qw.options().requires_grad(false));
     dw[1] = at::empty({D}, kw.options().requires_grad(false));
   }
-  const size_t bytes = gs_qk_sample_dots_workspace(D);
-  const Tensor ws = scratch(bytes, samples);
+  const size_t bytes = gs_qk_sample_dots_workspace(B, D);
+  Tensor ws;
+  if (bytes > 0) ws = scratch(bytes, samples);
   c10::DeviceGuard guard(dev);
   check(gs_qk_sample_dots(static_cast<const float*>(ptr(samples)), B, D, n_val,
                           val_start.value_or(n_train), static_cast<float*>(mut(dots[0])),

@@ -455,8 +455,8 @@ int gs_qk_rotary_dots(const gs_qk_shape* shape, const gs_qk_rows x[3], const gs_
                       size_t workspace_bytes, void* stream);
 
 /* The same from the sample_grads of gs_qk_rotary_grad, where the layer's backward pass formed them
- * beside its input gradients. */
-size_t gs_qk_sample_dots_workspace(int64_t D);
+ * beside its input gradients.  A workspace of 0 bytes may be NULL. */
+size_t gs_qk_sample_dots_workspace(int64_t B, int64_t D);
 int gs_qk_sample_dots(const float* sample_grads, int64_t B, int64_t D, int64_t n_val,
                       int64_t val_start, float* out_dot_q, float* out_dot_k, void* out_grad_q,
                       int grad_q_dtype, void* out_grad_k, int grad_k_dtype, float grad_scale,

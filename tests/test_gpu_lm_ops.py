@@ -419,7 +419,8 @@ def test_qk_beyond_32_bit_offsets(gpu):
     (2, 1, 1, (1, 1, 1), 64, 64, None), (5, 2, 33, (4, 1, 1), 128, 64, None),
     (7, 3, 300, (2, 2, 2), 80, 20, 0), (6, 1, 9, (3, 3, 3), 33, 10, 2),
     (40, 30, 3, (2, 1, 1), 48, 48, 5), (3, 1, 7001, (5, 1, 1), 64, 32, None),
-    (65533, 2, 1, (260, 1, 1), 2, 2, None)])
+    (65533, 2, 1, (260, 1, 1), 2, 2, None), (128, 100, 2, (2, 1, 1), 70, 70, 20),
+    (129, 3, 2, (2, 1, 1), 130, 8, 64)])
 def test_qk_dots(gpu, dtype, B, n_val, T, heads, D, n_rot, val_start):
     plan = L.plan(heads, gs.rotary_table(T, n_rot, device=gpu))
     x, qw, kw, grads = qk_inputs(gpu, B, T, heads, D, dtype, 71)

@@ -155,10 +155,11 @@ def test_qk_pointers_and_workspaces_are_checked_on_the_host():
 
 def test_qk_sample_dots_arguments_are_checked_on_the_host():
     f = _native.load_library().gs_qk_sample_dots
-    need = _native.load_library().gs_qk_sample_dots_workspace(64)
-    ok = [P16, 5, 64, 2, 3, P16, P16, P16, 0, P16, 1, 1.0, P16, need, None]
-    for change, status in (({0: None}, -1), ({1: 0}, -1), ({2: 0}, -1), ({3: 0}, -1), ({3: 5}, -1),
-                           ({4: 4}, -1), ({4: -1}, -1), ({8: 2}, -2), ({10: 7}, -2),
+    need = _native.load_library().gs_qk_sample_dots_workspace(129, 64)
+    assert need > 0 == _native.load_library().gs_qk_sample_dots_workspace(128, 64)
+    ok = [P16, 129, 64, 2, 127, P16, P16, P16, 0, P16, 1, 1.0, P16, need, None]
+    for change, status in (({0: None}, -1), ({1: 0}, -1), ({2: 0}, -1), ({3: 0}, -1), ({3: 129}, -1),
+                           ({4: 128}, -1), ({4: -1}, -1), ({8: 2}, -2), ({10: 7}, -2),
                            ({1: 65534}, -5), ({2: 513, 13: 1 << 20}, -5), ({12: None}, -3),
                            ({13: need - 1}, -3)):
         args = [change.get(i, v) for i, v in enumerate(ok)]
