@@ -114,34 +114,43 @@ struct LkRaw {
   }
 };
 
-// The gradient of few tokens in one launch: a wave owns 16 rows of the table, looks at all the ids (kept
-// one to a lane), and sums each row's tokens in order in fp32; most rows are written as zeros, which bounds
-// it.  Nothing is sorted, and no wave waits for another.  Lookup and gradient, 768 features in bf16, 64
-// tokens of 1000 ids spread / all one id, then of 50257 (us; in brackets by the sorted list): 18 (24) /
-// 22 (23), 20 (34) / 29 (34), and three launches less for the host, 30 -> 24 us a pass; of 128 tokens
-// 27 (25) / 34 (23), 24 (35) / 43 (33).
-constexpr int LK_FEW = 64, LK_ROWS = 16, LK_BATCH = 8;   // tokens; rows of a wave; loads in flight
+// The gradient of few tokens in one launch: a wave owns a piece for each lane of 4 rows of the table, looks
+// at all the ids (kept, 4 to a lane), and sums each row's tokens in order in fp32; most rows are written as
+// zeros, which bounds it.  Nothing is sorted, and no wave waits for another.  Lookup and gradient, 768
+// features in bf16, of 64 / 256 tokens spread over 1000 ids, then 50257 (us; in brackets by the sorted
+// list): 9 (24) / 14 (26), 18 (34) / 20 (36), and three launches less for the host, 30 -> 24 a pass; 256
+// tokens of one id 29 (25), 42 (35), 512 would be twice that.  (16 rows to a wave, all their features in
+// turn: 20 / 43, 20 / 34.)
+constexpr int LK_FEW = 256, LK_SETS = LK_FEW / 64;   // tokens; of a lane
+constexpr int LK_ROWS = 4, LK_BATCH = 8;             // rows of a wave; loads in flight
 template <class E, int V, int ALIGN>
 __global__ void __launch_bounds__(LK_THREADS) lookup_few_grad_kernel(
     const int64_t* __restrict__ ids, int n, const E* __restrict__ G, int64_t vocab, int64_t d,
     float scale, E* __restrict__ grad) {
-  static_assert(LK_FEW == 64, "a lane for every token");
   struct alignas(ALIGN) Piece { E e[V]; };
   const int lane = threadIdx.x & 63;
   const int64_t v0 =
       (static_cast<int64_t>(blockIdx.x) * (LK_THREADS / 64) + (threadIdx.x >> 6)) * LK_ROWS;
-  // the lane's token's row among the wave's (any other number: not among them)
-  const uint64_t row =
-      lane < n ? static_cast<uint64_t>(ids[lane]) - static_cast<uint64_t>(v0) : ~uint64_t{0};
-  for (int r = 0; r < LK_ROWS && v0 + r < vocab; ++r) {
-    const unsigned long long mine = __ballot(row == static_cast<uint64_t>(r));
-    E* out = grad + (v0 + r) * d;
-    for (int64_t f0 = static_cast<int64_t>(lane) * V; f0 < d; f0 += 64 * V) {
-      const int64_t f = min(f0, d - V);   // a row's last piece ends with the row
-      float acc[V];
+  // the rows of the lane's tokens among the wave's (any other number: not among them)
+  uint64_t row[LK_SETS];
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] = 0.f;
-      for (unsigned long long left = mine; left != 0;) {   // the same for the whole wave
+  for (int k = 0; k < LK_SETS; ++k) {
+    const int i = 64 * k + lane;
+    row[k] = i < n ? static_cast<uint64_t>(ids[i]) - static_cast<uint64_t>(v0) : ~uint64_t{0};
+  }
+  const int64_t f0 = (static_cast<int64_t>(blockIdx.y) * 64 + lane) * V;
+  const int64_t f = min(f0, d - V);   // a row's last piece ends with the row
+  for (int r = 0; r < LK_ROWS && v0 + r < vocab; ++r) {
+    unsigned long long mine[LK_SETS];
+#pragma unroll
+    for (int k = 0; k < LK_SETS; ++k) mine[k] = __ballot(row[k] == static_cast<uint64_t>(r));
+    if (f0 >= d) continue;
+    float acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < LK_SETS; ++k)
+      for (unsigned long long left = mine[k]; left != 0;) {   // the same for the whole wave
         // all loads are made (past the last token its row again), so that none waits for another
         LkRaw<E, V> x[LK_BATCH];
         const int count = min(LK_BATCH, __popcll(left));
@@ -150,7 +159,8 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_few_grad_kernel(
         for (int q = 0; q < LK_BATCH; ++q) {
           token = left != 0 ? __builtin_ctzll(left) : token;
           left &= left - 1;
-          __builtin_memcpy(&x[q], reinterpret_cast<const Piece*>(G + token * d + f), sizeof(Piece));
+          __builtin_memcpy(&x[q], reinterpret_cast<const Piece*>(G + (64 * k + token) * d + f),
+                           sizeof(Piece));
         }
 #pragma unroll
         for (int q = 0; q < LK_BATCH; ++q)
@@ -159,11 +169,10 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_few_grad_kernel(
             for (int e = 0; e < V; ++e) acc[e] += x[q].get(e);
           }
       }
-      Piece o;
+    Piece o;
 #pragma unroll
-      for (int e = 0; e < V; ++e) o.e[e] = from_f32<E>(scale * acc[e]);
-      *reinterpret_cast<Piece*>(out + f) = o;
-    }
+    for (int e = 0; e < V; ++e) o.e[e] = from_f32<E>(scale * acc[e]);
+    *reinterpret_cast<Piece*>(grad + (v0 + r) * d + f) = o;
   }
 }
 
@@ -172,7 +181,9 @@ int launch_few_grad(const int64_t* ids, int64_t n, const void* G, int64_t vocab,
                     float scale, void* grad, hipStream_t s) {
   constexpr int V = 16 / sizeof(E), A = sizeof(E);
   constexpr int64_t rows = LK_ROWS * (LK_THREADS / 64);
-  const dim3 grid(static_cast<unsigned>((vocab + rows - 1) / rows));
+  const int64_t width = d >= V ? 64 * V : 64;   // a wave's features
+  const dim3 grid(static_cast<unsigned>((vocab + rows - 1) / rows),
+                  static_cast<unsigned>((d + width - 1) / width));
   const E* g = static_cast<const E*>(G);
   E* out = static_cast<E*>(grad);
   const int m = static_cast<int>(n);
@@ -189,8 +200,10 @@ int launch_few_grad(const int64_t* ids, int64_t n, const void* G, int64_t vocab,
   return check_launch("lookup_few_grad_kernel");
 }
 
-bool lookup_is_few(int64_t n, int64_t vocab) {
-  return n <= LK_FEW && vocab <= LK_MAX_BLOCKS * LK_ROWS;
+// Few tokens, and a grid's limits: 65535 pieces of a row, below 2^32 threads.
+bool lookup_is_few(int64_t n, int64_t vocab, int64_t d) {
+  const int64_t y = (d + 255) / 256;
+  return n <= LK_FEW && y <= 65535 && vocab <= LK_MAX_BLOCKS * LK_ROWS / y;
 }
 
 }  // namespace
@@ -199,7 +212,7 @@ bool lookup_is_few(int64_t n, int64_t vocab) {
 using namespace gs;
 
 extern "C" size_t gs_embedding_lookup_grad_workspace(int64_t n, int64_t vocab, int64_t d) {
-  return n > 0 && lookup_is_few(n, vocab) ? 0
+  return n > 0 && lookup_is_few(n, vocab, d) ? 0
                                           : gs_embedding_train_grad_workspace(1, 0, n, d, vocab);
 }
 
@@ -211,7 +224,7 @@ extern "C" int gs_embedding_lookup_grad(const int64_t* ids, const void* G, int d
   if (ids == nullptr || G == nullptr || grad == nullptr || n <= 0 || vocab <= 0 || d <= 0)
     return fail(GS_ERR_INVALID, "gs_embedding_lookup_grad: invalid arguments");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (!lookup_is_few(n, vocab))   // one sample of all the tokens, none of them for validation
+  if (!lookup_is_few(n, vocab, d))   // one sample of all the tokens, none of them for validation
     return gs_embedding_train_grad(ids, G, dtype, 1, 0, 1, n, d, vocab, scale, grad, dtype, 0,
                                    workspace, workspace_bytes, stream);
   return dtype == GS_DTYPE_BF16 ? launch_few_grad<uint16_t>(ids, n, G, vocab, d, scale, grad, s)

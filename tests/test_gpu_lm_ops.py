@@ -72,11 +72,11 @@ def test_lookup_rows_off_16_byte_boundaries(gpu, dtype, d, off):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
-@pytest.mark.parametrize("n", [2, 63, 64, 65, 513])
-@pytest.mark.parametrize("d", [3, 64, 333])
+@pytest.mark.parametrize("n", [2, 63, 65, 255, 256, 257])
+@pytest.mark.parametrize("d", [3, 64, 333, 1100])
 @pytest.mark.parametrize("ids", ["all", "one", "few", "outside"])
 def test_lookup_gradient_around_its_two_ways(gpu, dtype, n, d, ids):
-    """Up to 64 tokens are summed without a sort: ids spread, all the same, a dozen, or extreme."""
+    """Up to 256 tokens are summed without a sort: ids spread, all the same, a dozen, or extreme."""
     vocab = 1003
     x = {"all": torch.randint(0, vocab, (n,), generator=gen(n)), "one": torch.full((n,), vocab - 1),
          "few": torch.randint(0, 12, (n,), generator=gen(n)) * 90,

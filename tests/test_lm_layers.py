@@ -223,13 +223,13 @@ def test_lookup_arguments_are_checked_on_the_host():
 def test_lookup_gradient_arguments_are_checked_on_the_host():
     lib = _native.load_library()
     f, size = lib.gs_embedding_lookup_grad, lib.gs_embedding_lookup_grad_workspace
-    assert size(64, 50257, 768) == 0 < size(65, 50257, 768)
+    assert size(256, 50257, 768) == 0 < size(257, 50257, 768)
     assert f(P16, P16, 2, 4, 10, 8, 1.0, P16, None, 0, None) == -2
     for bad in ((None, P16, 0, 4, 10, 8), (P16, None, 0, 4, 10, 8), (P16, P16, 0, 0, 10, 8),
                 (P16, P16, 0, 4, 0, 8), (P16, P16, 0, 4, 10, 0)):
         assert f(*bad, 1.0, P16, None, 0, None) == -1
     assert f(P16, P16, 0, 4, 10, 8, 1.0, None, None, 0, None) == -1
-    assert f(P16, P16, 0, 65, 10, 8, 1.0, P16, None, 0, None) == -3
+    assert f(P16, P16, 0, 257, 10, 8, 1.0, P16, None, 0, None) == -3
 
 
 # ---------------------------------------------------------------- the forms, by differences
