@@ -107,7 +107,10 @@ def _prepare_sample_grad_or_dotprod(layer: nn.Module, grad_output: Tuple[torch.T
     others = ()
     if isinstance(layer, QKNormRotary):   # three outputs, any of which may have no gradient
         backprops = next(g for g in grad_output if g is not None).detach()
-        if d.get("_gs_sample_grads") is None:   # else the output gradients have been used
+        samples = d.get("_gs_sample_grads")
+        if samples is not None and samples._version == d["_gs_sample_version"]:
+            samples = d["_gs_sample_grads"] = None   # no backward pass has written them
+        if samples is None:   # else the output gradients have been used
             d["_gs_grad_outputs"] = others = tuple(None if g is None else g.detach()
                                                    for g in grad_output)
             others += (d.get("_gs_positions"),)

@@ -209,7 +209,8 @@ struct QkHow {
   int64_t heads[3];
   bool norm, interleaved;
   double eps;
-  Tensor samples;   // where the backward pass writes each sample's weight gradients, or undefined
+  Tensor samples;   // where the backward pass writes each sample's weight gradients, or undefined;
+                    // its version counts the passes
   int edge[4];      // each input's place among the node's edges, or -1
 };
 
@@ -387,6 +388,7 @@ struct QkNormRotary : torch::autograd::Function<QkNormRotary> {
                               stream_on(c.dev)),
             "gs_qk_rotary_grad");
     }
+    if (how.samples.defined()) how.samples.unsafeGetTensorImpl()->bump_version();   // written
     return once({da, db, dw[0], dw[1], Tensor(), Tensor(), Tensor()});
   }
 };

@@ -156,12 +156,19 @@ class QKNormRotary(nn.Module):
         if self.norm and self._backward_hooks and hasattr(self.q_weight, "initially_requires_grad"):
             # An engine's backward hook reads these: the positions, and each sample's gradients of
             # the weights, which the backward pass forms on its way (it runs before the hook when
-            # the input has a gradient).
+            # the input has a gradient).  A forward whose tensor no hook has taken yet leaves it to
+            # the next one: activation checkpointing runs the forward again within the backward pass
+            # of the first run's nodes, which write the tensor they were given.
+            d = self.__dict__
             if torch.is_grad_enabled() and qkv.requires_grad:
-                sample_grads = torch.empty(2, qkv.shape[0], self.head_dim, device=qkv.device,
-                                           dtype=torch.float32)
-            self.__dict__["_gs_positions"] = positions
-            self.__dict__["_gs_sample_grads"] = sample_grads
+                shape = (2, qkv.shape[0], self.head_dim)
+                sample_grads = d.get("_gs_sample_grads")
+                if sample_grads is None or sample_grads.shape != shape or \
+                        sample_grads.device != qkv.device:
+                    sample_grads = torch.empty(shape, device=qkv.device, dtype=torch.float32)
+                d["_gs_sample_version"] = sample_grads._version   # a backward pass counts it up
+            d["_gs_positions"] = positions
+            d["_gs_sample_grads"] = sample_grads
         q, k, v = ops().qk_norm_rotary(
             qkv, None, (self.n_head, self.n_kv_head, self.n_kv_head), self.table, positions,
             self.q_weight, self.k_weight, self.norm, self.eps, self.interleaved, sample_grads)
