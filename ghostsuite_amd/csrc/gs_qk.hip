@@ -147,11 +147,25 @@ struct QkUnit {
   float a[V], b[V];
 };
 
-// The rotation of a unit by its angles (sign +1) or back (-1).
+// Which pairs of a unit turn: all or none ([0]), or where neighbours turn each for itself.
 template <int V, bool INTER>
-__device__ __forceinline__ void qk_rotate(QkUnit<V>& u, const float (&c)[V], const float (&s)[V],
-                                          float sign) {
+struct QkTurns {
+  bool pair[INTER ? V : 1];
+  __device__ __forceinline__ void set(const QkPlace<V, INTER>& pl, int rot) {
+#pragma unroll
+    for (int i = 0; i < (INTER ? V : 1); ++i)
+      pair[i] = (!INTER || i < V / 2 ? pl.pair0 + i : pl.pair1 + i - V / 2) < rot / 2;
+  }
+};
+
+// The rotation of a unit's pairs that turn by their angles (sign +1) or back (-1).  Others stay as
+// they are, not turned by an angle of zero: an infinity times its sine would reach the pair's other
+// feature.
+template <int V, bool INTER>
+__device__ __forceinline__ void qk_rotate(QkUnit<V>& u, const QkTurns<V, INTER>& t,
+                                          const float (&c)[V], const float (&s)[V], float sign) {
   if constexpr (!INTER) {
+    if (!t.pair[0]) return;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float x = u.a[i], y = u.b[i], si = sign * s[i];
@@ -166,8 +180,8 @@ __device__ __forceinline__ void qk_rotate(QkUnit<V>& u, const float (&c)[V], con
       float& y = 2 * i + 1 < V ? u.a[2 * i + 1 < V ? 2 * i + 1 : 0]
                                : u.b[2 * i + 1 < V ? 0 : 2 * i + 1 - V];
       const float x0 = x, y0 = y, si = sign * s[i];
-      x = x0 * c[i] - y0 * si;
-      y = y0 * c[i] + x0 * si;
+      x = t.pair[i] ? x0 * c[i] - y0 * si : x0;
+      y = t.pair[i] ? y0 * c[i] + x0 * si : y0;
     }
   }
 }
@@ -191,7 +205,7 @@ __device__ __forceinline__ int64_t qk_position(const QkArgs& a, int64_t b, int64
                           : static_cast<const int64_t*>(a.pos)[i];
 }
 
-// Cosines and sines of a unit's pairs at a position; those past the rotated features: 1 and 0; a
+// Cosines and sines of a unit's pairs at a position (past the rotated ones 1 and 0, not used); a
 // position outside the table: NaN.  In whole vectors where the table's rows split there: 20 x 1024
 // tokens of 12 + 12 + 12 heads of 64, bf16, 16 loads of one number take 46.6 us forward, 4 of four 43.4.
 template <int V>
@@ -283,6 +297,10 @@ __global__ void __launch_bounds__(QK_THREADS) qk_forward_kernel(QkArgs a) {
   const int lane = threadIdx.x & (lanes - 1);
   const bool turn = blk.part < 2 && a.rot > 0, norm = blk.part < 2 && a.norm;
   QkUnit<V> w[UPL];
+  QkTurns<V, INTER> turns[UPL];
+#pragma unroll
+  for (int j = 0; j < UPL; ++j)
+    turns[j].set(QkPlace<V, INTER>(lane + j * lanes, a.D, a.rot), a.rot);
   if (norm) {
 #pragma unroll
     for (int j = 0; j < UPL; ++j) {
@@ -342,7 +360,7 @@ __global__ void __launch_bounds__(QK_THREADS) qk_forward_kernel(QkArgs a) {
               u[j].b[i] *= r * w[j].b[i];
             }
           }
-          if (turn) qk_rotate<V, INTER>(u[j], c[j], s[j], 1.f);
+          if (turn) qk_rotate<V, INTER>(u[j], turns[j], c[j], s[j], 1.f);
           const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
           qk_store<E, V>(yr + (h + q) * out.sh, pl.o0, a.D, u[j].a);
           qk_store<E, V>(yr + (h + q) * out.sh, pl.o1, a.D, u[j].b);
@@ -362,9 +380,11 @@ __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(QkArgs a) {
   const bool turn = blk.part < 2 && a.rot > 0 && any_g, norm = blk.part < 2 && a.norm && any_g;
   const bool want_w = blk.part < 2 && a.part[blk.part] != nullptr;
   QkUnit<V> w[UPL], dw[UPL];
+  QkTurns<V, INTER> turns[UPL];
 #pragma unroll
   for (int j = 0; j < UPL; ++j) {
     const QkPlace<V, INTER> pl(lane + j * lanes, a.D, a.rot);
+    turns[j].set(pl, a.rot);
     qk_weights<V>(a, norm ? blk.part : 2, pl.o0, w[j].a);
     qk_weights<V>(a, norm ? blk.part : 2, pl.o1, w[j].b);
 #pragma unroll
@@ -418,7 +438,7 @@ __global__ void __launch_bounds__(QK_THREADS) qk_backward_kernel(QkArgs a) {
       if (h + 1 < blk.h1) fetch(h + 1);
       if (turn) {
 #pragma unroll
-        for (int j = 0; j < UPL; ++j) qk_rotate<V, INTER>(g[j], c[j], s[j], -1.f);
+        for (int j = 0; j < UPL; ++j) qk_rotate<V, INTER>(g[j], turns[j], c[j], s[j], -1.f);
       }
       if (norm) {
         float ss = 0.f, sd = 0.f;

@@ -1,0 +1,93 @@
+"""The language-model operators on the GPU at infinities, NaN and the ends of their ranges."""
+import math
+
+import pytest
+import torch
+
+import ghostsuite_amd as gs
+from tests.helpers import randn
+
+pytestmark = pytest.mark.gpu
+BF16, FP32 = torch.bfloat16, torch.float32
+
+
+def same(got, want, what):
+    """The same values, NaN in the same places."""
+    torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True, msg=lambda m: f"{what}: {m}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("D,n_rot", [(64, 32), (64, 16), (80, 20), (33, 10), (33, 32), (256, 64),
+                                     (66, 2), (100, 6), (64, 2), (24, 0)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_qk_features_past_the_rotated_ones_stay_by_themselves(gpu, dtype, interleaved, norm, D,
+                                                              n_rot, bad):
+    """An infinity or NaN in one of them, or in its output gradient, reaches no other feature but
+    through the row's norm.  Token t has it at feature n_rot + t, of the last query head for even
+    tokens, of the key head for odd ones."""
+    B, T, heads = 2, D - n_rot, (2, 1, 1)
+    table = gs.rotary_table(T, n_rot, device=gpu)
+    x = randn((B, T, sum(heads), D), 1).to(dtype).to(gpu)
+    grads = [randn((B, h, T, D), 2 + i, 1.0, dtype).to(gpu) for i, h in enumerate(heads)]
+    w = [(1 + 0.2 * randn((D,), 5 + i)).to(dtype).to(gpu).requires_grad_() for i in range(2)] \
+        if norm else [None, None]
+
+    def run(x, grads):
+        x = x.clone().requires_grad_()
+        y = gs.qkv_norm_rotary(x, 2, 1, table, None, *w, norm=norm, interleaved=interleaved)
+        got = torch.autograd.grad(y, [x] + (w if norm else []), grads)
+        return torch.cat([o.detach() for o in y], 1).transpose(1, 2), got[0], got[1:]
+
+    y, dx, dw = run(x, grads)
+    t = torch.arange(T, device=gpu)
+    head, f = 1 + t % 2, n_rot + t
+    at = (1, t, head, f)                           # sample 1 alone
+    xb = x.clone()
+    xb[at] = bad
+    got, got_dx, _ = run(xb, grads)
+    row = torch.zeros(B, T, sum(heads), dtype=torch.bool, device=gpu)
+    row[1, t, head] = True
+    want = y.clone()
+    if norm:                                       # an infinite row length
+        want[row] = math.nan if math.isnan(bad) else 0.0
+        want[at] = math.nan
+    else:
+        want[at] = bad
+    same(got, want, "forward")
+    if not norm:
+        same(got_dx, dx, "gradient of a row that was not read")
+    else:
+        same(got_dx[~row], dx[~row], "gradient of other rows")
+    gb = [g.clone() for g in grads]
+    gb[0][1, 1, t[::2], f[::2]] = bad
+    gb[1][1, 0, t[1::2], f[1::2]] = bad
+    got, got_dx, got_dw = run(x, gb)
+    same(got, y, "forward of the same")
+    if norm:
+        same(got_dx[~row], dx[~row], "gradient of other rows")
+        assert not got_dx[row].isfinite().any()
+        for part in range(2):
+            hit = torch.zeros(D, dtype=torch.bool, device=gpu)
+            hit[f[part::2]] = True
+            assert not got_dw[part][hit].isfinite().any()
+            same(got_dw[part][~hit], dw[part][~hit], "gradient of other weights")
+    else:
+        want = dx.clone()
+        want[at] = bad
+        same(got_dx, want, "gradient")
+
+
+@pytest.mark.parametrize("n_rot", [0, 16, 48])
+def test_qk_rotated_features_of_a_bad_row_alone(gpu, n_rot):
+    """A position outside the table: NaN in the rotated features, the others as at any position."""
+    D, x = 48, randn((1, 3, 3 * 48), 1).to(gpu)
+    table = gs.rotary_table(4, n_rot, device=gpu)
+    for interleaved in (False, True):
+        y = [gs.qkv_norm_rotary(x, 1, 1, table, torch.tensor(p, device=gpu), interleaved=interleaved)
+             for p in ([0, 1, 2], [0, 9, 2])]
+        for a, b in zip(y[0][:2], y[1][:2]):
+            assert b[:, :, 1, :n_rot].isnan().all()
+            same(b[:, :, 1, n_rot:], a[:, :, 1, n_rot:], "not rotated")
+            same(b[:, :, ::2], a[:, :, ::2], "other tokens")
