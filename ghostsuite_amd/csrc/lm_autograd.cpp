@@ -15,6 +15,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/custom_class.h>
 
 #include <optional>
@@ -54,6 +55,27 @@ int gs_dtype_of(const Tensor& t, const char* what) {
   if (t.scalar_type() == at::kBFloat16) return GS_DTYPE_BF16;
   if (t.scalar_type() == at::kFloat) return GS_DTYPE_F32;
   refuse(what, ": bf16 or fp32, got ", t.scalar_type());
+}
+
+// A tensor that is its memory: no wrapper of a function transform or subclass, no compressed layout, no
+// sign or zeros that are only marked.
+bool in_memory(const Tensor& t) {
+  return t.layout() == at::kStrided && t.has_storage() && !t.is_nested() && !t.is_neg() &&
+         !t._is_zerotensor() && !t.unsafeGetTensorImpl()->is_python_dispatch() &&
+         !t.key_set().has(c10::DispatchKey::Functionalize);
+}
+
+// The operators are no operators of torch's dispatcher: what it does around those (forward-mode
+// differentiation, function transforms, tracing) would pass them by unseen, so it is refused.
+void check_plain(std::initializer_list<const Tensor*> ts) {
+  require(!torch::jit::tracer::isTracing(), "the language-model operators cannot be traced");
+  for (const Tensor* t : ts) {
+    if (!t->defined()) continue;
+    require(in_memory(*t), "the language-model operators take plain strided tensors (no sparse or nested "
+            "ones, no subclasses, no lazily negated views, no function transforms)");
+    require(!t->_fw_grad(0).defined(),
+            "the language-model operators have no forward-mode differentiation");
+  }
 }
 
 // All tensors (undefined ones aside) on one GPU.
@@ -198,6 +220,7 @@ struct Lookup : torch::autograd::Function<Lookup> {
 
 Tensor embedding_lookup(const Tensor& ids, const Tensor& weight, double scale,
                         std::optional<int64_t> padding_idx) {
+  check_plain({&ids, &weight});
   LookupHow how{scale, padding_idx.value_or(-1), {}, weight.scalar_type()};
   if (recorded({&weight})) return Lookup::apply(ids, weight, std::move(how));
   return lookup(ids, weight, how, nullptr);
@@ -404,8 +427,10 @@ variable_list qk_norm_rotary(const Tensor& a, const OptTensor& b, const std::vec
                              const Tensor& table, const OptTensor& positions, const OptTensor& qw,
                              const OptTensor& kw, bool norm, double eps, bool interleaved,
                              const OptTensor& samples) {
+  const Tensor bt = given(b), q = given(qw), k = given(kw), pos = given(positions);
   QkHow how = qk_how(heads, norm, eps, interleaved);
   how.samples = given(samples);
+  check_plain({&a, &bt, &q, &k, &table, &pos, &how.samples});
   if (how.samples.defined())
     require(norm && how.samples.is_cuda() && how.samples.device() == a.device() &&
                 how.samples.scalar_type() == at::kFloat && how.samples.is_contiguous() &&
@@ -414,10 +439,9 @@ variable_list qk_norm_rotary(const Tensor& a, const OptTensor& b, const std::vec
                 how.samples.size(2) * (heads[0] + heads[1] + heads[2]) * a.size(1) * a.size(0) ==
                     a.numel(),
             "sample gradients ", how.samples.sizes(), ": fp32 [2, B, D] for a packed input expected");
-  const Tensor bt = given(b), q = given(qw), k = given(kw);
   if (recorded({&a, &bt, &q, &k}))
     return QkNormRotary::apply(a, b, qw, kw, table, positions, how);
-  return qk_forward(a, bt, q, k, table, given(positions), how);
+  return qk_forward(a, bt, q, k, table, pos, how);
 }
 
 // (dot_q, dot_k, train gradient of q's weight, of k's; the gradients undefined without a scale).
@@ -428,8 +452,9 @@ std::vector<OptTensor> qk_norm_rotary_dots(const Tensor& a, const OptTensor& b,
                                            const std::vector<OptTensor>& given_grads, int64_t n_val,
                                            std::optional<int64_t> val_start,
                                            std::optional<double> grad_scale) {
-  const QkCall c(a, given(b), given(qw), given(kw), table, given(positions),
-                 qk_how(heads, true, eps, interleaved));
+  const Tensor bt = given(b), q = given(qw), k = given(kw), pos = given(positions);
+  check_plain({&a, &bt, &q, &k, &table, &pos});
+  const QkCall c(a, bt, q, k, table, pos, qk_how(heads, true, eps, interleaved));
   require(!c.empty(), "qk_norm_rotary_dots: no tokens");
   const int64_t n_train = c.B - n_val;
   require(n_train > 0, "qk_norm_rotary_dots: ", n_val, " validation samples of ", c.B);
@@ -458,6 +483,7 @@ std::vector<OptTensor> qk_norm_rotary_dots(const Tensor& a, const OptTensor& b,
 std::vector<OptTensor> qk_sample_dots(const Tensor& samples, const Tensor& qw, const Tensor& kw,
                                       int64_t n_val, std::optional<int64_t> val_start,
                                       std::optional<double> grad_scale) {
+  check_plain({&samples, &qw, &kw});
   const c10::Device dev = device_of({&samples, &qw, &kw});
   require(samples.dim() == 3 && samples.size(0) == 2 && samples.scalar_type() == at::kFloat &&
               samples.is_contiguous(),
@@ -622,10 +648,12 @@ struct Distillation : torch::autograd::Function<Distillation> {
 Tensor distillation_loss(const Tensor& logits, const Tensor& ids, const Tensor& t,
                          const OptTensor& labels, double temperature, double alpha,
                          int64_t ignore_index, int reduction) {
+  const Tensor y = given(labels);
+  check_plain({&logits, &ids, &t, &y});
   DistillHow how{temperature, alpha, ignore_index, reduction, {}, {}};
   if (recorded({&logits}))
     return Distillation::apply(logits, ids.detach(), t.detach(), labels, std::move(how));
-  return distill_loss(logits, ids, t, given(labels), how, nullptr, nullptr);
+  return distill_loss(logits, ids, t, y, how, nullptr, nullptr);
 }
 
 }  // namespace

@@ -9,7 +9,8 @@
     labels' cross entropy, with its gradient.
 
 All are differentiable (once), run on the current stream and take bf16 or fp32 tensors on a ROCm
-GPU; anything else raises ``GhostHipError``.  ``ScaledEmbedding`` and ``QKNormRotary`` are layers
+GPU; anything else raises ``GhostHipError``, as do forward-mode differentiation, function
+transforms (``torch.func``) and ``torch.jit`` tracing.  ``ScaledEmbedding`` and ``QKNormRotary`` are layers
 the engines know: ``GradDotProdEngine`` gives their weights gradient dot products and train
 gradients, ``GradProjLoraEngine`` projects a ``ScaledEmbedding``.
 """
