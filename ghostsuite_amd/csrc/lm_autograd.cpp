@@ -78,6 +78,16 @@ void check_plain(std::initializer_list<const Tensor*> ts) {
   }
 }
 
+// An output gradient in memory: marked zeros and signs are written.
+Tensor gradient_in_memory(const Tensor& g) {
+  if (in_memory(g)) return g;
+  if (g._is_zerotensor())
+    return at::zeros(g.sizes(), at::TensorOptions().dtype(g.dtype()).device(g.device()));
+  const Tensor r = g.is_neg() ? g.resolve_neg() : g;
+  require(in_memory(r), "an output gradient that is no plain strided tensor");
+  return r;
+}
+
 // All tensors (undefined ones aside) on one GPU.
 c10::Device device_of(std::initializer_list<const Tensor*> ts) {
   std::optional<c10::Device> dev;
@@ -183,7 +193,8 @@ Tensor lookup(const Tensor& ids_in, const Tensor& weight_in, const LookupHow& ho
   return out;
 }
 
-Tensor lookup_grad(const Tensor& ids, const Tensor& g_in, const LookupHow& how) {
+Tensor lookup_grad(const Tensor& ids, const Tensor& g_given, const LookupHow& how) {
+  const Tensor g_in = gradient_in_memory(g_given);
   const c10::Device dev = device_of({&ids, &g_in});
   const auto options = g_in.options().dtype(how.dtype).requires_grad(false);
   const int64_t n = ids.numel(), vocab = how.table[0], d = how.table[1];
@@ -332,6 +343,7 @@ variable_list output_gradients(const QkCall& c, const variable_list& given_grads
   for (size_t k = 0; k < given_grads.size() && k < 3; ++k) {
     Tensor g = given_grads[k];
     if (g.defined()) {
+      g = gradient_in_memory(g);
       device_of({&c.held[0], &g});
       require(g.dim() == 4 && g.size(0) == c.B && g.size(1) == c.shape.heads[k] && g.size(2) == c.T &&
                   g.size(3) == c.D && g.scalar_type() == c.held[0].scalar_type(),
@@ -631,7 +643,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
     how.unit = how.ws = Tensor();
     const DistillCall c(s[0], s[1], s[2], s[3], how);
     if (c.d.N == 0) return once({at::empty_like(s[0]), Tensor(), Tensor(), Tensor(), Tensor()});
-    const Tensor up = g[0].to(at::kFloat).contiguous();
+    const Tensor up = gradient_in_memory(g[0]).to(at::kFloat).contiguous();
     const bool filled = grad.defined() && c.fits(grad);   // autograd may have moved the logits
     if (!filled) grad = c.empty_gradient(), ws = c.workspace();
     {

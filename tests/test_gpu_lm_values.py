@@ -91,3 +91,40 @@ def test_qk_rotated_features_of_a_bad_row_alone(gpu, n_rot):
             assert b[:, :, 1, :n_rot].isnan().all()
             same(b[:, :, 1, n_rot:], a[:, :, 1, n_rot:], "not rotated")
             same(b[:, :, ::2], a[:, :, ::2], "other tokens")
+
+
+def _calls(gpu):
+    """(outputs, inputs) of each operator."""
+    w = randn((9, 8), 1).to(gpu).requires_grad_()
+    yield [gs.embedding_lookup(torch.arange(5, device=gpu), w, 2.0)], [w]
+    big = torch.arange(600, device=gpu) % 9        # more tokens than one launch sums
+    yield [gs.embedding_lookup(big, w, 2.0)], [w]
+    x = randn((2, 3, 4 * 16), 2).to(gpu).requires_grad_()
+    q = torch.ones(16, device=gpu, requires_grad=True)
+    yield list(gs.qkv_norm_rotary(x, 2, 1, gs.rotary_table(3, 16, device=gpu), None, q, q)), [x, q]
+    z = randn((4, 31), 3).to(gpu).requires_grad_()
+    ids, t = torch.arange(8, device=gpu).view(4, 2), randn((4, 2), 4).to(gpu)
+    for reduction in ("none", "mean"):
+        yield [gs.distillation_loss(z, ids, t, temperature=2.0, reduction=reduction)], [z]
+
+
+def test_output_gradients_that_are_not_their_memory(gpu):
+    """Zeros that are only marked, and signs that are only marked, as complex torch code gives them."""
+    for outs, inputs in _calls(gpu):
+        g = [torch.randn_like(o) for o in outs]
+        for marked in ([torch._efficientzerotensor(o.shape, device=gpu) for o in outs],
+                       [torch.complex(x, x).conj().imag for x in g]):
+            written = [m.clone().resolve_neg() + 0.0 if m.is_neg() else torch.zeros(m.shape, device=gpu)
+                       for m in marked]
+            got = torch.autograd.grad(outs, inputs, marked, retain_graph=True)
+            want = torch.autograd.grad(outs, inputs, written, retain_graph=True)
+            for a, b in zip(got, want):
+                same(a, b, "gradient")
+    x = randn((2, 3, 4 * 16), 2).to(gpu).requires_grad_()
+    y = gs.qkv_norm_rotary(x, 2, 1, gs.rotary_table(3, 16, device=gpu))[0]
+    c = torch.randn(2, 2, 3, 16, dtype=torch.complex64, device=gpu)
+    got, = torch.autograd.grad(torch.view_as_real(torch.complex(y, y).conj() * c).sum(), x)
+    y = gs.qkv_norm_rotary(x, 2, 1, gs.rotary_table(3, 16, device=gpu))[0]
+    z = torch.complex(y, -y) * c
+    want, = torch.autograd.grad(z.real.sum() + z.imag.sum(), x)
+    torch.testing.assert_close(got, want, rtol=1e-4, atol=1e-6)
