@@ -317,7 +317,9 @@ __global__ void __launch_bounds__(THREADS, WPE) distill_kernel(DsArgs a) {
     if (!TWO) s1 = sq;   // temperature one, or only one of the two counts
     const bool teacher = a.alpha != 0.f && ts != 0.f;   // NaN counts
 
-    // ---- the entries' part: the loss, and each id's mass in the gradient
+    // ---- the entries' part: the loss, and each id's mass in the gradient.  The loss adds up tau (log p -
+    // log q), from differences of logits as they are: divided by a temperature below one, a student's
+    // logit at its type's lowest value would be infinite.
     float w = a.upstream != nullptr ? a.upstream[a.per_row ? n : 0] : 1.f;
     if (a.mean) w /= a.count != nullptr ? a.count[0] : static_cast<float>(counted);
     const float nan_or_one = ts != ts ? ts : 1.f;   // a NaN entry leaves no element of the row as if valid
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, WPE) distill_kernel(DsArgs a) {
           mass = w1;
         } else if (teacher && id >= 0) {
           const float d = ent.t[k] - tm, p = ds_exp(d, kq) * inv_ts;
-          if (p != 0.f) kl += p * (d * a.inv_tau - lts - ((ent.z[k] - m) * a.inv_tau - ltq));
+          if (p != 0.f) kl += a.alpha * a.tau * p * (d - (ent.z[k] - m) - a.tau * (lts - ltq));
           mass = wq * p;
         }
         ent.t[k] = mass;
@@ -355,7 +357,6 @@ __global__ void __launch_bounds__(THREADS, WPE) distill_kernel(DsArgs a) {
       float loss = 0.f;
 #pragma unroll
       for (int q = 0; q < WAVES; ++q) loss += red[2][q][0];
-      loss *= a.alpha * a.tau * a.tau;
       if (hard) loss += (1.f - a.alpha) * (in ? logf(s1) - (ent.z[K] - m) : __builtin_nanf(""));
       a.rows[n] = loss;
     }

@@ -5,7 +5,8 @@ import pytest
 import torch
 
 import ghostsuite_amd as gs
-from tests.helpers import randn
+from tests import lm_forms as L
+from tests.helpers import gen, randn
 
 pytestmark = pytest.mark.gpu
 BF16, FP32 = torch.bfloat16, torch.float32
@@ -128,3 +129,67 @@ def test_output_gradients_that_are_not_their_memory(gpu):
     z = torch.complex(y, -y) * c
     want, = torch.autograd.grad(z.real.sum() + z.imag.sum(), x)
     torch.testing.assert_close(got, want, rtol=1e-4, atol=1e-6)
+
+
+def _loss64(z, ids, t, labels, tau, alpha):
+    z, t = z.double().cpu().requires_grad_(), t.double().cpu()
+    rows, _ = L.distill_rows(z, ids.cpu(), t, labels.cpu(), tau, alpha)
+    return rows.detach(), torch.autograd.grad(rows.sum(), z)[0]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("tau", [0.25, 0.4, 0.5, 1.0, 3.0])
+@pytest.mark.parametrize("V", [29, 5000, 50257])
+def test_distill_teacher_entries_at_masked_logits(gpu, dtype, tau, V):
+    """The student's logits at some or all of the teacher's ids are the type's lowest value: losses of
+    the order of that value, finite where they are in the type."""
+    N, K = 6, 4
+    z, t = randn((N, V), 1, 2.0, dtype), randn((N, K), 2, 2.0, dtype)
+    ids = torch.stack([torch.randperm(V, generator=gen(n))[:K] for n in range(N)])
+    low = torch.finfo(dtype).min
+    z[0, ids[0, 0]] = low
+    z[1, ids[1]] = low
+    z[2] = low
+    z[2, 3] = 1.0
+    z[3, ids[3, 1:]] = low / 64
+    z[4] = low / 64
+    z[4, ids[4, 0]] = 0.0
+    labels = ids[:, 0].contiguous()
+    for alpha in (1.0, 0.25):
+        zg = z.to(gpu).requires_grad_()
+        loss = gs.distillation_loss(zg, ids.to(gpu), t.to(gpu), labels.to(gpu), temperature=tau,
+                                    alpha=alpha, reduction="none")
+        g, = torch.autograd.grad(loss, zg, torch.ones_like(loss))
+        want, dwant = _loss64(z, ids, t, labels, tau, alpha)
+        # within the comparison's 1e-5 of the largest number either side of it is right
+        top = torch.finfo(FP32).max
+        fits = want < top * (1 - 1e-5)
+        assert fits[0] and fits[5]
+        # a loss is K shares times differences of logits, all positive: some tens of roundings each
+        off = (loss.double().cpu() - want).abs()
+        assert (off <= 1e-5 * want.abs() + 1e-5)[fits].all(), (off, want)
+        assert loss.cpu()[want > top * (1 + 1e-5)].isinf().all() and not loss.isnan().any()
+        # shares and their differences from sums of exponentials: see the bound's smallest terms
+        assert ((g.double().cpu() - dwant).abs() <= dwant.abs() * 2 ** -8 * (dtype == BF16) +
+                2e-5).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("tau", [1e-37, 1e-30, 1e-23, 1e-20, 1e-12, 1e-6, 1e3, 1e9])
+def test_distill_far_temperatures(gpu, dtype, tau):
+    """Close to zero the shares are one and zero, the loss tau times a difference of logits."""
+    N, V, K = 5, 301, 6
+    z, t = randn((N, V), 3, 2.0, dtype), randn((N, K), 4, 2.0, dtype)
+    ids = torch.stack([torch.randperm(V, generator=gen(n))[:K] for n in range(N)])
+    labels = ids[:, 0].contiguous()
+    zg = z.to(gpu).requires_grad_()
+    loss = gs.distillation_loss(zg, ids.to(gpu), t.to(gpu), labels.to(gpu), temperature=tau,
+                                reduction="none")
+    g, = torch.autograd.grad(loss, zg, torch.ones_like(loss))
+    tau32 = float(torch.tensor(tau, dtype=FP32))
+    want, dwant = _loss64(z, ids, t, labels, tau32, 1.0)
+    # tau^2 log(V / K) and above; a logarithm's rounding counts tau^2 times, a difference's tau times
+    off = (loss.double().cpu() - want).abs()
+    assert (off <= 1e-5 * (want.abs() + tau32 ** 2)).all(), (off, want)
+    # an element is tau times a difference of shares up to one
+    assert ((g.double().cpu() - dwant).abs() <= tau32 * (2 ** -8 * (dtype == BF16) + 2e-5)).all()
