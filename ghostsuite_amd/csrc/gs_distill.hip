@@ -514,7 +514,7 @@ int ds_args(DsArgs& a, const char* name, const gs_distill* d) {
       d->V <= 0 || d->K <= 0 || d->inner <= 0 || d->inner > d->N || d->N % d->inner != 0 ||
       (d->inner > 1 && d->stride_inner < d->V) || (d->N > d->inner && d->stride_outer < d->V) ||
       !(d->temperature > 0.f) || !std::isfinite(d->temperature * d->temperature) ||
-      !std::isfinite(1.f / d->temperature) || !(d->alpha >= 0.f && d->alpha <= 1.f) ||
+      !std::isfinite(DS_LOG2E / d->temperature) || !(d->alpha >= 0.f && d->alpha <= 1.f) ||
       (d->labels == nullptr && d->alpha != 1.f) || d->reduction < GS_REDUCE_NONE ||
       d->reduction > GS_REDUCE_MEAN ||
       reinterpret_cast<uintptr_t>(d->Z) % elem_size(d->dtype) != 0)

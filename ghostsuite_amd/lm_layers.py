@@ -197,8 +197,9 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor,
     whose logit is -inf takes no part; a row with none left has no first term; an id that stands
     twice counts twice.  labels: [...]; rows whose label is ignore_index count for nothing, their
     gradient is zero; may be None with alpha = 1.  Another label outside [0, V) makes its row NaN
-    (alpha < 1).  reduction: 'mean' (over the rows not ignored; NaN when there are none), 'sum', or
-    'none' ([...]).  The loss is fp32; no gradient reaches the teacher.
+    (alpha < 1).  temperature: positive, its square and 1.45 times its inverse within fp32.
+    reduction: 'mean' (over the rows not ignored; NaN when there are none), 'sum', or 'none' ([...]).
+    The loss is fp32; no gradient reaches the teacher.
 
     The logits are read once and their gradient written in the same pass (except with 'none')."""
     if reduction not in ("mean", "sum", "none"):

@@ -468,6 +468,7 @@ int gs_qk_sample_dots(const float* sample_grads, int64_t B, int64_t D, int64_t n
  *   q = softmax of z / temperature, s = softmax of z
  *   loss = alpha temperature^2 sum_k p_k (log p_k - log q[id_k]) + (1 - alpha) (-log s_y)
  * A row without such an entry has no first term; a repeated id counts as often as it stands.
+ * temperature: positive, its square and log2(e) times its inverse within fp32.
  * labels NULL: alpha must be 1.  Rows whose label is ignore_index have loss 0 and gradient 0; another
  * label outside [0, V) makes the row's loss and gradient NaN (alpha < 1), as does a NaN logit, the
  * teacher's among the entries that count.

@@ -101,3 +101,14 @@ def test_dots_of_the_norm_weights():
     refused("plain strided", ops.qk_sample_dots, samples, w, marked, 1)
     refused("plain strided", ops.qk_norm_rotary, x, None, (1, 1, 1), TABLE, None, w, w, True, 1e-6,
             False, samples.to_sparse())
+
+
+def test_temperatures_whose_inverse_overflows():
+    import ctypes
+    from tests.test_lm_layers import P16, _distill
+    lib = _native.load_library()
+    for tau, status in ((3e-39, -1), (4.2e-39, -1), (4.3e-39, -3), (1e-30, -3), (1.8e19, -3),
+                        (1.9e19, -1)):           # -3: as far as the workspace
+        ref = ctypes.byref(_distill(temperature=tau))
+        assert lib.gs_distill_loss(ref, P16, None, None, 0, None) == status, tau
+        assert lib.gs_distill_grad(ref, P16, 0, P16, None, 0, None) == status, tau
