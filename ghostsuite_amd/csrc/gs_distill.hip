@@ -6,9 +6,9 @@
 //   dz   = w (alpha tau (q - P) + (1 - alpha) (s - 1_y)),   P the p_k at their ids
 //
 // A workgroup owns a row.  The row is read once, in 16-byte pieces that stay in registers as they
-// came: the maximum, then both sums of exponentials, then the gradient are formed from them, so a
-// training step's loss and gradient cost one read and one write of the logits, and the rate of a
-// copy bounds them (8192 rows of 50257 bf16: 390 us, 4.2 of a copy's 4.7 TB/s; with two softmaxes the
+// came: the maximum, then both sums of exponentials, then the gradient are formed from them, so the
+// loss and the gradient for an upstream of one cost one read and one write of the logits, and the rate
+// of a copy bounds them (8192 rows of 50257 bf16: 390 us, 4.2 of a copy's 4.7 TB/s; with two softmaxes the
 // exponentials, four to an element, come close behind).  Rows too long for the registers are read
 // again in a second sweep, out of the caches (running maximum and sums in the first).  The gradient is
 // written for the whole row as if no entry stood there; the elements of the K entries and the label are
@@ -479,6 +479,7 @@ void ds_launch(const DsArgs& a, bool two, int64_t grid, hipStream_t s) {
 //     65000: kept by 512 (18, 32 pieces) 444 / 773, read twice 425 / 807
 //    128256: kept by 512 (32) 511 / -, read twice by 512 415 / 938, by 1024 456 / 822
 //    262144: read twice by 512 448 / 924, by 1024 446 / 866
+// (The tiers count pieces, not types: at 65000 ids both types get the slower of their two, by 4%.)
 template <class E>
 int ds_run(const DsArgs& a, bool two, int64_t grid, hipStream_t s) {
   constexpr int VE = 16 / sizeof(E);
@@ -619,7 +620,9 @@ extern "C" int gs_distill_grad(const gs_distill* d, const float* upstream, int f
   const bool two = ds_two(a);
   a.grad = grad;
   a.upstream = upstream;
-  // A filled gradient is mostly left as it is: few workgroups then look at the upstream and end.
+  // A filled gradient is mostly left as it is: few workgroups then look at the upstream and end.  For
+  // another upstream they form it again, in 520 us for 8192 rows of 50257 bf16 (as many as fit the card
+  // would be 768 or 1024; not measured).
   const int64_t grid = a.filled ? std::min<int64_t>(a.N, 512) : std::min(a.N, DS_MAX_BLOCKS);
   return d->dtype == GS_DTYPE_BF16 ? ds_run<uint16_t>(a, two, grid, s)
                                    : ds_run<float>(a, two, grid, s);

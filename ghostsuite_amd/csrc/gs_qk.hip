@@ -766,7 +766,7 @@ int qk_args(QkArgs& a, const char* name, const gs_qk_shape* sh, const gs_qk_rows
     return fail(GS_ERR_INVALID, n + ": invalid arguments");
   if (sh->D > QK_MAX_D)
     return fail(GS_ERR_UNSUPPORTED, n + ": more than 512 features to a head");
-  // the grid's y, 32-bit head numbers, and the token count in the grid's x
+  // tokens, and the workgroups of one sample's head groups, are numbered in 32 bits with room to spare
   if (static_cast<int64_t>(sh->heads[0]) + sh->heads[1] + sh->heads[2] > 65535 ||
       sh->B > INT32_MAX / sh->T)
     return fail(GS_ERR_UNSUPPORTED, n + ": more than 65535 heads or 2^31 tokens");

@@ -1,7 +1,7 @@
 """Layers and a loss of a language model's training step, on the gfx950 kernels.
 
-  - ``embedding_lookup`` / ``ScaledEmbedding``: rows of an embedding table times a scale; the
-    table's gradient by sorted tokens.
+  - ``embedding_lookup`` / ``ScaledEmbedding``: rows of an embedding table times a scale, and the
+    table's gradient.
   - ``qkv_norm_rotary`` / ``qk_norm_rotary`` / ``QKNormRotary``: each head's root-mean-square
     norm of the queries and keys, their rotation by position, and the heads-first layout
     attention takes, in one pass forward and one backward.
@@ -10,8 +10,8 @@
 
 All are differentiable (once), run on the current stream and take bf16 or fp32 tensors on a ROCm
 GPU; anything else raises ``GhostHipError``, as do forward-mode differentiation, function
-transforms (``torch.func``) and ``torch.jit`` tracing.  ``ScaledEmbedding`` and ``QKNormRotary`` are layers
-the engines know: ``GradDotProdEngine`` gives their weights gradient dot products and train
+transforms (``torch.func``) and ``torch.jit`` tracing.  ``ScaledEmbedding`` and ``QKNormRotary`` are
+layers the engines know: ``GradDotProdEngine`` gives their weights gradient dot products and train
 gradients, ``GradProjLoraEngine`` projects a ``ScaledEmbedding``.
 """
 from __future__ import annotations
@@ -201,7 +201,10 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor,
     reduction: 'mean' (over the rows not ignored; NaN when there are none), 'sum', or 'none' ([...]).
     The loss is fp32; no gradient reaches the teacher.
 
-    The logits are read once and their gradient written in the same pass (except with 'none')."""
+    With 'mean' and 'sum' the loss's pass also writes the logits' gradient for an upstream gradient
+    of one.  Any other, of a loss that is scaled or weighted, has the backward pass form it again:
+    951 us instead of 432 for 8192 x 50257 bf16 logits, loss and gradient.  'none' with the weights
+    as the rows' upstream gradients takes 583 us whatever they are."""
     if reduction not in ("mean", "sum", "none"):
         raise GhostHipError(f"reduction {reduction!r}: 'mean', 'sum' or 'none'")
     if labels is None and alpha != 1.0:
