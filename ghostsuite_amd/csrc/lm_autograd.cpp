@@ -531,15 +531,23 @@ struct DistillHow {
   Tensor unit, ws;   // the gradient for an upstream of one, and the scratch of the call that wrote it
 };
 
+// Elements from a tensor's first to its last.
+int64_t span_of(const Tensor& x) {
+  int64_t span = 1;
+  for (int64_t k = 0; k < x.dim(); ++k) span += (x.size(k) - 1) * x.stride(k);
+  return span;
+}
+
 // Logits as [N, V] or [B, T, V] with contiguous rows that do not overlap; a copy where the strides do
-// not allow that.
+// not allow that, or where the rows are less than half of what they lie in: their gradient has the same
+// strides, and would take its memory.
 Tensor rows_of_logits(const Tensor& logits) {
   const int64_t V = logits.size(-1);
   const Tensor z = logits.dim() == 3 ? logits : logits.reshape({-1, V});
   const int64_t T = z.size(-2);
   bool ok = (V == 1 || z.stride(-1) == 1) && (T == 1 || z.stride(-2) >= V);
   if (z.dim() == 3 && z.size(0) > 1) ok = ok && z.stride(0) >= (T - 1) * z.stride(1) + V;
-  return ok ? z : z.contiguous();
+  return ok && span_of(z) <= 2 * z.numel() ? z : z.contiguous();
 }
 
 struct DistillCall {
@@ -591,9 +599,7 @@ struct DistillCall {
   }
   Tensor empty_gradient() const {
     const auto options = z.options().requires_grad(false);
-    int64_t span = 1;
-    for (int64_t k = 0; k < z.dim(); ++k) span += (z.size(k) - 1) * z.stride(k);
-    const int64_t off = offset(z);
+    const int64_t span = span_of(z), off = offset(z);
     if (off == 0 && span == z.numel()) return at::empty(z.sizes(), options);
     return at::empty({off + span}, options).as_strided(z.sizes(), z.strides(), off);
   }

@@ -193,3 +193,33 @@ def test_distill_far_temperatures(gpu, dtype, tau):
     assert (off <= 1e-5 * (want.abs() + tau32 ** 2)).all(), (off, want)
     # an element is tau times a difference of shares up to one
     assert ((g.double().cpu() - dwant).abs() <= tau32 * (2 ** -8 * (dtype == BF16) + 2e-5)).all()
+
+
+@pytest.mark.parametrize("index", [(slice(None), -1), (slice(None), slice(3, None, 100)),
+                                   (slice(None, None, 8), slice(5, 9))])
+def test_distill_of_few_rows_of_large_logits(gpu, index):
+    """The last positions of a batch, every hundredth, a few of some samples: scratch and gradient of the
+    size of the rows, not of what lies between them; as for a copy of the rows."""
+    whole = torch.zeros(32, 400, 8192, dtype=BF16, device=gpu)
+    z = whole[index]
+    z.copy_(randn(z.shape, 1, 2.0, BF16))
+    ids = torch.randint(0, 8192, (*z.shape[:-1], 5), generator=gen(2)).to(gpu)
+    t = randn(ids.shape, 3).to(gpu)
+    labels = torch.randint(0, 8192, z.shape[:-1], generator=gen(4)).to(gpu)
+
+    def run(z):
+        z = z.detach().requires_grad_()
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        loss = gs.distillation_loss(z, ids, t, labels, temperature=2.0, alpha=0.5)
+        got = torch.autograd.grad(loss, z, retain_graph=True)[0]
+        again = torch.autograd.grad(loss, z, torch.tensor(0.5, device=gpu))[0]
+        return loss.detach(), got, again, torch.cuda.max_memory_allocated() - before
+
+    loss, got, again, peak = run(z)
+    assert peak < 8 * z.numel() * 2 + (1 << 22)     # a few copies of the rows
+    want = run(z.clone().contiguous())
+    same(loss, want[0], "loss")
+    same(got, want[1], "gradient")
+    same(again, want[2], "gradient of half the loss")
