@@ -76,6 +76,14 @@ def add_hooks(model: nn.Module, val_batch_size: int, loss_reduction: str = 'mean
             # state_dict keys stay as they were.
             lin.__dict__["_gs_tied_embedding"] = emb
     handles.append(model.register_forward_pre_hook(_new_step))
+    normed = [m for m in model.modules() if isinstance(m, QKNormRotary)]
+    if normed:
+        def forget_sample_grads(module, inputs):
+            # Tensors of a forward without a backward pass: a captured graph, whose replays write
+            # them, would not own their memory.
+            for m in normed:
+                m.__dict__.pop("_gs_sample_grads", None)
+        handles.append(model.register_forward_pre_hook(forget_sample_grads))
     model.__dict__.setdefault("autograd_grad_sample_hooks", []).extend(handles)
 
 

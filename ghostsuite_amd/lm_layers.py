@@ -158,8 +158,8 @@ class QKNormRotary(nn.Module):
             # An engine's backward hook reads these: the positions, and each sample's gradients of
             # the weights, which the backward pass forms on its way (it runs before the hook when
             # the input has a gradient).  A forward whose tensor no hook has taken yet leaves it to
-            # the next one: activation checkpointing runs the forward again within the backward pass
-            # of the first run's nodes, which write the tensor they were given.
+            # the next one of the model's step: activation checkpointing runs the forward again within
+            # the backward pass of the first run's nodes, which write the tensor they were given.
             d = self.__dict__
             if torch.is_grad_enabled() and qkv.requires_grad:
                 shape = (2, qkv.shape[0], self.head_dim)

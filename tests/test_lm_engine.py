@@ -107,3 +107,19 @@ def test_engine_dots_without_what_a_backward_pass_left(oracle_ops, monkeypatch):
     for a, b in zip(results(), want):
         assert_close(a, b, 1e-6)
     eng.detach()
+
+
+def test_sample_gradients_of_an_earlier_step_are_not_used_again(oracle_ops):
+    """A step without a backward pass leaves nothing that a later one, which may be captured into a
+    graph, would write."""
+    net = _Net()
+    eng = GradDotProdEngine(net, val_batch_size=2, use_dummy_bias=False, precision="fp32")
+    eng.attach(torch.optim.SGD(net.parameters(), lr=0.0))
+    ids = torch.randint(0, 13, (5, 4))
+    net(ids)
+    first = net.qk._gs_sample_grads
+    loss = net(ids).sum()
+    assert first is not None and net.qk._gs_sample_grads is not first
+    loss.backward()
+    assert net.qk.__dict__.get("_gs_sample_grads") is None and first._version == 0
+    eng.detach()
