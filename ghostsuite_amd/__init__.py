@@ -10,13 +10,16 @@ import torch  # noqa: F401  (loads the HIP runtime that libghost_hip.so binds to
 from .graddotprod_engine import GradDotProdEngine
 from .engine_manager import GhostEngineManager
 from .gradProjection.gradproj_engine import GradProjLoraEngine, GradProjLoRAEngine
-from .lm_layers import (QKNormRotary, ScaledEmbedding, distillation_loss, embedding_lookup,
-                        qk_norm_rotary, qkv_norm_rotary, rotary_table)
+from .lm_layers import (HeadCrossEntropy, QKNormRotary, RMSNorm, ScaledEmbedding, add_rms_norm,
+                        distillation_loss, embedding_lookup, head_cross_entropy, qk_norm_rotary,
+                        qkv_norm_rotary, rms_norm, rotary_table)
+from .optim import AdamW
 
 __all__ = ['GradDotProdEngine', 'GhostEngineManager', 'GradProjLoraEngine',
            'GradProjLoRAEngine', 'install_as_ghostEngines', 'ScaledEmbedding', 'QKNormRotary',
            'embedding_lookup', 'rotary_table', 'qkv_norm_rotary', 'qk_norm_rotary',
-           'distillation_loss']
+           'distillation_loss', 'head_cross_entropy', 'HeadCrossEntropy', 'rms_norm',
+           'add_rms_norm', 'RMSNorm', 'AdamW']
 
 
 def install_as_ghostEngines() -> None:

@@ -45,6 +45,7 @@ _I64 = ctypes.c_int64
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
+_D = ctypes.c_double
 _SZ = ctypes.c_size_t
 
 _SIGNATURES = {
@@ -117,6 +118,19 @@ _SIGNATURES = {
     "gs_distill_workspace": (_SZ, [_P]),
     "gs_distill_loss": (_I, [_P, _P, _P, _P, _SZ, _P]),
     "gs_distill_grad": (_I, [_P, _P, _I, _P, _P, _SZ, _P]),
+    "gs_head_loss_workspace": (_SZ, [_P]),
+    "gs_head_loss": (_I, [_P, _P, _P, _P, _SZ, _P]),
+    "gs_head_grad_workspace": (_SZ, [_P]),
+    "gs_head_grad": (_I, [_P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "gs_head_logit_grad_workspace": (_SZ, [_P, _I64, _I64]),
+    "gs_head_logit_grad": (_I, [_P, _P, _P, _I64, _I64, _P, _I64, _P, _SZ, _P]),
+    "gs_rms_norm": (_I, [_P, _P, _P, _I, _I64, _I64, _F, _P, _P, _P]),
+    "gs_rms_norm_grad_workspace": (_SZ, [_I64, _I64]),
+    "gs_rms_norm_grad": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _F, _P, _P, _P, _SZ, _P]),
+    "gs_rms_norm_dot_workspace": (_SZ, [_I64, _I64, _I64]),
+    "gs_rms_norm_dot": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _I64, _F, _P, _P, _I, _F, _P, _SZ,
+                             _P]),
+    "gs_adamw": (_I, [_P, _I64, _I, _I, _D, _D, _D, _D, _D, _I64, ctypes.c_uint32, _P]),
 }
 
 
@@ -829,6 +843,40 @@ class HipOps:
         """gs_distill_loss; its gradient gs_distill_grad."""
         return _lm().distillation_loss(logits, teacher_ids, teacher_logits, labels, temperature,
                                        alpha, ignore_index, REDUCTIONS[reduction])
+
+    # ---- output projection with its cross entropy, root-mean-square norm (lm_layers), AdamW (optim)
+
+    def head_cross_entropy(self, x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
+                           ignore_index: int, reduction: str,
+                           lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """gs_head_loss; its gradient gs_head_grad.  lse ([rows] fp32): the forward pass writes each
+        counted row's log2 of the sum of exponentials there, for head_logit_grad."""
+        return _lm().head_cross_entropy(x, weight, labels, ignore_index, REDUCTIONS[reduction], lse)
+
+    def head_logit_grad(self, x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
+                        lse: torch.Tensor, grad: torch.Tensor, v0: int, n: int, ignore_index: int,
+                        reduction: str) -> torch.Tensor:
+        """The gradient of the logits [v0, v0 + n), [*labels.shape, n up to a multiple of 8] with zeros
+        behind, from the loss's: gs_head_logit_grad."""
+        return _lm().head_logit_grad(x, weight, labels, lse, grad, v0, n, ignore_index,
+                                     REDUCTIONS[reduction])
+
+    def rms_norm(self, x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor,
+                 eps: float):
+        """[y], or with a residual [y, h]: gs_rms_norm; its gradient gs_rms_norm_grad."""
+        return _lm().rms_norm(x, residual, weight, eps)
+
+    def rms_norm_dot(self, h: torch.Tensor, grad: torch.Tensor, weight: torch.Tensor, eps: float,
+                     n_val: int, *, val_start: Optional[int] = None,
+                     grad_scale: Optional[float] = None):
+        """[dots, train gradient of the weight] (the gradient None without grad_scale), h as the norm
+        took it: gs_rms_norm_dot."""
+        return _lm().rms_norm_dot(h, grad, weight, eps, n_val, val_start, grad_scale)
+
+    def adamw(self, params, states, bits: int, lr: float, beta1: float, beta2: float, eps: float,
+              weight_decay: float, step: int, seed: int) -> None:
+        """One step of the parameters, in place, from their .grad and states (dicts): gs_adamw."""
+        _lm().adamw(params, states, bits, lr, beta1, beta2, eps, weight_decay, step, seed)
 
 
 _backend = None

@@ -19,7 +19,7 @@ import torch
 import torch.nn as nn
 
 from . import _overlap
-from .lm_layers import QKNormRotary
+from .lm_layers import HeadCrossEntropy, QKNormRotary, RMSNorm
 from .supported_layers_grad_samplers_dotprod import (
     APPLIED,
     _param,
@@ -104,7 +104,9 @@ def _new_step(module, inputs):
 def _capture_activations(layer: nn.Module, inputs: Tuple, outputs: Tuple):
     """Forward hook: caches the (detached) layer input (reference :92-94)."""
     d = layer.__dict__   # plain attributes, without nn.Module.__setattr__'s searches
-    d["activations"] = inputs[0].detach()
+    # an RMSNorm with a residual returns the rows that it normed beside what became of them
+    rows = outputs[1] if isinstance(layer, RMSNorm) and isinstance(outputs, tuple) else inputs[0]
+    d["activations"] = rows.detach()
     d["_gs_fwd_seq"] = (_current_step[0], next(_fwd_counter))
 
 
@@ -122,13 +124,20 @@ def _prepare_sample_grad_or_dotprod(layer: nn.Module, grad_output: Tuple[torch.T
             d["_gs_grad_outputs"] = others = tuple(None if g is None else g.detach()
                                                    for g in grad_output)
             others += (d.get("_gs_positions"),)
+    elif grad_output[0] is None and isinstance(layer, RMSNorm):   # only its residual stream was used
+        backprops = torch.zeros_like(d["activations"])
     else:
         backprops = grad_output[0].detach()
     d.setdefault("activations", None)
+    # the loss that a HeadCrossEntropy ended in: samples are those of its input
+    head = isinstance(layer, HeadCrossEntropy) and d.get("_gs_head")
+    samples_in = d["activations"] if head else backprops
+    if head:
+        others = head
     compute_layer_dotprod, _ = _supported_layers_dotprod.get(type(layer))
 
-    scale = float(backprops.shape[0]) if loss_reduction == 'mean' else 1.0
-    n_train = backprops.shape[0] - val_batch_size
+    scale = float(samples_in.shape[0]) if loss_reduction == 'mean' else 1.0
+    n_train = samples_in.shape[0] - val_batch_size
     if n_train > 0:
         # Train-gradient scales for the fused bias / LayerNorm passes.  The bias path always
         # divides by n_train (_apply_train_grad is called without loss_reduction, :67).
@@ -141,7 +150,9 @@ def _prepare_sample_grad_or_dotprod(layer: nn.Module, grad_output: Tuple[torch.T
         if options["overlap"] and _worth_overlapping(layer, acts, backprops) else \
         contextlib.nullcontext()
     with side:
-        if acts is not None and acts.dtype != backprops.dtype and acts.is_floating_point():
+        if head:
+            compute_layer_dotprod(layer, acts, backprops, val_batch_size=val_batch_size)
+        elif acts is not None and acts.dtype != backprops.dtype and acts.is_floating_point():
             common = torch.promote_types(acts.dtype, backprops.dtype)
             compute_layer_dotprod(layer, acts.to(common), backprops.to(common),
                                   val_batch_size=val_batch_size)
@@ -184,7 +195,7 @@ def _apply_train_grad(layer: nn.Module, val_batch_size: int, loss_reduction: str
         for attr in ('activations', 'backprops', 'backprops_scale', '_gs_bias_train_grad',
                      '_gs_weight_train_grad', '_gs_ln_train_grads', '_gs_bias_grad_scale',
                      '_gs_ln_grad_scale', '_gs_grad_outputs', '_gs_positions',
-                     '_gs_sample_grads'):
+                     '_gs_sample_grads', '_gs_head'):
             layer.__dict__.pop(attr, None)
 
 
@@ -209,8 +220,10 @@ def _worth_overlapping(layer: nn.Module, acts, backprops) -> bool:
         return False   # each sample's gradients are there: a few kilobytes are left to do
     if acts.numel() + backprops.numel() > _INLINE_ELEMENTS:
         return True
-    if isinstance(layer, (nn.LayerNorm, nn.Embedding, QKNormRotary)):
+    if isinstance(layer, (nn.LayerNorm, nn.Embedding, QKNormRotary, RMSNorm)):
         return False
+    if layer.__dict__.get("_gs_head") is not None:
+        return 2.0 * acts.numel() * layer.weight.shape[0] > _INLINE_FLOPS
     if isinstance(layer, nn.Conv2d):   # channels first: every output element takes a filter's size
         return 2.0 * backprops.numel() * layer.weight[0].numel() > _INLINE_FLOPS
     return 2.0 * acts.numel() * backprops.shape[-1] > _INLINE_FLOPS
@@ -219,7 +232,7 @@ def _worth_overlapping(layer: nn.Module, acts, backprops) -> bool:
 def _train_grads_parked(layer: nn.Module) -> bool:
     """True when the dot stage parked every train gradient this layer applies."""
     d = layer.__dict__
-    if isinstance(layer, (nn.LayerNorm, QKNormRotary)):
+    if isinstance(layer, (nn.LayerNorm, QKNormRotary, RMSNorm)):
         return "_gs_ln_train_grads" in d
     w = _param(layer, "weight")
     if w is None or not getattr(w, "initially_requires_grad", False) or \
@@ -233,7 +246,7 @@ def _train_grads_parked(layer: nn.Module) -> bool:
 def _apply_train_grad_body(layer: nn.Module, compute_layer_train_grad, val_batch_size: int,
                            scale: float, loss_reduction: str):
     """The train gradients of one layer (weight, then bias) into ``param.train_grad``."""
-    if isinstance(layer, (nn.LayerNorm, QKNormRotary)):   # apply their gradients themselves
+    if isinstance(layer, (nn.LayerNorm, QKNormRotary, RMSNorm)):   # apply their gradients themselves
         compute_layer_train_grad(layer, layer.activations, layer.backprops, val_batch_size,
                                  scale=scale)
     else:

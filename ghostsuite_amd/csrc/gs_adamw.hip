@@ -1,0 +1,290 @@
+// One step of AdamW over many tensors at once, its averages held in 32 or in 8 bits.
+//
+// Per element, t the steps taken with this one:
+//   m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2
+//   p = (1 - lr decay) p - lr / (1 - b1^t) m / ((v / (1 - b2^t))^(1/2) + eps)
+// in fp32, p rounded once to its type.  Bound by memory: every array is read once and written once.
+// A launch takes many tensors (their addresses travel in its arguments); its workgroups take runs
+// of CHUNK elements, a tensor's last one shorter, and find their tensor by its first run.
+//
+// In 8 bits, 256 consecutive elements (a block) share a scale, the largest magnitude over 448, and
+// each holds its value over the scale as a float of 4 exponent and 3 mantissa bits.  Held are m and
+// the root of v: the root halves v's range in powers of two, so that an element 2^-17 of its block's
+// largest root still counts.  A nearest rounding would keep an average where it is whenever one
+// step moves it by less than half of an eighth: with b2 = 0.999 nearly always.  So the rounding
+// goes up or down by chance, with the odds that keep m and the root right on average: t + u rounded
+// down, u spread evenly over [0, 1) by a hash of the element's place, the step and the seed, the
+// same on every run.  (v, the root's square, comes out high by the rounding's variance: at most the
+// sixteenth of its drift, a few hundredths of it where gradients are noise.)  A root that is not
+// zero never becomes zero, nor less than half of itself: where the gradient stops, m is not divided
+// by eps alone.  p is formed from m and v before their rounding.  A value that is not finite is held
+// as NaN and has no part in its block's scale.
+
+#include <algorithm>
+#include <cmath>
+
+#include "gs_common.h"
+
+namespace gs {
+namespace {
+
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+constexpr int NT = 256, BLOCK = GS_ADAMW_BLOCK, VE = 8;
+constexpr int CHUNK = 8192;          // elements of a workgroup
+constexpr int MOST = 48;             // tensors of a launch (3.5 KB of arguments)
+constexpr float TOP = 448.f;
+
+struct Tensors {
+  gs_adamw_tensor t[MOST];
+  int32_t first[MOST + 1];           // each tensor's first run
+  int count;
+};
+struct Factors {
+  float keep, b1, b2, rest1, rest2;  // 1 - lr decay, b1, b2, 1 - b1, 1 - b2
+  float step, root, eps;             // lr / (1 - b1^t), (1 - b2^t)^(-1/2)
+  uint32_t key;
+};
+
+// The tensor of a run, by halves; uniform over the workgroup.
+__device__ __forceinline__ int tensor_of(const Tensors& a, int run) {
+  int lo = 0, hi = a.count;          // first[lo] <= run < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (a.first[mid] <= run) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+template <class E>
+struct Eight {
+  float v[VE];
+  __device__ __forceinline__ void load(const E* p, bool vec, int64_t left) {
+    if (vec && left >= VE) {
+      union { uint4 u[sizeof(E) / 2]; E e[VE]; } w;
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(E) / 2); ++i)
+        w.u[i] = reinterpret_cast<const uint4*>(p)[i];
+#pragma unroll
+      for (int i = 0; i < VE; ++i) v[i] = to_f32<E>(w.e[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) v[i] = i < left ? to_f32<E>(p[i]) : 0.f;
+    }
+  }
+  __device__ __forceinline__ void store(E* p, bool vec, int64_t left) const {
+    if (vec && left >= VE) {
+      union { uint4 u[sizeof(E) / 2]; E e[VE]; } w;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) w.e[i] = from_f32<E>(v[i]);
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(E) / 2); ++i)
+        reinterpret_cast<uint4*>(p)[i] = w.u[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i)
+        if (i < left) p[i] = from_f32<E>(v[i]);
+    }
+  }
+};
+
+__device__ __forceinline__ float update(float p, float m, float root, const Factors& f) {
+  return f.keep * p - f.step * m / (root * f.root + f.eps);
+}
+
+template <class E>
+__global__ void __launch_bounds__(NT) adamw_kernel(Tensors a, Factors f) {
+  const int k = tensor_of(a, blockIdx.x);
+  const gs_adamw_tensor& t = a.t[k];
+  const int64_t first = static_cast<int64_t>(static_cast<int>(blockIdx.x) - a.first[k]) * CHUNK;
+  const bool vec = ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.g) |
+                     reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v)) & 15) == 0;
+  float* tm = static_cast<float*>(t.m);
+  float* tv = static_cast<float*>(t.v);
+#pragma unroll
+  for (int64_t o = 0; o < CHUNK; o += NT * VE) {
+    const int64_t i = first + o + threadIdx.x * VE, left = t.n - i;
+    if (left <= 0) return;
+    Eight<E> p, g;
+    Eight<float> m, v;
+    p.load(static_cast<const E*>(t.p) + i, vec, left);
+    g.load(static_cast<const E*>(t.g) + i, vec, left);
+    m.load(tm + i, vec, left);
+    v.load(tv + i, vec, left);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      m.v[e] = f.b1 * m.v[e] + f.rest1 * g.v[e];
+      v.v[e] = f.b2 * v.v[e] + f.rest2 * (g.v[e] * g.v[e]);
+      p.v[e] = update(p.v[e], m.v[e], sqrtf(v.v[e]), f);
+    }
+    p.store(static_cast<E*>(t.p) + i, vec, left);
+    m.store(tm + i, vec, left);
+    v.store(tv + i, vec, left);
+  }
+}
+
+// The largest of 32 lanes (half a wave holds a block), in each of them.
+__device__ __forceinline__ float half_max(float v) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+  return v;
+}
+
+// a of [0, 448] on the 8-bit values, up or down by u of [0, 1).
+__device__ __forceinline__ float eighth(float a, float u) {
+  // the values' steps: 2^-9 below 2^-6, then an eighth of each power of two; both powers exact
+  const uint32_t e = std::max(__float_as_uint(a) >> 23, 121u);
+  const float t = a * __uint_as_float((257u - e) << 23);    // a / 2^(e - 127 - 3)
+  return fminf(floorf(t + u) * __uint_as_float((e - 3u) << 23), TOP);
+}
+// Four 8-bit values from their floats, which they hold exactly, and back.
+__device__ __forceinline__ uint32_t pack8(const float* v) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true));
+}
+__device__ __forceinline__ void unpack8(uint32_t w, float* v) {
+  v[0] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(w), 0);
+  v[1] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(w), 1);
+  v[2] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(w), 2);
+  v[3] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(w), 3);
+}
+__device__ __forceinline__ void load8(const uint8_t* p, bool vec, int64_t left, float (&v)[VE]) {
+  uint32_t w[2] = {0, 0};
+  if (vec && left >= VE) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    w[0] = u.x, w[1] = u.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; ++i)
+      if (i < left) w[i / 4] |= static_cast<uint32_t>(p[i]) << (8 * (i % 4));
+  }
+  unpack8(w[0], v);
+  unpack8(w[1], v + 4);
+}
+__device__ __forceinline__ void store8(uint8_t* p, bool vec, int64_t left, const float (&v)[VE]) {
+  const uint32_t w[2] = {pack8(v), pack8(v + 4)};
+  if (vec && left >= VE) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; ++i)
+      if (i < left) p[i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i % 4)));
+  }
+}
+
+__device__ __forceinline__ bool is_finite(float v) { return fabsf(v) < INFINITY; }
+
+template <class E>
+__global__ void __launch_bounds__(NT) adamw8_kernel(Tensors a, Factors f) {
+  const int k = tensor_of(a, blockIdx.x);
+  const gs_adamw_tensor& t = a.t[k];
+  const int64_t first = static_cast<int64_t>(static_cast<int>(blockIdx.x) - a.first[k]) * CHUNK;
+  const bool vec = ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.g)) & 15) == 0;
+  uint8_t* tm = static_cast<uint8_t*>(t.m);
+  uint8_t* tv = static_cast<uint8_t*>(t.v);
+  const bool vec8 = ((reinterpret_cast<uintptr_t>(tm) | reinterpret_cast<uintptr_t>(tv)) & 7) == 0;
+#pragma unroll
+  for (int64_t o = 0; o < CHUNK; o += NT * VE) {
+    const int64_t i = first + o + threadIdx.x * VE, left = t.n - i;
+    const int64_t b = i / BLOCK;
+    const bool live = b * BLOCK < t.n;   // the same for the 32 lanes of a block
+    float sm = 0.f, sr = 0.f;
+    if (live) sm = t.m_scale[b], sr = t.v_scale[b];
+    Eight<E> p, g;
+    float m[VE], r[VE];
+    p.load(static_cast<const E*>(t.p) + i, vec, left);
+    g.load(static_cast<const E*>(t.g) + i, vec, left);
+    load8(tm + i, vec8, left, m);
+    load8(tv + i, vec8, left, r);
+    float top_m = 0.f, top_r = 0.f;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      m[e] = f.b1 * (m[e] * sm) + f.rest1 * g.v[e];
+      const float old = r[e] * sr;
+      r[e] = sqrtf(f.b2 * (old * old) + f.rest2 * (g.v[e] * g.v[e]));
+      p.v[e] = update(p.v[e], m[e], r[e], f);
+      top_m = fmaxf(top_m, is_finite(m[e]) ? fabsf(m[e]) : 0.f);
+      top_r = fmaxf(top_r, is_finite(r[e]) ? r[e] : 0.f);
+    }
+    p.store(static_cast<E*>(t.p) + i, vec, left);
+    top_m = half_max(top_m);
+    top_r = half_max(top_r);
+    const float im = top_m > 0.f ? TOP / top_m : 0.f, ir = top_r > 0.f ? TOP / top_r : 0.f;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      uint32_t x = (static_cast<uint32_t>(i + e) + f.key) * 0x9E3779B9u;
+      x = (x ^ (x >> 15)) * 0xBB67AE85u;
+      x ^= x >> 13;
+      const float um = (static_cast<float>(x & 0xFFFFu) + 0.5f) * 0x1p-16f;
+      const float ur = (static_cast<float>(x >> 16) + 0.5f) * 0x1p-16f;
+      m[e] = is_finite(m[e]) ? copysignf(eighth(fabsf(m[e]) * im, um), m[e]) : NAN;
+      const float held = r[e] > 0.f ? fmaxf(eighth(r[e] * ir, ur), 0x1p-9f) : 0.f;
+      r[e] = is_finite(r[e]) ? held : NAN;
+    }
+    store8(tm + i, vec8, left, m);
+    store8(tv + i, vec8, left, r);
+    if (live && (threadIdx.x & 31) == 0) t.m_scale[b] = top_m / TOP, t.v_scale[b] = top_r / TOP;
+  }
+}
+
+}  // namespace
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" int gs_adamw(const gs_adamw_tensor* tensors, int64_t count, int dtype, int state_bits,
+                        double lr, double beta1, double beta2, double eps, double weight_decay,
+                        int64_t step, uint32_t seed, void* stream) {
+  if (dtype != GS_DTYPE_BF16 && dtype != GS_DTYPE_F32)
+    return fail(GS_ERR_DTYPE, "gs_adamw: dtype must be bf16 or fp32");
+  if (count < 0 || (count > 0 && tensors == nullptr) || (state_bits != 8 && state_bits != 32) ||
+      step < 1 || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0))
+    return fail(GS_ERR_INVALID, "gs_adamw: invalid arguments");
+  for (int64_t i = 0; i < count; ++i) {
+    const gs_adamw_tensor& t = tensors[i];
+    if (t.n < 0 || (t.n > 0 && (t.p == nullptr || t.g == nullptr || t.m == nullptr || t.v == nullptr ||
+                                (state_bits == 8 && (t.m_scale == nullptr || t.v_scale == nullptr)))))
+      return fail(GS_ERR_INVALID, "gs_adamw: invalid tensor");
+    if (t.n > (int64_t{1} << 42))
+      return fail(GS_ERR_UNSUPPORTED, "gs_adamw: a tensor of more than 2^42 elements");
+  }
+  Factors f{};
+  f.keep = static_cast<float>(1.0 - lr * weight_decay);
+  f.b1 = static_cast<float>(beta1), f.b2 = static_cast<float>(beta2);
+  f.rest1 = static_cast<float>(1.0 - beta1), f.rest2 = static_cast<float>(1.0 - beta2);
+  f.step = static_cast<float>(lr / (1.0 - std::pow(beta1, static_cast<double>(step))));
+  f.root = static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(beta2, static_cast<double>(step))));
+  f.eps = static_cast<float>(eps);
+  f.key = static_cast<uint32_t>(step) * 0x9E3779B9u + seed * 0x6A09E667u;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  Tensors a;
+  bool launched = false;
+  for (int64_t i = 0; i < count;) {
+    a.count = 0;
+    int64_t runs = 0;
+    for (; i < count && a.count < MOST; ++i) {
+      if (tensors[i].n == 0) continue;
+      const int64_t more = cdiv(tensors[i].n, CHUNK);
+      if (runs + more > INT32_MAX && a.count > 0) break;
+      a.t[a.count] = tensors[i];
+      a.first[a.count++] = static_cast<int32_t>(runs);
+      runs += more;
+    }
+    if (a.count == 0) break;
+    launched = true;
+    a.first[a.count] = static_cast<int32_t>(runs);
+    const dim3 grid(static_cast<unsigned>(runs));
+    if (state_bits == 32) {
+      if (dtype == GS_DTYPE_BF16)
+        hipLaunchKernelGGL(adamw_kernel<uint16_t>, grid, dim3(NT), 0, s, a, f);
+      else
+        hipLaunchKernelGGL(adamw_kernel<float>, grid, dim3(NT), 0, s, a, f);
+    } else {
+      if (dtype == GS_DTYPE_BF16)
+        hipLaunchKernelGGL(adamw8_kernel<uint16_t>, grid, dim3(NT), 0, s, a, f);
+      else
+        hipLaunchKernelGGL(adamw8_kernel<float>, grid, dim3(NT), 0, s, a, f);
+    }
+  }
+  return launched ? check_launch("gs_adamw") : GS_OK;
+}

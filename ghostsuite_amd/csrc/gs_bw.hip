@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(BW_THREADS) colsum_kernel(const E* __restrict_
 // mean/rstd by wave reductions (two passes over registers), g*xhat and g accumulated per
 // lane over the block's tokens; the waves combine through LDS.
 constexpr int LN_WAVES = 8;
-template <class E, int PC>
+template <class E, int PC, bool RMS>
 __global__ void __launch_bounds__(64 * LN_WAVES) ln_sums_kernel(
     const E* __restrict__ X, const E* __restrict__ G, int64_t T, int64_t F, float eps,
     int64_t chunks, int vec, float* __restrict__ part_w, float* __restrict__ part_b) {
@@ -111,12 +111,15 @@ __global__ void __launch_bounds__(64 * LN_WAVES) ln_sums_kernel(
   if (t0 + wid < t1) load_row(t0 + wid, xv, gv);
   for (int64_t t = t0 + wid; t < t1; t += LN_WAVES) {
     if (t + LN_WAVES < t1) load_row(t + LN_WAVES, xn, gn);
-    float s = 0.f;
+    float mean = 0.f;
+    if constexpr (!RMS) {
+      float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < PC; ++k)
+      for (int k = 0; k < PC; ++k)
 #pragma unroll
-      for (int i = 0; i < VE; ++i) s += xv[k].v[i];
-    const float mean = wave_sum_dpp(s) * invF;
+        for (int i = 0; i < VE; ++i) s += xv[k].v[i];
+      mean = wave_sum_dpp(s) * invF;
+    }
     float var = 0.f;
 #pragma unroll
     for (int k = 0; k < PC; ++k) {
@@ -189,7 +192,7 @@ __global__ void __launch_bounds__(64 * LN_WAVES) ln_sums_kernel(
 // LN2_WAVES waves per block over LN_TOK_CHUNK tokens; the wave x row-group sums combine
 // through LDS [LN2_WAVES * RW][F] (x2) in a fixed order.
 constexpr int LN2_WAVES = 4;
-template <class E, int PC, int RW>
+template <class E, int PC, int RW, bool RMS>
 __global__ void __launch_bounds__(64 * LN2_WAVES) ln_rows_kernel(
     const E* __restrict__ X, const E* __restrict__ G, int64_t T, int64_t F, float eps,
     int64_t chunks, float* __restrict__ part_w, float* __restrict__ part_b) {
@@ -242,12 +245,15 @@ __global__ void __launch_bounds__(64 * LN2_WAVES) ln_rows_kernel(
       float x[PC][VE];
 #pragma unroll
       for (int k = 0; k < PC; ++k) widen(xr[k], x[k]);
-      float sx = 0.f;
+      float mean = 0.f;
+      if constexpr (!RMS) {
+        float sx = 0.f;
 #pragma unroll
-      for (int k = 0; k < PC; ++k)
+        for (int k = 0; k < PC; ++k)
 #pragma unroll
-        for (int i = 0; i < VE; ++i) sx += x[k][i];
-      const float mean = group_sum(sx) * invF;
+          for (int i = 0; i < VE; ++i) sx += x[k][i];
+        mean = group_sum(sx) * invF;
+      }
       float var = 0.f;
 #pragma unroll
       for (int k = 0; k < PC; ++k) {
@@ -310,7 +316,7 @@ __global__ void __launch_bounds__(64 * LN2_WAVES) ln_rows_kernel(
 // walking the chunk's tokens, and writes the same per-(sample, chunk) partials.
 constexpr int64_t LN_REG_MAX_F = 2048;
 constexpr int LNS_WAVES = 4;
-template <class E>
+template <class E, bool RMS>
 __global__ void __launch_bounds__(64 * LNS_WAVES) ln_row_stats_kernel(
     const E* __restrict__ X, int64_t rows, int64_t F, float eps, int vec,
     float2* __restrict__ stats) {
@@ -320,14 +326,17 @@ __global__ void __launch_bounds__(64 * LNS_WAVES) ln_row_stats_kernel(
   if (r >= rows) return;
   const E* xr = X + r * F;
   const float invF = 1.0f / static_cast<float>(F);
-  float s = 0.f;
-  for (int64_t f = static_cast<int64_t>(lane) * VE; f < F; f += 64 * VE) {
-    Vec<E> x;
-    x.load(xr + f, vec && f + VE <= F, F - f);
+  float mean = 0.f;
+  if constexpr (!RMS) {
+    float s = 0.f;
+    for (int64_t f = static_cast<int64_t>(lane) * VE; f < F; f += 64 * VE) {
+      Vec<E> x;
+      x.load(xr + f, vec && f + VE <= F, F - f);
 #pragma unroll
-    for (int i = 0; i < VE; ++i) s += x.v[i];
+      for (int i = 0; i < VE; ++i) s += x.v[i];
+    }
+    mean = wave_sum_dpp(s) * invF;
   }
-  const float mean = wave_sum_dpp(s) * invF;
   float q = 0.f;
   for (int64_t f = static_cast<int64_t>(lane) * VE; f < F; f += 64 * VE) {
     Vec<E> x;
@@ -636,27 +645,27 @@ bool batch_ok(int64_t N, int64_t n_val, int64_t val_start, int64_t T, int64_t F)
          F > 0;
 }
 
-template <class E, int PC>
+template <class E, bool RMS, int PC>
 void launch_ln(const void* X, const void* G, int64_t N, int64_t T, int64_t F, float eps,
                int64_t chunks, int vec, float* pw, float* pb, hipStream_t s) {
   const size_t lds = LN_WAVES * F * sizeof(float);
-  hipLaunchKernelGGL((ln_sums_kernel<E, PC>),
+  hipLaunchKernelGGL((ln_sums_kernel<E, PC, RMS>),
                      dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(N)),
                      dim3(64 * LN_WAVES), lds, s, static_cast<const E*>(X),
                      static_cast<const E*>(G), T, F, eps, chunks, vec, pw, pb);
 }
 
-template <class E, int PC, int RW>
+template <class E, bool RMS, int PC, int RW>
 void launch_ln_rows(const void* X, const void* G, int64_t N, int64_t T, int64_t F, float eps,
                     int64_t chunks, float* pw, float* pb, hipStream_t s) {
   const size_t lds = 2 * LN2_WAVES * RW * F * sizeof(float);
-  hipLaunchKernelGGL((ln_rows_kernel<E, PC, RW>),
+  hipLaunchKernelGGL((ln_rows_kernel<E, PC, RW, RMS>),
                      dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(N)),
                      dim3(64 * LN2_WAVES), lds, s, static_cast<const E*>(X),
                      static_cast<const E*>(G), T, F, eps, chunks, pw, pb);
 }
 
-template <class E>
+template <class E, bool RMS>
 int launch_ln_wide(const void* X, const void* G, int64_t N, int64_t T, int64_t F, float eps,
                    int64_t chunks, float* pw, float* pb, float2* stats, hipStream_t s) {
   constexpr int VE = Vec<E>::VE;
@@ -664,7 +673,7 @@ int launch_ln_wide(const void* X, const void* G, int64_t N, int64_t T, int64_t F
                   (reinterpret_cast<uintptr_t>(G) % 16 == 0) && (F * sizeof(E)) % 16 == 0;
   const int64_t rows = N * T, fblocks = cdiv(F, int64_t{BW_THREADS} * VE);
   if (fblocks > 65535) return fail(GS_ERR_UNSUPPORTED, "gs_layernorm_dot: grid too large");
-  hipLaunchKernelGGL(ln_row_stats_kernel<E>, dim3(static_cast<unsigned>(cdiv(rows, LNS_WAVES))),
+  hipLaunchKernelGGL((ln_row_stats_kernel<E, RMS>), dim3(static_cast<unsigned>(cdiv(rows, LNS_WAVES))),
                      dim3(64 * LNS_WAVES), 0, s, static_cast<const E*>(X), rows, F, eps, vec,
                      stats);
   hipLaunchKernelGGL(ln_feat_kernel<E>,
@@ -675,7 +684,7 @@ int launch_ln_wide(const void* X, const void* G, int64_t N, int64_t T, int64_t F
   return check_launch("ln_row_stats_kernel / ln_feat_kernel");
 }
 
-template <class E>
+template <class E, bool RMS>
 int launch_ln_any(const void* X, const void* G, int64_t N, int64_t T, int64_t F, float eps,
                   int64_t chunks, float* pw, float* pb, hipStream_t s) {
   constexpr int VE = 16 / sizeof(E);
@@ -687,30 +696,30 @@ int launch_ln_any(const void* X, const void* G, int64_t N, int64_t T, int64_t F,
   if (vec && 2 * LN2_WAVES * rw * F * static_cast<int64_t>(sizeof(float)) <= 64 * 1024) {
     // Aligned rows: two rows per wave while 32 lanes x 4 chunks cover a row, else one.
     if (fchunks <= 32 * 2)
-      launch_ln_rows<E, 2, 2>(X, G, N, T, F, eps, chunks, pw, pb, s);
+      launch_ln_rows<E, RMS, 2, 2>(X, G, N, T, F, eps, chunks, pw, pb, s);
     else if (fchunks <= 32 * 3)
-      launch_ln_rows<E, 3, 2>(X, G, N, T, F, eps, chunks, pw, pb, s);
+      launch_ln_rows<E, RMS, 3, 2>(X, G, N, T, F, eps, chunks, pw, pb, s);
     else if (fchunks <= 32 * 4)
-      launch_ln_rows<E, 4, 2>(X, G, N, T, F, eps, chunks, pw, pb, s);
+      launch_ln_rows<E, RMS, 4, 2>(X, G, N, T, F, eps, chunks, pw, pb, s);
     else if (fchunks <= 64 * 4)
-      launch_ln_rows<E, 4, 1>(X, G, N, T, F, eps, chunks, pw, pb, s);
+      launch_ln_rows<E, RMS, 4, 1>(X, G, N, T, F, eps, chunks, pw, pb, s);
     else if (fchunks <= 64 * 6)
-      launch_ln_rows<E, 6, 1>(X, G, N, T, F, eps, chunks, pw, pb, s);
+      launch_ln_rows<E, RMS, 6, 1>(X, G, N, T, F, eps, chunks, pw, pb, s);
     else if (fchunks <= 64 * 8)
-      launch_ln_rows<E, 8, 1>(X, G, N, T, F, eps, chunks, pw, pb, s);
+      launch_ln_rows<E, RMS, 8, 1>(X, G, N, T, F, eps, chunks, pw, pb, s);
     else
       return fail(GS_ERR_UNSUPPORTED, "gs_layernorm_dot: feature count too large");
     return check_launch("ln_rows_kernel");
   }
   if (pc <= 1)
-    launch_ln<E, 1>(X, G, N, T, F, eps, chunks, vec, pw, pb, s);
+    launch_ln<E, RMS, 1>(X, G, N, T, F, eps, chunks, vec, pw, pb, s);
   else if (pc <= 2)
-    launch_ln<E, 2>(X, G, N, T, F, eps, chunks, vec, pw, pb, s);
+    launch_ln<E, RMS, 2>(X, G, N, T, F, eps, chunks, vec, pw, pb, s);
   else if (pc <= 4)
-    launch_ln<E, 4>(X, G, N, T, F, eps, chunks, vec, pw, pb, s);
+    launch_ln<E, RMS, 4>(X, G, N, T, F, eps, chunks, vec, pw, pb, s);
   else if constexpr (VE == 4) {
     if (pc <= 8)
-      launch_ln<E, 8>(X, G, N, T, F, eps, chunks, vec, pw, pb, s);
+      launch_ln<E, RMS, 8>(X, G, N, T, F, eps, chunks, vec, pw, pb, s);
     else
       return fail(GS_ERR_UNSUPPORTED, "gs_layernorm_dot: feature count too large");
   } else {
@@ -876,43 +885,48 @@ extern "C" size_t gs_layernorm_dot_workspace(int64_t N, int64_t T, int64_t F) {
   return sz.used + 256;
 }
 
-extern "C" int gs_layernorm_dot(const void* X, const void* G, int dtype, int64_t N, int64_t n_val,
-                                int64_t val_start, int64_t T, int64_t F, float eps,
-                                float* out_dot_w, float* out_dot_b, void* out_grad_w,
-                                void* out_grad_b, int grad_dtype, float grad_scale,
-                                void* workspace, size_t workspace_bytes, void* stream) {
+namespace {
+// A LayerNorm's dots and train gradients; with RMS those of a root-mean-square norm's weight (no mean,
+// no bias).
+template <bool RMS>
+int norm_dot(const char* name, const void* X, const void* G, int dtype, int64_t N, int64_t n_val,
+             int64_t val_start, int64_t T, int64_t F, float eps, float* out_dot_w, float* out_dot_b,
+             void* out_grad_w, void* out_grad_b, int grad_dtype, float grad_scale, void* workspace,
+             size_t workspace_bytes, void* stream) {
+  const auto said = [&](const char* what) { return std::string(name) + what; };
   if (dtype != GS_DTYPE_BF16 && dtype != GS_DTYPE_F32)
-    return fail(GS_ERR_DTYPE, "gs_layernorm_dot: dtype must be bf16 or fp32");
+    return fail(GS_ERR_DTYPE, said(": dtype must be bf16 or fp32"));
   if (grad_dtype != GS_DTYPE_BF16 && grad_dtype != GS_DTYPE_F32)
-    return fail(GS_ERR_DTYPE, "gs_layernorm_dot: grad_dtype must be bf16 or fp32");
+    return fail(GS_ERR_DTYPE, said(": grad_dtype must be bf16 or fp32"));
   if (!batch_ok(N, n_val, val_start, T, F) || X == nullptr || G == nullptr)
-    return fail(GS_ERR_INVALID, "gs_layernorm_dot: invalid arguments");
+    return fail(GS_ERR_INVALID, said(": invalid arguments"));
   Sizer sz;
   carve_feature(sz, N, T, F, 1);
   if (F > LN_REG_MAX_F) sz.take<float2>(N * T);
   if (workspace == nullptr || workspace_bytes < sz.used)
-    return fail(GS_ERR_WORKSPACE, "gs_layernorm_dot: workspace too small");
+    return fail(GS_ERR_WORKSPACE, said(": workspace too small"));
   Carver cv(workspace, workspace_bytes);
   const int64_t chunks = cdiv(T, LN_TOK_CHUNK);
   if (N > 65535 || chunks > 65535)  // grid y / x of the stage-1 kernels
-    return fail(GS_ERR_UNSUPPORTED, "gs_layernorm_dot: more than 65535 samples or token chunks");
+    return fail(GS_ERR_UNSUPPORTED, said(": more than 65535 samples or token chunks"));
   float* pw = cv.take<float>(N * chunks * F);
   float* pb = cv.take<float>(N * chunks * F);
   float* Sw = cv.take<float>(N * F);
   float* Sb = cv.take<float>(N * F);
   float* vw = cv.take<float>(F);
   float* vb = cv.take<float>(F);
+  if (RMS) pb = nullptr;
   hipStream_t s = static_cast<hipStream_t>(stream);
   int rc;
   if (F > LN_REG_MAX_F) {
     float2* stats = cv.take<float2>(N * T);
     rc = dtype == GS_DTYPE_BF16
-             ? launch_ln_wide<uint16_t>(X, G, N, T, F, eps, chunks, pw, pb, stats, s)
-             : launch_ln_wide<float>(X, G, N, T, F, eps, chunks, pw, pb, stats, s);
+             ? launch_ln_wide<uint16_t, RMS>(X, G, N, T, F, eps, chunks, pw, pb, stats, s)
+             : launch_ln_wide<float, RMS>(X, G, N, T, F, eps, chunks, pw, pb, stats, s);
   } else {
     rc = dtype == GS_DTYPE_BF16
-             ? launch_ln_any<uint16_t>(X, G, N, T, F, eps, chunks, pw, pb, s)
-             : launch_ln_any<float>(X, G, N, T, F, eps, chunks, pw, pb, s);
+             ? launch_ln_any<uint16_t, RMS>(X, G, N, T, F, eps, chunks, pw, pb, s)
+             : launch_ln_any<float, RMS>(X, G, N, T, F, eps, chunks, pw, pb, s);
   }
   if (rc) return rc;
   FeatureSets sets{};
@@ -921,6 +935,29 @@ extern "C" int gs_layernorm_dot(const void* X, const void* G, int dtype, int64_t
   const int nsets = (out_dot_b != nullptr || out_grad_b != nullptr) ? 2 : 1;
   return finish_feature_any(grad_dtype, sets, nsets, N, chunks, F, n_val, val_start, T,
                             grad_scale, s);
+}
+}  // namespace
+
+extern "C" int gs_layernorm_dot(const void* X, const void* G, int dtype, int64_t N, int64_t n_val,
+                                int64_t val_start, int64_t T, int64_t F, float eps,
+                                float* out_dot_w, float* out_dot_b, void* out_grad_w,
+                                void* out_grad_b, int grad_dtype, float grad_scale,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  return norm_dot<false>("gs_layernorm_dot", X, G, dtype, N, n_val, val_start, T, F, eps, out_dot_w,
+                         out_dot_b, out_grad_w, out_grad_b, grad_dtype, grad_scale, workspace,
+                         workspace_bytes, stream);
+}
+
+extern "C" size_t gs_rms_norm_dot_workspace(int64_t N, int64_t T, int64_t F) {
+  return gs_layernorm_dot_workspace(N, T, F);
+}
+
+extern "C" int gs_rms_norm_dot(const void* H, const void* G, int dtype, int64_t N, int64_t n_val,
+                               int64_t val_start, int64_t T, int64_t F, float eps, float* out_dot,
+                               void* out_grad, int grad_dtype, float grad_scale, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  return norm_dot<true>("gs_rms_norm_dot", H, G, dtype, N, n_val, val_start, T, F, eps, out_dot, nullptr,
+                        out_grad, nullptr, grad_dtype, grad_scale, workspace, workspace_bytes, stream);
 }
 
 // ------------------------------------------------------------------------------ embedding

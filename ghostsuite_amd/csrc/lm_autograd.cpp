@@ -1,6 +1,6 @@
 // Host side of the language-model operators: argument checks, allocation and automatic
-// differentiation around gs_embedding_lookup*, gs_qk_rotary* and gs_distill_*
-// (include/ghost_hip.h), as a Python extension module.
+// differentiation around gs_embedding_lookup*, gs_qk_rotary*, gs_distill_*, gs_head_*, gs_rms_norm*
+// and gs_adamw (include/ghost_hip.h), as a Python extension module.
 //
 // C++ because a training step calls these in every layer: a Python autograd function costs the host
 // 50 to 100 us a forward and backward pass (its backward pass runs on the autograd engine's thread,
@@ -674,6 +674,329 @@ Tensor distillation_loss(const Tensor& logits, const Tensor& ids, const Tensor& 
   return distill_loss(logits, ids, t, y, how, nullptr, nullptr);
 }
 
+// ------------------------------------------- output projection with its cross entropy, in pieces
+
+struct HeadHow {
+  int64_t ignore_index;
+  int reduction;
+  Tensor lse;   // each row's log2 of the sum of exponentials, which the forward pass writes
+};
+
+// The arguments of a gs_head_* call.
+struct HeadCall {
+  c10::Device dev;
+  gs_head h{};
+  Tensor x, w, labels;   // what the pointers are into
+
+  HeadCall(const Tensor& x_in, const Tensor& w_in, const Tensor& labels_in, const HeadHow& how)
+      : dev(device_of({&x_in, &w_in, &labels_in})) {
+    require(x_in.dim() >= 1 && w_in.dim() == 2 && w_in.numel() > 0 && x_in.size(-1) == w_in.size(1) &&
+                labels_in.sizes() == x_in.sizes().slice(0, x_in.dim() - 1),
+            "hidden rows ", x_in.sizes(), ", weight ", w_in.sizes(), ", labels ", labels_in.sizes(),
+            ": [..., d], [vocab, d] and [...] expected");
+    require(at::isIntegralType(labels_in.scalar_type(), false), "labels have to be integers");
+    h.dtype = gs_dtype_of(x_in, "hidden rows");
+    require(w_in.scalar_type() == x_in.scalar_type(), "hidden rows of ", x_in.scalar_type(),
+            ", weight of ", w_in.scalar_type());
+    const int64_t d = w_in.size(1);
+    x = x_in.reshape({-1, d});
+    if (!((d == 1 || x.stride(1) == 1) && (x.size(0) <= 1 || x.stride(0) >= d))) x = x.contiguous();
+    w = w_in.contiguous();
+    labels = labels_in.to(at::kLong).contiguous();
+    h.X = ptr(x), h.W = ptr(w), h.labels = static_cast<const int64_t*>(ptr(labels));
+    h.N = x.size(0), h.V = w.size(0), h.d = d;
+    h.x_stride = h.N > 1 ? x.stride(0) : d;
+    h.ignore_index = how.ignore_index, h.reduction = how.reduction;
+  }
+  at::TensorOptions fp32() const { return x.options().dtype(at::kFloat).requires_grad(false); }
+};
+
+// The loss; how.lse is filled.
+Tensor head_loss(const Tensor& x, const Tensor& w, const Tensor& labels, HeadHow& how) {
+  const HeadCall c(x, w, labels, how);
+  Tensor& lse = how.lse;
+  const at::IntArrayRef shape = how.reduction == GS_REDUCE_NONE ? labels.sizes() : at::IntArrayRef();
+  if (lse.defined())
+    require(lse.is_cuda() && lse.device() == c.dev && lse.scalar_type() == at::kFloat &&
+                lse.is_contiguous() && lse.numel() == c.h.N && in_memory(lse),
+            "sums of exponentials ", lse.sizes(), ": contiguous fp32 of the labels' size expected");
+  else
+    lse = at::empty({c.h.N}, c.fp32());
+  if (c.h.N == 0)
+    return at::full(shape, how.reduction == GS_REDUCE_MEAN ? std::nan("") : 0.0, c.fp32());
+  const Tensor loss = at::empty(shape, c.fp32());
+  c10::DeviceGuard guard(c.dev);
+  const size_t bytes = gs_head_loss_workspace(&c.h);
+  const Tensor ws = scratch(bytes, c.x);
+  check(gs_head_loss(&c.h, static_cast<float*>(mut(loss)), static_cast<float*>(mut(lse)), mut(ws), bytes,
+                     stream_on(c.dev)),
+        "gs_head_loss");
+  return loss;
+}
+
+// A loss's upstream gradient as the kernels take it.
+Tensor upstream_of(const Tensor& g, const HeadCall& c) {
+  const Tensor up = gradient_in_memory(g).to(at::kFloat).contiguous();
+  require(up.numel() == (c.h.reduction == GS_REDUCE_NONE ? c.h.N : 1) && up.device() == c.dev,
+          "output gradient ", up.sizes(), " on ", up.device());
+  return up;
+}
+
+struct HeadLoss : torch::autograd::Function<HeadLoss> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& labels,
+                        HeadHow how) {
+    Tensor loss = head_loss(x, w, labels, how);
+    ctx->save_for_backward({x, w, labels});
+    keep(ctx, std::move(how));
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list s = ctx->get_saved_variables();
+    const HeadHow& how = kept<HeadHow>(ctx);
+    const HeadCall c(s[0], s[1], s[2], how);
+    Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) dx = at::empty(s[0].sizes(), s[0].options().requires_grad(false));
+    if (ctx->needs_input_grad(1)) dw = at::empty(s[1].sizes(), s[1].options().requires_grad(false));
+    if (c.h.N == 0) {
+      if (dw.defined()) dw.zero_();
+    } else if (dx.defined() || dw.defined()) {
+      const Tensor up = upstream_of(g[0], c);
+      c10::DeviceGuard guard(c.dev);
+      const size_t bytes = gs_head_grad_workspace(&c.h);
+      const Tensor ws = scratch(bytes, c.x);
+      check(gs_head_grad(&c.h, static_cast<const float*>(ptr(how.lse)),
+                         static_cast<const float*>(ptr(up)), mut(dx), mut(dw), mut(ws), bytes, stream_on(c.dev)),
+            "gs_head_grad");
+    }
+    return once({dx, dw, Tensor(), Tensor()});
+  }
+};
+
+Tensor head_cross_entropy(const Tensor& x, const Tensor& w, const Tensor& labels, int64_t ignore_index,
+                          int reduction, const OptTensor& lse_given) {
+  HeadHow how{ignore_index, reduction, given(lse_given)};
+  check_plain({&x, &w, &labels, &how.lse});
+  if (recorded({&x, &w})) return HeadLoss::apply(x, w, labels, std::move(how));
+  return head_loss(x, w, labels, how);
+}
+
+// The gradient of the logits [v0, v0 + n) as [..., n up to a multiple of 8], zeros behind.
+Tensor head_logit_grad(const Tensor& x, const Tensor& w, const Tensor& labels, const Tensor& lse,
+                       const Tensor& g, int64_t v0, int64_t n, int64_t ignore_index, int reduction) {
+  check_plain({&x, &w, &labels, &lse});
+  const HeadCall c(x, w, labels, HeadHow{ignore_index, reduction, {}});
+  require(lse.device() == c.dev && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+              lse.numel() == c.h.N,
+          "sums of exponentials ", lse.sizes());
+  require(v0 >= 0 && n > 0 && v0 + n <= c.h.V, "logits ", v0, " to ", v0 + n, " of ", c.h.V);
+  const int64_t stride = (n + 7) / 8 * 8;
+  std::vector<int64_t> shape = labels.sizes().vec();
+  shape.push_back(stride);
+  const Tensor out = at::empty(shape, c.x.options().requires_grad(false));
+  if (c.h.N == 0) return out;
+  const Tensor up = upstream_of(g, c);
+  c10::DeviceGuard guard(c.dev);
+  const size_t bytes = gs_head_logit_grad_workspace(&c.h, v0, n);
+  const Tensor ws = scratch(bytes, c.x);
+  check(gs_head_logit_grad(&c.h, static_cast<const float*>(ptr(lse)), static_cast<const float*>(ptr(up)),
+                           v0, n, mut(out), stride, mut(ws), bytes, stream_on(c.dev)),
+        "gs_head_logit_grad");
+  return out;
+}
+
+// ------------------------------------------------ root-mean-square norm with the residual's addition
+
+// Checks, and the number of rows.
+int64_t norm_rows(const Tensor& x, const Tensor& res, const Tensor& w) {
+  device_of({&x, &res, &w});
+  require(x.dim() >= 1 && x.size(-1) > 0 && w.dim() == 1 && w.size(0) == x.size(-1) &&
+              w.scalar_type() == x.scalar_type(),
+          "rows ", x.sizes(), " ", x.scalar_type(), " and norm weight ", w.sizes(), " ", w.scalar_type(),
+          ": [..., d] and [d] of one type expected");
+  gs_dtype_of(x, "rows");
+  if (res.defined())
+    require(res.sizes() == x.sizes() && res.scalar_type() == x.scalar_type(), "residual ", res.sizes(),
+            " ", res.scalar_type(), " of rows ", x.sizes(), " ", x.scalar_type());
+  return x.numel() / x.size(-1);
+}
+
+// (y) or, with a residual, (y, h).
+variable_list norm_forward(const Tensor& x_in, const Tensor& res_in, const Tensor& w_in, double eps) {
+  const int64_t rows = norm_rows(x_in, res_in, w_in);
+  const Tensor x = x_in.contiguous(), w = w_in.contiguous();
+  const auto options = x.options().requires_grad(false);
+  variable_list out = {at::empty(x.sizes(), options)};
+  Tensor res, h;
+  if (res_in.defined()) {
+    res = res_in.contiguous();
+    out.push_back(h = at::empty(x.sizes(), options));
+  }
+  if (rows > 0) {
+    c10::DeviceGuard guard(x.device());
+    check(gs_rms_norm(ptr(x), ptr(res), ptr(w), gs_dtype_of(x, "rows"), rows, x.size(-1),
+                      static_cast<float>(eps), mut(out[0]), mut(h), stream_on(x.device())),
+          "gs_rms_norm");
+  }
+  return out;
+}
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& res,
+                               const Tensor& w, double eps) {
+    ctx->set_materialize_grads(false);
+    variable_list out = norm_forward(x, given(res), w, eps);
+    ctx->save_for_backward({res ? out[1] : x, w});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["residual"] = res.has_value();
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list given_grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const bool residual = ctx->saved_data["residual"].toBool();
+    const size_t w_edge = residual ? 2 : 1;
+    const Tensor h = s[0].contiguous(), w = s[1].contiguous();
+    const int64_t rows = norm_rows(h, Tensor(), w), F = h.size(-1);
+    variable_list grads(2);
+    for (size_t k = 0; k < given_grads.size() && k < 2; ++k) {
+      if (!given_grads[k].defined()) continue;
+      grads[k] = gradient_in_memory(given_grads[k]).contiguous();
+      require(grads[k].sizes() == h.sizes() && grads[k].scalar_type() == h.scalar_type() &&
+                  grads[k].device() == h.device(),
+              "output gradient ", grads[k].sizes(), " ", grads[k].scalar_type());
+    }
+    Tensor dx, dw;
+    if (ctx->needs_input_grad(0) || (residual && ctx->needs_input_grad(1)))
+      dx = at::empty(h.sizes(), h.options().requires_grad(false));
+    if (ctx->needs_input_grad(w_edge)) dw = at::empty({F}, w.options().requires_grad(false));
+    if (rows == 0) {
+      if (dw.defined()) dw.zero_();
+    } else if (dx.defined() || dw.defined()) {
+      c10::DeviceGuard guard(h.device());
+      size_t bytes = 0;
+      Tensor ws;
+      if (dw.defined()) {
+        bytes = gs_rms_norm_grad_workspace(rows, F);
+        ws = scratch(bytes, h);
+      }
+      check(gs_rms_norm_grad(ptr(h), ptr(w), ptr(grads[0]), ptr(grads[1]), gs_dtype_of(h, "rows"), rows,
+                             F, static_cast<float>(ctx->saved_data["eps"].toDouble()), mut(dx), mut(dw),
+                             mut(ws), bytes, stream_on(h.device())),
+            "gs_rms_norm_grad");
+    }
+    // the residual's gradient is x's: one tensor for both
+    return once({dx, residual ? dx : Tensor(), dw, Tensor()});
+  }
+};
+
+variable_list rms_norm(const Tensor& x, const OptTensor& res, const Tensor& w, double eps) {
+  const Tensor r = given(res);
+  check_plain({&x, &r, &w});
+  if (recorded({&x, &r, &w})) return RmsNorm::apply(x, res, w, eps);
+  return norm_forward(x, r, w, eps);
+}
+
+// (dots, train gradient of the weight; the gradient undefined without a scale).
+std::vector<OptTensor> rms_norm_dot(const Tensor& h_in, const Tensor& g_in, const Tensor& w, double eps,
+                                    int64_t n_val, std::optional<int64_t> val_start,
+                                    std::optional<double> grad_scale) {
+  check_plain({&h_in, &w});
+  const Tensor h = h_in.contiguous(), g = gradient_in_memory(g_in).to(h.scalar_type()).contiguous();
+  const int64_t rows = norm_rows(h, g, Tensor(w).to(h.scalar_type()));
+  const int64_t N = h.size(0), F = h.size(-1), n_train = N - n_val;
+  require(n_train > 0 && h.dim() >= 2 && rows > 0, "rms_norm_dot: ", n_val, " validation samples of ",
+          h.sizes());
+  const Tensor dots = at::empty({n_train}, h.options().dtype(at::kFloat).requires_grad(false));
+  Tensor dw;
+  if (grad_scale) dw = at::empty({F}, w.options().requires_grad(false));
+  c10::DeviceGuard guard(h.device());
+  const size_t bytes = gs_rms_norm_dot_workspace(N, rows / N, F);
+  const Tensor ws = scratch(bytes, h);
+  check(gs_rms_norm_dot(ptr(h), ptr(g), gs_dtype_of(h, "rows"), N, n_val, val_start.value_or(n_train),
+                        rows / N, F, static_cast<float>(eps), static_cast<float*>(mut(dots)), mut(dw),
+                        gs_dtype_of(w, "norm weight"), static_cast<float>(grad_scale.value_or(0.0)),
+                        mut(ws), bytes, stream_on(h.device())),
+        "gs_rms_norm_dot");
+  return {dots, some(dw)};
+}
+
+// ----------------------------------------------------------------------------------------- AdamW
+
+// One step, the `step`-th, of the parameters, whose gradients are theirs and whose averages the states
+// hold (dicts, one for each).
+void adamw(const std::vector<Tensor>& params, const std::vector<py::dict>& states, int bits, double lr,
+           double beta1, double beta2, double eps, double weight_decay, int64_t step, uint32_t seed) {
+  require(params.size() == states.size(), params.size(), " parameters and ", states.size(), " states");
+  std::vector<gs_adamw_tensor> rows;
+  std::vector<Tensor> held;   // gradients laid out like their parameters, until the launch
+  const auto entry = [](const py::dict& state, const char* name) {
+    require(state.contains(name), "AdamW state without ", name);
+    return state[name].cast<Tensor>();
+  };
+  // all checks before the first launch
+  std::vector<std::pair<c10::Device, int>> kinds;
+  std::vector<size_t> kind_of;
+  for (size_t i = 0; i < params.size(); ++i) {
+    const Tensor& p = params[i];
+    Tensor g = p.grad();
+    require(g.defined(), "a parameter without a gradient");
+    check_plain({&p, &g});
+    const int dt = gs_dtype_of(p, "AdamW parameters");
+    device_of({&p, &g});
+    require(g.scalar_type() == p.scalar_type() && g.sizes() == p.sizes(), "gradient ", g.sizes(), " ",
+            g.scalar_type(), " of a parameter ", p.sizes(), " ", p.scalar_type());
+    require(p.is_non_overlapping_and_dense(), "AdamW takes parameters that fill their memory, got ",
+            p.sizes(), " with strides ", p.strides());
+    if (g.strides() != p.strides()) {
+      c10::DeviceGuard guard(p.device());
+      g = at::empty_strided(p.sizes(), p.strides(), g.options().requires_grad(false)).copy_(g);
+      held.push_back(g);
+    }
+    gs_adamw_tensor row{};
+    row.n = p.numel();
+    const int64_t blocks = (row.n + GS_ADAMW_BLOCK - 1) / GS_ADAMW_BLOCK;
+    const auto average = [&](const char* name) {
+      const Tensor a = entry(states[i], name);
+      require(in_memory(a) && a.device() == p.device() && a.sizes() == p.sizes() &&
+                  (row.n == 0 || a.strides() == p.strides()) &&
+                  a.scalar_type() == (bits == 8 ? at::kFloat8_e4m3fn : at::kFloat),
+              "AdamW state ", name, " ", a.sizes(), " ", a.scalar_type(), " of a parameter ", p.sizes(),
+              " ", p.scalar_type());
+      return mut(a);
+    };
+    const auto scales = [&](const char* name) {
+      const Tensor a = entry(states[i], name);
+      require(in_memory(a) && a.device() == p.device() && a.numel() == blocks && a.is_contiguous() &&
+                  a.scalar_type() == at::kFloat,
+              "AdamW state ", name, " ", a.sizes(), " ", a.scalar_type(), ": fp32 [", blocks, "] expected");
+      return static_cast<float*>(mut(a));
+    };
+    row.g = ptr(g);
+    row.m = average("exp_avg");
+    row.v = average(bits == 8 ? "root_avg_sq" : "exp_avg_sq");
+    if (bits == 8) {
+      row.m_scale = scales("exp_avg_scale");
+      row.v_scale = scales("root_avg_sq_scale");
+    }
+    row.p = mut(p);
+    rows.push_back(row);
+    const std::pair<c10::Device, int> kind(p.device(), dt);
+    size_t k = 0;
+    while (k < kinds.size() && kinds[k] != kind) ++k;
+    if (k == kinds.size()) kinds.push_back(kind);
+    kind_of.push_back(k);
+  }
+  for (size_t k = 0; k < kinds.size(); ++k) {
+    std::vector<gs_adamw_tensor> part;
+    for (size_t i = 0; i < rows.size(); ++i)
+      if (kind_of[i] == k) part.push_back(rows[i]);
+    c10::DeviceGuard guard(kinds[k].first);
+    check(gs_adamw(part.data(), static_cast<int64_t>(part.size()), kinds[k].second, bits, lr, beta1, beta2,
+                   eps, weight_decay, step, seed, stream_on(kinds[k].first)),
+          "gs_adamw");
+  }
+  for (const Tensor& p : params) p.unsafeGetTensorImpl()->bump_version();   // written
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_lm_autograd, m) {
@@ -692,4 +1015,9 @@ PYBIND11_MODULE(_lm_autograd, m) {
   m.def("qk_norm_rotary_dots", &qk_norm_rotary_dots);
   m.def("qk_sample_dots", &qk_sample_dots);
   m.def("distillation_loss", &distillation_loss);
+  m.def("head_cross_entropy", &head_cross_entropy);
+  m.def("head_logit_grad", &head_logit_grad);
+  m.def("rms_norm", &rms_norm);
+  m.def("rms_norm_dot", &rms_norm_dot);
+  m.def("adamw", &adamw);
 }

@@ -16,7 +16,7 @@ import torch.nn as nn
 
 from .. import _native, _overlap
 from .._native import ops
-from ..lm_layers import ScaledEmbedding
+from ..lm_layers import ScaledEmbedding, head_gradient_pieces
 
 
 def _flatten_tokens(x: torch.Tensor) -> torch.Tensor:
@@ -75,6 +75,10 @@ class GradProjHooks:
     def _compute_dense_proj(self, module: nn.Module, A_raw: torch.Tensor,
                             B_out: torch.Tensor) -> None:
         """Projected per-sample gradients of a dense layer (reference :120-165)."""
+        head = module.__dict__.pop("_gs_head", None)
+        if head is not None:   # a HeadCrossEntropy's loss
+            self._compute_head_proj(module, A_raw, B_out, *head)
+            return
         is_conv1d = module.__class__.__name__ == 'Conv1D'
         A = _flatten_tokens(A_raw)
         B = _flatten_tokens(B_out)
@@ -88,6 +92,19 @@ class GradProjHooks:
         layout = _native.PROJ_KI_KO if is_conv1d else _native.PROJ_KO_KI
         module._ghost_grad_proj = ops().kron_proj(A, B, P_i, P_o, float(batch_size),
                                                   layout=layout, out_dtype=torch.float32)
+
+    def _compute_head_proj(self, module: nn.Module, A: torch.Tensor, grad: torch.Tensor,
+                           labels: torch.Tensor, lse: torch.Tensor) -> None:
+        """An nn.Linear's projection of a layer that ended in its loss: the sum over the pieces of the
+        vocabulary, each with its columns of P_o."""
+        total = None
+        P_i, P_o = self._proj(A.dtype)
+        for v0, n, G in head_gradient_pieces(module, A, labels, lse, grad):
+            part = ops().kron_proj(_flatten_tokens(A), _flatten_tokens(G[..., :n]), P_i,
+                                   P_o[:, v0:v0 + n], float(A.shape[0]), layout=_native.PROJ_KO_KI,
+                                   out_dtype=torch.float32)
+            total = part if total is None else total.add_(part)
+        module._ghost_grad_proj = total
 
     def _compute_embedding_proj(self, module: nn.Module, indices: torch.Tensor,
                                 grad_output: torch.Tensor) -> None:

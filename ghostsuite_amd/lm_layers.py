@@ -7,12 +7,16 @@
     attention takes, in one pass forward and one backward.
   - ``distillation_loss``: the loss of logits against a teacher's top logits, alone or beside the
     labels' cross entropy, with its gradient.
+  - ``head_cross_entropy`` / ``HeadCrossEntropy``: the output projection with its softmax cross
+    entropy, in pieces of the vocabulary, without keeping the logits.
+  - ``rms_norm`` / ``add_rms_norm`` / ``RMSNorm``: the root-mean-square norm of a residual stream,
+    with the residual's addition.
 
 All are differentiable (once), run on the current stream and take bf16 or fp32 tensors on a ROCm
 GPU; anything else raises ``GhostHipError``, as do forward-mode differentiation, function
-transforms (``torch.func``) and ``torch.jit`` tracing.  ``ScaledEmbedding`` and ``QKNormRotary`` are
-layers the engines know: ``GradDotProdEngine`` gives their weights gradient dot products and train
-gradients, ``GradProjLoraEngine`` projects a ``ScaledEmbedding``.
+transforms (``torch.func``) and ``torch.jit`` tracing.  The layers are ones that the engines know:
+``GradDotProdEngine`` gives their weights gradient dot products and train gradients,
+``GradProjLoraEngine`` projects a ``ScaledEmbedding`` and a ``HeadCrossEntropy``.
 """
 from __future__ import annotations
 
@@ -25,7 +29,8 @@ from torch import nn
 from ._native import GhostHipError, ops
 
 __all__ = ["embedding_lookup", "ScaledEmbedding", "rotary_table", "qkv_norm_rotary",
-           "qk_norm_rotary", "QKNormRotary", "distillation_loss"]
+           "qk_norm_rotary", "QKNormRotary", "distillation_loss", "head_cross_entropy",
+           "HeadCrossEntropy", "rms_norm", "add_rms_norm", "RMSNorm"]
 
 
 # Embedding lookup ###########################################################################
@@ -205,9 +210,105 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor,
     of one.  Any other, of a loss that is scaled or weighted, has the backward pass form it again:
     951 us instead of 432 for 8192 x 50257 bf16 logits, loss and gradient.  'none' with the weights
     as the rows' upstream gradients takes 583 us whatever they are."""
-    if reduction not in ("mean", "sum", "none"):
-        raise GhostHipError(f"reduction {reduction!r}: 'mean', 'sum' or 'none'")
+    _check_reduction(reduction)
     if labels is None and alpha != 1.0:
         raise GhostHipError("labels are needed unless alpha is 1")
     return ops().distillation_loss(logits, teacher_ids, teacher_logits, labels, float(temperature),
                                    float(alpha), int(ignore_index), reduction)
+
+
+# Output projection with its cross entropy ####################################################
+
+def _check_reduction(reduction) -> None:
+    if reduction not in ("mean", "sum", "none"):
+        raise GhostHipError(f"reduction {reduction!r}: 'mean', 'sum' or 'none'")
+
+
+def head_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *,
+                       ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """``cross_entropy(x @ weight.T, labels)`` without the logits.
+
+    x: [..., d] hidden rows, weight: [vocab, d], of one type (bf16 or fp32); labels: [...] integers.
+    The logits are formed in fp32 a piece of the vocabulary at a time, once in the forward pass and
+    again in the backward pass, and never stored; the gradient of a piece is (bf16 in a bf16 model,
+    in up to 512 MiB), rounded once, before it is multiplied into the gradients of x and weight.
+    Rows whose label is ignore_index take no part and are not read; their loss and gradient are zero.
+    Another label outside [0, vocab) makes its row's loss and gradient NaN.
+    reduction: 'mean' (over the rows not ignored; NaN when there are none), 'sum', or 'none' ([...]).
+    The loss is fp32."""
+    _check_reduction(reduction)
+    return ops().head_cross_entropy(x, weight, labels, int(ignore_index), reduction)
+
+
+class HeadCrossEntropy(nn.Linear):
+    """An output projection without a bias that can end in its loss: ``layer(x)`` gives the logits as
+    an ``nn.Linear`` does, ``layer(x, labels)`` the loss of ``head_cross_entropy``."""
+
+    def __init__(self, in_features: int, out_features: int, ignore_index: int = -100,
+                 reduction: str = "mean", device=None, dtype=None):
+        super().__init__(in_features, out_features, bias=False, device=device, dtype=dtype)
+        _check_reduction(reduction)
+        self.ignore_index, self.reduction = int(ignore_index), reduction
+
+    def forward(self, input: torch.Tensor, labels: Optional[torch.Tensor] = None) -> torch.Tensor:
+        d, lse = self.__dict__, None
+        d.pop("_gs_head", None)
+        if labels is None:
+            return super().forward(input)
+        if self._backward_hooks and torch.is_grad_enabled():
+            # An engine's backward hook forms the gradient of the logits from these.
+            lse = torch.empty(labels.shape, device=labels.device, dtype=torch.float32)
+            d["_gs_head"] = (labels, lse)
+        return ops().head_cross_entropy(input, self.weight, labels, self.ignore_index, self.reduction,
+                                        lse)
+
+    def extra_repr(self) -> str:
+        return f"{super().extra_repr()}, reduction={self.reduction}"
+
+
+def head_gradient_pieces(layer: HeadCrossEntropy, x: torch.Tensor, labels: torch.Tensor,
+                         lse: torch.Tensor, grad: torch.Tensor):
+    """(first entry, entries, gradient of those logits [*labels.shape, entries up to a multiple of 8])
+    of a HeadCrossEntropy's loss, piece by piece of the vocabulary, in up to 512 MiB each."""
+    vocab = layer.weight.shape[0]
+    each = max(256, (512 << 20) // max(1, labels.numel() * x.element_size()) // 256 * 256)
+    each = -(-vocab // (-(-vocab // each)))               # pieces of a size
+    each = -(-each // 256) * 256
+    for v0 in range(0, vocab, each):
+        n = min(each, vocab - v0)
+        yield v0, n, ops().head_logit_grad(x, layer.weight.detach(), labels, lse, grad, v0, n,
+                                           layer.ignore_index, layer.reduction)
+
+
+# Root-mean-square norm of a residual stream ##################################################
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6) -> torch.Tensor:
+    """``weight * x / sqrt(mean(x^2) + eps)`` over the last dimension, in fp32, rounded once.
+    x: [..., d], weight: [d], of one type."""
+    return ops().rms_norm(x, None, weight, float(eps))[0]
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, *,
+                 eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(``rms_norm(h, weight)``, h) with h = x + residual (one rounding), in one pass; x and residual
+    of one shape and type."""
+    y, h = ops().rms_norm(x, residual, weight, float(eps))
+    return y, h
+
+
+class RMSNorm(nn.Module):
+    """``rms_norm`` as a layer: ``layer(x)`` gives the normed rows, ``layer(x, residual)`` those of
+    x + residual and that sum (``add_rms_norm``)."""
+
+    def __init__(self, dim: int, eps: float = 1e-6, device=None, dtype=None):
+        super().__init__()
+        self.dim, self.eps = dim, float(eps)
+        self.weight = nn.Parameter(torch.ones(dim, device=device, dtype=dtype))
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
+        if residual is None:
+            return rms_norm(x, self.weight, eps=self.eps)
+        return add_rms_norm(x, residual, self.weight, eps=self.eps)
+
+    def extra_repr(self) -> str:
+        return f"{self.dim}, eps={self.eps:g}"

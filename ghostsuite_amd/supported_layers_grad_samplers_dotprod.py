@@ -18,6 +18,7 @@ ghost kernel or the val-gradient form, by MFMA flop count when 'auto'.
 from __future__ import annotations
 
 import math
+from types import SimpleNamespace
 from typing import Optional
 
 import torch
@@ -26,7 +27,8 @@ from torch import nn
 
 from . import _native, _overlap
 from ._native import ops
-from .lm_layers import QKNormRotary, ScaledEmbedding
+from .lm_layers import (HeadCrossEntropy, QKNormRotary, RMSNorm, ScaledEmbedding,
+                        head_gradient_pieces)
 
 try:  # HF Conv1D is a registry key only when transformers is importable
     import transformers.pytorch_utils as _hf_utils
@@ -147,7 +149,8 @@ def _reference_dtypes(layer: nn.Module, weight_dtype: Optional[torch.dtype],
 def _dot_result_dtypes(layer: nn.Module, A: torch.Tensor, B: torch.Tensor, conv1d: bool):
     """The dtypes _reference_dtypes gives a Linear (Conv1D) layer's weight and bias dots, for
     kernels that write them directly."""
-    if options["dot_dtypes"] != "reference" or options["precision"] == "fp32":
+    if options["dot_dtypes"] != "reference" or options["precision"] == "fp32" or \
+            "_gs_dots_added" in layer.__dict__:
         return torch.float32, torch.float32
     weight = torch.float32 if layer.use_ghost_computation else \
         torch.bfloat16 if conv1d else A.dtype
@@ -599,6 +602,97 @@ def _compute_qk_norm_train_grad(layer: QKNormRotary, A: torch.Tensor, B: torch.T
     return None
 
 
+# Output projection with its cross entropy ####################################################
+
+def _compute_head_dot_product(layer: HeadCrossEntropy, A: torch.Tensor, B: torch.Tensor,
+                              val_batch_size: int):
+    """Dot-products of a HeadCrossEntropy's weight, and its train gradient: an nn.Linear's, of its
+    logits' gradient.  Where the layer ended in its loss, B is the loss's gradient, and that of the
+    logits is formed a piece of the vocabulary at a time; a dot is the sum of the pieces' dots."""
+    head = layer.__dict__.get("_gs_head")
+    if head is None:
+        _compute_linear_dot_product(layer, A, B, val_batch_size)
+        return
+    n_t = A.size(0) - val_batch_size
+    if n_t <= 0:
+        raise ValueError("No training samples to compute dot product, check batch sizes.")
+    A, labels, lse = A.detach(), *head
+    weight = _param(layer, "weight")
+    trains = getattr(weight, "initially_requires_grad", False)
+    _should_use_ghost_computation(layer, A, None)
+    dots = None if _overwritten_later(layer) else []
+    scale = layer.__dict__["_gs_bias_grad_scale"]
+    grad = torch.empty_like(weight) if trains else None
+    pairs = []
+    for v0, n, G in head_gradient_pieces(layer, A, labels, lse, B):
+        # an nn.Linear of these outputs alone
+        piece = SimpleNamespace(
+            weight=SimpleNamespace(dtype=weight.dtype, initially_requires_grad=trains), bias=None,
+            name=getattr(layer, "name", None), use_ghost_computation=layer.use_ghost_computation,
+            _gs_bias_grad_scale=scale, _gs_dots_added=True)
+        if dots is not None:
+            _linear_dots(piece, A, G, val_batch_size)
+            dots.append(piece.weight.grad_dot_prod.float())
+            if hasattr(piece.weight, "grad_dot_prod_pair"):
+                pairs.append(piece.weight.grad_dot_prod_pair)
+        if trains:
+            rows = _compute_linear_train_grad(piece, A, G, val_batch_size, scale * n_t)
+            grad[v0:v0 + n].copy_(rows[:n])
+    if trains:
+        layer.__dict__["_gs_weight_train_grad"] = grad.detach()
+    if dots is not None:
+        weight.grad_dot_prod = sum(dots[1:], dots[0])
+        if pairs:
+            weight.grad_dot_prod_pair = sum(pairs[1:], pairs[0])
+        _reference_dtypes(layer, None if layer.use_ghost_computation else A.dtype, None)
+
+
+def _compute_head_train_grad(layer: HeadCrossEntropy, A: torch.Tensor, B: torch.Tensor,
+                             val_batch_size: int, scale: float = 1.0):
+    """The train gradient that the dot stage formed; without labels an nn.Linear's."""
+    if layer.__dict__.pop("_gs_head", None) is None:
+        return _compute_linear_train_grad(layer, A, B, val_batch_size, scale)
+    return layer.__dict__.pop("_gs_weight_train_grad")
+
+
+# Root-mean-square norm ######################################################################
+
+def _compute_rms_norm_dot_product(layer: RMSNorm, A: torch.Tensor, B: torch.Tensor,
+                                  val_batch_size: int):
+    """Dot-products of an RMSNorm's weight, a LayerNorm's without mean and bias.  A holds the rows that
+    were normed (x, or its sum with the residual).  The same pass produces the train gradient when
+    the hook announced its scale."""
+    if A.size(0) - val_batch_size <= 0:
+        raise ValueError("No training samples to compute dot product, check batch sizes.")
+    dot, grad = _rms_norm_pass(layer, A, B, val_batch_size, layer.__dict__.get("_gs_ln_grad_scale"))
+    _param(layer, "weight").grad_dot_prod = dot
+    if grad is not None:
+        layer.__dict__["_gs_ln_train_grads"] = (grad,)
+
+
+def _rms_norm_pass(layer: RMSNorm, A, B, val_batch_size, grad_scale):
+    A, B = A.detach(), B.detach()
+    if options["precision"] == "fp32" or A.dtype not in (torch.bfloat16, torch.float32):
+        A, B = A.float(), B.float()
+    if A.dim() == 1 or A.numel() == 0:
+        raise ValueError(f"RMSNorm rows of shape {tuple(A.shape)} under the engine")
+    return ops().rms_norm_dot(A, B, _param(layer, "weight").detach(), layer.eps, val_batch_size,
+                              grad_scale=grad_scale)
+
+
+def _compute_rms_norm_train_grad(layer: RMSNorm, A: torch.Tensor, B: torch.Tensor,
+                                 val_batch_size: int, scale: float = 1.0) -> None:
+    """Applies an RMSNorm's train gradient itself and returns None."""
+    train_bs = A.size(0) - val_batch_size
+    if train_bs <= 0:
+        raise ValueError("No training samples to compute gradients, check batch sizes.")
+    grads = layer.__dict__.pop("_gs_ln_train_grads", None)
+    if grads is None:
+        grads = _rms_norm_pass(layer, A, B, val_batch_size, scale / train_bs)[1:]
+    _create_or_accumulate_train_grad(_param(layer, "weight"), grads[0])
+    return None
+
+
 # HF Conv1D (weight [d_in, d_out]) ##########################################################
 
 def _compute_Conv1D_dot_product(layer, A: torch.Tensor, B: torch.Tensor, val_batch_size: int):
@@ -739,6 +833,8 @@ _supported_layers_dotprod = {
     nn.Conv2d: (_compute_conv2d_dot_product, _compute_conv2d_train_grad),
     ScaledEmbedding: (_compute_scaled_embedding_dot_product, _compute_scaled_embedding_train_grad),
     QKNormRotary: (_compute_qk_norm_dot_product, _compute_qk_norm_train_grad),
+    HeadCrossEntropy: (_compute_head_dot_product, _compute_head_train_grad),
+    RMSNorm: (_compute_rms_norm_dot_product, _compute_rms_norm_train_grad),
 }
 if _HFConv1D is not None:
     _supported_layers_dotprod[_HFConv1D] = (_compute_Conv1D_dot_product,

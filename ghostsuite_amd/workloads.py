@@ -16,7 +16,8 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from .lm_layers import QKNormRotary, ScaledEmbedding, distillation_loss
+from .lm_layers import (HeadCrossEntropy, QKNormRotary, RMSNorm, ScaledEmbedding,
+                        distillation_loss)
 
 
 class MLP(nn.Module):
@@ -50,6 +51,10 @@ class LMConfig:
     qk_norm: bool = False
     # Token embeddings times this (ScaledEmbedding); None: a plain embedding.
     embed_scale: Optional[float] = None
+    # 'layer' (LayerNorm) or 'rms': RMSNorm, each with the addition to the residual stream before it.
+    norm: str = "layer"
+    # The labels' loss straight from the last hidden rows, without logits (HeadCrossEntropy).
+    head_loss: bool = False
 
 
 GPT2_SMALL = LMConfig()
@@ -75,26 +80,46 @@ def _rotary(x, cos, sin, n_rot):
     return torch.cat((xr * cos + rot * sin, xp), dim=-1)
 
 
+def _norm(cfg: "LMConfig") -> nn.Module:
+    if cfg.norm not in ("layer", "rms"):
+        raise ValueError(f"norm {cfg.norm!r}: 'layer' or 'rms'")
+    return RMSNorm(cfg.d_model) if cfg.norm == "rms" else nn.LayerNorm(cfg.d_model)
+
+
 class Block(nn.Module):
     def __init__(self, cfg: LMConfig):
         super().__init__()
         self.cfg = cfg
         d = cfg.d_model
-        self.ln_1 = nn.LayerNorm(d)
+        self.ln_1 = _norm(cfg)
         self.qkv = nn.Linear(d, 3 * d)
         self.proj = nn.Linear(d, d)
         if cfg.qk_norm:
             hd = d // cfg.n_head
             self.qk = QKNormRotary(cfg.n_head, cfg.n_head, hd, n_positions=cfg.n_ctx,
                                    n_rot=int(hd * cfg.rotary_pct) if cfg.rotary else 0)
-        self.ln_2 = nn.LayerNorm(d)
+        self.ln_2 = _norm(cfg)
         self.fc = nn.Linear(d, cfg.d_mlp)
         self.fc_out = nn.Linear(cfg.d_mlp, d)
 
-    def forward(self, x, rope=None):
-        B, T, d = x.shape
+    def forward(self, x, rope=None, stream=None):
+        """With cfg.norm 'layer' x is the residual stream, and so is the result.  With 'rms' the stream
+        comes beside x, which is still to be added to it (None: x is the stream): (what is to be added,
+        stream)."""
+        if self.cfg.norm == "rms":
+            u, stream = (self.ln_1(x), x) if stream is None else self.ln_1(x, stream)
+            u, stream = self.ln_2(self._attend(u, rope), stream)
+            return self._mlp(u), stream
+        x = x + self._attend(self.ln_1(x), rope)
+        return x + self._mlp(self.ln_2(x))
+
+    def _mlp(self, u):
+        return self.fc_out(F.gelu(self.fc(u), approximate="tanh"))
+
+    def _attend(self, u, rope):
+        B, T, d = u.shape
         H = self.cfg.n_head
-        qkv = self.qkv(self.ln_1(x))
+        qkv = self.qkv(u)
         if self.cfg.qk_norm:
             q, k, v = self.qk(qkv)
         else:
@@ -107,8 +132,7 @@ class Block(nn.Module):
                 q = _rotary(q, cos, sin, n_rot)
                 k = _rotary(k, cos, sin, n_rot)
         y = _attention(q.contiguous(), k.contiguous(), v.contiguous())
-        x = x + self.proj(y.transpose(1, 2).reshape(B, T, d))
-        return x + self.fc_out(F.gelu(self.fc(self.ln_2(x)), approximate="tanh"))
+        return self.proj(y.transpose(1, 2).reshape(B, T, d))
 
 
 class CausalLM(nn.Module):
@@ -122,8 +146,9 @@ class CausalLM(nn.Module):
         if not cfg.rotary:
             self.wpe = nn.Embedding(cfg.n_ctx, cfg.d_model)
         self.h = nn.ModuleList([Block(cfg) for _ in range(cfg.n_layer)])
-        self.ln_f = nn.LayerNorm(cfg.d_model)
-        self.lm_head = nn.Linear(cfg.d_model, cfg.vocab, bias=False)
+        self.ln_f = _norm(cfg)
+        self.lm_head = HeadCrossEntropy(cfg.d_model, cfg.vocab) if cfg.head_loss else \
+            nn.Linear(cfg.d_model, cfg.vocab, bias=False)
         if cfg.tied:
             self.lm_head.weight = self.wte.weight
         self.ghost_embeddings = ("wte",) if cfg.rotary else ("wte", "wpe")
@@ -158,9 +183,18 @@ class CausalLM(nn.Module):
             # per-sample position ids so the position embedding's hook sees [B, T]
             pos = torch.arange(T, device=input_ids.device).unsqueeze(0).repeat(B, 1)
             x = x + self.wpe(pos)
-        for blk in self.h:
-            x = blk(x, rope)
-        logits = self.lm_head(self.ln_f(x))
+        if self.cfg.norm == "rms":
+            stream = None
+            for blk in self.h:
+                x, stream = blk(x, rope, stream)
+            x = self.ln_f(x) if stream is None else self.ln_f(x, stream)[0]
+        else:
+            for blk in self.h:
+                x = blk(x, rope)
+            x = self.ln_f(x)
+        if self.cfg.head_loss and labels is not None and teacher is None:
+            return self.lm_head(x, labels)
+        logits = self.lm_head(x)
         if teacher is not None:
             return distillation_loss(logits, *teacher, labels, temperature=temperature,
                                      alpha=1.0 if labels is None else alpha)

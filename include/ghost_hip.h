@@ -502,6 +502,99 @@ int gs_distill_loss(const gs_distill* d, float* out_loss, void* grad, void* work
 int gs_distill_grad(const gs_distill* d, const float* upstream, int filled, void* grad,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Output projection with its softmax cross entropy -------------------------------------
+ * Per hidden row x with label y, and the projection's weight W (no counterpart among the
+ * reference's samplers):
+ *   z = W x,  loss = log sum_v exp(z_v) - z_y
+ * in pieces of the vocabulary, without keeping z.  Rows whose label is ignore_index are not read:
+ * their loss and gradient are zero; another label outside [0, V) makes the row's loss and gradient
+ * NaN.  Products and sums are fp32 (fp32 operands as sums of three bf16 parts each).
+ * X: N rows of d contiguous features, x_stride elements apart.  W: [V, d].  Both of dtype.
+ * reduction: GS_REDUCE_NONE (out_loss: [N]), GS_REDUCE_SUM, or GS_REDUCE_MEAN over the rows not
+ * ignored (NaN when there are none, as 0 / 0; their gradients are zeros then).
+ * lse: [N] fp32, what the backward pass takes of the forward one.
+ * gs_head_grad: dx [N, d] and dw [V, d] of dtype, either may be NULL; upstream: NULL (ones), or fp32,
+ * [N] with NONE and [1] otherwise.  dz = softmax(z) - 1_y (times a row's own upstream gradient) is
+ * rounded once to bf16 between the products with bf16 operands; other factors are applied in fp32
+ * before the one rounding of dx and dw.  Every sum has a fixed order.
+ * gs_head_logit_grad: dz of the vocabulary entries [v0, v0 + n) of all N rows, zeros where a row does
+ * not count, with every factor (upstream, count) applied before its rounding to dtype:
+ * out [N, out_stride], 16-byte aligned, entries past n up to out_stride zeros; out_stride: n up to the next
+ * multiple of 8. */
+typedef struct {
+  const void* X;
+  int64_t x_stride;
+  const void* W;
+  int dtype;
+  int64_t N, V, d;
+  const int64_t* labels;       /* [N] */
+  int64_t ignore_index;
+  int reduction;
+} gs_head;
+size_t gs_head_loss_workspace(const gs_head* h);
+int gs_head_loss(const gs_head* h, float* out_loss, float* lse, void* workspace,
+                 size_t workspace_bytes, void* stream);
+size_t gs_head_grad_workspace(const gs_head* h);
+int gs_head_grad(const gs_head* h, const float* lse, const float* upstream, void* dx, void* dw,
+                 void* workspace, size_t workspace_bytes, void* stream);
+size_t gs_head_logit_grad_workspace(const gs_head* h, int64_t v0, int64_t n);
+int gs_head_logit_grad(const gs_head* h, const float* lse, const float* upstream, int64_t v0, int64_t n,
+                       void* out, int64_t out_stride, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* ---- Root-mean-square norm with the residual's addition ------------------------------------
+ * Per row of F features (no counterpart among the reference's samplers):
+ *   h = x + residual, rounded to dtype (h = x without a residual)
+ *   y = weight h (mean h^2 + eps)^(-1/2), formed in fp32 from h as rounded
+ * x, residual (NULL: none; then h is NULL too), y, h: [rows, F]; weight [F]; all of dtype. */
+int gs_rms_norm(const void* x, const void* residual, const void* weight, int dtype, int64_t rows,
+                int64_t F, float eps, void* y, void* h, void* stream);
+
+/* Its backward: h as the norm took it, gy and gh the gradients of y and h (NULL: zeros).  dx: NULL, or
+ * [rows, F], the gradient of x and of the residual; dw: NULL, or [F] (sums in fp32 in a fixed order,
+ * rounded once).  The workspace is for dw. */
+size_t gs_rms_norm_grad_workspace(int64_t rows, int64_t F);
+int gs_rms_norm_grad(const void* h, const void* weight, const void* gy, const void* gh, int dtype,
+                     int64_t rows, int64_t F, float eps, void* dx, void* dw, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* The weight's gradient dot products and train gradient, as gs_layernorm_dot's: with s_i the sum over
+ * sample i's tokens of g h (mean h^2 + eps)^(-1/2),
+ *   out_dot[i] = <s_i, the sum of s_j over the val samples>,
+ *   out_grad   = NULL, or grad_scale * the sum of s_i over the train samples ([F], grad_dtype). */
+size_t gs_rms_norm_dot_workspace(int64_t N, int64_t T, int64_t F);
+int gs_rms_norm_dot(const void* H, const void* G, int dtype, int64_t N, int64_t n_val,
+                    int64_t val_start, int64_t T, int64_t F, float eps, float* out_dot,
+                    void* out_grad, int grad_dtype, float grad_scale, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* ---- AdamW over many tensors ----------------------------------------------------------------
+ * One step, the `step`-th (from 1), of every tensor (no counterpart among the reference's samplers):
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   p = (1 - lr weight_decay) p - lr / (1 - beta1^step) m / ((v / (1 - beta2^step))^(1/2) + eps)
+ * in fp32, p (dtype, as g) rounded once.  Elements in memory order; tensors of no elements are passed
+ * over.  `tensors` is a host array.
+ * state_bits 32: m, v are [n] fp32; the scales are not looked at.
+ * state_bits 8: blocks of GS_ADAMW_BLOCK elements share a scale, their largest magnitude over 448; m
+ * and v are [n] bytes, floats of 4 exponent and 3 mantissa bits (no infinities) whose products with
+ * the scale are the average of the gradients and the root of the average of their squares.  A value
+ * a = magnitude over scale is held as step floor(a / step + u), step the distance of those floats at a,
+ * u = (16 bits of a hash + 1/2) / 2^16: with k = step 0x9E3779B9 + seed 0x6A09E667 and i the element's
+ * place in its tensor, x = (i + k) 0x9E3779B9, x = (x ^ x >> 15) 0xBB67AE85, x ^= x >> 13 (32 bits), the
+ * lower half for m, the upper one for the root; a root above zero is held as 2^-9 at least.  A value that
+ * is not finite is held as NaN, and its block's scale is the others'. */
+#define GS_ADAMW_BLOCK 256
+typedef struct {
+  void* p;
+  const void* g;
+  void *m, *v;
+  float *m_scale, *v_scale;    /* [ceil(n / GS_ADAMW_BLOCK)] */
+  int64_t n;
+} gs_adamw_tensor;
+int gs_adamw(const gs_adamw_tensor* tensors, int64_t count, int dtype, int state_bits, double lr,
+             double beta1, double beta2, double eps, double weight_decay, int64_t step, uint32_t seed,
+             void* stream);
+
 #ifdef __cplusplus
 }
 #endif
