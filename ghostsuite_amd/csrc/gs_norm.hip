@@ -20,7 +20,8 @@ namespace {
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-constexpr int NT = 256;   // threads of a workgroup
+constexpr int NT = 256;    // threads of a workgroup, forward
+constexpr int NTB = 512;   // and backward: twice the rows in flight for as many rows of dw's parts
 
 struct NormArgs {
   const void *x, *res, *w;   // res null: no residual
@@ -32,72 +33,105 @@ struct NormArgs {
   float eps;
 };
 
-// VE elements at row + f, zeros past F (only with VE = 1 can a piece be cut).
+// VE elements as they lie in memory (16 bytes, or one), taken out where they are used: bf16 ones held
+// apart take twice the registers, and half of the rows in flight.
 template <class E, int VE>
 struct Piece {
-  E e[VE];
+  static constexpr int WORDS = VE == 1 ? 1 : 4;
+  uint32_t u[WORDS];
   __device__ __forceinline__ void load(const E* p, bool in) {
     if constexpr (VE == 1) {
-      e[0] = in ? *p : E(0);
+      if constexpr (sizeof(E) == 2)
+        u[0] = in ? static_cast<uint32_t>(*p) << 16 : 0u;
+      else
+        u[0] = in ? __float_as_uint(*p) : 0u;
     } else {
       static_assert(sizeof(E) * VE == 16, "16 bytes");
-      const uint4 u = in ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
-      __builtin_memcpy(e, &u, 16);
+      const uint4 w = in ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+      u[0] = w.x, u[1] = w.y, u[2] = w.z, u[3] = w.w;
+    }
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (VE == 8) return __uint_as_float(i & 1 ? u[i / 2] & 0xFFFF0000u : u[i / 2] << 16);
+    return __uint_as_float(u[i]);
+  }
+  // The piece of these values, each rounded.
+  __device__ __forceinline__ void set(const float (&v)[VE]) {
+    if constexpr (VE == 8) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i)
+        u[i] = __float_as_uint(sizeof(E) == 2 ? round_bf16(v[i]) : v[i]);
     }
   }
   __device__ __forceinline__ void store(E* p, bool in) const {
     if (!in) return;
-    if constexpr (VE == 1) {
-      *p = e[0];
-    } else {
-      uint4 u;
-      __builtin_memcpy(&u, e, 16);
-      *reinterpret_cast<uint4*>(p) = u;
-    }
+    if constexpr (VE != 1)
+      *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+    else if constexpr (sizeof(E) == 2)
+      *p = static_cast<E>(u[0] >> 16);
+    else
+      *p = __uint_as_float(u[0]);
   }
 };
 
-// The sum over a group of LANES lanes (32, 64, or the workgroup's 256), in each of them.
+// The sums of two values over a group of LANES lanes (32, 64, or 256 of the workgroup), in each of them.
 template <int LANES>
-__device__ __forceinline__ float group_sum(float v, float* red) {
-  if constexpr (LANES == 32) return half_sum_dpp(v);
-  if constexpr (LANES == 64) return wave_sum_dpp(v);
-  const float s = wave_sum_dpp(v);
+__device__ __forceinline__ float2 group_sums(float a, float b, float2* red) {
+  if constexpr (LANES == 32) return make_float2(half_sum_dpp(a), half_sum_dpp(b));
+  a = wave_sum_dpp(a), b = wave_sum_dpp(b);
+  if constexpr (LANES == 64) return make_float2(a, b);
+  const int wid = threadIdx.x >> 6;
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  if ((threadIdx.x & 63) == 0) red[wid] = make_float2(a, b);
   __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
+  const float2* g = red + wid / 4 * 4;
+  return make_float2((g[0].x + g[1].x) + (g[2].x + g[3].x), (g[0].y + g[1].y) + (g[2].y + g[3].y));
+}
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v, float2* red) {
+  return group_sums<LANES>(v, 0.f, red).x;
 }
 
 // LANES lanes to a row, PC pieces of VE elements a lane.
 template <class E, int VE, int PC, int LANES>
 __global__ void __launch_bounds__(NT) norm_forward_kernel(NormArgs a) {
-  __shared__ float red[4];
+  __shared__ float2 red[4];
   constexpr int GROUPS = NT / LANES;
   const int li = threadIdx.x % LANES, grp = threadIdx.x / LANES;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + grp;
   const bool live = row < a.rows;   // the same for the whole group
   const int64_t at = (live ? row : 0) * a.F;
-  float v[PC][VE];
+  Piece<E, VE> h[PC];
   float ss = 0.f;
 #pragma unroll
   for (int k = 0; k < PC; ++k) {
     const int64_t f = static_cast<int64_t>(li + k * LANES) * VE;
-    const bool in = live && f < a.F;
-    Piece<E, VE> p, q;
-    p.load(static_cast<const E*>(a.x) + at + f, in);
-    if (a.res != nullptr) {
-      q.load(static_cast<const E*>(a.res) + at + f, in);
+    h[k].load(static_cast<const E*>(a.x) + at + f, live && f < a.F);
+  }
+  if (a.res != nullptr) {
+    Piece<E, VE> q[PC];
 #pragma unroll
-      for (int i = 0; i < VE; ++i) p.e[i] = from_f32<E>(to_f32<E>(p.e[i]) + to_f32<E>(q.e[i]));
-      p.store(static_cast<E*>(a.h) + at + f, in);
+    for (int k = 0; k < PC; ++k) {
+      const int64_t f = static_cast<int64_t>(li + k * LANES) * VE;
+      q[k].load(static_cast<const E*>(a.res) + at + f, live && f < a.F);
     }
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      v[k][i] = to_f32<E>(p.e[i]);
-      ss += v[k][i] * v[k][i];
+    for (int k = 0; k < PC; ++k) {
+      const int64_t f = static_cast<int64_t>(li + k * LANES) * VE;
+      float v[VE];
+#pragma unroll
+      for (int i = 0; i < VE; ++i) v[i] = h[k].get(i) + q[k].get(i);
+      h[k].set(v);
+      h[k].store(static_cast<E*>(a.h) + at + f, live && f < a.F);
     }
   }
+#pragma unroll
+  for (int k = 0; k < PC; ++k)
+#pragma unroll
+    for (int i = 0; i < VE; ++i) ss += h[k].get(i) * h[k].get(i);
   const float r = rsqrtf(group_sum<LANES>(ss, red) / static_cast<float>(a.F) + a.eps);
 #pragma unroll
   for (int k = 0; k < PC; ++k) {
@@ -105,66 +139,69 @@ __global__ void __launch_bounds__(NT) norm_forward_kernel(NormArgs a) {
     const bool in = live && f < a.F;
     Piece<E, VE> w, y;
     w.load(static_cast<const E*>(a.w) + f, in);
+    float v[VE];
 #pragma unroll
-    for (int i = 0; i < VE; ++i) y.e[i] = from_f32<E>(to_f32<E>(w.e[i]) * (v[k][i] * r));
+    for (int i = 0; i < VE; ++i) v[i] = w.get(i) * (h[k].get(i) * r);
+    y.set(v);
     y.store(static_cast<E*>(a.y) + at + f, in);
   }
 }
 
 template <class E, int VE, int PC, int LANES>
-__global__ void __launch_bounds__(NT) norm_backward_kernel(NormArgs a) {
-  __shared__ float red[4];
+__global__ void __launch_bounds__(NTB) norm_backward_kernel(NormArgs a) {
+  __shared__ float2 red[NTB / 64];
   extern __shared__ float sums[];   // [groups - 1][F], with dw
-  constexpr int GROUPS = NT / LANES;
+  constexpr int GROUPS = NTB / LANES;
   const int li = threadIdx.x % LANES, grp = threadIdx.x / LANES;
   float dw[PC][VE];
+  Piece<E, VE> w[PC];
 #pragma unroll
-  for (int k = 0; k < PC; ++k)
+  for (int k = 0; k < PC; ++k) {
+    const int64_t f = static_cast<int64_t>(li + k * LANES) * VE;
+    w[k].load(static_cast<const E*>(a.w) + f, f < a.F);
 #pragma unroll
     for (int i = 0; i < VE; ++i) dw[k][i] = 0.f;
+  }
   const float inv = 1.f / static_cast<float>(a.F);
   const int64_t step = static_cast<int64_t>(gridDim.x) * GROUPS;
-  // every group of the workgroup makes the same number of turns: group_sum may be a barrier
+  // every group of the workgroup makes the same number of turns: group_sums may be a barrier
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * GROUPS; base < a.rows; base += step) {
     const bool live = base + grp < a.rows;
     const int64_t at = (live ? base + grp : 0) * a.F;
-    Piece<E, VE> h[PC], g[PC];
+    Piece<E, VE> h[PC], g[PC], gh[PC];
 #pragma unroll
     for (int k = 0; k < PC; ++k) {
       const int64_t f = static_cast<int64_t>(li + k * LANES) * VE;
       const bool in = live && f < a.F;
       h[k].load(static_cast<const E*>(a.x) + at + f, in);
       g[k].load(static_cast<const E*>(a.g) + at + f, in && a.g != nullptr);
+      gh[k].load(static_cast<const E*>(a.gh) + at + f, in && a.gh != nullptr);
     }
     float ss = 0.f, dot = 0.f;
 #pragma unroll
-    for (int k = 0; k < PC; ++k) {
-      const int64_t f = static_cast<int64_t>(li + k * LANES) * VE;
-      Piece<E, VE> w;
-      w.load(static_cast<const E*>(a.w) + f, f < a.F);
+    for (int k = 0; k < PC; ++k)
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        const float u = to_f32<E>(h[k].e[i]);
+        const float u = h[k].get(i);
         ss += u * u;
-        dot += to_f32<E>(w.e[i]) * to_f32<E>(g[k].e[i]) * u;
+        dot += w[k].get(i) * g[k].get(i) * u;
       }
-    }
-    const float r = rsqrtf(group_sum<LANES>(ss, red) * inv + a.eps);
-    const float mean = group_sum<LANES>(dot, red) * r * inv;   // of w g h r
+    const float2 s = group_sums<LANES>(ss, dot, red);
+    const float r = rsqrtf(s.x * inv + a.eps);
+    const float mean = s.y * r * inv;   // of w g h r
 #pragma unroll
     for (int k = 0; k < PC; ++k) {
       const int64_t f = static_cast<int64_t>(li + k * LANES) * VE;
-      const bool in = live && f < a.F;
-      Piece<E, VE> w, gh, o;
-      w.load(static_cast<const E*>(a.w) + f, in);
-      gh.load(static_cast<const E*>(a.gh) + at + f, in && a.gh != nullptr);
+      Piece<E, VE> o;
+      float v[VE];
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        const float n = to_f32<E>(h[k].e[i]) * r, gi = to_f32<E>(g[k].e[i]);
+        const float n = h[k].get(i) * r, gi = g[k].get(i);
         dw[k][i] += gi * n;
-        o.e[i] = from_f32<E>(r * (to_f32<E>(w.e[i]) * gi - n * mean) + to_f32<E>(gh.e[i]));
+        v[i] = r * (w[k].get(i) * gi - n * mean) + gh[k].get(i);
       }
-      if (a.dx != nullptr) o.store(static_cast<E*>(a.dx) + at + f, in);
+      o.set(v);
+      if (a.dx != nullptr) o.store(static_cast<E*>(a.dx) + at + f, live && f < a.F);
     }
   }
   if (a.dw == nullptr) return;
@@ -195,7 +232,7 @@ __global__ void __launch_bounds__(NT) norm_backward_kernel(NormArgs a) {
 // Rows of more features than a workgroup's registers hold: read again from the caches.
 template <class E, bool BACKWARD>
 __global__ void __launch_bounds__(NT) norm_wide_kernel(NormArgs a) {
-  __shared__ float red[4];
+  __shared__ float2 red[4];
   const float inv = 1.f / static_cast<float>(a.F);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const int64_t at = row * a.F;
@@ -249,25 +286,30 @@ __global__ void __launch_bounds__(NT) norm_wide_dw_kernel(NormArgs a, const floa
   part[c * a.F + f] = s;
 }
 
-// dw[f] = the sum of n rows, rounded once.  64 features a workgroup, four threads to each.
+// dw[f] = the sum of n rows, rounded once.  64 features a workgroup, sixteen waves to them: 512 rows of
+// 2048 features, 4 MB, are 21 us with four.
+constexpr int DW_WAVES = 16;
 template <class E>
-__global__ void __launch_bounds__(NT) norm_dw_kernel(const float* part, int64_t n, int64_t F, E* dw) {
-  __shared__ float red[4][64];
+__global__ void __launch_bounds__(64 * DW_WAVES) norm_dw_kernel(const float* part, int64_t n, int64_t F,
+                                                                E* dw) {
+  __shared__ float red[DW_WAVES][64];
   const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
   const int64_t f = static_cast<int64_t>(blockIdx.x) * 64 + lane;
-  float s0 = 0.f, s1 = 0.f;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
   if (f < F) {
     int64_t i = g;
-    for (; i + 4 < n; i += 8) {
-      s0 += part[i * F + f];
-      s1 += part[(i + 4) * F + f];
-    }
-    if (i < n) s0 += part[i * F + f];
+    for (; i + 3 * DW_WAVES < n; i += 4 * DW_WAVES)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s[u] += part[(i + u * DW_WAVES) * F + f];
+    for (; i < n; i += DW_WAVES) s[0] += part[i * F + f];
   }
-  red[g][lane] = s0 + s1;
+  red[g][lane] = (s[0] + s[1]) + (s[2] + s[3]);
   __syncthreads();
-  if (g == 0 && f < F)
-    dw[f] = from_f32<E>((red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]));
+  if (g != 0 || f >= F) return;
+  float t = 0.f;
+#pragma unroll
+  for (int k = 0; k < DW_WAVES; ++k) t += red[k][lane];
+  dw[f] = from_f32<E>(t);
 }
 
 // ------------------------------------------------------------------------------ host side
@@ -289,9 +331,9 @@ void launch(const NormArgs& a, bool backward, int64_t groups, hipStream_t s) {
     hipLaunchKernelGGL((norm_forward_kernel<E, VE, PC, LANES>),
                        dim3(static_cast<unsigned>(cdiv(a.rows, G))), dim3(NT), 0, s, a);
   } else {
-    const size_t lds = a.dw != nullptr ? (G - 1) * a.F * sizeof(float) : 0;
+    const size_t lds = a.dw != nullptr ? (NTB / LANES - 1) * a.F * sizeof(float) : 0;
     hipLaunchKernelGGL((norm_backward_kernel<E, VE, PC, LANES>),
-                       dim3(static_cast<unsigned>(groups)), dim3(NT), lds, s, a);
+                       dim3(static_cast<unsigned>(groups)), dim3(NTB), lds, s, a);
   }
 }
 
@@ -306,10 +348,9 @@ int rows_kernel(const NormArgs* a, bool backward, int64_t groups, hipStream_t s,
     return LANES;                                           \
   } while (0)
   if (pieces <= 32) GS_NORM(1, 32);
-  if (pieces <= 64) GS_NORM(2, 32);
-  if (pieces <= 96) GS_NORM(3, 32);
+  if (pieces <= 64) GS_NORM(1, 64);
   if (pieces <= 128) GS_NORM(2, 64);
-  if (pieces <= 256) GS_NORM(4, 64);
+  if (pieces <= 256) GS_NORM(1, 256);
   if (pieces <= 512) GS_NORM(2, 256);
   if (pieces <= 1024) GS_NORM(4, 256);
   if constexpr (VE != 8) {
@@ -419,7 +460,7 @@ extern "C" int gs_rms_norm_grad(const void* h, const void* weight, const void* g
     const bool vec = whole_pieces(dtype, F) && aligned16({h, weight, gy, gh, dx});
     const int lanes = bf16 ? pick<uint16_t>(nullptr, vec, true, 0, s, F)
                            : pick<float>(nullptr, vec, true, 0, s, F);
-    parts = std::min(cdiv(rows, NT / lanes), BACKWARD_GROUPS);
+    parts = std::min(cdiv(rows, NTB / lanes), BACKWARD_GROUPS);
     if (bf16)
       pick<uint16_t>(&a, vec, true, parts, s, F);
     else
@@ -428,10 +469,10 @@ extern "C" int gs_rms_norm_grad(const void* h, const void* weight, const void* g
   if (dw != nullptr) {
     const dim3 grid(static_cast<unsigned>(cdiv(F, 64)));
     if (bf16)
-      hipLaunchKernelGGL(norm_dw_kernel<uint16_t>, grid, dim3(NT), 0, s, part, parts, F,
+      hipLaunchKernelGGL(norm_dw_kernel<uint16_t>, grid, dim3(64 * DW_WAVES), 0, s, part, parts, F,
                          static_cast<uint16_t*>(dw));
     else
-      hipLaunchKernelGGL(norm_dw_kernel<float>, grid, dim3(NT), 0, s, part, parts, F,
+      hipLaunchKernelGGL(norm_dw_kernel<float>, grid, dim3(64 * DW_WAVES), 0, s, part, parts, F,
                          static_cast<float*>(dw));
   }
   return check_launch("gs_rms_norm_grad");
