@@ -5,7 +5,9 @@
 //   p = (1 - lr decay) p - lr / (1 - b1^t) m / ((v / (1 - b2^t))^(1/2) + eps)
 // in fp32, p rounded once to its type.  Bound by memory: every array is read once and written once.
 // A launch takes many tensors (their addresses travel in its arguments); its workgroups take runs
-// of CHUNK elements, a tensor's last one shorter, and find their tensor by its first run.
+// of CHUNK elements, a tensor's last one shorter, and find their tensor by its first run (runs of 8192
+// elements take 611 us for GPT-2-small's tensors in bf16 with averages in 32 bits, of 2048 586: more
+// workgroups at work at once, above all where a launch has few).
 //
 // In 8 bits, 256 consecutive elements (a block) share a scale, the largest magnitude over 448, and
 // each holds its value over the scale as a float of 4 exponent and 3 mantissa bits.  Held are m and
@@ -31,8 +33,8 @@ namespace {
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 constexpr int NT = 256, BLOCK = GS_ADAMW_BLOCK, VE = 8;
-constexpr int CHUNK = 8192;          // elements of a workgroup
-constexpr int MOST = 48;             // tensors of a launch (3.5 KB of arguments)
+constexpr int CHUNK = NT * VE;       // elements of a workgroup, eight to a thread
+constexpr int MOST = 64;             // tensors of a launch (3.8 KB of arguments)
 constexpr float TOP = 448.f;
 
 struct Tensors {
@@ -88,10 +90,6 @@ struct Eight {
   }
 };
 
-__device__ __forceinline__ float update(float p, float m, float root, const Factors& f) {
-  return f.keep * p - f.step * m / (root * f.root + f.eps);
-}
-
 template <class E>
 __global__ void __launch_bounds__(NT) adamw_kernel(Tensors a, Factors f) {
   const int k = tensor_of(a, blockIdx.x);
@@ -101,26 +99,23 @@ __global__ void __launch_bounds__(NT) adamw_kernel(Tensors a, Factors f) {
                      reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v)) & 15) == 0;
   float* tm = static_cast<float*>(t.m);
   float* tv = static_cast<float*>(t.v);
+  const int64_t i = first + threadIdx.x * VE, left = t.n - i;
+  if (left <= 0) return;
+  Eight<E> p, g;
+  Eight<float> m, v;
+  p.load(static_cast<const E*>(t.p) + i, vec, left);
+  g.load(static_cast<const E*>(t.g) + i, vec, left);
+  m.load(tm + i, vec, left);
+  v.load(tv + i, vec, left);
 #pragma unroll
-  for (int64_t o = 0; o < CHUNK; o += NT * VE) {
-    const int64_t i = first + o + threadIdx.x * VE, left = t.n - i;
-    if (left <= 0) return;
-    Eight<E> p, g;
-    Eight<float> m, v;
-    p.load(static_cast<const E*>(t.p) + i, vec, left);
-    g.load(static_cast<const E*>(t.g) + i, vec, left);
-    m.load(tm + i, vec, left);
-    v.load(tv + i, vec, left);
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      m.v[e] = f.b1 * m.v[e] + f.rest1 * g.v[e];
-      v.v[e] = f.b2 * v.v[e] + f.rest2 * (g.v[e] * g.v[e]);
-      p.v[e] = update(p.v[e], m.v[e], sqrtf(v.v[e]), f);
-    }
-    p.store(static_cast<E*>(t.p) + i, vec, left);
-    m.store(tm + i, vec, left);
-    v.store(tv + i, vec, left);
+  for (int e = 0; e < VE; ++e) {
+    m.v[e] = f.b1 * m.v[e] + f.rest1 * g.v[e];
+    v.v[e] = f.b2 * v.v[e] + f.rest2 * (g.v[e] * g.v[e]);
+    p.v[e] = f.keep * p.v[e] - f.step * m.v[e] / (sqrtf(v.v[e]) * f.root + f.eps);
   }
+  p.store(static_cast<E*>(t.p) + i, vec, left);
+  m.store(tm + i, vec, left);
+  v.store(tv + i, vec, left);
 }
 
 // The largest of 32 lanes (half a wave holds a block), in each of them.
@@ -130,12 +125,13 @@ __device__ __forceinline__ float half_max(float v) {
   return v;
 }
 
-// a of [0, 448] on the 8-bit values, up or down by u of [0, 1).
-__device__ __forceinline__ float eighth(float a, float u) {
-  // the values' steps: 2^-9 below 2^-6, then an eighth of each power of two; both powers exact
-  const uint32_t e = std::max(__float_as_uint(a) >> 23, 121u);
-  const float t = a * __uint_as_float((257u - e) << 23);    // a / 2^(e - 127 - 3)
-  return fminf(floorf(t + u) * __uint_as_float((e - 3u) << 23), TOP);
+// a of [0, 448] on the 8-bit values, up or down by the chance (u << 4) + 8 of 2^20: an integer addition
+// to the 20 mantissa bits that are cut off, which is floor(a / step + (u + 1/2) / 2^16) step.  Below 2^-6
+// the values' steps stay 2^-9: 2^-6 is added first, whose mantissa's steps are those, and taken off again.
+__device__ __forceinline__ float eighth(float a, uint32_t chance) {
+  const float low = a < 0x1p-6f ? 0x1p-6f : 0.f;
+  const float q = __uint_as_float((__float_as_uint(a + low) + chance) & 0xFFF00000u);
+  return fminf(q - low, TOP);
 }
 // Four 8-bit values from their floats, which they hold exactly, and back.
 __device__ __forceinline__ uint32_t pack8(const float* v) {
@@ -172,8 +168,6 @@ __device__ __forceinline__ void store8(uint8_t* p, bool vec, int64_t left, const
   }
 }
 
-__device__ __forceinline__ bool is_finite(float v) { return fabsf(v) < INFINITY; }
-
 template <class E>
 __global__ void __launch_bounds__(NT) adamw8_kernel(Tensors a, Factors f) {
   const int k = tensor_of(a, blockIdx.x);
@@ -183,48 +177,55 @@ __global__ void __launch_bounds__(NT) adamw8_kernel(Tensors a, Factors f) {
   uint8_t* tm = static_cast<uint8_t*>(t.m);
   uint8_t* tv = static_cast<uint8_t*>(t.v);
   const bool vec8 = ((reinterpret_cast<uintptr_t>(tm) | reinterpret_cast<uintptr_t>(tv)) & 7) == 0;
+  const int64_t i = first + threadIdx.x * VE, left = t.n - i;
+  const int64_t b = i / BLOCK;
+  const bool live = b * BLOCK < t.n;   // the same for the 32 lanes of a block
+  float sm = 0.f, sr = 0.f;
+  if (live) sm = t.m_scale[b], sr = t.v_scale[b];
+  Eight<E> p, g;
+  float m[VE], r[VE];
+  p.load(static_cast<const E*>(t.p) + i, vec, left);
+  g.load(static_cast<const E*>(t.g) + i, vec, left);
+  load8(tm + i, vec8, left, m);
+  load8(tv + i, vec8, left, r);
+  float top_m = 0.f, top_r = 0.f, any = 0.f;
 #pragma unroll
-  for (int64_t o = 0; o < CHUNK; o += NT * VE) {
-    const int64_t i = first + o + threadIdx.x * VE, left = t.n - i;
-    const int64_t b = i / BLOCK;
-    const bool live = b * BLOCK < t.n;   // the same for the 32 lanes of a block
-    float sm = 0.f, sr = 0.f;
-    if (live) sm = t.m_scale[b], sr = t.v_scale[b];
-    Eight<E> p, g;
-    float m[VE], r[VE];
-    p.load(static_cast<const E*>(t.p) + i, vec, left);
-    g.load(static_cast<const E*>(t.g) + i, vec, left);
-    load8(tm + i, vec8, left, m);
-    load8(tv + i, vec8, left, r);
-    float top_m = 0.f, top_r = 0.f;
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      m[e] = f.b1 * (m[e] * sm) + f.rest1 * g.v[e];
-      const float old = r[e] * sr;
-      r[e] = sqrtf(f.b2 * (old * old) + f.rest2 * (g.v[e] * g.v[e]));
-      p.v[e] = update(p.v[e], m[e], r[e], f);
-      top_m = fmaxf(top_m, is_finite(m[e]) ? fabsf(m[e]) : 0.f);
-      top_r = fmaxf(top_r, is_finite(r[e]) ? r[e] : 0.f);
-    }
-    p.store(static_cast<E*>(t.p) + i, vec, left);
-    top_m = half_max(top_m);
-    top_r = half_max(top_r);
-    const float im = top_m > 0.f ? TOP / top_m : 0.f, ir = top_r > 0.f ? TOP / top_r : 0.f;
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      uint32_t x = (static_cast<uint32_t>(i + e) + f.key) * 0x9E3779B9u;
-      x = (x ^ (x >> 15)) * 0xBB67AE85u;
-      x ^= x >> 13;
-      const float um = (static_cast<float>(x & 0xFFFFu) + 0.5f) * 0x1p-16f;
-      const float ur = (static_cast<float>(x >> 16) + 0.5f) * 0x1p-16f;
-      m[e] = is_finite(m[e]) ? copysignf(eighth(fabsf(m[e]) * im, um), m[e]) : NAN;
-      const float held = r[e] > 0.f ? fmaxf(eighth(r[e] * ir, ur), 0x1p-9f) : 0.f;
-      r[e] = is_finite(r[e]) ? held : NAN;
-    }
-    store8(tm + i, vec8, left, m);
-    store8(tv + i, vec8, left, r);
-    if (live && (threadIdx.x & 31) == 0) t.m_scale[b] = top_m / TOP, t.v_scale[b] = top_r / TOP;
+  for (int e = 0; e < VE; ++e) {
+    m[e] = f.b1 * (m[e] * sm) + f.rest1 * g.v[e];
+    const float old = r[e] * sr;
+    // the hardware's root and reciprocal, each within one unit: p is off by as much of its move
+    r[e] = __builtin_amdgcn_sqrtf(f.b2 * (old * old) + f.rest2 * (g.v[e] * g.v[e]));
+    p.v[e] = f.keep * p.v[e] -
+             f.step * m[e] * __builtin_amdgcn_rcpf(fmaxf(r[e] * f.root + f.eps, 0x1p-126f));
+    top_m = fmaxf(top_m, fabsf(m[e]));
+    top_r = fmaxf(top_r, r[e]);
+    any += fabsf(m[e]) + r[e];
   }
+  p.store(static_cast<E*>(t.p) + i, vec, left);
+  const bool whole = any < INFINITY;   // all of them finite (or their sum too large: the same result)
+  if (!whole) {
+    top_m = top_r = 0.f;
+    for (int e = 0; e < VE; ++e) {
+      top_m = fmaxf(top_m, fabsf(m[e]) < INFINITY ? fabsf(m[e]) : 0.f);
+      top_r = fmaxf(top_r, r[e] < INFINITY ? r[e] : 0.f);
+    }
+  }
+  top_m = half_max(top_m);
+  top_r = half_max(top_r);
+  const float im = top_m > 0.f ? TOP / top_m : 0.f, ir = top_r > 0.f ? TOP / top_r : 0.f;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    uint32_t x = (static_cast<uint32_t>(i + e) + f.key) * 0x9E3779B9u;
+    x = (x ^ (x >> 15)) * 0xBB67AE85u;
+    x ^= x >> 13;
+    const float hm = eighth(fabsf(m[e]) * im, ((x & 0xFFFFu) << 4) + 8u);
+    const float hr = eighth(r[e] * ir, ((x >> 16) << 4) + 8u);
+    m[e] = whole || fabsf(m[e]) < INFINITY ? copysignf(hm, m[e]) : NAN;
+    r[e] = whole || r[e] < INFINITY ? (r[e] > 0.f ? fmaxf(hr, 0x1p-9f) : 0.f) : NAN;
+  }
+  store8(tm + i, vec8, left, m);
+  store8(tv + i, vec8, left, r);
+  if (live && (threadIdx.x & 31) == 0) t.m_scale[b] = top_m / TOP, t.v_scale[b] = top_r / TOP;
 }
 
 }  // namespace

@@ -928,9 +928,18 @@ void adamw(const std::vector<Tensor>& params, const std::vector<py::dict>& state
   require(params.size() == states.size(), params.size(), " parameters and ", states.size(), " states");
   std::vector<gs_adamw_tensor> rows;
   std::vector<Tensor> held;   // gradients laid out like their parameters, until the launch
-  const auto entry = [](const py::dict& state, const char* name) {
-    require(state.contains(name), "AdamW state without ", name);
-    return state[name].cast<Tensor>();
+  // an entry of a state (by a Python string made once: 148 tensors have 600 of them)
+  struct Name {
+    const char* text;
+    py::str key;
+    explicit Name(const char* t) : text(t), key(t) {}
+  };
+  const Name names[4] = {Name("exp_avg"), Name(bits == 8 ? "root_avg_sq" : "exp_avg_sq"),
+                         Name("exp_avg_scale"), Name("root_avg_sq_scale")};
+  const auto entry = [](const py::dict& state, const Name& name) {
+    PyObject* o = PyDict_GetItem(state.ptr(), name.key.ptr());
+    require(o != nullptr && THPVariable_Check(o), "AdamW state without ", name.text);
+    return THPVariable_Unpack(o);
   };
   // all checks before the first launch
   std::vector<std::pair<c10::Device, int>> kinds;
@@ -954,28 +963,28 @@ void adamw(const std::vector<Tensor>& params, const std::vector<py::dict>& state
     gs_adamw_tensor row{};
     row.n = p.numel();
     const int64_t blocks = (row.n + GS_ADAMW_BLOCK - 1) / GS_ADAMW_BLOCK;
-    const auto average = [&](const char* name) {
+    const auto average = [&](const Name& name) {
       const Tensor a = entry(states[i], name);
       require(in_memory(a) && a.device() == p.device() && a.sizes() == p.sizes() &&
                   (row.n == 0 || a.strides() == p.strides()) &&
                   a.scalar_type() == (bits == 8 ? at::kFloat8_e4m3fn : at::kFloat),
-              "AdamW state ", name, " ", a.sizes(), " ", a.scalar_type(), " of a parameter ", p.sizes(),
+              "AdamW state ", name.text, " ", a.sizes(), " ", a.scalar_type(), " of a parameter ", p.sizes(),
               " ", p.scalar_type());
       return mut(a);
     };
-    const auto scales = [&](const char* name) {
+    const auto scales = [&](const Name& name) {
       const Tensor a = entry(states[i], name);
       require(in_memory(a) && a.device() == p.device() && a.numel() == blocks && a.is_contiguous() &&
                   a.scalar_type() == at::kFloat,
-              "AdamW state ", name, " ", a.sizes(), " ", a.scalar_type(), ": fp32 [", blocks, "] expected");
+              "AdamW state ", name.text, " ", a.sizes(), " ", a.scalar_type(), ": fp32 [", blocks, "] expected");
       return static_cast<float*>(mut(a));
     };
     row.g = ptr(g);
-    row.m = average("exp_avg");
-    row.v = average(bits == 8 ? "root_avg_sq" : "exp_avg_sq");
+    row.m = average(names[0]);
+    row.v = average(names[1]);
     if (bits == 8) {
-      row.m_scale = scales("exp_avg_scale");
-      row.v_scale = scales("root_avg_sq_scale");
+      row.m_scale = scales(names[2]);
+      row.v_scale = scales(names[3]);
     }
     row.p = mut(p);
     rows.push_back(row);

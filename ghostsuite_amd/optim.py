@@ -61,22 +61,22 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             _check(group)
             bits = group["state_bits"]
-            steps = {}   # parameters and states by the steps taken: as a rule all the same
-            for p in group["params"]:
-                if p.grad is None:
-                    continue
-                state = self.state[p]
+            params = [p for p in group["params"] if p.grad is not None]
+            states = [self.state[p] for p in params]
+            for p, state in zip(params, states):
                 if not state:
                     state.update(_new_state(p, bits))
-                params, states = steps.setdefault(state["step"] + 1, ([], []))
-                params.append(p)
-                states.append(state)
             beta1, beta2 = group["betas"]
-            for step, (params, states) in steps.items():
-                ops().adamw(params, states, bits, group["lr"], beta1, beta2, group["eps"],
-                            group["weight_decay"], step, group["seed"] & 0xFFFFFFFF)
-                for state in states:
-                    state["step"] = step
+            taken = [state["step"] for state in states]
+            counts = dict.fromkeys(taken)   # as a rule one number
+            for before in counts:
+                at = [i for i, t in enumerate(taken) if t == before] if len(counts) > 1 else None
+                some_p, some_s = (params, states) if at is None else \
+                    ([params[i] for i in at], [states[i] for i in at])
+                ops().adamw(some_p, some_s, bits, group["lr"], beta1, beta2, group["eps"],
+                            group["weight_decay"], before + 1, group["seed"] & 0xFFFFFFFF)
+                for state in some_s:
+                    state["step"] = before + 1
         return loss
 
     def load_state_dict(self, state_dict) -> None:
