@@ -26,6 +26,7 @@
 // 8 (e / 4) + 4 (l / 32) + e % 4 of the A side, column l % 32 of the B side.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "gs_common.h"
 
@@ -37,7 +38,6 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x8_t __attribute__((ext_vector_type(8)));
 
-constexpr int HK = 64;                 // contraction of a stage
 constexpr unsigned OOB = 0x80000000u;  // past every buffer range: such lanes load zeros
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
@@ -72,6 +72,13 @@ __device__ __forceinline__ void wait_vmcnt() {
   __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | 0x0F70);
   asm volatile("" ::: "memory");
 }
+// The builtin, not assembly: the compiler has to know that the fragments are there, or it waits for later
+// reads with them.
+__device__ __forceinline__ void wait_lgkmcnt0() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  asm volatile("" ::: "memory");
+}
 // A barrier that leaves the DMA in flight; the caller waits for what it needs.
 __device__ __forceinline__ void raw_barrier() {
   asm volatile("" ::: "memory");
@@ -83,19 +90,22 @@ __device__ __forceinline__ s16x4_t lds_tr16(const unsigned char* p) {
       (__attribute__((address_space(3))) s16x4_t*)(p));
 }
 
-// WM x WN waves of MI x NI blocks of 32 x 32; NS stage slots.
-template <int WM_, int WN_, int MI_, int NI_, int NS_>
+// WM x WN waves of MI x NI blocks of 32 x 32; NS slots for stages of K of the contraction.
+template <int WM_, int WN_, int MI_, int NI_, int NS_, int K_ = 64>
 struct Tile {
-  static constexpr int WM = WM_, WN = WN_, MI = MI_, NI = NI_, NS = NS_;
+  static constexpr int WM = WM_, WN = WN_, MI = MI_, NI = NI_, NS = NS_, K = K_;
   static constexpr int NW = WM * WN, NT = 64 * NW;
   static constexpr int BM = WM * MI * 32, BN = WN * NI * 32;
-  static constexpr int A_BYTES = BM * HK * 2, STAGE = (BM + BN) * HK * 2;
+  static constexpr int A_BYTES = BM * K * 2, STAGE = (BM + BN) * K * 2;
   static constexpr int LDS = NS * STAGE;
 };
-
-using Wide = Tile<2, 4, 4, 2, 2>;   // 256 x 256, eight waves of 128 x 64
-using Few = Tile<4, 1, 1, 1, 4>;    // 128 x 32, four waves
-using FewT = Tile<1, 4, 1, 1, 4>;   // 32 x 128
+using Wide = Tile<2, 4, 4, 2, 2>;    // 256 x 256, eight waves of 128 x 64
+using Mid = Tile<2, 2, 2, 2, 2>;     // 128 x 128, four waves of 64 x 64, two workgroups to a unit
+using Small = Tile<2, 2, 1, 1, 4>;   // 64 x 64, four waves of 32 x 32
+using Few = Tile<4, 1, 1, 1, 4>;     // 128 x 32
+using FewT = Tile<1, 4, 1, 1, 4>;    // 32 x 128
+using FewW = Tile<4, 1, 2, 2, 2>;    // 256 x 64: whole rows of dW leave at a time
+constexpr int FEW_ROWS = 32;
 
 // The bf16 parts that dz is held in between the products: three for fp32; two of a few rows, whose
 // products are bound by W's and dW's memory (rounded once, a label's p - 1 would be most of dW's error);
@@ -112,17 +122,17 @@ struct Side {
   int64_t ld, part;
 };
 
-// The DMA of one side's stages.  KC: LDS row r (128 bytes) holds its 16-byte chunk c at slot
-// c ^ (r / 2 % 8), so that the 16 rows of a fragment read lie in 16 different bank groups.
-// KR: LDS row = contraction index, chunk c at slot c ^ swz(row): the 4 rows x 4 chunks of a
-// transpose read in 16 different ones.
-template <int B, int NW, bool KR>
+// The DMA of one side's stages.  KC: LDS row r (K elements) holds its 16-byte chunk c at slot c ^ swz(r),
+// so that the 16 rows of a fragment read lie in 16 different bank groups.  KR: LDS row = contraction
+// index, chunk c at slot c ^ swz(row): the 4 rows x 4 chunks of a transpose read in 16 different ones.
+template <int B, int NW, bool KR, int K>
 struct Stream {
-  static constexpr int Q = B * HK * 2 / 1024 / NW;   // loads of a wave
-  static_assert(Q > 0 && B * HK * 2 % (1024 * NW) == 0, "stage bytes split over waves");
-  static constexpr int RB = B * 2, CH = B / 8;
+  static constexpr int Q = B * K * 2 / 1024 / NW;   // loads of a wave
+  static_assert(Q > 0 && B * K * 2 % (1024 * NW) == 0, "stage bytes split over waves");
+  static constexpr int RB = KR ? B * 2 : K * 2, CH = RB / 16;   // bytes and chunks of an LDS row
   __device__ static constexpr int swz(int r) {
-    return CH >= 16 ? 4 * (r & 3) : CH == 8 ? 4 * ((r >> 1) & 1) : 0;
+    if (KR) return CH >= 16 ? 4 * (r & 3) : CH == 8 ? 4 * ((r >> 1) & 1) : 0;
+    return CH == 8 ? (r >> 1) & 7 : (r >> 2) & 3;
   }
   unsigned off[Q];
   int k[Q];
@@ -132,25 +142,23 @@ struct Stream {
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      if constexpr (KR) {
-        const int byte = (wid + NW * q) * 1024 + lane * 16;
-        const int r = byte / RB, c = (byte % RB) / 16 ^ swz(r);
-        k[q] = r;
-        off[q] = c * 8 < extent ? static_cast<unsigned>(r * ld * 2 + c * 16) : OOB;
-      } else {
-        const int r = 8 * (wid + NW * q) + lane / 8, c = lane % 8 ^ ((r >> 1) & 7);
-        k[q] = c * 8;
-        off[q] = r < extent ? static_cast<unsigned>(r * ld * 2 + c * 16) : OOB;
-      }
+      const int byte = (wid + NW * q) * 1024 + lane * 16;
+      const int r = byte / RB, c = (byte % RB) / 16 ^ swz(r);
+      k[q] = KR ? r : c * 8;
+      off[q] = (KR ? c * 8 : r) < extent ? static_cast<unsigned>(r * ld * 2 + c * 16) : OOB;
     }
   }
-  // The stage whose first element is at `base`; contraction indices at or past `lim` as zeros.
-  __device__ __forceinline__ void issue(const uint16_t* base, int lim, unsigned lds) const {
+  // The stage whose first element is at `base` to the LDS address `lds` (of this wave's first load);
+  // contraction indices at or past `lim` as zeros.
+  __device__ __forceinline__ void issue(const uint16_t* base, unsigned lds) const {
     const __amdgpu_buffer_rsrc_t r = rsrc(base);
-    const unsigned w = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
 #pragma unroll
-    for (int q = 0; q < Q; ++q)
-      dma16(r, k[q] < lim ? off[q] : OOB, lds + (w + NW * q) * 1024);
+    for (int q = 0; q < Q; ++q) dma16(r, off[q], lds + NW * q * 1024);
+  }
+  __device__ __forceinline__ void issue_cut(const uint16_t* base, unsigned lds, int lim) const {
+    const __amdgpu_buffer_rsrc_t r = rsrc(base);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) dma16(r, k[q] < lim ? off[q] : OOB, lds + NW * q * 1024);
   }
 };
 
@@ -163,14 +171,14 @@ __device__ __forceinline__ void sched_kstep() {
 }
 
 // The fragments of one side: F blocks of 32 rows from row `first` on, k-step ks of the stage.
-template <int B, int F, bool KR>
+template <int B, int F, bool KR, int K>
 struct Fragments {
+  using S = Stream<B, 1, KR, K>;
   int at[KR ? F : 1];
   int lo, hi;
   __device__ __forceinline__ void init(int first) {
     const int lane = threadIdx.x & 63;
     if constexpr (KR) {
-      using S = Stream<B, 1, true>;
       const int g = lane >> 4, row = 8 * (g >> 1) + ((lane >> 2) & 3);
 #pragma unroll
       for (int i = 0; i < F; ++i) {
@@ -179,8 +187,8 @@ struct Fragments {
       }
       lo = hi = 0;
     } else {
-      at[0] = (first + (lane & 31)) * 128;
-      lo = ((lane & 31) >> 1) & 7, hi = lane >> 5;
+      at[0] = (first + (lane & 31)) * S::RB;
+      lo = S::swz(lane & 31), hi = lane >> 5;   // blocks start at multiples of 32 rows
     }
   }
   __device__ __forceinline__ void load(const unsigned char* side, int ks, bf16x8_t (&f)[F]) const {
@@ -192,15 +200,23 @@ struct Fragments {
             bf16x8_t, __builtin_shufflevector(lds_tr16(p), lds_tr16(p + 4 * B * 2), 0, 1, 2, 3, 4,
                                               5, 6, 7));
       } else {
-        f[i] = *reinterpret_cast<const bf16x8_t*>(side + at[0] + i * 32 * 128 +
+        f[i] = *reinterpret_cast<const bf16x8_t*>(side + at[0] + i * 32 * S::RB +
                                                   ((2 * ks + hi) ^ lo) * 16);
       }
     }
   }
 };
 
-// acc = sum over the contraction [k0, k1) of A B^T, with six products of parts for fp32 (TERMS 6, the
-// small ones first), two where A alone has two parts (TERMS 2).
+// Which products of parts a product is: the operands as they are; one side (dz) in two parts; both in
+// three, of which six products count, the small ones first.
+enum Terms { ONE = 1, TWO_A = 2, TWO_B = 3, SIX = 6 };
+
+// acc = sum over the contraction [k0, k1) of A B^T.
+//
+// The waves meet once a stage, before its last k-step's MFMAs: by then every wave holds that step's
+// fragments, so the stage's slot can be loaded again, and the next stage has arrived, so its first
+// fragments are read while those MFMAs run.  (Meeting between the stages left the matrix cores idle
+// for the loads' issue and the first reads' latency.)
 template <class C, bool AKR, bool BKR, int TERMS>
 __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_t b_extent,
                                         int64_t k0, int64_t k1, unsigned char* lds,
@@ -208,16 +224,17 @@ __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_
   a.p = reinterpret_cast<const uint16_t*>(scalar(reinterpret_cast<int64_t>(a.p)));
   b.p = reinterpret_cast<const uint16_t*>(scalar(reinterpret_cast<int64_t>(b.p)));
   k0 = scalar(k0), k1 = scalar(k1);
-  constexpr int AHEAD = C::NS - 1;
-  Stream<C::BM, C::NW, AKR> sa;
-  Stream<C::BN, C::NW, BKR> sb;
+  constexpr int KS = C::K / 16;   // k-steps of a stage
+  static_assert(KS % 2 == 0, "the fragments' two buffers take turns");
+  Stream<C::BM, C::NW, AKR, C::K> sa;
+  Stream<C::BN, C::NW, BKR, C::K> sb;
   sa.init(a.ld, a_extent);
   sb.init(b.ld, b_extent);
   constexpr int NQ = sa.Q + sb.Q;
-  static_assert(NQ * (AHEAD - 1) < 64, "vmcnt range");
+  static_assert(NQ * (C::NS - 2) < 64, "vmcnt range");
   const int wid = threadIdx.x >> 6, wm = wid / C::WN, wn = wid % C::WN;
-  Fragments<C::BM, C::MI, AKR> fa;
-  Fragments<C::BN, C::NI, BKR> fb;
+  Fragments<C::BM, C::MI, AKR, C::K> fa;
+  Fragments<C::BN, C::NI, BKR, C::K> fb;
   fa.init(wm * C::MI * 32);
   fb.init(wn * C::NI * 32);
 #pragma unroll
@@ -227,64 +244,94 @@ __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  const unsigned lds0 = lds_addr(lds);
-  const int nk = k1 > k0 ? static_cast<int>((k1 - k0 + HK - 1) / HK) : 0, total = nk * TERMS;
-  // the next stage to load: its slot, its place in the contraction, and its term
-  int slot_in = 0, kt = 0, term = 0;
+  const unsigned lds0 =
+      lds_addr(lds) + static_cast<unsigned>(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 1024u;
+  const int nk = k1 > k0 ? static_cast<int>((k1 - k0 + C::K - 1) / C::K) : 0;
+  const int total = nk * (TERMS == TWO_B ? 2 : TERMS);
+  // The next stage to load: its slot, its first elements, and how many stages its term has left.  Only
+  // these change from stage to stage, in scalar registers.
+  const int last = static_cast<int>((k1 - k0) % C::K);   // contraction of a term's last stage, 0: a whole one
+  const int64_t step_a = AKR ? C::K * a.ld : C::K, step_b = BKR ? C::K * b.ld : C::K;
+  const uint16_t* first_a = a.p + (AKR ? k0 * a.ld : k0);
+  const uint16_t* first_b = b.p + (BKR ? k0 * b.ld : k0);
+  int term = 0, left = nk;
+  const uint16_t *pa, *pb;
+  auto begin_term = [&] {
+    pa = first_a, pb = first_b;
+    if constexpr (TERMS == SIX) {   // (l h) (h l) (m m) (m h) (h m) (h h)
+      pa += (term == 0 ? 2 : term == 2 || term == 3 ? 1 : 0) * a.part;
+      pb += (term == 1 ? 2 : term == 2 || term == 4 ? 1 : 0) * b.part;
+    } else if constexpr (TERMS == TWO_A) {
+      pa += term == 0 ? a.part : 0;
+    } else if constexpr (TERMS == TWO_B) {
+      pb += term == 0 ? b.part : 0;
+    }
+  };
+  begin_term();
+  unsigned slot_in = lds0;
   auto issue = [&] {
-    const int64_t k = k0 + static_cast<int64_t>(kt) * HK;
-    const int lim = k1 - k < HK ? static_cast<int>(k1 - k) : HK;
-    int64_t pa = 0, pb = 0;
-    if constexpr (TERMS == 6) {   // (l h) (h l) (m m) (m h) (h m) (h h)
-      pa = (term == 0 ? 2 : term == 2 || term == 3 ? 1 : 0) * a.part;
-      pb = (term == 1 ? 2 : term == 2 || term == 4 ? 1 : 0) * b.part;
-    } else if constexpr (TERMS == 2) {   // (m h) (h h)
-      pa = (term == 0 ? 1 : 0) * a.part;
+    if (left > 1 || last == 0) {
+      sa.issue(pa, slot_in);
+      sb.issue(pb, slot_in + C::A_BYTES);
+    } else {
+      sa.issue_cut(pa, slot_in, last);
+      sb.issue_cut(pb, slot_in + C::A_BYTES, last);
     }
-    const unsigned at = lds0 + slot_in * C::STAGE;
-    sa.issue(a.p + pa + (AKR ? k * a.ld : k), lim, at);
-    sb.issue(b.p + pb + (BKR ? k * b.ld : k), lim, at + C::A_BYTES);
-    slot_in = slot_in + 1 == C::NS ? 0 : slot_in + 1;
-    if (++kt == nk) kt = 0, ++term;
-  };
-  auto compute = [&](const unsigned char* stage) {
-    bf16x8_t af[2][C::MI], bf[2][C::NI];
-    fa.load(stage, 0, af[0]);
-    fb.load(stage + C::A_BYTES, 0, bf[0]);
-#pragma unroll
-    for (int ks = 0; ks < HK / 16; ++ks) {
-      if (ks + 1 < HK / 16) {
-        fa.load(stage, ks + 1, af[(ks + 1) & 1]);
-        fb.load(stage + C::A_BYTES, ks + 1, bf[(ks + 1) & 1]);
-      }
-#pragma unroll
-      for (int i = 0; i < C::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < C::NI; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[ks & 1][i], bf[ks & 1][j],
-                                                              acc[i][j], 0, 0, 0);
+    slot_in = slot_in + C::STAGE == lds0 + C::LDS ? lds0 : slot_in + C::STAGE;
+    pa += step_a, pb += step_b;
+    if (--left == 0) {
+      left = nk;
+      if constexpr (TERMS != ONE) ++term, begin_term();
     }
-    // order: the first k-step's reads, then each k-step's MFMAs with the next one's reads between
-    constexpr int RD = (AKR ? 2 : 1) * C::MI + (BKR ? 2 : 1) * C::NI, M = C::MI * C::NI;
-    __builtin_amdgcn_sched_group_barrier(0x100, RD, 0);
-#pragma unroll
-    for (int ks = 0; ks + 1 < HK / 16; ++ks) sched_kstep<RD, M>();
-    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
   };
+  bf16x8_t af[2][C::MI], bf[2][C::NI];
+  auto load = [&](int buf, const unsigned char* stage, int ks) {
+    fa.load(stage, ks, af[buf]);
+    fb.load(stage + C::A_BYTES, ks, bf[buf]);
+  };
+  auto mma = [&](int buf) {
 #pragma unroll
-  for (int s = 0; s < AHEAD; ++s)
-    if (s < total) issue();
-  int slot = 0;
-  for (int s = 0; s < total; ++s) {
-    // in flight behind stage s: the loads of the AHEAD - 1 stages after it, where there are any
-    if (AHEAD == 1 || s + AHEAD > total)
-      wait_vmcnt<0>();
+    for (int i = 0; i < C::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < C::NI; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[buf][i], bf[buf][j], acc[i][j], 0, 0, 0);
+  };
+  constexpr int RD = (AKR ? 2 : 1) * C::MI + (BKR ? 2 : 1) * C::NI, M = C::MI * C::NI;
+  if (total > 0) {
+#pragma unroll
+    for (int s = 0; s < C::NS - 1; ++s)
+      if (s < total) issue();
+    if (C::NS - 1 <= total)
+      wait_vmcnt<(C::NS - 2) * NQ>();
     else
-      wait_vmcnt<(AHEAD - 1) * NQ>();
+      wait_vmcnt<0>();
     raw_barrier();
-    if (s + AHEAD < total) issue();
-    compute(lds + slot * C::STAGE);
-    slot = slot + 1 == C::NS ? 0 : slot + 1;
+    load(0, lds, 0);
+    const unsigned char* stage = lds;
+    // A stage: MORE: another one is loaded meanwhile; PENDING: loads that may be in flight when the next
+    // one is read.  (Past the last stage the next slot's fragments are read and not used.)
+    auto run = [&](auto more, auto pending) {
+      const unsigned char* next = stage + C::STAGE == lds + C::LDS ? lds : stage + C::STAGE;
+      if constexpr (decltype(more)::value) issue();   // into the slot before, which every wave has read
+#pragma unroll
+      for (int ks = 0; ks + 1 < KS; ++ks) {
+        load((ks + 1) & 1, stage, ks + 1);
+        mma(ks & 1);
+        sched_kstep<RD, M>();
+      }
+      wait_lgkmcnt0();
+      wait_vmcnt<decltype(pending)::value>();
+      raw_barrier();
+      load(0, next, 0);
+      mma((KS - 1) & 1);
+      sched_kstep<RD, M>();
+      stage = next;
+    };
+    using Steady = std::integral_constant<int, (C::NS - 2) * NQ>;
+    using None = std::integral_constant<int, 0>;
+    int s = 0;
+    for (; s + C::NS - 1 < total; ++s) run(std::true_type{}, Steady{});
+    for (; s < total; ++s) run(std::false_type{}, None{});
   }
   raw_barrier();   // every wave is done reading: LDS is the caller's
 }
@@ -480,7 +527,7 @@ __device__ __forceinline__ void behind(f32x16_t (&acc)[C::MI][C::NI], int left, 
 enum { FORWARD, GRADIENT, ROWS };
 
 template <class C, int TERMS, int MODE>
-__global__ void __launch_bounds__(C::NT, C::NT / 256) head_logits_kernel(LogitsArgs p) {
+__global__ void __launch_bounds__(C::NT, 2) head_logits_kernel(LogitsArgs p) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
   const int64_t count = *p.count;
   int64_t vt, tt;
@@ -549,7 +596,7 @@ __global__ void __launch_bounds__(C::NT, C::NT / 256) head_logits_kernel(LogitsA
   } else {
     // dz in place of the logits, then through LDS to rows of BM entries; chunk c (8 entries) of
     // row r at slot c ^ r % CH, so that neither side of the turn meets in a bank
-    constexpr int CH = C::BM / 8, PARTS = MODE == ROWS ? 1 : dz_parts<C>(TERMS > 1);
+    constexpr int CH = C::BM / 8, PARTS = MODE == ROWS ? 1 : dz_parts<C>(TERMS == SIX);
     static_assert(C::BN * C::BM * 2 <= C::LDS, "the tile of dz fits the stages");
 #pragma unroll
     for (int j = 0; j < C::NI; ++j) {
@@ -574,7 +621,7 @@ __global__ void __launch_bounds__(C::NT, C::NT / 256) head_logits_kernel(LogitsA
       }
     }
     if (ragged) behind<C>(acc, static_cast<int>(p.V - m0) - row0, 0.f);   // also where the row is NaN
-    if constexpr (MODE == ROWS && TERMS > 1) {   // fp32, straight from the lanes
+    if constexpr (MODE == ROWS && TERMS == SIX) {   // fp32, straight from the lanes
 #pragma unroll
       for (int j = 0; j < C::NI; ++j) {
         const int64_t n = n0 + (wn * C::NI + j) * 32 + (lane & 31);
@@ -628,8 +675,8 @@ __global__ void __launch_bounds__(C::NT, C::NT / 256) head_logits_kernel(LogitsA
   }
 }
 
-// Each row's log2 of the sum of exponentials from the tiles' parts, and its loss; the losses' sum of
-// 64 rows.  Four threads to a row, each over every fourth tile.
+// Each row's log2 of the sum of exponentials from the tiles' parts, and its loss; the losses' sum of a
+// workgroup's rows, or of all of them where there is one workgroup.
 struct FinishArgs {
   const float2* part;
   const float* label_z;
@@ -640,42 +687,46 @@ struct FinishArgs {
   float* lse;
   float* loss;       // null, or [N]
   float* sums;       // null, or [blocks]
+  float* total;      // null, or where the sum or mean of one workgroup's rows goes
+  int mean;
 };
-__global__ void __launch_bounds__(256) head_finish_kernel(FinishArgs p) {
-  __shared__ float2 red[4][64];
-  const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * 64 + lane, count = *p.count;
+// The two parts as one.
+__device__ __forceinline__ float2 joined(float2 t, float2 u) {
+  const float m = fmaxf(t.x, u.x);
+  return make_float2(m, t.y * __builtin_amdgcn_exp2f(t.x - m) + u.y * __builtin_amdgcn_exp2f(u.x - m));
+}
+// ROWS rows to a workgroup of 1024 threads: 64 where there are many, 32 of at most as many.  Its other
+// threads share the tiles (four threads to a row and its 393 tiles are 11 us for eight rows).
+template <int ROWS>
+__global__ void __launch_bounds__(1024) head_finish_kernel(FinishArgs p) {
+  constexpr int G = 1024 / ROWS;
+  __shared__ float2 red[G][ROWS];
+  const int r = threadIdx.x % ROWS, g = threadIdx.x / ROWS;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * ROWS + r, count = *p.count;
   float2 t = make_float2(-3e38f, 0.f);
   if (n < count) {
 #pragma unroll 4
-    for (int64_t k = g; k < p.tiles; k += 4) {
-      const float2 u = p.part[k * p.N + n];
-      const float m = fmaxf(t.x, u.x);
-      t.y = t.y * __builtin_amdgcn_exp2f(t.x - m) + u.y * __builtin_amdgcn_exp2f(u.x - m);
-      t.x = m;
-    }
+    for (int64_t k = g; k < p.tiles; k += G) t = joined(t, p.part[k * p.N + n]);
   }
-  red[g][lane] = t;
-  __syncthreads();
-  if (g != 0) return;
+  red[g][r] = t;
 #pragma unroll
-  for (int k = 1; k < 4; ++k) {
-    const float2 u = red[k][lane];
-    const float m = fmaxf(t.x, u.x);
-    t.y = t.y * __builtin_amdgcn_exp2f(t.x - m) + u.y * __builtin_amdgcn_exp2f(u.x - m);
-    t.x = m;
+  for (int w = G / 2; w > 0; w /= 2) {
+    __syncthreads();
+    if (g < w) red[g][r] = joined(red[g][r], red[g + w][r]);
   }
+  if (threadIdx.x >= 64) return;
   float loss = 0.f;
-  if (n < count) {
+  if (g == 0 && n < count) {
+    t = red[0][r];
     const float lse = t.x + __log2f(t.y);
     loss = p.label[n] >= 0 ? LN2 * (lse - p.label_z[n]) : NAN;
     p.lse[n] = lse;
     if (p.loss != nullptr) p.loss[p.rows[n]] = loss;
   }
-  if (p.sums != nullptr) {
-    loss = wave_sum(loss);
-    if (lane == 0) p.sums[blockIdx.x] = loss;
-  }
+  loss = wave_sum(loss);
+  if (threadIdx.x != 0) return;
+  if (p.total != nullptr) *p.total = p.mean ? loss / static_cast<float>(count) : loss;
+  else if (p.sums != nullptr) p.sums[blockIdx.x] = loss;
 }
 __global__ void __launch_bounds__(256) head_total_kernel(const float* sums, int64_t n,
                                                          const int32_t* count, int mean,
@@ -706,7 +757,7 @@ struct DxArgs {
   int add;                 // to what is there
 };
 template <class C, int TERMS>
-__global__ void __launch_bounds__(C::NT, C::NT / 256) head_dx_kernel(DxArgs p) {
+__global__ void __launch_bounds__(C::NT, 2) head_dx_kernel(DxArgs p) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
   const int64_t count = *p.count, t_tiles = (count + C::BM - 1) / C::BM;
   const int64_t tiles = p.f_tiles * t_tiles, total = tiles * p.splits;
@@ -737,20 +788,58 @@ __global__ void __launch_bounds__(C::NT, C::NT / 256) head_dx_kernel(DxArgs p) {
   }
 }
 
-// dx of every row: its sums over the splits, scaled and rounded once; zeros where it does not count.
+// dx of every row: its sums over the splits, scaled and rounded once; zeros where it does not count.  A
+// workgroup takes 64 features of a row, its four waves every fourth split (a row's 42 splits of 768
+// features by one wave: 119 us for eight rows).
 template <class E>
 __global__ void __launch_bounds__(256) head_dx_finish_kernel(
     const float* sums, int64_t splits, const int32_t* at, const int32_t* count, int64_t N, int64_t d,
-    int64_t dp, const float* up, int mean, E* dx) {
+    int64_t dp, int64_t f_blocks, const float* up, int mean, E* dx) {
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
+  const int64_t r = blockIdx.x / f_blocks, f = (blockIdx.x - r * f_blocks) * 64 + lane;
+  const int64_t j = at[r];
+  float s = 0.f;
+  if (j >= 0 && f < d) {
+#pragma unroll 4
+    for (int64_t k = g; k < splits; k += 4) s += sums[(k * N + j) * dp + f];
+  }
+  red[g][lane] = s;
+  __syncthreads();
+  if (g != 0 || f >= d) return;
+  s = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+  dx[r * d + f] = from_f32<E>(j >= 0 ? s * gradient_scale(up, mean, *count) : 0.f);
+}
+// The same of one split: a wave to a row.
+template <class E>
+__global__ void __launch_bounds__(256) head_dx_round_kernel(const float* sums, const int32_t* at,
+                                                            const int32_t* count, int64_t N, int64_t d,
+                                                            int64_t dp, const float* up, int mean, E* dx) {
   const float scale = gradient_scale(up, mean, *count);
   const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (r >= N) return;
   const int64_t j = at[r];
-  for (int64_t f = threadIdx.x & 63; f < d; f += 64) {
-    float s = 0.f;
-    if (j >= 0)
-      for (int64_t k = 0; k < splits; ++k) s += sums[(k * N + j) * dp + f];
-    dx[r * d + f] = from_f32<E>(j >= 0 ? s * scale : 0.f);
+  const bool vec = d % 8 == 0 && reinterpret_cast<uintptr_t>(dx) % 16 == 0;
+  for (int64_t f = (threadIdx.x & 63) * 8; f < d; f += 64 * 8) {
+    float v[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {   // rows of sums are whole eights
+      const float4 q = j >= 0 ? reinterpret_cast<const float4*>(sums + j * dp + f)[h]
+                              : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[4 * h] = q.x, v[4 * h + 1] = q.y, v[4 * h + 2] = q.z, v[4 * h + 3] = q.w;
+    }
+    union { uint4 u[sizeof(E) / 2]; E e[8]; } o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o.e[i] = from_f32<E>(j >= 0 ? v[i] * scale : 0.f);
+    E* out = dx + r * d + f;
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(E) / 2); ++i) reinterpret_cast<uint4*>(out)[i] = o.u[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (f + i < d) out[i] = o.e[i];
+    }
   }
 }
 
@@ -763,36 +852,91 @@ struct DwArgs {
   int mean;
   void* out;               // the piece's rows of dW; or with several splits [splits][V][d] fp32 sums
 };
+// Features on the A side, so that a lane holds fours of neighbours of an entry's row.  bf16 rows leave
+// through LDS, whole rows of the tile at a time (straight from the lanes, two bytes each: 83 us for the
+// 77 MB of GPT-2's dW, eight rows).
 template <class C, int TERMS, class E>
-__global__ void __launch_bounds__(C::NT, C::NT / 256) head_dw_kernel(DwArgs p) {
+__global__ void __launch_bounds__(C::NT, 2) head_dw_kernel(DwArgs p) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
   const int64_t count = *p.count, tiles = p.v_tiles * p.f_tiles;
   const int64_t i0 = xcd_order(blockIdx.x, tiles * p.splits), split = i0 / tiles;
   const int64_t r0 = i0 - split * tiles;
-  const int64_t m0 = r0 / p.f_tiles * C::BM, n0 = r0 % p.f_tiles * C::BN;
+  const int64_t m0 = r0 % p.f_tiles * C::BM, n0 = r0 / p.f_tiles * C::BN;
   const int64_t k0 = split * p.kper, k1 = k0 + p.kper < count ? k0 + p.kper : count;
   f32x16_t acc[C::MI][C::NI];
-  Side a = p.dz, b = p.x;
+  Side a = p.x, b = p.dz;
   a.p += m0, b.p += n0;
-  product<C, true, true, TERMS>(a, C::BM, b, p.dp - n0, k0, k1, lds, acc);
+  product<C, true, true, TERMS>(a, p.dp - m0, b, p.dz.ld - n0, k0, k1, lds, acc);
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int wm = wid / C::WN, wn = wid % C::WN;
+  const int wm = wid / C::WN, wn = wid % C::WN, half = lane >> 5;
+  const int64_t f0 = m0 + wm * C::MI * 32 + 4 * half;   // this lane's first feature
   const bool sums = p.splits > 1;
+  const bool fours = p.d % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
   const float scale = sums ? 1.f : gradient_scale(p.up, p.mean, count);
 #pragma unroll
-  for (int j = 0; j < C::NI; ++j) {
-    const int64_t f = n0 + (wn * C::NI + j) * 32 + (lane & 31);
+  for (int i = 0; i < C::MI; ++i)
 #pragma unroll
-    for (int i = 0; i < C::MI; ++i)
+    for (int j = 0; j < C::NI; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int64_t v = m0 + (wm * C::MI + i) * 32 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
-        if (v >= p.V || f >= p.d) continue;
-        if (sums)
-          static_cast<float*>(p.out)[(split * p.V + v) * p.d + f] = acc[i][j][e];
-        else
-          static_cast<E*>(p.out)[v * p.d + f] = from_f32<E>(acc[i][j][e] * scale);
+      for (int e = 0; e < 16; ++e) acc[i][j][e] *= scale;
+  if (sums || sizeof(E) == 4) {
+    float* out = sums ? static_cast<float*>(p.out) + split * p.V * p.d : static_cast<float*>(p.out);
+#pragma unroll
+    for (int j = 0; j < C::NI; ++j) {
+      const int64_t v = n0 + (wn * C::NI + j) * 32 + (lane & 31);
+      if (v >= p.V) continue;
+#pragma unroll
+      for (int i = 0; i < C::MI; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int64_t f = f0 + 32 * i + 8 * g;
+          float* o = out + v * p.d + f;
+          if (fours && f < p.d) {
+            *reinterpret_cast<float4*>(o) = make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1],
+                                                        acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (f + q < p.d) o[q] = acc[i][j][4 * g + q];
+          }
+        }
+    }
+    return;
+  }
+  if constexpr (sizeof(E) == 2) {
+    constexpr int CH = C::BM / 8;
+    static_assert(C::BN * C::BM * 2 <= C::LDS, "the tile of dW fits the stages");
+#pragma unroll
+    for (int j = 0; j < C::NI; ++j) {
+      const int r = (wn * C::NI + j) * 32 + (lane & 31);
+#pragma unroll
+      for (int i = 0; i < C::MI; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          uint2 u;
+          u.x = pack_bf16x2(acc[i][j][4 * g], acc[i][j][4 * g + 1]);
+          u.y = pack_bf16x2(acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+          const int c = (wm * C::MI + i) * 4 + g;
+          *reinterpret_cast<uint2*>(lds + r * C::BM * 2 + ((c ^ (r & (CH - 1))) * 16) + half * 8) = u;
+        }
+    }
+    __syncthreads();
+    uint16_t* out = static_cast<uint16_t*>(p.out);
+    if (p.d % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+      for (int i = threadIdx.x; i < C::BN * CH; i += C::NT) {
+        const int r = i / CH, c = i % CH;
+        if (n0 + r < p.V && m0 + c * 8 < p.d)
+          *reinterpret_cast<uint4*>(out + (n0 + r) * p.d + m0 + c * 8) =
+              *reinterpret_cast<const uint4*>(lds + r * C::BM * 2 + ((c ^ (r & (CH - 1))) * 16));
       }
+    } else {
+      for (int i = threadIdx.x; i < C::BN * C::BM; i += C::NT) {
+        const int r = i / C::BM, f = i % C::BM;
+        if (n0 + r < p.V && m0 + f < p.d)
+          out[(n0 + r) * p.d + m0 + f] = *reinterpret_cast<const uint16_t*>(
+              lds + r * C::BM * 2 + (((f / 8) ^ (r & (CH - 1))) * 16) + f % 8 * 2);
+      }
+    }
   }
 }
 template <class E>
@@ -809,17 +953,51 @@ __global__ void __launch_bounds__(256) head_dw_finish_kernel(const float* sums, 
 
 // ------------------------------------------------------------------------------ host side
 
-constexpr int64_t PIECE_BYTES = int64_t{512} << 20;   // of dz
-constexpr int64_t FEW_ROWS = 32;
-constexpr int64_t SLOTS = 512;      // workgroups that a product is split into at least
+constexpr int64_t PIECE_BYTES = int64_t{1} << 30;   // of dz at most
+constexpr int64_t CUS = 256;
+
+enum Size { WIDE, MID, SMALL, FEW };
+
+// How a product is made: its tiles, and how often its contraction is split.
+struct Shape {
+  Size size;
+  int64_t splits, per;   // per: the contraction of a share
+};
 
 struct Plan {
   bool f32, few, copy_w;
   int64_t parts, dz_parts;   // bf16 parts of the operands, and of dz
-  int64_t dp, cols, pieces, v_tiles_all;   // cols: vocabulary entries of a piece
+  int64_t dp, cols, pieces;  // cols: vocabulary entries of a piece
+  int64_t tiles_all;         // vocabulary tiles of all pieces of the forward pass
   int64_t chunks, blocks;
-  int64_t dx_splits, dx_kper, dw_splits, dw_kper;
+  Shape dx;
+  int64_t dw_sums;           // fp32 elements that a split piece of dW needs
 };
+
+// The tiles of an m x n product over k (in `terms` products of parts), by what they were measured to take:
+// a stage of 64 of the contraction 1.75 us with 256 x 256 tiles, one workgroup to a unit; 1.15 with 128 x
+// 128 and 0.5 with 64 x 64 tiles, two to a unit; 4 us to begin and end a tile.  Splits cost a pass over the
+// shares' sums at 2 TB/s.  (43 rows of 791 fp32 features, 3655 entries: 314 us in 256 x 256 tiles, of which
+// there are 15.)
+Shape shape_of(int64_t m, int64_t n, int64_t k, int64_t terms, bool split) {
+  static const struct { Size size; int64_t b, slots; double stage; } T[] = {
+      {WIDE, 256, 256, 1.75}, {MID, 128, 512, 1.15}, {SMALL, 64, 512, 0.5}};
+  Shape best{WIDE, 1, round_up(k, 64)};
+  double least = 1e300;
+  for (const auto& t : T) {
+    const int64_t tiles = cdiv(m, t.b) * cdiv(n, t.b), stages = cdiv(k, 64);
+    // shares that fill the units once or twice
+    const int64_t fill[3] = {1, t.slots / tiles, 2 * t.slots / tiles};
+    for (int i = 0; i < (split ? 3 : 1); ++i) {
+      const int64_t want = std::max<int64_t>(1, std::min(fill[i], cdiv(stages, 4)));
+      const int64_t per = cdiv(stages, want), splits = cdiv(stages, per);
+      const double us = cdiv(tiles * splits, t.slots) * (per * terms * t.stage + 4.0) +
+                        (splits > 1 ? 4.0 + splits * m * n * 8 / 2e6 : 0.0);
+      if (us < least) least = us, best = Shape{t.size, splits, per * 64};
+    }
+  }
+  return best;
+}
 
 int check_head(const gs_head* h, const char* what) {
   if (h == nullptr) return fail(GS_ERR_INVALID, std::string(what) + ": no arguments");
@@ -835,7 +1013,28 @@ int check_head(const gs_head* h, const char* what) {
   return GS_OK;
 }
 
-// The plan of a call.  `h` with null pointers is fine.
+int64_t terms_of(const Plan& p) { return p.f32 ? 6 : 1; }
+
+Shape logits_shape(const gs_head& h, const Plan& p, int64_t n) {
+  if (p.few) return Shape{FEW, 1, 0};
+  return shape_of(n, h.N, h.d, terms_of(p), false);
+}
+// dx of a piece of `most` entries.
+Shape dx_shape(const gs_head& h, const Plan& p, int64_t most) {
+  if (!p.few) return shape_of(h.N, p.dp, most, terms_of(p), true);
+  // a few rows: shares of at least 256 entries, for every unit one
+  const int64_t tiles = cdiv(p.dp, FewT::BN);
+  const int64_t splits = std::max<int64_t>(1, std::min(CUS / tiles, cdiv(most, 256)));
+  const int64_t per = round_up(cdiv(most, splits), 64);
+  return Shape{FEW, cdiv(most, per), per};
+}
+Shape dw_shape(const gs_head& h, const Plan& p, int64_t n) {
+  if (p.few) return Shape{FEW, 1, 64};
+  return shape_of(n, h.d, h.N, terms_of(p), true);
+}
+int64_t rows_of(Size s) { return s == WIDE ? 256 : s == MID ? 128 : s == SMALL ? 64 : Few::BM; }
+
+// The plan of a call.
 Plan plan_of(const gs_head& h, bool w_aligned) {
   Plan p{};
   p.f32 = h.dtype == GS_DTYPE_F32;
@@ -844,28 +1043,29 @@ Plan plan_of(const gs_head& h, bool w_aligned) {
   p.copy_w = p.f32 || h.d % 8 != 0 || !w_aligned;
   p.few = h.N <= FEW_ROWS;
   p.dz_parts = p.few ? dz_parts<Few>(p.f32) : dz_parts<Wide>(p.f32);
-  const int64_t tile = p.few ? Few::BM : Wide::BM;
-  const int64_t all = cdiv(h.V, tile);
-  const int64_t per = std::max<int64_t>(1, PIECE_BYTES / (h.N * 2 * p.dz_parts * tile));
-  p.pieces = cdiv(all, per);
-  p.cols = cdiv(all, p.pieces) * tile;
+  const int64_t all = cdiv(h.V, 256);
+  const int64_t most = std::max<int64_t>(1, PIECE_BYTES / (h.N * 2 * p.dz_parts * 256));
+  if (all <= most) {
+    p.cols = all * 256;
+  } else {
+    // Pieces whose tiles of dW are just below a whole number of rounds over the compute units, and a rest
+    // that is split over its rows: GPT-2's 197 x 3 tiles in pieces of 85 x 3, 85 x 3 and 27 x 3 in shares of
+    // a third each; in four pieces of 50 x 3 two fifths of the units had nothing to do.
+    const int64_t f_tiles = cdiv(h.d, 256), rounds = std::max<int64_t>(1, most * f_tiles / CUS);
+    p.cols = std::max<int64_t>(1, std::min(most, rounds * CUS / f_tiles)) * 256;
+  }
   p.pieces = cdiv(h.V, p.cols);
-  p.v_tiles_all = 0;
-  for (int64_t i = 0; i < p.pieces; ++i)
-    p.v_tiles_all += cdiv(std::min(p.cols, h.V - i * p.cols), tile);
+  p.tiles_all = 0;
+  p.dw_sums = 0;
+  for (int64_t v0 = 0; v0 < h.V; v0 += p.cols) {
+    const int64_t n = std::min(p.cols, h.V - v0);
+    p.tiles_all += cdiv(n, rows_of(logits_shape(h, p, n).size));
+    const Shape w = dw_shape(h, p, n);
+    if (w.splits > 1) p.dw_sums = std::max(p.dw_sums, w.splits * n * h.d);
+  }
+  p.dx = dx_shape(h, p, std::min(p.cols, h.V));
   p.chunks = h.N > CHUNK ? cdiv(h.N, CHUNK) : 0;
   p.blocks = cdiv(h.N, 64);
-  // dx: the piece split until every workgroup slot has a share of at least 256 entries
-  const int64_t xt = p.few ? cdiv(h.N, FewT::BM) * cdiv(p.dp, FewT::BN)
-                           : cdiv(h.N, Wide::BM) * cdiv(p.dp, Wide::BN);
-  const int64_t most = std::min(p.cols, h.V);
-  p.dx_splits = std::max<int64_t>(1, std::min(SLOTS / 2 / xt, cdiv(most, 256)));
-  p.dx_kper = round_up(cdiv(most, p.dx_splits), HK);
-  p.dx_splits = cdiv(most, p.dx_kper);
-  const int64_t wt = cdiv(most, tile) * cdiv(h.d, p.few ? Few::BN : Wide::BN);
-  p.dw_splits = std::max<int64_t>(1, std::min(SLOTS / 2 / wt, cdiv(h.N, 256)));
-  p.dw_kper = round_up(cdiv(h.N, p.dw_splits), HK);
-  p.dw_splits = cdiv(h.N, p.dw_kper);
   return p;
 }
 
@@ -886,13 +1086,13 @@ Buffers carve(S& s, const gs_head& h, const Plan& p, bool grad) {
   b.chunk = s.template take<int32_t>(std::max<int64_t>(1, p.chunks));
   if (p.copy_w) b.wc = s.template take<uint16_t>(p.parts * std::min(p.cols, h.V) * p.dp);
   if (!grad) {
-    b.part = s.template take<float2>(p.v_tiles_all * h.N);
+    b.part = s.template take<float2>(p.tiles_all * h.N);
     b.label_z = s.template take<float>(h.N);
     b.sums = s.template take<float>(p.blocks);
   } else {
     b.dz = s.template take<uint16_t>(p.dz_parts * h.N * p.cols);
-    b.dx = s.template take<float>(p.dx_splits * h.N * p.dp);
-    if (p.dw_splits > 1) b.dw = s.template take<float>(p.dw_splits * std::min(p.cols, h.V) * h.d);
+    b.dx = s.template take<float>(p.dx.splits * h.N * p.dp);
+    if (p.dw_sums > 0) b.dw = s.template take<float>(p.dw_sums);
   }
   return b;
 }
@@ -932,35 +1132,70 @@ Side weight_side(const gs_head& h, const Plan& p, const Buffers& b, int64_t v0, 
 }
 
 template <class C, int MODE>
-void launch_logits(const LogitsArgs& a, bool f32, hipStream_t s) {
+void launch_logits_as(LogitsArgs& a, bool f32, hipStream_t s) {
+  a.v_tiles = cdiv(a.V, C::BM);
   const dim3 grid(grid_of(a.v_tiles * cdiv(a.N, C::BN)));
   if (f32)
-    hipLaunchKernelGGL((head_logits_kernel<C, 6, MODE>), grid, dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((head_logits_kernel<C, SIX, MODE>), grid, dim3(C::NT), 0, s, a);
   else
-    hipLaunchKernelGGL((head_logits_kernel<C, 1, MODE>), grid, dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((head_logits_kernel<C, ONE, MODE>), grid, dim3(C::NT), 0, s, a);
 }
-template <class C>
-void launch_dx(const DxArgs& a, bool f32, hipStream_t s) {
+template <int MODE>
+void launch_logits(LogitsArgs& a, Size size, bool f32, hipStream_t s) {
+  if (size == WIDE) launch_logits_as<Wide, MODE>(a, f32, s);
+  if (size == MID) launch_logits_as<Mid, MODE>(a, f32, s);
+  if (size == SMALL) launch_logits_as<Small, MODE>(a, f32, s);
+  if (size == FEW) launch_logits_as<Few, MODE>(a, f32, s);
+}
+template <class C, int TERMS>
+void launch_dx_as(DxArgs& a, bool f32, hipStream_t s) {
+  a.f_tiles = cdiv(a.dp, C::BN);
   const dim3 grid(grid_of(a.f_tiles * cdiv(a.N, C::BM) * a.splits));
   if (f32)
-    hipLaunchKernelGGL((head_dx_kernel<C, 6>), grid, dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((head_dx_kernel<C, SIX>), grid, dim3(C::NT), 0, s, a);
   else
-    hipLaunchKernelGGL((head_dx_kernel<C, C::BM == FewT::BM ? 2 : 1>), grid, dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((head_dx_kernel<C, TERMS>), grid, dim3(C::NT), 0, s, a);
 }
-template <class C>
-void launch_dw(const DwArgs& a, bool f32, hipStream_t s) {
+void launch_dx(DxArgs& a, Size size, bool f32, hipStream_t s) {
+  if (size == WIDE) launch_dx_as<Wide, ONE>(a, f32, s);
+  if (size == MID) launch_dx_as<Mid, ONE>(a, f32, s);
+  if (size == SMALL) launch_dx_as<Small, ONE>(a, f32, s);
+  if (size == FEW) launch_dx_as<FewT, TWO_A>(a, f32, s);
+}
+template <class C, int TERMS>
+void launch_dw_as(DwArgs& a, bool f32, hipStream_t s) {
+  a.v_tiles = cdiv(a.V, C::BN), a.f_tiles = cdiv(a.d, C::BM);
   const dim3 grid(grid_of(a.v_tiles * a.f_tiles * a.splits));
   if (f32)
-    hipLaunchKernelGGL((head_dw_kernel<C, 6, float>), grid, dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((head_dw_kernel<C, SIX, float>), grid, dim3(C::NT), 0, s, a);
   else
-    hipLaunchKernelGGL((head_dw_kernel<C, dz_parts<C>(false), uint16_t>), grid, dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((head_dw_kernel<C, TERMS, uint16_t>), grid, dim3(C::NT), 0, s, a);
+}
+void launch_dw(DwArgs& a, Size size, bool f32, hipStream_t s) {
+  if (size == WIDE) launch_dw_as<Wide, ONE>(a, f32, s);
+  if (size == MID) launch_dw_as<Mid, ONE>(a, f32, s);
+  if (size == SMALL) launch_dw_as<Small, ONE>(a, f32, s);
+  if (size == FEW) launch_dw_as<FewW, TWO_B>(a, f32, s);
 }
 
-// The larger of the grids of a call (workgroups).
+template <class E>
+void launch_dx_finish(const gs_head& h, const Plan& p, const Buffers& b, const float* up, int mean, void* dx,
+                      hipStream_t s) {
+  E* out = static_cast<E*>(dx);
+  if (p.dx.splits == 1) {
+    hipLaunchKernelGGL(head_dx_round_kernel<E>, dim3(grid_of(cdiv(h.N, 4))), dim3(256), 0, s, b.dx, b.at,
+                       b.count, h.N, h.d, p.dp, up, mean, out);
+    return;
+  }
+  const int64_t f_blocks = cdiv(h.d, 64);
+  hipLaunchKernelGGL(head_dx_finish_kernel<E>, dim3(grid_of(h.N * f_blocks)), dim3(256), 0, s, b.dx,
+                     p.dx.splits, b.at, b.count, h.N, h.d, p.dp, f_blocks, up, mean, out);
+}
+
+// Whether every grid of a call can be launched: shares are at most 2 * 512 where tiles are few.
 bool grids_fit(const gs_head& h, const Plan& p) {
-  const int64_t t = cdiv(h.N, p.few ? Few::BN : Wide::BN);
-  const int64_t v = cdiv(p.cols, p.few ? Few::BM : Wide::BM);
-  return v * t < INT32_MAX && v * cdiv(h.d, 32) * p.dw_splits < INT32_MAX;
+  const int64_t t = cdiv(h.N, FEW_ROWS), v = cdiv(p.cols, 64), f = cdiv(p.dp, 64), most = INT32_MAX / 2048;
+  return t <= most / f && v <= most / f && cdiv(p.cols, 256) <= INT32_MAX / cdiv(h.N, 256);
 }
 
 LogitsArgs logits_args(const gs_head& h, const Plan& p, const Buffers& b) {
@@ -1002,11 +1237,7 @@ extern "C" int gs_head_loss(const gs_head* h, float* out_loss, float* lse, void*
   for (int64_t v0 = 0; v0 < h->V; v0 += p.cols) {
     a.v0 = v0, a.V = std::min(p.cols, h->V - v0);
     a.w = weight_side(*h, p, b, v0, a.V, s);
-    a.v_tiles = cdiv(a.V, p.few ? Few::BM : Wide::BM);
-    if (p.few)
-      launch_logits<Few, FORWARD>(a, p.f32, s);
-    else
-      launch_logits<Wide, FORWARD>(a, p.f32, s);
+    launch_logits<FORWARD>(a, logits_shape(*h, p, a.V).size, p.f32, s);
     a.tile0 += a.v_tiles;
   }
   FinishArgs f{};
@@ -1014,8 +1245,13 @@ extern "C" int gs_head_loss(const gs_head* h, float* out_loss, float* lse, void*
   f.N = h->N, f.tiles = a.tile0, f.lse = lse;
   f.loss = rows ? out_loss : nullptr;
   f.sums = rows ? nullptr : b.sums;
-  hipLaunchKernelGGL(head_finish_kernel, dim3(grid_of(p.blocks)), dim3(256), 0, s, f);
-  if (!rows)
+  f.total = rows || !p.few ? nullptr : out_loss;
+  f.mean = h->reduction == GS_REDUCE_MEAN;
+  if (p.few)
+    hipLaunchKernelGGL(head_finish_kernel<FEW_ROWS>, dim3(1), dim3(1024), 0, s, f);
+  else
+    hipLaunchKernelGGL(head_finish_kernel<64>, dim3(grid_of(p.blocks)), dim3(1024), 0, s, f);
+  if (!rows && !p.few)
     hipLaunchKernelGGL(head_total_kernel, dim3(1), dim3(256), 0, s, b.sums, p.blocks, b.count,
                        h->reduction == GS_REDUCE_MEAN, out_loss);
   return check_launch("gs_head_loss");
@@ -1049,54 +1285,41 @@ extern "C" int gs_head_grad(const gs_head* h, const float* lse, const float* ups
   for (int64_t v0 = 0; v0 < h->V; v0 += p.cols) {
     a.v0 = v0, a.V = std::min(p.cols, h->V - v0);
     a.w = weight_side(*h, p, b, v0, a.V, s);
-    a.v_tiles = cdiv(a.V, p.few ? Few::BM : Wide::BM);
     a.vp = p.cols;
-    if (p.few)
-      launch_logits<Few, GRADIENT>(a, p.f32, s);
-    else
-      launch_logits<Wide, GRADIENT>(a, p.f32, s);
+    launch_logits<GRADIENT>(a, logits_shape(*h, p, a.V).size, p.f32, s);
     const Side dz{b.dz, p.cols, h->N * p.cols};
     if (dx != nullptr) {
       DxArgs x{};
       x.dz = dz, x.w = a.w, x.count = b.count, x.N = h->N, x.V = a.V, x.dp = p.dp;
-      x.f_tiles = cdiv(p.dp, p.few ? FewT::BN : Wide::BN);
-      x.splits = p.dx_splits, x.kper = p.dx_kper, x.out = b.dx, x.add = v0 > 0;
-      if (p.few)
-        launch_dx<FewT>(x, p.f32, s);
-      else
-        launch_dx<Wide>(x, p.f32, s);
+      x.splits = p.dx.splits, x.kper = p.dx.per, x.out = b.dx, x.add = v0 > 0;
+      launch_dx(x, p.dx.size, p.f32, s);
     }
     if (dw != nullptr) {
+      const Shape shape = dw_shape(*h, p, a.V);
+      const int64_t splits = shape.splits;
       DwArgs w{};
       w.dz = dz, w.x = a.x, w.count = b.count, w.V = a.V, w.d = h->d, w.dp = p.dp;
-      w.v_tiles = a.v_tiles, w.f_tiles = cdiv(h->d, p.few ? Few::BN : Wide::BN);
-      w.splits = p.dw_splits, w.kper = p.dw_kper, w.up = up, w.mean = mean;
+      w.splits = splits, w.kper = shape.per, w.up = up, w.mean = mean;
       void* out = static_cast<char*>(dw) + v0 * h->d * static_cast<int64_t>(elem_size(h->dtype));
-      w.out = p.dw_splits > 1 ? b.dw : out;
-      if (p.few)
-        launch_dw<Few>(w, p.f32, s);
-      else
-        launch_dw<Wide>(w, p.f32, s);
-      if (p.dw_splits > 1) {
+      w.out = splits > 1 ? b.dw : out;
+      launch_dw(w, shape.size, p.f32, s);
+      if (splits > 1) {
         const int64_t n = a.V * h->d;
         const dim3 grid(grid_of(cdiv(n, 256)));
         if (p.f32)
-          hipLaunchKernelGGL(head_dw_finish_kernel<float>, grid, dim3(256), 0, s, b.dw, p.dw_splits,
-                             n, b.count, up, mean, static_cast<float*>(out));
+          hipLaunchKernelGGL(head_dw_finish_kernel<float>, grid, dim3(256), 0, s, b.dw, splits, n,
+                             b.count, up, mean, static_cast<float*>(out));
         else
-          hipLaunchKernelGGL(head_dw_finish_kernel<uint16_t>, grid, dim3(256), 0, s, b.dw,
-                             p.dw_splits, n, b.count, up, mean, static_cast<uint16_t*>(out));
+          hipLaunchKernelGGL(head_dw_finish_kernel<uint16_t>, grid, dim3(256), 0, s, b.dw, splits, n,
+                             b.count, up, mean, static_cast<uint16_t*>(out));
       }
     }
   }
   if (dx != nullptr) {
-    const dim3 grid(grid_of(cdiv(h->N, 4)));
     if (p.f32)
-      hipLaunchKernelGGL(head_dx_finish_kernel<float>, grid, dim3(256), 0, s, b.dx, p.dx_splits, b.at,
-                         b.count, h->N, h->d, p.dp, up, mean, static_cast<float*>(dx));
+      launch_dx_finish<float>(*h, p, b, up, mean, dx, s);
     else
-      hipLaunchKernelGGL(head_dx_finish_kernel<uint16_t>, grid, dim3(256), 0, s, b.dx, p.dx_splits,
-                         b.at, b.count, h->N, h->d, p.dp, up, mean, static_cast<uint16_t*>(dx));
+      launch_dx_finish<uint16_t>(*h, p, b, up, mean, dx, s);
   }
   return check_launch("gs_head_grad");
 }
@@ -1106,7 +1329,7 @@ static Plan piece_plan(const gs_head& h, int64_t n, bool w_aligned) {
   gs_head piece = h;
   piece.V = n;
   Plan p = plan_of(piece, w_aligned);
-  p.cols = round_up(n, p.few ? Few::BM : Wide::BM);
+  p.cols = round_up(n, 256);
   return p;
 }
 static bool piece_aligned(const gs_head& h, int64_t v0) {
@@ -1157,11 +1380,7 @@ extern "C" int gs_head_logit_grad(const gs_head* h, const float* lse, const floa
   a.mean = h->reduction == GS_REDUCE_MEAN;
   a.v0 = v0, a.V = n, a.vp = out_stride, a.out = out;
   a.w = weight_side(*h, p, b, v0, n, s);
-  a.v_tiles = cdiv(n, p.few ? Few::BM : Wide::BM);
-  if (p.few)
-    launch_logits<Few, ROWS>(a, p.f32, s);
-  else
-    launch_logits<Wide, ROWS>(a, p.f32, s);
+  launch_logits<ROWS>(a, logits_shape(*h, p, n).size, p.f32, s);
   hipLaunchKernelGGL(head_zero_rows_kernel, dim3(grid_of(cdiv(h->N, 4))), dim3(256), 0, s, b.at, h->N,
                      static_cast<uint4*>(out), out_stride * static_cast<int64_t>(elem_size(h->dtype)) / 16);
   return check_launch("gs_head_logit_grad");
