@@ -14,10 +14,10 @@
 // listed first, in order, and copied next to each other (with rows of a multiple of 8 features,
 // which the 16-byte loads need).  Their number stays on the device; tiles past it end at once.
 //
-// fp32 operands are taken as three bf16 parts each, x = h + m + l with 8 bits apiece, and a
-// product as the six products of parts above 2^-24 of it, accumulated in fp32 like the bf16
-// one: the same kernels over six times the contraction, which at the bf16 matrix rate is still
-// faster than fp32 matrix instructions (measured below).
+// fp32 operands of many rows are taken as three bf16 parts each, x = h + m + l with 8 bits apiece, and a
+// product as the six products of parts above 2^-24 of it, accumulated in fp32 like the bf16 one: the
+// same kernels over six times the contraction, which at the bf16 matrix rate is still faster than fp32
+// matrix instructions.  A few rows are bound by W's memory, and take it as it is, on those.
 //
 // Tiles: BM x BN outputs, 64 of the contraction a stage, staged through LDS by wave-level
 // 16-byte DMA, MFMA 32x32x16 (fp32 accumulators).  A side whose contraction index is contiguous
@@ -35,6 +35,7 @@ namespace {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x8_t __attribute__((ext_vector_type(8)));
 
@@ -107,9 +108,9 @@ using FewT = Tile<1, 4, 1, 1, 4>;    // 32 x 128
 using FewW = Tile<4, 1, 2, 2, 2>;    // 256 x 64: whole rows of dW leave at a time
 constexpr int FEW_ROWS = 32;
 
-// The bf16 parts that dz is held in between the products: three for fp32; two of a few rows, whose
-// products are bound by W's and dW's memory (rounded once, a label's p - 1 would be most of dW's error);
-// one beyond.
+// The bf16 parts that dz is held in between the products: three for fp32 (of a few rows fp32 itself); two
+// of a few rows, whose products are bound by W's and dW's memory (rounded once, a label's p - 1 would be
+// most of dW's error); one beyond.
 template <class C>
 __host__ __device__ constexpr int dz_parts(bool f32) {
   return f32 ? 3 : C::BN == Few::BN ? 2 : 1;
@@ -118,20 +119,28 @@ __host__ __device__ constexpr int dz_parts(bool f32) {
 // One side of a product: the tile's first element, the stride between rows (of the side with
 // KC, of the contraction with KR) and between the bf16 parts of an fp32 operand, in elements.
 struct Side {
-  const uint16_t* p;
+  const unsigned char* p;
   int64_t ld, part;
+  // `i` elements of ES bytes further on.
+  template <int ES>
+  __device__ __forceinline__ void move(int64_t i) { p += i * ES; }
 };
+Side side_of(const void* p, int64_t ld, int64_t part) {
+  return Side{static_cast<const unsigned char*>(p), ld, part};
+}
 
 // The DMA of one side's stages.  KC: LDS row r (K elements) holds its 16-byte chunk c at slot c ^ swz(r),
 // so that the 16 rows of a fragment read lie in 16 different bank groups.  KR: LDS row = contraction
 // index, chunk c at slot c ^ swz(row): the 4 rows x 4 chunks of a transpose read in 16 different ones.
-template <int B, int NW, bool KR, int K>
+// A stage is as many bytes with elements of 4 (ES) as with those of 2: half the contraction.
+template <int B, int NW, bool KR, int K, int ES>
 struct Stream {
   static constexpr int Q = B * K * 2 / 1024 / NW;   // loads of a wave
   static_assert(Q > 0 && B * K * 2 % (1024 * NW) == 0, "stage bytes split over waves");
-  static constexpr int RB = KR ? B * 2 : K * 2, CH = RB / 16;   // bytes and chunks of an LDS row
+  static constexpr int RB = KR ? B * ES : K * 2, CH = RB / 16;   // bytes and chunks of an LDS row
+  static constexpr int VE = 16 / ES;                             // elements of a chunk
   __device__ static constexpr int swz(int r) {
-    if (KR) return CH >= 16 ? 4 * (r & 3) : CH == 8 ? 4 * ((r >> 1) & 1) : 0;
+    if (KR) return ES == 4 ? 0 : CH >= 16 ? 4 * (r & 3) : CH == 8 ? 4 * ((r >> 1) & 1) : 0;
     return CH == 8 ? (r >> 1) & 7 : (r >> 2) & 3;
   }
   unsigned off[Q];
@@ -144,18 +153,18 @@ struct Stream {
     for (int q = 0; q < Q; ++q) {
       const int byte = (wid + NW * q) * 1024 + lane * 16;
       const int r = byte / RB, c = (byte % RB) / 16 ^ swz(r);
-      k[q] = KR ? r : c * 8;
-      off[q] = (KR ? c * 8 : r) < extent ? static_cast<unsigned>(r * ld * 2 + c * 16) : OOB;
+      k[q] = KR ? r : c * VE;
+      off[q] = (KR ? c * VE : r) < extent ? static_cast<unsigned>(r * ld * ES + c * 16) : OOB;
     }
   }
   // The stage whose first element is at `base` to the LDS address `lds` (of this wave's first load);
   // contraction indices at or past `lim` as zeros.
-  __device__ __forceinline__ void issue(const uint16_t* base, unsigned lds) const {
+  __device__ __forceinline__ void issue(const unsigned char* base, unsigned lds) const {
     const __amdgpu_buffer_rsrc_t r = rsrc(base);
 #pragma unroll
     for (int q = 0; q < Q; ++q) dma16(r, off[q], lds + NW * q * 1024);
   }
-  __device__ __forceinline__ void issue_cut(const uint16_t* base, unsigned lds, int lim) const {
+  __device__ __forceinline__ void issue_cut(const unsigned char* base, unsigned lds, int lim) const {
     const __amdgpu_buffer_rsrc_t r = rsrc(base);
 #pragma unroll
     for (int q = 0; q < Q; ++q) dma16(r, k[q] < lim ? off[q] : OOB, lds + NW * q * 1024);
@@ -170,46 +179,57 @@ __device__ __forceinline__ void sched_kstep() {
   if constexpr (G + 1 < M) sched_kstep<RD, M, G + 1>();
 }
 
-// The fragments of one side: F blocks of 32 rows from row `first` on, k-step ks of the stage.
-template <int B, int F, bool KR, int K>
+// The fragments of one side: F blocks of 32 rows from row `first` on, k-step ks (32 bytes of every row) of
+// the stage.  bf16: a lane holds 8 of a k-step's 16 elements; fp32: 4 of its 8, those from 4 (lane / 32) on,
+// whichever way they lie, one for each of four MFMAs.
+template <int B, int F, bool KR, int K, int ES>
 struct Fragments {
-  using S = Stream<B, 1, KR, K>;
+  using S = Stream<B, 1, KR, K, ES>;
   int at[KR ? F : 1];
   int lo, hi;
   __device__ __forceinline__ void init(int first) {
     const int lane = threadIdx.x & 63;
-    if constexpr (KR) {
+    lo = hi = 0;
+    if constexpr (KR && ES == 4) {
+#pragma unroll
+      for (int i = 0; i < F; ++i) at[i] = 4 * (lane >> 5) * S::RB + (first + i * 32 + (lane & 31)) * 4;
+    } else if constexpr (KR) {
       const int g = lane >> 4, row = 8 * (g >> 1) + ((lane >> 2) & 3);
 #pragma unroll
       for (int i = 0; i < F; ++i) {
         const int col = first + i * 32 + 16 * (g & 1) + 4 * (lane & 3);
         at[i] = row * S::RB + ((col >> 3) ^ S::swz(row)) * 16 + (col & 7) * 2;
       }
-      lo = hi = 0;
     } else {
       at[0] = (first + (lane & 31)) * S::RB;
       lo = S::swz(lane & 31), hi = lane >> 5;   // blocks start at multiples of 32 rows
     }
   }
-  __device__ __forceinline__ void load(const unsigned char* side, int ks, bf16x8_t (&f)[F]) const {
+  __device__ __forceinline__ void load(const unsigned char* side, int ks, f32x4_t (&f)[F]) const {
 #pragma unroll
     for (int i = 0; i < F; ++i) {
-      if constexpr (KR) {
-        const unsigned char* p = side + at[i] + ks * 16 * B * 2;
+      if constexpr (KR && ES == 4) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          f[i][q] = *reinterpret_cast<const float*>(side + at[i] + (8 * ks + q) * S::RB);
+      } else if constexpr (KR) {
+        const unsigned char* p = side + at[i] + ks * 16 * S::RB;
         f[i] = __builtin_bit_cast(
-            bf16x8_t, __builtin_shufflevector(lds_tr16(p), lds_tr16(p + 4 * B * 2), 0, 1, 2, 3, 4,
-                                              5, 6, 7));
+            f32x4_t, __builtin_shufflevector(lds_tr16(p), lds_tr16(p + 4 * S::RB), 0, 1, 2, 3, 4, 5, 6,
+                                             7));
       } else {
-        f[i] = *reinterpret_cast<const bf16x8_t*>(side + at[0] + i * 32 * S::RB +
-                                                  ((2 * ks + hi) ^ lo) * 16);
+        f[i] = *reinterpret_cast<const f32x4_t*>(side + at[0] + i * 32 * S::RB +
+                                                 ((2 * ks + hi) ^ lo) * 16);
       }
     }
   }
 };
 
-// Which products of parts a product is: the operands as they are; one side (dz) in two parts; both in
-// three, of which six products count, the small ones first.
-enum Terms { ONE = 1, TWO_A = 2, TWO_B = 3, SIX = 6 };
+// Which products a product is made of: the operands as they are; of dz in two parts on one side; of three
+// parts on both, of which six count, the small ones first; of fp32 operands as they are, on fp32 MFMAs.
+enum Terms { ONE = 1, TWO_A = 2, TWO_B = 3, SIX = 6, FULL = 7 };
+constexpr int size_of(int terms) { return terms == FULL ? 4 : 2; }   // of an operand's element
+constexpr int terms_in(int terms) { return terms == TWO_B ? 2 : terms == FULL ? 1 : terms; }
 
 // acc = sum over the contraction [k0, k1) of A B^T.
 //
@@ -221,20 +241,21 @@ template <class C, bool AKR, bool BKR, int TERMS>
 __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_t b_extent,
                                         int64_t k0, int64_t k1, unsigned char* lds,
                                         f32x16_t (&acc)[C::MI][C::NI]) {
-  a.p = reinterpret_cast<const uint16_t*>(scalar(reinterpret_cast<int64_t>(a.p)));
-  b.p = reinterpret_cast<const uint16_t*>(scalar(reinterpret_cast<int64_t>(b.p)));
+  a.p = reinterpret_cast<const unsigned char*>(scalar(reinterpret_cast<int64_t>(a.p)));
+  b.p = reinterpret_cast<const unsigned char*>(scalar(reinterpret_cast<int64_t>(b.p)));
   k0 = scalar(k0), k1 = scalar(k1);
-  constexpr int KS = C::K / 16;   // k-steps of a stage
+  constexpr int ES = size_of(TERMS), KE = C::K * 2 / ES;   // contraction of a stage
+  constexpr int KS = C::K / 16;                            // k-steps of a stage
   static_assert(KS % 2 == 0, "the fragments' two buffers take turns");
-  Stream<C::BM, C::NW, AKR, C::K> sa;
-  Stream<C::BN, C::NW, BKR, C::K> sb;
+  Stream<C::BM, C::NW, AKR, C::K, ES> sa;
+  Stream<C::BN, C::NW, BKR, C::K, ES> sb;
   sa.init(a.ld, a_extent);
   sb.init(b.ld, b_extent);
   constexpr int NQ = sa.Q + sb.Q;
   static_assert(NQ * (C::NS - 2) < 64, "vmcnt range");
   const int wid = threadIdx.x >> 6, wm = wid / C::WN, wn = wid % C::WN;
-  Fragments<C::BM, C::MI, AKR, C::K> fa;
-  Fragments<C::BN, C::NI, BKR, C::K> fb;
+  Fragments<C::BM, C::MI, AKR, C::K, ES> fa;
+  Fragments<C::BN, C::NI, BKR, C::K, ES> fb;
   fa.init(wm * C::MI * 32);
   fb.init(wn * C::NI * 32);
 #pragma unroll
@@ -246,25 +267,25 @@ __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_
 
   const unsigned lds0 =
       lds_addr(lds) + static_cast<unsigned>(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 1024u;
-  const int nk = k1 > k0 ? static_cast<int>((k1 - k0 + C::K - 1) / C::K) : 0;
-  const int total = nk * (TERMS == TWO_B ? 2 : TERMS);
+  const int nk = k1 > k0 ? static_cast<int>((k1 - k0 + KE - 1) / KE) : 0;
+  const int total = nk * terms_in(TERMS);
   // The next stage to load: its slot, its first elements, and how many stages its term has left.  Only
   // these change from stage to stage, in scalar registers.
-  const int last = static_cast<int>((k1 - k0) % C::K);   // contraction of a term's last stage, 0: a whole one
-  const int64_t step_a = AKR ? C::K * a.ld : C::K, step_b = BKR ? C::K * b.ld : C::K;
-  const uint16_t* first_a = a.p + (AKR ? k0 * a.ld : k0);
-  const uint16_t* first_b = b.p + (BKR ? k0 * b.ld : k0);
+  const int last = static_cast<int>((k1 - k0) % KE);   // contraction of a term's last stage, 0: a whole one
+  const int64_t step_a = (AKR ? KE * a.ld : KE) * ES, step_b = (BKR ? KE * b.ld : KE) * ES;
+  const unsigned char* first_a = a.p + (AKR ? k0 * a.ld : k0) * ES;
+  const unsigned char* first_b = b.p + (BKR ? k0 * b.ld : k0) * ES;
   int term = 0, left = nk;
-  const uint16_t *pa, *pb;
+  const unsigned char *pa, *pb;
   auto begin_term = [&] {
     pa = first_a, pb = first_b;
     if constexpr (TERMS == SIX) {   // (l h) (h l) (m m) (m h) (h m) (h h)
-      pa += (term == 0 ? 2 : term == 2 || term == 3 ? 1 : 0) * a.part;
-      pb += (term == 1 ? 2 : term == 2 || term == 4 ? 1 : 0) * b.part;
+      pa += (term == 0 ? 2 : term == 2 || term == 3 ? 1 : 0) * a.part * ES;
+      pb += (term == 1 ? 2 : term == 2 || term == 4 ? 1 : 0) * b.part * ES;
     } else if constexpr (TERMS == TWO_A) {
-      pa += term == 0 ? a.part : 0;
+      pa += term == 0 ? a.part * ES : 0;
     } else if constexpr (TERMS == TWO_B) {
-      pb += term == 0 ? b.part : 0;
+      pb += term == 0 ? b.part * ES : 0;
     }
   };
   begin_term();
@@ -281,10 +302,10 @@ __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_
     pa += step_a, pb += step_b;
     if (--left == 0) {
       left = nk;
-      if constexpr (TERMS != ONE) ++term, begin_term();
+      if constexpr (terms_in(TERMS) > 1) ++term, begin_term();
     }
   };
-  bf16x8_t af[2][C::MI], bf[2][C::NI];
+  f32x4_t af[2][C::MI], bf[2][C::NI];
   auto load = [&](int buf, const unsigned char* stage, int ks) {
     fa.load(stage, ks, af[buf]);
     fb.load(stage + C::A_BYTES, ks, bf[buf]);
@@ -293,10 +314,21 @@ __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_
 #pragma unroll
     for (int i = 0; i < C::MI; ++i)
 #pragma unroll
-      for (int j = 0; j < C::NI; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[buf][i], bf[buf][j], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < C::NI; ++j) {
+        if constexpr (ES == 4) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(af[buf][i][q], bf[buf][j][q], acc[i][j], 0, 0, 0);
+        } else {
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, af[buf][i]),
+                                                              __builtin_bit_cast(bf16x8_t, bf[buf][j]),
+                                                              acc[i][j], 0, 0, 0);
+        }
+      }
   };
-  constexpr int RD = (AKR ? 2 : 1) * C::MI + (BKR ? 2 : 1) * C::NI, M = C::MI * C::NI;
+  constexpr int KRD = ES == 4 ? 4 : 2;   // reads of a fragment whose contraction index is the row
+  constexpr int RD = (AKR ? KRD : 1) * C::MI + (BKR ? KRD : 1) * C::NI;
+  constexpr int M = C::MI * C::NI * (ES == 4 ? 4 : 1);
   if (total > 0) {
 #pragma unroll
     for (int s = 0; s < C::NS - 1; ++s)
@@ -353,7 +385,7 @@ struct RowsArgs {
   int64_t x_stride;
   const int64_t* labels;
   int64_t ignore_index, N, V, d, dp;
-  uint16_t* Xc;        // [parts][N][dp]
+  void* Xc;            // [N][dp], for fp32 of many rows [parts][N][dp] bf16
   int32_t* at;         // [N]: the row's place among those that count, or -1
   int32_t* rows;       // [N]: the rows that count
   int32_t* label;      // [N]: their labels, -1 outside the vocabulary
@@ -384,12 +416,11 @@ __device__ __forceinline__ void split3(float x, uint16_t (&p)[3]) {
   p[2] = f32_to_bf16(r - bf16_to_f32(p[1]));
 }
 
-// One row of `n` elements to a row of np (a multiple of 8) bf16 ones, zeros behind; fp32 into three
-// parts `part` elements apart.  `t` of `nt` threads.
-template <class E>
-__device__ __forceinline__ void copy_row(const E* src, int64_t n, uint16_t* dst, int64_t np,
-                                         int64_t part, int t, int nt) {
-  constexpr bool F32 = sizeof(E) == 4;
+// One row of `n` elements to a row of np (a multiple of 8), zeros behind; with SPLIT fp32 ones into three
+// bf16 parts `part` elements apart.  `t` of `nt` threads.
+template <class E, bool SPLIT>
+__device__ __forceinline__ void copy_row(const E* src, int64_t n, void* to, int64_t np, int64_t part, int t,
+                                         int nt) {
   const bool vec = n % 8 == 0 && reinterpret_cast<uintptr_t>(src) % 16 == 0;
   for (int64_t f = static_cast<int64_t>(t) * 8; f < np; f += nt * 8) {
     union { uint4 u[sizeof(E) / 2]; E e[8]; } w;
@@ -401,9 +432,12 @@ __device__ __forceinline__ void copy_row(const E* src, int64_t n, uint16_t* dst,
 #pragma unroll
       for (int i = 0; i < 8; ++i) w.e[i] = f + i < n ? src[f + i] : E(0);
     }
-    if constexpr (!F32) {
-      *reinterpret_cast<uint4*>(dst + f) = w.u[0];
+    if constexpr (!SPLIT) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(E) / 2); ++i)
+        reinterpret_cast<uint4*>(static_cast<E*>(to) + f)[i] = w.u[i];
     } else {
+      uint16_t* dst = static_cast<uint16_t*>(to);
       union { uint4 u; uint16_t e[8]; } o[3];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -418,8 +452,9 @@ __device__ __forceinline__ void copy_row(const E* src, int64_t n, uint16_t* dst,
   }
 }
 
-template <class E>
+template <class E, bool SPLIT>
 __global__ void __launch_bounds__(256) head_rows_kernel(RowsArgs a) {
+  using O = std::conditional_t<SPLIT, uint16_t, E>;
   __shared__ int red[4];
   const int64_t first = static_cast<int64_t>(blockIdx.x) * GROUP;
   const int64_t c = first / CHUNK;
@@ -450,20 +485,22 @@ __global__ void __launch_bounds__(256) head_rows_kernel(RowsArgs a) {
         }
       }
       if (keep)
-        copy_row(static_cast<const E*>(a.X) + r * a.x_stride, a.d, a.Xc + place * a.dp, a.dp,
-                 a.N * a.dp, lane, 64);
+        copy_row<E, SPLIT>(static_cast<const E*>(a.X) + r * a.x_stride, a.d,
+                           static_cast<O*>(a.Xc) + place * a.dp, a.dp, a.N * a.dp, lane, 64);
     }
     place += keep;
   }
   if (first + GROUP >= a.N && threadIdx.x == 0) *a.count = place;
 }
 
-// A piece of W as the products take it: rows of dp elements, in three parts for fp32.
-template <class E>
-__global__ void __launch_bounds__(256) head_weight_kernel(const E* W, int64_t rows, int64_t d,
-                                                          uint16_t* out, int64_t dp) {
+// A piece of W as the products take it: rows of dp elements, in three parts for fp32 of many rows.
+template <class E, bool SPLIT>
+__global__ void __launch_bounds__(256) head_weight_kernel(const E* W, int64_t rows, int64_t d, void* out,
+                                                          int64_t dp) {
+  using O = std::conditional_t<SPLIT, uint16_t, E>;
   const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (r < rows) copy_row(W + r * d, d, out + r * dp, dp, rows * dp, threadIdx.x & 63, 64);
+  if (r < rows)
+    copy_row<E, SPLIT>(W + r * d, d, static_cast<O*>(out) + r * dp, dp, rows * dp, threadIdx.x & 63, 64);
 }
 
 // ------------------------------------------------------------------------------ logits
@@ -535,7 +572,7 @@ __global__ void __launch_bounds__(C::NT, 2) head_logits_kernel(LogitsArgs p) {
   const int64_t m0 = vt * C::BM, n0 = tt * C::BN;
   f32x16_t acc[C::MI][C::NI];
   Side a = p.w, b = p.x;
-  a.p += m0 * a.ld, b.p += n0 * b.ld;
+  a.move<size_of(TERMS)>(m0 * a.ld), b.move<size_of(TERMS)>(n0 * b.ld);
   product<C, false, false, TERMS>(a, p.V - m0, b, count - n0, 0, p.dp, lds, acc);
 
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
@@ -596,7 +633,7 @@ __global__ void __launch_bounds__(C::NT, 2) head_logits_kernel(LogitsArgs p) {
   } else {
     // dz in place of the logits, then through LDS to rows of BM entries; chunk c (8 entries) of
     // row r at slot c ^ r % CH, so that neither side of the turn meets in a bank
-    constexpr int CH = C::BM / 8, PARTS = MODE == ROWS ? 1 : dz_parts<C>(TERMS == SIX);
+    constexpr int CH = C::BM / 8, PARTS = MODE == ROWS || TERMS == FULL ? 1 : dz_parts<C>(TERMS == SIX);
     static_assert(C::BN * C::BM * 2 <= C::LDS, "the tile of dz fits the stages");
 #pragma unroll
     for (int j = 0; j < C::NI; ++j) {
@@ -621,12 +658,14 @@ __global__ void __launch_bounds__(C::NT, 2) head_logits_kernel(LogitsArgs p) {
       }
     }
     if (ragged) behind<C>(acc, static_cast<int>(p.V - m0) - row0, 0.f);   // also where the row is NaN
-    if constexpr (MODE == ROWS && TERMS == SIX) {   // fp32, straight from the lanes
+    if constexpr (TERMS == FULL || (MODE == ROWS && TERMS == SIX)) {   // fp32, straight from the lanes
 #pragma unroll
       for (int j = 0; j < C::NI; ++j) {
         const int64_t n = n0 + (wn * C::NI + j) * 32 + (lane & 31);
         if (n >= count) continue;
-        float* out = static_cast<float*>(p.out) + p.rows[n] * p.vp + m0 + row0;
+        float* out = MODE == ROWS ? static_cast<float*>(p.out) + p.rows[n] * p.vp
+                                  : reinterpret_cast<float*>(p.dz) + n * p.vp;
+        out += m0 + row0;
 #pragma unroll
         for (int i = 0; i < C::MI; ++i)
 #pragma unroll
@@ -748,30 +787,42 @@ __global__ void __launch_bounds__(256) head_zero_rows_kernel(const int32_t* at, 
 
 // ------------------------------------------------------------------------------ gradients
 
+// How often a piece's vocabulary is split among the workgroups for dx, by the rows that count, whose number
+// only the device knows: `slots` workgroups for the tiles there are, in up to `most` shares.  (By the
+// rows that came, a batch half of which is padding has every second unit without work.)
+struct DxSplit {
+  int64_t tile, f_tiles, slots, most;   // tile: rows of one
+  __host__ __device__ int64_t operator()(int64_t count) const {
+    const int64_t tiles = f_tiles * ((count + tile - 1) / tile);
+    const int64_t s = tiles > 0 ? slots / tiles : 1;
+    return s < 1 ? 1 : s < most ? s : most;
+  }
+};
 struct DxArgs {
   Side dz, w;              // [count][vp], [V of the piece][dp]
   const int32_t* count;
   int64_t N, V, dp;        // V: the piece's entries
-  int64_t f_tiles, splits, kper;
-  float* out;              // [splits][N][dp]
+  DxSplit split;
+  float* out;              // [splits][count][dp]
   int add;                 // to what is there
 };
 template <class C, int TERMS>
 __global__ void __launch_bounds__(C::NT, 2) head_dx_kernel(DxArgs p) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
-  const int64_t count = *p.count, t_tiles = (count + C::BM - 1) / C::BM;
-  const int64_t tiles = p.f_tiles * t_tiles, total = tiles * p.splits;
+  const int64_t count = *p.count, t_tiles = (count + C::BM - 1) / C::BM, f_tiles = p.split.f_tiles;
+  const int64_t tiles = f_tiles * t_tiles, splits = p.split(count), total = tiles * splits;
   if (blockIdx.x >= total) return;
   const int64_t i0 = xcd_order(blockIdx.x, total), split = i0 / tiles, r0 = i0 - split * tiles;
-  const int64_t m0 = r0 / p.f_tiles * C::BM, n0 = r0 % p.f_tiles * C::BN;
-  const int64_t k0 = split * p.kper, k1 = k0 + p.kper < p.V ? k0 + p.kper : p.V;
+  const int64_t m0 = r0 / f_tiles * C::BM, n0 = r0 % f_tiles * C::BN;
+  const int64_t per = ((p.V + splits - 1) / splits + 63) / 64 * 64;
+  const int64_t k0 = split * per, k1 = k0 + per < p.V ? k0 + per : p.V;
   f32x16_t acc[C::MI][C::NI];
   Side a = p.dz, b = p.w;
-  a.p += m0 * a.ld, b.p += n0;
+  a.move<size_of(TERMS)>(m0 * a.ld), b.move<size_of(TERMS)>(n0);
   product<C, false, true, TERMS>(a, count - m0, b, p.dp - n0, k0, k1, lds, acc);
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int wm = wid / C::WN, wn = wid % C::WN;
-  float* out = p.out + split * p.N * p.dp;
+  float* out = p.out + split * count * p.dp;
 #pragma unroll
   for (int j = 0; j < C::NI; ++j) {
     const int64_t f = n0 + (wn * C::NI + j) * 32 + (lane & 31);
@@ -788,57 +839,71 @@ __global__ void __launch_bounds__(C::NT, 2) head_dx_kernel(DxArgs p) {
   }
 }
 
-// dx of every row: its sums over the splits, scaled and rounded once; zeros where it does not count.  A
-// workgroup takes 64 features of a row, its four waves every fourth split (a row's 42 splits of 768
+// dx of every row: its sums over the splits, scaled and rounded once; zeros where it does not count.
+struct DxFinishArgs {
+  const float* sums;
+  DxSplit split;
+  const int32_t *at, *count;
+  int64_t N, d, dp, f_blocks;
+  const float* up;
+  int mean;
+  void* dx;
+};
+// A workgroup takes 64 features of a row, its four waves every fourth split (a row's 42 splits of 768
 // features by one wave: 119 us for eight rows).
 template <class E>
-__global__ void __launch_bounds__(256) head_dx_finish_kernel(
-    const float* sums, int64_t splits, const int32_t* at, const int32_t* count, int64_t N, int64_t d,
-    int64_t dp, int64_t f_blocks, const float* up, int mean, E* dx) {
+__global__ void __launch_bounds__(256) head_dx_finish_kernel(DxFinishArgs p) {
   __shared__ float red[4][64];
   const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
-  const int64_t r = blockIdx.x / f_blocks, f = (blockIdx.x - r * f_blocks) * 64 + lane;
-  const int64_t j = at[r];
+  const int64_t r = blockIdx.x / p.f_blocks, f = (blockIdx.x - r * p.f_blocks) * 64 + lane;
+  const int64_t j = p.at[r], count = *p.count;
   float s = 0.f;
-  if (j >= 0 && f < d) {
+  if (j >= 0 && f < p.d) {
+    const int splits = static_cast<int>(p.split(count));
 #pragma unroll 4
-    for (int64_t k = g; k < splits; k += 4) s += sums[(k * N + j) * dp + f];
+    for (int k = g; k < splits; k += 4) s += p.sums[(k * count + j) * p.dp + f];
   }
   red[g][lane] = s;
   __syncthreads();
-  if (g != 0 || f >= d) return;
+  if (g != 0 || f >= p.d) return;
   s = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
-  dx[r * d + f] = from_f32<E>(j >= 0 ? s * gradient_scale(up, mean, *count) : 0.f);
+  static_cast<E*>(p.dx)[r * p.d + f] =
+      from_f32<E>(j >= 0 ? s * gradient_scale(p.up, p.mean, count) : 0.f);
 }
-// The same of one split: a wave to a row.
+// The same of many rows and few splits: a wave to a row, 16 bytes and more a lane.
 template <class E>
-__global__ void __launch_bounds__(256) head_dx_round_kernel(const float* sums, const int32_t* at,
-                                                            const int32_t* count, int64_t N, int64_t d,
-                                                            int64_t dp, const float* up, int mean, E* dx) {
-  const float scale = gradient_scale(up, mean, *count);
+__global__ void __launch_bounds__(256) head_dx_rows_kernel(DxFinishArgs p) {
+  const int64_t count = *p.count;
+  const float scale = gradient_scale(p.up, p.mean, count);
   const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (r >= N) return;
-  const int64_t j = at[r];
-  const bool vec = d % 8 == 0 && reinterpret_cast<uintptr_t>(dx) % 16 == 0;
-  for (int64_t f = (threadIdx.x & 63) * 8; f < d; f += 64 * 8) {
+  if (r >= p.N) return;
+  const int64_t j = p.at[r];
+  const int splits = static_cast<int>(p.split(count));
+  E* dx = static_cast<E*>(p.dx);
+  const bool vec = p.d % 8 == 0 && reinterpret_cast<uintptr_t>(dx) % 16 == 0;
+  for (int64_t f = (threadIdx.x & 63) * 8; f < p.d; f += 64 * 8) {
     float v[8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {   // rows of sums are whole eights
-      const float4 q = j >= 0 ? reinterpret_cast<const float4*>(sums + j * dp + f)[h]
-                              : make_float4(0.f, 0.f, 0.f, 0.f);
-      v[4 * h] = q.x, v[4 * h + 1] = q.y, v[4 * h + 2] = q.z, v[4 * h + 3] = q.w;
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    for (int k = 0; j >= 0 && k < splits; ++k) {   // rows of sums are whole eights
+      const float4* q = reinterpret_cast<const float4*>(p.sums + (k * count + j) * p.dp + f);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 u = q[h];
+        v[4 * h] += u.x, v[4 * h + 1] += u.y, v[4 * h + 2] += u.z, v[4 * h + 3] += u.w;
+      }
     }
     union { uint4 u[sizeof(E) / 2]; E e[8]; } o;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o.e[i] = from_f32<E>(j >= 0 ? v[i] * scale : 0.f);
-    E* out = dx + r * d + f;
+    E* out = dx + r * p.d + f;
     if (vec) {
 #pragma unroll
       for (int i = 0; i < static_cast<int>(sizeof(E) / 2); ++i) reinterpret_cast<uint4*>(out)[i] = o.u[i];
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (f + i < d) out[i] = o.e[i];
+        if (f + i < p.d) out[i] = o.e[i];
     }
   }
 }
@@ -865,7 +930,7 @@ __global__ void __launch_bounds__(C::NT, 2) head_dw_kernel(DwArgs p) {
   const int64_t k0 = split * p.kper, k1 = k0 + p.kper < count ? k0 + p.kper : count;
   f32x16_t acc[C::MI][C::NI];
   Side a = p.x, b = p.dz;
-  a.p += m0, b.p += n0;
+  a.move<size_of(TERMS)>(m0), b.move<size_of(TERMS)>(n0);
   product<C, true, true, TERMS>(a, p.dp - m0, b, p.dz.ld - n0, k0, k1, lds, acc);
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int wm = wid / C::WN, wn = wid % C::WN, half = lane >> 5;
@@ -962,15 +1027,18 @@ enum Size { WIDE, MID, SMALL, FEW };
 struct Shape {
   Size size;
   int64_t splits, per;   // per: the contraction of a share
+  int64_t slots;         // workgroups that the splits fill
 };
 
 struct Plan {
   bool f32, few, copy_w;
-  int64_t parts, dz_parts;   // bf16 parts of the operands, and of dz
+  bool full;                 // fp32 operands as they are: a few rows, bound by W's memory
+  int64_t row_bytes, dz_bytes;   // of the operands' elements, all parts, and of dz's
   int64_t dp, cols, pieces;  // cols: vocabulary entries of a piece
   int64_t tiles_all;         // vocabulary tiles of all pieces of the forward pass
   int64_t chunks, blocks;
-  Shape dx;
+  Size dx_size;
+  DxSplit dx;
   int64_t dw_sums;           // fp32 elements that a split piece of dW needs
 };
 
@@ -982,7 +1050,7 @@ struct Plan {
 Shape shape_of(int64_t m, int64_t n, int64_t k, int64_t terms, bool split) {
   static const struct { Size size; int64_t b, slots; double stage; } T[] = {
       {WIDE, 256, 256, 1.75}, {MID, 128, 512, 1.15}, {SMALL, 64, 512, 0.5}};
-  Shape best{WIDE, 1, round_up(k, 64)};
+  Shape best{WIDE, 1, round_up(k, 64), 256};
   double least = 1e300;
   for (const auto& t : T) {
     const int64_t tiles = cdiv(m, t.b) * cdiv(n, t.b), stages = cdiv(k, 64);
@@ -993,7 +1061,7 @@ Shape shape_of(int64_t m, int64_t n, int64_t k, int64_t terms, bool split) {
       const int64_t per = cdiv(stages, want), splits = cdiv(stages, per);
       const double us = cdiv(tiles * splits, t.slots) * (per * terms * t.stage + 4.0) +
                         (splits > 1 ? 4.0 + splits * m * n * 8 / 2e6 : 0.0);
-      if (us < least) least = us, best = Shape{t.size, splits, per * 64};
+      if (us < least) least = us, best = Shape{t.size, splits, per * 64, i == 2 ? 2 * t.slots : t.slots};
     }
   }
   return best;
@@ -1013,38 +1081,48 @@ int check_head(const gs_head* h, const char* what) {
   return GS_OK;
 }
 
+int64_t rows_of(Size s) { return s == WIDE ? 256 : s == MID ? 128 : s == SMALL ? 64 : Few::BM; }
 int64_t terms_of(const Plan& p) { return p.f32 ? 6 : 1; }
 
 Shape logits_shape(const gs_head& h, const Plan& p, int64_t n) {
-  if (p.few) return Shape{FEW, 1, 0};
+  if (p.few) return Shape{FEW, 1, 0, 0};
   return shape_of(n, h.N, h.d, terms_of(p), false);
 }
 // dx of a piece of `most` entries.
-Shape dx_shape(const gs_head& h, const Plan& p, int64_t most) {
-  if (!p.few) return shape_of(h.N, p.dp, most, terms_of(p), true);
-  // a few rows: shares of at least 256 entries, for every unit one
-  const int64_t tiles = cdiv(p.dp, FewT::BN);
-  const int64_t splits = std::max<int64_t>(1, std::min(CUS / tiles, cdiv(most, 256)));
-  const int64_t per = round_up(cdiv(most, splits), 64);
-  return Shape{FEW, cdiv(most, per), per};
+Size dx_shape(const gs_head& h, const Plan& p, int64_t most, DxSplit& split) {
+  if (p.few) {   // a share of at least 256 entries for every unit
+    split = DxSplit{FewT::BM, cdiv(p.dp, FewT::BN), CUS, cdiv(most, 256)};
+    return FEW;
+  }
+  const Shape s = shape_of(h.N, p.dp, most, terms_of(p), true);
+  const int64_t tile = rows_of(s.size);
+  split = DxSplit{tile, cdiv(p.dp, tile), s.slots, cdiv(most, 256)};
+  return s.size;
+}
+// The fp32 sums that dx's shares take, for any number of rows that count.
+int64_t dx_sums(const gs_head& h, const Plan& p) {
+  int64_t most = h.N;
+  for (int64_t n = p.dx.tile; n < h.N + p.dx.tile && p.dx(n) > 1; n += p.dx.tile)
+    most = std::max(most, p.dx(n) * std::min(n, h.N));
+  return most * p.dp;
 }
 Shape dw_shape(const gs_head& h, const Plan& p, int64_t n) {
-  if (p.few) return Shape{FEW, 1, 64};
+  if (p.few) return Shape{FEW, 1, 64, 0};
   return shape_of(n, h.d, h.N, terms_of(p), true);
 }
-int64_t rows_of(Size s) { return s == WIDE ? 256 : s == MID ? 128 : s == SMALL ? 64 : Few::BM; }
 
 // The plan of a call.
 Plan plan_of(const gs_head& h, bool w_aligned) {
   Plan p{};
   p.f32 = h.dtype == GS_DTYPE_F32;
-  p.parts = p.f32 ? 3 : 1;
-  p.dp = round_up(h.d, 8);
-  p.copy_w = p.f32 || h.d % 8 != 0 || !w_aligned;
   p.few = h.N <= FEW_ROWS;
-  p.dz_parts = p.few ? dz_parts<Few>(p.f32) : dz_parts<Wide>(p.f32);
+  p.full = p.f32 && p.few;
+  p.dp = round_up(h.d, 8);
+  p.copy_w = (p.f32 && !p.full) || h.d % 8 != 0 || !w_aligned;
+  p.row_bytes = p.full ? 4 : p.f32 ? 6 : 2;
+  p.dz_bytes = p.full ? 4 : 2 * (p.few ? dz_parts<Few>(p.f32) : dz_parts<Wide>(p.f32));
   const int64_t all = cdiv(h.V, 256);
-  const int64_t most = std::max<int64_t>(1, PIECE_BYTES / (h.N * 2 * p.dz_parts * 256));
+  const int64_t most = std::max<int64_t>(1, PIECE_BYTES / (h.N * p.dz_bytes * 256));
   if (all <= most) {
     p.cols = all * 256;
   } else {
@@ -1063,14 +1141,14 @@ Plan plan_of(const gs_head& h, bool w_aligned) {
     const Shape w = dw_shape(h, p, n);
     if (w.splits > 1) p.dw_sums = std::max(p.dw_sums, w.splits * n * h.d);
   }
-  p.dx = dx_shape(h, p, std::min(p.cols, h.V));
+  p.dx_size = dx_shape(h, p, std::min(p.cols, h.V), p.dx);
   p.chunks = h.N > CHUNK ? cdiv(h.N, CHUNK) : 0;
   p.blocks = cdiv(h.N, 64);
   return p;
 }
 
 struct Buffers {
-  uint16_t *xc, *wc, *dz;
+  unsigned char *xc, *wc, *dz;
   int32_t *at, *rows, *label, *count, *chunk;
   float2* part;
   float *label_z, *sums, *dx, *dw;
@@ -1078,20 +1156,20 @@ struct Buffers {
 template <class S>
 Buffers carve(S& s, const gs_head& h, const Plan& p, bool grad) {
   Buffers b{};
-  b.xc = s.template take<uint16_t>(p.parts * h.N * p.dp);
+  b.xc = s.template take<unsigned char>(p.row_bytes * h.N * p.dp);
   b.at = s.template take<int32_t>(h.N);
   b.rows = s.template take<int32_t>(h.N);
   b.label = s.template take<int32_t>(h.N);
   b.count = s.template take<int32_t>(1);
   b.chunk = s.template take<int32_t>(std::max<int64_t>(1, p.chunks));
-  if (p.copy_w) b.wc = s.template take<uint16_t>(p.parts * std::min(p.cols, h.V) * p.dp);
+  if (p.copy_w) b.wc = s.template take<unsigned char>(p.row_bytes * std::min(p.cols, h.V) * p.dp);
   if (!grad) {
     b.part = s.template take<float2>(p.tiles_all * h.N);
     b.label_z = s.template take<float>(h.N);
     b.sums = s.template take<float>(p.blocks);
   } else {
-    b.dz = s.template take<uint16_t>(p.dz_parts * h.N * p.cols);
-    b.dx = s.template take<float>(p.dx.splits * h.N * p.dp);
+    b.dz = s.template take<unsigned char>(p.dz_bytes * h.N * p.cols);
+    b.dx = s.template take<float>(dx_sums(h, p));
     if (p.dw_sums > 0) b.dw = s.template take<float>(p.dw_sums);
   }
   return b;
@@ -1111,24 +1189,30 @@ void launch_rows(const gs_head& h, const Plan& p, const Buffers& b, float* loss,
   if (p.chunks > 0)
     hipLaunchKernelGGL(head_count_kernel, dim3(grid_of(p.chunks)), dim3(256), 0, s, a, b.chunk);
   const dim3 grid(grid_of(cdiv(h.N, GROUP)));
-  if (p.f32)
-    hipLaunchKernelGGL(head_rows_kernel<float>, grid, dim3(256), 0, s, a);
+  if (p.full)
+    hipLaunchKernelGGL((head_rows_kernel<float, false>), grid, dim3(256), 0, s, a);
+  else if (p.f32)
+    hipLaunchKernelGGL((head_rows_kernel<float, true>), grid, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL(head_rows_kernel<uint16_t>, grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((head_rows_kernel<uint16_t, false>), grid, dim3(256), 0, s, a);
 }
 
 // W's rows [v0, v0 + n) as the products take them.
 Side weight_side(const gs_head& h, const Plan& p, const Buffers& b, int64_t v0, int64_t n,
                  hipStream_t s) {
-  if (!p.copy_w) return Side{static_cast<const uint16_t*>(h.W) + v0 * h.d, h.d, 0};
+  const void* w = static_cast<const char*>(h.W) + v0 * h.d * static_cast<int64_t>(elem_size(h.dtype));
+  if (!p.copy_w) return side_of(w, h.d, 0);
   const dim3 grid(grid_of(cdiv(n, 4)));
-  if (p.f32)
-    hipLaunchKernelGGL(head_weight_kernel<float>, grid, dim3(256), 0, s,
-                       static_cast<const float*>(h.W) + v0 * h.d, n, h.d, b.wc, p.dp);
+  if (p.full)
+    hipLaunchKernelGGL((head_weight_kernel<float, false>), grid, dim3(256), 0, s,
+                       static_cast<const float*>(w), n, h.d, b.wc, p.dp);
+  else if (p.f32)
+    hipLaunchKernelGGL((head_weight_kernel<float, true>), grid, dim3(256), 0, s,
+                       static_cast<const float*>(w), n, h.d, b.wc, p.dp);
   else
-    hipLaunchKernelGGL(head_weight_kernel<uint16_t>, grid, dim3(256), 0, s,
-                       static_cast<const uint16_t*>(h.W) + v0 * h.d, n, h.d, b.wc, p.dp);
-  return Side{b.wc, p.dp, n * p.dp};
+    hipLaunchKernelGGL((head_weight_kernel<uint16_t, false>), grid, dim3(256), 0, s,
+                       static_cast<const uint16_t*>(w), n, h.d, b.wc, p.dp);
+  return side_of(b.wc, p.dp, n * p.dp);
 }
 
 template <class C, int MODE>
@@ -1136,7 +1220,7 @@ void launch_logits_as(LogitsArgs& a, bool f32, hipStream_t s) {
   a.v_tiles = cdiv(a.V, C::BM);
   const dim3 grid(grid_of(a.v_tiles * cdiv(a.N, C::BN)));
   if (f32)
-    hipLaunchKernelGGL((head_logits_kernel<C, SIX, MODE>), grid, dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((head_logits_kernel<C, C::BN == Few::BN ? FULL : SIX, MODE>), grid, dim3(C::NT), 0, s, a);
   else
     hipLaunchKernelGGL((head_logits_kernel<C, ONE, MODE>), grid, dim3(C::NT), 0, s, a);
 }
@@ -1149,10 +1233,9 @@ void launch_logits(LogitsArgs& a, Size size, bool f32, hipStream_t s) {
 }
 template <class C, int TERMS>
 void launch_dx_as(DxArgs& a, bool f32, hipStream_t s) {
-  a.f_tiles = cdiv(a.dp, C::BN);
-  const dim3 grid(grid_of(a.f_tiles * cdiv(a.N, C::BM) * a.splits));
+  const dim3 grid(grid_of(std::max(a.split.slots, a.split.f_tiles * cdiv(a.N, C::BM))));
   if (f32)
-    hipLaunchKernelGGL((head_dx_kernel<C, SIX>), grid, dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((head_dx_kernel<C, C::BM == FewT::BM ? FULL : SIX>), grid, dim3(C::NT), 0, s, a);
   else
     hipLaunchKernelGGL((head_dx_kernel<C, TERMS>), grid, dim3(C::NT), 0, s, a);
 }
@@ -1167,7 +1250,7 @@ void launch_dw_as(DwArgs& a, bool f32, hipStream_t s) {
   a.v_tiles = cdiv(a.V, C::BN), a.f_tiles = cdiv(a.d, C::BM);
   const dim3 grid(grid_of(a.v_tiles * a.f_tiles * a.splits));
   if (f32)
-    hipLaunchKernelGGL((head_dw_kernel<C, SIX, float>), grid, dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((head_dw_kernel<C, C::BM == FewW::BM && C::BN == FewW::BN ? FULL : SIX, float>), grid, dim3(C::NT), 0, s, a);
   else
     hipLaunchKernelGGL((head_dw_kernel<C, TERMS, uint16_t>), grid, dim3(C::NT), 0, s, a);
 }
@@ -1181,15 +1264,11 @@ void launch_dw(DwArgs& a, Size size, bool f32, hipStream_t s) {
 template <class E>
 void launch_dx_finish(const gs_head& h, const Plan& p, const Buffers& b, const float* up, int mean, void* dx,
                       hipStream_t s) {
-  E* out = static_cast<E*>(dx);
-  if (p.dx.splits == 1) {
-    hipLaunchKernelGGL(head_dx_round_kernel<E>, dim3(grid_of(cdiv(h.N, 4))), dim3(256), 0, s, b.dx, b.at,
-                       b.count, h.N, h.d, p.dp, up, mean, out);
-    return;
-  }
-  const int64_t f_blocks = cdiv(h.d, 64);
-  hipLaunchKernelGGL(head_dx_finish_kernel<E>, dim3(grid_of(h.N * f_blocks)), dim3(256), 0, s, b.dx,
-                     p.dx.splits, b.at, b.count, h.N, h.d, p.dp, f_blocks, up, mean, out);
+  const DxFinishArgs a{b.dx, p.dx, b.at, b.count, h.N, h.d, p.dp, cdiv(h.d, 64), up, mean, dx};
+  if (h.N > 4096)
+    hipLaunchKernelGGL(head_dx_rows_kernel<E>, dim3(grid_of(cdiv(h.N, 4))), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(head_dx_finish_kernel<E>, dim3(grid_of(h.N * a.f_blocks)), dim3(256), 0, s, a);
 }
 
 // Whether every grid of a call can be launched: shares are at most 2 * 512 where tiles are few.
@@ -1200,7 +1279,7 @@ bool grids_fit(const gs_head& h, const Plan& p) {
 
 LogitsArgs logits_args(const gs_head& h, const Plan& p, const Buffers& b) {
   LogitsArgs a{};
-  a.x = Side{b.xc, p.dp, h.N * p.dp};
+  a.x = side_of(b.xc, p.dp, h.N * p.dp);
   a.count = b.count, a.label = b.label, a.rows = b.rows;
   a.N = h.N, a.dp = p.dp;
   return a;
@@ -1281,18 +1360,18 @@ extern "C" int gs_head_grad(const gs_head* h, const float* lse, const float* ups
   const float* up = own ? nullptr : upstream;
   launch_rows(*h, p, b, nullptr, s);
   LogitsArgs a = logits_args(*h, p, b);
-  a.lse = lse, a.up = own ? upstream : nullptr, a.dz = b.dz;
+  a.lse = lse, a.up = own ? upstream : nullptr, a.dz = reinterpret_cast<uint16_t*>(b.dz);
   for (int64_t v0 = 0; v0 < h->V; v0 += p.cols) {
     a.v0 = v0, a.V = std::min(p.cols, h->V - v0);
     a.w = weight_side(*h, p, b, v0, a.V, s);
     a.vp = p.cols;
     launch_logits<GRADIENT>(a, logits_shape(*h, p, a.V).size, p.f32, s);
-    const Side dz{b.dz, p.cols, h->N * p.cols};
+    const Side dz = side_of(b.dz, p.cols, h->N * p.cols);
     if (dx != nullptr) {
       DxArgs x{};
       x.dz = dz, x.w = a.w, x.count = b.count, x.N = h->N, x.V = a.V, x.dp = p.dp;
-      x.splits = p.dx.splits, x.kper = p.dx.per, x.out = b.dx, x.add = v0 > 0;
-      launch_dx(x, p.dx.size, p.f32, s);
+      x.split = p.dx, x.out = b.dx, x.add = v0 > 0;
+      launch_dx(x, p.dx_size, p.f32, s);
     }
     if (dw != nullptr) {
       const Shape shape = dw_shape(*h, p, a.V);
@@ -1341,13 +1420,13 @@ static Buffers carve_piece(S& s, const gs_head& h, int64_t n, const Plan& p) {
   gs_head piece = h;
   piece.V = n;
   Buffers b{};
-  b.xc = s.template take<uint16_t>(p.parts * h.N * p.dp);
+  b.xc = s.template take<unsigned char>(p.row_bytes * h.N * p.dp);
   b.at = s.template take<int32_t>(h.N);
   b.rows = s.template take<int32_t>(h.N);
   b.label = s.template take<int32_t>(h.N);
   b.count = s.template take<int32_t>(1);
   b.chunk = s.template take<int32_t>(std::max<int64_t>(1, p.chunks));
-  if (p.copy_w) b.wc = s.template take<uint16_t>(p.parts * n * p.dp);
+  if (p.copy_w) b.wc = s.template take<unsigned char>(p.row_bytes * n * p.dp);
   return b;
 }
 
