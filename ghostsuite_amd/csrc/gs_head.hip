@@ -171,6 +171,7 @@ struct Stream {
   }
 };
 
+// Order of a k-step: its M MFMAs, with the next k-step's RD reads spread between them.
 template <int RD, int M, int G = 0>
 __device__ __forceinline__ void sched_kstep() {
   __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -307,8 +308,8 @@ __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_
   };
   f32x4_t af[2][C::MI], bf[2][C::NI];
   auto load = [&](int buf, const unsigned char* stage, int ks) {
+    fb.load(stage + C::A_BYTES, ks, bf[buf]);   // the first MFMAs take all of B and one of A
     fa.load(stage, ks, af[buf]);
-    fb.load(stage + C::A_BYTES, ks, bf[buf]);
   };
   auto mma = [&](int buf) {
 #pragma unroll
