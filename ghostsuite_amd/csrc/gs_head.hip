@@ -49,12 +49,19 @@ __device__ __forceinline__ unsigned lds_addr(const void* p) {
   typedef const __attribute__((address_space(3))) unsigned char* lds_ptr;
   return static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_ptr)p));
 }
-// 64 lanes' 16 bytes at base + voff to LDS address lds + 16 lane.  Nothing else here uses M0.
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, unsigned voff, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :
-               : "s"(lds), "v"(voff), "s"(r)
-               : "memory");
+// 64 lanes' G (16 or 4) bytes at base + voff to LDS address lds + G lane.  Nothing else here uses M0.
+template <int G>
+__device__ __forceinline__ void dma(__amdgpu_buffer_rsrc_t r, unsigned voff, unsigned lds) {
+  if constexpr (G == 16)
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(lds), "v"(voff), "s"(r)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :
+                 : "s"(lds), "v"(voff), "s"(r)
+                 : "memory");
 }
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* base) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0,
@@ -133,9 +140,10 @@ Side side_of(const void* p, int64_t ld, int64_t part) {
 // so that the 16 rows of a fragment read lie in 16 different bank groups.  KR: LDS row = contraction
 // index, chunk c at slot c ^ swz(row): the 4 rows x 4 chunks of a transpose read in 16 different ones.
 // A stage is as many bytes with elements of 4 (ES) as with those of 2: half the contraction.
-template <int B, int NW, bool KR, int K, int ES>
+// G: the bytes of a lane's load; rows that do not begin at multiples of 16 bytes are loaded by 4.
+template <int B, int NW, bool KR, int K, int ES, int G>
 struct Stream {
-  static constexpr int Q = B * K * 2 / 1024 / NW;   // loads of a wave
+  static constexpr int P = 16 / G, Q = B * K * 2 / 1024 / NW * P;   // loads of a wave
   static_assert(Q > 0 && B * K * 2 % (1024 * NW) == 0, "stage bytes split over waves");
   static constexpr int RB = KR ? B * ES : K * 2, CH = RB / 16;   // bytes and chunks of an LDS row
   static constexpr int VE = 16 / ES;                             // elements of a chunk
@@ -143,6 +151,8 @@ struct Stream {
     if (KR) return ES == 4 ? 0 : CH >= 16 ? 4 * (r & 3) : CH == 8 ? 4 * ((r >> 1) & 1) : 0;
     return CH == 8 ? (r >> 1) & 7 : (r >> 2) & 3;
   }
+  // Where load q of a wave begins, from the wave's first.
+  __device__ static constexpr int at(int q) { return NW * (q / P) * 1024 + q % P * 64 * G; }
   unsigned off[Q];
   int k[Q];
   // `extent`: how many of the side's rows (columns of memory with KR) there are from the tile's
@@ -151,10 +161,10 @@ struct Stream {
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      const int byte = (wid + NW * q) * 1024 + lane * 16;
-      const int r = byte / RB, c = (byte % RB) / 16 ^ swz(r);
-      k[q] = KR ? r : c * VE;
-      off[q] = (KR ? c * VE : r) < extent ? static_cast<unsigned>(r * ld * ES + c * 16) : OOB;
+      const int byte = wid * 1024 + at(q) + lane * G;
+      const int r = byte / RB, c = (byte % RB) / 16 ^ swz(r), e = c * VE + byte % 16 / ES;
+      k[q] = KR ? r : e;
+      off[q] = (KR ? e : r) < extent ? static_cast<unsigned>((r * ld + e) * ES) : OOB;
     }
   }
   // The stage whose first element is at `base` to the LDS address `lds` (of this wave's first load);
@@ -162,12 +172,12 @@ struct Stream {
   __device__ __forceinline__ void issue(const unsigned char* base, unsigned lds) const {
     const __amdgpu_buffer_rsrc_t r = rsrc(base);
 #pragma unroll
-    for (int q = 0; q < Q; ++q) dma16(r, off[q], lds + NW * q * 1024);
+    for (int q = 0; q < Q; ++q) dma<G>(r, off[q], lds + at(q));
   }
   __device__ __forceinline__ void issue_cut(const unsigned char* base, unsigned lds, int lim) const {
     const __amdgpu_buffer_rsrc_t r = rsrc(base);
 #pragma unroll
-    for (int q = 0; q < Q; ++q) dma16(r, k[q] < lim ? off[q] : OOB, lds + NW * q * 1024);
+    for (int q = 0; q < Q; ++q) dma<G>(r, k[q] < lim ? off[q] : OOB, lds + at(q));
   }
 };
 
@@ -185,7 +195,7 @@ __device__ __forceinline__ void sched_kstep() {
 // whichever way they lie, one for each of four MFMAs.
 template <int B, int F, bool KR, int K, int ES>
 struct Fragments {
-  using S = Stream<B, 1, KR, K, ES>;
+  using S = Stream<B, 1, KR, K, ES, 16>;
   int at[KR ? F : 1];
   int lo, hi;
   __device__ __forceinline__ void init(int first) {
@@ -238,7 +248,7 @@ constexpr int terms_in(int terms) { return terms == TWO_B ? 2 : terms == FULL ? 
 // fragments, so the stage's slot can be loaded again, and the next stage has arrived, so its first
 // fragments are read while those MFMAs run.  (Meeting between the stages left the matrix cores idle
 // for the loads' issue and the first reads' latency.)
-template <class C, bool AKR, bool BKR, int TERMS>
+template <class C, bool AKR, bool BKR, int TERMS, int GA = 16, int GB = 16>
 __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_t b_extent,
                                         int64_t k0, int64_t k1, unsigned char* lds,
                                         f32x16_t (&acc)[C::MI][C::NI]) {
@@ -248,8 +258,8 @@ __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_
   constexpr int ES = size_of(TERMS), KE = C::K * 2 / ES;   // contraction of a stage
   constexpr int KS = C::K / 16;                            // k-steps of a stage
   static_assert(KS % 2 == 0, "the fragments' two buffers take turns");
-  Stream<C::BM, C::NW, AKR, C::K, ES> sa;
-  Stream<C::BN, C::NW, BKR, C::K, ES> sb;
+  Stream<C::BM, C::NW, AKR, C::K, ES, GA> sa;
+  Stream<C::BN, C::NW, BKR, C::K, ES, GB> sb;
   sa.init(a.ld, a_extent);
   sb.init(b.ld, b_extent);
   constexpr int NQ = sa.Q + sb.Q;
@@ -507,10 +517,10 @@ __global__ void __launch_bounds__(256) head_weight_kernel(const E* W, int64_t ro
 // ------------------------------------------------------------------------------ logits
 
 struct LogitsArgs {
-  Side w, x;                 // [V of the piece][dp], [count][dp]
+  Side w, x;                 // [V of the piece][dp or d], [count][dp]
   const int32_t* count;
   const int32_t* label;
-  int64_t N, V, v0, dp;      // v0: the piece's first entry; V: the piece's entries
+  int64_t N, V, v0, k;       // v0: the piece's first entry; V: the piece's entries; k: W's features
   int64_t v_tiles;
   // forward: per vocabulary tile (of all pieces) and row
   float2* part;              // [tiles][N]: maximum of z log2(e), sum of 2^(z log2(e) - maximum)
@@ -564,7 +574,7 @@ __device__ __forceinline__ void behind(f32x16_t (&acc)[C::MI][C::NI], int left, 
 // What becomes of a tile of logits: the forward pass's parts, dz for the products, or dz for the caller.
 enum { FORWARD, GRADIENT, ROWS };
 
-template <class C, int TERMS, int MODE>
+template <class C, int TERMS, int MODE, int GW>
 __global__ void __launch_bounds__(C::NT, 2) head_logits_kernel(LogitsArgs p) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
   const int64_t count = *p.count;
@@ -574,7 +584,7 @@ __global__ void __launch_bounds__(C::NT, 2) head_logits_kernel(LogitsArgs p) {
   f32x16_t acc[C::MI][C::NI];
   Side a = p.w, b = p.x;
   a.move<size_of(TERMS)>(m0 * a.ld), b.move<size_of(TERMS)>(n0 * b.ld);
-  product<C, false, false, TERMS>(a, p.V - m0, b, count - n0, 0, p.dp, lds, acc);
+  product<C, false, false, TERMS, GW>(a, p.V - m0, b, count - n0, 0, p.k, lds, acc);
 
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int wm = wid / C::WN, wn = wid % C::WN, half = lane >> 5;
@@ -800,14 +810,14 @@ struct DxSplit {
   }
 };
 struct DxArgs {
-  Side dz, w;              // [count][vp], [V of the piece][dp]
+  Side dz, w;              // [count][vp], [V of the piece][k]
   const int32_t* count;
-  int64_t N, V, dp;        // V: the piece's entries
+  int64_t N, V, dp, k;     // V: the piece's entries; k: W's features
   DxSplit split;
   float* out;              // [splits][count][dp]
   int add;                 // to what is there
 };
-template <class C, int TERMS>
+template <class C, int TERMS, int GW>
 __global__ void __launch_bounds__(C::NT, 2) head_dx_kernel(DxArgs p) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
   const int64_t count = *p.count, t_tiles = (count + C::BM - 1) / C::BM, f_tiles = p.split.f_tiles;
@@ -820,7 +830,7 @@ __global__ void __launch_bounds__(C::NT, 2) head_dx_kernel(DxArgs p) {
   f32x16_t acc[C::MI][C::NI];
   Side a = p.dz, b = p.w;
   a.move<size_of(TERMS)>(m0 * a.ld), b.move<size_of(TERMS)>(n0);
-  product<C, false, true, TERMS>(a, count - m0, b, p.dp - n0, k0, k1, lds, acc);
+  product<C, false, true, TERMS, 16, GW>(a, count - m0, b, p.k - n0, k0, k1, lds, acc);
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int wm = wid / C::WN, wn = wid % C::WN;
   float* out = p.out + split * count * p.dp;
@@ -1034,8 +1044,9 @@ struct Shape {
 struct Plan {
   bool f32, few, copy_w;
   bool full;                 // fp32 operands as they are: a few rows, bound by W's memory
+  bool by4;                  // W's rows as they are, loaded by 4 bytes
   int64_t row_bytes, dz_bytes;   // of the operands' elements, all parts, and of dz's
-  int64_t dp, cols, pieces;  // cols: vocabulary entries of a piece
+  int64_t dp, k, cols, pieces;   // k: features of W's rows as the products take them; cols: vocabulary entries of a piece
   int64_t tiles_all;         // vocabulary tiles of all pieces of the forward pass
   int64_t chunks, blocks;
   Size dx_size;
@@ -1113,13 +1124,18 @@ Shape dw_shape(const gs_head& h, const Plan& p, int64_t n) {
 }
 
 // The plan of a call.
-Plan plan_of(const gs_head& h, bool w_aligned) {
+Plan plan_of(const gs_head& h, int w_align) {
   Plan p{};
   p.f32 = h.dtype == GS_DTYPE_F32;
   p.few = h.N <= FEW_ROWS;
   p.full = p.f32 && p.few;
   p.dp = round_up(h.d, 8);
-  p.copy_w = (p.f32 && !p.full) || h.d % 8 != 0 || !w_aligned;
+  // A few rows are bound by W's memory: rows of it at multiples of 4 bytes are loaded by 4, without a copy.
+  const int64_t row = h.d * static_cast<int64_t>(elem_size(h.dtype));
+  const bool whole = h.d % 8 == 0 && w_align >= 16;
+  p.by4 = p.few && !whole && row % 4 == 0 && w_align >= 4;
+  p.copy_w = !p.by4 && ((p.f32 && !p.full) || !whole);
+  p.k = p.by4 ? h.d : p.dp;
   p.row_bytes = p.full ? 4 : p.f32 ? 6 : 2;
   p.dz_bytes = p.full ? 4 : 2 * (p.few ? dz_parts<Few>(p.f32) : dz_parts<Wide>(p.f32));
   const int64_t all = cdiv(h.V, 256);
@@ -1176,7 +1192,8 @@ Buffers carve(S& s, const gs_head& h, const Plan& p, bool grad) {
   return b;
 }
 
-bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+int align_of(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 ? 16 : reinterpret_cast<uintptr_t>(p) % 4 == 0 ? 4 : 1; }
+bool aligned16(const void* p) { return align_of(p) == 16; }
 
 unsigned grid_of(int64_t n) { return static_cast<unsigned>(n); }
 
@@ -1216,35 +1233,39 @@ Side weight_side(const gs_head& h, const Plan& p, const Buffers& b, int64_t v0, 
   return side_of(b.wc, p.dp, n * p.dp);
 }
 
-template <class C, int MODE>
+template <class C, int MODE, int GW = 16>
 void launch_logits_as(LogitsArgs& a, bool f32, hipStream_t s) {
   a.v_tiles = cdiv(a.V, C::BM);
   const dim3 grid(grid_of(a.v_tiles * cdiv(a.N, C::BN)));
+  constexpr int F32 = C::BN == Few::BN ? FULL : SIX;
   if (f32)
-    hipLaunchKernelGGL((head_logits_kernel<C, C::BN == Few::BN ? FULL : SIX, MODE>), grid, dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((head_logits_kernel<C, F32, MODE, GW>), grid, dim3(C::NT), 0, s, a);
   else
-    hipLaunchKernelGGL((head_logits_kernel<C, ONE, MODE>), grid, dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((head_logits_kernel<C, ONE, MODE, GW>), grid, dim3(C::NT), 0, s, a);
 }
 template <int MODE>
-void launch_logits(LogitsArgs& a, Size size, bool f32, hipStream_t s) {
-  if (size == WIDE) launch_logits_as<Wide, MODE>(a, f32, s);
-  if (size == MID) launch_logits_as<Mid, MODE>(a, f32, s);
-  if (size == SMALL) launch_logits_as<Small, MODE>(a, f32, s);
-  if (size == FEW) launch_logits_as<Few, MODE>(a, f32, s);
+void launch_logits(LogitsArgs& a, Size size, const Plan& p, hipStream_t s) {
+  if (size == WIDE) launch_logits_as<Wide, MODE>(a, p.f32, s);
+  if (size == MID) launch_logits_as<Mid, MODE>(a, p.f32, s);
+  if (size == SMALL) launch_logits_as<Small, MODE>(a, p.f32, s);
+  if (size == FEW && !p.by4) launch_logits_as<Few, MODE>(a, p.f32, s);
+  if (size == FEW && p.by4) launch_logits_as<Few, MODE, 4>(a, p.f32, s);
 }
-template <class C, int TERMS>
+template <class C, int TERMS, int GW = 16>
 void launch_dx_as(DxArgs& a, bool f32, hipStream_t s) {
   const dim3 grid(grid_of(std::max(a.split.slots, a.split.f_tiles * cdiv(a.N, C::BM))));
+  constexpr int F32 = C::BM == FewT::BM ? FULL : SIX;
   if (f32)
-    hipLaunchKernelGGL((head_dx_kernel<C, C::BM == FewT::BM ? FULL : SIX>), grid, dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((head_dx_kernel<C, F32, GW>), grid, dim3(C::NT), 0, s, a);
   else
-    hipLaunchKernelGGL((head_dx_kernel<C, TERMS>), grid, dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((head_dx_kernel<C, TERMS, GW>), grid, dim3(C::NT), 0, s, a);
 }
-void launch_dx(DxArgs& a, Size size, bool f32, hipStream_t s) {
-  if (size == WIDE) launch_dx_as<Wide, ONE>(a, f32, s);
-  if (size == MID) launch_dx_as<Mid, ONE>(a, f32, s);
-  if (size == SMALL) launch_dx_as<Small, ONE>(a, f32, s);
-  if (size == FEW) launch_dx_as<FewT, TWO_A>(a, f32, s);
+void launch_dx(DxArgs& a, const Plan& p, hipStream_t s) {
+  if (p.dx_size == WIDE) launch_dx_as<Wide, ONE>(a, p.f32, s);
+  if (p.dx_size == MID) launch_dx_as<Mid, ONE>(a, p.f32, s);
+  if (p.dx_size == SMALL) launch_dx_as<Small, ONE>(a, p.f32, s);
+  if (p.dx_size == FEW && !p.by4) launch_dx_as<FewT, TWO_A>(a, p.f32, s);
+  if (p.dx_size == FEW && p.by4) launch_dx_as<FewT, TWO_A, 4>(a, p.f32, s);
 }
 template <class C, int TERMS>
 void launch_dw_as(DwArgs& a, bool f32, hipStream_t s) {
@@ -1282,7 +1303,7 @@ LogitsArgs logits_args(const gs_head& h, const Plan& p, const Buffers& b) {
   LogitsArgs a{};
   a.x = side_of(b.xc, p.dp, h.N * p.dp);
   a.count = b.count, a.label = b.label, a.rows = b.rows;
-  a.N = h.N, a.dp = p.dp;
+  a.N = h.N, a.k = p.k;
   return a;
 }
 
@@ -1294,7 +1315,7 @@ using namespace gs;
 extern "C" size_t gs_head_loss_workspace(const gs_head* h) {
   if (check_head(h, "gs_head_loss") != GS_OK) return 0;
   Sizer s;
-  carve(s, *h, plan_of(*h, aligned16(h->W)), false);
+  carve(s, *h, plan_of(*h, align_of(h->W)), false);
   return s.used + 256;
 }
 
@@ -1303,7 +1324,7 @@ extern "C" int gs_head_loss(const gs_head* h, float* out_loss, float* lse, void*
   if (const int rc = check_head(h, "gs_head_loss")) return rc;
   if (out_loss == nullptr || lse == nullptr)
     return fail(GS_ERR_INVALID, "gs_head_loss: no place for the loss");
-  const Plan p = plan_of(*h, aligned16(h->W));
+  const Plan p = plan_of(*h, align_of(h->W));
   if (!grids_fit(*h, p)) return fail(GS_ERR_UNSUPPORTED, "gs_head_loss: grid too large");
   Carver c(workspace, workspace_bytes);
   const Buffers b = carve(c, *h, p, false);
@@ -1317,7 +1338,7 @@ extern "C" int gs_head_loss(const gs_head* h, float* out_loss, float* lse, void*
   for (int64_t v0 = 0; v0 < h->V; v0 += p.cols) {
     a.v0 = v0, a.V = std::min(p.cols, h->V - v0);
     a.w = weight_side(*h, p, b, v0, a.V, s);
-    launch_logits<FORWARD>(a, logits_shape(*h, p, a.V).size, p.f32, s);
+    launch_logits<FORWARD>(a, logits_shape(*h, p, a.V).size, p, s);
     a.tile0 += a.v_tiles;
   }
   FinishArgs f{};
@@ -1340,7 +1361,7 @@ extern "C" int gs_head_loss(const gs_head* h, float* out_loss, float* lse, void*
 extern "C" size_t gs_head_grad_workspace(const gs_head* h) {
   if (check_head(h, "gs_head_grad") != GS_OK) return 0;
   Sizer s;
-  carve(s, *h, plan_of(*h, aligned16(h->W)), true);
+  carve(s, *h, plan_of(*h, align_of(h->W)), true);
   return s.used + 256;
 }
 
@@ -1348,7 +1369,7 @@ extern "C" int gs_head_grad(const gs_head* h, const float* lse, const float* ups
                             void* dw, void* workspace, size_t workspace_bytes, void* stream) {
   if (const int rc = check_head(h, "gs_head_grad")) return rc;
   if (lse == nullptr) return fail(GS_ERR_INVALID, "gs_head_grad: the forward pass's sums are missing");
-  const Plan p = plan_of(*h, aligned16(h->W));
+  const Plan p = plan_of(*h, align_of(h->W));
   if (!grids_fit(*h, p)) return fail(GS_ERR_UNSUPPORTED, "gs_head_grad: grid too large");
   Carver c(workspace, workspace_bytes);
   const Buffers b = carve(c, *h, p, true);
@@ -1366,13 +1387,13 @@ extern "C" int gs_head_grad(const gs_head* h, const float* lse, const float* ups
     a.v0 = v0, a.V = std::min(p.cols, h->V - v0);
     a.w = weight_side(*h, p, b, v0, a.V, s);
     a.vp = p.cols;
-    launch_logits<GRADIENT>(a, logits_shape(*h, p, a.V).size, p.f32, s);
+    launch_logits<GRADIENT>(a, logits_shape(*h, p, a.V).size, p, s);
     const Side dz = side_of(b.dz, p.cols, h->N * p.cols);
     if (dx != nullptr) {
       DxArgs x{};
-      x.dz = dz, x.w = a.w, x.count = b.count, x.N = h->N, x.V = a.V, x.dp = p.dp;
+      x.dz = dz, x.w = a.w, x.count = b.count, x.N = h->N, x.V = a.V, x.dp = p.dp, x.k = p.k;
       x.split = p.dx, x.out = b.dx, x.add = v0 > 0;
-      launch_dx(x, p.dx_size, p.f32, s);
+      launch_dx(x, p, s);
     }
     if (dw != nullptr) {
       const Shape shape = dw_shape(*h, p, a.V);
@@ -1405,16 +1426,15 @@ extern "C" int gs_head_grad(const gs_head* h, const float* lse, const float* ups
 }
 
 // A call for one piece of dz has a plan of its own: the piece is the vocabulary.
-static Plan piece_plan(const gs_head& h, int64_t n, bool w_aligned) {
+static Plan piece_plan(const gs_head& h, int64_t n, int w_align) {
   gs_head piece = h;
   piece.V = n;
-  Plan p = plan_of(piece, w_aligned);
+  Plan p = plan_of(piece, w_align);
   p.cols = round_up(n, 256);
   return p;
 }
-static bool piece_aligned(const gs_head& h, int64_t v0) {
-  return h.W != nullptr &&
-         aligned16(static_cast<const char*>(h.W) + v0 * h.d * static_cast<int64_t>(elem_size(h.dtype)));
+static int piece_align(const gs_head& h, int64_t v0) {
+  return align_of(static_cast<const char*>(h.W) + v0 * h.d * static_cast<int64_t>(elem_size(h.dtype)));
 }
 template <class S>
 static Buffers carve_piece(S& s, const gs_head& h, int64_t n, const Plan& p) {
@@ -1434,7 +1454,7 @@ static Buffers carve_piece(S& s, const gs_head& h, int64_t n, const Plan& p) {
 extern "C" size_t gs_head_logit_grad_workspace(const gs_head* h, int64_t v0, int64_t n) {
   if (check_head(h, "gs_head_logit_grad") != GS_OK || v0 < 0 || n <= 0 || n > h->V - v0) return 0;
   Sizer s;
-  carve_piece(s, *h, n, piece_plan(*h, n, piece_aligned(*h, v0)));
+  carve_piece(s, *h, n, piece_plan(*h, n, piece_align(*h, v0)));
   return s.used + 256;
 }
 
@@ -1445,7 +1465,7 @@ extern "C" int gs_head_logit_grad(const gs_head* h, const float* lse, const floa
   if (lse == nullptr || out == nullptr || !aligned16(out) || v0 < 0 || n <= 0 || n > h->V - v0 ||
       out_stride != round_up(n, 8))
     return fail(GS_ERR_INVALID, "gs_head_logit_grad: invalid arguments");
-  const Plan p = piece_plan(*h, n, piece_aligned(*h, v0));
+  const Plan p = piece_plan(*h, n, piece_align(*h, v0));
   if (!grids_fit(*h, p))
     return fail(GS_ERR_UNSUPPORTED, "gs_head_logit_grad: grid too large");
   Carver c(workspace, workspace_bytes);
@@ -1460,7 +1480,7 @@ extern "C" int gs_head_logit_grad(const gs_head* h, const float* lse, const floa
   a.mean = h->reduction == GS_REDUCE_MEAN;
   a.v0 = v0, a.V = n, a.vp = out_stride, a.out = out;
   a.w = weight_side(*h, p, b, v0, n, s);
-  launch_logits<ROWS>(a, logits_shape(*h, p, n).size, p.f32, s);
+  launch_logits<ROWS>(a, logits_shape(*h, p, n).size, p, s);
   hipLaunchKernelGGL(head_zero_rows_kernel, dim3(grid_of(cdiv(h->N, 4))), dim3(256), 0, s, b.at, h->N,
                      static_cast<uint4*>(out), out_stride * static_cast<int64_t>(elem_size(h->dtype)) / 16);
   return check_launch("gs_head_logit_grad");
