@@ -148,6 +148,29 @@ def test_head_strides_alignment_and_shapes(gpu, dtype):
     assert one.shape == ()
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("d", [2, 7, 12, 34, 68, 101])
+def test_head_operands_among_nan(gpu, dtype, d):
+    """What lies around the rows and the weight takes no part, however a row's length divides."""
+    V = 150
+    for N in (3, 32, 70):
+        x, w, labels = head_inputs(N, V, d, dtype, N + d, 0.3)
+        rows = torch.full((N + 2, d + 3), math.nan, dtype=dtype, device=gpu)[1:-1, 2:2 + d]
+        rows.copy_(x)
+        for off in (0, 2, 9):
+            flat = torch.full((V * d + 32,), math.nan, dtype=dtype, device=gpu)
+            wt = flat[off:off + V * d].view(V, d)
+            wt.copy_(w)
+            for reduction in ("mean", "none"):
+                got = []
+                for a, b in ((rows, wt), (x.to(gpu), w.to(gpu))):
+                    a, b = a.detach().requires_grad_(), b.detach().requires_grad_()
+                    loss = gs.head_cross_entropy(a, b, labels.to(gpu), reduction=reduction)
+                    got.append((loss, *torch.autograd.grad(loss, (a, b), torch.ones_like(loss))))
+                assert all(p.isfinite().all() and torch.equal(p, q) for p, q in zip(*got))
+    check_head(x, w, labels, "mean", gpu)
+
+
 def test_head_of_no_rows(gpu):
     w = randn((9, 8), 1).to(gpu).requires_grad_()
     x = torch.zeros(2, 0, 8, device=gpu, requires_grad=True)
