@@ -35,6 +35,7 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr int NT = 256, BLOCK = GS_ADAMW_BLOCK, VE = 8;
 constexpr int CHUNK = NT * VE;       // elements of a workgroup, eight to a thread
 constexpr int MOST = 64;             // tensors of a launch (3.8 KB of arguments)
+constexpr int64_t MOST_RUNS = 1 << 23;   // runs of a launch: 2^31 threads
 constexpr float TOP = 448.f;
 
 struct Tensors {
@@ -246,8 +247,8 @@ extern "C" int gs_adamw(const gs_adamw_tensor* tensors, int64_t count, int dtype
     if (t.n < 0 || (t.n > 0 && (t.p == nullptr || t.g == nullptr || t.m == nullptr || t.v == nullptr ||
                                 (state_bits == 8 && (t.m_scale == nullptr || t.v_scale == nullptr)))))
       return fail(GS_ERR_INVALID, "gs_adamw: invalid tensor");
-    if (t.n > (int64_t{1} << 42))
-      return fail(GS_ERR_UNSUPPORTED, "gs_adamw: a tensor of more than 2^42 elements");
+    if (t.n > MOST_RUNS * CHUNK)
+      return fail(GS_ERR_UNSUPPORTED, "gs_adamw: a tensor of more than 2^34 elements");
   }
   Factors f{};
   f.keep = static_cast<float>(1.0 - lr * weight_decay);
@@ -266,7 +267,7 @@ extern "C" int gs_adamw(const gs_adamw_tensor* tensors, int64_t count, int dtype
     for (; i < count && a.count < MOST; ++i) {
       if (tensors[i].n == 0) continue;
       const int64_t more = cdiv(tensors[i].n, CHUNK);
-      if (runs + more > INT32_MAX && a.count > 0) break;
+      if (runs + more > MOST_RUNS && a.count > 0) break;
       a.t[a.count] = tensors[i];
       a.first[a.count++] = static_cast<int32_t>(runs);
       runs += more;

@@ -1296,7 +1296,8 @@ void launch_dx_finish(const gs_head& h, const Plan& p, const Buffers& b, const f
 // Whether every grid of a call can be launched: shares are at most 2 * 512 where tiles are few.
 bool grids_fit(const gs_head& h, const Plan& p) {
   const int64_t t = cdiv(h.N, FEW_ROWS), v = cdiv(p.cols, 64), f = cdiv(p.dp, 64), most = INT32_MAX / 2048;
-  return t <= most / f && v <= most / f && cdiv(p.cols, 256) <= INT32_MAX / cdiv(h.N, 256);
+  return t <= most / f && v <= most / f && p.cols <= (1 << 25) &&
+         cdiv(p.cols, 256) <= INT32_MAX / cdiv(h.N, 256);
 }
 
 LogitsArgs logits_args(const gs_head& h, const Plan& p, const Buffers& b) {

@@ -328,8 +328,17 @@ template <class E, int VE, int PC, int LANES>
 void launch(const NormArgs& a, bool backward, int64_t groups, hipStream_t s) {
   constexpr int G = NT / LANES;
   if (!backward) {
-    hipLaunchKernelGGL((norm_forward_kernel<E, VE, PC, LANES>),
-                       dim3(static_cast<unsigned>(cdiv(a.rows, G))), dim3(NT), 0, s, a);
+    // at most 2^30 threads to a launch
+    constexpr int64_t MOST = int64_t{G} << 22;
+    for (int64_t at = 0; at < a.rows; at += MOST) {
+      NormArgs b = a;
+      const int64_t by = at * a.F;
+      b.rows = std::min(a.rows - at, MOST);
+      b.x = static_cast<const E*>(a.x) + by, b.y = static_cast<E*>(a.y) + by;
+      if (a.res != nullptr) b.res = static_cast<const E*>(a.res) + by, b.h = static_cast<E*>(a.h) + by;
+      hipLaunchKernelGGL((norm_forward_kernel<E, VE, PC, LANES>),
+                         dim3(static_cast<unsigned>(cdiv(b.rows, G))), dim3(NT), 0, s, b);
+    }
   } else {
     const size_t lds = a.dw != nullptr ? (NTB / LANES - 1) * a.F * sizeof(float) : 0;
     hipLaunchKernelGGL((norm_backward_kernel<E, VE, PC, LANES>),

@@ -45,7 +45,10 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
         try:
             _check(self.param_groups[-1])
-        except GhostHipError:
+            params = self.param_groups[-1]["params"]
+            if len(set(params)) < len(params):   # each would be written twice at once
+                raise GhostHipError("AdamW: a parameter is in its group twice")
+        except Exception:
             del self.param_groups[-1]
             raise
 
@@ -80,13 +83,22 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict) -> None:
+        """A state of this class, or one of ``torch.optim.AdamW`` for fp32 parameters (32 bits)."""
+        for group in state_dict["param_groups"]:
+            if group.get("amsgrad") or group.get("maximize"):
+                raise GhostHipError("AdamW: a state with amsgrad or maximize")
         super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            group.setdefault("state_bits", 32)
+            group.setdefault("seed", 0)
         # The averages keep their types: the base class casts them to their parameters'.
         given = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         mine = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
         for key, p in zip(given, mine):
             for name, value in state_dict["state"].get(key, {}).items():
-                if isinstance(value, torch.Tensor):
+                if name == "step":
+                    self.state[p][name] = int(value)
+                elif isinstance(value, torch.Tensor):
                     self.state[p][name] = value.detach().to(p.device, copy=True)
 
 

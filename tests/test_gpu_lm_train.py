@@ -360,6 +360,20 @@ def test_norm_rows_stay_apart(gpu):
         within(g[clean.to(gpu)], *want["dh"], "dx")
 
 
+def test_norm_of_more_rows_than_a_launch(gpu):
+    rows = (1 << 25) + 5
+    x = torch.randn(rows, 1, device=gpu, dtype=BF16)
+    res = torch.randn(rows, 1, device=gpu, dtype=BF16)
+    w = torch.full((1,), 1.5, device=gpu, dtype=BF16)
+    y, h = gs.add_rms_norm(x, res, w)
+    alone = gs.rms_norm(h, w)
+    assert torch.equal(h, x + res) and torch.equal(alone, y)
+    for at in (0, (1 << 25) - 500, rows - 1000):
+        part = slice(at, at + 1000)
+        some, _ = gs.add_rms_norm(x[part], res[part], w)
+        assert torch.equal(some, y[part])
+
+
 def test_norm_refusals(gpu):
     x, w = randn((4, 8), 1).to(gpu), torch.ones(8, device=gpu)
     for bad in (lambda: gs.rms_norm(x.half(), w.half()), lambda: gs.rms_norm(x, w[:4]),

@@ -4,6 +4,7 @@ side, and what the C entry points refuse."""
 import copy
 import ctypes
 import math
+import warnings
 
 import pytest
 import torch
@@ -355,6 +356,41 @@ def test_adamw_refuses(bad):
     assert len(opt.param_groups) == 1
 
 
+def test_adamw_refuses_a_parameter_twice():
+    p, q = (nn.Parameter(torch.zeros(2)) for _ in range(2))
+    opt = AdamW([q])
+    with pytest.raises(_native.GhostHipError, match="twice"), warnings.catch_warnings():
+        warnings.simplefilter("ignore")   # torch's own
+        AdamW([("a", p), ("b", p)])
+    for params in ([p, p], iter([p, p])):
+        with pytest.raises(_native.GhostHipError, match="twice"), warnings.catch_warnings():
+            warnings.simplefilter("ignore")
+            opt.add_param_group({"params": params})
+        assert len(opt.param_groups) == 1
+
+
+def test_adamw_goes_on_from_torchs_state(oracle_ops):
+    """Of fp32 parameters: the same next step, within an fp32 rounding of each of its seven operations."""
+    a, b = (nn.Parameter(randn((40, 7), 1)) for _ in range(2))
+    ta = torch.optim.AdamW([a], lr=0.02, betas=(0.8, 0.95), weight_decay=0.3)
+    for k in range(3):
+        a.grad = randn((40, 7), 5 + k)
+        ta.step()
+    ob = AdamW([b])
+    with torch.no_grad():
+        b.copy_(a)
+    ob.load_state_dict(copy.deepcopy(ta.state_dict()))
+    assert ob.state[b]["step"] == 3 and isinstance(ob.state[b]["step"], int)
+    a.grad = b.grad = randn((40, 7), 9)
+    ta.step()
+    ob.step()
+    assert (a - b).abs().max() <= 7 * 2 ** -24 * 4   # |p| and the steps of it below 4
+    for how in ("amsgrad", "maximize"):
+        other = torch.optim.AdamW([a], **{how: True})
+        with pytest.raises(_native.GhostHipError, match=how):
+            ob.load_state_dict(other.state_dict())
+
+
 def test_averages_in_8_bits_come_out_right_on_average(oracle_ops):
     """Steady noisy gradients: with b2 = 0.999 a nearest rounding would leave v where it started.
 
@@ -466,6 +502,7 @@ def test_adamw_entry_point_refuses():
     assert call(tensor=TensorStruct(P16, P16, P16, P16, None, P16, 8), bits=8) == -1
     assert call(tensor=TensorStruct(P16, P16, P16, P16, P16, P16, -1)) == -1
     assert call(tensor=TensorStruct(P16, P16, P16, P16, P16, P16, 2 ** 43)) == -5
+    assert call(tensor=TensorStruct(P16, P16, P16, P16, P16, P16, 2 ** 34 + 1)) == -5
     assert call(tensor=None, count=0) == 0
     assert call(tensor=TensorStruct(None, None, None, None, None, None, 0)) == 0
 
