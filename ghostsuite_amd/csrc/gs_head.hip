@@ -107,12 +107,14 @@ struct Tile {
   static constexpr int A_BYTES = BM * K * 2, STAGE = (BM + BN) * K * 2;
   static constexpr int LDS = NS * STAGE;
 };
+constexpr int FEW_K = 32;
 using Wide = Tile<2, 4, 4, 2, 2>;    // 256 x 256, eight waves of 128 x 64
 using Mid = Tile<2, 2, 2, 2, 2>;     // 128 x 128, four waves of 64 x 64, two workgroups to a unit
 using Small = Tile<2, 2, 1, 1, 4>;   // 64 x 64, four waves of 32 x 32
 using Few = Tile<4, 1, 1, 1, 4>;     // 128 x 32
 using FewT = Tile<1, 4, 1, 1, 4>;    // 32 x 128
-using FewW = Tile<4, 1, 2, 2, 2>;    // 256 x 64: whole rows of dW leave at a time
+using FewT2 = Tile<1, 4, 2, 1, 4>;   // 64 x 128
+using FewW = Tile<4, 1, 2, 2, 2, FEW_K>;   // 256 x 64: whole rows of dW leave at a time
 constexpr int FEW_ROWS = 32;
 
 // The bf16 parts that dz is held in between the products: three for fp32 (of a few rows fp32 itself); two
@@ -238,9 +240,9 @@ struct Fragments {
 
 // Which products a product is made of: the operands as they are; of dz in two parts on one side; of three
 // parts on both, of which six count, the small ones first; of fp32 operands as they are, on fp32 MFMAs.
-enum Terms { ONE = 1, TWO_A = 2, TWO_B = 3, SIX = 6, FULL = 7 };
+enum Terms { ONE = 1, TWO_B = 2, SIX = 6, FULL = 7 };
 constexpr int size_of(int terms) { return terms == FULL ? 4 : 2; }   // of an operand's element
-constexpr int terms_in(int terms) { return terms == TWO_B ? 2 : terms == FULL ? 1 : terms; }
+constexpr int terms_in(int terms) { return terms == FULL ? 1 : terms; }
 
 // acc = sum over the contraction [k0, k1) of A B^T.
 //
@@ -293,8 +295,6 @@ __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_
     if constexpr (TERMS == SIX) {   // (l h) (h l) (m m) (m h) (h m) (h h)
       pa += (term == 0 ? 2 : term == 2 || term == 3 ? 1 : 0) * a.part * ES;
       pb += (term == 1 ? 2 : term == 2 || term == 4 ? 1 : 0) * b.part * ES;
-    } else if constexpr (TERMS == TWO_A) {
-      pa += term == 0 ? a.part * ES : 0;
     } else if constexpr (TERMS == TWO_B) {
       pb += term == 0 ? b.part * ES : 0;
     }
@@ -814,7 +814,8 @@ struct DxArgs {
   const int32_t* count;
   int64_t N, V, dp, k;     // V: the piece's entries; k: W's features
   DxSplit split;
-  float* out;              // [splits][count][dp]
+  int64_t low;             // 0, or N: dz's rows from there on are its low part, two shares to a split
+  float* out;              // [shares][count][dp]
   int add;                 // to what is there
 };
 template <class C, int TERMS, int GW>
@@ -830,10 +831,10 @@ __global__ void __launch_bounds__(C::NT, 2) head_dx_kernel(DxArgs p) {
   f32x16_t acc[C::MI][C::NI];
   Side a = p.dz, b = p.w;
   a.move<size_of(TERMS)>(m0 * a.ld), b.move<size_of(TERMS)>(n0);
-  product<C, false, true, TERMS, 16, GW>(a, count - m0, b, p.k - n0, k0, k1, lds, acc);
+  product<C, false, true, TERMS, 16, GW>(a, p.low + count - m0, b, p.k - n0, k0, k1, lds, acc);
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int wm = wid / C::WN, wn = wid % C::WN;
-  float* out = p.out + split * count * p.dp;
+  float* out = p.out + (p.low > 0 ? 2 * split : split) * count * p.dp;
 #pragma unroll
   for (int j = 0; j < C::NI; ++j) {
     const int64_t f = n0 + (wn * C::NI + j) * 32 + (lane & 31);
@@ -841,9 +842,11 @@ __global__ void __launch_bounds__(C::NT, 2) head_dx_kernel(DxArgs p) {
     for (int i = 0; i < C::MI; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int64_t r = m0 + (wm * C::MI + i) * 32 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
+        int64_t r = m0 + (wm * C::MI + i) * 32 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
+        float* o = out;
+        if (p.low > 0 && r >= p.low) r -= p.low, o += count * p.dp;
         if (r < count && f < p.dp) {
-          float* o = out + r * p.dp + f;
+          o += r * p.dp + f;
           *o = p.add ? *o + acc[i][j][e] : acc[i][j][e];
         }
       }
@@ -854,6 +857,7 @@ __global__ void __launch_bounds__(C::NT, 2) head_dx_kernel(DxArgs p) {
 struct DxFinishArgs {
   const float* sums;
   DxSplit split;
+  int shares;              // of a split
   const int32_t *at, *count;
   int64_t N, d, dp, f_blocks;
   const float* up;
@@ -870,7 +874,7 @@ __global__ void __launch_bounds__(256) head_dx_finish_kernel(DxFinishArgs p) {
   const int64_t j = p.at[r], count = *p.count;
   float s = 0.f;
   if (j >= 0 && f < p.d) {
-    const int splits = static_cast<int>(p.split(count));
+    const int splits = static_cast<int>(p.split(count)) * p.shares;
 #pragma unroll 4
     for (int k = g; k < splits; k += 4) s += p.sums[(k * count + j) * p.dp + f];
   }
@@ -889,7 +893,7 @@ __global__ void __launch_bounds__(256) head_dx_rows_kernel(DxFinishArgs p) {
   const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (r >= p.N) return;
   const int64_t j = p.at[r];
-  const int splits = static_cast<int>(p.split(count));
+  const int splits = static_cast<int>(p.split(count)) * p.shares;
   E* dx = static_cast<E*>(p.dx);
   const bool vec = p.d % 8 == 0 && reinterpret_cast<uintptr_t>(dx) % 16 == 0;
   for (int64_t f = (threadIdx.x & 63) * 8; f < p.d; f += 64 * 8) {
@@ -1051,6 +1055,7 @@ struct Plan {
   int64_t chunks, blocks;
   Size dx_size;
   DxSplit dx;
+  int dx_shares;             // of a split: dz's parts in one product's rows
   int64_t dw_sums;           // fp32 elements that a split piece of dW needs
 };
 
@@ -1116,7 +1121,7 @@ int64_t dx_sums(const gs_head& h, const Plan& p) {
   int64_t most = h.N;
   for (int64_t n = p.dx.tile; n < h.N + p.dx.tile && p.dx(n) > 1; n += p.dx.tile)
     most = std::max(most, p.dx(n) * std::min(n, h.N));
-  return most * p.dp;
+  return most * p.dx_shares * p.dp;
 }
 Shape dw_shape(const gs_head& h, const Plan& p, int64_t n) {
   if (p.few) return Shape{FEW, 1, 64, 0};
@@ -1158,6 +1163,7 @@ Plan plan_of(const gs_head& h, int w_align) {
     const Shape w = dw_shape(h, p, n);
     if (w.splits > 1) p.dw_sums = std::max(p.dw_sums, w.splits * n * h.d);
   }
+  p.dx_shares = p.few && !p.f32 ? dz_parts<Few>(false) : 1;
   p.dx_size = dx_shape(h, p, std::min(p.cols, h.V), p.dx);
   p.chunks = h.N > CHUNK ? cdiv(h.N, CHUNK) : 0;
   p.blocks = cdiv(h.N, 64);
@@ -1252,20 +1258,26 @@ void launch_logits(LogitsArgs& a, Size size, const Plan& p, hipStream_t s) {
   if (size == FEW && p.by4) launch_logits_as<Few, MODE, 4>(a, p.f32, s);
 }
 template <class C, int TERMS, int GW = 16>
-void launch_dx_as(DxArgs& a, bool f32, hipStream_t s) {
+void launch_dx_as(DxArgs& a, hipStream_t s) {
   const dim3 grid(grid_of(std::max(a.split.slots, a.split.f_tiles * cdiv(a.N, C::BM))));
-  constexpr int F32 = C::BM == FewT::BM ? FULL : SIX;
+  hipLaunchKernelGGL((head_dx_kernel<C, TERMS, GW>), grid, dim3(C::NT), 0, s, a);
+}
+// A few rows: both parts of bf16's dz are one product's rows, so W is read once.  (As two terms of the
+// contraction: 24 us for eight rows of GPT-2's, the logits' product 15.)
+template <int GW>
+void launch_dx_few(DxArgs& a, bool f32, hipStream_t s) {
   if (f32)
-    hipLaunchKernelGGL((head_dx_kernel<C, F32, GW>), grid, dim3(C::NT), 0, s, a);
+    launch_dx_as<FewT, FULL, GW>(a, s);
+  else if (2 * a.N <= FewT::BM)
+    launch_dx_as<FewT, ONE, GW>(a, s);
   else
-    hipLaunchKernelGGL((head_dx_kernel<C, TERMS, GW>), grid, dim3(C::NT), 0, s, a);
+    launch_dx_as<FewT2, ONE, GW>(a, s);
 }
 void launch_dx(DxArgs& a, const Plan& p, hipStream_t s) {
-  if (p.dx_size == WIDE) launch_dx_as<Wide, ONE>(a, p.f32, s);
-  if (p.dx_size == MID) launch_dx_as<Mid, ONE>(a, p.f32, s);
-  if (p.dx_size == SMALL) launch_dx_as<Small, ONE>(a, p.f32, s);
-  if (p.dx_size == FEW && !p.by4) launch_dx_as<FewT, TWO_A>(a, p.f32, s);
-  if (p.dx_size == FEW && p.by4) launch_dx_as<FewT, TWO_A, 4>(a, p.f32, s);
+  if (p.dx_size == WIDE) p.f32 ? launch_dx_as<Wide, SIX>(a, s) : launch_dx_as<Wide, ONE>(a, s);
+  if (p.dx_size == MID) p.f32 ? launch_dx_as<Mid, SIX>(a, s) : launch_dx_as<Mid, ONE>(a, s);
+  if (p.dx_size == SMALL) p.f32 ? launch_dx_as<Small, SIX>(a, s) : launch_dx_as<Small, ONE>(a, s);
+  if (p.dx_size == FEW) p.by4 ? launch_dx_few<4>(a, p.f32, s) : launch_dx_few<16>(a, p.f32, s);
 }
 template <class C, int TERMS>
 void launch_dw_as(DwArgs& a, bool f32, hipStream_t s) {
@@ -1286,7 +1298,7 @@ void launch_dw(DwArgs& a, Size size, bool f32, hipStream_t s) {
 template <class E>
 void launch_dx_finish(const gs_head& h, const Plan& p, const Buffers& b, const float* up, int mean, void* dx,
                       hipStream_t s) {
-  const DxFinishArgs a{b.dx, p.dx, b.at, b.count, h.N, h.d, p.dp, cdiv(h.d, 64), up, mean, dx};
+  const DxFinishArgs a{b.dx, p.dx, p.dx_shares, b.at, b.count, h.N, h.d, p.dp, cdiv(h.d, 64), up, mean, dx};
   if (h.N > 4096)
     hipLaunchKernelGGL(head_dx_rows_kernel<E>, dim3(grid_of(cdiv(h.N, 4))), dim3(256), 0, s, a);
   else
@@ -1393,7 +1405,7 @@ extern "C" int gs_head_grad(const gs_head* h, const float* lse, const float* ups
     if (dx != nullptr) {
       DxArgs x{};
       x.dz = dz, x.w = a.w, x.count = b.count, x.N = h->N, x.V = a.V, x.dp = p.dp, x.k = p.k;
-      x.split = p.dx, x.out = b.dx, x.add = v0 > 0;
+      x.split = p.dx, x.low = p.dx_shares > 1 ? h->N : 0, x.out = b.dx, x.add = v0 > 0;
       launch_dx(x, p, s);
     }
     if (dw != nullptr) {
