@@ -389,7 +389,6 @@ __device__ __forceinline__ int64_t xcd_order(int64_t w, int64_t total) {
 // ------------------------------------------------------------------------------ rows that count
 
 constexpr int CHUNK = 1024;   // labels counted by one workgroup
-constexpr int GROUP = 16;     // rows copied by one workgroup
 
 struct RowsArgs {
   const void* X;
@@ -463,7 +462,9 @@ __device__ __forceinline__ void copy_row(const E* src, int64_t n, void* to, int6
   }
 }
 
-template <class E, bool SPLIT>
+// GROUP rows to a workgroup: a row to a wave while those are few (138 rows of 629 fp32 features by sixteens:
+// 13 us), more where each workgroup's own count of the labels before it would be most of the work.
+template <class E, bool SPLIT, int GROUP>
 __global__ void __launch_bounds__(256) head_rows_kernel(RowsArgs a) {
   using O = std::conditional_t<SPLIT, uint16_t, E>;
   __shared__ int red[4];
@@ -482,8 +483,11 @@ __global__ void __launch_bounds__(256) head_rows_kernel(RowsArgs a) {
   __syncthreads();
   int place = red[0] + red[1] + red[2] + red[3];
   const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int g = 0; g < GROUP && first + g < a.N; ++g) {
-    const int64_t r = first + g, y = a.labels[r];
+#pragma unroll
+  for (int g = 0; g < GROUP; ++g) {
+    const int64_t r = first + g;
+    if (r >= a.N) break;
+    const int64_t y = a.labels[r];
     const bool keep = y != a.ignore_index;
     if (g % 4 == wid) {
       if (lane == 0) {
@@ -1203,6 +1207,13 @@ bool aligned16(const void* p) { return align_of(p) == 16; }
 
 unsigned grid_of(int64_t n) { return static_cast<unsigned>(n); }
 
+template <class E, bool SPLIT>
+void launch_rows_of(const RowsArgs& a, hipStream_t s) {
+  if (a.N <= 8192)
+    hipLaunchKernelGGL((head_rows_kernel<E, SPLIT, 4>), dim3(grid_of(cdiv(a.N, 4))), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((head_rows_kernel<E, SPLIT, 16>), dim3(grid_of(cdiv(a.N, 16))), dim3(256), 0, s, a);
+}
 void launch_rows(const gs_head& h, const Plan& p, const Buffers& b, float* loss, hipStream_t s) {
   RowsArgs a{};
   a.X = h.X, a.x_stride = h.x_stride, a.labels = h.labels, a.ignore_index = h.ignore_index;
@@ -1212,13 +1223,12 @@ void launch_rows(const gs_head& h, const Plan& p, const Buffers& b, float* loss,
   a.loss = loss;
   if (p.chunks > 0)
     hipLaunchKernelGGL(head_count_kernel, dim3(grid_of(p.chunks)), dim3(256), 0, s, a, b.chunk);
-  const dim3 grid(grid_of(cdiv(h.N, GROUP)));
   if (p.full)
-    hipLaunchKernelGGL((head_rows_kernel<float, false>), grid, dim3(256), 0, s, a);
+    launch_rows_of<float, false>(a, s);
   else if (p.f32)
-    hipLaunchKernelGGL((head_rows_kernel<float, true>), grid, dim3(256), 0, s, a);
+    launch_rows_of<float, true>(a, s);
   else
-    hipLaunchKernelGGL((head_rows_kernel<uint16_t, false>), grid, dim3(256), 0, s, a);
+    launch_rows_of<uint16_t, false>(a, s);
 }
 
 // W's rows [v0, v0 + n) as the products take them.
