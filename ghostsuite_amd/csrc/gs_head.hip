@@ -105,7 +105,9 @@ struct Tile {
   static constexpr int NW = WM * WN, NT = 64 * NW;
   static constexpr int BM = WM * MI * 32, BN = WN * NI * 32;
   static constexpr int A_BYTES = BM * K * 2, STAGE = (BM + BN) * K * 2;
-  static constexpr int LDS = NS * STAGE;
+  // Two slots of equal sides are five halves: see product.
+  static constexpr bool HALVES = NS == 2 && BM == BN;
+  static constexpr int LDS = HALVES ? 5 * A_BYTES : NS * STAGE;
 };
 constexpr int FEW_K = 32;
 using Wide = Tile<2, 4, 4, 2, 2>;    // 256 x 256, eight waves of 128 x 64
@@ -282,44 +284,55 @@ __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_
       lds_addr(lds) + static_cast<unsigned>(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 1024u;
   const int nk = k1 > k0 ? static_cast<int>((k1 - k0 + KE - 1) / KE) : 0;
   const int total = nk * terms_in(TERMS);
-  // The next stage to load: its slot, its first elements, and how many stages its term has left.  Only
-  // these change from stage to stage, in scalar registers.
+  // The next stage of a side to load: its first elements, its term, and how many stages the term has left.
+  // Only these change from stage to stage, in scalar registers.
   const int last = static_cast<int>((k1 - k0) % KE);   // contraction of a term's last stage, 0: a whole one
+  struct Next {
+    const unsigned char* p;
+    int term, left;
+  };
+  Next na{nullptr, 0, nk}, nb{nullptr, 0, nk};
   const int64_t step_a = (AKR ? KE * a.ld : KE) * ES, step_b = (BKR ? KE * b.ld : KE) * ES;
-  const unsigned char* first_a = a.p + (AKR ? k0 * a.ld : k0) * ES;
-  const unsigned char* first_b = b.p + (BKR ? k0 * b.ld : k0) * ES;
-  int term = 0, left = nk;
-  const unsigned char *pa, *pb;
-  auto begin_term = [&] {
-    pa = first_a, pb = first_b;
-    if constexpr (TERMS == SIX) {   // (l h) (h l) (m m) (m h) (h m) (h h)
-      pa += (term == 0 ? 2 : term == 2 || term == 3 ? 1 : 0) * a.part * ES;
-      pb += (term == 1 ? 2 : term == 2 || term == 4 ? 1 : 0) * b.part * ES;
-    } else if constexpr (TERMS == TWO_B) {
-      pb += term == 0 ? b.part * ES : 0;
+  auto begin_a = [&] {   // SIX: (l h) (h l) (m m) (m h) (h m) (h h)
+    na.p = a.p + (AKR ? k0 * a.ld : k0) * ES;
+    if constexpr (TERMS == SIX)
+      na.p += (na.term == 0 ? 2 : na.term == 2 || na.term == 3 ? 1 : 0) * a.part * ES;
+  };
+  auto begin_b = [&] {
+    nb.p = b.p + (BKR ? k0 * b.ld : k0) * ES;
+    if constexpr (TERMS == SIX)
+      nb.p += (nb.term == 1 ? 2 : nb.term == 2 || nb.term == 4 ? 1 : 0) * b.part * ES;
+    else if constexpr (TERMS == TWO_B)
+      nb.p += nb.term == 0 ? b.part * ES : 0;
+  };
+  begin_a();
+  begin_b();
+  auto issue_a = [&](unsigned to) {
+    if (na.left > 1 || last == 0)
+      sa.issue(na.p, to);
+    else
+      sa.issue_cut(na.p, to, last);
+    na.p += step_a;
+    if (--na.left == 0) {
+      na.left = nk;
+      if constexpr (terms_in(TERMS) > 1) ++na.term, begin_a();
     }
   };
-  begin_term();
-  unsigned slot_in = lds0;
-  auto issue = [&] {
-    if (left > 1 || last == 0) {
-      sa.issue(pa, slot_in);
-      sb.issue(pb, slot_in + C::A_BYTES);
-    } else {
-      sa.issue_cut(pa, slot_in, last);
-      sb.issue_cut(pb, slot_in + C::A_BYTES, last);
-    }
-    slot_in = slot_in + C::STAGE == lds0 + C::LDS ? lds0 : slot_in + C::STAGE;
-    pa += step_a, pb += step_b;
-    if (--left == 0) {
-      left = nk;
-      if constexpr (terms_in(TERMS) > 1) ++term, begin_term();
+  auto issue_b = [&](unsigned to) {
+    if (nb.left > 1 || last == 0)
+      sb.issue(nb.p, to);
+    else
+      sb.issue_cut(nb.p, to, last);
+    nb.p += step_b;
+    if (--nb.left == 0) {
+      nb.left = nk;
+      if constexpr (terms_in(TERMS) > 1) ++nb.term, begin_b();
     }
   };
   f32x4_t af[2][C::MI], bf[2][C::NI];
-  auto load = [&](int buf, const unsigned char* stage, int ks) {
-    fb.load(stage + C::A_BYTES, ks, bf[buf]);   // the first MFMAs take all of B and one of A
-    fa.load(stage, ks, af[buf]);
+  auto load = [&](int buf, const unsigned char* la, const unsigned char* lb, int ks) {
+    fb.load(lb, ks, bf[buf]);   // the first MFMAs take all of B and one of A
+    fa.load(la, ks, af[buf]);
   };
   auto mma = [&](int buf) {
 #pragma unroll
@@ -340,7 +353,65 @@ __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_
   constexpr int KRD = ES == 4 ? 4 : 2;   // reads of a fragment whose contraction index is the row
   constexpr int RD = (AKR ? KRD : 1) * C::MI + (BKR ? KRD : 1) * C::NI;
   constexpr int M = C::MI * C::NI * (ES == 4 ? 4 : 1);
-  if (total > 0) {
+  // The k-steps of the stage whose sides are at la and lb; the next stage's are at ma and mb.  PENDING:
+  // loads that may be in flight when that one is read.  (Past the last stage the fragments are read and
+  // not used.)
+  auto steps = [&](const unsigned char* la, const unsigned char* lb, const unsigned char* ma,
+                   const unsigned char* mb, auto pending) {
+#pragma unroll
+    for (int ks = 0; ks + 1 < KS; ++ks) {
+      load((ks + 1) & 1, la, lb, ks + 1);
+      mma(ks & 1);
+      sched_kstep<RD, M>();
+    }
+    wait_lgkmcnt0();
+    wait_vmcnt<decltype(pending)::value>();
+    raw_barrier();
+    load(0, ma, mb, 0);
+    mma((KS - 1) & 1);
+    sched_kstep<RD, M>();
+  };
+  using None = std::integral_constant<int, 0>;
+  if constexpr (C::HALVES) {
+    // Five halves of a stage: A of stage s in half 2s mod 5, B in the next.  While stage s is read, B of
+    // stage s + 1 and A of s + 2 are loaded into the two that the stage before left, and only the former
+    // has to be there at the end.  (With two slots all of the next stage has three k-steps' time to
+    // arrive: 1.59 us a stage of 256 x 256 x 64.)
+    constexpr unsigned H = C::A_BYTES;
+    const auto two_on = [](unsigned at) { return at >= 3 * H ? at - 3 * H : at + 2 * H; };
+    const auto one_on = [](unsigned at) { return at == 4 * H ? 0 : at + H; };
+    if (total > 0) {
+      issue_a(lds0);
+      issue_b(lds0 + H);
+      if (total > 1) {
+        issue_a(lds0 + 2 * H);
+        wait_vmcnt<sa.Q>();
+      } else {
+        wait_vmcnt<0>();
+      }
+      raw_barrier();
+      load(0, lds, lds + H, 0);
+      unsigned at = 0;   // A of the stage that is read
+      auto run = [&](auto b_more, auto a_more, auto pending) {
+        const unsigned next = two_on(at);
+        if constexpr (decltype(b_more)::value) issue_b(lds0 + one_on(next));
+        if constexpr (decltype(a_more)::value) issue_a(lds0 + two_on(next));
+        steps(lds + at, lds + one_on(at), lds + next, lds + one_on(next), pending);
+        at = next;
+      };
+      using Half = std::integral_constant<int, sa.Q>;
+      int s = 0;
+      for (; s + 2 < total; ++s) run(std::true_type{}, std::true_type{}, Half{});
+      if (s + 1 < total) run(std::true_type{}, std::false_type{}, None{});
+      run(std::false_type{}, std::false_type{}, None{});
+    }
+  } else if (total > 0) {
+    unsigned slot_in = lds0;
+    auto issue = [&] {
+      issue_a(slot_in);
+      issue_b(slot_in + C::A_BYTES);
+      slot_in = slot_in + C::STAGE == lds0 + C::LDS ? lds0 : slot_in + C::STAGE;
+    };
 #pragma unroll
     for (int s = 0; s < C::NS - 1; ++s)
       if (s < total) issue();
@@ -349,29 +420,15 @@ __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_
     else
       wait_vmcnt<0>();
     raw_barrier();
-    load(0, lds, 0);
+    load(0, lds, lds + C::A_BYTES, 0);
     const unsigned char* stage = lds;
-    // A stage: MORE: another one is loaded meanwhile; PENDING: loads that may be in flight when the next
-    // one is read.  (Past the last stage the next slot's fragments are read and not used.)
     auto run = [&](auto more, auto pending) {
       const unsigned char* next = stage + C::STAGE == lds + C::LDS ? lds : stage + C::STAGE;
       if constexpr (decltype(more)::value) issue();   // into the slot before, which every wave has read
-#pragma unroll
-      for (int ks = 0; ks + 1 < KS; ++ks) {
-        load((ks + 1) & 1, stage, ks + 1);
-        mma(ks & 1);
-        sched_kstep<RD, M>();
-      }
-      wait_lgkmcnt0();
-      wait_vmcnt<decltype(pending)::value>();
-      raw_barrier();
-      load(0, next, 0);
-      mma((KS - 1) & 1);
-      sched_kstep<RD, M>();
+      steps(stage, stage + C::A_BYTES, next, next + C::A_BYTES, pending);
       stage = next;
     };
     using Steady = std::integral_constant<int, (C::NS - 2) * NQ>;
-    using None = std::integral_constant<int, 0>;
     int s = 0;
     for (; s + C::NS - 1 < total; ++s) run(std::true_type{}, Steady{});
     for (; s < total; ++s) run(std::false_type{}, None{});
