@@ -651,12 +651,6 @@ __global__ void __launch_bounds__(C::NT, 2) head_logits_kernel(LogitsArgs p) {
   const int wm = wid / C::WN, wn = wid % C::WN, half = lane >> 5;
   const int row0 = wm * C::MI * 32 + 4 * half;     // this lane's first row of the tile
   const bool ragged = m0 + C::BM > p.V;
-#pragma unroll
-  for (int j = 0; j < C::NI; ++j)
-#pragma unroll
-    for (int i = 0; i < C::MI; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] *= LOG2E;
   if (ragged) behind<C>(acc, static_cast<int>(p.V - m0) - row0, -INFINITY);
 
   if constexpr (MODE == FORWARD) {
@@ -670,12 +664,12 @@ __global__ void __launch_bounds__(C::NT, 2) head_logits_kernel(LogitsArgs p) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
       m = fmaxf(m, __shfl_xor(m, 32, 64));
-      const float ref = fmaxf(m, -3e38f);   // rows of -inf: exponentials of zero, no NaN
+      const float ref = fmaxf(m * LOG2E, -3e38f);   // rows of -inf: exponentials of zero, no NaN
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < C::MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(acc[i][j][e] - ref);
+        for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], LOG2E, -ref));
       s += __shfl_xor(s, 32, 64);
       if (half == 0) red[wm * C::BN + col] = make_float2(ref, s);
       const int64_t n = n0 + col;
@@ -686,7 +680,7 @@ __global__ void __launch_bounds__(C::NT, 2) head_logits_kernel(LogitsArgs p) {
         for (int i = 0; i < C::MI; ++i)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (mine && rel == 32 * i + 8 * (e / 4) + e % 4) p.label_z[n] = acc[i][j][e];
+            if (mine && rel == 32 * i + 8 * (e / 4) + e % 4) p.label_z[n] = acc[i][j][e] * LOG2E;
       }
     }
     __syncthreads();
@@ -718,7 +712,7 @@ __global__ void __launch_bounds__(C::NT, 2) head_logits_kernel(LogitsArgs p) {
 #pragma unroll
       for (int i = 0; i < C::MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = w * __builtin_amdgcn_exp2f(acc[i][j][e] - lse);
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = w * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], LOG2E, -lse));
       const int64_t rel = live ? y - p.v0 - m0 - row0 : -1;
       const bool mine = rel >= 0 && rel < C::MI * 32 && (rel & 4) == 0;
       if (__ballot(mine)) {
