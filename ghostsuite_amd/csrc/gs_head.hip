@@ -940,52 +940,50 @@ __global__ void __launch_bounds__(256) head_dx_finish_kernel(DxFinishArgs p) {
   static_cast<E*>(p.dx)[r * p.d + f] =
       from_f32<E>(j >= 0 ? s * gradient_scale(p.up, p.mean, count) : 0.f);
 }
-// The same of many rows and few splits: a wave to a row, 16 bytes and more a lane.
+// The same of many rows and few splits: a thread to four features, whichever row they are in.  (4096 rows
+// of 768 features in five splits 50 us by the kernel above.)
 template <class E>
 __global__ void __launch_bounds__(256) head_dx_rows_kernel(DxFinishArgs p) {
-  const int64_t count = *p.count;
-  const float scale = gradient_scale(p.up, p.mean, count);
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (r >= p.N) return;
-  const int64_t j = p.at[r];
-  const int splits = static_cast<int>(p.split(count)) * p.shares;
-  E* dx = static_cast<E*>(p.dx);
-  const bool vec = p.d % 8 == 0 && reinterpret_cast<uintptr_t>(dx) % 16 == 0;
-  for (int64_t f = (threadIdx.x & 63) * 8; f < p.d; f += 64 * 8) {
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    for (int k = 0; j >= 0 && k < splits; ++k) {   // rows of sums are whole eights
-      const float4* q = reinterpret_cast<const float4*>(p.sums + (k * count + j) * p.dp + f);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float4 u = q[h];
-        v[4 * h] += u.x, v[4 * h + 1] += u.y, v[4 * h + 2] += u.z, v[4 * h + 3] += u.w;
-      }
+  const int64_t fours = p.dp / 4, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= p.N * fours) return;
+  const int64_t r = i / fours, f = (i - r * fours) * 4;
+  const int64_t j = p.at[r], count = *p.count;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (j >= 0) {
+    const int splits = static_cast<int>(p.split(count)) * p.shares;
+    const float scale = gradient_scale(p.up, p.mean, count);
+    const float* sums = p.sums + j * p.dp + f;
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      const float4 u = *reinterpret_cast<const float4*>(sums + k * count * p.dp);
+      v[0] += u.x, v[1] += u.y, v[2] += u.z, v[3] += u.w;
     }
-    union { uint4 u[sizeof(E) / 2]; E e[8]; } o;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o.e[i] = from_f32<E>(j >= 0 ? v[i] * scale : 0.f);
-    E* out = dx + r * p.d + f;
-    if (vec) {
+    for (int q = 0; q < 4; ++q) v[q] *= scale;
+  }
+  union { uint2 u[sizeof(E) / 2]; E e[4]; } o;
 #pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(E) / 2); ++i) reinterpret_cast<uint4*>(out)[i] = o.u[i];
-    } else {
+  for (int q = 0; q < 4; ++q) o.e[q] = from_f32<E>(v[q]);
+  E* out = static_cast<E*>(p.dx) + r * p.d + f;
+  if (p.d % 4 == 0 && reinterpret_cast<uintptr_t>(p.dx) % 16 == 0) {
+    if (f >= p.d) return;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (f + i < p.d) out[i] = o.e[i];
-    }
+    for (int q = 0; q < static_cast<int>(sizeof(E) / 2); ++q) reinterpret_cast<uint2*>(out)[q] = o.u[q];
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (f + q < p.d) out[q] = o.e[q];
   }
 }
 
 struct DwArgs {
   Side dz, x;              // [count][vp], [count][dp]: the contraction is their rows
   const int32_t* count;
-  int64_t V, d, dp;        // V: the piece's entries
-  int64_t v_tiles, f_tiles, splits, kper;
+  int64_t V, d, dp, cols;  // V: the entries; cols: dz's columns from the first of them on
+  int64_t v_tiles, f_tiles, splits;
   const float* up;
   int mean;
-  void* out;               // the piece's rows of dW; or with several splits [splits][V][d] fp32 sums
+  void* out;               // their rows of dW; or with several splits [splits][V][d] fp32 sums
 };
 // Features on the A side, so that a lane holds fours of neighbours of an entry's row.  bf16 rows leave
 // through LDS, whole rows of the tile at a time (straight from the lanes, two bytes each: 83 us for the
@@ -997,11 +995,13 @@ __global__ void __launch_bounds__(C::NT, 2) head_dw_kernel(DwArgs p) {
   const int64_t i0 = xcd_order(blockIdx.x, tiles * p.splits), split = i0 / tiles;
   const int64_t r0 = i0 - split * tiles;
   const int64_t m0 = r0 % p.f_tiles * C::BM, n0 = r0 / p.f_tiles * C::BN;
-  const int64_t k0 = split * p.kper, k1 = k0 + p.kper < count ? k0 + p.kper : count;
+  // shares of the rows that count, not of those that came
+  const int64_t per = ((count + p.splits - 1) / p.splits + 63) / 64 * 64;
+  const int64_t k0 = split * per, k1 = k0 + per < count ? k0 + per : count;
   f32x16_t acc[C::MI][C::NI];
   Side a = p.x, b = p.dz;
   a.move<size_of(TERMS)>(m0), b.move<size_of(TERMS)>(n0);
-  product<C, true, true, TERMS>(a, p.dp - m0, b, p.dz.ld - n0, k0, k1, lds, acc);
+  product<C, true, true, TERMS>(a, p.dp - m0, b, p.cols - n0, k0, k1, lds, acc);
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int wm = wid / C::WN, wn = wid % C::WN, half = lane >> 5;
   const int64_t f0 = m0 + wm * C::MI * 32 + 4 * half;   // this lane's first feature
@@ -1096,8 +1096,9 @@ enum Size { WIDE, MID, SMALL, FEW };
 // How a product is made: its tiles, and how often its contraction is split.
 struct Shape {
   Size size;
-  int64_t splits, per;   // per: the contraction of a share
+  int64_t splits;
   int64_t slots;         // workgroups that the splits fill
+  double us;
 };
 
 struct Plan {
@@ -1115,15 +1116,15 @@ struct Plan {
 };
 
 // The tiles of an m x n product over k (in `terms` products of parts), by what they were measured to take:
-// a stage of 64 of the contraction 1.75 us with 256 x 256 tiles, one workgroup to a unit; 1.15 with 128 x
-// 128 and 0.5 with 64 x 64 tiles, two to a unit; 4 us to begin and end a tile.  Splits cost a pass over the
-// shares' sums at 2 TB/s.  (43 rows of 791 fp32 features, 3655 entries: 314 us in 256 x 256 tiles, of which
-// there are 15.)
+// a stage of 64 of the contraction 1.45 us with 256 x 256 tiles, one workgroup to a unit; 0.93 with 128 x
+// 128 and 0.36 with 64 x 64 tiles, two to a unit (fp32's parts, of which there is more to read, 1.8, 1.05
+// and 0.38); 8, 3 and 1.5 us to begin and end a tile.  Splits cost
+// writing and reading the shares' sums at 4 TB/s.  (43 rows of 791 fp32 features, 3655 entries: 314 us in
+// 256 x 256 tiles, of which there are 15.)
 Shape shape_of(int64_t m, int64_t n, int64_t k, int64_t terms, bool split) {
-  static const struct { Size size; int64_t b, slots; double stage; } T[] = {
-      {WIDE, 256, 256, 1.75}, {MID, 128, 512, 1.15}, {SMALL, 64, 512, 0.5}};
-  Shape best{WIDE, 1, round_up(k, 64), 256};
-  double least = 1e300;
+  static const struct { Size size; int64_t b, slots; double stage, parts, ends; } T[] = {
+      {WIDE, 256, 256, 1.45, 1.8, 8.0}, {MID, 128, 512, 0.93, 1.05, 3.0}, {SMALL, 64, 512, 0.36, 0.38, 1.5}};
+  Shape best{WIDE, 1, 256, 1e300};
   for (const auto& t : T) {
     const int64_t tiles = cdiv(m, t.b) * cdiv(n, t.b), stages = cdiv(k, 64);
     // shares that fill the units once or twice
@@ -1131,9 +1132,9 @@ Shape shape_of(int64_t m, int64_t n, int64_t k, int64_t terms, bool split) {
     for (int i = 0; i < (split ? 3 : 1); ++i) {
       const int64_t want = std::max<int64_t>(1, std::min(fill[i], cdiv(stages, 4)));
       const int64_t per = cdiv(stages, want), splits = cdiv(stages, per);
-      const double us = cdiv(tiles * splits, t.slots) * (per * terms * t.stage + 4.0) +
-                        (splits > 1 ? 4.0 + splits * m * n * 8 / 2e6 : 0.0);
-      if (us < least) least = us, best = Shape{t.size, splits, per * 64, i == 2 ? 2 * t.slots : t.slots};
+      const double us = cdiv(tiles * splits, t.slots) * (per * terms * (terms > 1 ? t.parts : t.stage) + t.ends) +
+                        (splits > 1 ? 4.0 + splits * m * n * 8 / 4e6 : 0.0);
+      if (us < best.us) best = Shape{t.size, splits, i == 2 ? 2 * t.slots : t.slots, us};
     }
   }
   return best;
@@ -1157,7 +1158,7 @@ int64_t rows_of(Size s) { return s == WIDE ? 256 : s == MID ? 128 : s == SMALL ?
 int64_t terms_of(const Plan& p) { return p.f32 ? 6 : 1; }
 
 Shape logits_shape(const gs_head& h, const Plan& p, int64_t n) {
-  if (p.few) return Shape{FEW, 1, 0, 0};
+  if (p.few) return Shape{FEW, 1, 0, 0.0};
   return shape_of(n, h.N, h.d, terms_of(p), false);
 }
 // dx of a piece of `most` entries.
@@ -1178,9 +1179,24 @@ int64_t dx_sums(const gs_head& h, const Plan& p) {
     most = std::max(most, p.dx(n) * std::min(n, h.N));
   return most * p.dx_shares * p.dp;
 }
-Shape dw_shape(const gs_head& h, const Plan& p, int64_t n) {
-  if (p.few) return Shape{FEW, 1, 64, 0};
-  return shape_of(n, h.d, h.N, terms_of(p), true);
+// dW of n entries of the vocabulary, in one product or in two: as many entries as fill whole rounds over
+// the compute units, and the rest, which is split over its rows.  (197 x 3 tiles of 8192 rows take three
+// rounds in one product, 606 us.)
+struct DwParts {
+  int64_t n[2];
+  Shape shape[2];
+};
+DwParts dw_parts(const gs_head& h, const Plan& p, int64_t n) {
+  if (p.few) return DwParts{{n, 0}, {Shape{FEW, 1, 0, 0.0}, {}}};
+  const auto shape = [&](int64_t n) { return shape_of(n, h.d, h.N, terms_of(p), true); };
+  const Shape all = shape(n);
+  const int64_t f = cdiv(h.d, 256), whole = cdiv(n, 256) * f / CUS * CUS / f * 256;
+  if (whole > 0 && whole < n) {
+    const Shape a = shape(whole), b = shape(n - whole);
+    // an eighth to gain, for the rows that count may be fewer
+    if (a.us + b.us < 0.875 * all.us) return DwParts{{whole, n - whole}, {a, b}};
+  }
+  return DwParts{{n, 0}, {all, {}}};
 }
 
 // The plan of a call.
@@ -1215,8 +1231,9 @@ Plan plan_of(const gs_head& h, int w_align) {
   for (int64_t v0 = 0; v0 < h.V; v0 += p.cols) {
     const int64_t n = std::min(p.cols, h.V - v0);
     p.tiles_all += cdiv(n, rows_of(logits_shape(h, p, n).size));
-    const Shape w = dw_shape(h, p, n);
-    if (w.splits > 1) p.dw_sums = std::max(p.dw_sums, w.splits * n * h.d);
+    const DwParts w = dw_parts(h, p, n);
+    for (int i = 0; i < 2; ++i)
+      if (w.shape[i].splits > 1) p.dw_sums = std::max(p.dw_sums, w.shape[i].splits * w.n[i] * h.d);
   }
   p.dx_shares = p.few && !p.f32 ? dz_parts<Few>(false) : 1;
   p.dx_size = dx_shape(h, p, std::min(p.cols, h.V), p.dx);
@@ -1356,12 +1373,32 @@ void launch_dw(DwArgs& a, Size size, bool f32, hipStream_t s) {
   if (size == FEW) launch_dw_as<FewW, TWO_B>(a, f32, s);
 }
 
+// dW of n entries from entry v of a piece on, to `out`.
+void launch_dw_part(const gs_head& h, const Plan& p, const Buffers& b, const LogitsArgs& a, int64_t n,
+                    const Shape& shape, int64_t v, const float* up, int mean, void* out, hipStream_t s) {
+  DwArgs w{};
+  w.dz = side_of(b.dz + v * (p.full ? 4 : 2), p.cols, h.N * p.cols);
+  w.cols = p.cols - v, w.x = a.x, w.count = b.count, w.V = n, w.d = h.d, w.dp = p.dp;
+  w.splits = shape.splits, w.up = up, w.mean = mean;
+  w.out = shape.splits > 1 ? b.dw : out;
+  launch_dw(w, shape.size, p.f32, s);
+  if (shape.splits == 1) return;
+  const int64_t all = n * h.d;
+  const dim3 grid(grid_of(cdiv(all, 256)));
+  if (p.f32)
+    hipLaunchKernelGGL(head_dw_finish_kernel<float>, grid, dim3(256), 0, s, b.dw, shape.splits, all, b.count,
+                       up, mean, static_cast<float*>(out));
+  else
+    hipLaunchKernelGGL(head_dw_finish_kernel<uint16_t>, grid, dim3(256), 0, s, b.dw, shape.splits, all,
+                       b.count, up, mean, static_cast<uint16_t*>(out));
+}
+
 template <class E>
 void launch_dx_finish(const gs_head& h, const Plan& p, const Buffers& b, const float* up, int mean, void* dx,
                       hipStream_t s) {
   const DxFinishArgs a{b.dx, p.dx, p.dx_shares, b.at, b.count, h.N, h.d, p.dp, cdiv(h.d, 64), up, mean, dx};
-  if (h.N > 4096)
-    hipLaunchKernelGGL(head_dx_rows_kernel<E>, dim3(grid_of(cdiv(h.N, 4))), dim3(256), 0, s, a);
+  if (h.N >= 1024)
+    hipLaunchKernelGGL(head_dx_rows_kernel<E>, dim3(grid_of(cdiv(h.N * (p.dp / 4), 256))), dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL(head_dx_finish_kernel<E>, dim3(grid_of(h.N * a.f_blocks)), dim3(256), 0, s, a);
 }
@@ -1470,24 +1507,11 @@ extern "C" int gs_head_grad(const gs_head* h, const float* lse, const float* ups
       launch_dx(x, p, s);
     }
     if (dw != nullptr) {
-      const Shape shape = dw_shape(*h, p, a.V);
-      const int64_t splits = shape.splits;
-      DwArgs w{};
-      w.dz = dz, w.x = a.x, w.count = b.count, w.V = a.V, w.d = h->d, w.dp = p.dp;
-      w.splits = splits, w.kper = shape.per, w.up = up, w.mean = mean;
-      void* out = static_cast<char*>(dw) + v0 * h->d * static_cast<int64_t>(elem_size(h->dtype));
-      w.out = splits > 1 ? b.dw : out;
-      launch_dw(w, shape.size, p.f32, s);
-      if (splits > 1) {
-        const int64_t n = a.V * h->d;
-        const dim3 grid(grid_of(cdiv(n, 256)));
-        if (p.f32)
-          hipLaunchKernelGGL(head_dw_finish_kernel<float>, grid, dim3(256), 0, s, b.dw, splits, n,
-                             b.count, up, mean, static_cast<float*>(out));
-        else
-          hipLaunchKernelGGL(head_dw_finish_kernel<uint16_t>, grid, dim3(256), 0, s, b.dw, splits, n,
-                             b.count, up, mean, static_cast<uint16_t*>(out));
-      }
+      const DwParts parts = dw_parts(*h, p, a.V);
+      int64_t v = 0;   // the part's first entry, in the piece
+      for (int i = 0; i < 2 && parts.n[i] > 0; v += parts.n[i++])
+        launch_dw_part(*h, p, b, a, parts.n[i], parts.shape[i], v, up, mean,
+                       static_cast<char*>(dw) + (v0 + v) * h->d * static_cast<int64_t>(elem_size(h->dtype)), s);
     }
   }
   if (dx != nullptr) {
