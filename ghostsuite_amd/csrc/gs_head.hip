@@ -1117,13 +1117,13 @@ struct Plan {
 
 // The tiles of an m x n product over k (in `terms` products of parts), by what they were measured to take:
 // a stage of 64 of the contraction 1.45 us with 256 x 256 tiles, one workgroup to a unit; 0.93 with 128 x
-// 128 and 0.36 with 64 x 64 tiles, two to a unit (fp32's parts, of which there is more to read, 1.8, 1.05
-// and 0.38); 8, 3 and 1.5 us to begin and end a tile.  Splits cost
+// 128 and 0.36 with 64 x 64 tiles, two to a unit (fp32's parts, of which there is more to read, 1.85,
+// 1.15 and 0.5); 8, 3 and 1.5 us to begin and end a tile.  Splits cost
 // writing and reading the shares' sums at 4 TB/s.  (43 rows of 791 fp32 features, 3655 entries: 314 us in
 // 256 x 256 tiles, of which there are 15.)
 Shape shape_of(int64_t m, int64_t n, int64_t k, int64_t terms, bool split) {
   static const struct { Size size; int64_t b, slots; double stage, parts, ends; } T[] = {
-      {WIDE, 256, 256, 1.45, 1.8, 8.0}, {MID, 128, 512, 0.93, 1.05, 3.0}, {SMALL, 64, 512, 0.36, 0.38, 1.5}};
+      {WIDE, 256, 256, 1.45, 1.85, 8.0}, {MID, 128, 512, 0.93, 1.15, 3.0}, {SMALL, 64, 512, 0.36, 0.5, 1.5}};
   Shape best{WIDE, 1, 256, 1e300};
   for (const auto& t : T) {
     const int64_t tiles = cdiv(m, t.b) * cdiv(n, t.b), stages = cdiv(k, 64);
@@ -1193,8 +1193,8 @@ DwParts dw_parts(const gs_head& h, const Plan& p, int64_t n) {
   const int64_t f = cdiv(h.d, 256), whole = cdiv(n, 256) * f / CUS * CUS / f * 256;
   if (whole > 0 && whole < n) {
     const Shape a = shape(whole), b = shape(n - whole);
-    // an eighth to gain, for the rows that count may be fewer
-    if (a.us + b.us < 0.875 * all.us) return DwParts{{whole, n - whole}, {a, b}};
+    // a seventh to gain: where half of the rows count, a tenth has been lost
+    if (a.us + b.us < 0.85 * all.us) return DwParts{{whole, n - whole}, {a, b}};
   }
   return DwParts{{n, 0}, {all, {}}};
 }
