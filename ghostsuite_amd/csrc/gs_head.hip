@@ -10,6 +10,13 @@
 // into dx and into the piece's rows of dW.  Four products where keeping the logits takes three,
 // for a workspace of one piece of dz.
 //
+// Bound by the matrix cores but for a few rows, which are bound by W's memory.  18432 of 20480 rows of
+// GPT-2's output projection (768 features, 50257 entries, bf16) 5.25 to 5.6 ms for 5.69 TFLOP, a stage of
+// 256 x 256 x 64 in 1.48 us on every compute unit (1.45 PFLOP/s); the rest is the tiles' ends, 6 us with
+// their exponentials and 11 with those and dz's writing, and the units that the last round of tiles leaves
+// (dx's 72 x 3).  Matrix cores busy 56% of the forward product's cycles, 49% of dz's, 49% of dx's, 69% of
+// dW's, at 1.7 to 1.9 GHz.  Eight rows 90 us: W read in 14 to 15 us three times, dW written in 19.
+//
 // Rows that do not count (label ignore_index) take no part in any product: the rows that do are
 // listed first, in order, and copied next to each other (with rows of a multiple of 8 features,
 // which the 16-byte loads need).  Their number stays on the device; tiles past it end at once.
@@ -19,8 +26,8 @@
 // same kernels over six times the contraction, which at the bf16 matrix rate is still faster than fp32
 // matrix instructions.  A few rows are bound by W's memory, and take it as it is, on those.
 //
-// Tiles: BM x BN outputs, 64 of the contraction a stage, staged through LDS by wave-level
-// 16-byte DMA, MFMA 32x32x16 (fp32 accumulators).  A side whose contraction index is contiguous
+// Tiles: BM x BN outputs, 64 of the contraction a stage, staged through LDS by wave-level DMA
+// of 16 bytes a lane (4 where a weight's rows are off 16-byte boundaries), MFMA 32x32x16 (fp32 accumulators).  A side whose contraction index is contiguous
 // in memory (KC) is read from LDS as 16-byte fragments, one whose contraction index is the row
 // (KR) through the transpose read.  Result layout of the MFMA: lane l, element e is row
 // 8 (e / 4) + 4 (l / 32) + e % 4 of the A side, column l % 32 of the B side.
