@@ -444,9 +444,10 @@ __device__ __forceinline__ void product(Side a, int64_t a_extent, Side b, int64_
 }
 
 // Workgroup w of `total` to its place in an order of which each XCD takes a contiguous run
-// (workgroup w runs on XCD w mod 8).
-__device__ __forceinline__ int64_t xcd_order(int64_t w, int64_t total) {
-  const int64_t q = total / 8, r = total % 8, x = w % 8;
+// (workgroup w runs on XCD w mod 8).  Places are 32-bit, as grids are: divisions of 64 bits cost the kernels
+// of eight rows up to half a microsecond each.
+__device__ __forceinline__ uint32_t xcd_order(uint32_t w, uint32_t total) {
+  const uint32_t q = total / 8, r = total % 8, x = w % 8;
   return x * q + (x < r ? x : r) + w / 8;
 }
 
@@ -618,11 +619,12 @@ __device__ __forceinline__ float gradient_scale(const float* up, int mean, int64
 // L2 while the vocabulary goes by.
 __device__ __forceinline__ bool logits_item(int64_t v_tiles, int64_t t_tiles, int64_t& vt,
                                             int64_t& tt) {
-  const int64_t total = v_tiles * t_tiles, w = blockIdx.x;
-  if (w >= total) return false;
-  const int64_t i = xcd_order(w, total), per = 8 * v_tiles, g = i / per, r = i - g * per;
-  const int64_t size = t_tiles - 8 * g < 8 ? t_tiles - 8 * g : 8;
-  tt = 8 * g + r % size, vt = r / size;
+  const uint32_t vts = static_cast<uint32_t>(v_tiles), tts = static_cast<uint32_t>(t_tiles);
+  const uint32_t total = vts * tts;
+  if (blockIdx.x >= total) return false;
+  const uint32_t i = xcd_order(blockIdx.x, total), per = 8 * vts, g = i / per, r = i - g * per;
+  const uint32_t size = tts - 8 * g < 8 ? tts - 8 * g : 8, v = r / size;
+  tt = 8 * g + (r - v * size), vt = v;
   return true;
 }
 
@@ -866,8 +868,9 @@ __global__ void __launch_bounds__(256) head_zero_rows_kernel(const int32_t* at, 
 struct DxSplit {
   int64_t tile, f_tiles, slots, most;   // tile: rows of one
   __host__ __device__ int64_t operator()(int64_t count) const {
-    const int64_t tiles = f_tiles * ((count + tile - 1) / tile);
-    const int64_t s = tiles > 0 ? slots / tiles : 1;
+    const uint32_t b = static_cast<uint32_t>(tile);
+    const uint32_t tiles = static_cast<uint32_t>(f_tiles) * ((static_cast<uint32_t>(count) + b - 1) / b);
+    const int64_t s = tiles > 0 ? static_cast<uint32_t>(slots) / tiles : 1;
     return s < 1 ? 1 : s < most ? s : most;
   }
 };
@@ -884,11 +887,12 @@ template <class C, int TERMS, int GW>
 __global__ void __launch_bounds__(C::NT, 2) head_dx_kernel(DxArgs p) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
   const int64_t count = *p.count, t_tiles = (count + C::BM - 1) / C::BM, f_tiles = p.split.f_tiles;
-  const int64_t tiles = f_tiles * t_tiles, splits = p.split(count), total = tiles * splits;
+  const uint32_t fs = static_cast<uint32_t>(f_tiles), tiles = fs * static_cast<uint32_t>(t_tiles);
+  const uint32_t splits = static_cast<uint32_t>(p.split(count)), total = tiles * splits;
   if (blockIdx.x >= total) return;
-  const int64_t i0 = xcd_order(blockIdx.x, total), split = i0 / tiles, r0 = i0 - split * tiles;
-  const int64_t m0 = r0 / f_tiles * C::BM, n0 = r0 % f_tiles * C::BN;
-  const int64_t per = ((p.V + splits - 1) / splits + 63) / 64 * 64;
+  const uint32_t i0 = xcd_order(blockIdx.x, total), part = i0 / tiles, r0 = i0 - part * tiles, tr = r0 / fs;
+  const int64_t split = part, m0 = static_cast<int64_t>(tr) * C::BM, n0 = static_cast<int64_t>(r0 - tr * fs) * C::BN;
+  const int64_t per = ((static_cast<uint32_t>(p.V) + splits - 1) / splits + 63) / 64 * 64;
   const int64_t k0 = split * per, k1 = k0 + per < p.V ? k0 + per : p.V;
   f32x16_t acc[C::MI][C::NI];
   Side a = p.dz, b = p.w;
@@ -932,7 +936,8 @@ template <class E>
 __global__ void __launch_bounds__(256) head_dx_finish_kernel(DxFinishArgs p) {
   __shared__ float red[4][64];
   const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
-  const int64_t r = blockIdx.x / p.f_blocks, f = (blockIdx.x - r * p.f_blocks) * 64 + lane;
+  const int64_t r = blockIdx.x / static_cast<uint32_t>(p.f_blocks);
+  const int64_t f = (blockIdx.x - r * p.f_blocks) * 64 + lane;
   const int64_t j = p.at[r], count = *p.count;
   float s = 0.f;
   if (j >= 0 && f < p.d) {
@@ -953,7 +958,8 @@ template <class E>
 __global__ void __launch_bounds__(256) head_dx_rows_kernel(DxFinishArgs p) {
   const int64_t fours = p.dp / 4, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= p.N * fours) return;
-  const int64_t r = i / fours, f = (i - r * fours) * 4;
+  const int64_t r = i >> 32 ? i / fours : static_cast<uint32_t>(i) / static_cast<uint32_t>(fours);
+  const int64_t f = (i - r * fours) * 4;
   const int64_t j = p.at[r], count = *p.count;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
   if (j >= 0) {
@@ -998,12 +1004,14 @@ struct DwArgs {
 template <class C, int TERMS, class E>
 __global__ void __launch_bounds__(C::NT, 2) head_dw_kernel(DwArgs p) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[C::LDS];
-  const int64_t count = *p.count, tiles = p.v_tiles * p.f_tiles;
-  const int64_t i0 = xcd_order(blockIdx.x, tiles * p.splits), split = i0 / tiles;
-  const int64_t r0 = i0 - split * tiles;
-  const int64_t m0 = r0 % p.f_tiles * C::BM, n0 = r0 / p.f_tiles * C::BN;
+  const int64_t count = *p.count;
+  const uint32_t fs = static_cast<uint32_t>(p.f_tiles), tiles = static_cast<uint32_t>(p.v_tiles) * fs;
+  const uint32_t i0 = xcd_order(blockIdx.x, tiles * static_cast<uint32_t>(p.splits)), split = i0 / tiles;
+  const uint32_t r0 = i0 - split * tiles, tv = r0 / fs;
+  const int64_t m0 = static_cast<int64_t>(r0 - tv * fs) * C::BM, n0 = static_cast<int64_t>(tv) * C::BN;
   // shares of the rows that count, not of those that came
-  const int64_t per = ((count + p.splits - 1) / p.splits + 63) / 64 * 64;
+  const uint32_t shares = static_cast<uint32_t>(p.splits);
+  const int64_t per = ((static_cast<uint32_t>(count) + shares - 1) / shares + 63) / 64 * 64;
   const int64_t k0 = split * per, k1 = k0 + per < count ? k0 + per : count;
   f32x16_t acc[C::MI][C::NI];
   Side a = p.x, b = p.dz;

@@ -234,6 +234,25 @@ def test_head_of_many_rows_in_pieces(gpu):
         within(dw[v0:v0 + 1000], ref.cpu(), (ref.abs() * HALF[BF16] + (N + 64) * U * size).cpu(), "dw")
 
 
+@pytest.mark.parametrize("ignored", [0.0, 0.7])
+def test_head_weight_gradient_in_whole_rounds_and_shares(gpu, ignored):
+    """A few tiles of dW more than compute units: the rest is a product of its own, over shares of the rows
+    that count."""
+    N, V, d = 4096, 65536 + 264, 256
+    x, w, labels = head_inputs(N, V, d, BF16, 6, ignored)
+    xg, wg, yg = x.to(gpu).requires_grad_(), w.to(gpu).requires_grad_(), labels.to(gpu)
+    dw, = torch.autograd.grad(gs.head_cross_entropy(xg, wg, yg, reduction="none"), wg,
+                              torch.ones(N, device=gpu))
+    lse = torch.empty(N, device=gpu)
+    _native.ops().head_cross_entropy(xg.detach(), wg.detach(), yg, -100, "none", lse)
+    for v0 in (0, 32000, 65536 - 300, V - 300):
+        dz = _native.ops().head_logit_grad(xg.detach(), wg.detach(), yg, lse, torch.ones(N, device=gpu), v0,
+                                           300, -100, "none")[:, :300]
+        ref = dz.double().t() @ xg.detach().double()
+        size = dz.double().abs().t() @ xg.detach().double().abs()
+        within(dw[v0:v0 + 300], ref.cpu(), (ref.abs() * HALF[BF16] + (N + 64) * U * size).cpu(), "dw")
+
+
 def test_head_gradients_by_differences(gpu):
     x, w, labels = head_inputs(40, 60, 12, FP32, 8)
     x, w, labels = x.to(gpu).requires_grad_(), w.to(gpu).requires_grad_(), labels.to(gpu)
