@@ -196,6 +196,39 @@ def test_engine_head_is_a_linear_of_its_logits(oracle_ops):
                 assert_close(got[0][k][1], got[1][k][1], 1e-5, k)
 
 
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+@pytest.mark.parametrize("again", [False, True])
+def test_engine_head_with_weighted_losses_and_recomputation(oracle_ops, reduction, again):
+    """The rows' losses weighted outside the layer, the forward pass run again within the backward one:
+    still a Linear of its logits."""
+    from torch.utils.checkpoint import checkpoint
+    torch.manual_seed(2)
+    a = _Net()
+    a.head.reduction = reduction
+    b = copy.deepcopy(a)
+    ids, labels = torch.randint(0, 13, (5, 3)), torch.randint(0, 13, (5, 3))
+    labels[1, 1] = -100
+    weights = torch.rand(5, 3) + 0.5 if reduction == "none" else torch.tensor(0.3)
+
+    def theirs(net):
+        loss = nn.functional.cross_entropy(net(ids).flatten(0, 1), labels.flatten(), reduction=reduction)
+        return (loss * weights.reshape(loss.shape)).sum()
+
+    def ours(net):
+        loss = checkpoint(net, ids, labels, use_reentrant=False) if again else net(ids, labels)
+        return (loss * weights).sum()
+    got = []
+    for net, loss in ((a, ours), (b, theirs)):
+        eng = GradDotProdEngine(net, val_batch_size=2, use_dummy_bias=False, precision="fp32")
+        eng.attach(torch.optim.SGD(net.parameters(), lr=0.0))
+        loss(net).backward()
+        got.append({k: (p.grad_dot_prod.clone(), p.train_grad.clone()) for k, p in net.named_parameters()})
+        eng.detach()
+    for k in got[0]:
+        assert_close(got[0][k][0], got[1][k][0], 1e-5, k)
+        assert_close(got[0][k][1], got[1][k][1], 1e-5, k)
+
+
 def test_engine_with_an_unused_norm_output(oracle_ops):
     """A norm of whose outputs only the stream is used has dots and a gradient of zero."""
     net = nn.ModuleDict({"n": gs.RMSNorm(4)})
