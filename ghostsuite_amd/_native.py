@@ -849,8 +849,8 @@ class HipOps:
     def head_cross_entropy(self, x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
                            ignore_index: int, reduction: str,
                            lse: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """gs_head_loss; its gradient gs_head_grad.  lse ([rows] fp32): the forward pass writes each
-        counted row's log2 of the sum of exponentials there, for head_logit_grad."""
+        """gs_head_loss; its gradient gs_head_grad.  lse ([rows, 2] fp32): the forward pass writes each
+        counted row's largest logit and sum of exponentials there, for head_logit_grad."""
         return _lm().head_cross_entropy(x, weight, labels, ignore_index, REDUCTIONS[reduction], lse)
 
     def head_logit_grad(self, x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,

@@ -594,9 +594,9 @@ struct LogitsArgs {
   // forward: per vocabulary tile (of all pieces) and row
   float2* part;              // [tiles][N]: maximum of z log2(e), sum of 2^(z log2(e) - maximum)
   int64_t tile0;
-  float* label_z;            // [N]: the label's z log2(e)
+  float* label_z;            // [N]: the label's z
   // backward
-  const float* lse;          // [N]: log2 of the row's sum of exponentials
+  const float* lse;          // [N][2]: as FinishArgs::lse
   const float* up;           // null, or the rows' upstream gradients
   const int32_t* rows;
   uint16_t* dz;              // [parts][N][vp]
@@ -689,7 +689,7 @@ __global__ void __launch_bounds__(C::NT, 2) head_logits_kernel(LogitsArgs p) {
         for (int i = 0; i < C::MI; ++i)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (mine && rel == 32 * i + 8 * (e / 4) + e % 4) p.label_z[n] = acc[i][j][e] * LOG2E;
+            if (mine && rel == 32 * i + 8 * (e / 4) + e % 4) p.label_z[n] = acc[i][j][e];
       }
     }
     __syncthreads();
@@ -715,13 +715,14 @@ __global__ void __launch_bounds__(C::NT, 2) head_logits_kernel(LogitsArgs p) {
       const int64_t n = n0 + (wn * C::NI + j) * 32 + (lane & 31);
       const bool live = n < count;
       const int32_t y = live ? p.label[n] : 0;
-      const float lse = live && y >= 0 ? p.lse[n] : NAN;
+      const float ref = live && y >= 0 ? p.lse[2 * n] : NAN;
       float w = live && p.up != nullptr ? p.up[p.rows[n]] : 1.f;
       if constexpr (MODE == ROWS) w *= gradient_scale(p.up_all, p.mean, count);
+      const float share = live ? w / p.lse[2 * n + 1] : 0.f;
 #pragma unroll
       for (int i = 0; i < C::MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = w * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], LOG2E, -lse));
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = share * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], LOG2E, -ref));
       const int64_t rel = live ? y - p.v0 - m0 - row0 : -1;
       const bool mine = rel >= 0 && rel < C::MI * 32 && (rel & 4) == 0;
       if (__ballot(mine)) {
@@ -798,6 +799,9 @@ struct FinishArgs {
   const int32_t* rows;
   const int32_t* label;
   int64_t N, tiles;
+  // [N][2]: the row's reference, its largest z log2(e), and its sum of 2^(z log2(e) - reference).  Apart,
+  // because in one number they would cost a row whose label has most of the mass its digits: the loss and
+  // p - 1 would be what is left of numbers of the logits' size.
   float* lse;
   float* loss;       // null, or [N]
   float* sums;       // null, or [blocks]
@@ -832,9 +836,8 @@ __global__ void __launch_bounds__(1024) head_finish_kernel(FinishArgs p) {
   float loss = 0.f;
   if (g == 0 && n < count) {
     t = red[0][r];
-    const float lse = t.x + __log2f(t.y);
-    loss = p.label[n] >= 0 ? LN2 * (lse - p.label_z[n]) : NAN;
-    p.lse[n] = lse;
+    loss = p.label[n] >= 0 ? LN2 * (log2f(t.y) - fmaf(p.label_z[n], LOG2E, -t.x)) : NAN;
+    p.lse[2 * n] = t.x, p.lse[2 * n + 1] = t.y;
     if (p.loss != nullptr) p.loss[p.rows[n]] = loss;
   }
   loss = wave_sum(loss);

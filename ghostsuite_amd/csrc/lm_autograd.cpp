@@ -679,7 +679,7 @@ Tensor distillation_loss(const Tensor& logits, const Tensor& ids, const Tensor& 
 struct HeadHow {
   int64_t ignore_index;
   int reduction;
-  Tensor lse;   // each row's log2 of the sum of exponentials, which the forward pass writes
+  Tensor lse;   // each row's largest logit and sum of exponentials, which the forward pass writes
 };
 
 // The arguments of a gs_head_* call.
@@ -718,10 +718,10 @@ Tensor head_loss(const Tensor& x, const Tensor& w, const Tensor& labels, HeadHow
   const at::IntArrayRef shape = how.reduction == GS_REDUCE_NONE ? labels.sizes() : at::IntArrayRef();
   if (lse.defined())
     require(lse.is_cuda() && lse.device() == c.dev && lse.scalar_type() == at::kFloat &&
-                lse.is_contiguous() && lse.numel() == c.h.N && in_memory(lse),
-            "sums of exponentials ", lse.sizes(), ": contiguous fp32 of the labels' size expected");
+                lse.is_contiguous() && lse.numel() == 2 * c.h.N && in_memory(lse),
+            "sums of exponentials ", lse.sizes(), ": contiguous fp32, two for each label expected");
   else
-    lse = at::empty({c.h.N}, c.fp32());
+    lse = at::empty({c.h.N, 2}, c.fp32());
   if (c.h.N == 0)
     return at::full(shape, how.reduction == GS_REDUCE_MEAN ? std::nan("") : 0.0, c.fp32());
   const Tensor loss = at::empty(shape, c.fp32());
@@ -786,7 +786,7 @@ Tensor head_logit_grad(const Tensor& x, const Tensor& w, const Tensor& labels, c
   check_plain({&x, &w, &labels, &lse});
   const HeadCall c(x, w, labels, HeadHow{ignore_index, reduction, {}});
   require(lse.device() == c.dev && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
-              lse.numel() == c.h.N,
+              lse.numel() == 2 * c.h.N,
           "sums of exponentials ", lse.sizes());
   require(v0 >= 0 && n > 0 && v0 + n <= c.h.V, "logits ", v0, " to ", v0 + n, " of ", c.h.V);
   const int64_t stride = (n + 7) / 8 * 8;

@@ -257,7 +257,7 @@ class HeadCrossEntropy(nn.Linear):
             return super().forward(input)
         if self._backward_hooks and torch.is_grad_enabled():
             # An engine's backward hook forms the gradient of the logits from these.
-            lse = torch.empty(labels.shape, device=labels.device, dtype=torch.float32)
+            lse = torch.empty((*labels.shape, 2), device=labels.device, dtype=torch.float32)
             d["_gs_head"] = (labels, lse)
         return ops().head_cross_entropy(input, self.weight, labels, self.ignore_index, self.reduction,
                                         lse)

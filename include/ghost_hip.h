@@ -508,11 +508,11 @@ int gs_distill_grad(const gs_distill* d, const float* upstream, int filled, void
  *   z = W x,  loss = log sum_v exp(z_v) - z_y
  * in pieces of the vocabulary, without keeping z.  Rows whose label is ignore_index are not read:
  * their loss and gradient are zero; another label outside [0, V) makes the row's loss and gradient
- * NaN.  Products and sums are fp32 (fp32 operands as sums of three bf16 parts each).
+ * NaN.  Products and sums are fp32 (fp32 operands of more than 32 rows as sums of three bf16 parts each).
  * X: N rows of d contiguous features, x_stride elements apart.  W: [V, d].  Both of dtype.
  * reduction: GS_REDUCE_NONE (out_loss: [N]), GS_REDUCE_SUM, or GS_REDUCE_MEAN over the rows not
  * ignored (NaN when there are none, as 0 / 0; their gradients are zeros then).
- * lse: [N] fp32, what the backward pass takes of the forward one.
+ * lse: [N, 2] fp32, what the backward pass takes of the forward one.
  * gs_head_grad: dx [N, d] and dw [V, d] of dtype, either may be NULL; upstream: NULL (ones), or fp32,
  * [N] with NONE and [1] otherwise.  dz = softmax(z) - 1_y (times a row's own upstream gradient) is
  * rounded once to bf16 between the products with bf16 operands; other factors are applied in fp32

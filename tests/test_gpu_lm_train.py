@@ -115,6 +115,34 @@ def test_head_extreme_logits(gpu, N):
     assert_close(got, want[torch.arange(N), at], 1e-5)
 
 
+@pytest.mark.parametrize("N", [4, 260])
+def test_head_labels_with_most_of_the_mass(gpu, N):
+    """Logits of a hundred, all but a ten thousandth of the mass on the label: the loss and the label's
+    gradient keep what one rounding of the sum of exponentials (at least 1) and of p leaves them."""
+    V, d = 300, 8
+    w = torch.zeros(V, d)
+    w[:, 0] = 100.0                                # the same for all
+    w[:, 1] = torch.linspace(0, 1, V)
+    w[7, 2] = 1.0
+    x = torch.zeros(N, d)
+    x[:, 0], x[:, 1], x[:, 2] = 1.0, 0.25, 15.0    # exact products
+    labels = torch.full((N,), 7)
+    xg, wg = x.to(gpu).requires_grad_(), w.to(gpu).requires_grad_()
+    loss = gs.head_cross_entropy(xg, wg, labels.to(gpu), reduction="none")
+    lp = torch.log_softmax(f64(x) @ f64(w).t(), 1)
+    rest = -torch.expm1(lp[:, 7])                  # 1 - p
+    assert 5e-5 < rest[0] < 2e-4
+    # z: sums of three products, fp32 (three of its roundings at 100, of which the masses move by as much).
+    # The sum of exponentials: a lane adds up to 64 to the label's 1, each sum rounded there (U), then sixteen
+    # roundings at most of exponentials, joins, logarithm and quotient: the small ones lie below U's
+    # multiples, so the roundings all go one way.
+    share, sums = 3 * 128 * U, (64 + 16) * U
+    assert ((loss.detach().cpu().double() + lp[:, 7]).abs() <= share * -lp[:, 7] * 4 + sums).all()
+    dx, = torch.autograd.grad(loss, xg, torch.ones_like(loss))
+    want = (lp.exp() - torch.nn.functional.one_hot(labels, V)) @ f64(w)
+    assert ((dx.cpu().double() - want)[:, 2].abs() <= share * rest * 4 + sums).all()
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_head_strides_alignment_and_shapes(gpu, dtype):
     """Rows apart, overlapping or reversed, off 16-byte boundaries, transposed weights, more dimensions."""
@@ -191,7 +219,7 @@ def test_head_in_pieces(gpu, N, dtype, monkeypatch):
     xg, wg, yg = x.to(gpu).requires_grad_(), w.to(gpu).requires_grad_(), labels.to(gpu)
     up = torch.tensor(0.7, device=gpu)
     loss = gs.head_cross_entropy(xg, wg, yg)
-    lse = torch.empty(N, device=gpu)
+    lse = torch.empty(N, 2, device=gpu)
     _native.ops().head_cross_entropy(xg.detach(), wg.detach(), yg, -100, "mean", lse)
     want = L.head_all(x, w, labels, up.cpu(), "mean", dtype)
     whole = torch.cat([_native.ops().head_logit_grad(xg.detach(), wg.detach(), yg, lse, up, v0,
@@ -223,7 +251,7 @@ def test_head_of_many_rows_in_pieces(gpu):
     within(loss[part.to(gpu)], *want["loss"], "loss")
     dx, dw = torch.autograd.grad(loss, (xg, wg), torch.ones_like(loss))
     within(dx[part.to(gpu)], *want["dx"], "dx")
-    lse = torch.empty(N, device=gpu)
+    lse = torch.empty(N, 2, device=gpu)
     _native.ops().head_cross_entropy(xg.detach(), wg.detach(), yg, -100, "none", lse)
     for v0 in range(0, V, 1000):
         dz = _native.ops().head_logit_grad(xg.detach(), wg.detach(), yg, lse, torch.ones(N, device=gpu), v0,
@@ -243,7 +271,7 @@ def test_head_weight_gradient_in_whole_rounds_and_shares(gpu, ignored):
     xg, wg, yg = x.to(gpu).requires_grad_(), w.to(gpu).requires_grad_(), labels.to(gpu)
     dw, = torch.autograd.grad(gs.head_cross_entropy(xg, wg, yg, reduction="none"), wg,
                               torch.ones(N, device=gpu))
-    lse = torch.empty(N, device=gpu)
+    lse = torch.empty(N, 2, device=gpu)
     _native.ops().head_cross_entropy(xg.detach(), wg.detach(), yg, -100, "none", lse)
     for v0 in (0, 32000, 65536 - 300, V - 300):
         dz = _native.ops().head_logit_grad(xg.detach(), wg.detach(), yg, lse, torch.ones(N, device=gpu), v0,

@@ -188,7 +188,10 @@ class TrainOracleOps(LmOracleOps):
         rows, y = x.double().reshape(-1, w.shape[1]), labels.reshape(-1)
         if lse is not None:
             with torch.no_grad():
-                lse.copy_((torch.logsumexp(rows @ w.t(), 1) / math.log(2)).reshape(lse.shape))
+                z = rows @ w.t()
+                top = z.amax(1, keepdim=True)
+                lse.copy_(torch.cat((top / math.log(2), (z - top).exp().sum(1, keepdim=True)), 1)
+                          .reshape(lse.shape))
         loss = head_loss(rows, w, y, reduction, ignore_index).float()
         return loss.reshape(labels.shape if reduction == "none" else ())
 
@@ -198,7 +201,8 @@ class TrainOracleOps(LmOracleOps):
         rows = x.double().reshape(-1, w.shape[1])
         want = torch.logsumexp(rows @ w.t(), 1) / math.log(2)
         kept = labels.reshape(-1) != ignore_index
-        assert torch.allclose(lse.reshape(-1).double()[kept], want[kept], atol=1e-4)
+        ref, s = lse.reshape(-1, 2).double().unbind(1)
+        assert torch.allclose((ref + s.log2())[kept], want[kept], atol=1e-4)
         dz = head_dz(rows, w, labels.reshape(-1), grad.reshape(-1), v0, n, reduction, ignore_index)
         out = torch.zeros(len(rows), -(-n // 8) * 8, dtype=x.dtype)
         out[:, :n] = dz.to(x.dtype)
