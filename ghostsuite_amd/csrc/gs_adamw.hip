@@ -4,8 +4,11 @@
 //   m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2
 //   p = (1 - lr decay) p - lr / (1 - b1^t) m / ((v / (1 - b2^t))^(1/2) + eps)
 // in fp32, p rounded once to its type.  Bound by memory: every array is read once and written once
-// (GPT-2-small's 124 M bf16 parameters: 560 us with averages in 32 bits, 4.9 TB/s; 248 to 260 in 8 bits,
-// 4.8 TB/s, where the two hashes' products and the rounding keep the vector units about as long).
+// (GPT-2-small's 124 M bf16 parameters: 560 us with averages in 32 bits, 4.9 TB/s) but for 8 bits, where the
+// vector units take a little longer (280 us, 4.5 TB/s: every product, sum, root and quotient rounded as
+// fp32 rounds it; with contraction and the hardware's approximate root and reciprocal 255, but then an
+// average is a unit off, about one chance in 10^6 falls the other way and an element is held an eighth
+// away, and where it is its block's largest on the next step, so is the block's scale).
 // A launch takes many tensors (their addresses travel in its arguments); its workgroups take runs
 // of CHUNK elements, a tensor's last one shorter, and find their tensor by its first run (runs of 8192
 // elements were 4% slower than runs of 2048: more workgroups at work at once, above all where a launch has
@@ -122,20 +125,34 @@ __global__ void __launch_bounds__(NT) adamw_kernel(Tensors a, Factors f) {
 }
 
 // The largest of 32 lanes (half a wave holds a block), in each of them.
-__device__ __forceinline__ float half_max(float v) {
+__device__ __forceinline__ uint32_t half_max(uint32_t v) {
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+  for (int off = 16; off > 0; off >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), off, 64)));
   return v;
 }
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+constexpr uint32_t INF_BITS = 0x7F800000u, TOP_BITS = 0x43E00000u;   // of infinity and of 448
 
-// a of [0, 448] on the 8-bit values, up or down by the chance (u << 4) + 8 of 2^20: an integer addition
-// to the 20 mantissa bits that are cut off, which is floor(a / step + (u + 1/2) / 2^16) step.  Below 2^-6
-// the values' steps stay 2^-9: 2^-6 is added first, whose mantissa's steps are those, and taken off again.
+// a of [2^-6, 448] on the 8-bit values, up or down by the chance (u << 4) + 8 of 2^20: an integer addition
+// to the 20 mantissa bits that are cut off, which is floor(a / step + (u + 1/2) / 2^16) step (the sum has
+// no more than 24 bits).  So is zero, at zero.
 __device__ __forceinline__ float eighth(float a, uint32_t chance) {
-  const float low = a < 0x1p-6f ? 0x1p-6f : 0.f;
-  const float q = __uint_as_float((__float_as_uint(a + low) + chance) & 0xFFF00000u);
-  return fminf(q - low, TOP);
+  return __uint_as_float(min((__float_as_uint(a) + chance) & 0xFFF00000u, TOP_BITS));
 }
+// The same of any a: below 2^-6 the steps stay 2^-9, a may have bits below the chance's, and the sum is
+// rounded to fp32 before its floor.
+__device__ __forceinline__ float eighth_or_less(float a, uint32_t chance) {
+  const float low = floorf(__fmaf_rn(a, 0x1p29f, static_cast<float>(chance)) * 0x1p-20f) * 0x1p-9f;
+  return a < 0x1p-6f ? low : eighth(a, chance);
+}
+// The root of x, correctly rounded, for x of [2^-96, 2^96): from the hardware's inverse root, and what its
+// product with x leaves of x.  (Every such x was compared with a float64 root's rounding.  Comparing the
+// hardware's root's neighbours, as sqrtf does: 287 us for GPT-2-small's parameters, this 280.)
+__device__ __forceinline__ float root_of(float x) {
+  const float y = __builtin_amdgcn_rsqf(x), s = x * y;
+  return __fmaf_rn(__fmaf_rn(-s, s, x), 0.5f * y, s);
+}
+constexpr uint32_t ROOT_FROM = 0x0F800000u, ROOT_TO = 0x6F7FFFFFu;   // 2^-96, the last below 2^96
 // Four 8-bit values from their floats, which they hold exactly, and back.
 __device__ __forceinline__ uint32_t pack8(const float* v) {
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
@@ -173,6 +190,8 @@ __device__ __forceinline__ void store8(uint8_t* p, bool vec, int64_t left, const
 
 template <class E>
 __global__ void __launch_bounds__(NT) adamw8_kernel(Tensors a, Factors f) {
+  // each product and sum rounded by itself, in the order written
+#pragma clang fp contract(off)
   const int k = tensor_of(a, blockIdx.x);
   const gs_adamw_tensor& t = a.t[k];
   const int64_t first = static_cast<int64_t>(static_cast<int>(blockIdx.x) - a.first[k]) * CHUNK;
@@ -191,44 +210,68 @@ __global__ void __launch_bounds__(NT) adamw8_kernel(Tensors a, Factors f) {
   g.load(static_cast<const E*>(t.g) + i, vec, left);
   load8(tm + i, vec8, left, m);
   load8(tv + i, vec8, left, r);
-  float top_m = 0.f, top_r = 0.f, any = 0.f;
+  uint32_t beyond = 0;
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
     m[e] = f.b1 * (m[e] * sm) + f.rest1 * g.v[e];
     const float old = r[e] * sr;
-    // the hardware's root and reciprocal, each within one unit: p is off by as much of its move
-    r[e] = __builtin_amdgcn_sqrtf(f.b2 * (old * old) + f.rest2 * (g.v[e] * g.v[e]));
-    p.v[e] = f.keep * p.v[e] -
-             f.step * m[e] * __builtin_amdgcn_rcpf(fmaxf(r[e] * f.root + f.eps, 0x1p-126f));
-    top_m = fmaxf(top_m, fabsf(m[e]));
-    top_r = fmaxf(top_r, r[e]);
-    any += fabsf(m[e]) + r[e];
+    r[e] = f.b2 * (old * old) + f.rest2 * (g.v[e] * g.v[e]);
+    beyond = max(beyond, __float_as_uint(r[e]) - ROOT_FROM);
   }
-  p.store(static_cast<E*>(t.p) + i, vec, left);
-  const bool whole = any < INFINITY;   // all of them finite (or their sum too large: the same result)
-  if (!whole) {
-    top_m = top_r = 0.f;
-    for (int e = 0; e < VE; ++e) {
-      top_m = fmaxf(top_m, fabsf(m[e]) < INFINITY ? fabsf(m[e]) : 0.f);
-      top_r = fmaxf(top_r, r[e] < INFINITY ? r[e] : 0.f);
-    }
+  if (beyond <= ROOT_TO - ROOT_FROM) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) r[e] = root_of(r[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) r[e] = sqrtf(r[e]);
   }
-  top_m = half_max(top_m);
-  top_r = half_max(top_r);
-  const float im = top_m > 0.f ? TOP / top_m : 0.f, ir = top_r > 0.f ? TOP / top_r : 0.f;
+  uint32_t top_m = 0, top_r = 0;   // magnitudes by their bits: larger than infinity's, a NaN
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
+    p.v[e] = f.keep * p.v[e] - f.step * m[e] / fmaxf(r[e] * f.root + f.eps, 0x1p-126f);
+    top_m = max(top_m, magnitude(m[e]));
+    top_r = max(top_r, magnitude(r[e]));
+  }
+  p.store(static_cast<E*>(t.p) + i, vec, left);
+  const bool whole = max(top_m, top_r) < INF_BITS;   // all of them finite
+  if (!whole) {
+    top_m = top_r = 0;
+    for (int e = 0; e < VE; ++e) {
+      top_m = max(top_m, magnitude(m[e]) < INF_BITS ? magnitude(m[e]) : 0u);
+      top_r = max(top_r, magnitude(r[e]) < INF_BITS ? magnitude(r[e]) : 0u);
+    }
+  }
+  const float most_m = __uint_as_float(half_max(top_m)), most_r = __uint_as_float(half_max(top_r));
+  const float im = most_m > 0.f ? 1.f / most_m * TOP : 0.f, ir = most_r > 0.f ? 1.f / most_r * TOP : 0.f;
+  const auto chances = [&](int e) {
     uint32_t x = (static_cast<uint32_t>(i + e) + f.key) * 0x9E3779B9u;
     x = (x ^ (x >> 15)) * 0xBB67AE85u;
-    x ^= x >> 13;
-    const float hm = eighth(fabsf(m[e]) * im, ((x & 0xFFFFu) << 4) + 8u);
-    const float hr = eighth(r[e] * ir, ((x >> 16) << 4) + 8u);
-    m[e] = whole || fabsf(m[e]) < INFINITY ? copysignf(hm, m[e]) : NAN;
-    r[e] = whole || r[e] < INFINITY ? (r[e] > 0.f ? fmaxf(hr, 0x1p-9f) : 0.f) : NAN;
+    return x ^ (x >> 13);
+  };
+  const auto chance_m = [](uint32_t x) { return ((x & 0xFFFFu) << 4) + 8u; };
+  const auto chance_r = [](uint32_t x) { return ((x >> 16) << 4) + 8u; };
+  float least = INFINITY;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) least = fminf(least, fminf(fabsf(m[e]) * im, r[e] * ir));
+  if (whole && least >= 0x1p-6f) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const uint32_t x = chances(e);
+      m[e] = copysignf(eighth(fabsf(m[e]) * im, chance_m(x)), m[e]);
+      r[e] = eighth(r[e] * ir, chance_r(x));
+    }
+  } else {
+    for (int e = 0; e < VE; ++e) {
+      const uint32_t x = chances(e);
+      const float hm = eighth_or_less(fabsf(m[e]) * im, chance_m(x));
+      const float hr = eighth_or_less(r[e] * ir, chance_r(x));
+      m[e] = magnitude(m[e]) < INF_BITS ? copysignf(hm, m[e]) : NAN;
+      r[e] = magnitude(r[e]) < INF_BITS ? (r[e] > 0.f ? fmaxf(hr, 0x1p-9f) : 0.f) : NAN;
+    }
   }
   store8(tm + i, vec8, left, m);
   store8(tv + i, vec8, left, r);
-  if (live && (threadIdx.x & 31) == 0) t.m_scale[b] = top_m / TOP, t.v_scale[b] = top_r / TOP;
+  if (live && (threadIdx.x & 31) == 0) t.m_scale[b] = most_m * (1.f / TOP), t.v_scale[b] = most_r * (1.f / TOP);
 }
 
 }  // namespace

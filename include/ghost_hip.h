@@ -577,8 +577,14 @@ int gs_rms_norm_dot(const void* H, const void* G, int dtype, int64_t N, int64_t 
  * state_bits 32: m, v are [n] fp32; the scales are not looked at.
  * state_bits 8: blocks of GS_ADAMW_BLOCK elements share a scale, their largest magnitude over 448; m
  * and v are [n] bytes, floats of 4 exponent and 3 mantissa bits (no infinities) whose products with
- * the scale are the average of the gradients and the root of the average of their squares.  A value
- * a = magnitude over scale is held as step floor(a / step + u), step the distance of those floats at a,
+ * the scale are the average of the gradients and the root r of the average of their squares.  Every
+ * operation is rounded to fp32 by itself, in this order (largest: the magnitude; the factors of betas, lr
+ * and step are formed in double and rounded once):
+ *   m = beta1 (q scale) + (1 - beta1) g,  r = (beta2 (o o) + (1 - beta2) (g g))^(1/2) with o = q scale
+ *   p = keep p - (rate m) / (r root + eps),  keep = 1 - lr weight_decay, rate = lr / (1 - beta1^step),
+ *   root = (1 - beta2^step)^(-1/2);  scale = largest (1 / 448),  a = magnitude ((1 / largest) 448)
+ * so the same inputs give the same bits, step after step.
+ * a is held as step floor(a / step + u), step the distance of those floats at a, 448 at most,
  * u = (16 bits of a hash + 1/2) / 2^16: with k = step 0x9E3779B9 + seed 0x6A09E667 and i the element's
  * place in its tensor, x = (i + k) 0x9E3779B9, x = (x ^ x >> 15) 0xBB67AE85, x ^= x >> 13 (32 bits), the
  * lower half for m, the upper one for the root; a root above zero is held as 2^-9 at least.  A value that
