@@ -42,6 +42,9 @@ constexpr int CHUNK = NT * VE;       // elements of a workgroup, eight to a thre
 constexpr int MOST = 64;             // tensors of a launch (3.8 KB of arguments)
 constexpr int64_t MOST_RUNS = 1 << 23;   // runs of a launch: 2^31 threads
 constexpr float TOP = 448.f;
+// Blocks whose largest magnitude is below are held as zeros: where a gradient stops, m falls by b1 a step
+// until 448 over it is infinite, which zero times is not a number.
+constexpr float LEAST = 0x1p-100f;
 
 struct Tensors {
   gs_adamw_tensor t[MOST];
@@ -242,7 +245,8 @@ __global__ void __launch_bounds__(NT) adamw8_kernel(Tensors a, Factors f) {
     }
   }
   const float most_m = __uint_as_float(half_max(top_m)), most_r = __uint_as_float(half_max(top_r));
-  const float im = most_m > 0.f ? 1.f / most_m * TOP : 0.f, ir = most_r > 0.f ? 1.f / most_r * TOP : 0.f;
+  const bool some_m = most_m >= LEAST, some_r = most_r >= LEAST;
+  const float im = some_m ? 1.f / most_m * TOP : 0.f, ir = some_r ? 1.f / most_r * TOP : 0.f;
   const auto chances = [&](int e) {
     uint32_t x = (static_cast<uint32_t>(i + e) + f.key) * 0x9E3779B9u;
     x = (x ^ (x >> 15)) * 0xBB67AE85u;
@@ -266,12 +270,15 @@ __global__ void __launch_bounds__(NT) adamw8_kernel(Tensors a, Factors f) {
       const float hm = eighth_or_less(fabsf(m[e]) * im, chance_m(x));
       const float hr = eighth_or_less(r[e] * ir, chance_r(x));
       m[e] = magnitude(m[e]) < INF_BITS ? copysignf(hm, m[e]) : NAN;
-      r[e] = magnitude(r[e]) < INF_BITS ? (r[e] > 0.f ? fmaxf(hr, 0x1p-9f) : 0.f) : NAN;
+      r[e] = magnitude(r[e]) < INF_BITS ? (r[e] > 0.f && some_r ? fmaxf(hr, 0x1p-9f) : 0.f) : NAN;
     }
   }
   store8(tm + i, vec8, left, m);
   store8(tv + i, vec8, left, r);
-  if (live && (threadIdx.x & 31) == 0) t.m_scale[b] = most_m * (1.f / TOP), t.v_scale[b] = most_r * (1.f / TOP);
+  if (live && (threadIdx.x & 31) == 0) {
+    t.m_scale[b] = some_m ? most_m * (1.f / TOP) : 0.f;
+    t.v_scale[b] = some_r ? most_r * (1.f / TOP) : 0.f;
+  }
 }
 
 }  // namespace

@@ -587,7 +587,8 @@ int gs_rms_norm_dot(const void* H, const void* G, int dtype, int64_t N, int64_t 
  * a is held as step floor(a / step + u), step the distance of those floats at a, 448 at most,
  * u = (16 bits of a hash + 1/2) / 2^16: with k = step 0x9E3779B9 + seed 0x6A09E667 and i the element's
  * place in its tensor, x = (i + k) 0x9E3779B9, x = (x ^ x >> 15) 0xBB67AE85, x ^= x >> 13 (32 bits), the
- * lower half for m, the upper one for the root; a root above zero is held as 2^-9 at least.  A value that
+ * lower half for m, the upper one for the root; a root above zero is held as 2^-9 at least.  A block
+ * whose largest magnitude is below 2^-100 is held as zeros, its scale zero.  A value that
  * is not finite is held as NaN, and its block's scale is the others'. */
 #define GS_ADAMW_BLOCK 256
 typedef struct {

@@ -48,12 +48,14 @@ class Elementary:
         out = []
         for x, u in zip((m, root), chances(n, self.t, seed)):
             top = blocks(x).abs().amax(1)
+            top = torch.where(top >= 2.0 ** -100, top, 0.0)
             share = torch.where(top > 0, torch.ones(()) / top * f(TOP), f(0.0))
             a = (blocks(x).abs() * share[:, None]).view(-1)[:n]
             out += [held(a, u.float()), top * (f(1.0) / f(TOP))]
         q, self.m_scale, r, self.r_scale = out
         self.m = torch.copysign(q, m)
-        self.r = torch.where(root > 0, r.clamp(min=2.0 ** -9), 0.0)
+        some = self.r_scale.repeat_interleave(BLOCK)[:n] > 0
+        self.r = torch.where((root > 0) & some, r.clamp(min=2.0 ** -9), 0.0)
 
     def same_as(self, p, state):
         for name, mine, theirs in (("p", self.p, p), ("m", self.m, state["exp_avg"]),
@@ -92,3 +94,34 @@ def test_steps_are_the_elementary_ones(gpu, dtype, betas, spread):
         for p, e in zip(params, plain):
             e.step(p.grad.cpu(), 1e-3, betas, 1e-8, 0.1, 5)
             e.same_as(p, opt.state[p])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("largest", [2.0 ** -98, 1e-36, 1e-38, 1e-44])
+def test_blocks_of_next_to_nothing(gpu, dtype, largest):
+    """Averages that have fallen for hundreds of steps without a gradient, zeros among them: the zeros stay zeros,
+    and elements without a root never move, also with eps = 0."""
+    n = 4 * BLOCK
+    some = torch.arange(n) % 3 == 0                      # a third ever had a gradient
+    some[BLOCK:2 * BLOCK] = False
+    p = nn.Parameter(randn((n,), 1, 1.0, dtype).to(gpu))
+    plain = Elementary(p.detach().cpu())
+    opt = AdamW([p], lr=1e-3, eps=0.0, weight_decay=0.0, state_bits=8, seed=5)
+    p.grad = torch.zeros(n, dtype=dtype, device=gpu)
+    opt.step()
+    state = opt.state[p]
+    m, r = (torch.where(some, randn((n,), k, 100.0).abs().clamp(2.0, 448.0), 0.0).to(torch.float8_e4m3fn).float()
+            for k in (2, 3))
+    m_scale, r_scale = torch.full((4,), largest / 448), torch.full((4,), 1e-9)
+    for name, t in (("exp_avg", m), ("root_avg_sq", r), ("exp_avg_scale", m_scale), ("root_avg_sq_scale", r_scale)):
+        state[name].copy_(t)
+    plain.t, plain.m, plain.r, plain.m_scale, plain.r_scale = state["step"], m, r, m_scale, r_scale
+    before = p.detach().cpu()
+    for _ in range(25):
+        opt.step()
+        assert (state["exp_avg"].cpu().float()[~some] == 0).all()
+        assert torch.equal(p.detach().cpu()[~some], before[~some])
+        plain.step(p.grad.cpu(), 1e-3, (0.9, 0.999), 0.0, 0.0, 5)
+        plain.p = torch.where(some, plain.p, before)     # 0 / 0
+        plain.same_as(p, state)
+    assert (state["exp_avg_scale"] == 0).all() or largest > 2.0 ** -99
