@@ -25,7 +25,7 @@
 // sixteenth of its drift, a few hundredths of it where gradients are noise.)  A root that is not
 // zero never becomes zero, nor less than half of itself: where the gradient stops, m is not divided
 // by eps alone.  p is formed from m and v before their rounding.  A value that is not finite is held
-// as NaN and has no part in its block's scale.
+// as NaN and has no part in its block's scale; p is NaN from the next step on.
 
 #include <algorithm>
 #include <cmath>
@@ -231,7 +231,8 @@ __global__ void __launch_bounds__(NT) adamw8_kernel(Tensors a, Factors f) {
   uint32_t top_m = 0, top_r = 0;   // magnitudes by their bits: larger than infinity's, a NaN
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
-    p.v[e] = f.keep * p.v[e] - f.step * m[e] / fmaxf(r[e] * f.root + f.eps, 0x1p-126f);
+    const float by = r[e] * f.root + f.eps;   // NaN with the root; zero only with eps
+    p.v[e] = f.keep * p.v[e] - f.step * m[e] / (by == 0.f ? INFINITY : by);
     top_m = max(top_m, magnitude(m[e]));
     top_r = max(top_r, magnitude(r[e]));
   }

@@ -589,7 +589,8 @@ int gs_rms_norm_dot(const void* H, const void* G, int dtype, int64_t N, int64_t 
  * place in its tensor, x = (i + k) 0x9E3779B9, x = (x ^ x >> 15) 0xBB67AE85, x ^= x >> 13 (32 bits), the
  * lower half for m, the upper one for the root; a root above zero is held as 2^-9 at least.  A block
  * whose largest magnitude is below 2^-100 is held as zeros, its scale zero.  A value that
- * is not finite is held as NaN, and its block's scale is the others'. */
+ * is not finite (a gradient's square overflows from 1.8e19 on) is held as NaN, its block's scale is the
+ * others', and p is NaN from the next step on.  Where r root + eps is zero p does not move by it. */
 #define GS_ADAMW_BLOCK 256
 typedef struct {
   void* p;

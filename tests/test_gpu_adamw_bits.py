@@ -125,3 +125,35 @@ def test_blocks_of_next_to_nothing(gpu, dtype, largest):
         plain.p = torch.where(some, plain.p, before)     # 0 / 0
         plain.same_as(p, state)
     assert (state["exp_avg_scale"] == 0).all() or largest > 2.0 ** -99
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("eps", [1e-8, 0.0])
+def test_finite_gradients_whose_squares_are_not(gpu, dtype, eps):
+    """A gradient of 2e19, whose square is beyond fp32: no move on its own step (m over an infinite root), then NaN,
+    never a number without meaning; so with a root that a loaded state holds as NaN.  The others are untouched."""
+    n = 2 * BLOCK
+    g = randn((n,), 1, 1.0, dtype).to(gpu)
+    start = randn((n,), 2, 1.0, dtype).to(gpu)
+    p = nn.Parameter(start.clone())
+    opt = AdamW([p], lr=1e-3, eps=eps, weight_decay=0.0, state_bits=8)
+    big = torch.zeros(n, dtype=torch.bool, device=gpu)
+    big[[3, 300]] = True
+    for step in range(3):
+        p.grad = torch.where(big & (step == 0), torch.tensor(2e19, dtype=dtype, device=gpu), g)
+        opt.step()
+        assert torch.equal(p.detach().isnan(), big & (step > 0)), step
+        assert p.detach()[~big].isfinite().all() and ((p.detach() - start).abs()[~big] < 0.1).all()
+        if step == 0:
+            assert torch.equal(p.detach()[big], start[big])
+    assert torch.equal(opt.state[p]["root_avg_sq"].float().isnan(), big)
+    opt.state[p]["root_avg_sq"].copy_(torch.where(torch.arange(n, device=gpu) == 7, math.nan, 1.0))
+    opt.step()
+    assert p.detach()[7].isnan()
+    # where neither a gradient nor eps is there, nothing moves
+    z = nn.Parameter(start.clone())
+    opt = AdamW([z], lr=1e-3, eps=eps, weight_decay=0.0, state_bits=8)
+    for step in range(2):
+        z.grad = torch.zeros_like(z)
+        opt.step()
+        assert torch.equal(z.detach(), start)
