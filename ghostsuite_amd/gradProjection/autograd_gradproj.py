@@ -59,15 +59,18 @@ class GradProjHooks:
         if A_raw is None:
             raise RuntimeError(f'Missing cached activations for GradProjection in {self.layer_name}')
         B_out = grad_output[0]
+        head = module.__dict__.pop("_gs_head", None)   # labels and sums of a HeadCrossEntropy's loss
         if B_out is None:
             module._ghost_grad_proj = None
             delattr(module, '_ghost_A_raw')
             return
         B_out = B_out.detach()
         # The projection kernels run on a side stream, overlapped with the rest of backward.
-        with _overlap.on_side_stream(A_raw, B_out):
+        with _overlap.on_side_stream(A_raw, B_out, *(head or ())):
             if self.layer_type == 'Embedding':
                 self._compute_embedding_proj(module, A_raw, B_out)
+            elif head is not None:
+                self._compute_head_proj(module, A_raw, B_out, *head)
             else:
                 self._compute_dense_proj(module, A_raw, B_out)
         delattr(module, '_ghost_A_raw')
@@ -75,10 +78,6 @@ class GradProjHooks:
     def _compute_dense_proj(self, module: nn.Module, A_raw: torch.Tensor,
                             B_out: torch.Tensor) -> None:
         """Projected per-sample gradients of a dense layer (reference :120-165)."""
-        head = module.__dict__.pop("_gs_head", None)
-        if head is not None:   # a HeadCrossEntropy's loss
-            self._compute_head_proj(module, A_raw, B_out, *head)
-            return
         is_conv1d = module.__class__.__name__ == 'Conv1D'
         A = _flatten_tokens(A_raw)
         B = _flatten_tokens(B_out)
