@@ -1106,7 +1106,8 @@ __global__ void __launch_bounds__(256) head_dw_finish_kernel(const float* sums, 
 
 // ------------------------------------------------------------------------------ host side
 
-constexpr int64_t PIECE_BYTES = int64_t{1} << 30;   // of dz at most
+constexpr int64_t PIECE_BYTES = int64_t{1} << 30;   // of dz at most, but for a piece of 256 entries
+constexpr int64_t PIECE_ENTRIES = int64_t{1} << 25;
 constexpr int64_t CUS = 256;
 
 enum Size { WIDE, MID, SMALL, FEW };
@@ -1233,7 +1234,7 @@ Plan plan_of(const gs_head& h, int w_align) {
   p.row_bytes = p.full ? 4 : p.f32 ? 6 : 2;
   p.dz_bytes = p.full ? 4 : 2 * (p.few ? dz_parts<Few>(p.f32) : dz_parts<Wide>(p.f32));
   const int64_t all = cdiv(h.V, 256);
-  const int64_t most = std::max<int64_t>(1, PIECE_BYTES / (h.N * p.dz_bytes * 256));
+  const int64_t most = std::min(std::max<int64_t>(1, PIECE_BYTES / (h.N * p.dz_bytes * 256)), PIECE_ENTRIES / 256);
   if (all <= most) {
     p.cols = all * 256;
   } else {
@@ -1421,11 +1422,35 @@ void launch_dx_finish(const gs_head& h, const Plan& p, const Buffers& b, const f
     hipLaunchKernelGGL(head_dx_finish_kernel<E>, dim3(grid_of(h.N * a.f_blocks)), dim3(256), 0, s, a);
 }
 
-// Whether every grid of a call can be launched: shares are at most 2 * 512 where tiles are few.
-bool grids_fit(const gs_head& h, const Plan& p) {
-  const int64_t t = cdiv(h.N, FEW_ROWS), v = cdiv(p.cols, 64), f = cdiv(p.dp, 64), most = INT32_MAX / 2048;
-  return t <= most / f && v <= most / f && p.cols <= (1 << 25) &&
-         cdiv(p.cols, 256) <= INT32_MAX / cdiv(h.N, 256);
+// Whether every grid of a call can be launched: at most 2^31 threads.  dx, dw, rows: whether the call forms dx,
+// dW, or the logits' gradient as rows of the caller's.  `vocab`: the entries of the call.
+bool grids_fit(const gs_head& h, const Plan& p, int64_t vocab, bool dx, bool dw, bool rows) {
+  constexpr int64_t MOST = int64_t{1} << 31;
+  // a workgroup of 256 to 16 rows, of 1024 to 64, of 256 to 4
+  if (h.N > MOST / 16 || (rows && h.N > MOST / 64)) return false;
+  const auto threads = [](Size s) { return int64_t{s == WIDE ? Wide::NT : s == MID ? Mid::NT : s == SMALL ? Small::NT : Few::NT}; };
+  const auto fits = [](int64_t a, int64_t b, int64_t c) {   // the product of three, none negative
+    return a == 0 || b == 0 || c == 0 || (a <= MOST / b && a * b <= MOST / c);
+  };
+  for (int64_t v0 = 0; v0 < vocab; v0 += p.cols) {
+    const int64_t n = std::min(p.cols, vocab - v0);
+    if (n < p.cols || v0 == 0) {   // the pieces are alike but for the last
+      const Size s = logits_shape(h, p, n).size;
+      if (!fits(cdiv(n, rows_of(s)), cdiv(h.N, s == FEW ? Few::BN : rows_of(s)), threads(s))) return false;
+      const DwParts w = dw_parts(h, p, n);
+      for (int i = 0; i < 2 && dw; ++i) {
+        const Size z = w.shape[i].size;
+        const int64_t bv = z == FEW ? FewW::BN : rows_of(z), bf = z == FEW ? FewW::BM : rows_of(z);
+        if (!fits(cdiv(w.n[i], bv) * std::max<int64_t>(1, w.shape[i].splits), cdiv(h.d, bf), threads(z)) ||
+            (w.shape[i].splits > 1 && !fits(w.n[i], h.d, 1)))
+          return false;
+      }
+    }
+  }
+  if (!dx) return true;
+  const int64_t tiles = cdiv(h.N, p.dx_size == FEW ? FewT::BM : rows_of(p.dx_size));
+  return fits(p.dx.f_tiles, tiles, threads(p.dx_size)) && fits(p.dx.slots, threads(p.dx_size), 1) &&
+         (h.N >= 1024 ? fits(h.N, p.dp / 4, 1) : fits(h.N, cdiv(h.d, 64), 256));
 }
 
 LogitsArgs logits_args(const gs_head& h, const Plan& p, const Buffers& b) {
@@ -1454,7 +1479,8 @@ extern "C" int gs_head_loss(const gs_head* h, float* out_loss, float* lse, void*
   if (out_loss == nullptr || lse == nullptr)
     return fail(GS_ERR_INVALID, "gs_head_loss: no place for the loss");
   const Plan p = plan_of(*h, align_of(h->W));
-  if (!grids_fit(*h, p)) return fail(GS_ERR_UNSUPPORTED, "gs_head_loss: grid too large");
+  if (!grids_fit(*h, p, h->V, false, false, false))
+    return fail(GS_ERR_UNSUPPORTED, "gs_head_loss: grid too large");
   Carver c(workspace, workspace_bytes);
   const Buffers b = carve(c, *h, p, false);
   if (workspace == nullptr || !c.ok())
@@ -1499,7 +1525,8 @@ extern "C" int gs_head_grad(const gs_head* h, const float* lse, const float* ups
   if (const int rc = check_head(h, "gs_head_grad")) return rc;
   if (lse == nullptr) return fail(GS_ERR_INVALID, "gs_head_grad: the forward pass's sums are missing");
   const Plan p = plan_of(*h, align_of(h->W));
-  if (!grids_fit(*h, p)) return fail(GS_ERR_UNSUPPORTED, "gs_head_grad: grid too large");
+  if (!grids_fit(*h, p, h->V, dx != nullptr, dw != nullptr, false))
+    return fail(GS_ERR_UNSUPPORTED, "gs_head_grad: grid too large");
   Carver c(workspace, workspace_bytes);
   const Buffers b = carve(c, *h, p, true);
   if (workspace == nullptr || !c.ok())
@@ -1582,7 +1609,7 @@ extern "C" int gs_head_logit_grad(const gs_head* h, const float* lse, const floa
       out_stride != round_up(n, 8))
     return fail(GS_ERR_INVALID, "gs_head_logit_grad: invalid arguments");
   const Plan p = piece_plan(*h, n, piece_align(*h, v0));
-  if (!grids_fit(*h, p))
+  if (!grids_fit(*h, p, n, false, false, true))
     return fail(GS_ERR_UNSUPPORTED, "gs_head_logit_grad: grid too large");
   Carver c(workspace, workspace_bytes);
   const Buffers b = carve_piece(c, *h, n, p);

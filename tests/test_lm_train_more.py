@@ -1,13 +1,13 @@
 """The output projection's loss, the norm and the optimizer without a GPU: what the engines keep, mark and split
 on the way, and what the entry points take."""
+import ctypes
+
 import pytest
 import torch
-from torch import nn
 
-import ghostsuite_amd as gs
-from ghostsuite_amd import GradProjLoraEngine
+from ghostsuite_amd import GradProjLoraEngine, _native
 from ghostsuite_amd.gradProjection import autograd_gradproj
-from tests.test_lm_train import _Net, oracle_ops   # noqa: F401  (a fixture)
+from tests.test_lm_train import P16, _Net, _head, oracle_ops   # noqa: F401  (a fixture)
 
 
 def _projection(net, tmp_path, **how):
@@ -37,3 +37,28 @@ def test_projection_marks_what_the_side_stream_reads(oracle_ops, monkeypatch, tm
     loss.backward()
     assert any(t is kept for t in marked) and any(t is lse for t in marked)
     assert "_gs_head" not in net.head.__dict__ and net.head._ghost_grad_proj is not None
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("N,V,d", [(100, 2 ** 20, 4096), (524300, 50257, 4096), (262144, 300, 8192),
+                                   (2, 2 ** 26, 16), (1, 2 ** 30, 2), (2 ** 24, 9, 64), (40, 70, 2 ** 20)])
+def test_head_takes_every_shape_whose_grids_fit(N, V, d, dtype):
+    """Past the check of the grids the missing workspace is what is refused."""
+    lib = _native.load_library()
+    ref = ctypes.byref(_head(N=N, V=V, d=d, x_stride=d, dtype=dtype))
+    assert 0 < lib.gs_head_loss_workspace(ref) and 0 < lib.gs_head_grad_workspace(ref)
+    assert lib.gs_head_loss(ref, P16, P16, None, 0, None) == -3
+    assert lib.gs_head_grad(ref, P16, None, P16, P16, None, 0, None) == -3
+    assert lib.gs_head_logit_grad(ref, P16, None, 0, 8, P16, 8, None, 0, None) == -3
+
+
+@pytest.mark.parametrize("N,V,d,status", [(2 ** 27 + 1, 8, 8, -5), (2 ** 30, 2 ** 30, 8, -5), (2 ** 27, 8, 8, -3),
+                                          (2 ** 25, 8, 1024, -5)])
+def test_head_refuses_grids_beyond_a_launch(N, V, d, status):
+    """2^31 threads: 16 to a row, 64 to a row of the logits' gradient, and one to four features of dx."""
+    lib = _native.load_library()
+    ref = ctypes.byref(_head(N=N, V=V, d=d, x_stride=d))
+    assert lib.gs_head_grad(ref, P16, None, P16, P16, None, 0, None) == status
+    assert lib.gs_head_grad(ref, P16, None, None, P16, None, 0, None) == (-3 if N == 2 ** 25 else status)
+    assert lib.gs_head_loss(ref, P16, P16, None, 0, None) == (-3 if N == 2 ** 25 else status)
+    assert lib.gs_head_logit_grad(ref, P16, None, 0, 8, P16, 8, None, 0, None) == (-3 if N == 2 ** 25 else -5)
