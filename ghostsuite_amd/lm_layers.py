@@ -266,12 +266,16 @@ class HeadCrossEntropy(nn.Linear):
         return f"{super().extra_repr()}, reduction={self.reduction}"
 
 
+PIECE_BYTES = 512 << 20   # of a piece of the logits' gradient under an engine, but for one of 256 entries
+
+
 def head_gradient_pieces(layer: HeadCrossEntropy, x: torch.Tensor, labels: torch.Tensor,
                          lse: torch.Tensor, grad: torch.Tensor):
     """(first entry, entries, gradient of those logits [*labels.shape, entries up to a multiple of 8])
-    of a HeadCrossEntropy's loss, piece by piece of the vocabulary, in up to 512 MiB each."""
+    of a HeadCrossEntropy's loss, piece by piece of the vocabulary, in up to PIECE_BYTES each (but at
+    least 256 entries)."""
     vocab = layer.weight.shape[0]
-    each = max(256, (512 << 20) // max(1, labels.numel() * x.element_size()) // 256 * 256)
+    each = max(256, PIECE_BYTES // max(1, labels.numel() * x.element_size()) // 256 * 256)
     each = -(-vocab // (-(-vocab // each)))               # pieces of a size
     each = -(-each // 256) * 256
     for v0 in range(0, vocab, each):

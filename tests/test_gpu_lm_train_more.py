@@ -1,15 +1,19 @@
 """The output projection's loss and the norm on the GPU, under both engines and in calls with more than one piece
 of the vocabulary."""
+import ctypes
+
 import pytest
 import torch
 from torch import nn
 
 import ghostsuite_amd as gs
-from ghostsuite_amd import GradProjLoraEngine, _native
+from ghostsuite_amd import GradDotProdEngine, GradProjLoraEngine, _native, lm_layers
 from tests import train_forms as L
 from tests.helpers import BF16_TOL, assert_close, gen, randn
 from tests.lm_bounds import within
-from tests.lm_forms import HALF, U
+from tests.lm_forms import HALF, U, f64
+from tests.test_gpu_lm_train import head_inputs
+from tests.test_lm_train import _head
 
 pytestmark = pytest.mark.gpu
 BF16, FP32 = torch.bfloat16, torch.float32
@@ -117,3 +121,94 @@ def test_head_of_more_than_2_25_entries(gpu, dtype):
     within(loss, *want["loss"], "loss")
     within(dx, *want["dx"], "dx")
     within(dw, *want["dw"], "dw")
+
+
+# ------------------------------------------------------------- pieces of the vocabulary
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("n,T,n_val", [(6, 64, 2), (5, 50, 1), (4, 256, 2), (9, 1, 3)])
+@pytest.mark.parametrize("V", [512, 700])
+def test_engines_over_the_vocabularys_pieces(gpu, monkeypatch, tmp_path, dtype, n, T, n_val, V):
+    """Under both engines, in pieces of 256 entries and in one: dots, train gradient and projection of either
+    within the type's tolerance of the other's and of float64's."""
+    d = 128
+    x, w, labels = head_inputs(n * T, V, d, dtype, 7)
+    got, made = [], []
+    real = _native.ops().head_logit_grad
+
+    def counted(*args):
+        made.append(args[5:7])
+        return real(*args)
+    monkeypatch.setattr(_native.ops(), "head_logit_grad", counted)
+    for limit in (1 << 30, 1):
+        monkeypatch.setattr(lm_layers, "PIECE_BYTES", limit)
+        net = nn.Sequential()
+        net.add_module("head", gs.HeadCrossEntropy(d, V).to(gpu, dtype))
+        layer = net.head
+        with torch.no_grad():
+            layer.weight.copy_(w)
+        net.forward = layer.forward
+        for which in ("dots", "projection"):
+            del made[:]
+            if which == "dots":
+                eng = GradDotProdEngine(net, val_batch_size=n_val, use_dummy_bias=True,
+                                        precision="fp32" if dtype == FP32 else "reference")
+                eng.attach(torch.optim.SGD(layer.parameters(), lr=0.0))
+            else:
+                eng = projection(net, tmp_path)
+                P_i, P_o = (p.double().cpu() for p in eng.projection_matrices["head"])
+            xg = x.view(n, T, d).to(gpu).requires_grad_()
+            layer(xg, labels.view(n, T).to(gpu)).backward()
+            torch.cuda.synchronize()
+            assert made == ([(0, V)] if limit > 1 else [(v, min(256, V - v)) for v in range(0, V, 256)])
+            got += [layer.weight.grad_dot_prod.double().cpu(), layer.weight.train_grad.clone()] if which == "dots" \
+                else [layer._ghost_grad_proj.double().cpu().clone()]
+            eng.detach()
+    tol = BF16_TOL if dtype == BF16 else 1e-4
+    dz = L.head_dz(f64(x), f64(w), labels, torch.tensor(1.0), 0, V, "mean").view(n, T, V)
+    grads = torch.stack([dz[i].t() @ f64(x).view(n, T, d)[i] for i in range(n)])
+    # A dot of one branch is a sum over pairs of tokens of (dz_s dz_t)(x_s x_t), whose addends cancel.  With bf16
+    # operands each dz is rounded once (two HALF), and each of the two products once more (two HALF) before their
+    # product; dz itself is off by 10^-4 of itself at most (its logits' sums), so a dot by (4 HALF + 3e-4) of its
+    # addends' sizes, second-order terms in the rest; fp32 likewise with U.
+    sizes = torch.stack([dz[i].abs().t() @ f64(x).view(n, T, d)[i].abs() for i in range(n)])
+    exact, bound = ((t[:n - n_val] * t[n - n_val:].sum(0)).sum((1, 2)) for t in (grads, sizes))
+    bound = bound * (4 * HALF[dtype] + 3e-4)
+    mine = labels.clone()
+    mine[(n - n_val) * T:] = -100
+    # the train rows' part of the whole batch's mean, times samples over train samples
+    share = torch.tensor(float((mine != -100).sum()) / float((labels != -100).sum()) * n / (n - n_val))
+    for dots, train, proj in (got[:3], got[3:]):
+        if 2 * T * T <= V * d:   # the other branch sums the val samples' rows first: another quantity
+            within(dots, exact, bound, "dots")
+        within(train, *L.head_all(x, w, mine, share, "mean", dtype)["dw"], "train gradient")
+        want = n * torch.stack([P_o @ g @ P_i.t() for g in grads])
+        assert_close(proj.reshape(want.shape), want, tol, "projection")
+    if 2 * T * T > V * d:
+        assert_close(got[3], got[0], tol, "dots of the pieces")
+
+
+def test_head_fp32_gradients_of_several_pieces(gpu):
+    """fp32 rows whose pieces of 1 GiB of the logits' gradient are three: the weight is split into its parts a piece
+    at a time, dx added up over them, and the last one is shorter."""
+    N, V, d = 21000, 20000, 40
+    x, w, labels = head_inputs(N, V, d, FP32, 5)
+    up = torch.rand(N, generator=gen(6)) + 0.5
+    xg, wg, yg = x.to(gpu).requires_grad_(), w.to(gpu).requires_grad_(), labels.to(gpu)
+    need = _native.load_library().gs_head_grad_workspace(
+        ctypes.byref(_head(N=N, V=V, d=d, x_stride=d, dtype=1, reduction=0)))
+    assert 0 < need < 6 * N * V / 2   # less than half of the whole in three parts of 2 bytes
+    loss = gs.head_cross_entropy(xg, wg, yg, reduction="none")
+    dx, dw = torch.autograd.grad(loss, (xg, wg), up.to(gpu))
+    part = torch.randperm(N, generator=gen(1))[:200]
+    want = L.head_all(x[part], w, labels[part], up[part], "none", FP32)
+    within(loss[part.to(gpu)], *want["loss"], "loss")
+    within(dx[part.to(gpu)], *want["dx"], "dx")
+    lse = torch.empty(N, 2, device=gpu)
+    _native.ops().head_cross_entropy(xg.detach(), wg.detach(), yg, -100, "none", lse)
+    for v0 in (0, 8448 - 300, 2 * 8448 - 300, V - 300):
+        dz = _native.ops().head_logit_grad(xg.detach(), wg.detach(), yg, lse, up.to(gpu), v0, 300, -100,
+                                           "none")[:, :300].double().t().contiguous()
+        rows = xg.detach().double()
+        ref, size = dz @ rows, dz.abs() @ rows.abs()
+        # dz within U of either side's, six products of parts, the sums' terms and the output's rounding
+        within(dw[v0:v0 + 300], ref.cpu(), (ref.abs() * U + (18 * N + 64) * U * size).cpu(), "dw")

@@ -1,12 +1,14 @@
 """The output projection's loss, the norm and the optimizer without a GPU: what the engines keep, mark and split
 on the way, and what the entry points take."""
+import copy
 import ctypes
 
 import pytest
 import torch
 
-from ghostsuite_amd import GradProjLoraEngine, _native
+from ghostsuite_amd import GradDotProdEngine, GradProjLoraEngine, _native, lm_layers
 from ghostsuite_amd.gradProjection import autograd_gradproj
+from tests.helpers import assert_close
 from tests.test_lm_train import P16, _Net, _head, oracle_ops   # noqa: F401  (a fixture)
 
 
@@ -37,6 +39,38 @@ def test_projection_marks_what_the_side_stream_reads(oracle_ops, monkeypatch, tm
     loss.backward()
     assert any(t is kept for t in marked) and any(t is lse for t in marked)
     assert "_gs_head" not in net.head.__dict__ and net.head._ghost_grad_proj is not None
+
+
+@pytest.mark.parametrize("vocab,pieces", [(256, 1), (257, 2), (700, 3)])
+@pytest.mark.parametrize("T", [3, 40])
+def test_engines_sum_over_the_vocabularys_pieces(oracle_ops, monkeypatch, tmp_path, vocab, pieces, T):   # noqa: F811
+    """Dots, train gradient and projection of pieces of 256 entries, a shorter last one among them, are those of
+    the whole vocabulary; both branches of the dots (2 T^2 against the weights)."""
+    torch.manual_seed(3)
+    net = _Net(vocab=vocab)
+    ids, labels = torch.randint(0, vocab, (5, T)), torch.randint(0, vocab, (5, T))
+    labels[0, 0] = -100
+    got = []
+    for limit in (1 << 30, 1):
+        monkeypatch.setattr(lm_layers, "PIECE_BYTES", limit)
+        for make in (lambda m: GradDotProdEngine(m, val_batch_size=2, use_dummy_bias=False, precision="fp32"), None):
+            m = copy.deepcopy(net)
+            if make is None:
+                eng = _projection(m, tmp_path)
+            else:
+                eng = make(m)
+                eng.attach(torch.optim.SGD(m.parameters(), lr=0.0))
+            del oracle_ops.calls[:]
+            m(ids, labels).backward()
+            made = [c[1] for c in oracle_ops.calls if c[0] == "head_logit_grad"]
+            assert made == ([(0, vocab)] if limit > 1 else
+                            [(v, min(256, vocab - v)) for v in range(0, vocab, 256)])
+            assert len(made) == (1 if limit > 1 else pieces)
+            w = m.head.weight
+            got.append([m.head._ghost_grad_proj] if make is None else [w.grad_dot_prod, w.train_grad])
+    for whole, split in zip(got[:2], got[2:]):
+        for a, b in zip(whole, split):
+            assert_close(b, a, 1e-5)
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
