@@ -212,3 +212,33 @@ def test_head_fp32_gradients_of_several_pieces(gpu):
         ref, size = dz @ rows, dz.abs() @ rows.abs()
         # dz within U of either side's, six products of parts, the sums' terms and the output's rounding
         within(dw[v0:v0 + 300], ref.cpu(), (ref.abs() * U + (18 * N + 64) * U * size).cpu(), "dw")
+
+
+# --------------------------------------------------------------------------- autocast
+def test_norm_under_autocast(gpu):
+    """fp32 weights with bf16 rows, fp32 rows or both: in fp32, as torch's norms; operands of one type as they are."""
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        for dtypes in ((BF16, BF16), (BF16, FP32), (FP32, BF16), (FP32, FP32)):
+            x, res = (randn((5, 7, 96), k, 1.0, t).to(gpu).requires_grad_() for k, t in enumerate(dtypes))
+            norm = gs.RMSNorm(96).to(gpu)
+            with torch.no_grad():
+                norm.weight.copy_(1 + 0.3 * randn((96,), 9))
+            y, h = norm(x, res)
+            alone = norm(x)
+            assert y.dtype == h.dtype == alone.dtype == FP32
+            gy, gh = randn(y.shape, 3).to(gpu), randn(y.shape, 4).to(gpu)
+            dx, dres, dw = torch.autograd.grad((y, h), (x, res, norm.weight), (gy, gh))
+            assert (dx.dtype, dres.dtype, dw.dtype) == (*dtypes, FP32)
+            rows = x.detach().float() + res.detach().float()
+            assert torch.equal(h, rows)
+            want = L.norm_all(rows, norm.weight, gy, gh, 1e-6, FP32)
+            within(y, *want["y"], "y")
+            within(dw, *want["dw"], "dw")
+            for g, t in ((dx, dtypes[0]), (dres, dtypes[1])):
+                v, b = want["dh"]
+                within(g, v, b + v.abs() * HALF[t], "dx")
+            within(alone, *L.norm_all(x.detach().float(), norm.weight, None, None, 1e-6, FP32)["y"], "y alone")
+        half = gs.RMSNorm(96).to(gpu, BF16)
+        assert half(x.detach().bfloat16()).dtype == BF16
+    with pytest.raises(_native.GhostHipError):
+        norm(x.detach().bfloat16())
