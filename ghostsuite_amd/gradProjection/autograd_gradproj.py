@@ -59,7 +59,7 @@ class GradProjHooks:
         if A_raw is None:
             raise RuntimeError(f'Missing cached activations for GradProjection in {self.layer_name}')
         B_out = grad_output[0]
-        head = module.__dict__.pop("_gs_head", None)   # labels and sums of a HeadCrossEntropy's loss
+        head = module.__dict__.pop("_gs_head", None)   # what a HeadCrossEntropy's loss took and left
         if B_out is None:
             module._ghost_grad_proj = None
             delattr(module, '_ghost_A_raw')
@@ -70,7 +70,7 @@ class GradProjHooks:
             if self.layer_type == 'Embedding':
                 self._compute_embedding_proj(module, A_raw, B_out)
             elif head is not None:
-                self._compute_head_proj(module, A_raw, B_out, *head)
+                self._compute_head_proj(module, B_out, *head)
             else:
                 self._compute_dense_proj(module, A_raw, B_out)
         delattr(module, '_ghost_A_raw')
@@ -92,7 +92,7 @@ class GradProjHooks:
         module._ghost_grad_proj = ops().kron_proj(A, B, P_i, P_o, float(batch_size),
                                                   layout=layout, out_dtype=torch.float32)
 
-    def _compute_head_proj(self, module: nn.Module, A: torch.Tensor, grad: torch.Tensor,
+    def _compute_head_proj(self, module: nn.Module, grad: torch.Tensor, A: torch.Tensor,
                            labels: torch.Tensor, lse: torch.Tensor) -> None:
         """An nn.Linear's projection of a layer that ended in its loss: the sum over the pieces of the
         vocabulary, each with its columns of P_o."""

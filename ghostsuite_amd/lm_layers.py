@@ -217,6 +217,10 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor,
                                    float(alpha), int(ignore_index), reduction)
 
 
+def _autocast() -> bool:
+    return torch.is_autocast_enabled("cuda")
+
+
 # Output projection with its cross entropy ####################################################
 
 def _check_reduction(reduction) -> None:
@@ -235,9 +239,17 @@ def head_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tens
     Rows whose label is ignore_index take no part and are not read; their loss and gradient are zero.
     Another label outside [0, vocab) makes its row's loss and gradient NaN.
     reduction: 'mean' (over the rows not ignored; NaN when there are none), 'sum', or 'none' ([...]).
-    The loss is fp32."""
+    The loss is fp32.  Under autocast x and weight are cast to its type, as an ``nn.Linear``'s."""
     _check_reduction(reduction)
+    x, weight = _head_operands(x, weight)
     return ops().head_cross_entropy(x, weight, labels, int(ignore_index), reduction)
+
+
+def _head_operands(x: torch.Tensor, weight: torch.Tensor):
+    if not _autocast():
+        return x, weight
+    dtype = torch.get_autocast_dtype("cuda")
+    return x.to(dtype), weight.to(dtype)
 
 
 class HeadCrossEntropy(nn.Linear):
@@ -255,12 +267,12 @@ class HeadCrossEntropy(nn.Linear):
         d.pop("_gs_head", None)
         if labels is None:
             return super().forward(input)
+        x, weight = _head_operands(input, self.weight)
         if self._backward_hooks and torch.is_grad_enabled():
             # An engine's backward hook forms the gradient of the logits from these.
             lse = torch.empty((*labels.shape, 2), device=labels.device, dtype=torch.float32)
-            d["_gs_head"] = (labels, lse)
-        return ops().head_cross_entropy(input, self.weight, labels, self.ignore_index, self.reduction,
-                                        lse)
+            d["_gs_head"] = (x.detach(), labels, lse)
+        return ops().head_cross_entropy(x, weight, labels, self.ignore_index, self.reduction, lse)
 
     def extra_repr(self) -> str:
         return f"{super().extra_repr()}, reduction={self.reduction}"
@@ -273,22 +285,19 @@ def head_gradient_pieces(layer: HeadCrossEntropy, x: torch.Tensor, labels: torch
                          lse: torch.Tensor, grad: torch.Tensor):
     """(first entry, entries, gradient of those logits [*labels.shape, entries up to a multiple of 8])
     of a HeadCrossEntropy's loss, piece by piece of the vocabulary, in up to PIECE_BYTES each (but at
-    least 256 entries)."""
-    vocab = layer.weight.shape[0]
+    least 256 entries).  x: the rows as the loss took them."""
+    weight = layer.weight.detach().to(x.dtype)
+    vocab = weight.shape[0]
     each = max(256, PIECE_BYTES // max(1, labels.numel() * x.element_size()) // 256 * 256)
     each = -(-vocab // (-(-vocab // each)))               # pieces of a size
     each = -(-each // 256) * 256
     for v0 in range(0, vocab, each):
         n = min(each, vocab - v0)
-        yield v0, n, ops().head_logit_grad(x, layer.weight.detach(), labels, lse, grad, v0, n,
-                                           layer.ignore_index, layer.reduction)
+        yield v0, n, ops().head_logit_grad(x, weight, labels, lse, grad, v0, n, layer.ignore_index,
+                                           layer.reduction)
 
 
 # Root-mean-square norm of a residual stream ##################################################
-
-def _autocast() -> bool:
-    return torch.is_autocast_enabled("cuda")
-
 
 def _norm_operands(*tensors: Optional[torch.Tensor]):
     """Under autocast, tensors of several types all in fp32, as torch's norms take them there."""

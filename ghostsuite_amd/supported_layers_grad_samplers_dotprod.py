@@ -616,7 +616,7 @@ def _compute_head_dot_product(layer: HeadCrossEntropy, A: torch.Tensor, B: torch
     n_t = A.size(0) - val_batch_size
     if n_t <= 0:
         raise ValueError("No training samples to compute dot product, check batch sizes.")
-    A, labels, lse = A.detach(), *head
+    A, labels, lse = head   # the rows as the loss took them, which autocast may have cast
     weight = _param(layer, "weight")
     trains = getattr(weight, "initially_requires_grad", False)
     _should_use_ghost_computation(layer, A, None)

@@ -12,7 +12,7 @@ from tests import train_forms as L
 from tests.helpers import BF16_TOL, assert_close, gen, randn
 from tests.lm_bounds import within
 from tests.lm_forms import HALF, U, f64
-from tests.test_gpu_lm_train import head_inputs
+from tests.test_gpu_lm_train import _model, head_inputs
 from tests.test_lm_train import _head
 
 pytestmark = pytest.mark.gpu
@@ -242,3 +242,85 @@ def test_norm_under_autocast(gpu):
         assert half(x.detach().bfloat16()).dtype == BF16
     with pytest.raises(_native.GhostHipError):
         norm(x.detach().bfloat16())
+
+
+@pytest.mark.parametrize("N", [20, 300])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_head_under_autocast(gpu, dtype, N):
+    """fp32 weights and rows of either type: the loss and gradients of the operands cast to bf16, the gradients in
+    the operands' own types."""
+    V, d = 700, 96
+    x, w, labels = head_inputs(N, V, d, BF16, 3)
+    xg = x.to(dtype).to(gpu).requires_grad_()
+    layer = gs.HeadCrossEntropy(d, V).to(gpu)
+    with torch.no_grad():
+        layer.weight.copy_(w.float() + 1e-5 * randn((V, d), 4))
+    with pytest.raises(_native.GhostHipError):
+        layer(x.to(gpu), labels.to(gpu))
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = layer(xg, labels.to(gpu))
+        assert layer(xg).dtype == BF16
+    dx, dw = torch.autograd.grad(loss, (xg, layer.weight))
+    assert loss.dtype == FP32 and dx.dtype == dtype and dw.dtype == FP32
+    want = L.head_all(x, layer.weight.detach().bfloat16().cpu(), labels, torch.tensor(1.0), "mean", BF16)
+    for got, name in ((loss, "loss"), (dx, "dx"), (dw, "dw")):
+        within(got, *want[name], name)
+
+
+@pytest.mark.parametrize("tied", [True, False])
+def test_engine_step_of_a_model_under_autocast(gpu, tied):
+    """fp32 parameters under bf16 autocast: a model with the norm and the head's loss, its dots and train gradients
+    beside those of the model whose logits go into torch's loss."""
+    n, n_val, T = 6, 2, 32
+    ids = torch.randint(0, 501, (n, T), generator=gen(1)).to(gpu)
+    labels = torch.randint(0, 501, (n, T), generator=gen(2)).to(gpu)
+    labels[0, :5] = -100
+    got = []
+    for head, cast in ((True, True), (False, True), (False, False)):
+        model = _model(FP32, gpu, tied=tied, norm="rms", head_loss=head)
+        eng = GradDotProdEngine(model, val_batch_size=n_val, use_dummy_bias=True,
+                                precision="reference" if cast else "fp32")
+        opt = gs.AdamW(model.parameters(), lr=1e-3, state_bits=8)
+        eng.attach(opt)
+        eng.attach_train_batch(ids[:4], labels[:4], 0, 0)
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=cast):
+            loss = model(ids, labels)
+        loss.backward()
+        dots = {k: p.grad_dot_prod.double() for k, p in model.named_parameters() if hasattr(p, "grad_dot_prod")}
+        eng.prepare_gradients()
+        assert all(p.grad.dtype == FP32 for p in model.parameters() if p.grad is not None)
+        grads = {k: p.grad.double() for k, p in model.named_parameters() if p.grad is not None}
+        opt.step()
+        eng.aggregate_and_log()
+        eng.clear_gradients()
+        eng.detach()
+        got.append((loss.detach(), dots, grads))
+    ref = got.pop()
+    assert_close(got[0][0], got[1][0], BF16_TOL, "loss")
+    # Both casted models round on the way, and their sums' addends cancel, so no bound relative to an element holds;
+    # but the head's roundings are a part of the other's (no logits and no loss's gradient in bf16), so the 2-norm
+    # of its error against the fp32 model is at most the other's but for chance, which twice covers for 64 elements
+    # or more: a gradient's, and all dots together, each layer's as shares of their norm.
+    assert got[0][1].keys() == got[1][1].keys() == ref[1].keys() and got[0][2].keys() == got[1][2].keys()
+    ours, theirs = (torch.cat([(g[1][k] - v) / v.norm() for k, v in ref[1].items()]).norm() for g in got)
+    assert ref[1] and sum(v.numel() for v in ref[1].values()) >= 64
+    assert ours <= 2 * theirs, f"dots off by {ours:.3g}, from logits {theirs:.3g}"
+    for k, want in ref[2].items():
+        ours, theirs = ((g[2][k] - want).norm() for g in got)
+        assert ours <= 2 * theirs, f"gradient {k}: off by {ours:.3g}, from logits {theirs:.3g}"
+
+
+def test_projection_of_a_head_under_autocast(gpu, tmp_path):
+    n, T, V, d = 5, 60, 900, 64
+    net = Shifting(V, d, FP32, gpu)
+    x = randn((n, T, d), 1).to(gpu)
+    labels = torch.randint(0, V, (n, T), generator=gen(2)).to(gpu)
+    eng = projection(net, tmp_path)
+    got = []
+    for cast in (True, False):
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=cast):
+            loss = net(x, labels)
+        loss.backward()
+        got.append(net.head._ghost_grad_proj.clone())
+    assert_close(got[0], got[1], BF16_TOL, "projection")
+    eng.detach()
