@@ -299,17 +299,16 @@ def head_gradient_pieces(layer: HeadCrossEntropy, x: torch.Tensor, labels: torch
 
 # Root-mean-square norm of a residual stream ##################################################
 
-def _norm_operands(*tensors: Optional[torch.Tensor]):
-    """Under autocast, tensors of several types all in fp32, as torch's norms take them there."""
-    if _autocast() and len({t.dtype for t in tensors if t is not None}) > 1:
-        return tuple(t if t is None else t.float() for t in tensors)
-    return tensors
+def _norm_operands(*tensors: torch.Tensor):
+    """Tensors of several types: under autocast all in fp32, as torch's norms take them there."""
+    return tuple(t.float() for t in tensors) if _autocast() else tensors
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6) -> torch.Tensor:
     """``weight * x / sqrt(mean(x^2) + eps)`` over the last dimension, in fp32, rounded once.
     x: [..., d], weight: [d], of one type; of several under autocast, which gives fp32."""
-    x, weight = _norm_operands(x, weight)
+    if x.dtype != weight.dtype:
+        x, weight = _norm_operands(x, weight)
     return ops().rms_norm(x, None, weight, float(eps))[0]
 
 
@@ -317,7 +316,8 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
                  eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
     """(``rms_norm(h, weight)``, h) with h = x + residual (one rounding), in one pass; x and residual
     of one shape, all of one type (under autocast as ``rms_norm``)."""
-    x, residual, weight = _norm_operands(x, residual, weight)
+    if not x.dtype == residual.dtype == weight.dtype:
+        x, residual, weight = _norm_operands(x, residual, weight)
     y, h = ops().rms_norm(x, residual, weight, float(eps))
     return y, h
 
