@@ -107,6 +107,8 @@ def _capture_activations(layer: nn.Module, inputs: Tuple, outputs: Tuple):
     # an RMSNorm with a residual returns the rows that it normed beside what became of them
     rows = outputs[1] if isinstance(layer, RMSNorm) and isinstance(outputs, tuple) else inputs[0]
     d["activations"] = rows.detach()
+    if isinstance(layer, HeadCrossEntropy):   # each engine's own reference: another's hook drops the layer's
+        d["_gs_dot_head"] = d.get("_gs_head")
     d["_gs_fwd_seq"] = (_current_step[0], next(_fwd_counter))
 
 
@@ -130,7 +132,7 @@ def _prepare_sample_grad_or_dotprod(layer: nn.Module, grad_output: Tuple[torch.T
         backprops = grad_output[0].detach()
     d.setdefault("activations", None)
     # the loss that a HeadCrossEntropy ended in: samples are those of its input
-    head = isinstance(layer, HeadCrossEntropy) and d.get("_gs_head")
+    head = isinstance(layer, HeadCrossEntropy) and d.get("_gs_dot_head")
     samples_in = d["activations"] if head else backprops
     if head:
         others = head
@@ -195,7 +197,7 @@ def _apply_train_grad(layer: nn.Module, val_batch_size: int, loss_reduction: str
         for attr in ('activations', 'backprops', 'backprops_scale', '_gs_bias_train_grad',
                      '_gs_weight_train_grad', '_gs_ln_train_grads', '_gs_bias_grad_scale',
                      '_gs_ln_grad_scale', '_gs_grad_outputs', '_gs_positions',
-                     '_gs_sample_grads', '_gs_head'):
+                     '_gs_sample_grads', '_gs_head', '_gs_dot_head'):
             layer.__dict__.pop(attr, None)
 
 
@@ -222,7 +224,7 @@ def _worth_overlapping(layer: nn.Module, acts, backprops) -> bool:
         return True
     if isinstance(layer, (nn.LayerNorm, nn.Embedding, QKNormRotary, RMSNorm)):
         return False
-    if layer.__dict__.get("_gs_head") is not None:
+    if layer.__dict__.get("_gs_dot_head") is not None:
         return 2.0 * acts.numel() * layer.weight.shape[0] > _INLINE_FLOPS
     if isinstance(layer, nn.Conv2d):   # channels first: every output element takes a filter's size
         return 2.0 * backprops.numel() * layer.weight[0].numel() > _INLINE_FLOPS

@@ -51,6 +51,8 @@ class GradProjHooks:
     def forward_hook_store_inputs(self, module: nn.Module, inputs: Tuple[torch.Tensor, ...],
                                   output: torch.Tensor) -> None:
         module._ghost_A_raw = inputs[0].detach()
+        # what a HeadCrossEntropy's loss took and left: a reference of this engine's own
+        module.__dict__["_ghost_head"] = module.__dict__.get("_gs_head")
 
     def backward_hook_compute_proj(self, module: nn.Module,
                                    grad_input: Tuple[Optional[torch.Tensor], ...],
@@ -59,7 +61,8 @@ class GradProjHooks:
         if A_raw is None:
             raise RuntimeError(f'Missing cached activations for GradProjection in {self.layer_name}')
         B_out = grad_output[0]
-        head = module.__dict__.pop("_gs_head", None)   # what a HeadCrossEntropy's loss took and left
+        head = module.__dict__.pop("_ghost_head", None)
+        module.__dict__.pop("_gs_head", None)
         if B_out is None:
             module._ghost_grad_proj = None
             delattr(module, '_ghost_A_raw')

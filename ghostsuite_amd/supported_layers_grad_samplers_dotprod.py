@@ -609,7 +609,7 @@ def _compute_head_dot_product(layer: HeadCrossEntropy, A: torch.Tensor, B: torch
     """Dot-products of a HeadCrossEntropy's weight, and its train gradient: an nn.Linear's, of its
     logits' gradient.  Where the layer ended in its loss, B is the loss's gradient, and that of the
     logits is formed a piece of the vocabulary at a time; a dot is the sum of the pieces' dots."""
-    head = layer.__dict__.get("_gs_head")
+    head = layer.__dict__.get("_gs_dot_head")
     if head is None:
         _compute_linear_dot_product(layer, A, B, val_batch_size)
         return
@@ -650,7 +650,7 @@ def _compute_head_dot_product(layer: HeadCrossEntropy, A: torch.Tensor, B: torch
 def _compute_head_train_grad(layer: HeadCrossEntropy, A: torch.Tensor, B: torch.Tensor,
                              val_batch_size: int, scale: float = 1.0):
     """The train gradient that the dot stage formed; without labels an nn.Linear's."""
-    if layer.__dict__.pop("_gs_head", None) is None:
+    if layer.__dict__.pop("_gs_dot_head", None) is None:
         return _compute_linear_train_grad(layer, A, B, val_batch_size, scale)
     return layer.__dict__.pop("_gs_weight_train_grad")
 

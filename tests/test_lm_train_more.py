@@ -42,6 +42,43 @@ def test_projection_marks_what_the_side_stream_reads(oracle_ops, monkeypatch, tm
     assert "_gs_head" not in net.head.__dict__ and net.head._ghost_grad_proj is not None
 
 
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("first", ["dots", "projection"])
+def test_both_engines_at_once_on_a_heads_loss(oracle_ops, tmp_path, reduction, first):   # noqa: F811
+    """Either engine's hook may come first, as on an nn.Linear; each gives what it gives alone, step after step, with
+    a call without labels in between."""
+    torch.manual_seed(4)
+    net = _Net(reduction=reduction)
+    ids, labels = torch.randint(0, 13, (5, 4)), torch.randint(0, 13, (5, 4))
+
+    def dots(m):
+        eng = GradDotProdEngine(m, val_batch_size=2, use_dummy_bias=False, precision="fp32")
+        eng.attach(torch.optim.SGD(m.parameters(), lr=0.0))
+
+    def projection(m):
+        _projection(m, tmp_path)
+
+    def run(*engines):
+        m = copy.deepcopy(net)
+        for e in engines:
+            e(m)
+        for step in range(2):
+            m(ids, labels).sum().backward()
+            w = m.head.weight
+            got = [getattr(w, "grad_dot_prod", None), getattr(w, "train_grad", None),
+                   getattr(m.head, "_ghost_grad_proj", None)]
+            assert not any(k in m.head.__dict__ for k in ("_gs_head", "_gs_dot_head", "_ghost_head"))
+            for p in m.parameters():
+                p.__dict__.pop("train_grad", None)
+            with torch.no_grad():
+                m(ids)
+        return got
+    order = (dots, projection) if first == "dots" else (projection, dots)
+    both, alone, other = run(*order), run(dots), run(projection)
+    for a, b in zip(both, (*alone[:2], other[2])):
+        assert_close(a, b, 1e-6)
+
+
 @pytest.mark.parametrize("vocab,pieces", [(256, 1), (257, 2), (700, 3)])
 @pytest.mark.parametrize("T", [3, 40])
 def test_engines_sum_over_the_vocabularys_pieces(oracle_ops, monkeypatch, tmp_path, vocab, pieces, T):   # noqa: F811
