@@ -87,6 +87,8 @@ class AdamW(torch.optim.Optimizer):
         for group in state_dict["param_groups"]:
             if group.get("amsgrad") or group.get("maximize"):
                 raise GhostHipError("AdamW: a state with amsgrad or maximize")
+            if not group.get("decoupled_weight_decay", True) and group["weight_decay"]:
+                raise GhostHipError("AdamW: a state of Adam, whose weight decay is in its gradients")
         super().load_state_dict(state_dict)
         for group in self.param_groups:
             group.setdefault("state_bits", 32)

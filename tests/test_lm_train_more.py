@@ -6,7 +6,7 @@ import ctypes
 import pytest
 import torch
 
-from ghostsuite_amd import GradDotProdEngine, GradProjLoraEngine, _native, lm_layers
+from ghostsuite_amd import AdamW, GradDotProdEngine, GradProjLoraEngine, _native, lm_layers
 from ghostsuite_amd.gradProjection import autograd_gradproj
 from tests.helpers import assert_close
 from tests.test_lm_train import P16, _Net, _head, oracle_ops   # noqa: F401  (a fixture)
@@ -134,3 +134,20 @@ def test_head_refuses_grids_beyond_a_launch(N, V, d, status):
     assert lib.gs_head_grad(ref, P16, None, None, P16, None, 0, None) == (-3 if N == 2 ** 25 else status)
     assert lib.gs_head_loss(ref, P16, P16, None, 0, None) == (-3 if N == 2 ** 25 else status)
     assert lib.gs_head_logit_grad(ref, P16, None, 0, 8, P16, 8, None, 0, None) == (-3 if N == 2 ** 25 else -5)
+
+
+def test_adamw_refuses_a_state_of_adam():
+    """torch.optim.Adam adds its weight decay to the gradients; without weight decay the two are one."""
+    p, q = (torch.nn.Parameter(torch.ones(3)) for _ in range(2))
+    p.grad = torch.ones(3)
+    for decay in (0.1, 0.0):
+        adam = torch.optim.Adam([p], lr=0.02, weight_decay=decay)
+        adam.step()
+        opt = AdamW([q], lr=7.0)
+        if decay:
+            with pytest.raises(_native.GhostHipError, match="state of Adam"):
+                opt.load_state_dict(adam.state_dict())
+            assert opt.param_groups[0]["lr"] == 7.0 and not opt.state
+        else:
+            opt.load_state_dict(adam.state_dict())
+            assert opt.param_groups[0]["lr"] == 0.02 and opt.state[q]["step"] == 1
