@@ -4,11 +4,13 @@
 //   m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2
 //   p = (1 - lr decay) p - lr / (1 - b1^t) m / ((v / (1 - b2^t))^(1/2) + eps)
 // in fp32, p rounded once to its type.  Bound by memory: every array is read once and written once
-// (GPT-2-small's 124 M bf16 parameters: 560 us with averages in 32 bits, 4.9 TB/s) but for 8 bits, where the
-// vector units take a little longer (280 us, 4.5 TB/s: every product, sum, root and quotient rounded as
-// fp32 rounds it; with contraction and the hardware's approximate root and reciprocal 255, but then an
-// average is a unit off, about one chance in 10^6 falls the other way and an element is held an eighth
-// away, and where it is its block's largest on the next step, so is the block's scale).
+// (GPT-2-small's 124 M bf16 parameters: 560 us with averages in 32 bits, 4.9 TB/s; 261 in 8 bits, 4.8 TB/s,
+// where the vector units take as long).  In 8 bits every product, sum, root and quotient is rounded as fp32
+// rounds it: with contraction and the hardware's approximate root and reciprocal (255 us) an average is a unit
+// off, about one chance in 10^6 falls the other way and an element is held an eighth away, and where it is
+// its block's largest on the next step, so is the block's scale.  What few elements need is apart: roots of
+// numbers near the ends of fp32, values below 2^-6 of their scale (gradients over seven decades within a block:
+// 355 us, before 300) and ones that are not finite; so all of them within each element took 288 us.
 // A launch takes many tensors (their addresses travel in its arguments); its workgroups take runs
 // of CHUNK elements, a tensor's last one shorter, and find their tensor by its first run (runs of 8192
 // elements were 4% slower than runs of 2048: more workgroups at work at once, above all where a launch has
@@ -23,12 +25,14 @@
 // down, u spread evenly over [0, 1) by a hash of the element's place, the step and the seed, the
 // same on every run.  (v, the root's square, comes out high by the rounding's variance: at most the
 // sixteenth of its drift, a few hundredths of it where gradients are noise.)  A root that is not
-// zero never becomes zero, nor less than half of itself: where the gradient stops, m is not divided
-// by eps alone.  p is formed from m and v before their rounding.  A value that is not finite is held
-// as NaN and has no part in its block's scale; p is NaN from the next step on.
+// zero never becomes zero, nor less than half of itself, but for one below 2^-63, whose square leaves fp32:
+// where the gradient stops, m is not divided by eps alone.  p is formed from m and v before their
+// rounding.  A value that is not finite is held as NaN and has no part in its block's scale; p is NaN from
+// the next step on.
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "gs_common.h"
 
@@ -127,20 +131,30 @@ __global__ void __launch_bounds__(NT) adamw_kernel(Tensors a, Factors f) {
   v.store(tv + i, vec, left);
 }
 
-// The largest of 32 lanes (half a wave holds a block), in each of them.
+// The largest of 32 lanes (half a wave holds a block), in each of them: by row shifts, zeros beyond a row's
+// first lane, and the broadcast of a row's last one.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t max_dpp(uint32_t v) {
+  return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, true)));
+}
 __device__ __forceinline__ uint32_t half_max(uint32_t v) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), off, 64)));
-  return v;
+  v = max_dpp<0x111, 0xf>(v);   // row_shr 1, 2, 4, 8: lane 15 holds its row's
+  v = max_dpp<0x112, 0xf>(v);
+  v = max_dpp<0x114, 0xf>(v);
+  v = max_dpp<0x118, 0xf>(v);
+  v = max_dpp<0x142, 0xa>(v);   // row_bcast 15 into rows 1 and 3: lanes 31 and 63
+  const uint32_t lo = __builtin_amdgcn_readlane(v, 31), hi = __builtin_amdgcn_readlane(v, 63);
+  return threadIdx.x & 32 ? hi : lo;
 }
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-constexpr uint32_t INF_BITS = 0x7F800000u, TOP_BITS = 0x43E00000u;   // of infinity and of 448
+constexpr uint32_t INF_BITS = 0x7F800000u;
 
 // a of [2^-6, 448] on the 8-bit values, up or down by the chance (u << 4) + 8 of 2^20: an integer addition
 // to the 20 mantissa bits that are cut off, which is floor(a / step + (u + 1/2) / 2^16) step (the sum has
-// no more than 24 bits).  So is zero, at zero.
+// no more than 24 bits).  So is zero, at zero.  An a that rounding has left a few units above 448 stays there:
+// the chance is at most 2^20 - 8.
 __device__ __forceinline__ float eighth(float a, uint32_t chance) {
-  return __uint_as_float(min((__float_as_uint(a) + chance) & 0xFFF00000u, TOP_BITS));
+  return __uint_as_float((__float_as_uint(a) + chance) & 0xFFF00000u);
 }
 // The same of any a: below 2^-6 the steps stay 2^-9, a may have bits below the chance's, and the sum is
 // rounded to fp32 before its floor.
@@ -149,8 +163,7 @@ __device__ __forceinline__ float eighth_or_less(float a, uint32_t chance) {
   return a < 0x1p-6f ? low : eighth(a, chance);
 }
 // The root of x, correctly rounded, for x of [2^-96, 2^96): from the hardware's inverse root, and what its
-// product with x leaves of x.  (Every such x was compared with a float64 root's rounding.  Comparing the
-// hardware's root's neighbours, as sqrtf does: 287 us for GPT-2-small's parameters, this 280.)
+// product with x leaves of x.  (Every such x was compared with a float64 root's rounding.)
 __device__ __forceinline__ float root_of(float x) {
   const float y = __builtin_amdgcn_rsqf(x), s = x * y;
   return __fmaf_rn(__fmaf_rn(-s, s, x), 0.5f * y, s);
@@ -213,28 +226,30 @@ __global__ void __launch_bounds__(NT) adamw8_kernel(Tensors a, Factors f) {
   g.load(static_cast<const E*>(t.g) + i, vec, left);
   load8(tm + i, vec8, left, m);
   load8(tv + i, vec8, left, r);
-  uint32_t beyond = 0;
+  uint32_t beyond = 0, most = 0;
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
     m[e] = f.b1 * (m[e] * sm) + f.rest1 * g.v[e];
     const float old = r[e] * sr;
     r[e] = f.b2 * (old * old) + f.rest2 * (g.v[e] * g.v[e]);
     beyond = max(beyond, __float_as_uint(r[e]) - ROOT_FROM);
+    most = max(most, __float_as_uint(r[e]));
   }
   if (beyond <= ROOT_TO - ROOT_FROM) {
 #pragma unroll
     for (int e = 0; e < VE; ++e) r[e] = root_of(r[e]);
-  } else {
+  } else if (most > 0) {   // zeros stay: rows of an embedding that no batch has had
 #pragma unroll
     for (int e = 0; e < VE; ++e) r[e] = sqrtf(r[e]);
   }
   uint32_t top_m = 0, top_r = 0;   // magnitudes by their bits: larger than infinity's, a NaN
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
-    const float by = r[e] * f.root + f.eps;   // NaN with the root; zero only with eps
-    p.v[e] = f.keep * p.v[e] - f.step * m[e] / (by == 0.f ? INFINITY : by);
+    float by = r[e] * f.root + f.eps;   // NaN with the root
+    if (f.eps == 0.f && by == 0.f) by = INFINITY;
+    p.v[e] = f.keep * p.v[e] - f.step * m[e] / by;
     top_m = max(top_m, magnitude(m[e]));
-    top_r = max(top_r, magnitude(r[e]));
+    top_r = max(top_r, __float_as_uint(r[e]));   // not below zero
   }
   p.store(static_cast<E*>(t.p) + i, vec, left);
   const bool whole = max(top_m, top_r) < INF_BITS;   // all of them finite
@@ -248,32 +263,41 @@ __global__ void __launch_bounds__(NT) adamw8_kernel(Tensors a, Factors f) {
   const float most_m = __uint_as_float(half_max(top_m)), most_r = __uint_as_float(half_max(top_r));
   const bool some_m = most_m >= LEAST, some_r = most_r >= LEAST;
   const float im = some_m ? 1.f / most_m * TOP : 0.f, ir = some_r ? 1.f / most_r * TOP : 0.f;
-  const auto chances = [&](int e) {
-    uint32_t x = (static_cast<uint32_t>(i + e) + f.key) * 0x9E3779B9u;
-    x = (x ^ (x >> 15)) * 0xBB67AE85u;
-    return x ^ (x >> 13);
-  };
-  const auto chance_m = [](uint32_t x) { return ((x & 0xFFFFu) << 4) + 8u; };
-  const auto chance_r = [](uint32_t x) { return ((x >> 16) << 4) + 8u; };
-  float least = INFINITY;
+  float least_m = INFINITY, least_r = INFINITY;
 #pragma unroll
-  for (int e = 0; e < VE; ++e) least = fminf(least, fminf(fabsf(m[e]) * im, r[e] * ir));
-  if (whole && least >= 0x1p-6f) {
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      const uint32_t x = chances(e);
-      m[e] = copysignf(eighth(fabsf(m[e]) * im, chance_m(x)), m[e]);
-      r[e] = eighth(r[e] * ir, chance_r(x));
-    }
-  } else {
-    for (int e = 0; e < VE; ++e) {
-      const uint32_t x = chances(e);
-      const float hm = eighth_or_less(fabsf(m[e]) * im, chance_m(x));
-      const float hr = eighth_or_less(r[e] * ir, chance_r(x));
-      m[e] = magnitude(m[e]) < INF_BITS ? copysignf(hm, m[e]) : NAN;
-      r[e] = magnitude(r[e]) < INF_BITS ? (r[e] > 0.f && some_r ? fmaxf(hr, 0x1p-9f) : 0.f) : NAN;
-    }
+  for (int e = 0; e < VE; ++e) {
+    least_m = fminf(least_m, fabsf(m[e]) * im);
+    least_r = fminf(least_r, r[e] * ir);
   }
+  const auto hold = [&](auto any_size, auto any_value) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      uint32_t x = (static_cast<uint32_t>(i + e) + f.key) * 0x9E3779B9u;
+      x = (x ^ (x >> 15)) * 0xBB67AE85u;
+      x ^= x >> 13;
+      const uint32_t um = ((x & 0xFFFFu) << 4) + 8u, ur = ((x >> 16) << 4) + 8u;
+      const float am = fabsf(m[e]) * im, ar = r[e] * ir;
+      float hm, hr;
+      if constexpr (!decltype(any_size)::value) {
+        hm = eighth(am, um), hr = eighth(ar, ur);
+      } else {
+        hm = eighth_or_less(am, um);
+        hr = fmaxf(eighth_or_less(ar, ur), r[e] > 0.f && some_r ? 0x1p-9f : 0.f);
+      }
+      if constexpr (decltype(any_value)::value) {
+        m[e] = magnitude(m[e]) < INF_BITS ? copysignf(hm, m[e]) : NAN;
+        r[e] = magnitude(r[e]) < INF_BITS ? hr : NAN;
+      } else {
+        m[e] = copysignf(hm, m[e]), r[e] = hr;
+      }
+    }
+  };
+  if (!whole)
+    hold(std::true_type{}, std::true_type{});
+  else if ((some_m && least_m < 0x1p-6f) || (some_r && least_r < 0x1p-6f))
+    hold(std::true_type{}, std::false_type{});
+  else   // a block of zeros is one of these: a is zero all over
+    hold(std::false_type{}, std::false_type{});
   store8(tm + i, vec8, left, m);
   store8(tv + i, vec8, left, r);
   if (live && (threadIdx.x & 31) == 0) {
