@@ -234,8 +234,9 @@ def head_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tens
 
     x: [..., d] hidden rows, weight: [vocab, d], of one type (bf16 or fp32); labels: [...] integers.
     The logits are formed in fp32 a piece of the vocabulary at a time, once in the forward pass and
-    again in the backward pass, and never stored; the gradient of a piece is (bf16 in a bf16 model,
-    in up to 512 MiB), rounded once, before it is multiplied into the gradients of x and weight.
+    again in the backward pass, and never stored; the gradient of a piece is (in up to 1 GiB, but at
+    least 256 entries), before it is multiplied into the gradients of x and weight: rounded once to
+    bf16 in a bf16 model, for up to 32 rows in two bf16 parts.
     Rows whose label is ignore_index take no part and are not read; their loss and gradient are zero.
     Another label outside [0, vocab) makes its row's loss and gradient NaN.
     reduction: 'mean' (over the rows not ignored; NaN when there are none), 'sum', or 'none' ([...]).

@@ -515,8 +515,10 @@ int gs_distill_grad(const gs_distill* d, const float* upstream, int filled, void
  * lse: [N, 2] fp32, what the backward pass takes of the forward one.
  * gs_head_grad: dx [N, d] and dw [V, d] of dtype, either may be NULL; upstream: NULL (ones), or fp32,
  * [N] with NONE and [1] otherwise.  dz = softmax(z) - 1_y (times a row's own upstream gradient) is
- * rounded once to bf16 between the products with bf16 operands; other factors are applied in fp32
- * before the one rounding of dx and dw.  Every sum has a fixed order.
+ * rounded once to bf16 between the products with bf16 operands of more than 32 rows, and held in two bf16
+ * parts for up to 32; other factors are applied in fp32 before the one rounding of dx and dw.  dz's
+ * piece in the workspace takes up to 1 GiB, but at least 256 entries of the vocabulary.  Every sum has a
+ * fixed order.
  * gs_head_logit_grad: dz of the vocabulary entries [v0, v0 + n) of all N rows, zeros where a row does
  * not count, with every factor (upstream, count) applied before its rounding to dtype:
  * out [N, out_stride], 16-byte aligned, entries past n up to out_stride zeros; out_stride: n up to the next
