@@ -1435,6 +1435,7 @@ bool grids_fit(const gs_head& h, const Plan& p, int64_t vocab, bool dx, bool dw,
   for (int64_t v0 = 0; v0 < vocab; v0 += p.cols) {
     const int64_t n = std::min(p.cols, vocab - v0);
     if (n < p.cols || v0 == 0) {   // the pieces are alike but for the last
+      if (p.copy_w && !fits(n, 64, 1)) return false;   // a wave to an entry
       const Size s = logits_shape(h, p, n).size;
       if (!fits(cdiv(n, rows_of(s)), cdiv(h.N, s == FEW ? Few::BN : rows_of(s)), threads(s))) return false;
       const DwParts w = dw_parts(h, p, n);

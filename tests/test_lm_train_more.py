@@ -136,6 +136,15 @@ def test_head_refuses_grids_beyond_a_launch(N, V, d, status):
     assert lib.gs_head_logit_grad(ref, P16, None, 0, 8, P16, 8, None, 0, None) == (-3 if N == 2 ** 25 else -5)
 
 
+def test_head_logit_grad_refuses_a_copy_of_the_weight_beyond_a_launch():
+    """64 threads to an entry, of weights whose rows are copied; others have no copy."""
+    lib = _native.load_library()
+    for d, N, n, status in ((7, 40, 2 ** 25, -3), (7, 40, 2 ** 25 + 8, -5), (8, 40, 2 ** 25 + 8, -3),
+                            (7, 1, 2 ** 25 + 8, -5), (6, 1, 2 ** 25 + 8, -3)):
+        ref = ctypes.byref(_head(N=N, V=2 ** 28, d=d, x_stride=d))
+        assert lib.gs_head_logit_grad(ref, P16, None, 0, n, P16, n, None, 0, None) == status, (d, N, n)
+
+
 def test_adamw_refuses_a_state_of_adam():
     """torch.optim.Adam adds its weight decay to the gradients; without weight decay the two are one."""
     p, q = (torch.nn.Parameter(torch.ones(3)) for _ in range(2))
