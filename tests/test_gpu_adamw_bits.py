@@ -80,7 +80,7 @@ def gradients(n, seed, spread):
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 @pytest.mark.parametrize("betas,spread", [((0.9, 0.999), False), ((0.9, 0.999), True), ((0.5, 0.95), True)])
 def test_steps_are_the_elementary_ones(gpu, dtype, betas, spread):
-    """A hundred or so chances of a step's ten million lie within a unit of their line, so a single product that is
+    """Some ten of ten steps' ten million chances lie within a unit of their line, so a single product that is
     not rounded where it is stated shows."""
     sizes = (1 << 20, 65537, 255, 1)
     start = [randn((n,), n, 0.02, dtype) for n in sizes]
